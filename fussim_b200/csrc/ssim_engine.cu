@@ -3,7 +3,6 @@
 // include/fussim_b200.h. No torch, no Python: any host language can bind this library.
 #include <cuda_runtime.h>
 #include <cudaTypedefs.h>
-#include <nvtx3/nvToolsExt.h>
 
 #include <atomic>
 #include <climits>
@@ -14,28 +13,18 @@
 #include <mutex>
 #include <string>
 
+#include "engine_host.h"
 #include "fussim_b200.h"
 #include "ssim_kernels.cuh"
 #include "ssim_stream.cuh"
 
 namespace {
 
-thread_local std::string g_last_error;
-
-// NVTX range over an entry point's host-side work (argument checks and launches), so a
-// timeline tool shows the forward, backward and cross-GPU exchange by name. Without a tool
-// attached a push/pop costs a few nanoseconds.
-struct NvtxRange {
-  explicit NvtxRange(const char* name) { nvtxRangePushA(name); }
-  ~NvtxRange() { nvtxRangePop(); }
-  NvtxRange(const NvtxRange&) = delete;
-  NvtxRange& operator=(const NvtxRange&) = delete;
-};
-
-int fail(int code, const std::string& msg) {
-  g_last_error = msg;
-  return code;
-}
+using fssim_host::NvtxRange;
+using fssim_host::aligned;
+using fssim_host::device_sms;
+using fssim_host::fail;
+using fssim_host::g_last_error;
 
 std::string window_message(int ws) {
   // Same text as the reference's dispatch (csrc/ssim.cu:617).
@@ -46,8 +35,6 @@ int check_window(int ws) {
   if (ws == 7 || ws == 9 || ws == 11) return FSSIM_OK;
   return fail(FSSIM_ERR_WINDOW, window_message(ws));
 }
-
-bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
 
 // Shape checks shared by every entry point. Rows and columns are 32-bit inside the kernels.
 int check_shape(int64_t B, int64_t C, int64_t H, int64_t W) {
@@ -73,25 +60,6 @@ fssim::Geometry make_geometry(int64_t B, int64_t C, int64_t H, int64_t W) {
   g.B = static_cast<int>(B);
   g.LT = B * C * static_cast<int64_t>(g.S) * H;
   return g;
-}
-
-int device_sms(int* sms) {
-  static std::mutex mu;
-  static int cached[64] = {0};
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return fail(FSSIM_ERR_CUDA, std::string("cudaGetDevice: ") + cudaGetErrorString(e));
-  if (dev < 0 || dev >= 64) return fail(FSSIM_ERR_CUDA, "device ordinal out of range");
-  std::lock_guard<std::mutex> lock(mu);
-  if (cached[dev] == 0) {
-    int v = 0;
-    e = cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev);
-    if (e != cudaSuccess)
-      return fail(FSSIM_ERR_CUDA, std::string("cudaDeviceGetAttribute: ") + cudaGetErrorString(e));
-    cached[dev] = v;
-  }
-  *sms = cached[dev];
-  return FSSIM_OK;
 }
 
 // Opt a kernel in to its dynamic shared memory size on the current device and return the

@@ -41,6 +41,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "pdl.cuh"
+
 namespace fssim {
 
 constexpr int kThreads = 128;         // 4 warps per CTA
@@ -245,18 +247,6 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, i
       " [%0], [%1, {%2, %3, %4}], [%5];\n" ::"r"(smem_addr(dst)),
       "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(smem_addr(bar))
       : "memory");
-}
-
-// Programmatic dependent launch. The kernels are launched so that they may start while the
-// previous kernel on the stream is finishing; their set-up (barrier init, step cursor)
-// overlaps that tail, and griddepcontrol.wait, before the first access to global memory,
-// waits for the previous kernel to complete and its writes to be visible. (Both are no-ops
-// for a regular launch.) A kernel then allows its own dependent to launch.
-__device__ __forceinline__ void grid_dependency_wait() {
-  asm volatile("griddepcontrol.wait;\n" ::: "memory");
-}
-__device__ __forceinline__ void grid_launch_dependents() {
-  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
 }
 
 __device__ __forceinline__ float to_f(float v) { return v; }
