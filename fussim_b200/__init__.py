@@ -8,7 +8,11 @@ Drop-in for the public API of OpsiClear/fussim (``fussim/__init__.py``):
 * ``FusedSSIMMap`` / ``FusedSSIMMapFP16`` — the map-producing autograd Functions;
 * ``SUPPORTED_WINDOW_SIZES``, ``get_build_info``, ``check_compatibility``.
 
-Gradients flow to the first image only. Under ``torch.autocast`` the inputs are rounded
+Beside the losses, operators of the training step around them: ``group_norm_act`` /
+``GroupNormAct`` (group normalisation with its activation, channels last) and ``grad_norm`` /
+``clip_grad_norm`` / ``clip_grad_norm_`` (the global gradient norm and clipping).
+
+Gradients of the losses flow to the first image only. Under ``torch.autocast`` the inputs are rounded
 to FP16 (whatever the autocast dtype, as the reference does) and the arithmetic stays
 FP32. There is no CPU path: every call runs the hand-written sm_100a kernels of
 ``libfussim_b200.so`` and fails loudly if they are missing.
@@ -29,6 +33,13 @@ from .functional import (  # noqa: F401
     poll_device_error,
     ssim,
 )
+from .training import (  # noqa: F401
+    GroupNormAct,
+    clip_grad_norm,
+    clip_grad_norm_,
+    grad_norm,
+    group_norm_act,
+)
 
 __all__ = [
     # Primary API
@@ -37,6 +48,12 @@ __all__ = [
     # pytorch-msssim compatible API
     "ssim",
     "SSIM",
+    # Training step around the loss
+    "group_norm_act",
+    "GroupNormAct",
+    "grad_norm",
+    "clip_grad_norm",
+    "clip_grad_norm_",
     # Advanced/internal
     "FusedSSIMMap",
     "FusedSSIMMapFP16",

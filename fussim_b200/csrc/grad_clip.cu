@@ -1,0 +1,203 @@
+// C entry points of the global gradient norm and of clipping: argument checks, the tables of
+// tensors and the launches. The kernels are in grad_clip.cuh.
+#include "grad_clip.cuh"
+
+#include <climits>
+#include <cstdint>
+#include <exception>
+#include <memory>
+#include <string>
+
+#include "engine_host.h"
+
+namespace {
+
+using fssim::ClipTable;
+using fssim::kClipMaxCtas;
+using fssim::kClipThreads;
+using fssim::kClipUnit;
+using fssim_host::aligned;
+using fssim_host::fail;
+using fssim_host::NvtxRange;
+
+// Runs per launch: a small table (3 KB of parameters) or a large one (29 KB, of the 32 KB that
+// a launch may carry).
+constexpr int kFew = 96;
+constexpr int kMany = 832;
+static_assert(sizeof(ClipTable<kMany>) <= 32764, "kernel parameters are limited to 32764 bytes");
+
+size_t elem_size(int dtype) { return dtype == FSSIM_F32 ? 4 : 2; }
+bool known_dtype(int d) { return d == FSSIM_F32 || d == FSSIM_F16 || d == FSSIM_BF16; }
+
+template <typename... KA, typename... A>
+int launch(void (*k)(KA...), unsigned grid, cudaStream_t stream, const char* what, const A&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(kClipThreads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, k, args...);
+  if (e != cudaSuccess) {
+    (void)cudaGetLastError();
+    return fail(FSSIM_ERR_CUDA, std::string(what) + ": " + cudaGetErrorString(e));
+  }
+  return FSSIM_OK;
+}
+
+unsigned grid_for(int64_t units) {
+  return static_cast<unsigned>(units < kClipMaxCtas ? units : kClipMaxCtas);
+}
+
+int64_t units_of(int64_t size) { return (size + kClipUnit - 1) / kClipUnit; }
+
+// Launches of a call: runs of at most kMany non-empty tensors each.
+struct Cut {
+  int64_t begin, end;  // tensors
+  int64_t units;
+  int runs;
+};
+
+Cut next_cut(const fssim_grad_clip_args& a, int64_t begin) {
+  Cut c{begin, begin, 0, 0};
+  while (c.end < a.count && c.runs < kMany) {
+    if (a.sizes[c.end] > 0) {
+      c.units += units_of(a.sizes[c.end]);
+      ++c.runs;
+    }
+    ++c.end;
+  }
+  return c;
+}
+
+int total_partials(const fssim_grad_clip_args& a) {
+  int64_t n = 0;
+  for (int64_t i = 0; i < a.count;) {
+    const Cut c = next_cut(a, i);
+    n += grid_for(c.units);
+    i = c.end;
+  }
+  return static_cast<int>(n < INT_MAX ? n : INT_MAX);
+}
+
+int check(const fssim_grad_clip_args* a, bool clip) {
+  if (!a) return fail(FSSIM_ERR_NULLPTR, "args is NULL");
+  if (a->count < 0) return fail(FSSIM_ERR_SHAPE, "negative number of tensors");
+  if (!a->norm) return fail(FSSIM_ERR_NULLPTR, "norm is required");
+  if (a->count > 0 && (!a->grads || !a->sizes || !a->dtypes))
+    return fail(FSSIM_ERR_NULLPTR, "grads, sizes and dtypes are required");
+  if (clip && a->count > 0 && (!a->outs || !a->out_dtypes))
+    return fail(FSSIM_ERR_NULLPTR, "outs and out_dtypes are required");
+  if (clip && !(a->max_norm >= 0.f)) return fail(FSSIM_ERR_ARGUMENT, "max_norm must not be negative");
+  for (int64_t i = 0; i < a->count; ++i) {
+    if (a->sizes[i] < 0 || a->sizes[i] > (int64_t{1} << 60))
+      return fail(FSSIM_ERR_SHAPE, "a tensor's size is negative or too large");
+    if (!known_dtype(a->dtypes[i])) return fail(FSSIM_ERR_DTYPE, "gradients must be F32, F16 or BF16");
+    if (clip && a->out_dtypes[i] != a->dtypes[i] && a->out_dtypes[i] != FSSIM_F32)
+      return fail(FSSIM_ERR_DTYPE, "an output has its gradient's type or F32");
+    if (a->sizes[i] == 0) continue;
+    if (!a->grads[i] || (clip && !a->outs[i])) return fail(FSSIM_ERR_NULLPTR, "a tensor's pointer is NULL");
+    if (!aligned(a->grads[i], elem_size(a->dtypes[i])) ||
+        (clip && !aligned(a->outs[i], elem_size(a->out_dtypes[i]))))
+      return fail(FSSIM_ERR_ARGUMENT, "a tensor is not aligned to its element size");
+  }
+  const int64_t need = fssim_grad_clip_workspace_bytes(a);
+  if (need > 0 && (!a->workspace || a->workspace_bytes < static_cast<size_t>(need)))
+    return fail(FSSIM_ERR_WORKSPACE, "workspace smaller than fssim_grad_clip_workspace_bytes");
+  if (!aligned(a->workspace, 8)) return fail(FSSIM_ERR_WORKSPACE, "workspace must be 8-byte aligned");
+  return FSSIM_OK;
+}
+
+template <int K>
+int launch_cut(const fssim_grad_clip_args& a, const Cut& c, bool clip, int partials, int first,
+               cudaStream_t stream) {
+  auto t = std::make_unique<ClipTable<K>>();
+  int r = 0;
+  int64_t unit = 0;
+  for (int64_t i = c.begin; i < c.end; ++i) {
+    if (a.sizes[i] == 0) continue;
+    t->src[r] = a.grads[i];
+    t->dst[r] = clip ? a.outs[i] : nullptr;
+    t->size[r] = a.sizes[i];
+    t->unit0[r] = unit;
+    t->src_dtype[r] = static_cast<unsigned char>(a.dtypes[i]);
+    t->dst_dtype[r] = static_cast<unsigned char>(clip ? a.out_dtypes[i] : 0);
+    unit += units_of(a.sizes[i]);
+    ++r;
+  }
+  t->unit0[r] = unit;
+  t->count = r;
+  t->partials = static_cast<double*>(a.workspace);
+  t->num_partials = partials;
+  t->first_partial = first;
+  t->norm = clip && first == 0 ? a.norm : nullptr;
+  t->max_norm = a.max_norm;
+  const unsigned grid = grid_for(c.units);
+  return clip ? launch(fssim::grad_clip_kernel<K>, grid, stream, "gradient clipping launch", *t)
+              : launch(fssim::grad_squares_kernel<K>, grid, stream, "gradient norm launch", *t);
+}
+
+// One pass over all tensors: the partial sums (clip == false) or the scaling.
+int pass(const fssim_grad_clip_args& a, bool clip, int partials, cudaStream_t stream) {
+  int first = 0;
+  for (int64_t i = 0; i < a.count;) {
+    const Cut c = next_cut(a, i);
+    i = c.end;
+    if (c.runs == 0) continue;
+    const int st = c.runs <= kFew ? launch_cut<kFew>(a, c, clip, partials, first, stream)
+                                  : launch_cut<kMany>(a, c, clip, partials, first, stream);
+    if (st) return st;
+    first += static_cast<int>(grid_for(c.units));
+  }
+  return FSSIM_OK;
+}
+
+int run(const fssim_grad_clip_args* a, bool clip, cudaStream_t stream) {
+  int st = check(a, clip);
+  if (st) return st;
+  const int partials = total_partials(*a);
+  if (partials == 0) {
+    const cudaError_t e = cudaMemsetAsync(a->norm, 0, sizeof(float), stream);
+    return e == cudaSuccess ? FSSIM_OK : fail(FSSIM_ERR_CUDA, cudaGetErrorString(e));
+  }
+  st = pass(*a, false, partials, stream);
+  if (st) return st;
+  if (clip) return pass(*a, true, partials, stream);
+  return launch(fssim::grad_norm_kernel, 1u, stream, "gradient norm sum launch",
+                static_cast<const double*>(a->workspace), partials, a->norm);
+}
+
+// No exception crosses the C boundary.
+template <typename F>
+int guarded(F f) {
+  try {
+    fssim_host::g_last_error.clear();
+    return f();
+  } catch (const std::exception&) {
+    return FSSIM_ERR_CUDA;
+  }
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t fssim_grad_clip_workspace_bytes(const fssim_grad_clip_args* a) {
+  if (!a || a->count <= 0 || !a->sizes) return 0;
+  return sizeof(double) * static_cast<size_t>(total_partials(*a));
+}
+
+int fssim_grad_norm(const fssim_grad_clip_args* a, fssim_stream_t stream) {
+  NvtxRange range("fssim_grad_norm");
+  return guarded([&] { return run(a, false, stream); });
+}
+
+int fssim_grad_clip(const fssim_grad_clip_args* a, fssim_stream_t stream) {
+  NvtxRange range("fssim_grad_clip");
+  return guarded([&] { return run(a, true, stream); });
+}
+
+}  // extern "C"

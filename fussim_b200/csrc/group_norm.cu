@@ -1,0 +1,337 @@
+// C entry points of the group normalisation with an activation: argument checks, the split of
+// the work, and the launches. The kernels are in group_norm.cuh.
+#include "group_norm.cuh"
+
+#include <climits>
+#include <cstdint>
+#include <exception>
+#include <string>
+
+#include "engine_host.h"
+
+namespace {
+
+using fssim::NormGeometry;
+using fssim::NormParams;
+using fssim_host::aligned;
+using fssim_host::fail;
+using fssim_host::NvtxRange;
+
+constexpr int64_t kMaxChannels = int64_t{1} << 24;
+constexpr int64_t kMaxSamples = int64_t{1} << 30;
+// CTAs a launch aims at: four of 256 threads on each of 148 SMs.
+constexpr int64_t kTargetCtas = 148 * 4;
+// A part has at least this many pixels for each thread, so that its set-up is paid for.
+constexpr int64_t kMinSteps = 4;
+// Bytes of input that the reducing pass may leave for the applying pass to find in L2.
+constexpr int64_t kResidentBytes = int64_t{80} << 20;
+
+size_t elem_size(int dtype) { return dtype == FSSIM_F32 ? 4 : 2; }
+bool known_dtype(int d) { return d == FSSIM_F32 || d == FSSIM_F16 || d == FSSIM_BF16; }
+size_t round256(size_t n) { return (n + 255) / 256 * 256; }
+
+// Elements per vector: 16 bytes where the channels and every tensor's address allow it, else
+// 4 bytes, else one element.
+int vector_width(int64_t C, size_t esize, const void* a, const void* b, const void* c) {
+  for (size_t bytes : {size_t{16}, size_t{4}}) {
+    const int64_t v = static_cast<int64_t>(bytes / esize);
+    if (C % v == 0 && aligned(a, bytes) && aligned(b, bytes) && aligned(c, bytes))
+      return static_cast<int>(v);
+  }
+  return 1;
+}
+
+NormGeometry make_geometry(int64_t N, int64_t P, int64_t C, int64_t G, int V, float eps) {
+  NormGeometry g{};
+  g.N = N;
+  g.P = P;
+  g.C = static_cast<int>(C);
+  g.G = static_cast<int>(G);
+  g.Cg = static_cast<int>(C / G);
+  g.eps = eps;
+  const int64_t vectors = C / V;
+  const int64_t slices = (vectors + fssim::kNormThreads - 1) / fssim::kNormThreads;
+  g.lanes = static_cast<int>((vectors + slices - 1) / slices);
+  g.slices = static_cast<int>((vectors + g.lanes - 1) / g.lanes);
+  g.SC = g.lanes * V;
+  g.rows = fssim::kNormThreads / g.lanes;
+  g.GS = g.slices == 1 ? g.G : static_cast<int>((g.SC + g.Cg - 2) / g.Cg + 1);
+  if (g.GS > g.G) g.GS = g.G;
+  int64_t S = kTargetCtas / (N * g.slices);
+  const int64_t by_work = P / (g.rows * kMinSteps);
+  if (S > by_work) S = by_work;
+  if (S < 1) S = 1;
+  g.S = static_cast<int>(S);
+  return g;
+}
+
+// Samples per launch: as many as leave their input in L2 between the two passes, in equal cuts.
+int64_t samples_per_launch(int64_t N, int64_t bytes_per_sample) {
+  int64_t k = bytes_per_sample > 0 ? kResidentBytes / bytes_per_sample : N;
+  if (k < 1) k = 1;
+  if (k >= N) return N;
+  const int64_t cuts = (N + k - 1) / k;
+  return (N + cuts - 1) / cuts;
+}
+
+template <typename Kernel>
+int launch(Kernel k, dim3 grid, const NormParams& p, cudaStream_t stream, const char* what) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(fssim::kNormThreads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, k, p);
+  if (e != cudaSuccess) {
+    (void)cudaGetLastError();
+    return fail(FSSIM_ERR_CUDA, std::string(what) + ": " + cudaGetErrorString(e));
+  }
+  return FSSIM_OK;
+}
+
+dim3 tile_grid(const NormGeometry& g) {
+  return dim3(static_cast<unsigned>(g.N * g.S), static_cast<unsigned>(g.slices));
+}
+
+int check_common(int dtype, int weight_dtype, int activation, int64_t N, int64_t P, int64_t C,
+                 int64_t G, float eps) {
+  if (!known_dtype(dtype)) return fail(FSSIM_ERR_DTYPE, "dtype must be F32, F16 or BF16");
+  if (!known_dtype(weight_dtype)) return fail(FSSIM_ERR_DTYPE, "weight_dtype must be F32, F16 or BF16");
+  if (activation < FSSIM_ACT_NONE || activation > FSSIM_ACT_RELU)
+    return fail(FSSIM_ERR_ARGUMENT, "activation must be 0 (none), 1 (silu) or 2 (relu)");
+  if (N < 0 || P < 0 || C < 0) return fail(FSSIM_ERR_SHAPE, "negative dimension");
+  if (G < 1 || C < 1 || C % G != 0)
+    return fail(FSSIM_ERR_SHAPE, "the channels must divide into the groups (C = " +
+                                     std::to_string(C) + ", groups = " + std::to_string(G) + ")");
+  if (C > kMaxChannels) return fail(FSSIM_ERR_SHAPE, "C must be at most 2^24");
+  if (N > kMaxSamples) return fail(FSSIM_ERR_SHAPE, "N must be at most 2^30");
+  if (static_cast<double>(N) * P * C > 1.0e18) return fail(FSSIM_ERR_SHAPE, "N*P*C overflows int64");
+  if (!(eps >= 0.f)) return fail(FSSIM_ERR_ARGUMENT, "eps must not be negative");
+  return FSSIM_OK;
+}
+
+struct ForwardPlan {
+  int V;
+  int64_t cut;     // samples per launch
+  NormGeometry g;  // of a full cut
+  size_t bytes;    // workspace
+};
+
+ForwardPlan plan_forward(const fssim_group_norm_forward_args& a) {
+  ForwardPlan p{};
+  const size_t E = elem_size(a.dtype);
+  p.V = vector_width(a.C, E, a.x, a.y, nullptr);
+  p.cut = samples_per_launch(a.N, a.P * a.C * static_cast<int64_t>(E));
+  p.g = make_geometry(p.cut, a.P, a.C, a.groups, p.V, a.eps);
+  p.bytes = sizeof(float2) * static_cast<size_t>(p.cut) * p.g.S * p.g.slices * p.g.GS;
+  return p;
+}
+
+struct BackwardPlan {
+  int V;
+  int64_t cut;
+  NormGeometry g;
+  size_t partial, chan, coef, bytes;
+};
+
+BackwardPlan plan_backward(const fssim_group_norm_backward_args& a) {
+  BackwardPlan p{};
+  const size_t E = elem_size(a.dtype);
+  p.V = vector_width(a.C, E, a.x, a.dy, a.dx);
+  p.cut = samples_per_launch(a.N, 2 * a.P * a.C * static_cast<int64_t>(E));
+  p.g = make_geometry(p.cut, a.P, a.C, a.groups, p.V, 0.f);
+  p.partial = round256(sizeof(float2) * static_cast<size_t>(p.cut) * p.g.S * a.C);
+  p.chan = round256(sizeof(float2) * static_cast<size_t>(a.N) * a.C);
+  p.coef = round256(sizeof(float2) * static_cast<size_t>(p.cut) * a.groups);
+  p.bytes = p.partial + p.chan + p.coef;
+  return p;
+}
+
+template <typename T, int V, int ACT>
+int forward_kernels(const NormParams& p, cudaStream_t s) {
+  int st = launch(fssim::norm_stats_kernel<T, V, 8>, tile_grid(p.g), p, s, "group norm statistics launch");
+  if (st) return st;
+  return launch(fssim::norm_apply_kernel<T, V, ACT, 4>, tile_grid(p.g), p, s, "group norm launch");
+}
+
+template <typename T, int V, int ACT>
+int backward_kernels(const NormParams& p, cudaStream_t s) {
+  int st = launch(fssim::norm_grad_sums_kernel<T, V, ACT, 4>, tile_grid(p.g), p, s,
+                  "group norm gradient sums launch");
+  if (st) return st;
+  const unsigned y = static_cast<unsigned>(p.g.N < 32768 ? p.g.N : 32768);
+  const unsigned z = static_cast<unsigned>((p.g.N + y - 1) / y);
+  st = launch(fssim::norm_grad_coef_kernel, dim3(static_cast<unsigned>(p.g.G), y, z), p, s,
+              "group norm gradient means launch");
+  if (st || !p.out) return st;
+  return launch(fssim::norm_grad_apply_kernel<T, V, ACT, 4>, tile_grid(p.g), p, s,
+                "group norm gradient launch");
+}
+
+// One launch list per (element type, vector width, activation).
+template <template <typename, int, int> class Run, typename T, int V>
+int by_activation(int act, const NormParams& p, cudaStream_t s) {
+  switch (act) {
+    case FSSIM_ACT_SILU: return Run<T, V, fssim::kNormActSilu>::run(p, s);
+    case FSSIM_ACT_RELU: return Run<T, V, fssim::kNormActRelu>::run(p, s);
+    default: return Run<T, V, fssim::kNormActNone>::run(p, s);
+  }
+}
+template <template <typename, int, int> class Run, typename T>
+int by_width(int V, int act, const NormParams& p, cudaStream_t s) {
+  constexpr int full = 16 / sizeof(T), mid = 4 / sizeof(T);
+  if (V == full) return by_activation<Run, T, full>(act, p, s);
+  if constexpr (mid > 1) {
+    if (V == mid) return by_activation<Run, T, mid>(act, p, s);
+  }
+  return by_activation<Run, T, 1>(act, p, s);
+}
+template <template <typename, int, int> class Run>
+int dispatch(int dtype, int V, int act, const NormParams& p, cudaStream_t s) {
+  switch (dtype) {
+    case FSSIM_F32: return by_width<Run, float>(V, act, p, s);
+    case FSSIM_F16: return by_width<Run, __half>(V, act, p, s);
+    default: return by_width<Run, __nv_bfloat16>(V, act, p, s);
+  }
+}
+template <typename T, int V, int ACT>
+struct Forward {
+  static int run(const NormParams& p, cudaStream_t s) { return forward_kernels<T, V, ACT>(p, s); }
+};
+template <typename T, int V, int ACT>
+struct Backward {
+  static int run(const NormParams& p, cudaStream_t s) { return backward_kernels<T, V, ACT>(p, s); }
+};
+
+int forward_impl(const fssim_group_norm_forward_args* a, cudaStream_t stream) {
+  if (!a) return fail(FSSIM_ERR_NULLPTR, "args is NULL");
+  int st = check_common(a->dtype, a->weight_dtype, a->activation, a->N, a->P, a->C, a->groups, a->eps);
+  if (st) return st;
+  if ((a->mean == nullptr) != (a->rstd == nullptr))
+    return fail(FSSIM_ERR_NULLPTR, "mean and rstd are written together: give both or neither");
+  if (a->N == 0 || a->P == 0) return FSSIM_OK;
+  if (!a->x || !a->y) return fail(FSSIM_ERR_NULLPTR, "x and y are required");
+  const size_t E = elem_size(a->dtype);
+  if (!aligned(a->x, E) || !aligned(a->y, E))
+    return fail(FSSIM_ERR_ARGUMENT, "x and y must be aligned to their element size");
+  const ForwardPlan plan = plan_forward(*a);
+  if (!a->workspace || a->workspace_bytes < plan.bytes)
+    return fail(FSSIM_ERR_WORKSPACE, "workspace smaller than fssim_group_norm_forward_workspace_bytes");
+  if (!aligned(a->workspace, 16)) return fail(FSSIM_ERR_WORKSPACE, "workspace must be 16-byte aligned");
+  for (int64_t n = 0; n < a->N; n += plan.cut) {
+    NormParams p{};
+    p.g = plan.g;
+    p.g.N = a->N - n < plan.cut ? a->N - n : plan.cut;
+    const size_t at = static_cast<size_t>(n) * a->P * a->C * E;
+    p.x = static_cast<const char*>(a->x) + at;
+    p.out = static_cast<char*>(a->y) + at;
+    p.weight = a->weight;
+    p.bias = a->bias;
+    p.weight_dtype = a->weight_dtype;
+    p.mean = a->mean ? a->mean + n * a->groups : nullptr;
+    p.rstd = a->rstd ? a->rstd + n * a->groups : nullptr;
+    p.partial = static_cast<float2*>(a->workspace);
+    st = dispatch<Forward>(a->dtype, plan.V, a->activation, p, stream);
+    if (st) return st;
+  }
+  return FSSIM_OK;
+}
+
+int backward_impl(const fssim_group_norm_backward_args* a, cudaStream_t stream) {
+  if (!a) return fail(FSSIM_ERR_NULLPTR, "args is NULL");
+  int st = check_common(a->dtype, a->weight_dtype, a->activation, a->N, a->P, a->C, a->groups, 0.f);
+  if (st) return st;
+  const size_t WE = elem_size(a->weight_dtype);
+  if (a->N == 0 || a->P == 0) {
+    // nothing was summed: the parameters' gradients are zero
+    for (void* w : {a->dweight, a->dbias})
+      if (w) {
+        const cudaError_t e = cudaMemsetAsync(w, 0, WE * static_cast<size_t>(a->C), stream);
+        if (e != cudaSuccess) return fail(FSSIM_ERR_CUDA, cudaGetErrorString(e));
+      }
+    return FSSIM_OK;
+  }
+  if (!a->dx && !a->dweight && !a->dbias) return FSSIM_OK;
+  if (!a->x || !a->dy) return fail(FSSIM_ERR_NULLPTR, "x and dy are required");
+  if (!a->mean || !a->rstd) return fail(FSSIM_ERR_NULLPTR, "the forward's mean and rstd are required");
+  const size_t E = elem_size(a->dtype);
+  if (!aligned(a->x, E) || !aligned(a->dy, E) || !aligned(a->dx, E))
+    return fail(FSSIM_ERR_ARGUMENT, "x, dy and dx must be aligned to their element size");
+  const BackwardPlan plan = plan_backward(*a);
+  if (!a->workspace || a->workspace_bytes < plan.bytes)
+    return fail(FSSIM_ERR_WORKSPACE, "workspace smaller than fssim_group_norm_backward_workspace_bytes");
+  if (!aligned(a->workspace, 16)) return fail(FSSIM_ERR_WORKSPACE, "workspace must be 16-byte aligned");
+  char* ws = static_cast<char*>(a->workspace);
+  NormParams p{};
+  for (int64_t n = 0; n < a->N; n += plan.cut) {
+    p.g = plan.g;
+    p.g.N = a->N - n < plan.cut ? a->N - n : plan.cut;
+    const size_t at = static_cast<size_t>(n) * a->P * a->C * E;
+    p.x = static_cast<const char*>(a->x) + at;
+    p.dy = static_cast<const char*>(a->dy) + at;
+    p.out = a->dx ? static_cast<char*>(a->dx) + at : nullptr;
+    p.weight = a->weight;
+    p.bias = a->bias;
+    p.weight_dtype = a->weight_dtype;
+    p.mean = const_cast<float*>(a->mean) + n * a->groups;
+    p.rstd = const_cast<float*>(a->rstd) + n * a->groups;
+    p.partial = reinterpret_cast<float2*>(ws);
+    p.chan = reinterpret_cast<float2*>(ws + plan.partial) + n * a->C;
+    p.coef = reinterpret_cast<float2*>(ws + plan.partial + plan.chan);
+    st = dispatch<Backward>(a->dtype, plan.V, a->activation, p, stream);
+    if (st) return st;
+  }
+  if (!a->dweight && !a->dbias) return FSSIM_OK;
+  p.g.N = a->N;
+  p.chan = reinterpret_cast<float2*>(ws + plan.partial);
+  p.dweight = a->dweight;
+  p.dbias = a->dbias;
+  const unsigned blocks = static_cast<unsigned>((a->C + fssim::kNormThreads - 1) / fssim::kNormThreads);
+  return launch(fssim::norm_param_grad_kernel, dim3(blocks), p, stream,
+                "group norm parameter gradient launch");
+}
+
+// No exception crosses the C boundary.
+template <typename F>
+int guarded(F f) {
+  try {
+    fssim_host::g_last_error.clear();
+    return f();
+  } catch (const std::exception&) {
+    return FSSIM_ERR_CUDA;
+  }
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t fssim_group_norm_forward_workspace_bytes(const fssim_group_norm_forward_args* a) {
+  if (!a || a->N <= 0 || a->P <= 0 || a->groups < 1 || a->C < 1 || a->C > kMaxChannels ||
+      a->N > kMaxSamples || a->C % a->groups != 0)
+    return 0;
+  return plan_forward(*a).bytes;
+}
+
+size_t fssim_group_norm_backward_workspace_bytes(const fssim_group_norm_backward_args* a) {
+  if (!a || a->N <= 0 || a->P <= 0 || a->groups < 1 || a->C < 1 || a->C > kMaxChannels ||
+      a->N > kMaxSamples || a->C % a->groups != 0)
+    return 0;
+  return plan_backward(*a).bytes;
+}
+
+int fssim_group_norm_forward(const fssim_group_norm_forward_args* a, fssim_stream_t stream) {
+  NvtxRange range("fssim_group_norm_forward");
+  return guarded([&] { return forward_impl(a, stream); });
+}
+
+int fssim_group_norm_backward(const fssim_group_norm_backward_args* a, fssim_stream_t stream) {
+  NvtxRange range("fssim_group_norm_backward");
+  return guarded([&] { return backward_impl(a, stream); });
+}
+
+}  // extern "C"

@@ -14,6 +14,7 @@
 #include <unordered_map>
 
 #include "fussim_b200.h"
+#include "torch_training.h"
 
 namespace {
 
@@ -479,6 +480,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("ipc_open_handle", &ipc_open_handle);
   m.def("ipc_close_handle", &ipc_close_handle);
   m.def("version", &version);
+  bind_training(m);
   m.def("set_reserved_sms", [](int n) {
     const int st = fssim_set_reserved_sms(n);
     if (st != FSSIM_OK) throw std::invalid_argument(fssim_last_error());

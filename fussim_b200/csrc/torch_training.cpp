@@ -1,0 +1,312 @@
+// Torch binding of the training-step operators over the C ABI (include/fussim_b200.h, section
+// 4): group normalisation with an activation as a C++ autograd function, and the gradient norm
+// with clipping. Everything launches on torch's current CUDA stream of the tensors' device;
+// workspaces are allocated by the call from torch's caching allocator (so calls on different
+// streams, and captured graphs, never share one).
+#include "torch_training.h"
+
+#include <ATen/MemoryOverlap.h>
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+
+#include <algorithm>
+#include <stdexcept>
+#include <string>
+#include <vector>
+
+#include "fussim_b200.h"
+
+namespace {
+
+void check_status(int st) {
+  if (st == FSSIM_OK) return;
+  throw std::runtime_error(std::string("fussim_b200: ") + fssim_status_string(st) + ": " +
+                           fssim_last_error());
+}
+
+fssim_stream_t current_stream() {
+  return reinterpret_cast<fssim_stream_t>(at::cuda::getCurrentCUDAStream().stream());
+}
+
+int dtype_code(at::ScalarType t) {
+  switch (t) {
+    case at::kFloat: return FSSIM_F32;
+    case at::kHalf: return FSSIM_F16;
+    case at::kBFloat16: return FSSIM_BF16;
+    default: throw std::invalid_argument("unsupported dtype for fussim_b200");
+  }
+}
+
+at::Tensor workspace(size_t bytes, const at::Tensor& like) {
+  return at::empty({static_cast<int64_t>(bytes)}, like.options().dtype(at::kByte));
+}
+
+using OptTensor = std::optional<at::Tensor>;
+
+// Weight and bias as the C ABI takes them: dense, of one type (the Python layer has checked
+// device, shape and type).
+struct Affine {
+  at::Tensor weight, bias;
+  int dtype = FSSIM_F32;
+  Affine(const OptTensor& w, const OptTensor& b) {
+    if (w.has_value() && w->defined()) weight = w->contiguous();
+    if (b.has_value() && b->defined()) bias = b->contiguous();
+    if (weight.defined()) dtype = dtype_code(weight.scalar_type());
+    else if (bias.defined()) dtype = dtype_code(bias.scalar_type());
+  }
+  const void* w() const { return weight.defined() ? weight.data_ptr() : nullptr; }
+  const void* b() const { return bias.defined() ? bias.data_ptr() : nullptr; }
+};
+
+struct NormResult {
+  at::Tensor y, mean, rstd;
+};
+
+// x: dense channels-last.
+NormResult norm_forward(const at::Tensor& x, int64_t groups, const Affine& affine, double eps,
+                        int64_t activation, bool with_stats) {
+  const at::cuda::OptionalCUDAGuard guard(x.device());
+  NormResult r;
+  r.y = at::empty(x.sizes(), x.options(), at::MemoryFormat::ChannelsLast);
+  fssim_group_norm_forward_args a{};
+  a.dtype = dtype_code(x.scalar_type());
+  a.weight_dtype = affine.dtype;
+  a.activation = static_cast<int32_t>(activation);
+  a.N = x.size(0);
+  a.C = x.size(1);
+  a.P = x.size(2) * x.size(3);
+  a.groups = groups;
+  a.eps = static_cast<float>(eps);
+  a.x = x.data_ptr();
+  a.weight = affine.w();
+  a.bias = affine.b();
+  a.y = r.y.data_ptr();
+  if (with_stats) {
+    r.mean = at::empty({a.N, groups}, x.options().dtype(at::kFloat));
+    r.rstd = at::empty({a.N, groups}, x.options().dtype(at::kFloat));
+    a.mean = r.mean.data_ptr<float>();
+    a.rstd = r.rstd.data_ptr<float>();
+  }
+  a.workspace_bytes = fssim_group_norm_forward_workspace_bytes(&a);
+  at::Tensor ws;
+  if (a.workspace_bytes) {
+    ws = workspace(a.workspace_bytes, x);
+    a.workspace = ws.data_ptr();
+  }
+  check_status(fssim_group_norm_forward(&a, current_stream()));
+  return r;
+}
+
+struct GroupNormFn : public torch::autograd::Function<GroupNormFn> {
+  static at::Tensor forward(torch::autograd::AutogradContext* ctx, at::Tensor x, OptTensor weight,
+                            OptTensor bias, int64_t groups, double eps, int64_t activation) {
+    const at::Tensor dense = x.contiguous(at::MemoryFormat::ChannelsLast);
+    const Affine affine(weight, bias);
+    const NormResult r = norm_forward(dense, groups, affine, eps, activation, true);
+    ctx->save_for_backward({dense, affine.weight, affine.bias, r.mean, r.rstd});
+    ctx->saved_data["groups"] = groups;
+    ctx->saved_data["act"] = activation;
+    return r.y;
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    TORCH_CHECK(!at::GradMode::is_enabled(),
+                "group_norm_act is differentiable once: its backward cannot be recorded "
+                "(create_graph=True)");
+    const auto saved = ctx->get_saved_variables();
+    const at::Tensor &x = saved[0], &weight = saved[1], &bias = saved[2];
+    const Affine affine(weight, bias);
+    // the gradient slots of the inputs that are tensors, in their order
+    size_t slot = 0;
+    const bool need_x = ctx->needs_input_grad(slot++);
+    const bool need_w = weight.defined() && ctx->needs_input_grad(slot);
+    slot += weight.defined();
+    const bool need_b = bias.defined() && ctx->needs_input_grad(slot);
+    const at::cuda::OptionalCUDAGuard guard(x.device());
+    const at::Tensor dy = grads[0].to(x.scalar_type()).contiguous(at::MemoryFormat::ChannelsLast);
+    at::Tensor dx, dw, db;
+    if (need_x) dx = at::empty(x.sizes(), x.options(), at::MemoryFormat::ChannelsLast);
+    if (need_w) dw = at::empty_like(weight);
+    if (need_b) db = at::empty_like(bias);
+    fssim_group_norm_backward_args a{};
+    a.dtype = dtype_code(x.scalar_type());
+    a.weight_dtype = affine.dtype;
+    a.activation = static_cast<int32_t>(ctx->saved_data["act"].toInt());
+    a.N = x.size(0);
+    a.C = x.size(1);
+    a.P = x.size(2) * x.size(3);
+    a.groups = ctx->saved_data["groups"].toInt();
+    a.x = x.data_ptr();
+    a.dy = dy.data_ptr();
+    a.weight = affine.w();
+    a.bias = affine.b();
+    a.mean = saved[3].data_ptr<float>();
+    a.rstd = saved[4].data_ptr<float>();
+    a.dx = need_x ? dx.data_ptr() : nullptr;
+    a.dweight = need_w ? dw.data_ptr() : nullptr;
+    a.dbias = need_b ? db.data_ptr() : nullptr;
+    a.workspace_bytes = fssim_group_norm_backward_workspace_bytes(&a);
+    at::Tensor ws;
+    if (a.workspace_bytes) {
+      ws = workspace(a.workspace_bytes, x);
+      a.workspace = ws.data_ptr();
+    }
+    check_status(fssim_group_norm_backward(&a, current_stream()));
+    return {dx, dw, db, at::Tensor(), at::Tensor(), at::Tensor()};
+  }
+};
+
+at::Tensor group_norm_act(const at::Tensor& x, int64_t groups, const OptTensor& weight,
+                          const OptTensor& bias, double eps, int64_t activation, bool train) {
+  if (train) return GroupNormFn::apply(x, weight, bias, groups, eps, activation);
+  const at::NoGradGuard no_grad;
+  return norm_forward(x.contiguous(at::MemoryFormat::ChannelsLast), groups, Affine(weight, bias),
+                      eps, activation, false)
+      .y;
+}
+
+// ---- gradient norm and clipping ----
+
+// The memory of a dense tensor, and where the tensor stands in the call.
+struct Span {
+  uintptr_t begin, end;
+  int64_t index;
+  bool out;
+};
+
+Span span_of(const at::Tensor& t, int64_t index, bool out) {
+  const uintptr_t p = reinterpret_cast<uintptr_t>(t.data_ptr());
+  return {p, p + t.numel() * t.element_size(), index, out};
+}
+
+// Refuses outputs that overlap each other or a gradient (but for outs[i] being grads[i]): two
+// CTAs would write the same numbers, or read what another has already scaled. Tensors that
+// do not fill their memory are copied before and after the kernels, which touch the copies
+// alone; of those it is enough that no output is given twice or overlaps itself.
+void check_overlap(const std::vector<at::Tensor>& grads, const std::vector<at::Tensor>& outs) {
+  std::vector<Span> spans, others;
+  spans.reserve(2 * grads.size());
+  const auto refuse = [](int64_t index) {
+    throw std::invalid_argument(
+        "tensors that are written must not overlap themselves, each other or another gradient "
+        "(the same tensor twice, or views of the same memory; at index " +
+        std::to_string(index) + ")");
+  };
+  for (size_t i = 0; i < grads.size(); ++i) {
+    if (grads[i].numel() == 0) continue;
+    const Span o = span_of(outs[i], static_cast<int64_t>(i), true);
+    const Span g = span_of(grads[i], static_cast<int64_t>(i), false);
+    const bool o_dense = outs[i].is_non_overlapping_and_dense();
+    const bool in_place = g.begin == o.begin && g.end == o.end && grads[i].strides() == outs[i].strides();
+    if (o_dense) spans.push_back(o);
+    else if (at::has_internal_overlap(outs[i]) == at::MemOverlap::Yes) refuse(o.index);
+    else others.push_back(o);
+    if (!in_place && grads[i].is_non_overlapping_and_dense()) spans.push_back(g);
+  }
+  const auto by_begin = [](const Span& a, const Span& b) { return a.begin < b.begin; };
+  std::sort(spans.begin(), spans.end(), by_begin);
+  uintptr_t any_end = 0, out_end = 0;  // how far the spans so far reach
+  for (const Span& s : spans) {
+    if (s.begin < (s.out ? any_end : out_end)) refuse(s.index);
+    any_end = std::max(any_end, s.end);
+    if (s.out) out_end = std::max(out_end, s.end);
+  }
+  std::sort(others.begin(), others.end(), by_begin);
+  for (size_t i = 1; i < others.size(); ++i)
+    if (others[i].begin == others[i - 1].begin) refuse(others[i].index);
+}
+
+struct ClipArrays {
+  std::vector<const void*> grads;
+  std::vector<void*> outs;
+  std::vector<int64_t> sizes;
+  std::vector<int32_t> dtypes, out_dtypes;
+  fssim_grad_clip_args args{};
+
+  void add(const at::Tensor& g, const at::Tensor& o) {
+    grads.push_back(g.data_ptr());
+    outs.push_back(o.data_ptr());
+    sizes.push_back(g.numel());
+    dtypes.push_back(dtype_code(g.scalar_type()));
+    out_dtypes.push_back(dtype_code(o.scalar_type()));
+  }
+  const fssim_grad_clip_args* fill(float max_norm, float* norm) {
+    args.count = static_cast<int64_t>(grads.size());
+    args.grads = grads.data();
+    args.sizes = sizes.data();
+    args.dtypes = dtypes.data();
+    args.outs = outs.data();
+    args.out_dtypes = out_dtypes.data();
+    args.max_norm = max_norm;
+    args.norm = norm;
+    args.workspace_bytes = fssim_grad_clip_workspace_bytes(&args);
+    return &args;
+  }
+};
+
+// grads (and outs) are CUDA tensors of one device with matching shapes: the Python layer has
+// checked. Tensors whose numbers fill their memory are taken as they lie; others go through a
+// dense copy.
+at::Tensor grad_norm(const std::vector<at::Tensor>& grads) {
+  const at::NoGradGuard no_grad;
+  const at::cuda::OptionalCUDAGuard guard(grads.at(0).device());
+  at::Tensor norm = at::empty({}, grads[0].options().dtype(at::kFloat));
+  ClipArrays arrays;
+  std::vector<at::Tensor> dense;
+  for (const auto& g : grads) {
+    if (g.is_non_overlapping_and_dense()) {
+      arrays.add(g, g);
+    } else {
+      dense.push_back(g.contiguous());
+      arrays.add(dense.back(), dense.back());
+    }
+  }
+  auto* a = const_cast<fssim_grad_clip_args*>(arrays.fill(0.f, norm.data_ptr<float>()));
+  at::Tensor ws = workspace(a->workspace_bytes, grads[0]);
+  a->workspace = ws.data_ptr();
+  check_status(fssim_grad_norm(a, current_stream()));
+  return norm;
+}
+
+at::Tensor clip_grads(const std::vector<at::Tensor>& grads, const std::vector<at::Tensor>& outs,
+                      double max_norm) {
+  const at::NoGradGuard no_grad;
+  const at::cuda::OptionalCUDAGuard guard(grads.at(0).device());
+  TORCH_CHECK(grads.size() == outs.size(), "one output for each gradient");
+  check_overlap(grads, outs);
+  at::Tensor norm = at::empty({}, grads[0].options().dtype(at::kFloat));
+  ClipArrays arrays;
+  std::vector<at::Tensor> held;                              // dense stand-ins
+  std::vector<std::pair<at::Tensor, at::Tensor>> copy_back;  // (output, its stand-in)
+  for (size_t i = 0; i < grads.size(); ++i) {
+    at::Tensor g = grads[i], o = outs[i];
+    const bool alike = g.strides() == o.strides() && g.is_non_overlapping_and_dense();
+    if (!alike && !(g.is_contiguous() && o.is_contiguous())) {
+      g = g.contiguous();
+      at::Tensor d = at::empty(o.sizes(), o.options(), at::MemoryFormat::Contiguous);
+      held.push_back(g);
+      copy_back.emplace_back(o, d);
+      o = d;
+    }
+    arrays.add(g, o);
+  }
+  auto* a = const_cast<fssim_grad_clip_args*>(
+      arrays.fill(static_cast<float>(max_norm), norm.data_ptr<float>()));
+  at::Tensor ws = workspace(a->workspace_bytes, grads[0]);
+  a->workspace = ws.data_ptr();
+  // the kernels write past autograd's sight: a graph that saved an output has to notice
+  for (const auto& o : outs) o.unsafeGetTensorImpl()->bump_version();
+  check_status(fssim_grad_clip(a, current_stream()));
+  for (auto& [o, d] : copy_back) o.copy_(d);
+  return norm;
+}
+
+}  // namespace
+
+void bind_training(py::module& m) {
+  m.def("group_norm_act", &group_norm_act, py::arg("x"), py::arg("groups"), py::arg("weight"),
+        py::arg("bias"), py::arg("eps"), py::arg("activation"), py::arg("train"));
+  m.def("grad_norm", &grad_norm);
+  m.def("clip_grads", &clip_grads);
+}

@@ -287,6 +287,100 @@ int fssim_forward_dp(const fssim_forward_args* args, const fssim_dp_args* dp,
 /* out[0] = scale * (sum of the world ranks' published sums of step dp->seq, rank order). */
 int fssim_dp_gather(const fssim_dp_args* dp, float scale, float* out, fssim_stream_t stream);
 
+/* ------------------------------------------------------------------------------------
+ * 4. Operators of the training step around the loss (no counterpart in the reference)
+ * ------------------------------------------------------------------------------------ */
+
+typedef enum fssim_activation {
+  FSSIM_ACT_NONE = 0,
+  FSSIM_ACT_SILU = 1, /* z / (1 + exp(-z)) */
+  FSSIM_ACT_RELU = 2  /* max(z, 0) */
+} fssim_activation;
+
+/* Group normalisation with an activation, channels last: x is N samples of P pixels of C
+ * channels, the channels innermost and dense (NHWC). Group (n, g) is the P * C/groups numbers
+ * of sample n in the channels [g*C/groups, (g+1)*C/groups); with its mean and (biased)
+ * variance, rstd = 1/sqrt(var + eps),
+ *     y = act((x - mean) * rstd * weight[c] + bias[c]).
+ * Statistics and arithmetic are FP32 or wider whatever the types; y is rounded once. */
+typedef struct fssim_group_norm_forward_args {
+  int32_t dtype;          /* fssim_dtype of x and y */
+  int32_t weight_dtype;   /* fssim_dtype of weight and bias */
+  int32_t activation;     /* fssim_activation */
+  int64_t N, P, C;        /* samples, pixels per sample, channels (at most 2^24) */
+  int64_t groups;         /* divides C */
+  float eps;              /* >= 0 */
+  const void* x;
+  const void* weight;     /* C values, or NULL (ones) */
+  const void* bias;       /* C values, or NULL (zeros) */
+  void* y;                /* may be x */
+  float* mean;            /* N*groups each: the statistics the backward needs, written */
+  float* rstd;            /*   together; NULL for both when there is no backward */
+  void* workspace;        /* fssim_group_norm_forward_workspace_bytes(args) bytes, 16-byte */
+  size_t workspace_bytes; /*   aligned, contents arbitrary; in use until the call's work ends */
+} fssim_group_norm_forward_args;
+
+/* The gradients of that y for a given dy:
+ *     dz = dy * act'(z), dbias[c] = sum dz, dweight[c] = sum dz * xhat,
+ *     dx = rstd * (w dz - <w dz> - xhat <w dz xhat>), <> the mean over the group. */
+typedef struct fssim_group_norm_backward_args {
+  int32_t dtype;          /* fssim_dtype of x, dy and dx */
+  int32_t weight_dtype;   /* fssim_dtype of weight, bias, dweight and dbias */
+  int32_t activation;
+  int64_t N, P, C;
+  int64_t groups;
+  const void* x;
+  const void* dy;
+  const void* weight;     /* as in the forward */
+  const void* bias;
+  const float* mean;      /* as the forward wrote them */
+  const float* rstd;
+  void* dx;               /* NULL to skip; must not be x or dy */
+  void* dweight;          /* C values each, NULL to skip */
+  void* dbias;
+  void* workspace;        /* fssim_group_norm_backward_workspace_bytes(args) bytes, as above */
+  size_t workspace_bytes;
+} fssim_group_norm_backward_args;
+
+/* Workspace of a call with these arguments (their pointers included: alignment decides how
+ * the tensors are read; workspace and workspace_bytes are not looked at). 0 for arguments
+ * that the call refuses or that leave it nothing to do. */
+size_t fssim_group_norm_forward_workspace_bytes(const fssim_group_norm_forward_args* args);
+size_t fssim_group_norm_backward_workspace_bytes(const fssim_group_norm_backward_args* args);
+
+int fssim_group_norm_forward(const fssim_group_norm_forward_args* args, fssim_stream_t stream);
+int fssim_group_norm_backward(const fssim_group_norm_backward_args* args, fssim_stream_t stream);
+
+/* The 2-norm of many tensors taken together, and clipping by it:
+ *     norm = sqrt(sum over all tensors of g^2), coef = min(1, max_norm / (norm + 1e-6)),
+ *     outs[i] = coef * grads[i].
+ * Tensors are flat runs of device memory; the arrays below are host memory and are read
+ * during the call. Squares are summed in FP64 beyond eight numbers, in a fixed order. A norm
+ * that is NaN makes every output NaN; an infinite one gives 0 (NaN where g is infinite). */
+typedef struct fssim_grad_clip_args {
+  int64_t count;              /* tensors */
+  const void* const* grads;   /* device pointer of each (may be NULL where its size is 0) */
+  const int64_t* sizes;       /* numbers in each */
+  const int32_t* dtypes;      /* fssim_dtype of each */
+  void* const* outs;          /* fssim_grad_clip: where each goes; outs[i] may be grads[i] (in
+                               * place: left untouched when coef is 1); otherwise no output may
+                               * overlap a gradient or another output */
+  const int32_t* out_dtypes;  /* its gradient's type, or F32 */
+  float max_norm;             /* >= 0 */
+  float* norm;                /* device memory: one FP32, written */
+  void* workspace;            /* fssim_grad_clip_workspace_bytes(args) bytes of device memory, */
+  size_t workspace_bytes;     /*   8-byte aligned, contents arbitrary */
+} fssim_grad_clip_args;
+
+/* Workspace of a call with these count and sizes (nothing else is looked at). */
+size_t fssim_grad_clip_workspace_bytes(const fssim_grad_clip_args* args);
+
+/* The norm alone (outs, out_dtypes and max_norm are not looked at). */
+int fssim_grad_norm(const fssim_grad_clip_args* args, fssim_stream_t stream);
+
+/* Norm and clipping. */
+int fssim_grad_clip(const fssim_grad_clip_args* args, fssim_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
