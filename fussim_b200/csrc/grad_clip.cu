@@ -114,7 +114,7 @@ int check(const fssim_grad_clip_args* a, bool clip) {
 template <int K>
 int launch_cut(const fssim_grad_clip_args& a, const Cut& c, bool clip, int partials, int first,
                cudaStream_t stream) {
-  auto t = std::make_unique<ClipTable<K>>();
+  const std::unique_ptr<ClipTable<K>> t(new ClipTable<K>);
   int r = 0;
   int64_t unit = 0;
   for (int64_t i = c.begin; i < c.end; ++i) {

@@ -46,12 +46,17 @@ struct ClipTable {
   float max_norm;
 };
 
+// Eight consecutive numbers at a 16-byte boundary: as they lie in memory (16 or 32 bytes, so that
+// several such loads can be in flight before the first is converted), and as FP32.
 template <typename T> struct ClipVec;
 template <> struct ClipVec<float> {
-  static constexpr int n = 4;
-  static __device__ __forceinline__ void load(const float* p, float* f) {
-    const float4 v = *reinterpret_cast<const float4*>(p);
-    f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w;
+  struct Raw { float4 a, b; };
+  static __device__ __forceinline__ Raw load8(const float* p) {
+    return {reinterpret_cast<const float4*>(p)[0], reinterpret_cast<const float4*>(p)[1]};
+  }
+  static __device__ __forceinline__ void unpack(const Raw& r, float (&f)[8]) {
+    f[0] = r.a.x; f[1] = r.a.y; f[2] = r.a.z; f[3] = r.a.w;
+    f[4] = r.b.x; f[5] = r.b.y; f[6] = r.b.z; f[7] = r.b.w;
   }
   static __device__ __forceinline__ float one(const float* p) { return *p; }
   static __device__ __forceinline__ void store8(float* p, const float* f) {
@@ -60,57 +65,41 @@ template <> struct ClipVec<float> {
   }
   static __device__ __forceinline__ void put(float* p, float f) { *p = f; }
 };
-template <> struct ClipVec<__half> {
-  static constexpr int n = 8;
-  static __device__ __forceinline__ void load(const __half* p, float* f) {
-    const uint4 v = *reinterpret_cast<const uint4*>(p);
-    const __half2* h = reinterpret_cast<const __half2*>(&v);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 t = __half22float2(h[i]);
-      f[2 * i] = t.x;
-      f[2 * i + 1] = t.y;
-    }
-  }
-  static __device__ __forceinline__ float one(const __half* p) { return __half2float(*p); }
-  static __device__ __forceinline__ void store8(__half* p, const float* f) {
-    uint4 v;
-    __half2* h = reinterpret_cast<__half2*>(&v);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) h[i] = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
-    *reinterpret_cast<uint4*>(p) = v;
-  }
-  static __device__ __forceinline__ void put(__half* p, float f) { *p = __float2half_rn(f); }
-};
-template <> struct ClipVec<__nv_bfloat16> {
-  static constexpr int n = 8;
-  static __device__ __forceinline__ void load(const __nv_bfloat16* p, float* f) {
-    const uint4 v = *reinterpret_cast<const uint4*>(p);
-    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 t = __bfloat1622float2(h[i]);
-      f[2 * i] = t.x;
-      f[2 * i + 1] = t.y;
-    }
-  }
-  static __device__ __forceinline__ float one(const __nv_bfloat16* p) { return __bfloat162float(*p); }
-  static __device__ __forceinline__ void store8(__nv_bfloat16* p, const float* f) {
-    uint4 v;
-    __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&v);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) h[i] = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
-    *reinterpret_cast<uint4*>(p) = v;
-  }
-  static __device__ __forceinline__ void put(__nv_bfloat16* p, float f) { *p = __float2bfloat16_rn(f); }
-};
-
-// Eight consecutive numbers at a 16-byte boundary.
-template <typename T>
-__device__ __forceinline__ void clip_load8(const T* p, float (&f)[8]) {
-#pragma unroll
-  for (int i = 0; i < 8; i += ClipVec<T>::n) ClipVec<T>::load(p + i, f + i);
+__device__ __forceinline__ float2 clip_widen(__half2 v) { return __half22float2(v); }
+__device__ __forceinline__ float2 clip_widen(__nv_bfloat162 v) { return __bfloat1622float2(v); }
+__device__ __forceinline__ void clip_narrow(__half2& v, float a, float b) { v = __floats2half2_rn(a, b); }
+__device__ __forceinline__ void clip_narrow(__nv_bfloat162& v, float a, float b) {
+  v = __floats2bfloat162_rn(a, b);
 }
+__device__ __forceinline__ void clip_narrow(__half& v, float a) { v = __float2half_rn(a); }
+__device__ __forceinline__ void clip_narrow(__nv_bfloat16& v, float a) { v = __float2bfloat16_rn(a); }
+template <typename T, typename T2>
+struct ClipVec16 {
+  using Raw = uint4;
+  static __device__ __forceinline__ Raw load8(const T* p) { return *reinterpret_cast<const uint4*>(p); }
+  static __device__ __forceinline__ void unpack(const Raw& r, float (&f)[8]) {
+    const T2* h = reinterpret_cast<const T2*>(&r);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 t = clip_widen(h[i]);
+      f[2 * i] = t.x;
+      f[2 * i + 1] = t.y;
+    }
+  }
+  static __device__ __forceinline__ float one(const T* p) { return static_cast<float>(*p); }
+  static __device__ __forceinline__ void store8(T* p, const float* f) {
+    uint4 v;
+    T2* h = reinterpret_cast<T2*>(&v);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) clip_narrow(h[i], f[2 * i], f[2 * i + 1]);
+    *reinterpret_cast<uint4*>(p) = v;
+  }
+  static __device__ __forceinline__ void put(T* p, float f) { clip_narrow(*p, f); }
+};
+template <>
+struct ClipVec<__half> : ClipVec16<__half, __half2> {};
+template <>
+struct ClipVec<__nv_bfloat16> : ClipVec16<__nv_bfloat16, __nv_bfloat162> {};
 
 // Squares of eight numbers, added up. Between 2^-80 and 2^100 the FP32 sum is right to a few
 // of its roundings: no term overflowed, and what underflowed is below 2^-46 of the sum.
@@ -171,18 +160,23 @@ __device__ __forceinline__ double clip_piece_squares(const T* src, int64_t b, in
   const int64_t body = b + head;
   const int64_t n8 = (e - body) / 8;
   const int64_t tail = body + n8 * 8;
-  constexpr int U = 4;
+  using IO = ClipVec<T>;
+  constexpr int U = 128 / sizeof(typename IO::Raw);  // 128 bytes of a thread in flight
   int64_t i = threadIdx.x;
   for (; i + (U - 1) * kClipThreads < n8; i += U * kClipThreads) {
-    float f[U][8];
+    typename IO::Raw raw[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) clip_load8(src + body + (i + u * kClipThreads) * 8, f[u]);
+    for (int u = 0; u < U; ++u) raw[u] = IO::load8(src + body + (i + u * kClipThreads) * 8);
 #pragma unroll
-    for (int u = 0; u < U; ++u) acc += sum_squares8(f[u]);
+    for (int u = 0; u < U; ++u) {
+      float f[8];
+      IO::unpack(raw[u], f);
+      acc += sum_squares8(f);
+    }
   }
   for (; i < n8; i += kClipThreads) {
     float f[8];
-    clip_load8(src + body + i * 8, f);
+    IO::unpack(IO::load8(src + body + i * 8), f);
     acc += sum_squares8(f);
   }
   // what is left at the two ends: fewer than 8 numbers each
@@ -216,26 +210,24 @@ __device__ __forceinline__ void clip_piece_scale(const S* src, D* dst, int64_t b
   }
   const int64_t n8 = (e - body) / 8;
   const int64_t tail = body + n8 * 8;
-  constexpr int U = 2;
-  int64_t i = threadIdx.x;
-  for (; i + (U - 1) * kClipThreads < n8; i += U * kClipThreads) {
-    float f[U][8];
-#pragma unroll
-    for (int u = 0; u < U; ++u) clip_load8(src + body + (i + u * kClipThreads) * 8, f[u]);
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-#pragma unroll
-      for (int k = 0; k < 8; ++k) f[u][k] = coef * f[u][k];
-      ClipVec<D>::store8(dst + body + (i + u * kClipThreads) * 8, f[u]);
-    }
-  }
-  for (; i < n8; i += kClipThreads) {
+  using IO = ClipVec<S>;
+  constexpr int U = 64 / sizeof(typename IO::Raw);
+  const auto emit = [&](const typename IO::Raw& raw, int64_t at) {
     float f[8];
-    clip_load8(src + body + i * 8, f);
+    IO::unpack(raw, f);
 #pragma unroll
     for (int k = 0; k < 8; ++k) f[k] = coef * f[k];
-    ClipVec<D>::store8(dst + body + i * 8, f);
+    ClipVec<D>::store8(dst + body + at * 8, f);
+  };
+  int64_t i = threadIdx.x;
+  for (; i + (U - 1) * kClipThreads < n8; i += U * kClipThreads) {
+    typename IO::Raw raw[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) raw[u] = IO::load8(src + body + (i + u * kClipThreads) * 8);
+#pragma unroll
+    for (int u = 0; u < U; ++u) emit(raw[u], i + u * kClipThreads);
   }
+  for (; i < n8; i += kClipThreads) emit(IO::load8(src + body + i * 8), i);
   const int64_t ends = head + (e - tail);
   if (threadIdx.x < ends) {
     const int64_t at = threadIdx.x < head ? b + threadIdx.x : tail + (threadIdx.x - head);

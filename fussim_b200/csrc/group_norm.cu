@@ -19,8 +19,8 @@ using fssim_host::NvtxRange;
 
 constexpr int64_t kMaxChannels = int64_t{1} << 24;
 constexpr int64_t kMaxSamples = int64_t{1} << 30;
-// CTAs a launch aims at: four of 256 threads on each of 148 SMs.
-constexpr int64_t kTargetCtas = 148 * 4;
+// CTAs of one wave: two of 256 threads on each of 148 SMs.
+constexpr int64_t kWave = 148 * 2;
 // A part has at least this many pixels for each thread, so that its set-up is paid for.
 constexpr int64_t kMinSteps = 4;
 // Bytes of input that the reducing pass may leave for the applying pass to find in L2.
@@ -57,11 +57,16 @@ NormGeometry make_geometry(int64_t N, int64_t P, int64_t C, int64_t G, int V, fl
   g.rows = fssim::kNormThreads / g.lanes;
   g.GS = g.slices == 1 ? g.G : static_cast<int>((g.SC + g.Cg - 2) / g.Cg + 1);
   if (g.GS > g.G) g.GS = g.G;
-  int64_t S = kTargetCtas / (N * g.slices);
+  // Parts: one wave of CTAs, or where the samples are more than that, enough that the last
+  // wave's idle SMs weigh little.
+  const int64_t tiles = N * g.slices;
+  int64_t S = tiles <= kWave ? kWave / tiles : (4 * kWave + tiles - 1) / tiles;
   const int64_t by_work = P / (g.rows * kMinSteps);
   if (S > by_work) S = by_work;
   if (S < 1) S = 1;
   g.S = static_cast<int>(S);
+  g.base = P / S;
+  g.extra = static_cast<int>(P % S);
   return g;
 }
 
@@ -109,6 +114,7 @@ int check_common(int dtype, int weight_dtype, int activation, int64_t N, int64_t
                                      std::to_string(C) + ", groups = " + std::to_string(G) + ")");
   if (C > kMaxChannels) return fail(FSSIM_ERR_SHAPE, "C must be at most 2^24");
   if (N > kMaxSamples) return fail(FSSIM_ERR_SHAPE, "N must be at most 2^30");
+  if (N * G > INT_MAX) return fail(FSSIM_ERR_SHAPE, "N*groups must be < 2^31");
   if (static_cast<double>(N) * P * C > 1.0e18) return fail(FSSIM_ERR_SHAPE, "N*P*C overflows int64");
   if (!(eps >= 0.f)) return fail(FSSIM_ERR_ARGUMENT, "eps must not be negative");
   return FSSIM_OK;
@@ -118,7 +124,7 @@ struct ForwardPlan {
   int V;
   int64_t cut;     // samples per launch
   NormGeometry g;  // of a full cut
-  size_t bytes;    // workspace
+  size_t partial, bytes;
 };
 
 ForwardPlan plan_forward(const fssim_group_norm_forward_args& a) {
@@ -127,7 +133,8 @@ ForwardPlan plan_forward(const fssim_group_norm_forward_args& a) {
   p.V = vector_width(a.C, E, a.x, a.y, nullptr);
   p.cut = samples_per_launch(a.N, a.P * a.C * static_cast<int64_t>(E));
   p.g = make_geometry(p.cut, a.P, a.C, a.groups, p.V, a.eps);
-  p.bytes = sizeof(float2) * static_cast<size_t>(p.cut) * p.g.S * p.g.slices * p.g.GS;
+  p.partial = round256(sizeof(float2) * static_cast<size_t>(p.cut) * p.g.S * p.g.slices * p.g.GS);
+  p.bytes = p.partial + sizeof(float) * fssim::kNormForwardRows * static_cast<size_t>(p.cut) * a.C;
   return p;
 }
 
@@ -135,7 +142,7 @@ struct BackwardPlan {
   int V;
   int64_t cut;
   NormGeometry g;
-  size_t partial, chan, coef, bytes;
+  size_t partial, sums, bytes;
 };
 
 BackwardPlan plan_backward(const fssim_group_norm_backward_args& a) {
@@ -145,15 +152,19 @@ BackwardPlan plan_backward(const fssim_group_norm_backward_args& a) {
   p.cut = samples_per_launch(a.N, 2 * a.P * a.C * static_cast<int64_t>(E));
   p.g = make_geometry(p.cut, a.P, a.C, a.groups, p.V, 0.f);
   p.partial = round256(sizeof(float2) * static_cast<size_t>(p.cut) * p.g.S * a.C);
-  p.chan = round256(sizeof(float2) * static_cast<size_t>(a.N) * a.C);
-  p.coef = round256(sizeof(float2) * static_cast<size_t>(p.cut) * a.groups);
-  p.bytes = p.partial + p.chan + p.coef;
+  p.sums = round256(sizeof(float2) * static_cast<size_t>(a.N) * a.C);
+  p.bytes = p.partial + p.sums + sizeof(float) * fssim::kNormBackwardRows * static_cast<size_t>(p.cut) * a.C;
   return p;
 }
 
 template <typename T, int V, int ACT>
 int forward_kernels(const NormParams& p, cudaStream_t s) {
   int st = launch(fssim::norm_stats_kernel<T, V, 8>, tile_grid(p.g), p, s, "group norm statistics launch");
+  if (st) return st;
+  const int64_t groups = p.g.N * p.g.G;
+  st = launch(fssim::norm_merge_kernel,
+              dim3(static_cast<unsigned>((groups + fssim::kNormWarps - 1) / fssim::kNormWarps)), p, s,
+              "group norm merge launch");
   if (st) return st;
   return launch(fssim::norm_apply_kernel<T, V, ACT, 4>, tile_grid(p.g), p, s, "group norm launch");
 }
@@ -163,9 +174,7 @@ int backward_kernels(const NormParams& p, cudaStream_t s) {
   int st = launch(fssim::norm_grad_sums_kernel<T, V, ACT, 4>, tile_grid(p.g), p, s,
                   "group norm gradient sums launch");
   if (st) return st;
-  const unsigned y = static_cast<unsigned>(p.g.N < 32768 ? p.g.N : 32768);
-  const unsigned z = static_cast<unsigned>((p.g.N + y - 1) / y);
-  st = launch(fssim::norm_grad_coef_kernel, dim3(static_cast<unsigned>(p.g.G), y, z), p, s,
+  st = launch(fssim::norm_grad_coef_kernel, dim3(static_cast<unsigned>(p.g.N * p.g.G)), p, s,
               "group norm gradient means launch");
   if (st || !p.out) return st;
   return launch(fssim::norm_grad_apply_kernel<T, V, ACT, 4>, tile_grid(p.g), p, s,
@@ -235,6 +244,8 @@ int forward_impl(const fssim_group_norm_forward_args* a, cudaStream_t stream) {
     p.mean = a->mean ? a->mean + n * a->groups : nullptr;
     p.rstd = a->rstd ? a->rstd + n * a->groups : nullptr;
     p.partial = static_cast<float2*>(a->workspace);
+    p.channel = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + plan.partial);
+    p.early = n > 0;
     st = dispatch<Forward>(a->dtype, plan.V, a->activation, p, stream);
     if (st) return st;
   }
@@ -280,14 +291,15 @@ int backward_impl(const fssim_group_norm_backward_args* a, cudaStream_t stream) 
     p.mean = const_cast<float*>(a->mean) + n * a->groups;
     p.rstd = const_cast<float*>(a->rstd) + n * a->groups;
     p.partial = reinterpret_cast<float2*>(ws);
-    p.chan = reinterpret_cast<float2*>(ws + plan.partial) + n * a->C;
-    p.coef = reinterpret_cast<float2*>(ws + plan.partial + plan.chan);
+    p.sums = reinterpret_cast<float2*>(ws + plan.partial) + n * a->C;
+    p.channel = reinterpret_cast<float*>(ws + plan.partial + plan.sums);
+    p.early = n > 0 && a->dx != nullptr;
     st = dispatch<Backward>(a->dtype, plan.V, a->activation, p, stream);
     if (st) return st;
   }
   if (!a->dweight && !a->dbias) return FSSIM_OK;
   p.g.N = a->N;
-  p.chan = reinterpret_cast<float2*>(ws + plan.partial);
+  p.sums = reinterpret_cast<float2*>(ws + plan.partial);
   p.dweight = a->dweight;
   p.dbias = a->dbias;
   const unsigned blocks = static_cast<unsigned>((a->C + fssim::kNormThreads - 1) / fssim::kNormThreads);

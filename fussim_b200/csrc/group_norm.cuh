@@ -13,20 +13,23 @@
 // slice). A thread keeps one vector of channels for the whole part and steps over its pixels,
 // so the per-channel constants and sums stay in registers and a warp reads whole rows of
 // memory. The group's numbers must all be seen before its first output, so each direction is
-// a reducing pass and an applying pass; the second read comes from L2 when the samples that
-// are in flight fit it (the host cuts the batch accordingly).
+// a reducing pass, a small launch that merges the parts, and an applying pass; the second read
+// comes from L2 where the samples in flight fit it (the host cuts the batch accordingly), from
+// the end of each part backwards, because that is what the reducing pass read last.
 //
 // Statistics: a thread takes U pixels at a time, forms each channel's mean and sum of squared
 // deviations of those U values (two passes over registers), and merges them into its running
 // pair (the pairwise update of Chan, Golub and LeVeque, 1979). No sum of raw squares is ever
-// formed, so a mean far from zero costs no digits. Threads, parts and slices are merged the
-// same way, in a fixed order (results repeat bit for bit), across parts in FP64.
+// formed, so a mean far from zero costs no digits. Threads, channels, parts and slices are
+// merged likewise, in a fixed order (results repeat bit for bit), across parts in FP64.
 #pragma once
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
+
+#include <type_traits>
 
 #include "pdl.cuh"
 
@@ -49,7 +52,11 @@ struct NormGeometry {
   int GS;      // most groups that touch one slice
   float eps;
 
-  __host__ __device__ int64_t part_begin(int64_t s) const { return P / S * s + (P % S) * s / S; }
+  int64_t base;  // pixels of a part; the first `extra` parts have one more
+  int extra;
+
+  __device__ __forceinline__ int64_t part_pixels(int s) const { return base + (s < extra); }
+  __device__ __forceinline__ int64_t part_begin(int s) const { return base * s + min(s, extra); }
 };
 
 struct NormParams {
@@ -64,11 +71,17 @@ struct NormParams {
   float* rstd;          // N * G
   float2* partial;      // forward: (mean, M2) per (sample, part, slice, group of the slice)
                         // backward: (sum dz, sum dz (x - mean)) per (sample, part, channel)
-  float2* chan;         // backward: (sum dz, sum dz xhat) per (sample, channel)
-  float2* coef;         // backward: (rstd <w dz>, rstd^2 <w dz xhat>) per (sample, group)
+  float2* sums;         // backward: (sum dz, sum dz xhat) per (sample, channel)
+  float* channel;       // what the applying pass needs, C values each, per sample: the mean, the
+                        // factor a = rstd w and the shift b (kNormForwardRows rows); in the
+                        // backward also rstd <w dz> and rstd^2 <w dz xhat> (kNormBackwardRows)
+  int early;            // a reducing pass that need not wait for the launch before it to begin
   void* dweight;
   void* dbias;
 };
+
+constexpr int kNormForwardRows = 3;
+constexpr int kNormBackwardRows = 5;
 
 // ---- element types ----
 template <int BYTES> struct RawVec;
@@ -122,6 +135,21 @@ __device__ __forceinline__ void store_weight(void* p, int dtype, int c, float v)
   else static_cast<__nv_bfloat16*>(p)[c] = __float2bfloat16_rn(v);
 }
 
+// V consecutive values of a row of `channel`, which starts at a multiple of V floats.
+template <int V>
+__device__ __forceinline__ void load_channels(const float* p, float (&f)[V]) {
+  if constexpr (V % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i < V; i += 4) {
+      const float4 v = *reinterpret_cast<const float4*>(p + i);
+      f[i] = v.x; f[i + 1] = v.y; f[i + 2] = v.z; f[i + 3] = v.w;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) f[i] = p[i];
+  }
+}
+
 // ---- activations ----
 // The logistic function. For 16-bit tensors the hardware's approximate exponential and
 // reciprocal do (relative errors near 2^-21, against a half step of 2^-9 or 2^-12 in the
@@ -163,7 +191,7 @@ __device__ __forceinline__ double warp_sum(double v) {
 
 // A CTA's place in the work split.
 struct NormTile {
-  int64_t n;         // sample
+  int n;             // sample
   int s;             // part
   int slice;
   int c0, c1;        // channels of the slice
@@ -173,19 +201,79 @@ struct NormTile {
   bool active;
 
   __device__ __forceinline__ NormTile(const NormGeometry& g, int V) {
-    const int64_t b = blockIdx.x;
-    n = b / g.S;
-    s = static_cast<int>(b - n * g.S);
+    n = blockIdx.x / g.S;
+    s = blockIdx.x - n * g.S;
     slice = blockIdx.y;
     c0 = slice * g.SC;
     c1 = min(c0 + g.SC, g.C);
     g0 = c0 / g.Cg;
     g1 = (c1 - 1) / g.Cg + 1;
     p0 = g.part_begin(s);
-    p1 = g.part_begin(s + 1);
+    p1 = p0 + g.part_pixels(s);
     row = threadIdx.x / g.lanes;
     chan = (threadIdx.x - row * g.lanes) * V;
     active = row < g.rows && c0 + chan < c1;
+  }
+};
+
+// First channel, from the slice's first, of the group that channel c of the slice is in.
+__device__ __forceinline__ int group_begin(const NormGeometry& g, const NormTile& t, int c) {
+  return max((t.c0 + c) / g.Cg * g.Cg - t.c0, 0);
+}
+
+// out[c] = sum over the rows r of f(r, c), for the `width` channels of a slice: L lanes (a power
+// of two, at most a warp) for each channel. All threads take part.
+template <typename F>
+__device__ __forceinline__ void norm_sum_rows(int rows, int pitch, int width, float* out, F f) {
+  const int L = rows >= 32 ? 32 : 1 << (31 - __clz(rows));
+  const int sub = threadIdx.x & (L - 1), each = kNormThreads / L;
+  for (int b = 0; b < width; b += each) {
+    const int c = b + threadIdx.x / L;
+    float v = 0.f;
+    if (c < width)
+      for (int r = sub; r < rows; r += L) v += f(r, c);
+    for (int o = L / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if (c < width && sub == 0) out[c] = v;
+  }
+}
+
+// f(i, cb, w, sum of in[cb .. cb + w)) for the i-th group that touches the slice, its channels
+// [cb, cb + w) of the slice: a thread for each narrow group, a warp for each wide one.
+template <typename F>
+__device__ __forceinline__ void norm_sum_groups(const NormGeometry& g, const NormTile& t, const float* in, F f) {
+  const bool narrow = g.Cg <= 32;
+  const int lane = narrow ? 0 : threadIdx.x % 32, lanes = narrow ? 1 : 32;
+  for (int i = threadIdx.x / lanes; i < t.g1 - t.g0; i += kNormThreads / lanes) {
+    const int cb = max((t.g0 + i) * g.Cg, t.c0) - t.c0;
+    const int w = min((t.g0 + i + 1) * g.Cg, t.c1) - t.c0 - cb;
+    float v = 0.f;
+    for (int c = lane; c < w; c += lanes) v += in[cb + c];
+    if (!narrow) v = warp_sum(v);
+    if (lane == 0) f(i, cb, w, v);
+  }
+}
+
+// The pixels of a thread in the applying passes: from the end of its part to the beginning (what
+// the reducing pass read last is what L2 still holds), U at a time; the last step, at the
+// beginning of the part, may be short.
+template <int U>
+struct NormSteps {
+  int64_t at;      // first pixel of the current step
+  int64_t left;    // pixels still to do, the current step's among them
+  int rows;
+
+  __device__ __forceinline__ NormSteps(const NormGeometry& g, const NormTile& t) : rows(g.rows) {
+    const int64_t first = t.p0 + t.row;
+    left = t.active && first < t.p1 ? (t.p1 - first - 1) / rows + 1 : 0;
+    at = first + (left - U) * rows;
+  }
+  __device__ __forceinline__ bool more() const { return left > 0; }
+  // the short step lacks its first pixels
+  __device__ __forceinline__ bool has(int u) const { return left >= U || u >= U - left; }
+  __device__ __forceinline__ int64_t pixel(int u) const { return at + static_cast<int64_t>(u) * rows; }
+  __device__ __forceinline__ void next() {
+    at -= static_cast<int64_t>(U) * rows;
+    left -= U;
   }
 };
 
@@ -194,56 +282,58 @@ template <typename T, int V, int U>
 __global__ void __launch_bounds__(kNormThreads) norm_stats_kernel(const __grid_constant__ NormParams p) {
   __shared__ float sm_mean[kNormThreads * V];
   __shared__ float sm_m2[kNormThreads * V];
+  __shared__ float column[kNormThreads * V];
+  __shared__ float centre[kNormThreads * V];
   const NormGeometry& g = p.g;
   const NormTile t(g, V);
-  grid_dependency_wait();
+  if (!p.early) grid_dependency_wait();
   grid_launch_dependents();
   using IO = VecIO<T, V>;
   float mean[V], m2[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) mean[v] = m2[v] = 0.f;
   if (t.active) {
-    const T* x = static_cast<const T*>(p.x) + t.n * g.P * g.C + t.c0 + t.chan;
+    const T* x = static_cast<const T*>(p.x) + static_cast<int64_t>(t.n) * g.P * g.C + t.c0 + t.chan;
     const int64_t step = static_cast<int64_t>(g.rows);
     float count = 0.f;
     int64_t px = t.p0 + t.row;
-    for (; px + (U - 1) * step < t.p1; px += U * step) {
+    // U pixels, or the last k of them (k < U) with the missing ones left out
+    auto take = [&](auto whole, int k) {
+      constexpr bool kWhole = decltype(whole)::value;
       typename IO::Raw raw[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) raw[u] = IO::load(x + (px + u * step) * g.C);
+      for (int u = 0; u < U; ++u) {
+        if (kWhole || u < k) raw[u] = IO::load(x + (px + u * step) * g.C);
+        else raw[u] = typename IO::Raw{};
+      }
       float f[U][V];
 #pragma unroll
       for (int u = 0; u < U; ++u) IO::unpack(raw[u], f[u]);
-      const float total = count + U;
-      const float share = U / total;          // weight of the new values in the mean
-      const float cross = count * share;      // and of the squared distance of the two means
+      const float taken = kWhole ? U : k;
+      const float total = count + taken;
+      const float each = kWhole ? 1.f / U : 1.f / taken;
+      const float share = taken / total;   // weight of the new values in the mean
+      const float cross = count * share;   // and of the squared distance of the means
 #pragma unroll
       for (int v = 0; v < V; ++v) {
         float sum = 0.f;
 #pragma unroll
         for (int u = 0; u < U; ++u) sum += f[u][v];
-        const float m = sum * (1.f / U);
+        const float m = sum * each;
         float q = 0.f;
 #pragma unroll
-        for (int u = 0; u < U; ++u) q = fmaf(f[u][v] - m, f[u][v] - m, q);
+        for (int u = 0; u < U; ++u) {
+          const float d = kWhole || u < k ? f[u][v] - m : 0.f;
+          q = fmaf(d, d, q);
+        }
         const float d = m - mean[v];
         mean[v] = fmaf(d, share, mean[v]);
         m2[v] += fmaf(d * d, cross, q);
       }
       count = total;
-    }
-    for (; px < t.p1; px += step) {
-      float f[V];
-      IO::unpack(IO::load(x + px * g.C), f);
-      count += 1.f;
-      const float share = 1.f / count;
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        const float d = f[v] - mean[v];
-        mean[v] = fmaf(d, share, mean[v]);
-        m2[v] = fmaf(d, f[v] - mean[v], m2[v]);
-      }
-    }
+    };
+    for (; px + (U - 1) * step < t.p1; px += U * step) take(std::true_type{}, U);
+    if (px < t.p1) take(std::false_type{}, static_cast<int>((t.p1 - px - 1) / step) + 1);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       sm_mean[t.row * g.SC + t.chan + v] = mean[v];
@@ -251,115 +341,120 @@ __global__ void __launch_bounds__(kNormThreads) norm_stats_kernel(const __grid_c
     }
   }
   __syncthreads();
-  // one warp per group: the rows' and channels' pairs become one pair
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  // The rows' and channels' pairs become one pair per group: first the mean (as distances from
+  // one of the means, so that equal values give that value exactly), then the deviations.
   const int64_t pixels = t.p1 - t.p0;
-  const int64_t full = pixels / g.rows;                      // pixels that every row took
+  const int64_t full = pixels / g.rows;                        // pixels that every row took
   const int extra = static_cast<int>(pixels - full * g.rows);  // rows that took one more
-  for (int grp = t.g0 + warp; grp < t.g1; grp += kNormWarps) {
-    const int cb = max(grp * g.Cg, t.c0), width = min((grp + 1) * g.Cg, t.c1) - cb;
-    const int entries = g.rows * width;
-    // means are averaged as distances from one of them: equal values give that value exactly
-    const float ref = sm_mean[cb - t.c0];
-    float sum = 0.f;
-    for (int i = lane; i < entries; i += 32) {
-      const int r = i / width;
-      const float cnt = static_cast<float>(full + (r < extra));
-      sum += cnt > 0.f ? cnt * (sm_mean[r * g.SC + cb - t.c0 + i - r * width] - ref) : 0.f;
-    }
-    const float m = ref + warp_sum(sum) / (static_cast<float>(pixels) * width);
-    float q = 0.f;
-    for (int i = lane; i < entries; i += 32) {
-      const int r = i / width, at = r * g.SC + cb - t.c0 + i - r * width;
-      const float cnt = static_cast<float>(full + (r < extra));
-      const float d = sm_mean[at] - m;
-      q += cnt > 0.f ? fmaf(cnt * d, d, sm_m2[at]) : 0.f;
-    }
-    q = warp_sum(q);
-    if (lane == 0)
-      p.partial[((t.n * g.S + t.s) * g.slices + t.slice) * g.GS + grp - t.g0] = make_float2(m, q);
-  }
+  const int width = t.c1 - t.c0;
+  const auto count_of = [&](int row) { return static_cast<float>(full + (row < extra)); };
+  norm_sum_rows(g.rows, g.SC, width, column, [&](int r, int c) {
+    const float cnt = count_of(r);
+    return cnt > 0.f ? cnt * (sm_mean[r * g.SC + c] - sm_mean[group_begin(g, t, c)]) : 0.f;
+  });
+  __syncthreads();
+  float2* partial = p.partial + ((static_cast<int64_t>(t.n) * g.S + t.s) * g.slices + t.slice) * g.GS;
+  norm_sum_groups(g, t, column, [&](int i, int cb, int w, float sum) {
+    centre[i] = sm_mean[cb] + sum / (static_cast<float>(pixels) * w);
+  });
+  __syncthreads();
+  norm_sum_rows(g.rows, g.SC, width, column, [&](int r, int c) {
+    const float cnt = count_of(r);
+    const float d = sm_mean[r * g.SC + c] - centre[(t.c0 + c) / g.Cg - t.g0];
+    return cnt > 0.f ? fmaf(cnt * d, d, sm_m2[r * g.SC + c]) : 0.f;
+  });
+  __syncthreads();
+  norm_sum_groups(g, t, column, [&](int i, int cb, int w, float sum) {
+    partial[i] = make_float2(centre[i], sum);
+  });
+  if (p.early) grid_dependency_wait();
 }
 
-// Merge the parts' pairs of the groups [g0, g1) of sample n: stats[grp - g0] = (mean, rstd).
-__device__ __forceinline__ void merge_stats(const NormParams& p, int64_t n, int g0, int g1,
-                                            float2* stats) {
+// ---- forward: the parts' pairs become the groups' statistics. One warp per (sample, group) ----
+__global__ void __launch_bounds__(kNormThreads) norm_merge_kernel(const __grid_constant__ NormParams p) {
   const NormGeometry& g = p.g;
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  for (int grp = g0 + warp; grp < g1; grp += kNormWarps) {
-    const int first = grp * g.Cg / g.SC, last = ((grp + 1) * g.Cg - 1) / g.SC;
-    const int pieces = last - first + 1;
-    const int64_t total = static_cast<int64_t>(g.S) * pieces;
-    double sum = 0.0, q = 0.0, inv = 1.0 / (static_cast<double>(g.P) * g.Cg), m = 0.0;
-    for (int pass = 0; pass < 2; ++pass) {
-      for (int64_t i = lane; i < total; i += 32) {
-        const int64_t s = i / pieces;
-        const int k = first + static_cast<int>(i - s * pieces);
-        const int c0 = k * g.SC, c1 = min(c0 + g.SC, g.C);
-        const int width = min((grp + 1) * g.Cg, c1) - max(grp * g.Cg, c0);
-        const double cnt = static_cast<double>(g.part_begin(s + 1) - g.part_begin(s)) * width;
-        const float2 v = p.partial[((n * g.S + s) * g.slices + k) * g.GS + grp - c0 / g.Cg];
-        if (pass == 0) sum += cnt * v.x;
-        else q += v.y + cnt * (v.x - m) * (v.x - m);
-      }
-      if (pass == 0) m = warp_sum(sum) * inv;
+  const int64_t id = static_cast<int64_t>(blockIdx.x) * kNormWarps + threadIdx.x / 32;
+  const int lane = threadIdx.x % 32;
+  grid_dependency_wait();
+  grid_launch_dependents();
+  if (id >= g.N * g.G) return;
+  const int64_t n = id / g.G;
+  const int grp = static_cast<int>(id - n * g.G);
+  const int c0 = grp * g.Cg, c1 = c0 + g.Cg;
+  const int first = c0 / g.SC, last = (c1 - 1) / g.SC;
+  const double inv = 1.0 / (static_cast<double>(g.P) * g.Cg);
+  double ref = 0.0, sum = 0.0, q = 0.0;  // sums of distances from ref, and of squares around it
+  for (int k = first; k <= last; ++k) {  // the slices that hold a piece of the group
+    const int b = k * g.SC, width = min(c1, b + g.SC) - max(c0, b);
+    const float2* pairs = p.partial + (n * g.S * g.slices + k) * g.GS + grp - b / g.Cg;
+    if (k == first) ref = pairs[0].x;
+    for (int s = lane; s < g.S; s += 32) {
+      const float2 v = pairs[static_cast<int64_t>(s) * g.slices * g.GS];
+      const double cnt = static_cast<double>(g.part_pixels(s)) * width;
+      const double d = v.x - ref;
+      sum = fma(cnt, d, sum);
+      q += fma(cnt * d, d, static_cast<double>(v.y));
     }
-    const double var = warp_sum(q) * inv;
-    if (lane == 0)
-      stats[grp - g0] = make_float2(static_cast<float>(m),
-                                    static_cast<float>(1.0 / sqrt(var + static_cast<double>(g.eps))));
+  }
+  sum = warp_sum(sum) * inv;
+  double var = warp_sum(q) * inv - sum * sum;
+  if (var < 0.0) var = 0.0;  // a NaN stays
+  const float mean = static_cast<float>(ref + sum);
+  const float rstd = static_cast<float>(1.0 / sqrt(var + static_cast<double>(g.eps)));
+  if (p.mean && lane == 0) {
+    p.mean[id] = mean;
+    p.rstd[id] = rstd;
+  }
+  float* row = p.channel + n * kNormForwardRows * g.C;
+  for (int c = c0 + lane; c < c1; c += 32) {
+    row[c] = mean;
+    row[g.C + c] = p.weight ? rstd * load_weight(p.weight, p.weight_dtype, c) : rstd;
+    row[2 * static_cast<int64_t>(g.C) + c] = p.bias ? load_weight(p.bias, p.weight_dtype, c) : 0.f;
   }
 }
 
 // ---- forward: y ----
 template <typename T, int V, int ACT, int U>
 __global__ void __launch_bounds__(kNormThreads) norm_apply_kernel(const __grid_constant__ NormParams p) {
-  __shared__ float2 stats[kNormThreads * V];
   const NormGeometry& g = p.g;
   const NormTile t(g, V);
-  grid_dependency_wait();
-  grid_launch_dependents();
   using IO = VecIO<T, V>;
-  merge_stats(p, t.n, t.g0, t.g1, stats);
-  __syncthreads();
-  if (p.mean && t.s == 0) {
-    // the slice that holds a group's first channel writes its statistics
-    for (int grp = t.g0 + threadIdx.x; grp < t.g1; grp += kNormThreads)
-      if (grp * g.Cg >= t.c0) {
-        p.mean[t.n * g.G + grp] = stats[grp - t.g0].x;
-        p.rstd[t.n * g.G + grp] = stats[grp - t.g0].y;
-      }
-  }
-  if (!t.active) return;
-  float mean[V], a[V], b[V];
-#pragma unroll
-  for (int v = 0; v < V; ++v) {
-    const int c = t.c0 + t.chan + v;
-    const float2 st = stats[c / g.Cg - t.g0];
-    mean[v] = st.x;
-    a[v] = p.weight ? st.y * load_weight(p.weight, p.weight_dtype, c) : st.y;
-    b[v] = p.bias ? load_weight(p.bias, p.weight_dtype, c) : 0.f;
-  }
-  const int64_t base = t.n * g.P * g.C + t.c0 + t.chan;
+  const int64_t base = static_cast<int64_t>(t.n) * g.P * g.C + t.c0 + t.chan;
   const T* x = static_cast<const T*>(p.x) + base;
   T* y = static_cast<T*>(p.out) + base;
-  const int64_t step = g.rows;
-  int64_t px = t.p0 + t.row;
-  auto emit = [&](const typename IO::Raw& raw, int64_t at) {
+  NormSteps<U> steps(g, t);
+  // x was complete before the statistics' launch began its work, so the first reads need not
+  // wait for that launch to end
+  typename IO::Raw raw[U];
+  auto fetch = [&] {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (steps.has(u)) raw[u] = IO::load(x + steps.pixel(u) * g.C);
+  };
+  if (steps.more()) fetch();
+  grid_dependency_wait();
+  float mean[V], a[V], b[V];
+  if (t.active) {
+    const float* row = p.channel + static_cast<int64_t>(t.n) * kNormForwardRows * g.C + t.c0 + t.chan;
+    load_channels<V>(row, mean);
+    load_channels<V>(row + g.C, a);
+    load_channels<V>(row + 2 * static_cast<int64_t>(g.C), b);
+  }
+  grid_launch_dependents();  // the statistics have been read
+  auto emit = [&](const typename IO::Raw& r, int64_t at) {
     float f[V];
-    IO::unpack(raw, f);
+    IO::unpack(r, f);
 #pragma unroll
     for (int v = 0; v < V; ++v) f[v] = activate<T, ACT>(fmaf(f[v] - mean[v], a[v], b[v]));
     IO::store(y + at * g.C, IO::pack(f));
   };
-  for (; px + (U - 1) * step < t.p1; px += U * step) {
-    typename IO::Raw raw[U];
+  while (steps.more()) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) raw[u] = IO::load(x + (px + u * step) * g.C);
-#pragma unroll
-    for (int u = 0; u < U; ++u) emit(raw[u], px + u * step);
+    for (int u = 0; u < U; ++u)
+      if (steps.has(u)) emit(raw[u], steps.pixel(u));
+    steps.next();
+    if (steps.more()) fetch();
   }
-  for (; px < t.p1; px += step) emit(IO::load(x + px * g.C), px);
 }
 
 // ---- backward: per-channel sums of one part ----
@@ -367,23 +462,31 @@ template <typename T, int V, int ACT, int U>
 __global__ void __launch_bounds__(kNormThreads) norm_grad_sums_kernel(const __grid_constant__ NormParams p) {
   __shared__ float sm1[kNormThreads * V];
   __shared__ float sm2[kNormThreads * V];
+  __shared__ float column1[kNormThreads * V];
+  __shared__ float column2[kNormThreads * V];
   const NormGeometry& g = p.g;
   const NormTile t(g, V);
-  grid_dependency_wait();
+  if (!p.early) grid_dependency_wait();
   grid_launch_dependents();
   using IO = VecIO<T, V>;
   if (t.active) {
     float mean[V], a[V], b[V], s1[V], s2[V];
+    const int first = t.c0 + t.chan;
+    int grp = first / g.Cg, end = (grp + 1) * g.Cg;  // one division; the next channels follow
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      const int c = t.c0 + t.chan + v;
-      const int64_t at = t.n * g.G + c / g.Cg;
+      const int c = first + v;
+      if (c == end) {
+        ++grp;
+        end += g.Cg;
+      }
+      const int64_t at = static_cast<int64_t>(t.n) * g.G + grp;
       mean[v] = p.mean[at];
       a[v] = p.weight ? p.rstd[at] * load_weight(p.weight, p.weight_dtype, c) : p.rstd[at];
       b[v] = p.bias ? load_weight(p.bias, p.weight_dtype, c) : 0.f;
       s1[v] = s2[v] = 0.f;
     }
-    const int64_t base = t.n * g.P * g.C + t.c0 + t.chan;
+    const int64_t base = static_cast<int64_t>(t.n) * g.P * g.C + t.c0 + t.chan;
     const T* x = static_cast<const T*>(p.x) + base;
     const T* dy = static_cast<const T*>(p.dy) + base;
     const int64_t step = g.rows;
@@ -400,17 +503,19 @@ __global__ void __launch_bounds__(kNormThreads) norm_grad_sums_kernel(const __gr
         s2[v] = fmaf(dz, xc, s2[v]);
       }
     };
-    for (; px + (U - 1) * step < t.p1; px += U * step) {
+    for (; px < t.p1; px += U * step) {
       typename IO::Raw rx[U], rd[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        rx[u] = IO::load(x + (px + u * step) * g.C);
-        rd[u] = IO::load(dy + (px + u * step) * g.C);
+        if (px + u * step < t.p1) {
+          rx[u] = IO::load(x + (px + u * step) * g.C);
+          rd[u] = IO::load(dy + (px + u * step) * g.C);
+        }
       }
 #pragma unroll
-      for (int u = 0; u < U; ++u) take(rx[u], rd[u]);
+      for (int u = 0; u < U; ++u)
+        if (px + u * step < t.p1) take(rx[u], rd[u]);
     }
-    for (; px < t.p1; px += step) take(IO::load(x + px * g.C), IO::load(dy + px * g.C));
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       sm1[t.row * g.SC + t.chan + v] = s1[v];
@@ -418,42 +523,29 @@ __global__ void __launch_bounds__(kNormThreads) norm_grad_sums_kernel(const __gr
     }
   }
   __syncthreads();
-  // L lanes (a power of two, at most a warp) sum the rows of one channel
-  int L = 1;
-  while (L < 32 && 2 * L <= g.rows) L *= 2;
-  const int sub = threadIdx.x % L, width = t.c1 - t.c0;
-  const int passes = (width + kNormThreads / L - 1) / (kNormThreads / L);
-  for (int i = 0; i < passes; ++i) {
-    const int c = i * (kNormThreads / L) + threadIdx.x / L;
-    float v1 = 0.f, v2 = 0.f;
-    if (c < width)
-      for (int r = sub; r < g.rows; r += L) {
-        v1 += sm1[r * g.SC + c];
-        v2 += sm2[r * g.SC + c];
-      }
-    for (int o = L / 2; o > 0; o >>= 1) {
-      v1 += __shfl_xor_sync(0xffffffffu, v1, o);
-      v2 += __shfl_xor_sync(0xffffffffu, v2, o);
-    }
-    if (c < width && sub == 0)
-      p.partial[(t.n * g.S + t.s) * g.C + t.c0 + c] = make_float2(v1, v2);
-  }
+  const int width = t.c1 - t.c0;
+  norm_sum_rows(g.rows, g.SC, width, column1, [&](int r, int c) { return sm1[r * g.SC + c]; });
+  norm_sum_rows(g.rows, g.SC, width, column2, [&](int r, int c) { return sm2[r * g.SC + c]; });
+  __syncthreads();
+  float2* partial = p.partial + (static_cast<int64_t>(t.n) * g.S + t.s) * g.C + t.c0;
+  for (int c = threadIdx.x; c < width; c += kNormThreads) partial[c] = make_float2(column1[c], column2[c]);
+  if (p.early) grid_dependency_wait();
 }
 
 // ---- backward: sums over the parts, and each group's two means. One CTA per (group, sample) ----
 __global__ void __launch_bounds__(kNormThreads) norm_grad_coef_kernel(const __grid_constant__ NormParams p) {
   __shared__ double sm1[kNormThreads], sm2[kNormThreads];
+  __shared__ float means[2];
   const NormGeometry& g = p.g;
-  const int grp = blockIdx.x;
-  const int64_t n = blockIdx.y + static_cast<int64_t>(gridDim.y) * blockIdx.z;
-  if (n >= g.N) return;
+  const int64_t n = blockIdx.x / static_cast<unsigned>(g.G);
+  const int grp = static_cast<int>(blockIdx.x - n * g.G);
   grid_dependency_wait();
   grid_launch_dependents();
   // cols channels at a time (a power of two, at most 32), kNormThreads / cols threads each
   int cols = 1;
   while (cols < 32 && cols < g.Cg) cols *= 2;
   const int col = threadIdx.x % cols, sub = threadIdx.x / cols, subs = kNormThreads / cols;
-  const float rstd = p.rstd[n * g.G + grp];
+  const float mean = p.mean[n * g.G + grp], rstd = p.rstd[n * g.G + grp];
   double w1 = 0.0, w2 = 0.0;  // sum of w dz and of w dz xhat, kept by the threads with sub == 0
   for (int cb = 0; cb < g.Cg; cb += cols) {
     const int c = cb + col;
@@ -477,7 +569,7 @@ __global__ void __launch_bounds__(kNormThreads) norm_grad_coef_kernel(const __gr
     if (sub == 0 && c < g.Cg) {
       const int ch = grp * g.Cg + c;
       const double s1 = sm1[threadIdx.x], s2 = sm2[threadIdx.x] * rstd;
-      p.chan[n * g.C + ch] = make_float2(static_cast<float>(s1), static_cast<float>(s2));
+      p.sums[n * g.C + ch] = make_float2(static_cast<float>(s1), static_cast<float>(s2));
       const double w = p.weight ? load_weight(p.weight, p.weight_dtype, ch) : 1.0;
       w1 += w * s1;
       w2 += w * s2;
@@ -487,11 +579,21 @@ __global__ void __launch_bounds__(kNormThreads) norm_grad_coef_kernel(const __gr
   if (threadIdx.x < 32) {
     w1 = warp_sum(sub == 0 ? w1 : 0.0);
     w2 = warp_sum(sub == 0 ? w2 : 0.0);
+    const double m = static_cast<double>(g.P) * g.Cg;
     if (threadIdx.x == 0) {
-      const double m = static_cast<double>(g.P) * g.Cg;
-      p.coef[n * g.G + grp] = make_float2(static_cast<float>(rstd * (w1 / m)),
-                                          static_cast<float>(rstd * (rstd * (w2 / m))));
+      means[0] = static_cast<float>(rstd * (w1 / m));
+      means[1] = static_cast<float>(rstd * (rstd * (w2 / m)));
     }
+  }
+  __syncthreads();
+  float* row = p.channel + n * kNormBackwardRows * g.C;
+  for (int c = grp * g.Cg + threadIdx.x; c < (grp + 1) * g.Cg; c += kNormThreads) {
+    const int64_t C = g.C;
+    row[c] = mean;
+    row[C + c] = p.weight ? rstd * load_weight(p.weight, p.weight_dtype, c) : rstd;
+    row[2 * C + c] = p.bias ? load_weight(p.bias, p.weight_dtype, c) : 0.f;
+    row[3 * C + c] = means[0];
+    row[4 * C + c] = means[1];
   }
 }
 
@@ -503,7 +605,7 @@ __global__ void __launch_bounds__(kNormThreads) norm_param_grad_kernel(const __g
   if (c >= p.g.C) return;
   double db = 0.0, dw = 0.0;
   for (int64_t n = 0; n < p.g.N; ++n) {
-    const float2 v = p.chan[n * p.g.C + c];
+    const float2 v = p.sums[n * p.g.C + c];
     db += v.x;
     dw += v.y;
   }
@@ -516,32 +618,40 @@ template <typename T, int V, int ACT, int U>
 __global__ void __launch_bounds__(kNormThreads) norm_grad_apply_kernel(const __grid_constant__ NormParams p) {
   const NormGeometry& g = p.g;
   const NormTile t(g, V);
-  grid_dependency_wait();
-  grid_launch_dependents();
   using IO = VecIO<T, V>;
-  if (!t.active) return;
-  float mean[V], a[V], b[V], k1[V], k2[V];
-#pragma unroll
-  for (int v = 0; v < V; ++v) {
-    const int c = t.c0 + t.chan + v;
-    const int64_t at = t.n * g.G + c / g.Cg;
-    mean[v] = p.mean[at];
-    a[v] = p.weight ? p.rstd[at] * load_weight(p.weight, p.weight_dtype, c) : p.rstd[at];
-    b[v] = p.bias ? load_weight(p.bias, p.weight_dtype, c) : 0.f;
-    const float2 k = p.coef[at];
-    k1[v] = k.x;
-    k2[v] = k.y;
-  }
-  const int64_t base = t.n * g.P * g.C + t.c0 + t.chan;
+  const int64_t base = static_cast<int64_t>(t.n) * g.P * g.C + t.c0 + t.chan;
   const T* x = static_cast<const T*>(p.x) + base;
   const T* dy = static_cast<const T*>(p.dy) + base;
   T* dx = static_cast<T*>(p.out) + base;
-  const int64_t step = g.rows;
-  int64_t px = t.p0 + t.row;
-  auto emit = [&](const typename IO::Raw& rx, const typename IO::Raw& rd, int64_t at) {
+  NormSteps<U> steps(g, t);
+  // as in the forward, the first reads do not wait for the launch before
+  typename IO::Raw rx[U], rd[U];
+  auto fetch = [&] {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (steps.has(u)) {
+        rx[u] = IO::load(x + steps.pixel(u) * g.C);
+        rd[u] = IO::load(dy + steps.pixel(u) * g.C);
+      }
+    }
+  };
+  if (steps.more()) fetch();
+  grid_dependency_wait();
+  float mean[V], a[V], b[V], k1[V], k2[V];
+  if (t.active) {
+    const int64_t C = g.C;
+    const float* row = p.channel + t.n * kNormBackwardRows * C + t.c0 + t.chan;
+    load_channels<V>(row, mean);
+    load_channels<V>(row + C, a);
+    load_channels<V>(row + 2 * C, b);
+    load_channels<V>(row + 3 * C, k1);
+    load_channels<V>(row + 4 * C, k2);
+  }
+  grid_launch_dependents();  // the means have been read
+  auto emit = [&](const typename IO::Raw& ra, const typename IO::Raw& rb, int64_t at) {
     float f[V], d[V];
-    IO::unpack(rx, f);
-    IO::unpack(rd, d);
+    IO::unpack(ra, f);
+    IO::unpack(rb, d);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       const float xc = f[v] - mean[v];
@@ -550,17 +660,13 @@ __global__ void __launch_bounds__(kNormThreads) norm_grad_apply_kernel(const __g
     }
     IO::store(dx + at * g.C, IO::pack(f));
   };
-  for (; px + (U - 1) * step < t.p1; px += U * step) {
-    typename IO::Raw rx[U], rd[U];
+  while (steps.more()) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      rx[u] = IO::load(x + (px + u * step) * g.C);
-      rd[u] = IO::load(dy + (px + u * step) * g.C);
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) emit(rx[u], rd[u], px + u * step);
+    for (int u = 0; u < U; ++u)
+      if (steps.has(u)) emit(rx[u], rd[u], steps.pixel(u));
+    steps.next();
+    if (steps.more()) fetch();
   }
-  for (; px < t.p1; px += step) emit(IO::load(x + px * g.C), IO::load(dy + px * g.C), px);
 }
 
 }  // namespace fssim

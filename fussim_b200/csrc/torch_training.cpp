@@ -10,6 +10,7 @@
 #include <c10/cuda/CUDAGuard.h>
 
 #include <algorithm>
+#include <cmath>
 #include <stdexcept>
 #include <string>
 #include <vector>
@@ -157,12 +158,76 @@ struct GroupNormFn : public torch::autograd::Function<GroupNormFn> {
   }
 };
 
+[[noreturn]] void value_error(const std::string& msg) { throw std::invalid_argument(msg); }
+[[noreturn]] void runtime_error(const std::string& msg) { throw std::runtime_error(msg); }
+
+std::string shape_text(const at::Tensor& t) {
+  std::string s = "(";
+  for (int64_t i = 0; i < t.dim(); ++i) s += (i ? ", " : "") + std::to_string(t.size(i));
+  return s + (t.dim() == 1 ? ",)" : ")");
+}
+std::string type_text(at::ScalarType t) { return std::string(c10::toString(t)); }
+bool known_type(at::ScalarType t) { return t == at::kFloat || t == at::kHalf || t == at::kBFloat16; }
+
+void require_cuda(const char* what) {
+  if (!at::hasCUDA() || at::cuda::device_count() == 0)
+    runtime_error(std::string("CUDA is not available. ") + what + " requires a CUDA-capable GPU.");
+}
+
+int64_t activation_code(const std::optional<std::string>& name) {
+  if (!name.has_value()) return FSSIM_ACT_NONE;
+  if (*name == "silu") return FSSIM_ACT_SILU;
+  if (*name == "relu") return FSSIM_ACT_RELU;
+  value_error("activation must be one of (None, 'silu', 'relu'), got '" + *name + "'");
+}
+
+void check_norm_settings(int64_t groups, int64_t channels, double eps,
+                         const std::optional<std::string>& activation) {
+  activation_code(activation);
+  if (groups < 1 || channels < 1 || channels % groups != 0)
+    value_error("the channels must divide into the groups, got " + std::to_string(channels) +
+                " channels and " + std::to_string(groups) + " groups");
+  if (!(eps >= 0.0 && std::isfinite(eps)))
+    value_error("eps must be finite and not negative, got " + std::to_string(eps));
+}
+
+// Checks, then the operator: recorded for autograd where a gradient may be asked for.
 at::Tensor group_norm_act(const at::Tensor& x, int64_t groups, const OptTensor& weight,
-                          const OptTensor& bias, double eps, int64_t activation, bool train) {
-  if (train) return GroupNormFn::apply(x, weight, bias, groups, eps, activation);
+                          const OptTensor& bias, double eps,
+                          const std::optional<std::string>& activation) {
+  if (x.dim() != 4)
+    value_error("Expected 4D tensor (B, C, H, W), but got " + std::to_string(x.dim()) +
+                "D tensor with shape " + shape_text(x));
+  const int64_t channels = x.size(1);
+  check_norm_settings(groups, channels, eps, activation);
+  if (!known_type(x.scalar_type()))
+    value_error("x must be float32, float16 or bfloat16, got " + type_text(x.scalar_type()));
+  bool train = x.requires_grad();
+  for (const OptTensor* o : {&weight, &bias}) {
+    if (!o->has_value()) continue;
+    const at::Tensor& t = **o;
+    const std::string name = o == &weight ? "weight" : "bias";
+    if (t.dim() != 1 || t.size(0) != channels)
+      value_error(name + " must have shape (" + std::to_string(channels) + ",), got " + shape_text(t));
+    if (!known_type(t.scalar_type()))
+      value_error(name + " must be float32, float16 or bfloat16, got " + type_text(t.scalar_type()));
+    if (t.device() != x.device())
+      runtime_error(name + " must be on x's device.\nx: " + x.device().str() + ", " + name + ": " +
+                    t.device().str());
+    train = train || t.requires_grad();
+  }
+  if (weight.has_value() && bias.has_value() && weight->scalar_type() != bias->scalar_type())
+    value_error("weight and bias must have the same dtype, got " + type_text(weight->scalar_type()) +
+                " and " + type_text(bias->scalar_type()));
+  require_cuda("group_norm_act");
+  if (!x.is_cuda())
+    runtime_error("x must be on a CUDA device, but got device: " + x.device().str());
+  const int64_t act = activation_code(activation);
+  if (train && at::GradMode::is_enabled())
+    return GroupNormFn::apply(x, weight, bias, groups, eps, act);
   const at::NoGradGuard no_grad;
   return norm_forward(x.contiguous(at::MemoryFormat::ChannelsLast), groups, Affine(weight, bias),
-                      eps, activation, false)
+                      eps, act, false)
       .y;
 }
 
@@ -224,6 +289,13 @@ struct ClipArrays {
   std::vector<int32_t> dtypes, out_dtypes;
   fssim_grad_clip_args args{};
 
+  explicit ClipArrays(size_t n) {
+    grads.reserve(n);
+    outs.reserve(n);
+    sizes.reserve(n);
+    dtypes.reserve(n);
+    out_dtypes.reserve(n);
+  }
   void add(const at::Tensor& g, const at::Tensor& o) {
     grads.push_back(g.data_ptr());
     outs.push_back(o.data_ptr());
@@ -231,7 +303,7 @@ struct ClipArrays {
     dtypes.push_back(dtype_code(g.scalar_type()));
     out_dtypes.push_back(dtype_code(o.scalar_type()));
   }
-  const fssim_grad_clip_args* fill(float max_norm, float* norm) {
+  fssim_grad_clip_args& fill(float max_norm, float* norm) {
     args.count = static_cast<int64_t>(grads.size());
     args.grads = grads.data();
     args.sizes = sizes.data();
@@ -241,72 +313,148 @@ struct ClipArrays {
     args.max_norm = max_norm;
     args.norm = norm;
     args.workspace_bytes = fssim_grad_clip_workspace_bytes(&args);
-    return &args;
+    return args;
   }
 };
 
-// grads (and outs) are CUDA tensors of one device with matching shapes: the Python layer has
-// checked. Tensors whose numbers fill their memory are taken as they lie; others go through a
-// dense copy.
-at::Tensor grad_norm(const std::vector<at::Tensor>& grads) {
-  const at::NoGradGuard no_grad;
-  const at::cuda::OptionalCUDAGuard guard(grads.at(0).device());
-  at::Tensor norm = at::empty({}, grads[0].options().dtype(at::kFloat));
-  ClipArrays arrays;
-  std::vector<at::Tensor> dense;
-  for (const auto& g : grads) {
-    if (g.is_non_overlapping_and_dense()) {
-      arrays.add(g, g);
-    } else {
-      dense.push_back(g.contiguous());
-      arrays.add(dense.back(), dense.back());
-    }
+using Tensors = std::vector<at::Tensor>;
+
+void check_grads(const Tensors& grads, const char* what) {
+  for (size_t i = 0; i < grads.size(); ++i) {
+    const at::Tensor& g = grads[i];
+    const auto at = [&] { return " at index " + std::to_string(i) + " "; };
+    if (!g.defined()) value_error("the gradient" + at() + "is missing");
+    if (g.layout() != at::kStrided) value_error("gradients must be dense tensors, but that" + at() + "is not");
+    if (!known_type(g.scalar_type()))
+      value_error("gradients must be float32, float16 or bfloat16, but that" + at() + "is " +
+                  type_text(g.scalar_type()));
+    if (g.device() != grads[0].device())
+      runtime_error("gradients must be on one device.\nfirst: " + grads[0].device().str() + "," + at() +
+                    g.device().str());
   }
-  auto* a = const_cast<fssim_grad_clip_args*>(arrays.fill(0.f, norm.data_ptr<float>()));
-  at::Tensor ws = workspace(a->workspace_bytes, grads[0]);
-  a->workspace = ws.data_ptr();
-  check_status(fssim_grad_norm(a, current_stream()));
+  require_cuda(what);
+  if (!grads.empty() && !grads[0].is_cuda())
+    runtime_error("gradients must be on a CUDA device, but got device: " + grads[0].device().str());
+}
+
+at::Tensor zero_norm() {
+  return at::zeros({}, at::TensorOptions().dtype(at::kFloat).device(at::kCUDA));
+}
+
+// Tensors whose numbers fill their memory are taken as they lie; others go through a dense copy.
+at::Tensor norm_of(const Tensors& grads) {
+  const at::NoGradGuard no_grad;
+  const at::cuda::OptionalCUDAGuard guard(grads[0].device());
+  at::Tensor norm = at::empty({}, grads[0].options().dtype(at::kFloat));
+  ClipArrays arrays(grads.size());
+  Tensors held;
+  for (const auto& g : grads) {
+    if (!g.is_non_overlapping_and_dense()) held.push_back(g.contiguous());
+    const at::Tensor& d = g.is_non_overlapping_and_dense() ? g : held.back();
+    arrays.add(d, d);
+  }
+  fssim_grad_clip_args& a = arrays.fill(0.f, norm.data_ptr<float>());
+  at::Tensor ws = workspace(a.workspace_bytes, grads[0]);
+  a.workspace = ws.data_ptr();
+  check_status(fssim_grad_norm(&a, current_stream()));
   return norm;
 }
 
-at::Tensor clip_grads(const std::vector<at::Tensor>& grads, const std::vector<at::Tensor>& outs,
-                      double max_norm) {
+at::Tensor clip_into(const Tensors& grads, const Tensors& outs, double max_norm, bool error_if_nonfinite) {
   const at::NoGradGuard no_grad;
-  const at::cuda::OptionalCUDAGuard guard(grads.at(0).device());
-  TORCH_CHECK(grads.size() == outs.size(), "one output for each gradient");
+  const at::cuda::OptionalCUDAGuard guard(grads[0].device());
   check_overlap(grads, outs);
+  if (error_if_nonfinite) {
+    const double norm = norm_of(grads).item<double>();
+    if (!std::isfinite(norm))
+      runtime_error("the gradients' norm is " + std::to_string(norm) +
+                    "; nothing was clipped. Pass error_if_nonfinite=False to clip all the same");
+  }
   at::Tensor norm = at::empty({}, grads[0].options().dtype(at::kFloat));
-  ClipArrays arrays;
-  std::vector<at::Tensor> held;                              // dense stand-ins
+  ClipArrays arrays(grads.size());
+  Tensors held;                                              // dense stand-ins of gradients
   std::vector<std::pair<at::Tensor, at::Tensor>> copy_back;  // (output, its stand-in)
   for (size_t i = 0; i < grads.size(); ++i) {
-    at::Tensor g = grads[i], o = outs[i];
-    const bool alike = g.strides() == o.strides() && g.is_non_overlapping_and_dense();
-    if (!alike && !(g.is_contiguous() && o.is_contiguous())) {
-      g = g.contiguous();
-      at::Tensor d = at::empty(o.sizes(), o.options(), at::MemoryFormat::Contiguous);
-      held.push_back(g);
-      copy_back.emplace_back(o, d);
-      o = d;
+    const at::Tensor &g = grads[i], &o = outs[i];
+    if ((g.is_contiguous() && o.is_contiguous()) ||
+        (g.is_non_overlapping_and_dense() && g.strides() == o.strides())) {
+      arrays.add(g, o);
+      continue;
     }
-    arrays.add(g, o);
+    held.push_back(g.contiguous());
+    copy_back.emplace_back(o, at::empty(o.sizes(), o.options(), at::MemoryFormat::Contiguous));
+    arrays.add(held.back(), copy_back.back().second);
   }
-  auto* a = const_cast<fssim_grad_clip_args*>(
-      arrays.fill(static_cast<float>(max_norm), norm.data_ptr<float>()));
-  at::Tensor ws = workspace(a->workspace_bytes, grads[0]);
-  a->workspace = ws.data_ptr();
+  fssim_grad_clip_args& a = arrays.fill(static_cast<float>(max_norm), norm.data_ptr<float>());
+  at::Tensor ws = workspace(a.workspace_bytes, grads[0]);
+  a.workspace = ws.data_ptr();
   // the kernels write past autograd's sight: a graph that saved an output has to notice
   for (const auto& o : outs) o.unsafeGetTensorImpl()->bump_version();
-  check_status(fssim_grad_clip(a, current_stream()));
+  check_status(fssim_grad_clip(&a, current_stream()));
   for (auto& [o, d] : copy_back) o.copy_(d);
   return norm;
+}
+
+void check_max_norm(double max_norm) {
+  if (!(max_norm >= 0.0)) value_error("max_norm must not be negative, got " + std::to_string(max_norm));
+}
+
+at::Tensor grad_norm(const Tensors& grads) {
+  check_grads(grads, "grad_norm");
+  return grads.empty() ? zero_norm() : norm_of(grads);
+}
+
+std::tuple<Tensors, at::Tensor> clip_grad_norm(const Tensors& grads, double max_norm,
+                                               const std::optional<Tensors>& out,
+                                               bool error_if_nonfinite) {
+  check_max_norm(max_norm);
+  if (out.has_value() && out->size() != grads.size())
+    value_error("out must have a tensor for each gradient, got " + std::to_string(out->size()) + " for " +
+                std::to_string(grads.size()));
+  check_grads(grads, "clip_grad_norm");
+  if (grads.empty()) return {Tensors(), zero_norm()};
+  Tensors outs;
+  if (out.has_value()) {
+    outs = *out;
+    for (size_t i = 0; i < outs.size(); ++i) {
+      const at::Tensor &g = grads[i], &o = outs[i];
+      const std::string name = "out[" + std::to_string(i) + "]";
+      if (o.sizes() != g.sizes())
+        value_error(name + " must have shape " + shape_text(g) + ", got " + shape_text(o));
+      if (o.scalar_type() != g.scalar_type() && o.scalar_type() != at::kFloat)
+        value_error(name + " must be " + type_text(g.scalar_type()) + " or float32, got " +
+                    type_text(o.scalar_type()));
+      if (o.device() != g.device() || o.layout() != at::kStrided)
+        runtime_error(name + " must be a dense tensor on " + g.device().str());
+    }
+  } else {
+    outs.reserve(grads.size());
+    for (const auto& g : grads) outs.push_back(at::empty_like(g, g.options().requires_grad(false)));
+  }
+  at::Tensor norm = clip_into(grads, outs, max_norm, error_if_nonfinite);
+  return {std::move(outs), norm};
+}
+
+at::Tensor clip_grad_norm_(const Tensors& parameters, double max_norm, bool error_if_nonfinite) {
+  check_max_norm(max_norm);
+  Tensors grads;
+  grads.reserve(parameters.size());
+  for (const auto& p : parameters)
+    if (p.grad().defined()) grads.push_back(p.grad());
+  check_grads(grads, "clip_grad_norm_");
+  return grads.empty() ? zero_norm() : clip_into(grads, grads, max_norm, error_if_nonfinite);
 }
 
 }  // namespace
 
 void bind_training(py::module& m) {
-  m.def("group_norm_act", &group_norm_act, py::arg("x"), py::arg("groups"), py::arg("weight"),
-        py::arg("bias"), py::arg("eps"), py::arg("activation"), py::arg("train"));
-  m.def("grad_norm", &grad_norm);
-  m.def("clip_grads", &clip_grads);
+  m.def("group_norm_act", &group_norm_act, py::arg("x"), py::arg("num_groups"), py::arg("weight"),
+        py::arg("bias"), py::arg("eps"), py::arg("activation"));
+  m.def("check_norm_settings", &check_norm_settings, py::arg("num_groups"), py::arg("num_channels"),
+        py::arg("eps"), py::arg("activation"));
+  m.def("grad_norm", &grad_norm, py::arg("grads"));
+  m.def("clip_grad_norm", &clip_grad_norm, py::arg("grads"), py::arg("max_norm"), py::arg("out"),
+        py::arg("error_if_nonfinite"));
+  m.def("clip_grad_norm_", &clip_grad_norm_, py::arg("parameters"), py::arg("max_norm"),
+        py::arg("error_if_nonfinite"));
 }

@@ -14,36 +14,11 @@ Like the losses they run hand-written sm_100a kernels and have no CPU path. The 
 
 from __future__ import annotations
 
-import math
 from typing import Iterable, List, Optional, Sequence, Tuple
 
 import torch
 
 from .functional import _ensure_cuda_extension
-
-ALLOWED_ACTIVATIONS = (None, "silu", "relu")
-_ACTIVATION_CODE = {None: 0, "silu": 1, "relu": 2}
-_DTYPES = (torch.float32, torch.float16, torch.bfloat16)
-
-
-def _require_cuda(what: str) -> None:
-    if not torch.cuda.is_available():
-        raise RuntimeError(f"CUDA is not available. {what} requires a CUDA-capable GPU.")
-
-
-# ------------------------------------------------------------------------------------
-# Group normalisation with an activation
-# ------------------------------------------------------------------------------------
-def _check_norm(num_groups, num_channels, eps, activation):
-    if activation not in ALLOWED_ACTIVATIONS:
-        raise ValueError(f"activation must be one of {ALLOWED_ACTIVATIONS}, got {activation!r}")
-    if num_groups < 1 or num_channels < 1 or num_channels % num_groups != 0:
-        raise ValueError(
-            f"the channels must divide into the groups, got {num_channels} channels and "
-            f"{num_groups} groups"
-        )
-    if not (eps >= 0.0 and math.isfinite(eps)):
-        raise ValueError(f"eps must be finite and not negative, got {eps}")
 
 
 def group_norm_act(
@@ -68,38 +43,8 @@ def group_norm_act(
     weight and bias. The results repeat bit for bit. Under graph capture follow torch's rule
     for backward passes: the captured leaves must not have live eager graphs.
     """
-    if len(x.shape) != 4:
-        raise ValueError(
-            f"Expected 4D tensor (B, C, H, W), but got {len(x.shape)}D tensor with shape {x.shape}"
-        )
-    channels = x.shape[1]
-    _check_norm(num_groups, channels, eps, activation)
-    if x.dtype not in _DTYPES:
-        raise ValueError(f"x must be float32, float16 or bfloat16, got {x.dtype}")
-    for name, t in (("weight", weight), ("bias", bias)):
-        if t is None:
-            continue
-        if tuple(t.shape) != (channels,):
-            raise ValueError(f"{name} must have shape ({channels},), got {tuple(t.shape)}")
-        if t.dtype not in _DTYPES:
-            raise ValueError(f"{name} must be float32, float16 or bfloat16, got {t.dtype}")
-        if t.device != x.device:
-            raise RuntimeError(f"{name} must be on x's device.\nx: {x.device}, {name}: {t.device}")
-    if weight is not None and bias is not None and weight.dtype != bias.dtype:
-        raise ValueError(
-            f"weight and bias must have the same dtype, got {weight.dtype} and {bias.dtype}"
-        )
-    _require_cuda("group_norm_act")
-    if not x.is_cuda:
-        raise RuntimeError(f"x must be on a CUDA device, but got device: {x.device}")
-    train = torch.is_grad_enabled() and (
-        x.requires_grad
-        or (weight is not None and weight.requires_grad)
-        or (bias is not None and bias.requires_grad)
-    )
-    return _ensure_cuda_extension().group_norm_act(
-        x, num_groups, weight, bias, eps, _ACTIVATION_CODE[activation], train
-    )
+    # arguments are checked in the extension: the call costs little more than its launches
+    return _ensure_cuda_extension().group_norm_act(x, num_groups, weight, bias, eps, activation)
 
 
 class GroupNormAct(torch.nn.Module):
@@ -117,7 +62,7 @@ class GroupNormAct(torch.nn.Module):
         dtype=None,
     ):
         super().__init__()
-        _check_norm(num_groups, num_channels, eps, activation)
+        _ensure_cuda_extension().check_norm_settings(num_groups, num_channels, eps, activation)
         self.num_groups = num_groups
         self.num_channels = num_channels
         self.eps = eps
@@ -142,41 +87,6 @@ class GroupNormAct(torch.nn.Module):
         )
 
 
-# ------------------------------------------------------------------------------------
-# Global gradient norm and clipping
-# ------------------------------------------------------------------------------------
-def _check_grads(grads: Sequence[torch.Tensor], what: str) -> None:
-    device = grads[0].device
-    for i, g in enumerate(grads):
-        if g.layout != torch.strided:
-            raise ValueError(f"gradients must be dense tensors, but {i} is {g.layout}")
-        if g.dtype not in _DTYPES:
-            raise ValueError(f"gradients must be float32, float16 or bfloat16, but {i} is {g.dtype}")
-        if g.device != device:
-            raise RuntimeError(
-                f"gradients must be on one device.\nfirst: {device}, at index {i}: {g.device}"
-            )
-    _require_cuda(what)
-    if device.type != "cuda":
-        raise RuntimeError(f"gradients must be on a CUDA device, but got device: {device}")
-
-
-def _check_max_norm(max_norm) -> float:
-    value = float(max_norm)
-    if not value >= 0.0:
-        raise ValueError(f"max_norm must not be negative, got {max_norm}")
-    return value
-
-
-def _raise_if_nonfinite(grads) -> None:
-    norm = grad_norm(grads)
-    if not math.isfinite(norm.item()):
-        raise RuntimeError(
-            f"the gradients' norm is {norm.item()}; nothing was clipped. Pass "
-            "error_if_nonfinite=False to clip all the same"
-        )
-
-
 def grad_norm(grads: Iterable[torch.Tensor]) -> torch.Tensor:
     """The 2-norm of all the tensors' numbers taken together: a 0-d float32 CUDA tensor.
 
@@ -185,12 +95,7 @@ def grad_norm(grads: Iterable[torch.Tensor]) -> torch.Tensor:
     eight numbers and FP32's range does not limit them; the result repeats bit for bit. No
     host synchronisation. Not differentiable.
     """
-    grads = list(grads)
-    if not grads:
-        _require_cuda("grad_norm")
-        return torch.zeros((), device="cuda")
-    _check_grads(grads, "grad_norm")
-    return _ensure_cuda_extension().grad_norm(grads)
+    return _ensure_cuda_extension().grad_norm(list(grads))
 
 
 def clip_grad_norm(
@@ -210,28 +115,9 @@ def clip_grad_norm(
     anything is written, at the price of a host synchronisation. Tensors whose numbers do not
     fill their memory are copied once more.
     """
-    grads = list(grads)
-    max_norm = _check_max_norm(max_norm)
-    if out is not None:
-        out = list(out)
-        if len(out) != len(grads):
-            raise ValueError(f"out must have a tensor for each gradient, got {len(out)} for {len(grads)}")
-    if not grads:
-        _require_cuda("clip_grad_norm")
-        return [], torch.zeros((), device="cuda")
-    _check_grads(grads, "clip_grad_norm")
-    if out is None:
-        out = [torch.empty_like(g, requires_grad=False) for g in grads]
-    for i, (g, o) in enumerate(zip(grads, out)):
-        if o.shape != g.shape:
-            raise ValueError(f"out[{i}] must have shape {tuple(g.shape)}, got {tuple(o.shape)}")
-        if o.dtype != g.dtype and o.dtype != torch.float32:
-            raise ValueError(f"out[{i}] must be {g.dtype} or float32, got {o.dtype}")
-        if o.device != g.device or o.layout != torch.strided:
-            raise RuntimeError(f"out[{i}] must be a dense tensor on {g.device}")
-    if error_if_nonfinite:
-        _raise_if_nonfinite(grads)
-    return out, _ensure_cuda_extension().clip_grads(grads, out, max_norm)
+    return _ensure_cuda_extension().clip_grad_norm(
+        list(grads), float(max_norm), None if out is None else list(out), error_if_nonfinite
+    )
 
 
 def clip_grad_norm_(
@@ -245,14 +131,8 @@ def clip_grad_norm_(
     the limit the gradients are left untouched (and not read a second time); otherwise as
     ``clip_grad_norm`` with ``out=grads``. A gradient may be given once only.
     """
-    max_norm = _check_max_norm(max_norm)
     if isinstance(parameters, torch.Tensor):
         parameters = [parameters]
-    grads = [g for g in (p.grad for p in parameters) if g is not None]
-    if not grads:
-        _require_cuda("clip_grad_norm_")
-        return torch.zeros((), device="cuda")
-    _check_grads(grads, "clip_grad_norm_")
-    if error_if_nonfinite:
-        _raise_if_nonfinite(grads)
-    return _ensure_cuda_extension().clip_grads(grads, grads, max_norm)
+    return _ensure_cuda_extension().clip_grad_norm_(
+        list(parameters), float(max_norm), error_if_nonfinite
+    )
