@@ -19,8 +19,8 @@ using fssim_host::NvtxRange;
 
 constexpr int64_t kMaxChannels = int64_t{1} << 24;
 constexpr int64_t kMaxSamples = int64_t{1} << 30;
-// CTAs of one wave: two of 256 threads on each of 148 SMs.
-constexpr int64_t kWave = 148 * 2;
+// CTAs of one wave on 148 SMs.
+constexpr int64_t kWave = 148 * fssim::kNormResident;
 // A part has at least this many pixels for each thread, so that its set-up is paid for.
 constexpr int64_t kMinSteps = 4;
 // Bytes of input that the reducing pass may leave for the applying pass to find in L2.
@@ -65,6 +65,7 @@ NormGeometry make_geometry(int64_t N, int64_t P, int64_t C, int64_t G, int V, fl
   if (S > by_work) S = by_work;
   if (S < 1) S = 1;
   g.S = static_cast<int>(S);
+  g.inv_m = 1.0 / (static_cast<double>(P) * static_cast<double>(g.Cg));
   g.base = P / S;
   g.extra = static_cast<int>(P % S);
   return g;
@@ -79,8 +80,8 @@ int64_t samples_per_launch(int64_t N, int64_t bytes_per_sample) {
   return (N + cuts - 1) / cuts;
 }
 
-template <typename Kernel>
-int launch(Kernel k, dim3 grid, const NormParams& p, cudaStream_t stream, const char* what) {
+template <typename Kernel, typename... Extra>
+int launch(Kernel k, dim3 grid, const NormParams& p, cudaStream_t stream, const char* what, Extra... extra) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(fssim::kNormThreads);
@@ -90,7 +91,7 @@ int launch(Kernel k, dim3 grid, const NormParams& p, cudaStream_t stream, const 
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, k, p);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, k, p, extra...);
   if (e != cudaSuccess) {
     (void)cudaGetLastError();
     return fail(FSSIM_ERR_CUDA, std::string(what) + ": " + cudaGetErrorString(e));
@@ -157,27 +158,39 @@ BackwardPlan plan_backward(const fssim_group_norm_backward_args& a) {
   return p;
 }
 
+// Threads that merge one group, for this many partial results: a warp at least, a CTA at most.
+int team_threads(int64_t results) {
+  int t = 32;
+  while (t < fssim::kNormThreads && t < results) t *= 2;
+  return t;
+}
+dim3 team_grid(const NormGeometry& g, int team) {
+  const int64_t teams = fssim::kNormThreads / team;
+  return dim3(static_cast<unsigned>((g.N * g.G + teams - 1) / teams));
+}
+
 template <typename T, int V, int ACT>
 int forward_kernels(const NormParams& p, cudaStream_t s) {
-  int st = launch(fssim::norm_stats_kernel<T, V, 8>, tile_grid(p.g), p, s, "group norm statistics launch");
+  int st = launch(fssim::norm_stats_kernel<T, V, 4>, tile_grid(p.g), p, s, "group norm statistics launch");
   if (st) return st;
-  const int64_t groups = p.g.N * p.g.G;
-  st = launch(fssim::norm_merge_kernel,
-              dim3(static_cast<unsigned>((groups + fssim::kNormWarps - 1) / fssim::kNormWarps)), p, s,
-              "group norm merge launch");
+  const int team = team_threads(p.g.S);
+  st = launch(fssim::norm_merge_kernel, team_grid(p.g, team), p, s, "group norm merge launch", team);
   if (st) return st;
   return launch(fssim::norm_apply_kernel<T, V, ACT, 4>, tile_grid(p.g), p, s, "group norm launch");
 }
 
 template <typename T, int V, int ACT>
 int backward_kernels(const NormParams& p, cudaStream_t s) {
-  int st = launch(fssim::norm_grad_sums_kernel<T, V, ACT, 4>, tile_grid(p.g), p, s,
+  int st = launch(fssim::norm_grad_sums_kernel<T, V, ACT, 2>, tile_grid(p.g), p, s,
                   "group norm gradient sums launch");
   if (st) return st;
-  st = launch(fssim::norm_grad_coef_kernel, dim3(static_cast<unsigned>(p.g.N * p.g.G)), p, s,
-              "group norm gradient means launch");
+  int cols = 1;
+  while (cols < 32 && cols < p.g.Cg) cols *= 2;
+  const int team = team_threads(static_cast<int64_t>(p.g.S) * cols);
+  st = launch(fssim::norm_grad_merge_kernel, team_grid(p.g, team), p, s,
+              "group norm gradient merge launch", team, cols);
   if (st || !p.out) return st;
-  return launch(fssim::norm_grad_apply_kernel<T, V, ACT, 4>, tile_grid(p.g), p, s,
+  return launch(fssim::norm_grad_apply_kernel<T, V, ACT, 2>, tile_grid(p.g), p, s,
                 "group norm gradient launch");
 }
 
@@ -294,15 +307,16 @@ int backward_impl(const fssim_group_norm_backward_args* a, cudaStream_t stream) 
     p.sums = reinterpret_cast<float2*>(ws + plan.partial) + n * a->C;
     p.channel = reinterpret_cast<float*>(ws + plan.partial + plan.sums);
     p.early = n > 0 && a->dx != nullptr;
+    p.g.whole_batch = a->N == 1;
+    p.dweight = a->dweight;
+    p.dbias = a->dbias;
     st = dispatch<Backward>(a->dtype, plan.V, a->activation, p, stream);
     if (st) return st;
   }
-  if (!a->dweight && !a->dbias) return FSSIM_OK;
+  if (a->N == 1 || (!a->dweight && !a->dbias)) return FSSIM_OK;
   p.g.N = a->N;
   p.sums = reinterpret_cast<float2*>(ws + plan.partial);
-  p.dweight = a->dweight;
-  p.dbias = a->dbias;
-  const unsigned blocks = static_cast<unsigned>((a->C + fssim::kNormThreads - 1) / fssim::kNormThreads);
+  const unsigned blocks = static_cast<unsigned>((a->C + fssim::kNormWarps - 1) / fssim::kNormWarps);
   return launch(fssim::norm_param_grad_kernel, dim3(blocks), p, stream,
                 "group norm parameter gradient launch");
 }

@@ -37,6 +37,7 @@ namespace fssim {
 
 constexpr int kNormThreads = 256;
 constexpr int kNormWarps = kNormThreads / 32;
+constexpr int kNormResident = 3;  // CTAs of the passes on one SM
 
 enum NormAct { kNormActNone = 0, kNormActSilu = 1, kNormActRelu = 2 };
 
@@ -51,7 +52,8 @@ struct NormGeometry {
   int S;       // parts of a sample's pixels
   int GS;      // most groups that touch one slice
   float eps;
-
+  double inv_m;      // 1 / (P * Cg)
+  int whole_batch;   // the call has one sample, this one
   int64_t base;  // pixels of a part; the first `extra` parts have one more
   int extra;
 
@@ -89,39 +91,69 @@ template <> struct RawVec<16> { using type = uint4; };
 template <> struct RawVec<4> { using type = unsigned; };
 template <> struct RawVec<2> { using type = unsigned short; };
 
+// V elements in registers as pairs, for the packed FP32 instructions (one for two elements). A
+// lone element has a pair to itself, whose second half is zero and never stored.
+template <int V> constexpr int kPairs = (V + 1) / 2;
+
+__device__ __forceinline__ float2 norm_pair(unsigned w, __half) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+__device__ __forceinline__ float2 norm_pair(unsigned w, __nv_bfloat16) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+__device__ __forceinline__ unsigned norm_word(float2 f, __half) {
+  const __half2 h = __floats2half2_rn(f.x, f.y);
+  return *reinterpret_cast<const unsigned*>(&h);
+}
+__device__ __forceinline__ unsigned norm_word(float2 f, __nv_bfloat16) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(f.x, f.y);
+  return *reinterpret_cast<const unsigned*>(&h);
+}
+
 template <typename T, int V>
 struct VecIO {
   using Raw = typename RawVec<sizeof(T) * V>::type;
+  static constexpr int N = kPairs<V>;
   static __device__ __forceinline__ Raw load(const T* p) { return *reinterpret_cast<const Raw*>(p); }
   static __device__ __forceinline__ void store(T* p, const Raw& r) { *reinterpret_cast<Raw*>(p) = r; }
-  static __device__ __forceinline__ void unpack(const Raw& r, float (&f)[V]);
-  static __device__ __forceinline__ Raw pack(const float (&f)[V]);
+  static __device__ __forceinline__ void unpack(const Raw& r, float2 (&f)[N]) {
+    if constexpr (sizeof(T) == 4) {
+      const float* e = reinterpret_cast<const float*>(&r);
+#pragma unroll
+      for (int i = 0; i < N; ++i) f[i] = make_float2(e[2 * i], V > 1 ? e[2 * i + 1] : 0.f);
+    } else if constexpr (V == 1) {
+      f[0] = norm_pair(static_cast<unsigned>(r), T());
+    } else {
+      const unsigned* w = reinterpret_cast<const unsigned*>(&r);
+#pragma unroll
+      for (int i = 0; i < N; ++i) f[i] = norm_pair(w[i], T());
+    }
+  }
+  static __device__ __forceinline__ Raw pack(const float2 (&f)[N]) {
+    Raw r;
+    if constexpr (sizeof(T) == 4) {
+      float* e = reinterpret_cast<float*>(&r);
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        e[2 * i] = f[i].x;
+        if (V > 1) e[2 * i + 1] = f[i].y;
+      }
+    } else if constexpr (V == 1) {
+      r = static_cast<Raw>(norm_word(f[0], T()));
+    } else {
+      unsigned* w = reinterpret_cast<unsigned*>(&r);
+#pragma unroll
+      for (int i = 0; i < N; ++i) w[i] = norm_word(f[i], T());
+    }
+    return r;
+  }
 };
 
-__device__ __forceinline__ float norm_to_float(float v) { return v; }
-__device__ __forceinline__ float norm_to_float(__half v) { return __half2float(v); }
-__device__ __forceinline__ float norm_to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <typename T> __device__ __forceinline__ T norm_from_float(float v);
-template <> __device__ __forceinline__ float norm_from_float<float>(float v) { return v; }
-template <> __device__ __forceinline__ __half norm_from_float<__half>(float v) { return __float2half_rn(v); }
-template <> __device__ __forceinline__ __nv_bfloat16 norm_from_float<__nv_bfloat16>(float v) {
-  return __float2bfloat16_rn(v);
-}
-
-template <typename T, int V>
-__device__ __forceinline__ void VecIO<T, V>::unpack(const Raw& r, float (&f)[V]) {
-  const T* e = reinterpret_cast<const T*>(&r);
-#pragma unroll
-  for (int i = 0; i < V; ++i) f[i] = norm_to_float(e[i]);
-}
-template <typename T, int V>
-__device__ __forceinline__ typename VecIO<T, V>::Raw VecIO<T, V>::pack(const float (&f)[V]) {
-  Raw r;
-  T* e = reinterpret_cast<T*>(&r);
-#pragma unroll
-  for (int i = 0; i < V; ++i) e[i] = norm_from_float<T>(f[i]);
-  return r;
-}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) { return __fadd2_rn(a, b); }
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) { return __fmul2_rn(a, b); }
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
+__device__ __forceinline__ float2 neg2(float2 a) { return make_float2(-a.x, -a.y); }
+__device__ __forceinline__ float2 splat2(float a) { return make_float2(a, a); }
 
 // Weights come in any of the three types, whatever x's is; read once per thread.
 __device__ __forceinline__ float load_weight(const void* p, int dtype, int c) {
@@ -137,42 +169,57 @@ __device__ __forceinline__ void store_weight(void* p, int dtype, int c, float v)
 
 // V consecutive values of a row of `channel`, which starts at a multiple of V floats.
 template <int V>
-__device__ __forceinline__ void load_channels(const float* p, float (&f)[V]) {
+__device__ __forceinline__ void load_channels(const float* p, float2 (&f)[kPairs<V>]) {
   if constexpr (V % 4 == 0) {
 #pragma unroll
     for (int i = 0; i < V; i += 4) {
       const float4 v = *reinterpret_cast<const float4*>(p + i);
-      f[i] = v.x; f[i + 1] = v.y; f[i + 2] = v.z; f[i + 3] = v.w;
+      f[i / 2] = make_float2(v.x, v.y);
+      f[i / 2 + 1] = make_float2(v.z, v.w);
     }
+  } else if constexpr (V == 2) {
+    f[0] = *reinterpret_cast<const float2*>(p);
   } else {
-#pragma unroll
-    for (int i = 0; i < V; ++i) f[i] = p[i];
+    f[0] = make_float2(*p, 0.f);
   }
 }
 
-// ---- activations ----
-// The logistic function. For 16-bit tensors the hardware's approximate exponential and
-// reciprocal do (relative errors near 2^-21, against a half step of 2^-9 or 2^-12 in the
-// output); 32-bit tensors take the full-precision functions.
+// ---- activations, on pairs ----
+// The logistic function, from the hardware's approximate reciprocal (one unit in the last place)
+// and, for 16-bit tensors, its approximate power of two: together relative errors near 2^-21,
+// against a half step of 2^-9 or 2^-12 in the output. 32-bit tensors take expf.
 template <typename T>
-__device__ __forceinline__ float logistic(float z) {
-  if constexpr (sizeof(T) == 2) return __fdividef(1.f, 1.f + __expf(-z));
-  else return 1.f / (1.f + expf(-z));
+__device__ __forceinline__ float2 logistic(float2 z) {
+  float2 e;
+  if constexpr (sizeof(T) == 2) {
+    const float2 t = mul2(z, splat2(-1.44269504f));  // 2^(-z / ln 2) = exp(-z)
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(t.x));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(t.y));
+  } else {
+    e = make_float2(expf(-z.x), expf(-z.y));
+  }
+  e = add2(e, splat2(1.f));
+  float2 s;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s.x) : "f"(e.x));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s.y) : "f"(e.y));
+  return s;
 }
 template <typename T, int ACT>
-__device__ __forceinline__ float activate(float z) {
-  if constexpr (ACT == kNormActSilu) return z * logistic<T>(z);
-  else if constexpr (ACT == kNormActRelu) return z < 0.f ? 0.f : z;  // NaN stays NaN
+__device__ __forceinline__ float2 activate(float2 z) {
+  if constexpr (ACT == kNormActSilu) return mul2(z, logistic<T>(z));
+  else if constexpr (ACT == kNormActRelu)
+    return make_float2(z.x < 0.f ? 0.f : z.x, z.y < 0.f ? 0.f : z.y);  // NaN stays NaN
   else return z;
 }
 // dy * act'(z)
 template <typename T, int ACT>
-__device__ __forceinline__ float activate_grad(float z, float dy) {
+__device__ __forceinline__ float2 activate_grad(float2 z, float2 dy) {
   if constexpr (ACT == kNormActSilu) {
-    const float s = logistic<T>(z);
-    return dy * (s * fmaf(z, 1.f - s, 1.f));
+    const float2 s = logistic<T>(z);
+    const float2 rest = fma2(s, splat2(-1.f), splat2(1.f));
+    return mul2(mul2(dy, s), fma2(z, rest, splat2(1.f)));
   } else if constexpr (ACT == kNormActRelu) {
-    return z <= 0.f ? 0.f : dy;
+    return make_float2(z.x <= 0.f ? 0.f : dy.x, z.y <= 0.f ? 0.f : dy.y);
   } else {
     return dy;
   }
@@ -216,42 +263,56 @@ struct NormTile {
   }
 };
 
-// First channel, from the slice's first, of the group that channel c of the slice is in.
-__device__ __forceinline__ int group_begin(const NormGeometry& g, const NormTile& t, int c) {
-  return max((t.c0 + c) / g.Cg * g.Cg - t.c0, 0);
-}
-
-// out[c] = sum over the rows r of f(r, c), for the `width` channels of a slice: L lanes (a power
-// of two, at most a warp) for each channel. All threads take part.
-template <typename F>
-__device__ __forceinline__ void norm_sum_rows(int rows, int pitch, int width, float* out, F f) {
-  const int L = rows >= 32 ? 32 : 1 << (31 - __clz(rows));
-  const int sub = threadIdx.x & (L - 1), each = kNormThreads / L;
-  for (int b = 0; b < width; b += each) {
-    const int c = b + threadIdx.x / L;
-    float v = 0.f;
-    if (c < width)
-      for (int r = sub; r < rows; r += L) v += f(r, c);
-    for (int o = L / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    if (c < width && sub == 0) out[c] = v;
+// V values into shared memory.
+template <int V>
+__device__ __forceinline__ void norm_put(float* p, const float2 (&f)[kPairs<V>]) {
+#pragma unroll
+  for (int i = 0; i < kPairs<V>; ++i) {
+    p[2 * i] = f[i].x;
+    if (V > 1) p[2 * i + 1] = f[i].y;
   }
 }
 
-// f(i, cb, w, sum of in[cb .. cb + w)) for the i-th group that touches the slice, its channels
-// [cb, cb + w) of the slice: a thread for each narrow group, a warp for each wide one.
-template <typename F>
-__device__ __forceinline__ void norm_sum_groups(const NormGeometry& g, const NormTile& t, const float* in, F f) {
-  const bool narrow = g.Cg <= 32;
-  const int lane = narrow ? 0 : threadIdx.x % 32, lanes = narrow ? 1 : 32;
-  for (int i = threadIdx.x / lanes; i < t.g1 - t.g0; i += kNormThreads / lanes) {
-    const int cb = max((t.g0 + i) * g.Cg, t.c0) - t.c0;
-    const int w = min((t.g0 + i + 1) * g.Cg, t.c1) - t.c0 - cb;
-    float v = 0.f;
-    for (int c = lane; c < w; c += lanes) v += in[cb + c];
-    if (!narrow) v = warp_sum(v);
-    if (lane == 0) f(i, cb, w, v);
+// Sums over a CTA's rows, then over a group's channels. The rows are shared out over T threads for
+// each channel (all of the CTA's, where the slice has fewer channels than threads), which leave
+// T subtotals of each channel in out[j * SC + c]; f(c) gives the function of a row for channel c.
+struct NormColumns {
+  int cols, T, col, sub;
+  __device__ __forceinline__ explicit NormColumns(int width) {
+    cols = width > kNormThreads / 2 ? kNormThreads : 1 << (32 - __clz(width - 1));
+    if (width == 1) cols = 1;
+    T = kNormThreads / cols;
+    col = threadIdx.x & (cols - 1);
+    sub = threadIdx.x / cols;
   }
-}
+  template <typename F>
+  __device__ __forceinline__ void sum_rows(const NormGeometry& g, int width, float* out, F f) const {
+    for (int c = col; c < width; c += cols) {
+      const auto value = f(c);
+      float v = 0.f;
+#pragma unroll 4
+      for (int r = sub; r < g.rows; r += T) v += value(r);
+      out[sub * g.SC + c] = v;
+    }
+  }
+  // f(i, cb, w, sum of the subtotals of [cb, cb + w)) for the i-th group that touches the slice,
+  // its channels [cb, cb + w) of the slice: a thread for each where there is little to add, a
+  // warp for each otherwise.
+  template <typename F>
+  __device__ __forceinline__ void sum_groups(const NormGeometry& g, const NormTile& t, const float* in, F f) const {
+    const bool narrow = g.Cg * T <= 16;
+    const int lane = narrow ? 0 : threadIdx.x % 32, lanes = narrow ? 1 : 32;
+    for (int i = threadIdx.x / lanes; i < t.g1 - t.g0; i += kNormThreads / lanes) {
+      const int cb = max((t.g0 + i) * g.Cg, t.c0) - t.c0;
+      const int w = min((t.g0 + i + 1) * g.Cg, t.c1) - t.c0 - cb;
+      float v = 0.f;
+      for (int j = 0; j < T; ++j)
+        for (int c = lane; c < w; c += lanes) v += in[j * g.SC + cb + c];
+      if (!narrow) v = warp_sum(v);
+      if (lane == 0) f(i, cb, w, v);
+    }
+  }
+};
 
 // The pixels of a thread in the applying passes: from the end of its part to the beginning (what
 // the reducing pass read last is what L2 still holds), U at a time; the last step, at the
@@ -279,7 +340,7 @@ struct NormSteps {
 
 // ---- forward: statistics ----
 template <typename T, int V, int U>
-__global__ void __launch_bounds__(kNormThreads) norm_stats_kernel(const __grid_constant__ NormParams p) {
+__global__ void __launch_bounds__(kNormThreads, kNormResident) norm_stats_kernel(const __grid_constant__ NormParams p) {
   __shared__ float sm_mean[kNormThreads * V];
   __shared__ float sm_m2[kNormThreads * V];
   __shared__ float column[kNormThreads * V];
@@ -289,9 +350,10 @@ __global__ void __launch_bounds__(kNormThreads) norm_stats_kernel(const __grid_c
   if (!p.early) grid_dependency_wait();
   grid_launch_dependents();
   using IO = VecIO<T, V>;
-  float mean[V], m2[V];
+  constexpr int N = IO::N;
+  float2 mean[N], m2[N];
 #pragma unroll
-  for (int v = 0; v < V; ++v) mean[v] = m2[v] = 0.f;
+  for (int v = 0; v < N; ++v) mean[v] = m2[v] = splat2(0.f);
   if (t.active) {
     const T* x = static_cast<const T*>(p.x) + static_cast<int64_t>(t.n) * g.P * g.C + t.c0 + t.chan;
     const int64_t step = static_cast<int64_t>(g.rows);
@@ -306,39 +368,37 @@ __global__ void __launch_bounds__(kNormThreads) norm_stats_kernel(const __grid_c
         if (kWhole || u < k) raw[u] = IO::load(x + (px + u * step) * g.C);
         else raw[u] = typename IO::Raw{};
       }
-      float f[U][V];
+      float2 f[U][N];
 #pragma unroll
       for (int u = 0; u < U; ++u) IO::unpack(raw[u], f[u]);
       const float taken = kWhole ? U : k;
       const float total = count + taken;
-      const float each = kWhole ? 1.f / U : 1.f / taken;
+      const float2 each = splat2(kWhole ? 1.f / U : 1.f / taken);
       const float share = taken / total;   // weight of the new values in the mean
       const float cross = count * share;   // and of the squared distance of the means
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        float sum = 0.f;
+      for (int v = 0; v < N; ++v) {
+        float2 sum = f[0][v];
 #pragma unroll
-        for (int u = 0; u < U; ++u) sum += f[u][v];
-        const float m = sum * each;
-        float q = 0.f;
+        for (int u = 1; u < U; ++u) sum = add2(sum, f[u][v]);
+        const float2 m = mul2(sum, each), minus = neg2(m);
+        float2 q = splat2(0.f);
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const float d = kWhole || u < k ? f[u][v] - m : 0.f;
-          q = fmaf(d, d, q);
-        }
-        const float d = m - mean[v];
-        mean[v] = fmaf(d, share, mean[v]);
-        m2[v] += fmaf(d * d, cross, q);
+        for (int u = 0; u < U; ++u)
+          if (kWhole || u < k) {
+            const float2 d = add2(f[u][v], minus);
+            q = fma2(d, d, q);
+          }
+        const float2 d = add2(m, neg2(mean[v]));
+        mean[v] = fma2(d, splat2(share), mean[v]);
+        m2[v] = add2(m2[v], fma2(mul2(d, d), splat2(cross), q));
       }
       count = total;
     };
     for (; px + (U - 1) * step < t.p1; px += U * step) take(std::true_type{}, U);
     if (px < t.p1) take(std::false_type{}, static_cast<int>((t.p1 - px - 1) / step) + 1);
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      sm_mean[t.row * g.SC + t.chan + v] = mean[v];
-      sm_m2[t.row * g.SC + t.chan + v] = m2[v];
-    }
+    norm_put<V>(sm_mean + t.row * g.SC + t.chan, mean);
+    norm_put<V>(sm_m2 + t.row * g.SC + t.chan, m2);
   }
   __syncthreads();
   // The rows' and channels' pairs become one pair per group: first the mean (as distances from
@@ -347,75 +407,108 @@ __global__ void __launch_bounds__(kNormThreads) norm_stats_kernel(const __grid_c
   const int64_t full = pixels / g.rows;                        // pixels that every row took
   const int extra = static_cast<int>(pixels - full * g.rows);  // rows that took one more
   const int width = t.c1 - t.c0;
+  const NormColumns columns(width);
   const auto count_of = [&](int row) { return static_cast<float>(full + (row < extra)); };
-  norm_sum_rows(g.rows, g.SC, width, column, [&](int r, int c) {
-    const float cnt = count_of(r);
-    return cnt > 0.f ? cnt * (sm_mean[r * g.SC + c] - sm_mean[group_begin(g, t, c)]) : 0.f;
+  columns.sum_rows(g, width, column, [&](int c) {
+    const float ref = sm_mean[max((t.c0 + c) / g.Cg * g.Cg - t.c0, 0)];
+    return [&, c, ref](int r) {
+      const float cnt = count_of(r);
+      return cnt > 0.f ? cnt * (sm_mean[r * g.SC + c] - ref) : 0.f;
+    };
   });
   __syncthreads();
   float2* partial = p.partial + ((static_cast<int64_t>(t.n) * g.S + t.s) * g.slices + t.slice) * g.GS;
-  norm_sum_groups(g, t, column, [&](int i, int cb, int w, float sum) {
+  columns.sum_groups(g, t, column, [&](int i, int cb, int w, float sum) {
     centre[i] = sm_mean[cb] + sum / (static_cast<float>(pixels) * w);
   });
   __syncthreads();
-  norm_sum_rows(g.rows, g.SC, width, column, [&](int r, int c) {
-    const float cnt = count_of(r);
-    const float d = sm_mean[r * g.SC + c] - centre[(t.c0 + c) / g.Cg - t.g0];
-    return cnt > 0.f ? fmaf(cnt * d, d, sm_m2[r * g.SC + c]) : 0.f;
+  columns.sum_rows(g, width, column, [&](int c) {
+    const float m = centre[(t.c0 + c) / g.Cg - t.g0];
+    return [&, c, m](int r) {
+      const float cnt = count_of(r);
+      const float d = sm_mean[r * g.SC + c] - m;
+      return cnt > 0.f ? fmaf(cnt * d, d, sm_m2[r * g.SC + c]) : 0.f;
+    };
   });
   __syncthreads();
-  norm_sum_groups(g, t, column, [&](int i, int cb, int w, float sum) {
+  columns.sum_groups(g, t, column, [&](int i, int cb, int w, float sum) {
     partial[i] = make_float2(centre[i], sum);
   });
   if (p.early) grid_dependency_wait();
 }
 
-// ---- forward: the parts' pairs become the groups' statistics. One warp per (sample, group) ----
-__global__ void __launch_bounds__(kNormThreads) norm_merge_kernel(const __grid_constant__ NormParams p) {
+// ---- the merging launches: a team of kNormThreads / teams threads for each (sample, group) ----
+// Sums of two values over a team (a power of two of threads, a warp at least), in all its
+// threads. Every thread of the block takes part.
+__device__ __forceinline__ double2 team_sum(double a, double b, int team_threads, double2* sm) {
+  a = warp_sum(a);
+  b = warp_sum(b);
+  if (team_threads == 32) return make_double2(a, b);
+  __syncthreads();
+  if (threadIdx.x % 32 == 0) sm[threadIdx.x / 32] = make_double2(a, b);
+  __syncthreads();
+  const int first = threadIdx.x / team_threads * team_threads / 32;
+  double2 s = make_double2(0.0, 0.0);
+  for (int i = 0; i < team_threads / 32; ++i) {
+    s.x += sm[first + i].x;
+    s.y += sm[first + i].y;
+  }
+  return s;
+}
+
+// Forward: the parts' pairs become the group's statistics and its channels' constants.
+__global__ void __launch_bounds__(kNormThreads) norm_merge_kernel(const __grid_constant__ NormParams p,
+                                                                  int team_threads) {
+  __shared__ double2 sm[kNormWarps];
   const NormGeometry& g = p.g;
-  const int64_t id = static_cast<int64_t>(blockIdx.x) * kNormWarps + threadIdx.x / 32;
-  const int lane = threadIdx.x % 32;
+  const int teams = kNormThreads / team_threads;
+  const int64_t id = static_cast<int64_t>(blockIdx.x) * teams + threadIdx.x / team_threads;
+  const int lane = threadIdx.x % team_threads;
   grid_dependency_wait();
   grid_launch_dependents();
-  if (id >= g.N * g.G) return;
+  const bool real = id < g.N * g.G;
   const int64_t n = id / g.G;
   const int grp = static_cast<int>(id - n * g.G);
   const int c0 = grp * g.Cg, c1 = c0 + g.Cg;
-  const int first = c0 / g.SC, last = (c1 - 1) / g.SC;
-  const double inv = 1.0 / (static_cast<double>(g.P) * g.Cg);
   double ref = 0.0, sum = 0.0, q = 0.0;  // sums of distances from ref, and of squares around it
-  for (int k = first; k <= last; ++k) {  // the slices that hold a piece of the group
-    const int b = k * g.SC, width = min(c1, b + g.SC) - max(c0, b);
-    const float2* pairs = p.partial + (n * g.S * g.slices + k) * g.GS + grp - b / g.Cg;
-    if (k == first) ref = pairs[0].x;
-    for (int s = lane; s < g.S; s += 32) {
-      const float2 v = pairs[static_cast<int64_t>(s) * g.slices * g.GS];
-      const double cnt = static_cast<double>(g.part_pixels(s)) * width;
-      const double d = v.x - ref;
-      sum = fma(cnt, d, sum);
-      q += fma(cnt * d, d, static_cast<double>(v.y));
+  if (real) {
+    const int first = c0 / g.SC, last = (c1 - 1) / g.SC;
+    for (int k = first; k <= last; ++k) {  // the slices that hold a piece of the group
+      const int b = k * g.SC, width = min(c1, b + g.SC) - max(c0, b);
+      const float2* pairs = p.partial + (n * g.S * g.slices + k) * g.GS + grp - b / g.Cg;
+      if (k == first) ref = pairs[0].x;
+      for (int s = lane; s < g.S; s += team_threads) {
+        const float2 v = pairs[static_cast<int64_t>(s) * g.slices * g.GS];
+        const double cnt = static_cast<double>(g.part_pixels(s)) * width;
+        const double d = v.x - ref;
+        sum = fma(cnt, d, sum);
+        q += fma(cnt * d, d, static_cast<double>(v.y));
+      }
     }
   }
-  sum = warp_sum(sum) * inv;
-  double var = warp_sum(q) * inv - sum * sum;
+  const double2 total = team_sum(sum, q, team_threads, sm);
+  if (!real) return;
+  sum = total.x * g.inv_m;
+  double var = total.y * g.inv_m - sum * sum;
   if (var < 0.0) var = 0.0;  // a NaN stays
   const float mean = static_cast<float>(ref + sum);
-  const float rstd = static_cast<float>(1.0 / sqrt(var + static_cast<double>(g.eps)));
+  const float rstd = __frsqrt_rn(static_cast<float>(var + static_cast<double>(g.eps)));
   if (p.mean && lane == 0) {
     p.mean[id] = mean;
     p.rstd[id] = rstd;
   }
-  float* row = p.channel + n * kNormForwardRows * g.C;
-  for (int c = c0 + lane; c < c1; c += 32) {
-    row[c] = mean;
-    row[g.C + c] = p.weight ? rstd * load_weight(p.weight, p.weight_dtype, c) : rstd;
-    row[2 * static_cast<int64_t>(g.C) + c] = p.bias ? load_weight(p.bias, p.weight_dtype, c) : 0.f;
+  const int64_t C = g.C;
+  float* row = p.channel + n * kNormForwardRows * C;
+  for (int c = c0 + lane; c < c1; c += team_threads) {
+    row[c] = -mean;
+    row[C + c] = p.weight ? rstd * load_weight(p.weight, p.weight_dtype, c) : rstd;
+    row[2 * C + c] = p.bias ? load_weight(p.bias, p.weight_dtype, c) : 0.f;
   }
 }
 
 // ---- forward: y ----
 template <typename T, int V, int ACT, int U>
-__global__ void __launch_bounds__(kNormThreads) norm_apply_kernel(const __grid_constant__ NormParams p) {
+__global__ void __launch_bounds__(kNormThreads, kNormResident) norm_apply_kernel(const __grid_constant__ NormParams p) {
   const NormGeometry& g = p.g;
   const NormTile t(g, V);
   using IO = VecIO<T, V>;
@@ -433,19 +526,20 @@ __global__ void __launch_bounds__(kNormThreads) norm_apply_kernel(const __grid_c
   };
   if (steps.more()) fetch();
   grid_dependency_wait();
-  float mean[V], a[V], b[V];
+  constexpr int N = IO::N;
+  float2 minus[N], a[N], b[N];  // -mean, the factor and the shift
   if (t.active) {
     const float* row = p.channel + static_cast<int64_t>(t.n) * kNormForwardRows * g.C + t.c0 + t.chan;
-    load_channels<V>(row, mean);
+    load_channels<V>(row, minus);
     load_channels<V>(row + g.C, a);
     load_channels<V>(row + 2 * static_cast<int64_t>(g.C), b);
   }
   grid_launch_dependents();  // the statistics have been read
   auto emit = [&](const typename IO::Raw& r, int64_t at) {
-    float f[V];
+    float2 f[N];
     IO::unpack(r, f);
 #pragma unroll
-    for (int v = 0; v < V; ++v) f[v] = activate<T, ACT>(fmaf(f[v] - mean[v], a[v], b[v]));
+    for (int v = 0; v < N; ++v) f[v] = activate<T, ACT>(fma2(add2(f[v], minus[v]), a[v], b[v]));
     IO::store(y + at * g.C, IO::pack(f));
   };
   while (steps.more()) {
@@ -459,7 +553,7 @@ __global__ void __launch_bounds__(kNormThreads) norm_apply_kernel(const __grid_c
 
 // ---- backward: per-channel sums of one part ----
 template <typename T, int V, int ACT, int U>
-__global__ void __launch_bounds__(kNormThreads) norm_grad_sums_kernel(const __grid_constant__ NormParams p) {
+__global__ void __launch_bounds__(kNormThreads, kNormResident) norm_grad_sums_kernel(const __grid_constant__ NormParams p) {
   __shared__ float sm1[kNormThreads * V];
   __shared__ float sm2[kNormThreads * V];
   __shared__ float column1[kNormThreads * V];
@@ -470,152 +564,182 @@ __global__ void __launch_bounds__(kNormThreads) norm_grad_sums_kernel(const __gr
   grid_launch_dependents();
   using IO = VecIO<T, V>;
   if (t.active) {
-    float mean[V], a[V], b[V], s1[V], s2[V];
+    constexpr int N = IO::N;
+    float2 minus[N], a[N], b[N], s1[N], s2[N];
     const int first = t.c0 + t.chan;
     int grp = first / g.Cg, end = (grp + 1) * g.Cg;  // one division; the next channels follow
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
+    for (int v = 0; v < 2 * N; ++v) {
       const int c = first + v;
-      if (c == end) {
-        ++grp;
-        end += g.Cg;
+      float mv = 0.f, av = 0.f, bv = 0.f;
+      if (v < V) {
+        if (c == end) {
+          ++grp;
+          end += g.Cg;
+        }
+        const int64_t at = static_cast<int64_t>(t.n) * g.G + grp;
+        mv = -p.mean[at];
+        av = p.weight ? p.rstd[at] * load_weight(p.weight, p.weight_dtype, c) : p.rstd[at];
+        bv = p.bias ? load_weight(p.bias, p.weight_dtype, c) : 0.f;
       }
-      const int64_t at = static_cast<int64_t>(t.n) * g.G + grp;
-      mean[v] = p.mean[at];
-      a[v] = p.weight ? p.rstd[at] * load_weight(p.weight, p.weight_dtype, c) : p.rstd[at];
-      b[v] = p.bias ? load_weight(p.bias, p.weight_dtype, c) : 0.f;
-      s1[v] = s2[v] = 0.f;
+      (v & 1 ? minus[v / 2].y : minus[v / 2].x) = mv;
+      (v & 1 ? a[v / 2].y : a[v / 2].x) = av;
+      (v & 1 ? b[v / 2].y : b[v / 2].x) = bv;
     }
+#pragma unroll
+    for (int v = 0; v < N; ++v) s1[v] = s2[v] = splat2(0.f);
     const int64_t base = static_cast<int64_t>(t.n) * g.P * g.C + t.c0 + t.chan;
     const T* x = static_cast<const T*>(p.x) + base;
     const T* dy = static_cast<const T*>(p.dy) + base;
     const int64_t step = g.rows;
     int64_t px = t.p0 + t.row;
     auto take = [&](const typename IO::Raw& rx, const typename IO::Raw& rd) {
-      float f[V], d[V];
+      float2 f[N], d[N];
       IO::unpack(rx, f);
       IO::unpack(rd, d);
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        const float xc = f[v] - mean[v];
-        const float dz = activate_grad<T, ACT>(fmaf(xc, a[v], b[v]), d[v]);
-        s1[v] += dz;
-        s2[v] = fmaf(dz, xc, s2[v]);
+      for (int v = 0; v < N; ++v) {
+        const float2 xc = add2(f[v], minus[v]);
+        const float2 dz = activate_grad<T, ACT>(fma2(xc, a[v], b[v]), d[v]);
+        s1[v] = add2(s1[v], dz);
+        s2[v] = fma2(dz, xc, s2[v]);
       }
     };
-    for (; px < t.p1; px += U * step) {
+    auto step_of = [&](auto whole) {
+      constexpr bool kWhole = decltype(whole)::value;
       typename IO::Raw rx[U], rd[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        if (px + u * step < t.p1) {
+        if (kWhole || px + u * step < t.p1) {
           rx[u] = IO::load(x + (px + u * step) * g.C);
           rd[u] = IO::load(dy + (px + u * step) * g.C);
         }
       }
 #pragma unroll
       for (int u = 0; u < U; ++u)
-        if (px + u * step < t.p1) take(rx[u], rd[u]);
-    }
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      sm1[t.row * g.SC + t.chan + v] = s1[v];
-      sm2[t.row * g.SC + t.chan + v] = s2[v];
-    }
+        if (kWhole || px + u * step < t.p1) take(rx[u], rd[u]);
+    };
+    for (; px + (U - 1) * step < t.p1; px += U * step) step_of(std::true_type{});
+    if (px < t.p1) step_of(std::false_type{});
+    norm_put<V>(sm1 + t.row * g.SC + t.chan, s1);
+    norm_put<V>(sm2 + t.row * g.SC + t.chan, s2);
   }
   __syncthreads();
   const int width = t.c1 - t.c0;
-  norm_sum_rows(g.rows, g.SC, width, column1, [&](int r, int c) { return sm1[r * g.SC + c]; });
-  norm_sum_rows(g.rows, g.SC, width, column2, [&](int r, int c) { return sm2[r * g.SC + c]; });
+  const NormColumns columns(width);
+  columns.sum_rows(g, width, column1, [&](int c) { return [&, c](int r) { return sm1[r * g.SC + c]; }; });
+  columns.sum_rows(g, width, column2, [&](int c) { return [&, c](int r) { return sm2[r * g.SC + c]; }; });
   __syncthreads();
   float2* partial = p.partial + (static_cast<int64_t>(t.n) * g.S + t.s) * g.C + t.c0;
-  for (int c = threadIdx.x; c < width; c += kNormThreads) partial[c] = make_float2(column1[c], column2[c]);
+  for (int c = threadIdx.x; c < width; c += kNormThreads) {
+    float v1 = 0.f, v2 = 0.f;
+    for (int j = 0; j < columns.T; ++j) {
+      v1 += column1[j * g.SC + c];
+      v2 += column2[j * g.SC + c];
+    }
+    partial[c] = make_float2(v1, v2);
+  }
   if (p.early) grid_dependency_wait();
 }
 
-// ---- backward: sums over the parts, and each group's two means. One CTA per (group, sample) ----
-__global__ void __launch_bounds__(kNormThreads) norm_grad_coef_kernel(const __grid_constant__ NormParams p) {
-  __shared__ double sm1[kNormThreads], sm2[kNormThreads];
-  __shared__ float means[2];
+// Backward: sums over the parts, and the group's two means. `cols` (a power of two, at most 32)
+// channels are summed at a time, by team_threads / cols threads each.
+__global__ void __launch_bounds__(kNormThreads) norm_grad_merge_kernel(const __grid_constant__ NormParams p,
+                                                                       int team_threads, int cols) {
+  __shared__ double2 sm[kNormThreads];
   const NormGeometry& g = p.g;
-  const int64_t n = blockIdx.x / static_cast<unsigned>(g.G);
-  const int grp = static_cast<int>(blockIdx.x - n * g.G);
+  const int teams = kNormThreads / team_threads;
+  const int64_t id = static_cast<int64_t>(blockIdx.x) * teams + threadIdx.x / team_threads;
+  const int lane = threadIdx.x % team_threads;
   grid_dependency_wait();
   grid_launch_dependents();
-  // cols channels at a time (a power of two, at most 32), kNormThreads / cols threads each
-  int cols = 1;
-  while (cols < 32 && cols < g.Cg) cols *= 2;
-  const int col = threadIdx.x % cols, sub = threadIdx.x / cols, subs = kNormThreads / cols;
-  const float mean = p.mean[n * g.G + grp], rstd = p.rstd[n * g.G + grp];
+  const bool real = id < g.N * g.G;
+  const int64_t n = id / g.G;
+  const int grp = static_cast<int>(id - n * g.G);
+  const int col = lane % cols, sub = lane / cols, subs = team_threads / cols;
+  const float mean = real ? p.mean[id] : 0.f, rstd = real ? p.rstd[id] : 0.f;
   double w1 = 0.0, w2 = 0.0;  // sum of w dz and of w dz xhat, kept by the threads with sub == 0
   for (int cb = 0; cb < g.Cg; cb += cols) {
-    const int c = cb + col;
+    const int c = cb + col, ch = grp * g.Cg + c;
+    const bool mine = real && c < g.Cg;
     double v1 = 0.0, v2 = 0.0;
-    if (c < g.Cg)
+    if (mine) {
+      const float2* at = p.partial + n * g.S * g.C + ch;
+#pragma unroll 4
       for (int s = sub; s < g.S; s += subs) {
-        const float2 v = p.partial[(n * g.S + s) * g.C + grp * g.Cg + c];
+        const float2 v = at[static_cast<int64_t>(s) * g.C];
         v1 += v.x;
         v2 += v.y;
       }
-    sm1[threadIdx.x] = v1;
-    sm2[threadIdx.x] = v2;
-    __syncthreads();
-    for (int o = subs / 2; o > 0; o >>= 1) {
-      if (sub < o) {
-        sm1[threadIdx.x] += sm1[threadIdx.x + o * cols];
-        sm2[threadIdx.x] += sm2[threadIdx.x + o * cols];
-      }
+    }
+    // within the warp first, then over the team's warps
+    for (int o = 16; o >= cols; o >>= 1) {
+      v1 += __shfl_xor_sync(0xffffffffu, v1, o);
+      v2 += __shfl_xor_sync(0xffffffffu, v2, o);
+    }
+    if (team_threads > 32) {
       __syncthreads();
+      if (threadIdx.x % 32 < cols) sm[threadIdx.x / 32 * 32 + col] = make_double2(v1, v2);
+      __syncthreads();
+      if (sub == 0) {
+        v1 = v2 = 0.0;
+        for (int i = 0; i < team_threads; i += 32) {
+          v1 += sm[threadIdx.x + i].x;
+          v2 += sm[threadIdx.x + i].y;
+        }
+      }
     }
-    if (sub == 0 && c < g.Cg) {
-      const int ch = grp * g.Cg + c;
-      const double s1 = sm1[threadIdx.x], s2 = sm2[threadIdx.x] * rstd;
-      p.sums[n * g.C + ch] = make_float2(static_cast<float>(s1), static_cast<float>(s2));
+    if (mine && sub == 0) {
+      v2 *= rstd;
+      p.sums[n * g.C + ch] = make_float2(static_cast<float>(v1), static_cast<float>(v2));
       const double w = p.weight ? load_weight(p.weight, p.weight_dtype, ch) : 1.0;
-      w1 += w * s1;
-      w2 += w * s2;
-    }
-    __syncthreads();
-  }
-  if (threadIdx.x < 32) {
-    w1 = warp_sum(sub == 0 ? w1 : 0.0);
-    w2 = warp_sum(sub == 0 ? w2 : 0.0);
-    const double m = static_cast<double>(g.P) * g.Cg;
-    if (threadIdx.x == 0) {
-      means[0] = static_cast<float>(rstd * (w1 / m));
-      means[1] = static_cast<float>(rstd * (rstd * (w2 / m)));
+      w1 += w * v1;
+      w2 += w * v2;
+      if (g.whole_batch) {  // one sample: its sums are the parameters' gradients
+        if (p.dweight) store_weight(p.dweight, p.weight_dtype, ch, static_cast<float>(v2));
+        if (p.dbias) store_weight(p.dbias, p.weight_dtype, ch, static_cast<float>(v1));
+      }
     }
   }
-  __syncthreads();
-  float* row = p.channel + n * kNormBackwardRows * g.C;
-  for (int c = grp * g.Cg + threadIdx.x; c < (grp + 1) * g.Cg; c += kNormThreads) {
-    const int64_t C = g.C;
-    row[c] = mean;
+  const double2 total = team_sum(w1, w2, team_threads, sm);
+  if (!real) return;
+  const float k1 = static_cast<float>(rstd * (total.x * g.inv_m));
+  const float k2 = static_cast<float>(rstd * (rstd * (total.y * g.inv_m)));
+  const int64_t C = g.C;
+  float* row = p.channel + n * kNormBackwardRows * C;
+  for (int c = grp * g.Cg + lane; c < (grp + 1) * g.Cg; c += team_threads) {
+    row[c] = -mean;
     row[C + c] = p.weight ? rstd * load_weight(p.weight, p.weight_dtype, c) : rstd;
     row[2 * C + c] = p.bias ? load_weight(p.bias, p.weight_dtype, c) : 0.f;
-    row[3 * C + c] = means[0];
-    row[4 * C + c] = means[1];
+    row[3 * C + c] = -k1;
+    row[4 * C + c] = -k2;
   }
 }
 
-// ---- backward: dweight and dbias, sums over the samples in their order ----
+// ---- backward: dweight and dbias, sums over the samples: a warp for each channel ----
 __global__ void __launch_bounds__(kNormThreads) norm_param_grad_kernel(const __grid_constant__ NormParams p) {
   grid_dependency_wait();
   grid_launch_dependents();
-  const int c = blockIdx.x * kNormThreads + threadIdx.x;
+  const int c = blockIdx.x * kNormWarps + threadIdx.x / 32;
   if (c >= p.g.C) return;
   double db = 0.0, dw = 0.0;
-  for (int64_t n = 0; n < p.g.N; ++n) {
+#pragma unroll 4
+  for (int64_t n = threadIdx.x % 32; n < p.g.N; n += 32) {
     const float2 v = p.sums[n * p.g.C + c];
     db += v.x;
     dw += v.y;
   }
-  if (p.dweight) store_weight(p.dweight, p.weight_dtype, c, static_cast<float>(dw));
-  if (p.dbias) store_weight(p.dbias, p.weight_dtype, c, static_cast<float>(db));
+  db = warp_sum(db);
+  dw = warp_sum(dw);
+  if (threadIdx.x % 32 == 0) {
+    if (p.dweight) store_weight(p.dweight, p.weight_dtype, c, static_cast<float>(dw));
+    if (p.dbias) store_weight(p.dbias, p.weight_dtype, c, static_cast<float>(db));
+  }
 }
 
 // ---- backward: dx ----
 template <typename T, int V, int ACT, int U>
-__global__ void __launch_bounds__(kNormThreads) norm_grad_apply_kernel(const __grid_constant__ NormParams p) {
+__global__ void __launch_bounds__(kNormThreads, kNormResident) norm_grad_apply_kernel(const __grid_constant__ NormParams p) {
   const NormGeometry& g = p.g;
   const NormTile t(g, V);
   using IO = VecIO<T, V>;
@@ -637,11 +761,12 @@ __global__ void __launch_bounds__(kNormThreads) norm_grad_apply_kernel(const __g
   };
   if (steps.more()) fetch();
   grid_dependency_wait();
-  float mean[V], a[V], b[V], k1[V], k2[V];
+  constexpr int N = IO::N;
+  float2 minus[N], a[N], b[N], k1[N], k2[N];  // -mean, factor, shift, and the two means negated
   if (t.active) {
     const int64_t C = g.C;
     const float* row = p.channel + t.n * kNormBackwardRows * C + t.c0 + t.chan;
-    load_channels<V>(row, mean);
+    load_channels<V>(row, minus);
     load_channels<V>(row + C, a);
     load_channels<V>(row + 2 * C, b);
     load_channels<V>(row + 3 * C, k1);
@@ -649,14 +774,14 @@ __global__ void __launch_bounds__(kNormThreads) norm_grad_apply_kernel(const __g
   }
   grid_launch_dependents();  // the means have been read
   auto emit = [&](const typename IO::Raw& ra, const typename IO::Raw& rb, int64_t at) {
-    float f[V], d[V];
+    float2 f[N], d[N];
     IO::unpack(ra, f);
     IO::unpack(rb, d);
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const float xc = f[v] - mean[v];
-      const float dz = activate_grad<T, ACT>(fmaf(xc, a[v], b[v]), d[v]);
-      f[v] = fmaf(-xc, k2[v], fmaf(a[v], dz, -k1[v]));
+    for (int v = 0; v < N; ++v) {
+      const float2 xc = add2(f[v], minus[v]);
+      const float2 dz = activate_grad<T, ACT>(fma2(xc, a[v], b[v]), d[v]);
+      f[v] = fma2(xc, k2[v], fma2(a[v], dz, k1[v]));
     }
     IO::store(dx + at * g.C, IO::pack(f));
   };
