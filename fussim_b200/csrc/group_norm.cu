@@ -2,6 +2,7 @@
 // the work, and the launches. The kernels are in group_norm.cuh.
 #include "group_norm.cuh"
 
+#include <atomic>
 #include <climits>
 #include <cstdint>
 #include <exception>
@@ -25,6 +26,10 @@ constexpr int64_t kWave = 148 * fssim::kNormResident;
 constexpr int64_t kMinSteps = 4;
 // Bytes of input that the reducing pass may leave for the applying pass to find in L2.
 constexpr int64_t kResidentBytes = int64_t{80} << 20;
+
+// Vectors of a thread's batch: in the backward a batch has two tensors'.
+constexpr int kForwardU = 4;
+constexpr int kBackwardU = 2;
 
 size_t elem_size(int dtype) { return dtype == FSSIM_F32 ? 4 : 2; }
 bool known_dtype(int d) { return d == FSSIM_F32 || d == FSSIM_F16 || d == FSSIM_BF16; }
@@ -81,10 +86,12 @@ int64_t samples_per_launch(int64_t N, int64_t bytes_per_sample) {
 }
 
 template <typename Kernel, typename... Extra>
-int launch(Kernel k, dim3 grid, const NormParams& p, cudaStream_t stream, const char* what, Extra... extra) {
+int launch(Kernel k, dim3 grid, size_t smem, const NormParams& p, cudaStream_t stream, const char* what,
+           Extra... extra) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(fssim::kNormThreads);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -97,6 +104,27 @@ int launch(Kernel k, dim3 grid, const NormParams& p, cudaStream_t stream, const 
     return fail(FSSIM_ERR_CUDA, std::string(what) + ": " + cudaGetErrorString(e));
   }
   return FSSIM_OK;
+}
+
+// Opts a pass in to its ring of shared memory, once for each kernel and device. `done` belongs to
+// one kernel instantiation.
+template <typename Kernel>
+int allow_ring(Kernel k, size_t smem, std::atomic<bool> (&done)[64]) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && (dev < 0 || dev >= 64)) return fail(FSSIM_ERR_CUDA, "device ordinal out of range");
+  if (e == cudaSuccess && !done[dev].load(std::memory_order_acquire)) {
+    e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    if (e == cudaSuccess) done[dev].store(true, std::memory_order_release);
+  }
+  return e == cudaSuccess ? FSSIM_OK : fail(FSSIM_ERR_CUDA, cudaGetErrorString(e));
+}
+
+template <auto K, size_t SMEM>
+int launch_pass(dim3 grid, const NormParams& p, cudaStream_t stream, const char* what) {
+  static std::atomic<bool> done[64];
+  const int st = allow_ring(K, SMEM, done);
+  return st ? st : launch(K, grid, SMEM, p, stream, what);
 }
 
 dim3 tile_grid(const NormGeometry& g) {
@@ -117,6 +145,7 @@ int check_common(int dtype, int weight_dtype, int activation, int64_t N, int64_t
   if (N > kMaxSamples) return fail(FSSIM_ERR_SHAPE, "N must be at most 2^30");
   if (N * G > INT_MAX) return fail(FSSIM_ERR_SHAPE, "N*groups must be < 2^31");
   if (static_cast<double>(N) * P * C > 1.0e18) return fail(FSSIM_ERR_SHAPE, "N*P*C overflows int64");
+  if (P > (int64_t{1} << 38)) return fail(FSSIM_ERR_SHAPE, "P must be at most 2^38");
   if (!(eps >= 0.f)) return fail(FSSIM_ERR_ARGUMENT, "eps must not be negative");
   return FSSIM_OK;
 }
@@ -171,27 +200,33 @@ dim3 team_grid(const NormGeometry& g, int team) {
 
 template <typename T, int V, int ACT>
 int forward_kernels(const NormParams& p, cudaStream_t s) {
-  int st = launch(fssim::norm_stats_kernel<T, V, 4>, tile_grid(p.g), p, s, "group norm statistics launch");
+  using Walk = fssim::NormWalk<T, V, kForwardU, false>;
+  constexpr size_t ring = Walk::kSlotBytes, scratch = Walk::kScratchBytes;
+  int st = launch_pass<fssim::norm_stats_kernel<T, V, kForwardU>, (ring > scratch ? ring : scratch)>(tile_grid(p.g), p, s,
+                                                                        "group norm statistics launch");
   if (st) return st;
   const int team = team_threads(p.g.S);
-  st = launch(fssim::norm_merge_kernel, team_grid(p.g, team), p, s, "group norm merge launch", team);
+  st = launch(fssim::norm_merge_kernel, team_grid(p.g, team), 0, p, s, "group norm merge launch", team);
   if (st) return st;
-  return launch(fssim::norm_apply_kernel<T, V, ACT, 4>, tile_grid(p.g), p, s, "group norm launch");
+  return launch_pass<fssim::norm_apply_kernel<T, V, ACT, kForwardU>, ring>(tile_grid(p.g), p, s,
+                                                                           "group norm launch");
 }
 
 template <typename T, int V, int ACT>
 int backward_kernels(const NormParams& p, cudaStream_t s) {
-  int st = launch(fssim::norm_grad_sums_kernel<T, V, ACT, 2>, tile_grid(p.g), p, s,
-                  "group norm gradient sums launch");
+  using Walk = fssim::NormWalk<T, V, kBackwardU, false>;
+  constexpr size_t ring = 2 * Walk::kSlotBytes, scratch = Walk::kScratchBytes;
+  int st = launch_pass<fssim::norm_grad_sums_kernel<T, V, ACT, kBackwardU>, (ring > scratch ? ring : scratch)>(
+      tile_grid(p.g), p, s, "group norm gradient sums launch");
   if (st) return st;
   int cols = 1;
   while (cols < 32 && cols < p.g.Cg) cols *= 2;
   const int team = team_threads(static_cast<int64_t>(p.g.S) * cols);
-  st = launch(fssim::norm_grad_merge_kernel, team_grid(p.g, team), p, s,
+  st = launch(fssim::norm_grad_merge_kernel, team_grid(p.g, team), 0, p, s,
               "group norm gradient merge launch", team, cols);
   if (st || !p.out) return st;
-  return launch(fssim::norm_grad_apply_kernel<T, V, ACT, 2>, tile_grid(p.g), p, s,
-                "group norm gradient launch");
+  return launch_pass<fssim::norm_grad_apply_kernel<T, V, ACT, kBackwardU>, ring>(
+      tile_grid(p.g), p, s, "group norm gradient launch");
 }
 
 // One launch list per (element type, vector width, activation).
@@ -317,7 +352,7 @@ int backward_impl(const fssim_group_norm_backward_args* a, cudaStream_t stream) 
   p.g.N = a->N;
   p.sums = reinterpret_cast<float2*>(ws + plan.partial);
   const unsigned blocks = static_cast<unsigned>((a->C + fssim::kNormWarps - 1) / fssim::kNormWarps);
-  return launch(fssim::norm_param_grad_kernel, dim3(blocks), p, stream,
+  return launch(fssim::norm_param_grad_kernel, dim3(blocks), 0, p, stream,
                 "group norm parameter gradient launch");
 }
 

@@ -314,37 +314,88 @@ struct NormColumns {
   }
 };
 
-// The pixels of a thread in the applying passes: from the end of its part to the beginning (what
-// the reducing pass read last is what L2 still holds), U at a time; the last step, at the
-// beginning of the part, may be short.
-template <int U>
-struct NormSteps {
-  int64_t at;      // first pixel of the current step
-  int64_t left;    // pixels still to do, the current step's among them
-  int rows;
+// The vectors of one thread in a pass: pixel `row` of its part and every `rows`-th after it, in
+// that order or (REVERSED) from the last to the first, in batches of U; the last batch may be
+// short. Vectors of 16 bytes are copied asynchronously into shared memory, kBatches - 1 batches
+// ahead of their use (each thread into slots of its own, so that no barrier is needed): what a
+// thread has in flight is bounded by shared memory instead of registers and does not pause
+// while it computes. Narrower vectors are loaded when they are used.
+constexpr int kNormBatches = 4;
 
-  __device__ __forceinline__ NormSteps(const NormGeometry& g, const NormTile& t) : rows(g.rows) {
-    const int64_t first = t.p0 + t.row;
-    left = t.active && first < t.p1 ? (t.p1 - first - 1) / rows + 1 : 0;
-    at = first + (left - U) * rows;
+template <typename T, int V, int U, bool REVERSED>
+struct NormWalk {
+  using IO = VecIO<T, V>;
+  using Raw = typename IO::Raw;
+  static constexpr bool kAsync = sizeof(Raw) == 16;
+  // scratch of the merge that follows in the reducing passes: four floats per thread and channel
+  static constexpr int kScratchBytes = 4 * kNormThreads * V * static_cast<int>(sizeof(float));
+  static constexpr int kSlotBytes = kAsync ? kNormThreads * 16 * U * kNormBatches : 0;
+
+  int count;       // vectors of this thread
+  int64_t first;   // element offset of the first one
+  int64_t stride;  // and from one to the next
+
+  __device__ __forceinline__ NormWalk(const NormGeometry& g, const NormTile& t) {
+    const int64_t px = t.p0 + t.row;
+    count = t.active && px < t.p1 ? static_cast<int>((t.p1 - px - 1) / g.rows) + 1 : 0;
+    stride = static_cast<int64_t>(g.rows) * g.C;
+    first = (static_cast<int64_t>(t.n) * g.P + px) * g.C + t.c0 + t.chan;
+    if (REVERSED) {
+      first += static_cast<int64_t>(count - 1) * stride;
+      stride = -stride;
+    }
   }
-  __device__ __forceinline__ bool more() const { return left > 0; }
-  // the short step lacks its first pixels
-  __device__ __forceinline__ bool has(int u) const { return left >= U || u >= U - left; }
-  __device__ __forceinline__ int64_t pixel(int u) const { return at + static_cast<int64_t>(u) * rows; }
-  __device__ __forceinline__ void next() {
-    at -= static_cast<int64_t>(U) * rows;
-    left -= U;
+  __device__ __forceinline__ int batches() const { return (count + U - 1) / U; }
+  __device__ __forceinline__ bool has(int batch, int u) const { return batch * U + u < count; }
+  __device__ __forceinline__ int64_t offset(int batch, int u) const { return first + static_cast<int64_t>(batch * U + u) * stride; }
+
+  __device__ __forceinline__ static unsigned slot(unsigned ring, int batch, int u) {
+    return ring + ((static_cast<unsigned>(batch) % kNormBatches * U + u) * kNormThreads + threadIdx.x) * 16;
+  }
+  // start copying a batch of x (into the ring of shared memory at `ring`)
+  __device__ __forceinline__ void start(const T* x, unsigned ring, int batch) const {
+    if constexpr (kAsync) {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (has(batch, u))
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(slot(ring, batch, u)),
+                       "l"(x + offset(batch, u)) : "memory");
+    }
+  }
+  __device__ __forceinline__ static void commit() {
+    if constexpr (kAsync) asm volatile("cp.async.commit_group;" ::: "memory");
+  }
+  // all but the newest kNormBatches - 1 groups have arrived
+  __device__ __forceinline__ static void wait() {
+    if constexpr (kAsync) asm volatile("cp.async.wait_group %0;" ::"n"(kNormBatches - 1) : "memory");
+  }
+  __device__ __forceinline__ Raw get(const T* x, unsigned ring, int batch, int u) const {
+    if constexpr (kAsync) {
+      Raw r;
+      asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                   : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
+                   : "r"(slot(ring, batch, u)) : "memory");
+      return r;
+    } else {
+      return IO::load(x + offset(batch, u));
+    }
   }
 };
+
+// A pass's shared memory: the ring, and in the reducing passes the merge's scratch after it is used.
+extern __shared__ __align__(16) unsigned char norm_ring[];
+__device__ __forceinline__ unsigned norm_ring_address() {
+  return static_cast<unsigned>(__cvta_generic_to_shared(norm_ring));
+}
 
 // ---- forward: statistics ----
 template <typename T, int V, int U>
 __global__ void __launch_bounds__(kNormThreads, kNormResident) norm_stats_kernel(const __grid_constant__ NormParams p) {
-  __shared__ float sm_mean[kNormThreads * V];
-  __shared__ float sm_m2[kNormThreads * V];
-  __shared__ float column[kNormThreads * V];
-  __shared__ float centre[kNormThreads * V];
+  // the ring's memory again, once every thread is done with it
+  float* sm_mean = reinterpret_cast<float*>(norm_ring);
+  float* sm_m2 = sm_mean + kNormThreads * V;
+  float* column = sm_m2 + kNormThreads * V;
+  float* centre = column + kNormThreads * V;
   const NormGeometry& g = p.g;
   const NormTile t(g, V);
   if (!p.early) grid_dependency_wait();
@@ -354,49 +405,59 @@ __global__ void __launch_bounds__(kNormThreads, kNormResident) norm_stats_kernel
   float2 mean[N], m2[N];
 #pragma unroll
   for (int v = 0; v < N; ++v) mean[v] = m2[v] = splat2(0.f);
+  const NormWalk<T, V, U, false> walk(g, t);
+  const T* x = static_cast<const T*>(p.x);
+  const unsigned ring = norm_ring_address();
+  const int batches = walk.batches();
+#pragma unroll
+  for (int j = 0; j < kNormBatches - 1; ++j) {
+    walk.start(x, ring, j);
+    walk.commit();
+  }
+  float count = 0.f;
+  // a batch of U pixels, or the last one of k (k < U) with the missing ones left out
+  auto take = [&](auto whole, int j, int k) {
+    constexpr bool kWhole = decltype(whole)::value;
+    float2 f[U][N];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      typename IO::Raw raw{};
+      if (kWhole || u < k) raw = walk.get(x, ring, j, u);
+      IO::unpack(raw, f[u]);
+    }
+    const float taken = kWhole ? U : k;
+    const float total = count + taken;
+    const float2 each = splat2(kWhole ? 1.f / U : 1.f / taken);
+    const float share = taken / total;   // weight of the new values in the mean
+    const float cross = count * share;   // and of the squared distance of the means
+#pragma unroll
+    for (int v = 0; v < N; ++v) {
+      float2 sum = f[0][v];
+#pragma unroll
+      for (int u = 1; u < U; ++u) sum = add2(sum, f[u][v]);
+      const float2 m = mul2(sum, each), minus = neg2(m);
+      float2 q = splat2(0.f);
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (kWhole || u < k) {
+          const float2 d = add2(f[u][v], minus);
+          q = fma2(d, d, q);
+        }
+      const float2 d = add2(m, neg2(mean[v]));
+      mean[v] = fma2(d, splat2(share), mean[v]);
+      m2[v] = add2(m2[v], fma2(mul2(d, d), splat2(cross), q));
+    }
+    count = total;
+  };
+  for (int j = 0; j < batches; ++j) {
+    walk.start(x, ring, j + kNormBatches - 1);
+    walk.commit();
+    walk.wait();
+    if (walk.has(j, U - 1)) take(std::true_type{}, j, U);
+    else take(std::false_type{}, j, walk.count - j * U);
+  }
+  __syncthreads();
   if (t.active) {
-    const T* x = static_cast<const T*>(p.x) + static_cast<int64_t>(t.n) * g.P * g.C + t.c0 + t.chan;
-    const int64_t step = static_cast<int64_t>(g.rows);
-    float count = 0.f;
-    int64_t px = t.p0 + t.row;
-    // U pixels, or the last k of them (k < U) with the missing ones left out
-    auto take = [&](auto whole, int k) {
-      constexpr bool kWhole = decltype(whole)::value;
-      typename IO::Raw raw[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (kWhole || u < k) raw[u] = IO::load(x + (px + u * step) * g.C);
-        else raw[u] = typename IO::Raw{};
-      }
-      float2 f[U][N];
-#pragma unroll
-      for (int u = 0; u < U; ++u) IO::unpack(raw[u], f[u]);
-      const float taken = kWhole ? U : k;
-      const float total = count + taken;
-      const float2 each = splat2(kWhole ? 1.f / U : 1.f / taken);
-      const float share = taken / total;   // weight of the new values in the mean
-      const float cross = count * share;   // and of the squared distance of the means
-#pragma unroll
-      for (int v = 0; v < N; ++v) {
-        float2 sum = f[0][v];
-#pragma unroll
-        for (int u = 1; u < U; ++u) sum = add2(sum, f[u][v]);
-        const float2 m = mul2(sum, each), minus = neg2(m);
-        float2 q = splat2(0.f);
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-          if (kWhole || u < k) {
-            const float2 d = add2(f[u][v], minus);
-            q = fma2(d, d, q);
-          }
-        const float2 d = add2(m, neg2(mean[v]));
-        mean[v] = fma2(d, splat2(share), mean[v]);
-        m2[v] = add2(m2[v], fma2(mul2(d, d), splat2(cross), q));
-      }
-      count = total;
-    };
-    for (; px + (U - 1) * step < t.p1; px += U * step) take(std::true_type{}, U);
-    if (px < t.p1) take(std::false_type{}, static_cast<int>((t.p1 - px - 1) / step) + 1);
     norm_put<V>(sm_mean + t.row * g.SC + t.chan, mean);
     norm_put<V>(sm_m2 + t.row * g.SC + t.chan, m2);
   }
@@ -512,19 +573,18 @@ __global__ void __launch_bounds__(kNormThreads, kNormResident) norm_apply_kernel
   const NormGeometry& g = p.g;
   const NormTile t(g, V);
   using IO = VecIO<T, V>;
-  const int64_t base = static_cast<int64_t>(t.n) * g.P * g.C + t.c0 + t.chan;
-  const T* x = static_cast<const T*>(p.x) + base;
-  T* y = static_cast<T*>(p.out) + base;
-  NormSteps<U> steps(g, t);
+  const NormWalk<T, V, U, true> walk(g, t);
+  const T* x = static_cast<const T*>(p.x);
+  T* y = static_cast<T*>(p.out);
+  const unsigned ring = norm_ring_address();
+  const int batches = walk.batches();
   // x was complete before the statistics' launch began its work, so the first reads need not
-  // wait for that launch to end
-  typename IO::Raw raw[U];
-  auto fetch = [&] {
+  // wait for the launches in between to end
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (steps.has(u)) raw[u] = IO::load(x + steps.pixel(u) * g.C);
-  };
-  if (steps.more()) fetch();
+  for (int j = 0; j < kNormBatches - 1; ++j) {
+    walk.start(x, ring, j);
+    walk.commit();
+  }
   grid_dependency_wait();
   constexpr int N = IO::N;
   float2 minus[N], a[N], b[N];  // -mean, the factor and the shift
@@ -535,37 +595,52 @@ __global__ void __launch_bounds__(kNormThreads, kNormResident) norm_apply_kernel
     load_channels<V>(row + 2 * static_cast<int64_t>(g.C), b);
   }
   grid_launch_dependents();  // the statistics have been read
-  auto emit = [&](const typename IO::Raw& r, int64_t at) {
-    float2 f[N];
-    IO::unpack(r, f);
-#pragma unroll
-    for (int v = 0; v < N; ++v) f[v] = activate<T, ACT>(fma2(add2(f[v], minus[v]), a[v], b[v]));
-    IO::store(y + at * g.C, IO::pack(f));
-  };
-  while (steps.more()) {
+  for (int j = 0; j < batches; ++j) {
+    walk.start(x, ring, j + kNormBatches - 1);
+    walk.commit();
+    walk.wait();
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (steps.has(u)) emit(raw[u], steps.pixel(u));
-    steps.next();
-    if (steps.more()) fetch();
+      if (walk.has(j, u)) {
+        float2 f[N];
+        IO::unpack(walk.get(x, ring, j, u), f);
+#pragma unroll
+        for (int v = 0; v < N; ++v) f[v] = activate<T, ACT>(fma2(add2(f[v], minus[v]), a[v], b[v]));
+        IO::store(y + walk.offset(j, u), IO::pack(f));
+      }
   }
 }
 
 // ---- backward: per-channel sums of one part ----
 template <typename T, int V, int ACT, int U>
 __global__ void __launch_bounds__(kNormThreads, kNormResident) norm_grad_sums_kernel(const __grid_constant__ NormParams p) {
-  __shared__ float sm1[kNormThreads * V];
-  __shared__ float sm2[kNormThreads * V];
-  __shared__ float column1[kNormThreads * V];
-  __shared__ float column2[kNormThreads * V];
+  float* sm1 = reinterpret_cast<float*>(norm_ring);
+  float* sm2 = sm1 + kNormThreads * V;
+  float* column1 = sm2 + kNormThreads * V;
+  float* column2 = column1 + kNormThreads * V;
   const NormGeometry& g = p.g;
   const NormTile t(g, V);
   if (!p.early) grid_dependency_wait();
   grid_launch_dependents();
   using IO = VecIO<T, V>;
+  using Walk = NormWalk<T, V, U, false>;
+  const Walk walk(g, t);
+  const T* x = static_cast<const T*>(p.x);
+  const T* dy = static_cast<const T*>(p.dy);
+  const unsigned ring = norm_ring_address(), ring_dy = ring + Walk::kSlotBytes;
+  const int batches = walk.batches();
+#pragma unroll
+  for (int j = 0; j < kNormBatches - 1; ++j) {
+    walk.start(x, ring, j);
+    walk.start(dy, ring_dy, j);
+    walk.commit();
+  }
+  constexpr int N = IO::N;
+  float2 s1[N], s2[N];
+#pragma unroll
+  for (int v = 0; v < N; ++v) s1[v] = s2[v] = splat2(0.f);
   if (t.active) {
-    constexpr int N = IO::N;
-    float2 minus[N], a[N], b[N], s1[N], s2[N];
+    float2 minus[N], a[N], b[N];
     const int first = t.c0 + t.chan;
     int grp = first / g.Cg, end = (grp + 1) * g.Cg;  // one division; the next channels follow
 #pragma unroll
@@ -586,41 +661,29 @@ __global__ void __launch_bounds__(kNormThreads, kNormResident) norm_grad_sums_ke
       (v & 1 ? a[v / 2].y : a[v / 2].x) = av;
       (v & 1 ? b[v / 2].y : b[v / 2].x) = bv;
     }
-#pragma unroll
-    for (int v = 0; v < N; ++v) s1[v] = s2[v] = splat2(0.f);
-    const int64_t base = static_cast<int64_t>(t.n) * g.P * g.C + t.c0 + t.chan;
-    const T* x = static_cast<const T*>(p.x) + base;
-    const T* dy = static_cast<const T*>(p.dy) + base;
-    const int64_t step = g.rows;
-    int64_t px = t.p0 + t.row;
-    auto take = [&](const typename IO::Raw& rx, const typename IO::Raw& rd) {
-      float2 f[N], d[N];
-      IO::unpack(rx, f);
-      IO::unpack(rd, d);
-#pragma unroll
-      for (int v = 0; v < N; ++v) {
-        const float2 xc = add2(f[v], minus[v]);
-        const float2 dz = activate_grad<T, ACT>(fma2(xc, a[v], b[v]), d[v]);
-        s1[v] = add2(s1[v], dz);
-        s2[v] = fma2(dz, xc, s2[v]);
-      }
-    };
-    auto step_of = [&](auto whole) {
-      constexpr bool kWhole = decltype(whole)::value;
-      typename IO::Raw rx[U], rd[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (kWhole || px + u * step < t.p1) {
-          rx[u] = IO::load(x + (px + u * step) * g.C);
-          rd[u] = IO::load(dy + (px + u * step) * g.C);
-        }
-      }
+    for (int j = 0; j < batches; ++j) {
+      walk.start(x, ring, j + kNormBatches - 1);
+      walk.start(dy, ring_dy, j + kNormBatches - 1);
+      walk.commit();
+      walk.wait();
 #pragma unroll
       for (int u = 0; u < U; ++u)
-        if (kWhole || px + u * step < t.p1) take(rx[u], rd[u]);
-    };
-    for (; px + (U - 1) * step < t.p1; px += U * step) step_of(std::true_type{});
-    if (px < t.p1) step_of(std::false_type{});
+        if (walk.has(j, u)) {
+          float2 f[N], d[N];
+          IO::unpack(walk.get(x, ring, j, u), f);
+          IO::unpack(walk.get(dy, ring_dy, j, u), d);
+#pragma unroll
+          for (int v = 0; v < N; ++v) {
+            const float2 xc = add2(f[v], minus[v]);
+            const float2 dz = activate_grad<T, ACT>(fma2(xc, a[v], b[v]), d[v]);
+            s1[v] = add2(s1[v], dz);
+            s2[v] = fma2(dz, xc, s2[v]);
+          }
+        }
+    }
+  }
+  __syncthreads();
+  if (t.active) {
     norm_put<V>(sm1 + t.row * g.SC + t.chan, s1);
     norm_put<V>(sm2 + t.row * g.SC + t.chan, s2);
   }
@@ -743,23 +806,20 @@ __global__ void __launch_bounds__(kNormThreads, kNormResident) norm_grad_apply_k
   const NormGeometry& g = p.g;
   const NormTile t(g, V);
   using IO = VecIO<T, V>;
-  const int64_t base = static_cast<int64_t>(t.n) * g.P * g.C + t.c0 + t.chan;
-  const T* x = static_cast<const T*>(p.x) + base;
-  const T* dy = static_cast<const T*>(p.dy) + base;
-  T* dx = static_cast<T*>(p.out) + base;
-  NormSteps<U> steps(g, t);
-  // as in the forward, the first reads do not wait for the launch before
-  typename IO::Raw rx[U], rd[U];
-  auto fetch = [&] {
+  using Walk = NormWalk<T, V, U, true>;
+  const Walk walk(g, t);
+  const T* x = static_cast<const T*>(p.x);
+  const T* dy = static_cast<const T*>(p.dy);
+  T* dx = static_cast<T*>(p.out);
+  const unsigned ring = norm_ring_address(), ring_dy = ring + Walk::kSlotBytes;
+  const int batches = walk.batches();
+  // as in the forward, the first reads do not wait for the launches before
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (steps.has(u)) {
-        rx[u] = IO::load(x + steps.pixel(u) * g.C);
-        rd[u] = IO::load(dy + steps.pixel(u) * g.C);
-      }
-    }
-  };
-  if (steps.more()) fetch();
+  for (int j = 0; j < kNormBatches - 1; ++j) {
+    walk.start(x, ring, j);
+    walk.start(dy, ring_dy, j);
+    walk.commit();
+  }
   grid_dependency_wait();
   constexpr int N = IO::N;
   float2 minus[N], a[N], b[N], k1[N], k2[N];  // -mean, factor, shift, and the two means negated
@@ -773,24 +833,25 @@ __global__ void __launch_bounds__(kNormThreads, kNormResident) norm_grad_apply_k
     load_channels<V>(row + 4 * C, k2);
   }
   grid_launch_dependents();  // the means have been read
-  auto emit = [&](const typename IO::Raw& ra, const typename IO::Raw& rb, int64_t at) {
-    float2 f[N], d[N];
-    IO::unpack(ra, f);
-    IO::unpack(rb, d);
-#pragma unroll
-    for (int v = 0; v < N; ++v) {
-      const float2 xc = add2(f[v], minus[v]);
-      const float2 dz = activate_grad<T, ACT>(fma2(xc, a[v], b[v]), d[v]);
-      f[v] = fma2(xc, k2[v], fma2(a[v], dz, k1[v]));
-    }
-    IO::store(dx + at * g.C, IO::pack(f));
-  };
-  while (steps.more()) {
+  for (int j = 0; j < batches; ++j) {
+    walk.start(x, ring, j + kNormBatches - 1);
+    walk.start(dy, ring_dy, j + kNormBatches - 1);
+    walk.commit();
+    walk.wait();
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (steps.has(u)) emit(rx[u], rd[u], steps.pixel(u));
-    steps.next();
-    if (steps.more()) fetch();
+      if (walk.has(j, u)) {
+        float2 f[N], d[N];
+        IO::unpack(walk.get(x, ring, j, u), f);
+        IO::unpack(walk.get(dy, ring_dy, j, u), d);
+#pragma unroll
+        for (int v = 0; v < N; ++v) {
+          const float2 xc = add2(f[v], minus[v]);
+          const float2 dz = activate_grad<T, ACT>(fma2(xc, a[v], b[v]), d[v]);
+          f[v] = fma2(xc, k2[v], fma2(a[v], dz, k1[v]));
+        }
+        IO::store(dx + walk.offset(j, u), IO::pack(f));
+      }
   }
 }
 
