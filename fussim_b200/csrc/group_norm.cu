@@ -22,14 +22,16 @@ constexpr int64_t kMaxChannels = int64_t{1} << 24;
 constexpr int64_t kMaxSamples = int64_t{1} << 30;
 // CTAs of one wave on 148 SMs.
 constexpr int64_t kWave = 148 * fssim::kNormResident;
-// A part has at least this many pixels for each thread, so that its set-up is paid for.
-constexpr int64_t kMinSteps = 4;
-// Bytes of input that the reducing pass may leave for the applying pass to find in L2.
-constexpr int64_t kResidentBytes = int64_t{80} << 20;
+// Bytes of input that are to stay in L2 from the reducing pass to the applying one, of larger
+// tensors (1x64x1080x1920 16-bit forward 152 us without, 143 with; flat from 64 to 120 MB).
+constexpr double kKeptBytes = 80 << 20;
 
-// Vectors of a thread's batch: in the backward a batch has two tensors'.
-constexpr int kForwardU = 4;
-constexpr int kBackwardU = 2;
+// Vectors of a thread's batch and batches of its ring: 64 KB of ring for a CTA in every pass. The
+// statistics merge once a batch, so theirs are long; a batch of the backward has two tensors'.
+constexpr int kStatsU = 8, kStatsB = 2;
+constexpr int kApplyU = 4, kApplyB = 4;
+constexpr int kGradU = 2, kGradB = 4;
+constexpr int64_t kApplySteps = 32, kApplyWaves = 6;
 
 size_t elem_size(int dtype) { return dtype == FSSIM_F32 ? 4 : 2; }
 bool known_dtype(int d) { return d == FSSIM_F32 || d == FSSIM_F16 || d == FSSIM_BF16; }
@@ -46,7 +48,7 @@ int vector_width(int64_t C, size_t esize, const void* a, const void* b, const vo
   return 1;
 }
 
-NormGeometry make_geometry(int64_t N, int64_t P, int64_t C, int64_t G, int V, float eps) {
+NormGeometry make_geometry(int64_t N, int64_t P, int64_t C, int64_t G, int V, int reduce_batch, float eps) {
   NormGeometry g{};
   g.N = N;
   g.P = P;
@@ -54,6 +56,7 @@ NormGeometry make_geometry(int64_t N, int64_t P, int64_t C, int64_t G, int V, fl
   g.G = static_cast<int>(G);
   g.Cg = static_cast<int>(C / G);
   g.eps = eps;
+  g.inv_m = 1.0 / (static_cast<double>(P) * static_cast<double>(g.Cg));
   const int64_t vectors = C / V;
   const int64_t slices = (vectors + fssim::kNormThreads - 1) / fssim::kNormThreads;
   g.lanes = static_cast<int>((vectors + slices - 1) / slices);
@@ -62,27 +65,36 @@ NormGeometry make_geometry(int64_t N, int64_t P, int64_t C, int64_t G, int V, fl
   g.rows = fssim::kNormThreads / g.lanes;
   g.GS = g.slices == 1 ? g.G : static_cast<int>((g.SC + g.Cg - 2) / g.Cg + 1);
   if (g.GS > g.G) g.GS = g.G;
-  // Parts: one wave of CTAs, or where the samples are more than that, enough that the last
-  // wave's idle SMs weigh little.
-  const int64_t tiles = N * g.slices;
-  int64_t S = tiles <= kWave ? kWave / tiles : (4 * kWave + tiles - 1) / tiles;
-  const int64_t by_work = P / (g.rows * kMinSteps);
-  if (S > by_work) S = by_work;
-  if (S < 1) S = 1;
-  g.S = static_cast<int>(S);
-  g.inv_m = 1.0 / (static_cast<double>(P) * static_cast<double>(g.Cg));
-  g.base = P / S;
-  g.extra = static_cast<int>(P % S);
+  // Parts of the reducing pass: one wave of CTAs, or where the samples are more than that, enough
+  // that the last wave's idle SMs weigh little; no more than there are tiles.
+  g.tile = static_cast<int64_t>(g.rows) * reduce_batch;
+  g.tiles = (P + g.tile - 1) / g.tile;
+  const int64_t each = N * g.slices;
+  const int64_t S = each <= kWave ? kWave / each : (4 * kWave + each - 1) / each;
+  g.S = static_cast<int>(S < g.tiles ? S : g.tiles);
   return g;
 }
 
-// Samples per launch: as many as leave their input in L2 between the two passes, in equal cuts.
-int64_t samples_per_launch(int64_t N, int64_t bytes_per_sample) {
-  int64_t k = bytes_per_sample > 0 ? kResidentBytes / bytes_per_sample : N;
-  if (k < 1) k = 1;
-  if (k >= N) return N;
-  const int64_t cuts = (N + k - 1) / k;
-  return (N + cuts - 1) / cuts;
+// The same for the applying pass: one wave of CTAs with equal parts, or for large tensors short
+// parts of kApplySteps pixels for each thread, which the SMs take in their order. On a B200
+// short parts are faster from about kApplyWaves waves of them (8x128x512^2 16-bit training
+// pass 676 against 729 us), one wave below (8x128x256^2: 183 against 187 us), where the last
+// wave's idle SMs weigh more than the order of the accesses.
+NormGeometry apply_geometry(NormGeometry g) {
+  const int64_t each = g.N * g.slices, most = (g.P + g.rows - 1) / g.rows;
+  const int64_t step = static_cast<int64_t>(g.rows) * kApplySteps;
+  int64_t S = (g.P + step - 1) / step;
+  if (S * each < kApplyWaves * kWave) S = each <= kWave ? kWave / each : (4 * kWave + each - 1) / each;
+  if (S > most) S = most;
+  g.S = static_cast<int>(S);
+  g.base = g.P / S;
+  g.extra = static_cast<int>(g.P % S);
+  return g;
+}
+
+// Share of a launch's input that stays in L2 from the reducing pass to the applying one.
+float kept_share(double bytes) {
+  return bytes <= kKeptBytes ? 1.f : static_cast<float>(kKeptBytes / bytes);
 }
 
 template <typename Kernel, typename... Extra>
@@ -120,15 +132,14 @@ int allow_ring(Kernel k, size_t smem, std::atomic<bool> (&done)[64]) {
   return e == cudaSuccess ? FSSIM_OK : fail(FSSIM_ERR_CUDA, cudaGetErrorString(e));
 }
 
+// A pass over the tiles of g.
 template <auto K, size_t SMEM>
-int launch_pass(dim3 grid, const NormParams& p, cudaStream_t stream, const char* what) {
+int launch_pass(const NormGeometry& g, const NormParams& p, cudaStream_t stream, const char* what) {
+  if (g.N * g.S > INT_MAX) return fail(FSSIM_ERR_SHAPE, "more than 2^31 tiles");
   static std::atomic<bool> done[64];
   const int st = allow_ring(K, SMEM, done);
-  return st ? st : launch(K, grid, SMEM, p, stream, what);
-}
-
-dim3 tile_grid(const NormGeometry& g) {
-  return dim3(static_cast<unsigned>(g.N * g.S), static_cast<unsigned>(g.slices));
+  if (st) return st;
+  return launch(K, dim3(static_cast<unsigned>(g.N * g.S), static_cast<unsigned>(g.slices)), SMEM, p, stream, what);
 }
 
 int check_common(int dtype, int weight_dtype, int activation, int64_t N, int64_t P, int64_t C,
@@ -152,8 +163,7 @@ int check_common(int dtype, int weight_dtype, int activation, int64_t N, int64_t
 
 struct ForwardPlan {
   int V;
-  int64_t cut;     // samples per launch
-  NormGeometry g;  // of a full cut
+  NormGeometry g;
   size_t partial, bytes;
 };
 
@@ -161,16 +171,14 @@ ForwardPlan plan_forward(const fssim_group_norm_forward_args& a) {
   ForwardPlan p{};
   const size_t E = elem_size(a.dtype);
   p.V = vector_width(a.C, E, a.x, a.y, nullptr);
-  p.cut = samples_per_launch(a.N, a.P * a.C * static_cast<int64_t>(E));
-  p.g = make_geometry(p.cut, a.P, a.C, a.groups, p.V, a.eps);
-  p.partial = round256(sizeof(float2) * static_cast<size_t>(p.cut) * p.g.S * p.g.slices * p.g.GS);
-  p.bytes = p.partial + sizeof(float) * fssim::kNormForwardRows * static_cast<size_t>(p.cut) * a.C;
+  p.g = make_geometry(a.N, a.P, a.C, a.groups, p.V, kStatsU, a.eps);
+  p.partial = round256(sizeof(float2) * static_cast<size_t>(a.N) * p.g.S * p.g.slices * p.g.GS);
+  p.bytes = p.partial + sizeof(float) * fssim::kNormForwardRows * static_cast<size_t>(a.N) * a.C;
   return p;
 }
 
 struct BackwardPlan {
   int V;
-  int64_t cut;
   NormGeometry g;
   size_t partial, sums, bytes;
 };
@@ -179,11 +187,10 @@ BackwardPlan plan_backward(const fssim_group_norm_backward_args& a) {
   BackwardPlan p{};
   const size_t E = elem_size(a.dtype);
   p.V = vector_width(a.C, E, a.x, a.dy, a.dx);
-  p.cut = samples_per_launch(a.N, 2 * a.P * a.C * static_cast<int64_t>(E));
-  p.g = make_geometry(p.cut, a.P, a.C, a.groups, p.V, 0.f);
-  p.partial = round256(sizeof(float2) * static_cast<size_t>(p.cut) * p.g.S * a.C);
+  p.g = make_geometry(a.N, a.P, a.C, a.groups, p.V, kGradU, 0.f);
+  p.partial = round256(sizeof(float2) * static_cast<size_t>(a.N) * p.g.S * a.C);
   p.sums = round256(sizeof(float2) * static_cast<size_t>(a.N) * a.C);
-  p.bytes = p.partial + p.sums + sizeof(float) * fssim::kNormBackwardRows * static_cast<size_t>(p.cut) * a.C;
+  p.bytes = p.partial + p.sums + sizeof(float) * fssim::kNormBackwardRows * static_cast<size_t>(a.N) * a.C;
   return p;
 }
 
@@ -200,24 +207,27 @@ dim3 team_grid(const NormGeometry& g, int team) {
 
 template <typename T, int V, int ACT>
 int forward_kernels(const NormParams& p, cudaStream_t s) {
-  using Walk = fssim::NormWalk<T, V, kForwardU, false>;
-  constexpr size_t ring = Walk::kSlotBytes, scratch = Walk::kScratchBytes;
-  int st = launch_pass<fssim::norm_stats_kernel<T, V, kForwardU>, (ring > scratch ? ring : scratch)>(tile_grid(p.g), p, s,
-                                                                        "group norm statistics launch");
+  using Stats = fssim::NormWalk<T, V, kStatsU, kStatsB, false>;
+  using Apply = fssim::NormWalk<T, V, kApplyU, kApplyB, true>;
+  constexpr size_t scratch = Stats::kScratchBytes, ring = Stats::kRingBytes;
+  int st = launch_pass<fssim::norm_stats_kernel<T, V, kStatsU, kStatsB>, (ring > scratch ? ring : scratch)>(
+      p.g, p, s, "group norm statistics launch");
   if (st) return st;
   const int team = team_threads(p.g.S);
   st = launch(fssim::norm_merge_kernel, team_grid(p.g, team), 0, p, s, "group norm merge launch", team);
   if (st) return st;
-  return launch_pass<fssim::norm_apply_kernel<T, V, ACT, kForwardU>, ring>(tile_grid(p.g), p, s,
-                                                                           "group norm launch");
+  NormParams q = p;
+  q.g = apply_geometry(p.g);
+  return launch_pass<fssim::norm_apply_kernel<T, V, ACT, kApplyU, kApplyB>, Apply::kRingBytes>(
+      q.g, q, s, "group norm launch");
 }
 
 template <typename T, int V, int ACT>
 int backward_kernels(const NormParams& p, cudaStream_t s) {
-  using Walk = fssim::NormWalk<T, V, kBackwardU, false>;
-  constexpr size_t ring = 2 * Walk::kSlotBytes, scratch = Walk::kScratchBytes;
-  int st = launch_pass<fssim::norm_grad_sums_kernel<T, V, ACT, kBackwardU>, (ring > scratch ? ring : scratch)>(
-      tile_grid(p.g), p, s, "group norm gradient sums launch");
+  using Walk = fssim::NormWalk<T, V, kGradU, kGradB, false>;
+  constexpr size_t scratch = Walk::kScratchBytes, ring = 2 * Walk::kRingBytes;
+  int st = launch_pass<fssim::norm_grad_sums_kernel<T, V, ACT, kGradU, kGradB>, (ring > scratch ? ring : scratch)>(
+      p.g, p, s, "group norm gradient sums launch");
   if (st) return st;
   int cols = 1;
   while (cols < 32 && cols < p.g.Cg) cols *= 2;
@@ -225,8 +235,10 @@ int backward_kernels(const NormParams& p, cudaStream_t s) {
   st = launch(fssim::norm_grad_merge_kernel, team_grid(p.g, team), 0, p, s,
               "group norm gradient merge launch", team, cols);
   if (st || !p.out) return st;
-  return launch_pass<fssim::norm_grad_apply_kernel<T, V, ACT, kBackwardU>, ring>(
-      tile_grid(p.g), p, s, "group norm gradient launch");
+  NormParams q = p;
+  q.g = apply_geometry(p.g);
+  return launch_pass<fssim::norm_grad_apply_kernel<T, V, ACT, kGradU, kGradB>, ring>(
+      q.g, q, s, "group norm gradient launch");
 }
 
 // One launch list per (element type, vector width, activation).
@@ -279,25 +291,19 @@ int forward_impl(const fssim_group_norm_forward_args* a, cudaStream_t stream) {
   if (!a->workspace || a->workspace_bytes < plan.bytes)
     return fail(FSSIM_ERR_WORKSPACE, "workspace smaller than fssim_group_norm_forward_workspace_bytes");
   if (!aligned(a->workspace, 16)) return fail(FSSIM_ERR_WORKSPACE, "workspace must be 16-byte aligned");
-  for (int64_t n = 0; n < a->N; n += plan.cut) {
-    NormParams p{};
-    p.g = plan.g;
-    p.g.N = a->N - n < plan.cut ? a->N - n : plan.cut;
-    const size_t at = static_cast<size_t>(n) * a->P * a->C * E;
-    p.x = static_cast<const char*>(a->x) + at;
-    p.out = static_cast<char*>(a->y) + at;
-    p.weight = a->weight;
-    p.bias = a->bias;
-    p.weight_dtype = a->weight_dtype;
-    p.mean = a->mean ? a->mean + n * a->groups : nullptr;
-    p.rstd = a->rstd ? a->rstd + n * a->groups : nullptr;
-    p.partial = static_cast<float2*>(a->workspace);
-    p.channel = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + plan.partial);
-    p.early = n > 0;
-    st = dispatch<Forward>(a->dtype, plan.V, a->activation, p, stream);
-    if (st) return st;
-  }
-  return FSSIM_OK;
+  NormParams p{};
+  p.g = plan.g;
+  p.g.keep = kept_share(static_cast<double>(a->N) * a->P * a->C * E);
+  p.x = a->x;
+  p.out = a->y;
+  p.weight = a->weight;
+  p.bias = a->bias;
+  p.weight_dtype = a->weight_dtype;
+  p.mean = a->mean;
+  p.rstd = a->rstd;
+  p.partial = static_cast<float2*>(a->workspace);
+  p.channel = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + plan.partial);
+  return dispatch<Forward>(a->dtype, plan.V, a->activation, p, stream);
 }
 
 int backward_impl(const fssim_group_norm_backward_args* a, cudaStream_t stream) {
@@ -326,31 +332,25 @@ int backward_impl(const fssim_group_norm_backward_args* a, cudaStream_t stream) 
   if (!aligned(a->workspace, 16)) return fail(FSSIM_ERR_WORKSPACE, "workspace must be 16-byte aligned");
   char* ws = static_cast<char*>(a->workspace);
   NormParams p{};
-  for (int64_t n = 0; n < a->N; n += plan.cut) {
-    p.g = plan.g;
-    p.g.N = a->N - n < plan.cut ? a->N - n : plan.cut;
-    const size_t at = static_cast<size_t>(n) * a->P * a->C * E;
-    p.x = static_cast<const char*>(a->x) + at;
-    p.dy = static_cast<const char*>(a->dy) + at;
-    p.out = a->dx ? static_cast<char*>(a->dx) + at : nullptr;
-    p.weight = a->weight;
-    p.bias = a->bias;
-    p.weight_dtype = a->weight_dtype;
-    p.mean = const_cast<float*>(a->mean) + n * a->groups;
-    p.rstd = const_cast<float*>(a->rstd) + n * a->groups;
-    p.partial = reinterpret_cast<float2*>(ws);
-    p.sums = reinterpret_cast<float2*>(ws + plan.partial) + n * a->C;
-    p.channel = reinterpret_cast<float*>(ws + plan.partial + plan.sums);
-    p.early = n > 0 && a->dx != nullptr;
-    p.g.whole_batch = a->N == 1;
-    p.dweight = a->dweight;
-    p.dbias = a->dbias;
-    st = dispatch<Backward>(a->dtype, plan.V, a->activation, p, stream);
-    if (st) return st;
-  }
-  if (a->N == 1 || (!a->dweight && !a->dbias)) return FSSIM_OK;
-  p.g.N = a->N;
+  p.g = plan.g;
+  p.g.keep = kept_share(2.0 * a->N * a->P * a->C * E);
+  p.x = a->x;
+  p.dy = a->dy;
+  p.out = a->dx;
+  p.weight = a->weight;
+  p.bias = a->bias;
+  p.weight_dtype = a->weight_dtype;
+  p.mean = const_cast<float*>(a->mean);
+  p.rstd = const_cast<float*>(a->rstd);
+  p.partial = reinterpret_cast<float2*>(ws);
   p.sums = reinterpret_cast<float2*>(ws + plan.partial);
+  p.channel = reinterpret_cast<float*>(ws + plan.partial + plan.sums);
+  p.dweight = a->dweight;
+  p.dbias = a->dbias;
+  st = dispatch<Backward>(a->dtype, plan.V, a->activation, p, stream);
+  if (st) return st;
+  // (one sample's sums are the parameters' gradients: the merge has written them)
+  if (a->N == 1 || (!a->dweight && !a->dbias)) return FSSIM_OK;
   const unsigned blocks = static_cast<unsigned>((a->C + fssim::kNormWarps - 1) / fssim::kNormWarps);
   return launch(fssim::norm_param_grad_kernel, dim3(blocks), 0, p, stream,
                 "group norm parameter gradient launch");

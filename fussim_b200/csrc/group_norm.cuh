@@ -8,14 +8,16 @@
 //   backward  dz = dy * act'(z);  db_c = sum dz;  dw_c = sum dz * xhat  (over n and pixels)
 //             dx = rstd * (w dz - <w dz> - xhat <w dz xhat>),  <> the mean over the group
 //
-// Work split: a sample's pixels are cut into S parts (equal to within one pixel) and its
-// channels into slices of at most 256 vectors of V channels. A CTA takes one (sample, part,
-// slice). A thread keeps one vector of channels for the whole part and steps over its pixels,
-// so the per-channel constants and sums stay in registers and a warp reads whole rows of
-// memory. The group's numbers must all be seen before its first output, so each direction is
-// a reducing pass, a small launch that merges the parts, and an applying pass; the second read
-// comes from L2 where the samples in flight fit it (the host cuts the batch accordingly), from
-// the end of each part backwards, because that is what the reducing pass read last.
+// Work split: the group's numbers must all be seen before its first output, so each direction is a
+// reducing pass, a small launch that merges its results, and an applying pass. The channels are
+// cut into slices of at most 256 vectors of V channels. A thread keeps one vector of channels and
+// steps over pixels, so the per-channel constants and sums stay in registers and a warp reads
+// whole rows of memory.
+//   Reducing: a sample's pixels are cut into tiles and dealt out in turn to S parts, one CTA
+//   each and one wave of CTAs in all: few results to merge, and the GPU reads memory as one
+//   moving window.
+//   Applying: S short contiguous parts, a CTA each, from the end of the samples to their
+//   beginning: what the reducing pass read last is what L2 still holds.
 //
 // Statistics: a thread takes U pixels at a time, forms each channel's mean and sum of squared
 // deviations of those U values (two passes over registers), and merges them into its running
@@ -37,7 +39,8 @@ namespace fssim {
 
 constexpr int kNormThreads = 256;
 constexpr int kNormWarps = kNormThreads / 32;
-constexpr int kNormResident = 3;  // CTAs of the passes on one SM
+constexpr int kNormResident = 2;       // CTAs of a reducing pass on one SM
+constexpr int kNormApplyResident = 2;  // and of an applying pass
 
 enum NormAct { kNormActNone = 0, kNormActSilu = 1, kNormActRelu = 2 };
 
@@ -52,13 +55,22 @@ struct NormGeometry {
   int S;       // parts of a sample's pixels
   int GS;      // most groups that touch one slice
   float eps;
+  float keep;        // share of the input that may stay in L2 from pass to pass
   double inv_m;      // 1 / (P * Cg)
-  int whole_batch;   // the call has one sample, this one
-  int64_t base;  // pixels of a part; the first `extra` parts have one more
+  // Reducing passes: part s has the tiles s, s + S, ... of `tile` pixels; the last of all `tiles`
+  // may be short.
+  int64_t tile, tiles;
+  // Applying passes: contiguous parts of `base` pixels; the first `extra` have one more.
+  int64_t base;
   int extra;
 
-  __device__ __forceinline__ int64_t part_pixels(int s) const { return base + (s < extra); }
-  __device__ __forceinline__ int64_t part_begin(int s) const { return base * s + min(s, extra); }
+  __device__ __forceinline__ int64_t part_tiles(int s) const { return tiles / S + (s < tiles % S); }
+  // the part that has the last tile, and the pixels that tile lacks
+  __device__ __forceinline__ int last_part() const { return static_cast<int>((tiles - 1) % S); }
+  __device__ __forceinline__ int64_t lacking() const { return tiles * tile - P; }
+  __device__ __forceinline__ int64_t part_pixels(int s) const {
+    return part_tiles(s) * tile - (s == last_part() ? lacking() : 0);
+  }
 };
 
 struct NormParams {
@@ -77,7 +89,6 @@ struct NormParams {
   float* channel;       // what the applying pass needs, C values each, per sample: the mean, the
                         // factor a = rstd w and the shift b (kNormForwardRows rows); in the
                         // backward also rstd <w dz> and rstd^2 <w dz xhat> (kNormBackwardRows)
-  int early;            // a reducing pass that need not wait for the launch before it to begin
   void* dweight;
   void* dbias;
 };
@@ -243,20 +254,23 @@ struct NormTile {
   int slice;
   int c0, c1;        // channels of the slice
   int g0, g1;        // groups that touch it
-  int64_t p0, p1;    // pixels of the part
-  int row, chan;     // this thread's first pixel (from p0) and first channel (from c0)
+  int row, chan;     // this thread's row, and its first channel (from c0)
   bool active;
 
-  __device__ __forceinline__ NormTile(const NormGeometry& g, int V) {
-    n = blockIdx.x / g.S;
-    s = blockIdx.x - n * g.S;
+  __device__ __forceinline__ NormTile(const NormGeometry& g, int V, bool applying) {
+    if (applying) {
+      s = blockIdx.x / static_cast<unsigned>(g.N);
+      n = blockIdx.x - s * static_cast<unsigned>(g.N);
+      s = g.S - 1 - s;
+    } else {
+      n = blockIdx.x / static_cast<unsigned>(g.S);
+      s = blockIdx.x - n * g.S;
+    }
     slice = blockIdx.y;
     c0 = slice * g.SC;
     c1 = min(c0 + g.SC, g.C);
     g0 = c0 / g.Cg;
     g1 = (c1 - 1) / g.Cg + 1;
-    p0 = g.part_begin(s);
-    p1 = p0 + g.part_pixels(s);
     row = threadIdx.x / g.lanes;
     chan = (threadIdx.x - row * g.lanes) * V;
     active = row < g.rows && c0 + chan < c1;
@@ -314,82 +328,147 @@ struct NormColumns {
   }
 };
 
-// The vectors of one thread in a pass: pixel `row` of its part and every `rows`-th after it, in
-// that order or (REVERSED) from the last to the first, in batches of U; the last batch may be
-// short. Vectors of 16 bytes are copied asynchronously into shared memory, kBatches - 1 batches
-// ahead of their use (each thread into slots of its own, so that no barrier is needed): what a
-// thread has in flight is bounded by shared memory instead of registers and does not pause
-// while it computes. Narrower vectors are loaded when they are used.
-constexpr int kNormBatches = 4;
+// The vectors of one thread in a pass: its row's pixels of the part, in batches of U; the last batch
+// may be short. A reducing pass goes from tile to tile (a batch of each, `rows` pixels apart), an
+// applying one from the part's last pixel to its first. Vectors of 16 bytes are copied
+// asynchronously into a ring of B batches in shared memory, B - 1 batches ahead of their use
+// (each thread into slots of its own, so that no barrier is needed): what a thread has in flight
+// is bounded by shared memory instead of registers and does not pause while it computes.
+// Narrower vectors are loaded when they are used.
+// L2 priorities, for tensors that are larger than it (keep < 1): of what the reducing pass reads,
+// the last `keep` is to stay for the applying pass, which reads it first; all else, and what is
+// written, goes past it.
+struct NormPolicy {
+  uint64_t stay, pass;
+  __device__ __forceinline__ explicit NormPolicy(bool large) {
+    asm("createpolicy.fractional.L2::evict_normal.b64 %0;" : "=l"(stay));
+    asm("createpolicy.fractional.L2::evict_first.b64 %0;" : "=l"(pass));
+    if (!large) pass = stay;
+  }
+};
 
-template <typename T, int V, int U, bool REVERSED>
+template <typename T, int V, int U, int B, bool APPLYING>
 struct NormWalk {
   using IO = VecIO<T, V>;
   using Raw = typename IO::Raw;
   static constexpr bool kAsync = sizeof(Raw) == 16;
+  static constexpr int kU = U;
   // scratch of the merge that follows in the reducing passes: four floats per thread and channel
   static constexpr int kScratchBytes = 4 * kNormThreads * V * static_cast<int>(sizeof(float));
-  static constexpr int kSlotBytes = kAsync ? kNormThreads * 16 * U * kNormBatches : 0;
+  static constexpr int kRingBytes = kAsync ? kNormThreads * 16 * U * B : 0;
 
   int count;       // vectors of this thread
   int64_t first;   // element offset of the first one
-  int64_t stride;  // and from one to the next
+  int64_t stride;  // from one to the next in a batch
+  int64_t jump;    // and besides that from batch to batch
 
   __device__ __forceinline__ NormWalk(const NormGeometry& g, const NormTile& t) {
-    const int64_t px = t.p0 + t.row;
-    count = t.active && px < t.p1 ? static_cast<int>((t.p1 - px - 1) / g.rows) + 1 : 0;
     stride = static_cast<int64_t>(g.rows) * g.C;
-    first = (static_cast<int64_t>(t.n) * g.P + px) * g.C + t.c0 + t.chan;
-    if (REVERSED) {
-      first += static_cast<int64_t>(count - 1) * stride;
+    int64_t px;
+    if (APPLYING) {
+      const int64_t pixels = g.base + (t.s < g.extra);
+      count = t.row < pixels ? static_cast<int>((pixels - t.row - 1) / g.rows) + 1 : 0;
+      px = g.base * t.s + min(t.s, g.extra) + t.row + static_cast<int64_t>(count - 1) * g.rows;
       stride = -stride;
+      jump = 0;
+    } else {
+      const int missing = t.s == g.last_part() ? static_cast<int>(g.lacking()) : 0;
+      // pixels of a full tile that this row lacks in the last one
+      const int last = static_cast<int>(g.tile) - missing;
+      const int lost = missing == 0 ? 0 : U - (t.row < last ? (last - t.row - 1) / g.rows + 1 : 0);
+      count = static_cast<int>(g.part_tiles(t.s)) * U - lost;
+      px = t.s * g.tile + t.row;
+      jump = (g.S - 1) * g.tile * g.C;
     }
+    if (!t.active) count = 0;
+    first = (t.n * g.P + px) * g.C + t.c0 + t.chan;
   }
-  __device__ __forceinline__ int batches() const { return (count + U - 1) / U; }
-  __device__ __forceinline__ bool has(int batch, int u) const { return batch * U + u < count; }
-  __device__ __forceinline__ int64_t offset(int batch, int u) const { return first + static_cast<int64_t>(batch * U + u) * stride; }
+  // pixels of the reducing pass that come before those that are to stay in L2
+  __device__ __forceinline__ int passing(float keep) const {
+    return keep >= 1.f ? 0 : static_cast<int>(static_cast<float>(count) * (1.f - keep));
+  }
 
-  __device__ __forceinline__ static unsigned slot(unsigned ring, int batch, int u) {
-    return ring + ((static_cast<unsigned>(batch) % kNormBatches * U + u) * kNormThreads + threadIdx.x) * 16;
-  }
-  // start copying a batch of x (into the ring of shared memory at `ring`)
-  __device__ __forceinline__ void start(const T* x, unsigned ring, int batch) const {
-    if constexpr (kAsync) {
+  // start(slot, todo) begins copying the next batch, of which `todo` vectors are left, into that
+  // batch of the ring; use(slot, whole, k) takes one of k vectors (k == U when whole).
+  template <typename Start, typename Use>
+  __device__ __forceinline__ void run(int prefilled, Start start, Use use) const {
+    int todo = count - prefilled * U, left = count;
+    while (left > 0) {
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (has(batch, u))
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(slot(ring, batch, u)),
-                       "l"(x + offset(batch, u)) : "memory");
+      for (int b = 0; b < B; ++b) {
+        start((b + B - 1) % B, todo);
+        todo -= U;
+        if constexpr (kAsync) asm volatile("cp.async.wait_group %0;" ::"n"(B - 1) : "memory");
+        if (left >= U) use(b, std::true_type{}, U);
+        else use(b, std::false_type{}, left);
+        left -= U;
+        if (left <= 0) break;
+      }
     }
   }
-  __device__ __forceinline__ static void commit() {
-    if constexpr (kAsync) asm volatile("cp.async.commit_group;" ::: "memory");
+};
+
+// One tensor's side of a walk: where its next vector to copy lies, and its ring.
+template <typename W, typename T>
+struct NormSource {
+  const T* next;   // to copy (or, for narrow vectors, to load)
+  unsigned ring;
+
+  __device__ __forceinline__ NormSource(const W& w, const void* x, int offset)
+      : next(static_cast<const T*>(x) + w.first), ring(address() + offset + threadIdx.x * 16) {}
+  static __device__ __forceinline__ unsigned address() {
+    extern __shared__ __align__(16) unsigned char norm_ring[];
+    return static_cast<unsigned>(__cvta_generic_to_shared(norm_ring));
   }
-  // all but the newest kNormBatches - 1 groups have arrived
-  __device__ __forceinline__ static void wait() {
-    if constexpr (kAsync) asm volatile("cp.async.wait_group %0;" ::"n"(kNormBatches - 1) : "memory");
+  __device__ __forceinline__ void start(const W& w, int slot, int todo, uint64_t policy) {
+    if constexpr (W::kAsync) {
+#pragma unroll
+      for (int u = 0; u < W::kU; ++u) {
+        if (u < todo)
+          asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2;" ::"r"(
+                           ring + (slot * W::kU + u) * kNormThreads * 16),
+                       "l"(next), "l"(policy) : "memory");
+        next += w.stride;
+      }
+      next += w.jump;
+    }
   }
-  __device__ __forceinline__ Raw get(const T* x, unsigned ring, int batch, int u) const {
-    if constexpr (kAsync) {
-      Raw r;
+  static __device__ __forceinline__ void commit() {
+    if constexpr (W::kAsync) asm volatile("cp.async.commit_group;" ::: "memory");
+  }
+  // vector u of a batch that has arrived; each is taken once, in order
+  __device__ __forceinline__ typename W::Raw get(const W& w, int slot, int u) {
+    if constexpr (W::kAsync) {
+      typename W::Raw r;
       asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
                    : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
-                   : "r"(slot(ring, batch, u)) : "memory");
+                   : "r"(ring + (slot * W::kU + u) * kNormThreads * 16) : "memory");
       return r;
     } else {
-      return IO::load(x + offset(batch, u));
+      const typename W::Raw r = W::IO::load(next);
+      next += u + 1 < W::kU ? w.stride : w.stride + w.jump;
+      return r;
     }
+  }
+};
+
+template <typename W, typename T>
+struct NormSink {
+  T* next;
+  __device__ __forceinline__ NormSink(const W& w, void* y) : next(static_cast<T*>(y) + w.first) {}
+  __device__ __forceinline__ void put(const W& w, const typename W::Raw& r, uint64_t policy) {
+    if constexpr (W::kAsync)
+      asm volatile("st.global.L2::cache_hint.v4.u32 [%0], {%1, %2, %3, %4}, %5;" ::"l"(next), "r"(r.x),
+                   "r"(r.y), "r"(r.z), "r"(r.w), "l"(policy) : "memory");
+    else W::IO::store(next, r);
+    next += w.stride;
   }
 };
 
 // A pass's shared memory: the ring, and in the reducing passes the merge's scratch after it is used.
 extern __shared__ __align__(16) unsigned char norm_ring[];
-__device__ __forceinline__ unsigned norm_ring_address() {
-  return static_cast<unsigned>(__cvta_generic_to_shared(norm_ring));
-}
-
 // ---- forward: statistics ----
-template <typename T, int V, int U>
+template <typename T, int V, int U, int B>
 __global__ void __launch_bounds__(kNormThreads, kNormResident) norm_stats_kernel(const __grid_constant__ NormParams p) {
   // the ring's memory again, once every thread is done with it
   float* sm_mean = reinterpret_cast<float*>(norm_ring);
@@ -397,39 +476,41 @@ __global__ void __launch_bounds__(kNormThreads, kNormResident) norm_stats_kernel
   float* column = sm_m2 + kNormThreads * V;
   float* centre = column + kNormThreads * V;
   const NormGeometry& g = p.g;
-  const NormTile t(g, V);
-  if (!p.early) grid_dependency_wait();
+  const NormTile t(g, V, false);
+  grid_dependency_wait();
   grid_launch_dependents();
   using IO = VecIO<T, V>;
   constexpr int N = IO::N;
   float2 mean[N], m2[N];
 #pragma unroll
   for (int v = 0; v < N; ++v) mean[v] = m2[v] = splat2(0.f);
-  const NormWalk<T, V, U, false> walk(g, t);
-  const T* x = static_cast<const T*>(p.x);
-  const unsigned ring = norm_ring_address();
-  const int batches = walk.batches();
+  using Walk = NormWalk<T, V, U, B, false>;
+  const Walk walk(g, t);
+  NormSource<Walk, T> x(walk, p.x, 0);
+  const NormPolicy policy(g.keep < 1.f);
+  const int staying = walk.count - walk.passing(g.keep);
+  const auto start = [&](int slot, int todo) {
+    x.start(walk, slot, todo, todo > staying ? policy.pass : policy.stay);
+    x.commit();
+  };
 #pragma unroll
-  for (int j = 0; j < kNormBatches - 1; ++j) {
-    walk.start(x, ring, j);
-    walk.commit();
-  }
-  float count = 0.f;
-  // a batch of U pixels, or the last one of k (k < U) with the missing ones left out
-  auto take = [&](auto whole, int j, int k) {
+  for (int b = 0; b < B - 1; ++b) start(b, walk.count - b * U);
+  float before = 0.f;  // batches taken
+  walk.run(B - 1, start, [&](int slot, auto whole, int k) {
+    // a batch of U pixels, or the last one of k (k < U) with the missing ones left out
     constexpr bool kWhole = decltype(whole)::value;
     float2 f[U][N];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       typename IO::Raw raw{};
-      if (kWhole || u < k) raw = walk.get(x, ring, j, u);
+      if (kWhole || u < k) raw = x.get(walk, slot, u);
       IO::unpack(raw, f[u]);
     }
+    // the new values' weight in the mean, and that of the squared distance of the two means
     const float taken = kWhole ? U : k;
-    const float total = count + taken;
+    const float share = kWhole ? __fdividef(1.f, before + 1.f) : taken / fmaf(before, U, taken);
+    const float cross = before * U * share;
     const float2 each = splat2(kWhole ? 1.f / U : 1.f / taken);
-    const float share = taken / total;   // weight of the new values in the mean
-    const float cross = count * share;   // and of the squared distance of the means
 #pragma unroll
     for (int v = 0; v < N; ++v) {
       float2 sum = f[0][v];
@@ -447,15 +528,8 @@ __global__ void __launch_bounds__(kNormThreads, kNormResident) norm_stats_kernel
       mean[v] = fma2(d, splat2(share), mean[v]);
       m2[v] = add2(m2[v], fma2(mul2(d, d), splat2(cross), q));
     }
-    count = total;
-  };
-  for (int j = 0; j < batches; ++j) {
-    walk.start(x, ring, j + kNormBatches - 1);
-    walk.commit();
-    walk.wait();
-    if (walk.has(j, U - 1)) take(std::true_type{}, j, U);
-    else take(std::false_type{}, j, walk.count - j * U);
-  }
+    before += 1.f;
+  });
   __syncthreads();
   if (t.active) {
     norm_put<V>(sm_mean + t.row * g.SC + t.chan, mean);
@@ -464,7 +538,7 @@ __global__ void __launch_bounds__(kNormThreads, kNormResident) norm_stats_kernel
   __syncthreads();
   // The rows' and channels' pairs become one pair per group: first the mean (as distances from
   // one of the means, so that equal values give that value exactly), then the deviations.
-  const int64_t pixels = t.p1 - t.p0;
+  const int64_t pixels = g.part_pixels(t.s);
   const int64_t full = pixels / g.rows;                        // pixels that every row took
   const int extra = static_cast<int>(pixels - full * g.rows);  // rows that took one more
   const int width = t.c1 - t.c0;
@@ -495,7 +569,6 @@ __global__ void __launch_bounds__(kNormThreads, kNormResident) norm_stats_kernel
   columns.sum_groups(g, t, column, [&](int i, int cb, int w, float sum) {
     partial[i] = make_float2(centre[i], sum);
   });
-  if (p.early) grid_dependency_wait();
 }
 
 // ---- the merging launches: a team of kNormThreads / teams threads for each (sample, group) ----
@@ -568,23 +641,24 @@ __global__ void __launch_bounds__(kNormThreads) norm_merge_kernel(const __grid_c
 }
 
 // ---- forward: y ----
-template <typename T, int V, int ACT, int U>
-__global__ void __launch_bounds__(kNormThreads, kNormResident) norm_apply_kernel(const __grid_constant__ NormParams p) {
+template <typename T, int V, int ACT, int U, int B>
+__global__ void __launch_bounds__(kNormThreads, kNormApplyResident) norm_apply_kernel(const __grid_constant__ NormParams p) {
   const NormGeometry& g = p.g;
-  const NormTile t(g, V);
+  const NormTile t(g, V, true);
   using IO = VecIO<T, V>;
-  const NormWalk<T, V, U, true> walk(g, t);
-  const T* x = static_cast<const T*>(p.x);
-  T* y = static_cast<T*>(p.out);
-  const unsigned ring = norm_ring_address();
-  const int batches = walk.batches();
+  using Walk = NormWalk<T, V, U, B, true>;
+  const Walk walk(g, t);
+  NormSource<Walk, T> x(walk, p.x, 0);
+  NormSink<Walk, T> y(walk, p.out);
+  const NormPolicy policy(g.keep < 1.f);
+  const auto start = [&](int slot, int todo) {
+    x.start(walk, slot, todo, policy.pass);
+    x.commit();
+  };
   // x was complete before the statistics' launch began its work, so the first reads need not
   // wait for the launches in between to end
 #pragma unroll
-  for (int j = 0; j < kNormBatches - 1; ++j) {
-    walk.start(x, ring, j);
-    walk.commit();
-  }
+  for (int j = 0; j < B - 1; ++j) start(j, walk.count - j * U);
   grid_dependency_wait();
   constexpr int N = IO::N;
   float2 minus[N], a[N], b[N];  // -mean, the factor and the shift
@@ -595,46 +669,45 @@ __global__ void __launch_bounds__(kNormThreads, kNormResident) norm_apply_kernel
     load_channels<V>(row + 2 * static_cast<int64_t>(g.C), b);
   }
   grid_launch_dependents();  // the statistics have been read
-  for (int j = 0; j < batches; ++j) {
-    walk.start(x, ring, j + kNormBatches - 1);
-    walk.commit();
-    walk.wait();
+  walk.run(B - 1, start, [&](int slot, auto whole, int k) {
+    constexpr bool kWhole = decltype(whole)::value;
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (walk.has(j, u)) {
+      if (kWhole || u < k) {
         float2 f[N];
-        IO::unpack(walk.get(x, ring, j, u), f);
+        IO::unpack(x.get(walk, slot, u), f);
 #pragma unroll
         for (int v = 0; v < N; ++v) f[v] = activate<T, ACT>(fma2(add2(f[v], minus[v]), a[v], b[v]));
-        IO::store(y + walk.offset(j, u), IO::pack(f));
+        y.put(walk, IO::pack(f), policy.pass);
       }
-  }
+  });
 }
 
 // ---- backward: per-channel sums of one part ----
-template <typename T, int V, int ACT, int U>
+template <typename T, int V, int ACT, int U, int B>
 __global__ void __launch_bounds__(kNormThreads, kNormResident) norm_grad_sums_kernel(const __grid_constant__ NormParams p) {
   float* sm1 = reinterpret_cast<float*>(norm_ring);
   float* sm2 = sm1 + kNormThreads * V;
   float* column1 = sm2 + kNormThreads * V;
   float* column2 = column1 + kNormThreads * V;
   const NormGeometry& g = p.g;
-  const NormTile t(g, V);
-  if (!p.early) grid_dependency_wait();
+  const NormTile t(g, V, false);
+  grid_dependency_wait();
   grid_launch_dependents();
   using IO = VecIO<T, V>;
-  using Walk = NormWalk<T, V, U, false>;
+  using Walk = NormWalk<T, V, U, B, false>;
   const Walk walk(g, t);
-  const T* x = static_cast<const T*>(p.x);
-  const T* dy = static_cast<const T*>(p.dy);
-  const unsigned ring = norm_ring_address(), ring_dy = ring + Walk::kSlotBytes;
-  const int batches = walk.batches();
+  NormSource<Walk, T> x(walk, p.x, 0), dy(walk, p.dy, Walk::kRingBytes);
+  const NormPolicy policy(g.keep < 1.f);
+  const int staying = walk.count - walk.passing(g.keep);
+  const auto start = [&](int slot, int todo) {
+    const uint64_t how = todo > staying ? policy.pass : policy.stay;
+    x.start(walk, slot, todo, how);
+    dy.start(walk, slot, todo, how);
+    x.commit();
+  };
 #pragma unroll
-  for (int j = 0; j < kNormBatches - 1; ++j) {
-    walk.start(x, ring, j);
-    walk.start(dy, ring_dy, j);
-    walk.commit();
-  }
+  for (int j = 0; j < B - 1; ++j) start(j, walk.count - j * U);
   constexpr int N = IO::N;
   float2 s1[N], s2[N];
 #pragma unroll
@@ -661,17 +734,14 @@ __global__ void __launch_bounds__(kNormThreads, kNormResident) norm_grad_sums_ke
       (v & 1 ? a[v / 2].y : a[v / 2].x) = av;
       (v & 1 ? b[v / 2].y : b[v / 2].x) = bv;
     }
-    for (int j = 0; j < batches; ++j) {
-      walk.start(x, ring, j + kNormBatches - 1);
-      walk.start(dy, ring_dy, j + kNormBatches - 1);
-      walk.commit();
-      walk.wait();
+    walk.run(B - 1, start, [&](int slot, auto whole, int k) {
+      constexpr bool kWhole = decltype(whole)::value;
 #pragma unroll
       for (int u = 0; u < U; ++u)
-        if (walk.has(j, u)) {
+        if (kWhole || u < k) {
           float2 f[N], d[N];
-          IO::unpack(walk.get(x, ring, j, u), f);
-          IO::unpack(walk.get(dy, ring_dy, j, u), d);
+          IO::unpack(x.get(walk, slot, u), f);
+          IO::unpack(dy.get(walk, slot, u), d);
 #pragma unroll
           for (int v = 0; v < N; ++v) {
             const float2 xc = add2(f[v], minus[v]);
@@ -680,7 +750,7 @@ __global__ void __launch_bounds__(kNormThreads, kNormResident) norm_grad_sums_ke
             s2[v] = fma2(dz, xc, s2[v]);
           }
         }
-    }
+    });
   }
   __syncthreads();
   if (t.active) {
@@ -702,7 +772,6 @@ __global__ void __launch_bounds__(kNormThreads, kNormResident) norm_grad_sums_ke
     }
     partial[c] = make_float2(v1, v2);
   }
-  if (p.early) grid_dependency_wait();
 }
 
 // Backward: sums over the parts, and the group's two means. `cols` (a power of two, at most 32)
@@ -758,7 +827,7 @@ __global__ void __launch_bounds__(kNormThreads) norm_grad_merge_kernel(const __g
       const double w = p.weight ? load_weight(p.weight, p.weight_dtype, ch) : 1.0;
       w1 += w * v1;
       w2 += w * v2;
-      if (g.whole_batch) {  // one sample: its sums are the parameters' gradients
+      if (g.N == 1) {  // one sample: its sums are the parameters' gradients
         if (p.dweight) store_weight(p.dweight, p.weight_dtype, ch, static_cast<float>(v2));
         if (p.dbias) store_weight(p.dbias, p.weight_dtype, ch, static_cast<float>(v1));
       }
@@ -801,25 +870,24 @@ __global__ void __launch_bounds__(kNormThreads) norm_param_grad_kernel(const __g
 }
 
 // ---- backward: dx ----
-template <typename T, int V, int ACT, int U>
-__global__ void __launch_bounds__(kNormThreads, kNormResident) norm_grad_apply_kernel(const __grid_constant__ NormParams p) {
+template <typename T, int V, int ACT, int U, int B>
+__global__ void __launch_bounds__(kNormThreads, kNormApplyResident) norm_grad_apply_kernel(const __grid_constant__ NormParams p) {
   const NormGeometry& g = p.g;
-  const NormTile t(g, V);
+  const NormTile t(g, V, true);
   using IO = VecIO<T, V>;
-  using Walk = NormWalk<T, V, U, true>;
+  using Walk = NormWalk<T, V, U, B, true>;
   const Walk walk(g, t);
-  const T* x = static_cast<const T*>(p.x);
-  const T* dy = static_cast<const T*>(p.dy);
-  T* dx = static_cast<T*>(p.out);
-  const unsigned ring = norm_ring_address(), ring_dy = ring + Walk::kSlotBytes;
-  const int batches = walk.batches();
+  NormSource<Walk, T> x(walk, p.x, 0), dy(walk, p.dy, Walk::kRingBytes);
+  NormSink<Walk, T> dx(walk, p.out);
+  const NormPolicy policy(g.keep < 1.f);
+  const auto start = [&](int slot, int todo) {
+    x.start(walk, slot, todo, policy.pass);
+    dy.start(walk, slot, todo, policy.pass);
+    x.commit();
+  };
   // as in the forward, the first reads do not wait for the launches before
 #pragma unroll
-  for (int j = 0; j < kNormBatches - 1; ++j) {
-    walk.start(x, ring, j);
-    walk.start(dy, ring_dy, j);
-    walk.commit();
-  }
+  for (int j = 0; j < B - 1; ++j) start(j, walk.count - j * U);
   grid_dependency_wait();
   constexpr int N = IO::N;
   float2 minus[N], a[N], b[N], k1[N], k2[N];  // -mean, factor, shift, and the two means negated
@@ -833,26 +901,23 @@ __global__ void __launch_bounds__(kNormThreads, kNormResident) norm_grad_apply_k
     load_channels<V>(row + 4 * C, k2);
   }
   grid_launch_dependents();  // the means have been read
-  for (int j = 0; j < batches; ++j) {
-    walk.start(x, ring, j + kNormBatches - 1);
-    walk.start(dy, ring_dy, j + kNormBatches - 1);
-    walk.commit();
-    walk.wait();
+  walk.run(B - 1, start, [&](int slot, auto whole, int k) {
+    constexpr bool kWhole = decltype(whole)::value;
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (walk.has(j, u)) {
+      if (kWhole || u < k) {
         float2 f[N], d[N];
-        IO::unpack(walk.get(x, ring, j, u), f);
-        IO::unpack(walk.get(dy, ring_dy, j, u), d);
+        IO::unpack(x.get(walk, slot, u), f);
+        IO::unpack(dy.get(walk, slot, u), d);
 #pragma unroll
         for (int v = 0; v < N; ++v) {
           const float2 xc = add2(f[v], minus[v]);
           const float2 dz = activate_grad<T, ACT>(fma2(xc, a[v], b[v]), d[v]);
           f[v] = fma2(xc, k2[v], fma2(a[v], dz, k1[v]));
         }
-        IO::store(dx + walk.offset(j, u), IO::pack(f));
+        dx.put(walk, IO::pack(f), policy.pass);
       }
-  }
+  });
 }
 
 }  // namespace fssim
