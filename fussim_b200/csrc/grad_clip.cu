@@ -2,6 +2,7 @@
 // tensors and the launches. The kernels are in grad_clip.cuh.
 #include "grad_clip.cuh"
 
+#include <atomic>
 #include <climits>
 #include <cstdint>
 #include <exception>
@@ -24,16 +25,19 @@ using fssim_host::NvtxRange;
 // a launch may carry).
 constexpr int kFew = 96;
 constexpr int kMany = 832;
+// Bytes of the gradients that are to stay in L2 from the norm to the clipping, of larger ones.
+constexpr double kKeptBytes = 80 << 20;
 static_assert(sizeof(ClipTable<kMany>) <= 32764, "kernel parameters are limited to 32764 bytes");
 
 size_t elem_size(int dtype) { return dtype == FSSIM_F32 ? 4 : 2; }
 bool known_dtype(int d) { return d == FSSIM_F32 || d == FSSIM_F16 || d == FSSIM_BF16; }
 
 template <typename... KA, typename... A>
-int launch(void (*k)(KA...), unsigned grid, cudaStream_t stream, const char* what, const A&... args) {
+int launch(void (*k)(KA...), unsigned grid, size_t smem, cudaStream_t stream, const char* what, const A&... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid);
   cfg.blockDim = dim3(kClipThreads);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -111,8 +115,26 @@ int check(const fssim_grad_clip_args* a, bool clip) {
   return FSSIM_OK;
 }
 
+// Opts the two passes in to their ring of shared memory, once for each device.
 template <int K>
-int launch_cut(const fssim_grad_clip_args& a, const Cut& c, bool clip, int partials, int first,
+int allow_ring() {
+  static std::atomic<bool> done[64];
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && (dev < 0 || dev >= 64)) return fail(FSSIM_ERR_CUDA, "device ordinal out of range");
+  if (e == cudaSuccess && !done[dev].load(std::memory_order_acquire)) {
+    e = cudaFuncSetAttribute(fssim::grad_squares_kernel<K>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             fssim::kClipRingBytes);
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(fssim::grad_clip_kernel<K>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               fssim::kClipRingBytes);
+    if (e == cudaSuccess) done[dev].store(true, std::memory_order_release);
+  }
+  return e == cudaSuccess ? FSSIM_OK : fail(FSSIM_ERR_CUDA, cudaGetErrorString(e));
+}
+
+template <int K>
+int launch_cut(const fssim_grad_clip_args& a, const Cut& c, bool clip, int partials, int first, float keep,
                cudaStream_t stream) {
   const std::unique_ptr<ClipTable<K>> t(new ClipTable<K>);
   int r = 0;
@@ -135,20 +157,26 @@ int launch_cut(const fssim_grad_clip_args& a, const Cut& c, bool clip, int parti
   t->first_partial = first;
   t->norm = clip && first == 0 ? a.norm : nullptr;
   t->max_norm = a.max_norm;
+  t->keep = keep;
   const unsigned grid = grid_for(c.units);
-  return clip ? launch(fssim::grad_clip_kernel<K>, grid, stream, "gradient clipping launch", *t)
-              : launch(fssim::grad_squares_kernel<K>, grid, stream, "gradient norm launch", *t);
+  const int st = allow_ring<K>();
+  if (st) return st;
+  return clip ? launch(fssim::grad_clip_kernel<K>, grid, fssim::kClipRingBytes, stream, "gradient clipping launch", *t)
+              : launch(fssim::grad_squares_kernel<K>, grid, fssim::kClipRingBytes, stream, "gradient norm launch", *t);
 }
 
 // One pass over all tensors: the partial sums (clip == false) or the scaling.
 int pass(const fssim_grad_clip_args& a, bool clip, int partials, cudaStream_t stream) {
+  double bytes = 0.0;
+  for (int64_t i = 0; i < a.count; ++i) bytes += static_cast<double>(a.sizes[i]) * elem_size(a.dtypes[i]);
+  const float keep = bytes <= kKeptBytes ? 1.f : static_cast<float>(kKeptBytes / bytes);
   int first = 0;
   for (int64_t i = 0; i < a.count;) {
     const Cut c = next_cut(a, i);
     i = c.end;
     if (c.runs == 0) continue;
-    const int st = c.runs <= kFew ? launch_cut<kFew>(a, c, clip, partials, first, stream)
-                                  : launch_cut<kMany>(a, c, clip, partials, first, stream);
+    const int st = c.runs <= kFew ? launch_cut<kFew>(a, c, clip, partials, first, keep, stream)
+                                  : launch_cut<kMany>(a, c, clip, partials, first, keep, stream);
     if (st) return st;
     first += static_cast<int>(grid_for(c.units));
   }
@@ -166,7 +194,7 @@ int run(const fssim_grad_clip_args* a, bool clip, cudaStream_t stream) {
   st = pass(*a, false, partials, stream);
   if (st) return st;
   if (clip) return pass(*a, true, partials, stream);
-  return launch(fssim::grad_norm_kernel, 1u, stream, "gradient norm sum launch",
+  return launch(fssim::grad_norm_kernel, 1u, 0, stream, "gradient norm sum launch",
                 static_cast<const double*>(a->workspace), partials, a->norm);
 }
 

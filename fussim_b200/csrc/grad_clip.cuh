@@ -9,8 +9,8 @@
 // over the grid in equal contiguous ranges, so every CTA streams the same number of bytes
 // whatever the tensors' sizes. A CTA finds its first run by bisection and walks on from there.
 //
-// Norm: squares are summed in FP32 over the eight numbers of one step of a thread and in FP64
-// from there on; a step whose FP32 sum leaves the range where squares are exact enough is
+// Norm: squares are summed in FP32 over the four or eight numbers of a 16-byte vector and in FP64
+// from there on; a vector whose FP32 sum leaves the range where squares are exact enough is
 // summed again in FP64, where the square of an FP32 number neither overflows nor vanishes. One
 // FP64 partial per CTA, summed in a fixed order by whoever needs the norm: results repeat bit
 // for bit, and the workspace needs no initial value.
@@ -27,7 +27,13 @@ namespace fssim {
 
 constexpr int kClipThreads = 256;
 constexpr int kClipUnit = 2048;     // numbers: eight for each thread
-constexpr int kClipMaxCtas = 148 * 8;
+constexpr int kClipResident = 3;    // CTAs on one SM
+constexpr int kClipMaxCtas = 148 * kClipResident;
+// Vectors are copied asynchronously into a ring of kClipRing batches of kClipBatch vectors for each
+// thread in shared memory (slots of its own: no barrier), ahead of their use.
+constexpr int kClipBatch = 4;
+constexpr int kClipRing = 4;
+constexpr int kClipRingBytes = kClipThreads * 16 * kClipBatch * kClipRing;
 
 // Runs of one launch. Two capacities: launches copy the whole table, and most models need few.
 template <int K>
@@ -44,73 +50,92 @@ struct ClipTable {
   int first_partial;      // of this launch's CTAs
   float* norm;            // written by the launch that has it set
   float max_norm;
+  float keep;             // share of the gradients that may stay in L2 from the norm to the clipping
 };
 
-// Eight consecutive numbers at a 16-byte boundary: as they lie in memory (16 or 32 bytes, so that
-// several such loads can be in flight before the first is converted), and as FP32.
-template <typename T> struct ClipVec;
-template <> struct ClipVec<float> {
-  struct Raw { float4 a, b; };
-  static __device__ __forceinline__ Raw load8(const float* p) {
-    return {reinterpret_cast<const float4*>(p)[0], reinterpret_cast<const float4*>(p)[1]};
-  }
-  static __device__ __forceinline__ void unpack(const Raw& r, float (&f)[8]) {
-    f[0] = r.a.x; f[1] = r.a.y; f[2] = r.a.z; f[3] = r.a.w;
-    f[4] = r.b.x; f[5] = r.b.y; f[6] = r.b.z; f[7] = r.b.w;
-  }
-  static __device__ __forceinline__ float one(const float* p) { return *p; }
-  static __device__ __forceinline__ void store8(float* p, const float* f) {
-    reinterpret_cast<float4*>(p)[0] = make_float4(f[0], f[1], f[2], f[3]);
-    reinterpret_cast<float4*>(p)[1] = make_float4(f[4], f[5], f[6], f[7]);
-  }
-  static __device__ __forceinline__ void put(float* p, float f) { *p = f; }
-};
-__device__ __forceinline__ float2 clip_widen(__half2 v) { return __half22float2(v); }
-__device__ __forceinline__ float2 clip_widen(__nv_bfloat162 v) { return __bfloat1622float2(v); }
-__device__ __forceinline__ void clip_narrow(__half2& v, float a, float b) { v = __floats2half2_rn(a, b); }
-__device__ __forceinline__ void clip_narrow(__nv_bfloat162& v, float a, float b) {
-  v = __floats2bfloat162_rn(a, b);
+// N consecutive numbers in one access of up to 16 bytes.
+template <int BYTES> struct ClipRaw;
+template <> struct ClipRaw<16> { using type = uint4; };
+template <> struct ClipRaw<8> { using type = uint2; };
+
+__device__ __forceinline__ float clip_widen(float v) { return v; }
+__device__ __forceinline__ float clip_widen(__half v) { return __half2float(v); }
+__device__ __forceinline__ float clip_widen(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T> __device__ __forceinline__ T clip_narrow(float v);
+template <> __device__ __forceinline__ float clip_narrow<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half clip_narrow<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 clip_narrow<__nv_bfloat16>(float v) {
+  return __float2bfloat16_rn(v);
 }
-__device__ __forceinline__ void clip_narrow(__half& v, float a) { v = __float2half_rn(a); }
-__device__ __forceinline__ void clip_narrow(__nv_bfloat16& v, float a) { v = __float2bfloat16_rn(a); }
-template <typename T, typename T2>
-struct ClipVec16 {
-  using Raw = uint4;
-  static __device__ __forceinline__ Raw load8(const T* p) { return *reinterpret_cast<const uint4*>(p); }
-  static __device__ __forceinline__ void unpack(const Raw& r, float (&f)[8]) {
-    const T2* h = reinterpret_cast<const T2*>(&r);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 t = clip_widen(h[i]);
-      f[2 * i] = t.x;
-      f[2 * i + 1] = t.y;
-    }
-  }
-  static __device__ __forceinline__ float one(const T* p) { return static_cast<float>(*p); }
-  static __device__ __forceinline__ void store8(T* p, const float* f) {
-    uint4 v;
-    T2* h = reinterpret_cast<T2*>(&v);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) clip_narrow(h[i], f[2 * i], f[2 * i + 1]);
-    *reinterpret_cast<uint4*>(p) = v;
-  }
-  static __device__ __forceinline__ void put(T* p, float f) { clip_narrow(*p, f); }
-};
-template <>
-struct ClipVec<__half> : ClipVec16<__half, __half2> {};
-template <>
-struct ClipVec<__nv_bfloat16> : ClipVec16<__nv_bfloat16, __nv_bfloat162> {};
 
-// Squares of eight numbers, added up. Between 2^-80 and 2^100 the FP32 sum is right to a few
-// of its roundings: no term overflowed, and what underflowed is below 2^-46 of the sum.
-__device__ __forceinline__ double sum_squares8(const float (&f)[8]) {
-  float a = fmaf(f[1], f[1], f[0] * f[0]), b = fmaf(f[3], f[3], f[2] * f[2]);
-  float c = fmaf(f[5], f[5], f[4] * f[4]), d = fmaf(f[7], f[7], f[6] * f[6]);
-  const float s = (a + b) + (c + d);
-  if (s < 0x1p-80f || s > 0x1p100f) {
-    double w = 0.0;
+template <typename T, int N>
+struct ClipVec {
+  using Raw = typename ClipRaw<sizeof(T) * N>::type;
+  static __device__ __forceinline__ void copy(unsigned slot, const T* p, uint64_t policy) {
+    if constexpr (sizeof(Raw) == 16)
+      asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2;" ::"r"(slot), "l"(p),
+                   "l"(policy) : "memory");
+    else
+      asm volatile("cp.async.ca.shared.global.L2::cache_hint [%0], [%1], 8, %2;" ::"r"(slot), "l"(p),
+                   "l"(policy) : "memory");
+  }
+  static __device__ __forceinline__ Raw take(unsigned slot) {
+    Raw r;
+    if constexpr (sizeof(Raw) == 16)
+      asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                   : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(slot) : "memory");
+    else
+      asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(r.x), "=r"(r.y) : "r"(slot) : "memory");
+    return r;
+  }
+  static __device__ __forceinline__ void unpack(const Raw& r, float (&f)[N]) {
+    const T* e = reinterpret_cast<const T*>(&r);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) w = fma(static_cast<double>(f[i]), static_cast<double>(f[i]), w);
+    for (int i = 0; i < N; ++i) f[i] = clip_widen(e[i]);
+  }
+  static __device__ __forceinline__ void store(T* p, const float (&f)[N], uint64_t policy) {
+    Raw r;
+    T* e = reinterpret_cast<T*>(&r);
+#pragma unroll
+    for (int i = 0; i < N; ++i) e[i] = clip_narrow<T>(f[i]);
+    if constexpr (sizeof(Raw) == 16)
+      asm volatile("st.global.L2::cache_hint.v4.u32 [%0], {%1, %2, %3, %4}, %5;" ::"l"(p), "r"(r.x),
+                   "r"(r.y), "r"(r.z), "r"(r.w), "l"(policy) : "memory");
+    else
+      asm volatile("st.global.L2::cache_hint.v2.u32 [%0], {%1, %2}, %3;" ::"l"(p), "r"(r.x), "r"(r.y),
+                   "l"(policy) : "memory");
+  }
+};
+
+// L2 priorities, for gradients that are larger than it (keep < 1): the last `keep` of what a CTA
+// reads for the norm is to stay for the clipping, which reads it first; all else, and what is
+// written, goes past it.
+struct ClipPolicy {
+  uint64_t stay, pass;
+  __device__ __forceinline__ explicit ClipPolicy(bool large) {
+    asm("createpolicy.fractional.L2::evict_normal.b64 %0;" : "=l"(stay));
+    asm("createpolicy.fractional.L2::evict_first.b64 %0;" : "=l"(pass));
+    if (!large) pass = stay;
+  }
+};
+
+// Squares of a vector's numbers, added up. Between 2^-80 and 2^100 the FP32 sum is right to a few
+// of its roundings: no term overflowed, and what underflowed is below 2^-46 of the sum.
+template <int N>
+__device__ __forceinline__ double sum_squares(const float (&f)[N]) {
+  float part[N / 2];
+#pragma unroll
+  for (int i = 0; i < N / 2; ++i) part[i] = fmaf(f[2 * i + 1], f[2 * i + 1], f[2 * i] * f[2 * i]);
+  float s = part[0] + part[1];
+  if (N == 8) s += part[2] + part[3];
+  if (s < 0x1p-80f || s > 0x1p100f) {
+    unsigned bits = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) bits |= __float_as_uint(f[i]) << 1;
+    double w = 0.0;
+    if (bits == 0) return w;  // all zero, as gradients of what was not seen are
+#pragma unroll
+    for (int i = 0; i < N; ++i) w = fma(static_cast<double>(f[i]), static_cast<double>(f[i]), w);
     return w;
   }
   return s;  // NaN too
@@ -121,13 +146,10 @@ __device__ __forceinline__ int64_t clip_range(int64_t units, int64_t b, int64_t 
   return units / grid * b + (units % grid) * b / grid;
 }
 
-// Calls f(run, first number, one past the last) for each piece of a run in this CTA's range,
-// from the last piece to the first when BACKWARDS.
+// Calls f(run, first number, one past the last) for each piece of a run in the units [u0, u1), from
+// the last piece to the first when BACKWARDS.
 template <bool BACKWARDS, int K, typename F>
-__device__ __forceinline__ void clip_walk(const ClipTable<K>& t, F f) {
-  const int64_t units = t.unit0[t.count];
-  const int64_t u0 = clip_range(units, blockIdx.x, gridDim.x);
-  const int64_t u1 = clip_range(units, blockIdx.x + 1, gridDim.x);
+__device__ __forceinline__ void clip_walk(const ClipTable<K>& t, int64_t u0, int64_t u1, F f) {
   if (u0 >= u1) return;
   const int64_t key = BACKWARDS ? u1 - 1 : u0;
   int lo = 0, hi = t.count - 1;  // the last run whose first unit is at most key
@@ -153,39 +175,65 @@ __device__ __forceinline__ int64_t clip_head(const T* p, int64_t b, int64_t e) {
   return min(head, e - b);
 }
 
-template <typename T>
-__device__ __forceinline__ double clip_piece_squares(const T* src, int64_t b, int64_t e) {
-  double acc = 0.0;
-  const int64_t head = clip_head(src, b, e);
-  const int64_t body = b + head;
-  const int64_t n8 = (e - body) / 8;
-  const int64_t tail = body + n8 * 8;
-  using IO = ClipVec<T>;
-  constexpr int U = 128 / sizeof(typename IO::Raw);  // 128 bytes of a thread in flight
-  int64_t i = threadIdx.x;
-  for (; i + (U - 1) * kClipThreads < n8; i += U * kClipThreads) {
-    typename IO::Raw raw[U];
+// use(vector, address) for the vectors of N numbers [0, n) of a piece at `src`, those of a thread
+// kClipThreads apart: from the first to the last, or from the last to the first.
+template <bool BACKWARDS, int N, typename T, typename Use>
+__device__ __forceinline__ void clip_vectors(const T* src, int64_t n, uint64_t policy, Use use) {
+  using IO = ClipVec<T, N>;
+  constexpr int U = kClipBatch, B = kClipRing;
+  extern __shared__ __align__(16) unsigned char clip_ring[];
+  const unsigned ring = static_cast<unsigned>(__cvta_generic_to_shared(clip_ring)) + threadIdx.x * 16;
+  const int64_t count = threadIdx.x < n ? (n - threadIdx.x - 1) / kClipThreads + 1 : 0;
+  const int64_t first = BACKWARDS ? threadIdx.x + (count - 1) * kClipThreads : threadIdx.x;
+  constexpr int64_t step = (BACKWARDS ? -1 : 1) * static_cast<int64_t>(kClipThreads);
+  const T* next = src + first * N;
+  int64_t todo = count, left = count, at = first;
+  const auto start = [&](int slot) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) raw[u] = IO::load8(src + body + (i + u * kClipThreads) * 8);
+    for (int u = 0; u < U; ++u)
+      if (u < todo) IO::copy(ring + (slot * U + u) * kClipThreads * 16, next + u * step * N, policy);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    next += U * step * N;
+    todo -= U;
+  };
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      float f[8];
-      IO::unpack(raw[u], f);
-      acc += sum_squares8(f);
+  for (int b = 0; b < B - 1; ++b) start(b);
+  while (left > 0) {
+#pragma unroll
+    for (int b = 0; b < B; ++b) {
+      start((b + B - 1) % B);
+      asm volatile("cp.async.wait_group %0;" ::"n"(B - 1) : "memory");
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (u < left) {
+          float f[N];
+          IO::unpack(IO::take(ring + (b * U + u) * kClipThreads * 16), f);
+          use(f, at + u * step);
+        }
+      left -= U;
+      at += U * step;
+      if (left <= 0) break;
     }
   }
-  for (; i < n8; i += kClipThreads) {
-    float f[8];
-    IO::unpack(IO::load8(src + body + i * 8), f);
-    acc += sum_squares8(f);
-  }
-  // what is left at the two ends: fewer than 8 numbers each
+}
+
+template <typename T>
+__device__ __noinline__ double clip_piece_squares(const T* src, int64_t b, int64_t e, uint64_t policy) {
+  constexpr int N = 16 / sizeof(T);
+  const int64_t head = clip_head(src, b, e);
+  const int64_t body = b + head;
+  const int64_t n = (e - body) / N;
+  const int64_t tail = body + n * N;
+  double acc = 0.0;
+  // what is left at the two ends: fewer than N numbers each
   const int64_t ends = head + (e - tail);
   if (threadIdx.x < ends) {
     const int64_t at = threadIdx.x < head ? b + threadIdx.x : tail + (threadIdx.x - head);
-    const double v = ClipVec<T>::one(src + at);
-    acc = fma(v, v, acc);
+    const double v = clip_widen(src[at]);
+    acc = v * v;
   }
+  clip_vectors<false, N>(src + body, n, policy,
+                         [&](const float (&f)[N], int64_t) { acc += sum_squares<N>(f); });
   return acc;
 }
 
@@ -199,39 +247,31 @@ struct ClipFactor {
 };
 
 template <typename S, typename D>
-__device__ __forceinline__ void clip_piece_scale(const S* src, D* dst, int64_t b, int64_t e, ClipFactor coef) {
+__device__ __noinline__ void clip_piece_scale(const S* src, D* dst, int64_t b, int64_t e, ClipFactor coef,
+                                                 uint64_t policy) {
+  // 16 bytes of the wider type, so that the lanes of a warp write one run of memory
+  constexpr int N = 16 / (sizeof(S) > sizeof(D) ? sizeof(S) : sizeof(D));
   const int64_t head = clip_head(src, b, e);
   const int64_t body = b + head;
   if (reinterpret_cast<uintptr_t>(dst + body) % 16 != 0) {
     // the two sides' boundaries differ: number by number, still in whole rows of a warp
+#pragma unroll 8
     for (int64_t i = b + threadIdx.x; i < e; i += kClipThreads)
-      ClipVec<D>::put(dst + i, coef * ClipVec<S>::one(src + i));
+      dst[i] = clip_narrow<D>(coef * clip_widen(src[i]));
     return;
   }
-  const int64_t n8 = (e - body) / 8;
-  const int64_t tail = body + n8 * 8;
-  using IO = ClipVec<S>;
-  constexpr int U = 64 / sizeof(typename IO::Raw);
-  const auto emit = [&](const typename IO::Raw& raw, int64_t at) {
-    float f[8];
-    IO::unpack(raw, f);
+  const int64_t n = (e - body) / N;
+  const int64_t tail = body + n * N;
+  clip_vectors<true, N>(src + body, n, policy, [&](const float (&f)[N], int64_t i) {
+    float r[N];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) f[k] = coef * f[k];
-    ClipVec<D>::store8(dst + body + at * 8, f);
-  };
-  int64_t i = threadIdx.x;
-  for (; i + (U - 1) * kClipThreads < n8; i += U * kClipThreads) {
-    typename IO::Raw raw[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) raw[u] = IO::load8(src + body + (i + u * kClipThreads) * 8);
-#pragma unroll
-    for (int u = 0; u < U; ++u) emit(raw[u], i + u * kClipThreads);
-  }
-  for (; i < n8; i += kClipThreads) emit(IO::load8(src + body + i * 8), i);
+    for (int k = 0; k < N; ++k) r[k] = coef * f[k];
+    ClipVec<D, N>::store(dst + body + i * N, r, policy);
+  });
   const int64_t ends = head + (e - tail);
   if (threadIdx.x < ends) {
     const int64_t at = threadIdx.x < head ? b + threadIdx.x : tail + (threadIdx.x - head);
-    ClipVec<D>::put(dst + at, coef * ClipVec<S>::one(src + at));
+    dst[at] = clip_narrow<D>(coef * clip_widen(src[at]));
   }
 }
 
@@ -249,15 +289,23 @@ __device__ __forceinline__ double clip_block_sum(double v) {
 }
 
 template <int K>
-__global__ void __launch_bounds__(kClipThreads) grad_squares_kernel(const __grid_constant__ ClipTable<K> t) {
+__global__ void __launch_bounds__(kClipThreads, kClipResident)
+    grad_squares_kernel(const __grid_constant__ ClipTable<K> t) {
   grid_dependency_wait();
   grid_launch_dependents();
+  const int64_t units = t.unit0[t.count];
+  const int64_t u0 = clip_range(units, blockIdx.x, gridDim.x), u1 = clip_range(units, blockIdx.x + 1, gridDim.x);
+  const ClipPolicy policies(t.keep < 1.f);
+  const int64_t split = u1 - static_cast<int64_t>(static_cast<float>(u1 - u0) * min(t.keep, 1.f));
   double acc = 0.0;
-  clip_walk<false>(t, [&](int r, int64_t b, int64_t e) {
-    if (t.src_dtype[r] == 0) acc += clip_piece_squares(static_cast<const float*>(t.src[r]), b, e);
-    else if (t.src_dtype[r] == 1) acc += clip_piece_squares(static_cast<const __half*>(t.src[r]), b, e);
-    else acc += clip_piece_squares(static_cast<const __nv_bfloat16*>(t.src[r]), b, e);
-  });
+  for (int part = 0; part < 2; ++part) {  // what goes past L2, then what stays
+    const uint64_t policy = part ? policies.stay : policies.pass;
+    clip_walk<false>(t, part ? split : u0, part ? u1 : split, [&](int r, int64_t b, int64_t e) {
+      if (t.src_dtype[r] == 0) acc += clip_piece_squares(static_cast<const float*>(t.src[r]), b, e, policy);
+      else if (t.src_dtype[r] == 1) acc += clip_piece_squares(static_cast<const __half*>(t.src[r]), b, e, policy);
+      else acc += clip_piece_squares(static_cast<const __nv_bfloat16*>(t.src[r]), b, e, policy);
+    });
+  }
   acc = clip_block_sum(acc);
   if (threadIdx.x == 0) t.partials[t.first_partial + blockIdx.x] = acc;
 }
@@ -278,26 +326,28 @@ __global__ void __launch_bounds__(kClipThreads) grad_norm_kernel(const double* p
 // The second read goes through the CTA's range from its end, which the norm's pass read last
 // and L2 still holds.
 template <int K>
-__global__ void __launch_bounds__(kClipThreads) grad_clip_kernel(const __grid_constant__ ClipTable<K> t) {
+__global__ void __launch_bounds__(kClipThreads, kClipResident)
+    grad_clip_kernel(const __grid_constant__ ClipTable<K> t) {
   grid_dependency_wait();
   grid_launch_dependents();
   const double norm = grad_norm_of(t.partials, t.num_partials);
   if (t.norm && blockIdx.x == 0 && threadIdx.x == 0) *t.norm = static_cast<float>(norm);
   const double ratio = static_cast<double>(t.max_norm) / (norm + 1e-6);
   const ClipFactor coef(ratio >= 1.0 ? 1.0 : ratio);  // a NaN norm gives NaN
-  clip_walk<true>(t, [&](int r, int64_t b, int64_t e) {
-    const int kind = t.src_dtype[r] * 3 + t.dst_dtype[r];
+  const uint64_t policy = ClipPolicy(t.keep < 1.f).pass;
+  const int64_t units = t.unit0[t.count];
+  clip_walk<true>(t, clip_range(units, blockIdx.x, gridDim.x), clip_range(units, blockIdx.x + 1, gridDim.x),
+                  [&](int r, int64_t b, int64_t e) {
     if (ratio >= 1.0 && t.src[r] == t.dst[r]) return;  // in place and below the limit: as it was
     const void* s = t.src[r];
     void* d = t.dst[r];
-    switch (kind) {
-      case 0: clip_piece_scale(static_cast<const float*>(s), static_cast<float*>(d), b, e, coef); break;
-      case 3: clip_piece_scale(static_cast<const __half*>(s), static_cast<float*>(d), b, e, coef); break;
-      case 4: clip_piece_scale(static_cast<const __half*>(s), static_cast<__half*>(d), b, e, coef); break;
-      case 6: clip_piece_scale(static_cast<const __nv_bfloat16*>(s), static_cast<float*>(d), b, e, coef); break;
-      case 8:
-        clip_piece_scale(static_cast<const __nv_bfloat16*>(s), static_cast<__nv_bfloat16*>(d), b, e, coef);
-        break;
+    const auto scale = [&](auto* src, auto* dst) { clip_piece_scale(src, dst, b, e, coef, policy); };
+    switch (t.src_dtype[r] * 3 + t.dst_dtype[r]) {
+      case 0: scale(static_cast<const float*>(s), static_cast<float*>(d)); break;
+      case 3: scale(static_cast<const __half*>(s), static_cast<float*>(d)); break;
+      case 4: scale(static_cast<const __half*>(s), static_cast<__half*>(d)); break;
+      case 6: scale(static_cast<const __nv_bfloat16*>(s), static_cast<float*>(d)); break;
+      case 8: scale(static_cast<const __nv_bfloat16*>(s), static_cast<__nv_bfloat16*>(d)); break;
       default: break;  // refused by the host
     }
   });
