@@ -6,6 +6,7 @@
 #include <climits>
 #include <cstdint>
 #include <exception>
+#include <numeric>
 #include <string>
 
 #include "engine_host.h"
@@ -31,6 +32,11 @@ constexpr double kKeptBytes = 80 << 20;
 constexpr int kStatsU = 8, kStatsB = 2;
 constexpr int kApplyU = 4, kApplyB = 4;
 constexpr int kGradU = 2, kGradB = 4;
+// The resident kernels: the largest tensors they take (x, in the backward x and dy), their slices'
+// bytes a pixel, and a CTA's shared memory.
+constexpr double kResidentBytes = 8 << 20;
+constexpr int64_t kSliceBytes = 64;
+constexpr size_t kResidentSmem = 200 << 10;
 constexpr int64_t kApplySteps = 32, kApplyWaves = 6;
 
 size_t elem_size(int dtype) { return dtype == FSSIM_F32 ? 4 : 2; }
@@ -92,24 +98,74 @@ NormGeometry apply_geometry(NormGeometry g) {
   return g;
 }
 
+// The resident kernels' split, where they take the call: slices of whole groups of at least
+// kSliceBytes a pixel, clusters large enough to spread the work, and parts that fit the shared
+// memory (`tensors` of them at a time). slots is 0 where they do not take it.
+struct ResidentPlan {
+  NormGeometry g;
+  int slots;    // vectors of a thread
+  size_t smem;
+};
+
+ResidentPlan plan_resident(int64_t N, int64_t P, int64_t C, int64_t G, int V, size_t esize, float eps, int tensors) {
+  ResidentPlan r{};
+  if (V * esize != 16 || static_cast<double>(N) * P * C * esize * tensors > kResidentBytes) return r;
+  const int64_t Cg = C / G;
+  const int64_t unit = std::lcm(static_cast<int64_t>(V), Cg);
+  int64_t SC = unit * ((kSliceBytes / static_cast<int64_t>(esize) + unit - 1) / unit);
+  if (SC > C) SC = C;
+  if (SC / V > fssim::kNormThreads) return r;
+  NormGeometry& g = r.g;
+  g.N = N;
+  g.P = P;
+  g.C = static_cast<int>(C);
+  g.G = static_cast<int>(G);
+  g.Cg = static_cast<int>(Cg);
+  g.eps = eps;
+  g.keep = 1.f;
+  g.inv_m = 1.0 / (static_cast<double>(P) * static_cast<double>(Cg));
+  g.SC = static_cast<int>(SC);
+  g.lanes = static_cast<int>(SC / V);
+  g.slices = static_cast<int>((C + SC - 1) / SC);
+  g.rows = fssim::kNormThreads / g.lanes;
+  g.GS = static_cast<int>(SC / Cg);
+  const int64_t units = N * g.slices;
+  const auto slots = [&](int K) { return ((P + K - 1) / K + g.rows - 1) / g.rows; };
+  const size_t scratch = sizeof(float) * fssim::kNormScratch * fssim::kNormThreads * V;
+  const int64_t most = static_cast<int64_t>((kResidentSmem - scratch) / (16 * fssim::kNormThreads * tensors));
+  int K = 1;
+  while (K < 8 && (slots(K) > most || (slots(K) > 2 && units * K * 2 <= kWave))) K *= 2;
+  if (slots(K) > most || units * K > INT_MAX) return r;
+  g.S = K;
+  g.base = P / K;
+  g.extra = static_cast<int>(P % K);
+  r.slots = static_cast<int>(slots(K));
+  r.smem = scratch + static_cast<size_t>(r.slots) * 16 * fssim::kNormThreads * tensors;
+  return r;
+}
+
 // Share of a launch's input that stays in L2 from the reducing pass to the applying one.
 float kept_share(double bytes) {
   return bytes <= kKeptBytes ? 1.f : static_cast<float>(kKeptBytes / bytes);
 }
 
 template <typename Kernel, typename... Extra>
-int launch(Kernel k, dim3 grid, size_t smem, const NormParams& p, cudaStream_t stream, const char* what,
-           Extra... extra) {
+int launch(Kernel k, dim3 grid, int cluster, size_t smem, const NormParams& p, cudaStream_t stream,
+           const char* what, Extra... extra) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(fssim::kNormThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = static_cast<unsigned>(cluster);
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, k, p, extra...);
   if (e != cudaSuccess) {
     (void)cudaGetLastError();
@@ -139,7 +195,7 @@ int launch_pass(const NormGeometry& g, const NormParams& p, cudaStream_t stream,
   static std::atomic<bool> done[64];
   const int st = allow_ring(K, SMEM, done);
   if (st) return st;
-  return launch(K, dim3(static_cast<unsigned>(g.N * g.S), static_cast<unsigned>(g.slices)), SMEM, p, stream, what);
+  return launch(K, dim3(static_cast<unsigned>(g.N * g.S), static_cast<unsigned>(g.slices)), 1, SMEM, p, stream, what);
 }
 
 int check_common(int dtype, int weight_dtype, int activation, int64_t N, int64_t P, int64_t C,
@@ -163,6 +219,7 @@ int check_common(int dtype, int weight_dtype, int activation, int64_t N, int64_t
 
 struct ForwardPlan {
   int V;
+  ResidentPlan resident;
   NormGeometry g;
   size_t partial, bytes;
 };
@@ -171,6 +228,8 @@ ForwardPlan plan_forward(const fssim_group_norm_forward_args& a) {
   ForwardPlan p{};
   const size_t E = elem_size(a.dtype);
   p.V = vector_width(a.C, E, a.x, a.y, nullptr);
+  p.resident = plan_resident(a.N, a.P, a.C, a.groups, p.V, E, a.eps, 1);
+  if (p.resident.slots) return p;
   p.g = make_geometry(a.N, a.P, a.C, a.groups, p.V, kStatsU, a.eps);
   p.partial = round256(sizeof(float2) * static_cast<size_t>(a.N) * p.g.S * p.g.slices * p.g.GS);
   p.bytes = p.partial + sizeof(float) * fssim::kNormForwardRows * static_cast<size_t>(a.N) * a.C;
@@ -179,6 +238,7 @@ ForwardPlan plan_forward(const fssim_group_norm_forward_args& a) {
 
 struct BackwardPlan {
   int V;
+  ResidentPlan resident;
   NormGeometry g;
   size_t partial, sums, bytes;
 };
@@ -187,6 +247,12 @@ BackwardPlan plan_backward(const fssim_group_norm_backward_args& a) {
   BackwardPlan p{};
   const size_t E = elem_size(a.dtype);
   p.V = vector_width(a.C, E, a.x, a.dy, a.dx);
+  p.resident = plan_resident(a.N, a.P, a.C, a.groups, p.V, E, 0.f, 2);
+  if (p.resident.slots) {
+    // the samples' sums of the parameters' gradients, where there are several
+    if (a.N > 1 && (a.dweight || a.dbias)) p.bytes = sizeof(float2) * static_cast<size_t>(a.N) * a.C;
+    return p;
+  }
   p.g = make_geometry(a.N, a.P, a.C, a.groups, p.V, kGradU, 0.f);
   p.partial = round256(sizeof(float2) * static_cast<size_t>(a.N) * p.g.S * a.C);
   p.sums = round256(sizeof(float2) * static_cast<size_t>(a.N) * a.C);
@@ -214,7 +280,7 @@ int forward_kernels(const NormParams& p, cudaStream_t s) {
       p.g, p, s, "group norm statistics launch");
   if (st) return st;
   const int team = team_threads(p.g.S);
-  st = launch(fssim::norm_merge_kernel, team_grid(p.g, team), 0, p, s, "group norm merge launch", team);
+  st = launch(fssim::norm_merge_kernel, team_grid(p.g, team), 1, 0, p, s, "group norm merge launch", team);
   if (st) return st;
   NormParams q = p;
   q.g = apply_geometry(p.g);
@@ -232,7 +298,7 @@ int backward_kernels(const NormParams& p, cudaStream_t s) {
   int cols = 1;
   while (cols < 32 && cols < p.g.Cg) cols *= 2;
   const int team = team_threads(static_cast<int64_t>(p.g.S) * cols);
-  st = launch(fssim::norm_grad_merge_kernel, team_grid(p.g, team), 0, p, s,
+  st = launch(fssim::norm_grad_merge_kernel, team_grid(p.g, team), 1, 0, p, s,
               "group norm gradient merge launch", team, cols);
   if (st || !p.out) return st;
   NormParams q = p;
@@ -243,37 +309,62 @@ int backward_kernels(const NormParams& p, cudaStream_t s) {
 
 // One launch list per (element type, vector width, activation).
 template <template <typename, int, int> class Run, typename T, int V>
-int by_activation(int act, const NormParams& p, cudaStream_t s) {
+int by_activation(int act, const NormParams& p, const ResidentPlan& r, cudaStream_t s) {
   switch (act) {
-    case FSSIM_ACT_SILU: return Run<T, V, fssim::kNormActSilu>::run(p, s);
-    case FSSIM_ACT_RELU: return Run<T, V, fssim::kNormActRelu>::run(p, s);
-    default: return Run<T, V, fssim::kNormActNone>::run(p, s);
+    case FSSIM_ACT_SILU: return Run<T, V, fssim::kNormActSilu>::run(p, r, s);
+    case FSSIM_ACT_RELU: return Run<T, V, fssim::kNormActRelu>::run(p, r, s);
+    default: return Run<T, V, fssim::kNormActNone>::run(p, r, s);
   }
 }
 template <template <typename, int, int> class Run, typename T>
-int by_width(int V, int act, const NormParams& p, cudaStream_t s) {
+int by_width(int V, int act, const NormParams& p, const ResidentPlan& r, cudaStream_t s) {
   constexpr int full = 16 / sizeof(T), mid = 4 / sizeof(T);
-  if (V == full) return by_activation<Run, T, full>(act, p, s);
+  if (V == full) return by_activation<Run, T, full>(act, p, r, s);
   if constexpr (mid > 1) {
-    if (V == mid) return by_activation<Run, T, mid>(act, p, s);
+    if (V == mid) return by_activation<Run, T, mid>(act, p, r, s);
   }
-  return by_activation<Run, T, 1>(act, p, s);
+  return by_activation<Run, T, 1>(act, p, r, s);
 }
 template <template <typename, int, int> class Run>
-int dispatch(int dtype, int V, int act, const NormParams& p, cudaStream_t s) {
+int dispatch(int dtype, int V, int act, const NormParams& p, const ResidentPlan& r, cudaStream_t s) {
   switch (dtype) {
-    case FSSIM_F32: return by_width<Run, float>(V, act, p, s);
-    case FSSIM_F16: return by_width<Run, __half>(V, act, p, s);
-    default: return by_width<Run, __nv_bfloat16>(V, act, p, s);
+    case FSSIM_F32: return by_width<Run, float>(V, act, p, r, s);
+    case FSSIM_F16: return by_width<Run, __half>(V, act, p, r, s);
+    default: return by_width<Run, __nv_bfloat16>(V, act, p, r, s);
   }
 }
 template <typename T, int V, int ACT>
 struct Forward {
-  static int run(const NormParams& p, cudaStream_t s) { return forward_kernels<T, V, ACT>(p, s); }
+  static int run(const NormParams& p, const ResidentPlan&, cudaStream_t s) { return forward_kernels<T, V, ACT>(p, s); }
 };
 template <typename T, int V, int ACT>
 struct Backward {
-  static int run(const NormParams& p, cudaStream_t s) { return backward_kernels<T, V, ACT>(p, s); }
+  static int run(const NormParams& p, const ResidentPlan&, cudaStream_t s) { return backward_kernels<T, V, ACT>(p, s); }
+};
+
+template <auto K, typename... Extra>
+int launch_resident(const NormParams& p, const ResidentPlan& r, cudaStream_t s, const char* what, Extra... extra) {
+  static std::atomic<bool> done[64];
+  const int st = allow_ring(K, kResidentSmem, done);
+  if (st) return st;
+  const int64_t ctas = p.g.N * p.g.slices * p.g.S;
+  return launch(K, dim3(static_cast<unsigned>(ctas)), p.g.S, r.smem, p, s, what, extra...);
+}
+template <typename T, int V, int ACT>
+struct ForwardResident {
+  static int run(const NormParams& p, const ResidentPlan& r, cudaStream_t s) {
+    if constexpr (sizeof(T) * V == 16)
+      return launch_resident<fssim::norm_resident_kernel<T, V, ACT>>(p, r, s, "group norm launch");
+    else return fail(FSSIM_ERR_ARGUMENT, "resident kernels take 16-byte vectors");
+  }
+};
+template <typename T, int V, int ACT>
+struct BackwardResident {
+  static int run(const NormParams& p, const ResidentPlan& r, cudaStream_t s) {
+    if constexpr (sizeof(T) * V == 16)
+      return launch_resident<fssim::norm_grad_resident_kernel<T, V, ACT>>(p, r, s, "group norm gradient launch", r.slots);
+    else return fail(FSSIM_ERR_ARGUMENT, "resident kernels take 16-byte vectors");
+  }
 };
 
 int forward_impl(const fssim_group_norm_forward_args* a, cudaStream_t stream) {
@@ -288,12 +379,10 @@ int forward_impl(const fssim_group_norm_forward_args* a, cudaStream_t stream) {
   if (!aligned(a->x, E) || !aligned(a->y, E))
     return fail(FSSIM_ERR_ARGUMENT, "x and y must be aligned to their element size");
   const ForwardPlan plan = plan_forward(*a);
-  if (!a->workspace || a->workspace_bytes < plan.bytes)
+  if (plan.bytes && (!a->workspace || a->workspace_bytes < plan.bytes))
     return fail(FSSIM_ERR_WORKSPACE, "workspace smaller than fssim_group_norm_forward_workspace_bytes");
   if (!aligned(a->workspace, 16)) return fail(FSSIM_ERR_WORKSPACE, "workspace must be 16-byte aligned");
   NormParams p{};
-  p.g = plan.g;
-  p.g.keep = kept_share(static_cast<double>(a->N) * a->P * a->C * E);
   p.x = a->x;
   p.out = a->y;
   p.weight = a->weight;
@@ -301,9 +390,15 @@ int forward_impl(const fssim_group_norm_forward_args* a, cudaStream_t stream) {
   p.weight_dtype = a->weight_dtype;
   p.mean = a->mean;
   p.rstd = a->rstd;
+  if (plan.resident.slots) {
+    p.g = plan.resident.g;
+    return dispatch<ForwardResident>(a->dtype, plan.V, a->activation, p, plan.resident, stream);
+  }
+  p.g = plan.g;
+  p.g.keep = kept_share(static_cast<double>(a->N) * a->P * a->C * E);
   p.partial = static_cast<float2*>(a->workspace);
   p.channel = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + plan.partial);
-  return dispatch<Forward>(a->dtype, plan.V, a->activation, p, stream);
+  return dispatch<Forward>(a->dtype, plan.V, a->activation, p, plan.resident, stream);
 }
 
 int backward_impl(const fssim_group_norm_backward_args* a, cudaStream_t stream) {
@@ -327,13 +422,11 @@ int backward_impl(const fssim_group_norm_backward_args* a, cudaStream_t stream) 
   if (!aligned(a->x, E) || !aligned(a->dy, E) || !aligned(a->dx, E))
     return fail(FSSIM_ERR_ARGUMENT, "x, dy and dx must be aligned to their element size");
   const BackwardPlan plan = plan_backward(*a);
-  if (!a->workspace || a->workspace_bytes < plan.bytes)
+  if (plan.bytes && (!a->workspace || a->workspace_bytes < plan.bytes))
     return fail(FSSIM_ERR_WORKSPACE, "workspace smaller than fssim_group_norm_backward_workspace_bytes");
   if (!aligned(a->workspace, 16)) return fail(FSSIM_ERR_WORKSPACE, "workspace must be 16-byte aligned");
   char* ws = static_cast<char*>(a->workspace);
   NormParams p{};
-  p.g = plan.g;
-  p.g.keep = kept_share(2.0 * a->N * a->P * a->C * E);
   p.x = a->x;
   p.dy = a->dy;
   p.out = a->dx;
@@ -342,17 +435,25 @@ int backward_impl(const fssim_group_norm_backward_args* a, cudaStream_t stream) 
   p.weight_dtype = a->weight_dtype;
   p.mean = const_cast<float*>(a->mean);
   p.rstd = const_cast<float*>(a->rstd);
-  p.partial = reinterpret_cast<float2*>(ws);
-  p.sums = reinterpret_cast<float2*>(ws + plan.partial);
-  p.channel = reinterpret_cast<float*>(ws + plan.partial + plan.sums);
   p.dweight = a->dweight;
   p.dbias = a->dbias;
-  st = dispatch<Backward>(a->dtype, plan.V, a->activation, p, stream);
+  if (plan.resident.slots) {
+    p.g = plan.resident.g;
+    p.sums = plan.bytes ? reinterpret_cast<float2*>(ws) : nullptr;
+    st = dispatch<BackwardResident>(a->dtype, plan.V, a->activation, p, plan.resident, stream);
+  } else {
+    p.g = plan.g;
+    p.g.keep = kept_share(2.0 * a->N * a->P * a->C * E);
+    p.partial = reinterpret_cast<float2*>(ws);
+    p.sums = reinterpret_cast<float2*>(ws + plan.partial);
+    p.channel = reinterpret_cast<float*>(ws + plan.partial + plan.sums);
+    st = dispatch<Backward>(a->dtype, plan.V, a->activation, p, plan.resident, stream);
+  }
   if (st) return st;
   // (one sample's sums are the parameters' gradients: the merge has written them)
   if (a->N == 1 || (!a->dweight && !a->dbias)) return FSSIM_OK;
   const unsigned blocks = static_cast<unsigned>((a->C + fssim::kNormWarps - 1) / fssim::kNormWarps);
-  return launch(fssim::norm_param_grad_kernel, dim3(blocks), 0, p, stream,
+  return launch(fssim::norm_param_grad_kernel, dim3(blocks), 1, 0, p, stream,
                 "group norm parameter gradient launch");
 }
 

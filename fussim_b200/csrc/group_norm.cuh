@@ -26,6 +26,7 @@
 // merged likewise, in a fixed order (results repeat bit for bit), across parts in FP64.
 #pragma once
 
+#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -267,6 +268,17 @@ struct NormTile {
       s = blockIdx.x - n * g.S;
     }
     slice = blockIdx.y;
+    place(g, V);
+  }
+  // the resident kernels: a cluster of S CTAs for each sample and slice
+  __device__ __forceinline__ NormTile(const NormGeometry& g, int V) {
+    const unsigned unit = blockIdx.x / static_cast<unsigned>(g.S);
+    s = blockIdx.x - unit * g.S;
+    n = unit / static_cast<unsigned>(g.slices);
+    slice = unit - n * g.slices;
+    place(g, V);
+  }
+  __device__ __forceinline__ void place(const NormGeometry& g, int V) {
     c0 = slice * g.SC;
     c1 = min(c0 + g.SC, g.C);
     g0 = c0 / g.Cg;
@@ -467,43 +479,56 @@ struct NormSink {
 
 // A pass's shared memory: the ring, and in the reducing passes the merge's scratch after it is used.
 extern __shared__ __align__(16) unsigned char norm_ring[];
-// ---- forward: statistics ----
-template <typename T, int V, int U, int B>
-__global__ void __launch_bounds__(kNormThreads, kNormResident) norm_stats_kernel(const __grid_constant__ NormParams p) {
-  // the ring's memory again, once every thread is done with it
-  float* sm_mean = reinterpret_cast<float*>(norm_ring);
-  float* sm_m2 = sm_mean + kNormThreads * V;
-  float* column = sm_m2 + kNormThreads * V;
-  float* centre = column + kNormThreads * V;
+// A thread's channel constants: -mean, the factor rstd w and the shift, from stats(group) = (mean,
+// rstd).
+template <int V, typename Stats>
+__device__ __forceinline__ void norm_constants(const NormParams& p, const NormTile& t, Stats stats,
+                                               float2 (&minus)[kPairs<V>], float2 (&a)[kPairs<V>],
+                                               float2 (&b)[kPairs<V>]) {
   const NormGeometry& g = p.g;
-  const NormTile t(g, V, false);
-  grid_dependency_wait();
-  grid_launch_dependents();
+  const int first = t.c0 + t.chan;
+  int grp = first / g.Cg, end = (grp + 1) * g.Cg;  // one division; the next channels follow
+#pragma unroll
+  for (int v = 0; v < 2 * kPairs<V>; ++v) {
+    const int c = first + v;
+    float mv = 0.f, av = 0.f, bv = 0.f;
+    if (v < V) {
+      if (c == end) {
+        ++grp;
+        end += g.Cg;
+      }
+      const float2 st = stats(grp);
+      mv = -st.x;
+      av = p.weight ? st.y * load_weight(p.weight, p.weight_dtype, c) : st.y;
+      bv = p.bias ? load_weight(p.bias, p.weight_dtype, c) : 0.f;
+    }
+    (v & 1 ? minus[v / 2].y : minus[v / 2].x) = mv;
+    (v & 1 ? a[v / 2].y : a[v / 2].x) = av;
+    (v & 1 ? b[v / 2].y : b[v / 2].x) = bv;
+  }
+}
+
+// A thread's running statistics of its channels.
+template <typename T, int V, int U>
+struct NormMoments {
   using IO = VecIO<T, V>;
-  constexpr int N = IO::N;
+  static constexpr int N = IO::N;
   float2 mean[N], m2[N];
-#pragma unroll
-  for (int v = 0; v < N; ++v) mean[v] = m2[v] = splat2(0.f);
-  using Walk = NormWalk<T, V, U, B, false>;
-  const Walk walk(g, t);
-  NormSource<Walk, T> x(walk, p.x, 0);
-  const NormPolicy policy(g.keep < 1.f);
-  const int staying = walk.count - walk.passing(g.keep);
-  const auto start = [&](int slot, int todo) {
-    x.start(walk, slot, todo, todo > staying ? policy.pass : policy.stay);
-    x.commit();
-  };
-#pragma unroll
-  for (int b = 0; b < B - 1; ++b) start(b, walk.count - b * U);
   float before = 0.f;  // batches taken
-  walk.run(B - 1, start, [&](int slot, auto whole, int k) {
-    // a batch of U pixels, or the last one of k (k < U) with the missing ones left out
-    constexpr bool kWhole = decltype(whole)::value;
+
+  __device__ __forceinline__ NormMoments() {
+#pragma unroll
+    for (int v = 0; v < N; ++v) mean[v] = m2[v] = splat2(0.f);
+  }
+  // a batch of U pixels, or the last one of k (k < U); get(u) gives the vector of pixel u
+  template <typename Whole, typename Get>
+  __device__ __forceinline__ void take(Whole, int k, Get get) {
+    constexpr bool kWhole = Whole::value;
     float2 f[U][N];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       typename IO::Raw raw{};
-      if (kWhole || u < k) raw = x.get(walk, slot, u);
+      if (kWhole || u < k) raw = get(u);
       IO::unpack(raw, f[u]);
     }
     // the new values' weight in the mean, and that of the squared distance of the two means
@@ -529,16 +554,26 @@ __global__ void __launch_bounds__(kNormThreads, kNormResident) norm_stats_kernel
       m2[v] = add2(m2[v], fma2(mul2(d, d), splat2(cross), q));
     }
     before += 1.f;
-  });
-  __syncthreads();
+  }
+};
+
+// The threads' pairs of a CTA that has `pixels` pixels of its part become one pair per group: first
+// the mean (as distances from one of the means, so that equal values give that value exactly),
+// then the deviations. put(i, pair) takes the i-th group's. `scratch` has four floats for each
+// thread and channel.
+template <int V, typename Put>
+__device__ __forceinline__ void norm_merge_rows(const NormGeometry& g, const NormTile& t, int64_t pixels,
+                                                const float2 (&mean)[kPairs<V>], const float2 (&m2)[kPairs<V>],
+                                                float* scratch, Put put) {
+  float* sm_mean = scratch;
+  float* sm_m2 = sm_mean + kNormThreads * V;
+  float* column = sm_m2 + kNormThreads * V;
+  float* centre = column + kNormThreads * V;
   if (t.active) {
     norm_put<V>(sm_mean + t.row * g.SC + t.chan, mean);
     norm_put<V>(sm_m2 + t.row * g.SC + t.chan, m2);
   }
   __syncthreads();
-  // The rows' and channels' pairs become one pair per group: first the mean (as distances from
-  // one of the means, so that equal values give that value exactly), then the deviations.
-  const int64_t pixels = g.part_pixels(t.s);
   const int64_t full = pixels / g.rows;                        // pixels that every row took
   const int extra = static_cast<int>(pixels - full * g.rows);  // rows that took one more
   const int width = t.c1 - t.c0;
@@ -552,7 +587,6 @@ __global__ void __launch_bounds__(kNormThreads, kNormResident) norm_stats_kernel
     };
   });
   __syncthreads();
-  float2* partial = p.partial + ((static_cast<int64_t>(t.n) * g.S + t.s) * g.slices + t.slice) * g.GS;
   columns.sum_groups(g, t, column, [&](int i, int cb, int w, float sum) {
     centre[i] = sm_mean[cb] + sum / (static_cast<float>(pixels) * w);
   });
@@ -566,9 +600,73 @@ __global__ void __launch_bounds__(kNormThreads, kNormResident) norm_stats_kernel
     };
   });
   __syncthreads();
-  columns.sum_groups(g, t, column, [&](int i, int cb, int w, float sum) {
-    partial[i] = make_float2(centre[i], sum);
+  columns.sum_groups(g, t, column, [&](int i, int cb, int w, float sum) { put(i, make_float2(centre[i], sum)); });
+}
+
+// The threads' sums of a CTA become put(c, sums) for each channel of the slice.
+template <int V, typename Put>
+__device__ __forceinline__ void norm_merge_sums(const NormGeometry& g, const NormTile& t,
+                                                const float2 (&s1)[kPairs<V>], const float2 (&s2)[kPairs<V>],
+                                                float* scratch, Put put) {
+  float* sm1 = scratch;
+  float* sm2 = sm1 + kNormThreads * V;
+  float* column1 = sm2 + kNormThreads * V;
+  float* column2 = column1 + kNormThreads * V;
+  if (t.active) {
+    norm_put<V>(sm1 + t.row * g.SC + t.chan, s1);
+    norm_put<V>(sm2 + t.row * g.SC + t.chan, s2);
+  }
+  __syncthreads();
+  const int width = t.c1 - t.c0;
+  const NormColumns columns(width);
+  columns.sum_rows(g, width, column1, [&](int c) { return [&, c](int r) { return sm1[r * g.SC + c]; }; });
+  columns.sum_rows(g, width, column2, [&](int c) { return [&, c](int r) { return sm2[r * g.SC + c]; }; });
+  __syncthreads();
+  for (int c = threadIdx.x; c < width; c += kNormThreads) {
+    float v1 = 0.f, v2 = 0.f;
+    for (int j = 0; j < columns.T; ++j) {
+      v1 += column1[j * g.SC + c];
+      v2 += column2[j * g.SC + c];
+    }
+    put(c, make_float2(v1, v2));
+  }
+}
+
+// ---- forward: statistics ----
+template <typename T, int V, int U, int B>
+__global__ void __launch_bounds__(kNormThreads, kNormResident) norm_stats_kernel(const __grid_constant__ NormParams p) {
+  const NormGeometry& g = p.g;
+  const NormTile t(g, V, false);
+  grid_dependency_wait();
+  grid_launch_dependents();
+  using Walk = NormWalk<T, V, U, B, false>;
+  const Walk walk(g, t);
+  NormSource<Walk, T> x(walk, p.x, 0);
+  const NormPolicy policy(g.keep < 1.f);
+  const int staying = walk.count - walk.passing(g.keep);
+  const auto start = [&](int slot, int todo) {
+    x.start(walk, slot, todo, todo > staying ? policy.pass : policy.stay);
+    x.commit();
+  };
+#pragma unroll
+  for (int b = 0; b < B - 1; ++b) start(b, walk.count - b * U);
+  NormMoments<T, V, U> moments;
+  walk.run(B - 1, start, [&](int slot, auto whole, int k) {
+    moments.take(whole, k, [&](int u) { return x.get(walk, slot, u); });
   });
+  __syncthreads();  // the ring is done with: its memory is the merge's scratch
+  float2* partial = p.partial + ((static_cast<int64_t>(t.n) * g.S + t.s) * g.slices + t.slice) * g.GS;
+  norm_merge_rows<V>(g, t, g.part_pixels(t.s), moments.mean, moments.m2, reinterpret_cast<float*>(norm_ring),
+                     [&](int i, float2 pair) { partial[i] = pair; });
+}
+
+// (mean, rstd) of a group from its sums of distances from ref and of squares around it.
+__device__ __forceinline__ float2 norm_statistics(const NormGeometry& g, double ref, double sum, double q) {
+  sum *= g.inv_m;
+  double var = q * g.inv_m - sum * sum;
+  if (var < 0.0) var = 0.0;  // a NaN stays
+  return make_float2(static_cast<float>(ref + sum),
+                     __frsqrt_rn(static_cast<float>(var + static_cast<double>(g.eps))));
 }
 
 // ---- the merging launches: a team of kNormThreads / teams threads for each (sample, group) ----
@@ -622,11 +720,8 @@ __global__ void __launch_bounds__(kNormThreads) norm_merge_kernel(const __grid_c
   }
   const double2 total = team_sum(sum, q, team_threads, sm);
   if (!real) return;
-  sum = total.x * g.inv_m;
-  double var = total.y * g.inv_m - sum * sum;
-  if (var < 0.0) var = 0.0;  // a NaN stays
-  const float mean = static_cast<float>(ref + sum);
-  const float rstd = __frsqrt_rn(static_cast<float>(var + static_cast<double>(g.eps)));
+  const float2 st = norm_statistics(g, ref, total.x, total.y);
+  const float mean = st.x, rstd = st.y;
   if (p.mean && lane == 0) {
     p.mean[id] = mean;
     p.rstd[id] = rstd;
@@ -686,10 +781,6 @@ __global__ void __launch_bounds__(kNormThreads, kNormApplyResident) norm_apply_k
 // ---- backward: per-channel sums of one part ----
 template <typename T, int V, int ACT, int U, int B>
 __global__ void __launch_bounds__(kNormThreads, kNormResident) norm_grad_sums_kernel(const __grid_constant__ NormParams p) {
-  float* sm1 = reinterpret_cast<float*>(norm_ring);
-  float* sm2 = sm1 + kNormThreads * V;
-  float* column1 = sm2 + kNormThreads * V;
-  float* column2 = column1 + kNormThreads * V;
   const NormGeometry& g = p.g;
   const NormTile t(g, V, false);
   grid_dependency_wait();
@@ -714,26 +805,10 @@ __global__ void __launch_bounds__(kNormThreads, kNormResident) norm_grad_sums_ke
   for (int v = 0; v < N; ++v) s1[v] = s2[v] = splat2(0.f);
   if (t.active) {
     float2 minus[N], a[N], b[N];
-    const int first = t.c0 + t.chan;
-    int grp = first / g.Cg, end = (grp + 1) * g.Cg;  // one division; the next channels follow
-#pragma unroll
-    for (int v = 0; v < 2 * N; ++v) {
-      const int c = first + v;
-      float mv = 0.f, av = 0.f, bv = 0.f;
-      if (v < V) {
-        if (c == end) {
-          ++grp;
-          end += g.Cg;
-        }
-        const int64_t at = static_cast<int64_t>(t.n) * g.G + grp;
-        mv = -p.mean[at];
-        av = p.weight ? p.rstd[at] * load_weight(p.weight, p.weight_dtype, c) : p.rstd[at];
-        bv = p.bias ? load_weight(p.bias, p.weight_dtype, c) : 0.f;
-      }
-      (v & 1 ? minus[v / 2].y : minus[v / 2].x) = mv;
-      (v & 1 ? a[v / 2].y : a[v / 2].x) = av;
-      (v & 1 ? b[v / 2].y : b[v / 2].x) = bv;
-    }
+    norm_constants<V>(p, t, [&](int grp) {
+      const int64_t at = static_cast<int64_t>(t.n) * g.G + grp;
+      return make_float2(p.mean[at], p.rstd[at]);
+    }, minus, a, b);
     walk.run(B - 1, start, [&](int slot, auto whole, int k) {
       constexpr bool kWhole = decltype(whole)::value;
 #pragma unroll
@@ -753,25 +828,9 @@ __global__ void __launch_bounds__(kNormThreads, kNormResident) norm_grad_sums_ke
     });
   }
   __syncthreads();
-  if (t.active) {
-    norm_put<V>(sm1 + t.row * g.SC + t.chan, s1);
-    norm_put<V>(sm2 + t.row * g.SC + t.chan, s2);
-  }
-  __syncthreads();
-  const int width = t.c1 - t.c0;
-  const NormColumns columns(width);
-  columns.sum_rows(g, width, column1, [&](int c) { return [&, c](int r) { return sm1[r * g.SC + c]; }; });
-  columns.sum_rows(g, width, column2, [&](int c) { return [&, c](int r) { return sm2[r * g.SC + c]; }; });
-  __syncthreads();
   float2* partial = p.partial + (static_cast<int64_t>(t.n) * g.S + t.s) * g.C + t.c0;
-  for (int c = threadIdx.x; c < width; c += kNormThreads) {
-    float v1 = 0.f, v2 = 0.f;
-    for (int j = 0; j < columns.T; ++j) {
-      v1 += column1[j * g.SC + c];
-      v2 += column2[j * g.SC + c];
-    }
-    partial[c] = make_float2(v1, v2);
-  }
+  norm_merge_sums<V>(g, t, s1, s2, reinterpret_cast<float*>(norm_ring),
+                     [&](int c, float2 sums) { partial[c] = sums; });
 }
 
 // Backward: sums over the parts, and the group's two means. `cols` (a power of two, at most 32)
@@ -918,6 +977,210 @@ __global__ void __launch_bounds__(kNormThreads, kNormApplyResident) norm_grad_ap
         dx.put(walk, IO::pack(f), policy.pass);
       }
   });
+}
+
+// ---- small tensors: one launch for each direction ----
+// A cluster of S CTAs takes one sample's slice of whole groups, each CTA a contiguous part of the
+// pixels, which it keeps in shared memory: the statistics pass from CTA to CTA over distributed
+// shared memory, and the input is read once. No workspace; what bounds these is latency.
+constexpr int kNormScratch = 6;  // floats of scratch for each thread and channel
+
+// A resident part: vector i of a thread, in its own slots.
+template <typename T, int V>
+struct NormResidentPart {
+  using Walk = NormWalk<T, V, 1, 1, true>;
+  static_assert(Walk::kAsync, "16-byte vectors");
+  unsigned base;
+  __device__ __forceinline__ explicit NormResidentPart(int offset)
+      : base(NormSource<Walk, T>::address() + offset + threadIdx.x * 16) {}
+  __device__ __forceinline__ void start(const Walk& w, const void* x) const {
+    const T* next = static_cast<const T*>(x) + w.first;
+    for (int i = 0; i < w.count; ++i, next += w.stride)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(base + i * kNormThreads * 16), "l"(next)
+                   : "memory");
+  }
+  __device__ __forceinline__ uint4 get(int i) const {
+    uint4 r;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(base + i * kNormThreads * 16) : "memory");
+    return r;
+  }
+};
+__device__ __forceinline__ void norm_wait_resident() {
+  asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
+}
+
+template <typename T, int V, int ACT>
+__global__ void __launch_bounds__(kNormThreads) norm_resident_kernel(const __grid_constant__ NormParams p) {
+  namespace cg = cooperative_groups;
+  constexpr int U = 4, N = kPairs<V>;
+  using IO = VecIO<T, V>;
+  const NormGeometry& g = p.g;
+  const NormTile t(g, V);
+  const typename NormResidentPart<T, V>::Walk walk(g, t);
+  float* scratch = reinterpret_cast<float*>(norm_ring);
+  const NormResidentPart<T, V> x(kNormScratch * kNormThreads * V * 4);
+  grid_dependency_wait();
+  grid_launch_dependents();
+  x.start(walk, p.x);
+  norm_wait_resident();
+  NormMoments<T, V, U> moments;
+  for (int i = 0; i < walk.count; i += U) {
+    const auto get = [&](int u) { return x.get(i + u); };
+    if (i + U <= walk.count) moments.take(std::true_type{}, U, get);
+    else moments.take(std::false_type{}, walk.count - i, get);
+  }
+  // pairs: this CTA's, for the cluster to read; stats: the cluster's (mean, rstd) of each group
+  float2* pairs = reinterpret_cast<float2*>(scratch + 4 * kNormThreads * V);
+  float2* stats = reinterpret_cast<float2*>(scratch);
+  norm_merge_rows<V>(g, t, g.base + (t.s < g.extra), moments.mean, moments.m2, scratch,
+                     [&](int i, float2 pair) { pairs[i] = pair; });
+  const cg::cluster_group cluster = cg::this_cluster();
+  cluster.sync();
+  for (int i = threadIdx.x; i < t.g1 - t.g0; i += kNormThreads) {
+    const double ref = cluster.map_shared_rank(pairs, 0)[i].x;
+    double sum = 0.0, q = 0.0;
+    for (int r = 0; r < g.S; ++r) {
+      const float2 v = cluster.map_shared_rank(pairs, r)[i];
+      const double cnt = static_cast<double>(g.base + (r < g.extra)) * g.Cg;
+      const double d = v.x - ref;
+      sum = fma(cnt, d, sum);
+      q += fma(cnt * d, d, static_cast<double>(v.y));
+    }
+    const float2 st = norm_statistics(g, ref, sum, q);
+    stats[i] = st;
+    if (p.mean && t.s == 0) {
+      p.mean[static_cast<int64_t>(t.n) * g.G + t.g0 + i] = st.x;
+      p.rstd[static_cast<int64_t>(t.n) * g.G + t.g0 + i] = st.y;
+    }
+  }
+  cluster.sync();  // stats are written, and nobody reads another's pairs any more
+  if (!t.active) return;
+  float2 minus[N], a[N], b[N];
+  norm_constants<V>(p, t, [&](int grp) { return stats[grp - t.g0]; }, minus, a, b);
+  T* y = static_cast<T*>(p.out) + walk.first;
+  for (int i = 0; i < walk.count; ++i, y += walk.stride) {
+    float2 f[N];
+    IO::unpack(x.get(i), f);
+#pragma unroll
+    for (int v = 0; v < N; ++v) f[v] = activate<T, ACT>(fma2(add2(f[v], minus[v]), a[v], b[v]));
+    IO::store(y, IO::pack(f));
+  }
+}
+
+template <typename T, int V, int ACT>
+__global__ void __launch_bounds__(kNormThreads) norm_grad_resident_kernel(const __grid_constant__ NormParams p,
+                                                                          int slots) {
+  namespace cg = cooperative_groups;
+  constexpr int N = kPairs<V>;
+  using IO = VecIO<T, V>;
+  const NormGeometry& g = p.g;
+  const NormTile t(g, V);
+  const typename NormResidentPart<T, V>::Walk walk(g, t);
+  float* scratch = reinterpret_cast<float*>(norm_ring);
+  constexpr int kArray = kNormThreads * V;
+  const NormResidentPart<T, V> x(kNormScratch * kArray * 4), dy(kNormScratch * kArray * 4 + slots * kNormThreads * 16);
+  grid_dependency_wait();
+  grid_launch_dependents();
+  x.start(walk, p.x);
+  dy.start(walk, p.dy);
+  float2 minus[N], a[N], b[N], s1[N], s2[N];
+#pragma unroll
+  for (int v = 0; v < N; ++v) minus[v] = a[v] = b[v] = s1[v] = s2[v] = splat2(0.f);
+  if (t.active)
+    norm_constants<V>(p, t, [&](int grp) {
+      const int64_t at = static_cast<int64_t>(t.n) * g.G + grp;
+      return make_float2(p.mean[at], p.rstd[at]);
+    }, minus, a, b);
+  norm_wait_resident();
+  for (int i = 0; i < walk.count; ++i) {
+    float2 f[N], d[N];
+    IO::unpack(x.get(i), f);
+    IO::unpack(dy.get(i), d);
+#pragma unroll
+    for (int v = 0; v < N; ++v) {
+      const float2 xc = add2(f[v], minus[v]);
+      const float2 dz = activate_grad<T, ACT>(fma2(xc, a[v], b[v]), d[v]);
+      s1[v] = add2(s1[v], dz);
+      s2[v] = fma2(dz, xc, s2[v]);
+    }
+  }
+  // sums: this CTA's, for the cluster to read; weighted: the cluster's, times w, of each channel;
+  // means: of each group
+  float2* sums = reinterpret_cast<float2*>(scratch + 4 * kArray);
+  float2* weighted = reinterpret_cast<float2*>(scratch);
+  float2* means = reinterpret_cast<float2*>(scratch + 2 * kArray);
+  norm_merge_sums<V>(g, t, s1, s2, scratch, [&](int c, float2 v) { sums[c] = v; });
+  const cg::cluster_group cluster = cg::this_cluster();
+  cluster.sync();
+  for (int i = threadIdx.x; i < t.c1 - t.c0; i += kNormThreads) {
+    const int c = t.c0 + i;
+    double v1 = 0.0, v2 = 0.0;
+    for (int r = 0; r < g.S; ++r) {
+      const float2 v = cluster.map_shared_rank(sums, r)[i];
+      v1 += v.x;
+      v2 += v.y;
+    }
+    const float rstd = p.rstd[static_cast<int64_t>(t.n) * g.G + c / g.Cg];
+    v2 *= rstd;
+    const double w = p.weight ? load_weight(p.weight, p.weight_dtype, c) : 1.0;
+    weighted[i] = make_float2(static_cast<float>(w * v1 * g.inv_m), static_cast<float>(w * v2 * g.inv_m));
+    if (t.s == 0) {
+      if (g.N == 1) {  // one sample: its sums are the parameters' gradients
+        if (p.dweight) store_weight(p.dweight, p.weight_dtype, c, static_cast<float>(v2));
+        if (p.dbias) store_weight(p.dbias, p.weight_dtype, c, static_cast<float>(v1));
+      } else if (p.sums) {
+        p.sums[static_cast<int64_t>(t.n) * g.C + c] = make_float2(static_cast<float>(v1), static_cast<float>(v2));
+      }
+    }
+  }
+  cluster.sync();  // nobody reads another's sums any more
+  if (!p.out) return;
+  const int lane = threadIdx.x % 32;
+  for (int i = threadIdx.x / 32; i < t.g1 - t.g0; i += kNormWarps) {
+    const int cb = (t.g0 + i) * g.Cg - t.c0;
+    float v1 = 0.f, v2 = 0.f;
+    for (int c = lane; c < g.Cg; c += 32) {
+      v1 += weighted[cb + c].x;
+      v2 += weighted[cb + c].y;
+    }
+    v1 = warp_sum(v1);
+    v2 = warp_sum(v2);
+    if (lane == 0) {
+      const float rstd = p.rstd[static_cast<int64_t>(t.n) * g.G + t.g0 + i];
+      means[i] = make_float2(-rstd * v1, -rstd * rstd * v2);
+    }
+  }
+  __syncthreads();
+  if (!t.active) return;
+  float2 k1[N], k2[N];
+  {
+    const int first = t.c0 + t.chan;
+    int grp = first / g.Cg, end = (grp + 1) * g.Cg;
+#pragma unroll
+    for (int v = 0; v < 2 * N; ++v) {
+      if (v < V && first + v == end) {
+        ++grp;
+        end += g.Cg;
+      }
+      const float2 k = means[grp - t.g0];
+      (v & 1 ? k1[v / 2].y : k1[v / 2].x) = k.x;
+      (v & 1 ? k2[v / 2].y : k2[v / 2].x) = k.y;
+    }
+  }
+  T* dx = static_cast<T*>(p.out) + walk.first;
+  for (int i = 0; i < walk.count; ++i, dx += walk.stride) {
+    float2 f[N], d[N];
+    IO::unpack(x.get(i), f);
+    IO::unpack(dy.get(i), d);
+#pragma unroll
+    for (int v = 0; v < N; ++v) {
+      const float2 xc = add2(f[v], minus[v]);
+      const float2 dz = activate_grad<T, ACT>(fma2(xc, a[v], b[v]), d[v]);
+      f[v] = fma2(xc, k2[v], fma2(a[v], dz, k1[v]));
+    }
+    IO::store(dx, IO::pack(f));
+  }
 }
 
 }  // namespace fssim

@@ -136,7 +136,7 @@ SOME = 1 << 20  # a pointer that no refused call follows
 
 
 def _forward(**kw):
-    a = ForwardArgs(dtype=0, weight_dtype=0, activation=1, N=2, P=64, C=32, groups=4, eps=1e-5,
+    a = ForwardArgs(dtype=0, weight_dtype=0, activation=1, N=2, P=1 << 20, C=32, groups=4, eps=1e-5,
                     x=SOME, y=SOME)
     for k, v in kw.items():
         setattr(a, k, v)
@@ -160,7 +160,7 @@ def test_c_forward_refusals(lib, kw, status):
 
 
 def _backward(**kw):
-    a = BackwardArgs(dtype=1, weight_dtype=0, activation=1, N=2, P=64, C=32, groups=4, x=SOME,
+    a = BackwardArgs(dtype=1, weight_dtype=0, activation=1, N=2, P=1 << 20, C=32, groups=4, x=SOME,
                      dy=SOME, mean=SOME, rstd=SOME, dx=SOME)
     for k, v in kw.items():
         setattr(a, k, v)
