@@ -32,11 +32,15 @@ constexpr double kKeptBytes = 80 << 20;
 constexpr int kStatsU = 8, kStatsB = 2;
 constexpr int kApplyU = 4, kApplyB = 4;
 constexpr int kGradU = 2, kGradB = 4;
-// The resident kernels: the largest tensors they take (x, in the backward x and dy), their slices'
-// bytes a pixel, and a CTA's shared memory.
+// The resident kernels: the largest input they take (x, in the backward x and dy), the most vectors
+// of a thread, and their slices' bytes a pixel. On a B200 they are faster than the passes below
+// these (16-bit, device time, fwd / bwd us: 1x64x16^2 6.7 / 6.0 against 7.9 / 7.2, 4x512x32^2
+// 10.3 / 9.7 against 11.0 / 15.5) and slower above (1x128x128^2 with 32 vectors 16.1 against
+// 10.9 forward, 16x64x64^2 of 16 MB 23.6 against 16.9 backward); one launch in place of three
+// also saves 4 us of the host's time.
 constexpr double kResidentBytes = 8 << 20;
+constexpr int kResidentSlots = 8;
 constexpr int64_t kSliceBytes = 64;
-constexpr size_t kResidentSmem = 200 << 10;
 constexpr int64_t kApplySteps = 32, kApplyWaves = 6;
 
 size_t elem_size(int dtype) { return dtype == FSSIM_F32 ? 4 : 2; }
@@ -73,11 +77,15 @@ NormGeometry make_geometry(int64_t N, int64_t P, int64_t C, int64_t G, int V, in
   if (g.GS > g.G) g.GS = g.G;
   // Parts of the reducing pass: one wave of CTAs, or where the samples are more than that, enough
   // that the last wave's idle SMs weigh little; no more than there are tiles.
-  g.tile = static_cast<int64_t>(g.rows) * reduce_batch;
-  g.tiles = (P + g.tile - 1) / g.tile;
+  g.tile = g.rows * reduce_batch;
+  const int64_t tiles = (P + g.tile - 1) / g.tile;
   const int64_t each = N * g.slices;
   const int64_t S = each <= kWave ? kWave / each : (4 * kWave + each - 1) / each;
-  g.S = static_cast<int>(S < g.tiles ? S : g.tiles);
+  g.S = static_cast<int>(S < tiles ? S : tiles);
+  g.part_tiles = static_cast<int>(tiles / g.S);
+  g.extra_tiles = static_cast<int>(tiles % g.S);
+  g.last_part = static_cast<int>((tiles - 1) % g.S);
+  g.lacking = static_cast<int>(tiles * g.tile - P);
   return g;
 }
 
@@ -93,14 +101,14 @@ NormGeometry apply_geometry(NormGeometry g) {
   if (S * each < kApplyWaves * kWave) S = each <= kWave ? kWave / each : (4 * kWave + each - 1) / each;
   if (S > most) S = most;
   g.S = static_cast<int>(S);
-  g.base = g.P / S;
+  g.base = static_cast<int>(g.P / S);
   g.extra = static_cast<int>(g.P % S);
   return g;
 }
 
 // The resident kernels' split, where they take the call: slices of whole groups of at least
-// kSliceBytes a pixel, clusters large enough to spread the work, and parts that fit the shared
-// memory (`tensors` of them at a time). slots is 0 where they do not take it.
+// kSliceBytes a pixel, and clusters large enough to spread the work, for `tensors` tensors held
+// at a time. slots is 0 where they do not take it.
 struct ResidentPlan {
   NormGeometry g;
   int slots;    // vectors of a thread
@@ -132,12 +140,11 @@ ResidentPlan plan_resident(int64_t N, int64_t P, int64_t C, int64_t G, int V, si
   const int64_t units = N * g.slices;
   const auto slots = [&](int K) { return ((P + K - 1) / K + g.rows - 1) / g.rows; };
   const size_t scratch = sizeof(float) * fssim::kNormScratch * fssim::kNormThreads * V;
-  const int64_t most = static_cast<int64_t>((kResidentSmem - scratch) / (16 * fssim::kNormThreads * tensors));
   int K = 1;
-  while (K < 8 && (slots(K) > most || (slots(K) > 2 && units * K * 2 <= kWave))) K *= 2;
-  if (slots(K) > most || units * K > INT_MAX) return r;
+  while (K < 8 && (slots(K) > kResidentSlots || (slots(K) > 2 && units * K * 2 <= kWave))) K *= 2;
+  if (slots(K) > kResidentSlots) return r;
   g.S = K;
-  g.base = P / K;
+  g.base = static_cast<int>(P / K);
   g.extra = static_cast<int>(P % K);
   r.slots = static_cast<int>(slots(K));
   r.smem = scratch + static_cast<size_t>(r.slots) * 16 * fssim::kNormThreads * tensors;
@@ -260,14 +267,15 @@ BackwardPlan plan_backward(const fssim_group_norm_backward_args& a) {
   return p;
 }
 
-// Threads that merge one group, for this many partial results: a warp at least, a CTA at most.
-int team_threads(int64_t results) {
-  int t = 32;
-  while (t < fssim::kNormThreads && t < results) t *= 2;
+// Threads that merge one group, for this many partial results, as a power of two: a warp at least, a
+// CTA at most.
+int team_shift(int64_t results) {
+  int t = 5;
+  while ((1 << t) < fssim::kNormThreads && (1 << t) < results) ++t;
   return t;
 }
-dim3 team_grid(const NormGeometry& g, int team) {
-  const int64_t teams = fssim::kNormThreads / team;
+dim3 team_grid(const NormGeometry& g, int shift) {
+  const int64_t teams = fssim::kNormThreads >> shift;
   return dim3(static_cast<unsigned>((g.N * g.G + teams - 1) / teams));
 }
 
@@ -279,7 +287,7 @@ int forward_kernels(const NormParams& p, cudaStream_t s) {
   int st = launch_pass<fssim::norm_stats_kernel<T, V, kStatsU, kStatsB>, (ring > scratch ? ring : scratch)>(
       p.g, p, s, "group norm statistics launch");
   if (st) return st;
-  const int team = team_threads(p.g.S);
+  const int team = team_shift(p.g.S);
   st = launch(fssim::norm_merge_kernel, team_grid(p.g, team), 1, 0, p, s, "group norm merge launch", team);
   if (st) return st;
   NormParams q = p;
@@ -295,9 +303,9 @@ int backward_kernels(const NormParams& p, cudaStream_t s) {
   int st = launch_pass<fssim::norm_grad_sums_kernel<T, V, ACT, kGradU, kGradB>, (ring > scratch ? ring : scratch)>(
       p.g, p, s, "group norm gradient sums launch");
   if (st) return st;
-  int cols = 1;
-  while (cols < 32 && cols < p.g.Cg) cols *= 2;
-  const int team = team_threads(static_cast<int64_t>(p.g.S) * cols);
+  int cols = 0;  // channels merged at a time, likewise
+  while (cols < 5 && (1 << cols) < p.g.Cg) ++cols;
+  const int team = team_shift(static_cast<int64_t>(p.g.S) << cols);
   st = launch(fssim::norm_grad_merge_kernel, team_grid(p.g, team), 1, 0, p, s,
               "group norm gradient merge launch", team, cols);
   if (st || !p.out) return st;
@@ -345,7 +353,9 @@ struct Backward {
 template <auto K, typename... Extra>
 int launch_resident(const NormParams& p, const ResidentPlan& r, cudaStream_t s, const char* what, Extra... extra) {
   static std::atomic<bool> done[64];
-  const int st = allow_ring(K, kResidentSmem, done);
+  // (attribute for the most that any call may ask for)
+  constexpr size_t most = fssim::kNormThreads * 16 * (2 * kResidentSlots + 2 * fssim::kNormScratch);
+  const int st = allow_ring(K, most, done);
   if (st) return st;
   const int64_t ctas = p.g.N * p.g.slices * p.g.S;
   return launch(K, dim3(static_cast<unsigned>(ctas)), p.g.S, r.smem, p, s, what, extra...);
@@ -379,6 +389,8 @@ int forward_impl(const fssim_group_norm_forward_args* a, cudaStream_t stream) {
   if (!aligned(a->x, E) || !aligned(a->y, E))
     return fail(FSSIM_ERR_ARGUMENT, "x and y must be aligned to their element size");
   const ForwardPlan plan = plan_forward(*a);
+  if (!plan.resident.slots && a->P / plan.g.S >= (int64_t{1} << 30))
+    return fail(FSSIM_ERR_SHAPE, "a CTA's part has 2^30 pixels or more");
   if (plan.bytes && (!a->workspace || a->workspace_bytes < plan.bytes))
     return fail(FSSIM_ERR_WORKSPACE, "workspace smaller than fssim_group_norm_forward_workspace_bytes");
   if (!aligned(a->workspace, 16)) return fail(FSSIM_ERR_WORKSPACE, "workspace must be 16-byte aligned");
@@ -388,6 +400,7 @@ int forward_impl(const fssim_group_norm_forward_args* a, cudaStream_t stream) {
   p.weight = a->weight;
   p.bias = a->bias;
   p.weight_dtype = a->weight_dtype;
+  p.weight_vectors = aligned(a->weight, 16) && aligned(a->bias, 16);
   p.mean = a->mean;
   p.rstd = a->rstd;
   if (plan.resident.slots) {
@@ -422,6 +435,8 @@ int backward_impl(const fssim_group_norm_backward_args* a, cudaStream_t stream) 
   if (!aligned(a->x, E) || !aligned(a->dy, E) || !aligned(a->dx, E))
     return fail(FSSIM_ERR_ARGUMENT, "x, dy and dx must be aligned to their element size");
   const BackwardPlan plan = plan_backward(*a);
+  if (!plan.resident.slots && a->P / plan.g.S >= (int64_t{1} << 30))
+    return fail(FSSIM_ERR_SHAPE, "a CTA's part has 2^30 pixels or more");
   if (plan.bytes && (!a->workspace || a->workspace_bytes < plan.bytes))
     return fail(FSSIM_ERR_WORKSPACE, "workspace smaller than fssim_group_norm_backward_workspace_bytes");
   if (!aligned(a->workspace, 16)) return fail(FSSIM_ERR_WORKSPACE, "workspace must be 16-byte aligned");
@@ -433,6 +448,7 @@ int backward_impl(const fssim_group_norm_backward_args* a, cudaStream_t stream) 
   p.weight = a->weight;
   p.bias = a->bias;
   p.weight_dtype = a->weight_dtype;
+  p.weight_vectors = aligned(a->weight, 16) && aligned(a->bias, 16);
   p.mean = const_cast<float*>(a->mean);
   p.rstd = const_cast<float*>(a->rstd);
   p.dweight = a->dweight;

@@ -58,20 +58,19 @@ struct NormGeometry {
   float eps;
   float keep;        // share of the input that may stay in L2 from pass to pass
   double inv_m;      // 1 / (P * Cg)
-  // Reducing passes: part s has the tiles s, s + S, ... of `tile` pixels; the last of all `tiles`
-  // may be short.
-  int64_t tile, tiles;
+  // Reducing passes: part s has the tiles s, s + S, ... of `tile` pixels; the last of all, which
+  // `last_part` has, lacks `lacking` pixels. Parts have `part_tiles` tiles, the first `extra_tiles`
+  // one more. (A part's pixels fit 31 bits, and the kernels divide no 64-bit numbers: that
+  // alone took microseconds of a launch.)
+  int tile, part_tiles, extra_tiles, last_part, lacking;
   // Applying passes: contiguous parts of `base` pixels; the first `extra` have one more.
-  int64_t base;
-  int extra;
+  int base, extra;
 
-  __device__ __forceinline__ int64_t part_tiles(int s) const { return tiles / S + (s < tiles % S); }
-  // the part that has the last tile, and the pixels that tile lacks
-  __device__ __forceinline__ int last_part() const { return static_cast<int>((tiles - 1) % S); }
-  __device__ __forceinline__ int64_t lacking() const { return tiles * tile - P; }
-  __device__ __forceinline__ int64_t part_pixels(int s) const {
-    return part_tiles(s) * tile - (s == last_part() ? lacking() : 0);
+  __device__ __forceinline__ int tiles_of(int s) const { return part_tiles + (s < extra_tiles); }
+  __device__ __forceinline__ int part_pixels(int s) const {
+    return tiles_of(s) * tile - (s == last_part ? lacking : 0);
   }
+  __device__ __forceinline__ int run_pixels(int s) const { return base + (s < extra); }
 };
 
 struct NormParams {
@@ -81,6 +80,7 @@ struct NormParams {
   void* out;            // y or dx
   const void* weight;   // C values of weight_dtype, or nullptr (ones)
   const void* bias;     // C values of weight_dtype, or nullptr (zeros)
+  int weight_vectors;   // both start at a multiple of 16 bytes
   int weight_dtype;
   float* mean;          // N * G
   float* rstd;          // N * G
@@ -305,11 +305,11 @@ __device__ __forceinline__ void norm_put(float* p, const float2 (&f)[kPairs<V>])
 struct NormColumns {
   int cols, T, col, sub;
   __device__ __forceinline__ explicit NormColumns(int width) {
-    cols = width > kNormThreads / 2 ? kNormThreads : 1 << (32 - __clz(width - 1));
-    if (width == 1) cols = 1;
-    T = kNormThreads / cols;
+    const int shift = width > kNormThreads / 2 ? __ffs(kNormThreads) - 1 : width > 1 ? 32 - __clz(width - 1) : 0;
+    cols = 1 << shift;
+    T = kNormThreads >> shift;
     col = threadIdx.x & (cols - 1);
-    sub = threadIdx.x / cols;
+    sub = threadIdx.x >> shift;
   }
   template <typename F>
   __device__ __forceinline__ void sum_rows(const NormGeometry& g, int width, float* out, F f) const {
@@ -328,7 +328,8 @@ struct NormColumns {
   __device__ __forceinline__ void sum_groups(const NormGeometry& g, const NormTile& t, const float* in, F f) const {
     const bool narrow = g.Cg * T <= 16;
     const int lane = narrow ? 0 : threadIdx.x % 32, lanes = narrow ? 1 : 32;
-    for (int i = threadIdx.x / lanes; i < t.g1 - t.g0; i += kNormThreads / lanes) {
+    const int step = narrow ? kNormThreads : kNormWarps;
+    for (int i = narrow ? threadIdx.x : threadIdx.x / 32; i < t.g1 - t.g0; i += step) {
       const int cb = max((t.g0 + i) * g.Cg, t.c0) - t.c0;
       const int w = min((t.g0 + i + 1) * g.Cg, t.c1) - t.c0 - cb;
       float v = 0.f;
@@ -378,19 +379,19 @@ struct NormWalk {
     stride = static_cast<int64_t>(g.rows) * g.C;
     int64_t px;
     if (APPLYING) {
-      const int64_t pixels = g.base + (t.s < g.extra);
-      count = t.row < pixels ? static_cast<int>((pixels - t.row - 1) / g.rows) + 1 : 0;
-      px = g.base * t.s + min(t.s, g.extra) + t.row + static_cast<int64_t>(count - 1) * g.rows;
+      const int pixels = g.run_pixels(t.s);
+      count = t.row < pixels ? (pixels - t.row - 1) / g.rows + 1 : 0;
+      px = static_cast<int64_t>(g.base) * t.s + min(t.s, g.extra) + t.row + static_cast<int64_t>(count - 1) * g.rows;
       stride = -stride;
       jump = 0;
     } else {
-      const int missing = t.s == g.last_part() ? static_cast<int>(g.lacking()) : 0;
+      const int missing = t.s == g.last_part ? g.lacking : 0;
       // pixels of a full tile that this row lacks in the last one
-      const int last = static_cast<int>(g.tile) - missing;
+      const int last = g.tile - missing;
       const int lost = missing == 0 ? 0 : U - (t.row < last ? (last - t.row - 1) / g.rows + 1 : 0);
-      count = static_cast<int>(g.part_tiles(t.s)) * U - lost;
-      px = t.s * g.tile + t.row;
-      jump = (g.S - 1) * g.tile * g.C;
+      count = g.tiles_of(t.s) * U - lost;
+      px = static_cast<int64_t>(t.s) * g.tile + t.row;
+      jump = static_cast<int64_t>(g.S - 1) * g.tile * g.C;
     }
     if (!t.active) count = 0;
     first = (t.n * g.P + px) * g.C + t.c0 + t.chan;
@@ -479,32 +480,82 @@ struct NormSink {
 
 // A pass's shared memory: the ring, and in the reducing passes the merge's scratch after it is used.
 extern __shared__ __align__(16) unsigned char norm_ring[];
+// V weights (or `missing` for each) from channel c, a multiple of V.
+template <int V>
+__device__ __forceinline__ void load_weights(const NormParams& p, const void* w, float missing, int c,
+                                             float2 (&f)[kPairs<V>]) {
+  if (!w) {
+#pragma unroll
+    for (int i = 0; i < kPairs<V>; ++i) f[i] = splat2(missing);
+    return;
+  }
+  if constexpr (V % 4 == 0) {
+    if (p.weight_vectors) {
+      if (p.weight_dtype == 0) {
+        load_channels<V>(static_cast<const float*>(w) + c, f);
+      } else {
+        const unsigned* words = reinterpret_cast<const unsigned*>(static_cast<const __half*>(w) + c);
+        unsigned r[V / 2];
+#pragma unroll
+        for (int i = 0; i < V / 2; i += 2) {
+          const uint2 v = *reinterpret_cast<const uint2*>(words + i);
+          r[i] = v.x;
+          r[i + 1] = v.y;
+        }
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i)
+          f[i] = p.weight_dtype == 1 ? norm_pair(r[i], __half()) : norm_pair(r[i], __nv_bfloat16());
+      }
+      return;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kPairs<V>; ++i) {
+    f[i].x = load_weight(w, p.weight_dtype, c + 2 * i);
+    f[i].y = 2 * i + 1 < V ? load_weight(w, p.weight_dtype, c + 2 * i + 1) : 0.f;
+  }
+}
+
+// f = value(group).x and .y for each of V channels from c.
+template <int V, typename Value>
+__device__ __forceinline__ void by_group(const NormGeometry& g, int c, Value value, float2 (&x)[kPairs<V>],
+                                         float2 (&y)[kPairs<V>]) {
+  int grp = c / g.Cg, end = (grp + 1) * g.Cg;  // one division; the next channels follow
+  float2 now = value(grp);
+  if (end - c >= V) {
+#pragma unroll
+    for (int i = 0; i < kPairs<V>; ++i) {
+      x[i] = splat2(now.x);
+      y[i] = splat2(now.y);
+    }
+    return;
+  }
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    if (c + v == end) {
+      now = value(++grp);
+      end += g.Cg;
+    }
+    (v & 1 ? x[v / 2].y : x[v / 2].x) = now.x;
+    (v & 1 ? y[v / 2].y : y[v / 2].x) = now.y;
+  }
+}
+
 // A thread's channel constants: -mean, the factor rstd w and the shift, from stats(group) = (mean,
 // rstd).
 template <int V, typename Stats>
 __device__ __forceinline__ void norm_constants(const NormParams& p, const NormTile& t, Stats stats,
                                                float2 (&minus)[kPairs<V>], float2 (&a)[kPairs<V>],
                                                float2 (&b)[kPairs<V>]) {
-  const NormGeometry& g = p.g;
-  const int first = t.c0 + t.chan;
-  int grp = first / g.Cg, end = (grp + 1) * g.Cg;  // one division; the next channels follow
+  const int c = t.c0 + t.chan;
+  float2 w[kPairs<V>];
+  load_weights<V>(p, p.weight, 1.f, c, w);
+  load_weights<V>(p, p.bias, 0.f, c, b);
+  by_group<V>(p.g, c, stats, minus, a);
 #pragma unroll
-  for (int v = 0; v < 2 * kPairs<V>; ++v) {
-    const int c = first + v;
-    float mv = 0.f, av = 0.f, bv = 0.f;
-    if (v < V) {
-      if (c == end) {
-        ++grp;
-        end += g.Cg;
-      }
-      const float2 st = stats(grp);
-      mv = -st.x;
-      av = p.weight ? st.y * load_weight(p.weight, p.weight_dtype, c) : st.y;
-      bv = p.bias ? load_weight(p.bias, p.weight_dtype, c) : 0.f;
-    }
-    (v & 1 ? minus[v / 2].y : minus[v / 2].x) = mv;
-    (v & 1 ? a[v / 2].y : a[v / 2].x) = av;
-    (v & 1 ? b[v / 2].y : b[v / 2].x) = bv;
+  for (int i = 0; i < kPairs<V>; ++i) {
+    minus[i] = neg2(minus[i]);
+    a[i] = mul2(a[i], w[i]);
   }
 }
 
@@ -562,7 +613,7 @@ struct NormMoments {
 // then the deviations. put(i, pair) takes the i-th group's. `scratch` has four floats for each
 // thread and channel.
 template <int V, typename Put>
-__device__ __forceinline__ void norm_merge_rows(const NormGeometry& g, const NormTile& t, int64_t pixels,
+__device__ __forceinline__ void norm_merge_rows(const NormGeometry& g, const NormTile& t, int pixels,
                                                 const float2 (&mean)[kPairs<V>], const float2 (&m2)[kPairs<V>],
                                                 float* scratch, Put put) {
   float* sm_mean = scratch;
@@ -574,8 +625,8 @@ __device__ __forceinline__ void norm_merge_rows(const NormGeometry& g, const Nor
     norm_put<V>(sm_m2 + t.row * g.SC + t.chan, m2);
   }
   __syncthreads();
-  const int64_t full = pixels / g.rows;                        // pixels that every row took
-  const int extra = static_cast<int>(pixels - full * g.rows);  // rows that took one more
+  const int full = pixels / g.rows;          // pixels that every row took
+  const int extra = pixels - full * g.rows;  // rows that took one more
   const int width = t.c1 - t.c0;
   const NormColumns columns(width);
   const auto count_of = [&](int row) { return static_cast<float>(full + (row < extra)); };
@@ -672,16 +723,16 @@ __device__ __forceinline__ float2 norm_statistics(const NormGeometry& g, double 
 // ---- the merging launches: a team of kNormThreads / teams threads for each (sample, group) ----
 // Sums of two values over a team (a power of two of threads, a warp at least), in all its
 // threads. Every thread of the block takes part.
-__device__ __forceinline__ double2 team_sum(double a, double b, int team_threads, double2* sm) {
+__device__ __forceinline__ double2 team_sum(double a, double b, int team_shift, double2* sm) {
   a = warp_sum(a);
   b = warp_sum(b);
-  if (team_threads == 32) return make_double2(a, b);
+  if (team_shift == 5) return make_double2(a, b);
   __syncthreads();
   if (threadIdx.x % 32 == 0) sm[threadIdx.x / 32] = make_double2(a, b);
   __syncthreads();
-  const int first = threadIdx.x / team_threads * team_threads / 32;
+  const int warps = 1 << (team_shift - 5), first = threadIdx.x / 32 & ~(warps - 1);
   double2 s = make_double2(0.0, 0.0);
-  for (int i = 0; i < team_threads / 32; ++i) {
+  for (int i = 0; i < warps; ++i) {
     s.x += sm[first + i].x;
     s.y += sm[first + i].y;
   }
@@ -690,17 +741,18 @@ __device__ __forceinline__ double2 team_sum(double a, double b, int team_threads
 
 // Forward: the parts' pairs become the group's statistics and its channels' constants.
 __global__ void __launch_bounds__(kNormThreads) norm_merge_kernel(const __grid_constant__ NormParams p,
-                                                                  int team_threads) {
+                                                                  int team_shift) {
   __shared__ double2 sm[kNormWarps];
   const NormGeometry& g = p.g;
-  const int teams = kNormThreads / team_threads;
-  const int64_t id = static_cast<int64_t>(blockIdx.x) * teams + threadIdx.x / team_threads;
-  const int lane = threadIdx.x % team_threads;
+  const int team_threads = 1 << team_shift;
+  const unsigned id = blockIdx.x * (kNormThreads >> team_shift) + (threadIdx.x >> team_shift);
+  const int lane = threadIdx.x & (team_threads - 1);
   grid_dependency_wait();
   grid_launch_dependents();
   const bool real = id < g.N * g.G;
-  const int64_t n = id / g.G;
-  const int grp = static_cast<int>(id - n * g.G);
+  const unsigned sample = id / static_cast<unsigned>(g.G);
+  const int grp = static_cast<int>(id - sample * g.G);
+  const int64_t n = sample;
   const int c0 = grp * g.Cg, c1 = c0 + g.Cg;
   double ref = 0.0, sum = 0.0, q = 0.0;  // sums of distances from ref, and of squares around it
   if (real) {
@@ -718,7 +770,7 @@ __global__ void __launch_bounds__(kNormThreads) norm_merge_kernel(const __grid_c
       }
     }
   }
-  const double2 total = team_sum(sum, q, team_threads, sm);
+  const double2 total = team_sum(sum, q, team_shift, sm);
   if (!real) return;
   const float2 st = norm_statistics(g, ref, total.x, total.y);
   const float mean = st.x, rstd = st.y;
@@ -833,21 +885,23 @@ __global__ void __launch_bounds__(kNormThreads, kNormResident) norm_grad_sums_ke
                      [&](int c, float2 sums) { partial[c] = sums; });
 }
 
-// Backward: sums over the parts, and the group's two means. `cols` (a power of two, at most 32)
-// channels are summed at a time, by team_threads / cols threads each.
+// Backward: sums over the parts, and the group's two means. `cols` channels (at most 32) are summed
+// at a time, by team_threads / cols threads each.
 __global__ void __launch_bounds__(kNormThreads) norm_grad_merge_kernel(const __grid_constant__ NormParams p,
-                                                                       int team_threads, int cols) {
+                                                                       int team_shift, int col_shift) {
   __shared__ double2 sm[kNormThreads];
   const NormGeometry& g = p.g;
-  const int teams = kNormThreads / team_threads;
-  const int64_t id = static_cast<int64_t>(blockIdx.x) * teams + threadIdx.x / team_threads;
-  const int lane = threadIdx.x % team_threads;
+  const int team_threads = 1 << team_shift;
+  const unsigned id = blockIdx.x * (kNormThreads >> team_shift) + (threadIdx.x >> team_shift);
+  const int lane = threadIdx.x & (team_threads - 1);
   grid_dependency_wait();
   grid_launch_dependents();
   const bool real = id < g.N * g.G;
-  const int64_t n = id / g.G;
-  const int grp = static_cast<int>(id - n * g.G);
-  const int col = lane % cols, sub = lane / cols, subs = team_threads / cols;
+  const unsigned sample = id / static_cast<unsigned>(g.G);
+  const int grp = static_cast<int>(id - sample * g.G);
+  const int64_t n = sample;
+  const int cols = 1 << col_shift, col = lane & (cols - 1), sub = lane >> col_shift;
+  const int subs = team_threads >> col_shift;
   const float mean = real ? p.mean[id] : 0.f, rstd = real ? p.rstd[id] : 0.f;
   double w1 = 0.0, w2 = 0.0;  // sum of w dz and of w dz xhat, kept by the threads with sub == 0
   for (int cb = 0; cb < g.Cg; cb += cols) {
@@ -892,7 +946,7 @@ __global__ void __launch_bounds__(kNormThreads) norm_grad_merge_kernel(const __g
       }
     }
   }
-  const double2 total = team_sum(w1, w2, team_threads, sm);
+  const double2 total = team_sum(w1, w2, team_shift, sm);
   if (!real) return;
   const float k1 = static_cast<float>(rstd * (total.x * g.inv_m));
   const float k2 = static_cast<float>(rstd * (rstd * (total.y * g.inv_m)));
@@ -1033,7 +1087,7 @@ __global__ void __launch_bounds__(kNormThreads) norm_resident_kernel(const __gri
   // pairs: this CTA's, for the cluster to read; stats: the cluster's (mean, rstd) of each group
   float2* pairs = reinterpret_cast<float2*>(scratch + 4 * kNormThreads * V);
   float2* stats = reinterpret_cast<float2*>(scratch);
-  norm_merge_rows<V>(g, t, g.base + (t.s < g.extra), moments.mean, moments.m2, scratch,
+  norm_merge_rows<V>(g, t, g.run_pixels(t.s), moments.mean, moments.m2, scratch,
                      [&](int i, float2 pair) { pairs[i] = pair; });
   const cg::cluster_group cluster = cg::this_cluster();
   cluster.sync();
@@ -1042,7 +1096,7 @@ __global__ void __launch_bounds__(kNormThreads) norm_resident_kernel(const __gri
     double sum = 0.0, q = 0.0;
     for (int r = 0; r < g.S; ++r) {
       const float2 v = cluster.map_shared_rank(pairs, r)[i];
-      const double cnt = static_cast<double>(g.base + (r < g.extra)) * g.Cg;
+      const double cnt = static_cast<double>(g.run_pixels(r)) * g.Cg;
       const double d = v.x - ref;
       sum = fma(cnt, d, sum);
       q += fma(cnt * d, d, static_cast<double>(v.y));
@@ -1154,20 +1208,7 @@ __global__ void __launch_bounds__(kNormThreads) norm_grad_resident_kernel(const 
   __syncthreads();
   if (!t.active) return;
   float2 k1[N], k2[N];
-  {
-    const int first = t.c0 + t.chan;
-    int grp = first / g.Cg, end = (grp + 1) * g.Cg;
-#pragma unroll
-    for (int v = 0; v < 2 * N; ++v) {
-      if (v < V && first + v == end) {
-        ++grp;
-        end += g.Cg;
-      }
-      const float2 k = means[grp - t.g0];
-      (v & 1 ? k1[v / 2].y : k1[v / 2].x) = k.x;
-      (v & 1 ? k2[v / 2].y : k2[v / 2].x) = k.y;
-    }
-  }
+  by_group<V>(g, t.c0 + t.chan, [&](int grp) { return means[grp - t.g0]; }, k1, k2);
   T* dx = static_cast<T*>(p.out) + walk.first;
   for (int i = 0; i < walk.count; ++i, dx += walk.stride) {
     float2 f[N], d[N];
