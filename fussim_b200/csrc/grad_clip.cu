@@ -25,6 +25,8 @@ using fssim_host::NvtxRange;
 // a launch may carry).
 constexpr int kFew = 96;
 constexpr int kMany = 832;
+// Units of a CTA of the clipping, in large calls.
+constexpr int64_t kCutUnits = 16;
 // Bytes of the gradients that are to stay in L2 from the norm to the clipping, of larger ones.
 constexpr double kKeptBytes = 80 << 20;
 static_assert(sizeof(ClipTable<kMany>) <= 32764, "kernel parameters are limited to 32764 bytes");
@@ -54,6 +56,12 @@ int launch(void (*k)(KA...), unsigned grid, size_t smem, cudaStream_t stream, co
 
 unsigned grid_for(int64_t units) {
   return static_cast<unsigned>(units < kClipMaxCtas ? units : kClipMaxCtas);
+}
+
+// CTAs of the clipping for each range of the norm's pass.
+int cuts_of(int64_t units) {
+  const int64_t cuts = units / (grid_for(units) * kCutUnits);
+  return static_cast<int>(cuts < 1 ? 1 : cuts < 4096 ? cuts : 4096);
 }
 
 int64_t units_of(int64_t size) { return (size + kClipUnit - 1) / kClipUnit; }
@@ -134,8 +142,8 @@ int allow_ring() {
 }
 
 template <int K>
-int launch_cut(const fssim_grad_clip_args& a, const Cut& c, bool clip, int partials, int first, float keep,
-               cudaStream_t stream) {
+int launch_cut(const fssim_grad_clip_args& a, const Cut& c, bool clip, bool summed, int partials, int first,
+               float keep, cudaStream_t stream) {
   const std::unique_ptr<ClipTable<K>> t(new ClipTable<K>);
   int r = 0;
   int64_t unit = 0;
@@ -152,21 +160,26 @@ int launch_cut(const fssim_grad_clip_args& a, const Cut& c, bool clip, int parti
   }
   t->unit0[r] = unit;
   t->count = r;
-  t->partials = static_cast<double*>(a.workspace);
-  t->num_partials = partials;
+  // (the sum of the partial sums follows them)
+  t->partials = static_cast<double*>(a.workspace) + (clip && summed ? partials : 0);
+  t->num_partials = clip && summed ? 1 : partials;
   t->first_partial = first;
-  t->norm = clip && first == 0 ? a.norm : nullptr;
+  t->norm = clip && !summed && first == 0 ? a.norm : nullptr;
   t->max_norm = a.max_norm;
   t->keep = keep;
-  const unsigned grid = grid_for(c.units);
+  const unsigned ranges = grid_for(c.units);
+  t->ranges = static_cast<int>(ranges);
+  t->cuts = summed ? cuts_of(c.units) : 1;
   const int st = allow_ring<K>();
   if (st) return st;
-  return clip ? launch(fssim::grad_clip_kernel<K>, grid, fssim::kClipRingBytes, stream, "gradient clipping launch", *t)
-              : launch(fssim::grad_squares_kernel<K>, grid, fssim::kClipRingBytes, stream, "gradient norm launch", *t);
+  if (!clip)
+    return launch(fssim::grad_squares_kernel<K>, ranges, fssim::kClipRingBytes, stream, "gradient norm launch", *t);
+  return launch(fssim::grad_clip_kernel<K>, ranges * static_cast<unsigned>(t->cuts), fssim::kClipRingBytes, stream,
+                "gradient clipping launch", *t);
 }
 
 // One pass over all tensors: the partial sums (clip == false) or the scaling.
-int pass(const fssim_grad_clip_args& a, bool clip, int partials, cudaStream_t stream) {
+int pass(const fssim_grad_clip_args& a, bool clip, bool summed, int partials, cudaStream_t stream) {
   double bytes = 0.0;
   for (int64_t i = 0; i < a.count; ++i) bytes += static_cast<double>(a.sizes[i]) * elem_size(a.dtypes[i]);
   const float keep = bytes <= kKeptBytes ? 1.f : static_cast<float>(kKeptBytes / bytes);
@@ -175,8 +188,8 @@ int pass(const fssim_grad_clip_args& a, bool clip, int partials, cudaStream_t st
     const Cut c = next_cut(a, i);
     i = c.end;
     if (c.runs == 0) continue;
-    const int st = c.runs <= kFew ? launch_cut<kFew>(a, c, clip, partials, first, keep, stream)
-                                  : launch_cut<kMany>(a, c, clip, partials, first, keep, stream);
+    const int st = c.runs <= kFew ? launch_cut<kFew>(a, c, clip, summed, partials, first, keep, stream)
+                                  : launch_cut<kMany>(a, c, clip, summed, partials, first, keep, stream);
     if (st) return st;
     first += static_cast<int>(grid_for(c.units));
   }
@@ -191,11 +204,25 @@ int run(const fssim_grad_clip_args* a, bool clip, cudaStream_t stream) {
     const cudaError_t e = cudaMemsetAsync(a->norm, 0, sizeof(float), stream);
     return e == cudaSuccess ? FSSIM_OK : fail(FSSIM_ERR_CUDA, cudaGetErrorString(e));
   }
-  st = pass(*a, false, partials, stream);
+  // Large calls add the partial sums up in a launch of their own, so that the clipping can come in
+  // many short CTAs, which the SMs take in their order, without each adding them up again.
+  // (Not in place, where the usual call finds the norm within the limit and has nothing to do.)
+  bool summed = !clip, moves = false;
+  for (int64_t i = 0; i < a->count && clip && !moves; ++i) moves = a->sizes[i] > 0 && a->outs[i] != a->grads[i];
+  for (int64_t i = 0; i < a->count && moves && !summed;) {
+    const Cut c = next_cut(*a, i);
+    summed = cuts_of(c.units) > 1;
+    i = c.end;
+  }
+  st = pass(*a, false, summed, partials, stream);
   if (st) return st;
-  if (clip) return pass(*a, true, partials, stream);
-  return launch(fssim::grad_norm_kernel, 1u, 0, stream, "gradient norm sum launch",
-                static_cast<const double*>(a->workspace), partials, a->norm);
+  if (summed) {
+    double* sums = static_cast<double*>(a->workspace);
+    st = launch(fssim::grad_norm_kernel, 1u, 0, stream, "gradient norm sum launch",
+                static_cast<const double*>(sums), partials, sums + partials, a->norm);
+    if (st || !clip) return st;
+  }
+  return pass(*a, true, summed, partials, stream);
 }
 
 // No exception crosses the C boundary.
@@ -215,7 +242,8 @@ extern "C" {
 
 size_t fssim_grad_clip_workspace_bytes(const fssim_grad_clip_args* a) {
   if (!a || a->count <= 0 || !a->sizes) return 0;
-  return sizeof(double) * static_cast<size_t>(total_partials(*a));
+  const size_t partials = static_cast<size_t>(total_partials(*a));
+  return partials ? sizeof(double) * (partials + 1) : 0;
 }
 
 int fssim_grad_norm(const fssim_grad_clip_args* a, fssim_stream_t stream) {

@@ -45,11 +45,13 @@ struct ClipTable {
   unsigned char src_dtype[K];
   unsigned char dst_dtype[K];
   int count;
-  double* partials;       // of the whole call
+  double* partials;       // of the whole call, or their sum
   int num_partials;       // of the whole call
   int first_partial;      // of this launch's CTAs
   float* norm;            // written by the launch that has it set
   float max_norm;
+  int ranges;             // CTAs of the norm's pass, each with a range of units
+  int cuts;               // CTAs of the clipping for each range
   float keep;             // share of the gradients that may stay in L2 from the norm to the clipping
 };
 
@@ -310,33 +312,41 @@ __global__ void __launch_bounds__(kClipThreads, kClipResident)
   if (threadIdx.x == 0) t.partials[t.first_partial + blockIdx.x] = acc;
 }
 
-__device__ __forceinline__ double grad_norm_of(const double* partials, int n) {
+__device__ __forceinline__ double grad_sum_of(const double* partials, int n) {
   double v = 0.0;
   for (int i = threadIdx.x; i < n; i += kClipThreads) v += partials[i];
-  return sqrt(clip_block_sum(v));
+  return clip_block_sum(v);
 }
 
-__global__ void __launch_bounds__(kClipThreads) grad_norm_kernel(const double* partials, int n, float* norm) {
+// The partial sums' sum, in `total` (if given), and its root.
+__global__ void __launch_bounds__(kClipThreads) grad_norm_kernel(const double* partials, int n, double* total,
+                                                                 float* norm) {
   grid_dependency_wait();
   grid_launch_dependents();
-  const double v = grad_norm_of(partials, n);
-  if (threadIdx.x == 0) *norm = static_cast<float>(v);
+  const double v = grad_sum_of(partials, n);
+  if (threadIdx.x == 0) {
+    if (total) *total = v;
+    *norm = static_cast<float>(sqrt(v));
+  }
 }
 
-// The second read goes through the CTA's range from its end, which the norm's pass read last
-// and L2 still holds.
+// The second read begins at the ends of the norm's pass's ranges, which that pass read last and L2
+// still holds: a range is cut into `cuts` pieces, and the CTAs take the last piece of every range
+// first.
 template <int K>
 __global__ void __launch_bounds__(kClipThreads, kClipResident)
     grad_clip_kernel(const __grid_constant__ ClipTable<K> t) {
   grid_dependency_wait();
   grid_launch_dependents();
-  const double norm = grad_norm_of(t.partials, t.num_partials);
+  const double norm = sqrt(grad_sum_of(t.partials, t.num_partials));
   if (t.norm && blockIdx.x == 0 && threadIdx.x == 0) *t.norm = static_cast<float>(norm);
   const double ratio = static_cast<double>(t.max_norm) / (norm + 1e-6);
   const ClipFactor coef(ratio >= 1.0 ? 1.0 : ratio);  // a NaN norm gives NaN
   const uint64_t policy = ClipPolicy(t.keep < 1.f).pass;
   const int64_t units = t.unit0[t.count];
-  clip_walk<true>(t, clip_range(units, blockIdx.x, gridDim.x), clip_range(units, blockIdx.x + 1, gridDim.x),
+  const int cut = t.cuts - 1 - blockIdx.x / t.ranges, range = blockIdx.x % t.ranges;
+  const int64_t u0 = clip_range(units, range, t.ranges), n = clip_range(units, range + 1, t.ranges) - u0;
+  clip_walk<true>(t, u0 + clip_range(n, cut, t.cuts), u0 + clip_range(n, cut + 1, t.cuts),
                   [&](int r, int64_t b, int64_t e) {
     if (ratio >= 1.0 && t.src[r] == t.dst[r]) return;  // in place and below the limit: as it was
     const void* s = t.src[r];

@@ -232,52 +232,70 @@ at::Tensor group_norm_act(const at::Tensor& x, int64_t groups, const OptTensor& 
 }
 
 // ---- gradient norm and clipping ----
+// Models have hundreds of gradients and a call's device time is tens of microseconds, so the
+// tensors are read where the caller's list holds them (no copies of their handles) and in one pass.
+using Refs = std::vector<const at::Tensor*>;
 
-// The memory of a dense tensor, and where the tensor stands in the call.
+const at::Tensor& tensor_of(py::handle h, const char* what, size_t index) {
+  if (!THPVariable_Check(h.ptr()))
+    throw py::type_error(std::string(what) + " must be tensors, but that at index " + std::to_string(index) +
+                         " is not");
+  return THPVariable_Unpack(h.ptr());
+}
+
+Refs refs_of(const py::list& list, const char* what) {
+  Refs refs;
+  refs.reserve(list.size());
+  for (size_t i = 0; i < list.size(); ++i) refs.push_back(&tensor_of(PyList_GET_ITEM(list.ptr(), i), what, i));
+  return refs;
+}
+
+void check_grads(const Refs& grads, const char* what) {
+  for (size_t i = 0; i < grads.size(); ++i) {
+    const at::Tensor& g = *grads[i];
+    const auto at = [&] { return " at index " + std::to_string(i) + " "; };
+    if (g.layout() != at::kStrided) value_error("gradients must be dense tensors, but that" + at() + "is not");
+    if (!known_type(g.scalar_type()))
+      value_error("gradients must be float32, float16 or bfloat16, but that" + at() + "is " +
+                  type_text(g.scalar_type()));
+    if (g.device() != grads[0]->device())
+      runtime_error("gradients must be on one device.\nfirst: " + grads[0]->device().str() + "," + at() +
+                    g.device().str());
+  }
+  require_cuda(what);
+  if (!grads.empty() && !grads[0]->is_cuda())
+    runtime_error("gradients must be on a CUDA device, but got device: " + grads[0]->device().str());
+}
+
+// The memory of a tensor, and where the tensor stands in the call.
 struct Span {
   uintptr_t begin, end;
   int64_t index;
   bool out;
 };
 
-Span span_of(const at::Tensor& t, int64_t index, bool out) {
-  const uintptr_t p = reinterpret_cast<uintptr_t>(t.data_ptr());
-  return {p, p + t.numel() * t.element_size(), index, out};
-}
-
 // Refuses outputs that overlap each other or a gradient (but for outs[i] being grads[i]): two
-// CTAs would write the same numbers, or read what another has already scaled. Tensors that
-// do not fill their memory are copied before and after the kernels, which touch the copies
-// alone; of those it is enough that no output is given twice or overlaps itself.
-void check_overlap(const std::vector<at::Tensor>& grads, const std::vector<at::Tensor>& outs) {
-  std::vector<Span> spans, others;
-  spans.reserve(2 * grads.size());
-  const auto refuse = [](int64_t index) {
-    throw std::invalid_argument(
-        "tensors that are written must not overlap themselves, each other or another gradient "
-        "(the same tensor twice, or views of the same memory; at index " +
-        std::to_string(index) + ")");
-  };
-  for (size_t i = 0; i < grads.size(); ++i) {
-    if (grads[i].numel() == 0) continue;
-    const Span o = span_of(outs[i], static_cast<int64_t>(i), true);
-    const Span g = span_of(grads[i], static_cast<int64_t>(i), false);
-    const bool o_dense = outs[i].is_non_overlapping_and_dense();
-    const bool in_place = g.begin == o.begin && g.end == o.end && grads[i].strides() == outs[i].strides();
-    if (o_dense) spans.push_back(o);
-    else if (at::has_internal_overlap(outs[i]) == at::MemOverlap::Yes) refuse(o.index);
-    else others.push_back(o);
-    if (!in_place && grads[i].is_non_overlapping_and_dense()) spans.push_back(g);
-  }
+// CTAs would write the same numbers, or read what another has already scaled. Tensors that do
+// not fill their memory (`others`) are copied before and after the kernels, which touch the
+// copies alone; of those it is enough that no output is given twice or overlaps itself.
+void check_overlap(std::vector<Span>& spans, std::vector<Span>& others) {
   const auto by_begin = [](const Span& a, const Span& b) { return a.begin < b.begin; };
-  std::sort(spans.begin(), spans.end(), by_begin);
+  const auto sort = [&](std::vector<Span>& v) {
+    if (!std::is_sorted(v.begin(), v.end(), by_begin)) std::sort(v.begin(), v.end(), by_begin);
+  };
+  const auto refuse = [](int64_t index) {
+    value_error("tensors that are written must not overlap themselves, each other or another gradient "
+                "(the same tensor twice, or views of the same memory; at index " +
+                std::to_string(index) + ")");
+  };
+  sort(spans);
   uintptr_t any_end = 0, out_end = 0;  // how far the spans so far reach
   for (const Span& s : spans) {
     if (s.begin < (s.out ? any_end : out_end)) refuse(s.index);
     any_end = std::max(any_end, s.end);
     if (s.out) out_end = std::max(out_end, s.end);
   }
-  std::sort(others.begin(), others.end(), by_begin);
+  sort(others);
   for (size_t i = 1; i < others.size(); ++i)
     if (others[i].begin == others[i - 1].begin) refuse(others[i].index);
 }
@@ -296,12 +314,12 @@ struct ClipArrays {
     dtypes.reserve(n);
     out_dtypes.reserve(n);
   }
-  void add(const at::Tensor& g, const at::Tensor& o) {
-    grads.push_back(g.data_ptr());
-    outs.push_back(o.data_ptr());
-    sizes.push_back(g.numel());
-    dtypes.push_back(dtype_code(g.scalar_type()));
-    out_dtypes.push_back(dtype_code(o.scalar_type()));
+  void add(const void* g, void* o, int64_t size, int32_t dtype, int32_t out_dtype) {
+    grads.push_back(g);
+    outs.push_back(o);
+    sizes.push_back(size);
+    dtypes.push_back(dtype);
+    out_dtypes.push_back(out_dtype);
   }
   fssim_grad_clip_args& fill(float max_norm, float* norm) {
     args.count = static_cast<int64_t>(grads.size());
@@ -317,81 +335,86 @@ struct ClipArrays {
   }
 };
 
-using Tensors = std::vector<at::Tensor>;
-
-void check_grads(const Tensors& grads, const char* what) {
-  for (size_t i = 0; i < grads.size(); ++i) {
-    const at::Tensor& g = grads[i];
-    const auto at = [&] { return " at index " + std::to_string(i) + " "; };
-    if (!g.defined()) value_error("the gradient" + at() + "is missing");
-    if (g.layout() != at::kStrided) value_error("gradients must be dense tensors, but that" + at() + "is not");
-    if (!known_type(g.scalar_type()))
-      value_error("gradients must be float32, float16 or bfloat16, but that" + at() + "is " +
-                  type_text(g.scalar_type()));
-    if (g.device() != grads[0].device())
-      runtime_error("gradients must be on one device.\nfirst: " + grads[0].device().str() + "," + at() +
-                    g.device().str());
-  }
-  require_cuda(what);
-  if (!grads.empty() && !grads[0].is_cuda())
-    runtime_error("gradients must be on a CUDA device, but got device: " + grads[0].device().str());
-}
-
 at::Tensor zero_norm() {
   return at::zeros({}, at::TensorOptions().dtype(at::kFloat).device(at::kCUDA));
 }
 
 // Tensors whose numbers fill their memory are taken as they lie; others go through a dense copy.
-at::Tensor norm_of(const Tensors& grads) {
+at::Tensor norm_of(const Refs& grads) {
   const at::NoGradGuard no_grad;
-  const at::cuda::OptionalCUDAGuard guard(grads[0].device());
-  at::Tensor norm = at::empty({}, grads[0].options().dtype(at::kFloat));
+  const at::cuda::OptionalCUDAGuard guard(grads[0]->device());
+  at::Tensor norm = at::empty({}, grads[0]->options().dtype(at::kFloat));
   ClipArrays arrays(grads.size());
-  Tensors held;
-  for (const auto& g : grads) {
-    if (!g.is_non_overlapping_and_dense()) held.push_back(g.contiguous());
-    const at::Tensor& d = g.is_non_overlapping_and_dense() ? g : held.back();
-    arrays.add(d, d);
+  std::vector<at::Tensor> held;
+  for (const at::Tensor* g : grads) {
+    const bool dense = g->is_non_overlapping_and_dense();
+    if (!dense) held.push_back(g->contiguous());
+    void* data = (dense ? *g : held.back()).data_ptr();
+    const int32_t dtype = dtype_code(g->scalar_type());
+    arrays.add(data, data, g->numel(), dtype, dtype);
   }
   fssim_grad_clip_args& a = arrays.fill(0.f, norm.data_ptr<float>());
-  at::Tensor ws = workspace(a.workspace_bytes, grads[0]);
+  at::Tensor ws = workspace(a.workspace_bytes, *grads[0]);
   a.workspace = ws.data_ptr();
   check_status(fssim_grad_norm(&a, current_stream()));
   return norm;
 }
 
-at::Tensor clip_into(const Tensors& grads, const Tensors& outs, double max_norm, bool error_if_nonfinite) {
+at::Tensor clip_into(const Refs& grads, const Refs& outs, double max_norm, bool error_if_nonfinite) {
   const at::NoGradGuard no_grad;
-  const at::cuda::OptionalCUDAGuard guard(grads[0].device());
-  check_overlap(grads, outs);
+  const at::cuda::OptionalCUDAGuard guard(grads[0]->device());
+  const size_t n = grads.size();
+  ClipArrays arrays(n);
+  std::vector<Span> spans, others;
+  spans.reserve(n);
+  std::vector<at::Tensor> held;                         // dense stand-ins of gradients
+  std::vector<std::pair<size_t, at::Tensor>> copy_back;  // (index of an output, its stand-in)
+  for (size_t i = 0; i < n; ++i) {
+    const at::Tensor &g = *grads[i], &o = *outs[i];
+    const int64_t size = g.numel(), index = static_cast<int64_t>(i);
+    const int32_t dtype = dtype_code(g.scalar_type());
+    void* const gp = g.data_ptr();
+    const bool g_dense = g.is_non_overlapping_and_dense();
+    const bool same = &g == &o || (o.data_ptr() == gp && o.dtype() == g.dtype() && o.strides() == g.strides());
+    void* const op = same ? gp : o.data_ptr();
+    const int32_t out_dtype = same ? dtype : dtype_code(o.scalar_type());
+    const bool o_dense = same ? g_dense : o.is_non_overlapping_and_dense();
+    if (size) {
+      const uintptr_t gb = reinterpret_cast<uintptr_t>(gp), ob = reinterpret_cast<uintptr_t>(op);
+      if (o_dense) spans.push_back({ob, ob + size * o.element_size(), index, true});
+      else if (at::has_internal_overlap(o) == at::MemOverlap::Yes) others.push_back({ob, ob, index, true});
+      if (!o_dense) others.push_back({ob, ob, index, true});  // (twice where it overlaps itself: refused)
+      if (!same && g_dense) spans.push_back({gb, gb + size * g.element_size(), index, false});
+    }
+    if (same ? g_dense
+             : (g.is_contiguous() && o.is_contiguous()) || (g_dense && g.strides() == o.strides())) {
+      arrays.add(gp, op, size, dtype, out_dtype);
+    } else {
+      arrays.add(nullptr, nullptr, size, dtype, out_dtype);
+      copy_back.emplace_back(i, at::Tensor());
+    }
+  }
+  check_overlap(spans, others);
   if (error_if_nonfinite) {
     const double norm = norm_of(grads).item<double>();
     if (!std::isfinite(norm))
       runtime_error("the gradients' norm is " + std::to_string(norm) +
                     "; nothing was clipped. Pass error_if_nonfinite=False to clip all the same");
   }
-  at::Tensor norm = at::empty({}, grads[0].options().dtype(at::kFloat));
-  ClipArrays arrays(grads.size());
-  Tensors held;                                              // dense stand-ins of gradients
-  std::vector<std::pair<at::Tensor, at::Tensor>> copy_back;  // (output, its stand-in)
-  for (size_t i = 0; i < grads.size(); ++i) {
-    const at::Tensor &g = grads[i], &o = outs[i];
-    if ((g.is_contiguous() && o.is_contiguous()) ||
-        (g.is_non_overlapping_and_dense() && g.strides() == o.strides())) {
-      arrays.add(g, o);
-      continue;
-    }
-    held.push_back(g.contiguous());
-    copy_back.emplace_back(o, at::empty(o.sizes(), o.options(), at::MemoryFormat::Contiguous));
-    arrays.add(held.back(), copy_back.back().second);
+  for (auto& [i, d] : copy_back) {
+    held.push_back(grads[i]->contiguous());
+    d = at::empty(outs[i]->sizes(), outs[i]->options(), at::MemoryFormat::Contiguous);
+    arrays.grads[i] = held.back().data_ptr();
+    arrays.outs[i] = d.data_ptr();
   }
+  at::Tensor norm = at::empty({}, grads[0]->options().dtype(at::kFloat));
   fssim_grad_clip_args& a = arrays.fill(static_cast<float>(max_norm), norm.data_ptr<float>());
-  at::Tensor ws = workspace(a.workspace_bytes, grads[0]);
+  at::Tensor ws = workspace(a.workspace_bytes, *grads[0]);
   a.workspace = ws.data_ptr();
   // the kernels write past autograd's sight: a graph that saved an output has to notice
-  for (const auto& o : outs) o.unsafeGetTensorImpl()->bump_version();
+  for (const at::Tensor* o : outs) o->unsafeGetTensorImpl()->bump_version();
   check_status(fssim_grad_clip(&a, current_stream()));
-  for (auto& [o, d] : copy_back) o.copy_(d);
+  for (auto& [i, d] : copy_back) outs[i]->copy_(d);
   return norm;
 }
 
@@ -399,48 +422,51 @@ void check_max_norm(double max_norm) {
   if (!(max_norm >= 0.0)) value_error("max_norm must not be negative, got " + std::to_string(max_norm));
 }
 
-at::Tensor grad_norm(const Tensors& grads) {
+at::Tensor grad_norm(const py::list& list) {
+  const Refs grads = refs_of(list, "gradients");
   check_grads(grads, "grad_norm");
   return grads.empty() ? zero_norm() : norm_of(grads);
 }
 
-std::tuple<Tensors, at::Tensor> clip_grad_norm(const Tensors& grads, double max_norm,
-                                               const std::optional<Tensors>& out,
-                                               bool error_if_nonfinite) {
+std::tuple<py::list, at::Tensor> clip_grad_norm(const py::list& list, double max_norm,
+                                                const std::optional<py::list>& out, bool error_if_nonfinite) {
   check_max_norm(max_norm);
-  if (out.has_value() && out->size() != grads.size())
+  if (out.has_value() && out->size() != list.size())
     value_error("out must have a tensor for each gradient, got " + std::to_string(out->size()) + " for " +
-                std::to_string(grads.size()));
+                std::to_string(list.size()));
+  const Refs grads = refs_of(list, "gradients");
   check_grads(grads, "clip_grad_norm");
-  if (grads.empty()) return {Tensors(), zero_norm()};
-  Tensors outs;
+  if (grads.empty()) return {py::list(), zero_norm()};
+  py::list result;
   if (out.has_value()) {
-    outs = *out;
-    for (size_t i = 0; i < outs.size(); ++i) {
-      const at::Tensor &g = grads[i], &o = outs[i];
-      const std::string name = "out[" + std::to_string(i) + "]";
-      if (o.sizes() != g.sizes())
-        value_error(name + " must have shape " + shape_text(g) + ", got " + shape_text(o));
-      if (o.scalar_type() != g.scalar_type() && o.scalar_type() != at::kFloat)
-        value_error(name + " must be " + type_text(g.scalar_type()) + " or float32, got " +
-                    type_text(o.scalar_type()));
-      if (o.device() != g.device() || o.layout() != at::kStrided)
-        runtime_error(name + " must be a dense tensor on " + g.device().str());
-    }
+    result = *out;
   } else {
-    outs.reserve(grads.size());
-    for (const auto& g : grads) outs.push_back(at::empty_like(g, g.options().requires_grad(false)));
+    for (const at::Tensor* g : grads)
+      result.append(py::cast(at::empty_like(*g, g->options().requires_grad(false))));
+  }
+  const Refs outs = refs_of(result, "outputs");
+  for (size_t i = 0; i < outs.size() && out.has_value(); ++i) {
+    const at::Tensor &g = *grads[i], &o = *outs[i];
+    const auto name = [&] { return "out[" + std::to_string(i) + "]"; };
+    if (o.sizes() != g.sizes()) value_error(name() + " must have shape " + shape_text(g) + ", got " + shape_text(o));
+    if (o.scalar_type() != g.scalar_type() && o.scalar_type() != at::kFloat)
+      value_error(name() + " must be " + type_text(g.scalar_type()) + " or float32, got " +
+                  type_text(o.scalar_type()));
+    if (o.device() != g.device() || o.layout() != at::kStrided)
+      runtime_error(name() + " must be a dense tensor on " + g.device().str());
   }
   at::Tensor norm = clip_into(grads, outs, max_norm, error_if_nonfinite);
-  return {std::move(outs), norm};
+  return {std::move(result), norm};
 }
 
-at::Tensor clip_grad_norm_(const Tensors& parameters, double max_norm, bool error_if_nonfinite) {
+at::Tensor clip_grad_norm_(const py::list& parameters, double max_norm, bool error_if_nonfinite) {
   check_max_norm(max_norm);
-  Tensors grads;
+  Refs grads;
   grads.reserve(parameters.size());
-  for (const auto& p : parameters)
-    if (p.grad().defined()) grads.push_back(p.grad());
+  for (size_t i = 0; i < parameters.size(); ++i) {
+    const at::Tensor& g = tensor_of(PyList_GET_ITEM(parameters.ptr(), i), "parameters", i).grad();
+    if (g.defined()) grads.push_back(&g);
+  }
   check_grads(grads, "clip_grad_norm_");
   return grads.empty() ? zero_norm() : clip_into(grads, grads, max_norm, error_if_nonfinite);
 }
