@@ -123,7 +123,7 @@ int check(const fssim_grad_clip_args* a, bool clip) {
   return FSSIM_OK;
 }
 
-// Opts the two passes in to their ring of shared memory, once for each device.
+// Opts the clipping in to its ring of shared memory, once for each device.
 template <int K>
 int allow_ring() {
   static std::atomic<bool> done[64];
@@ -131,11 +131,8 @@ int allow_ring() {
   cudaError_t e = cudaGetDevice(&dev);
   if (e == cudaSuccess && (dev < 0 || dev >= 64)) return fail(FSSIM_ERR_CUDA, "device ordinal out of range");
   if (e == cudaSuccess && !done[dev].load(std::memory_order_acquire)) {
-    e = cudaFuncSetAttribute(fssim::grad_squares_kernel<K>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    e = cudaFuncSetAttribute(fssim::grad_clip_kernel<K>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              fssim::kClipRingBytes);
-    if (e == cudaSuccess)
-      e = cudaFuncSetAttribute(fssim::grad_clip_kernel<K>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                               fssim::kClipRingBytes);
     if (e == cudaSuccess) done[dev].store(true, std::memory_order_release);
   }
   return e == cudaSuccess ? FSSIM_OK : fail(FSSIM_ERR_CUDA, cudaGetErrorString(e));
@@ -173,7 +170,7 @@ int launch_cut(const fssim_grad_clip_args& a, const Cut& c, bool clip, bool summ
   const int st = allow_ring<K>();
   if (st) return st;
   if (!clip)
-    return launch(fssim::grad_squares_kernel<K>, ranges, fssim::kClipRingBytes, stream, "gradient norm launch", *t);
+    return launch(fssim::grad_squares_kernel<K>, ranges, 0, stream, "gradient norm launch", *t);
   return launch(fssim::grad_clip_kernel<K>, ranges * static_cast<unsigned>(t->cuts), fssim::kClipRingBytes, stream,
                 "gradient clipping launch", *t);
 }

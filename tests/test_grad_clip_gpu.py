@@ -1,8 +1,9 @@
 """grad_norm, clip_grad_norm and clip_grad_norm_ against their definition in 64 bits.
 
-Tolerances. u = 2^-24. Squares of eight numbers are summed in FP32 (all positive: at most 4 u
-relative), everything else in FP64, so the norm before its rounding is off by 2 u and by 3 u
-after; the factor by 4 u, and a scaled number by that and half a step of its type.
+Tolerances. u = 2^-24. Squares of up to 32 numbers are summed in FP32 as a tree with at most six
+roundings on the way of any term (all positive: 6 u relative), everything else in FP64, so the
+norm before its rounding is off by 3 u and by 4 u after; the factor by 4 u (3 u and its own
+rounding), a scaled number by 5 u (the product's) and half a step of its type.
 """
 
 import math
@@ -31,10 +32,10 @@ def exact(grads, max_norm):
 def check(outs, norm, grads, max_norm):
     want, coef = exact(grads, max_norm)
     assert norm.dtype == F32 and norm.shape == () and norm.is_cuda
-    assert abs(norm.item() - want) <= 3 * U * want
+    assert abs(norm.item() - want) <= 4 * U * want
     for o, g in zip(outs, grads):
         ref = g.double() * coef
-        tol = 4 * U * ref.abs() + half_step(o.dtype, ref)
+        tol = 5 * U * ref.abs() + half_step(o.dtype, ref)
         assert ((o.double() - ref).abs() <= tol).all()
 
 
@@ -60,7 +61,7 @@ SIZES = {
 def test_values(sizes, dtypes):
     grads = tensors(SIZES[sizes], dtypes, 3)
     norm, _ = exact(grads, 1.0)
-    assert abs(fb.grad_norm(grads).item() - norm) <= 3 * U * norm
+    assert abs(fb.grad_norm(grads).item() - norm) <= 4 * U * norm
     for limit in (0.0, 0.25 * norm, 4 * norm, float("inf")):
         kept = [g.clone() for g in grads]
         out, got = fb.clip_grad_norm(grads, limit)                      # new tensors
@@ -275,13 +276,13 @@ def test_more_than_two_to_the_31_numbers():
     g[-1] = 64.0
     want = math.sqrt(0.25 * (n - 1) + 4096.0)
     norm = fb.grad_norm([g]).item()
-    assert abs(norm - want) <= 3 * U * want
+    assert abs(norm - want) <= 4 * U * want
     _, got = fb.clip_grad_norm([g], 1.0, out=[g])
     assert got.item() == norm
     coef = 1.0 / (want + 1e-6)
     for at, v in ((0, 0.5), (n - 2, 0.5), (n - 1, 64.0), (2 ** 31 + 1, 0.5)):
         ref = torch.tensor(v * coef, dtype=torch.float64)
-        assert abs(g[at].double().item() - ref.item()) <= (half_step(BF16, ref) + 4 * U * ref).item()
+        assert abs(g[at].double().item() - ref.item()) <= (half_step(BF16, ref) + 5 * U * ref).item()
     assert (g[:-1] == g[0]).all()
 
 

@@ -145,6 +145,15 @@ SHAPES = [  # (N, C, H, W), groups
     ((700, 8, 3, 3), 4),        # many samples
     ((1, 16, 300, 301), 4),     # many parts
     ((1, 128, 1, 1000), 32),
+    # larger: two passes over tiles and parts, their last ones short
+    ((2, 320, 67, 121), 32),
+    ((1, 48, 130, 199), 16),    # groups of three
+    ((3, 2056, 20, 21), 8),     # two slices
+    ((1, 1283, 40, 30), 1),     # a group over six slices
+    ((1, 12, 300, 251), 3),
+    ((40, 64, 40, 41), 8),
+    ((600, 32, 20, 20), 4),     # more samples than a wave of CTAs
+    ((1, 1024, 9, 8), 32),
 ]
 
 
@@ -432,3 +441,32 @@ def test_a_second_device():
     want = grads(x, 4, w, b, 1e-5, "silu", dy)
     got = grads(*(t.to("cuda:1") if torch.is_tensor(t) else t for t in (x, 4, w, b, 1e-5, "silu", dy)))
     assert all(torch.equal(p.to("cuda:0"), q) for p, q in zip(got, want))
+
+
+def test_c_entry_point_in_place():
+    """The C call with y == x, a strided batch of two calls on one workspace, and mean and rstd."""
+    import ctypes
+
+    from .test_training_cpu import LIB, ForwardArgs
+
+    lib = ctypes.CDLL(LIB)
+    lib.fssim_group_norm_forward_workspace_bytes.restype = ctypes.c_size_t
+    for shape in ((2, 32, 16, 16), (2, 32, 300, 301)):  # the resident kernel, and the passes
+        x, _, w, b = make(shape, F16, F32, 50)
+        want = fb.group_norm_act(x, 4, w, b)
+        n, c, h, wd = shape
+        _, xhat, _, rs = plain(x, 4, w, b, 1e-5, None)
+        mean, rstd = torch.empty(2, 4, device="cuda"), torch.empty(2, 4, device="cuda")
+        args = ForwardArgs(dtype=1, weight_dtype=0, activation=1, N=n, P=h * wd, C=c, groups=4,
+                           eps=1e-5, x=x.data_ptr(), y=x.data_ptr(), weight=w.data_ptr(),
+                           bias=b.data_ptr(), mean=mean.data_ptr(), rstd=rstd.data_ptr())
+        size = lib.fssim_group_norm_forward_workspace_bytes(ctypes.byref(args))
+        ws = torch.full((size + 16,), 255, dtype=torch.uint8, device="cuda")  # contents arbitrary
+        args.workspace, args.workspace_bytes = ws.data_ptr(), size
+        stream = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+        assert lib.fssim_group_norm_forward(ctypes.byref(args), stream) == 0
+        torch.cuda.synchronize()
+        assert torch.equal(x, want)
+        assert (ws[size:] == 255).all()
+        ref = rs.view(2, 4, 8)[:, :, 0]
+        assert ((rstd.double() - ref).abs() <= 32 * U * 8 * ref).all()
