@@ -41,6 +41,11 @@ constexpr int kGradU = 2, kGradB = 4;
 constexpr double kResidentBytes = 8 << 20;
 constexpr int kResidentSlots = 8;
 constexpr int64_t kSliceBytes = 64;
+// An applying pass of one wave merges the statistics itself, without a launch between, where a
+// sample has at most this many parts times groups: each CTA reads them all. On a B200 the
+// 8x128x256^2 forward (37 parts, 32 groups) takes 70.8 us so and 73.2 with the launch,
+// 1x128x128^2 (128 parts) 13.7 and 10.9.
+constexpr int kMergeMost = 2048;
 constexpr int64_t kApplySteps = 32, kApplyWaves = 6;
 
 size_t elem_size(int dtype) { return dtype == FSSIM_F32 ? 4 : 2; }
@@ -227,7 +232,8 @@ int check_common(int dtype, int weight_dtype, int activation, int64_t N, int64_t
 struct ForwardPlan {
   int V;
   ResidentPlan resident;
-  NormGeometry g;
+  NormGeometry g, apply;
+  int merges;  // of the applying pass, or 0
   size_t partial, bytes;
 };
 
@@ -238,6 +244,9 @@ ForwardPlan plan_forward(const fssim_group_norm_forward_args& a) {
   p.resident = plan_resident(a.N, a.P, a.C, a.groups, p.V, E, a.eps, 1);
   if (p.resident.slots) return p;
   p.g = make_geometry(a.N, a.P, a.C, a.groups, p.V, kStatsU, a.eps);
+  p.apply = apply_geometry(p.g);
+  const bool wave = static_cast<int64_t>(p.apply.S) * a.N <= kWave && p.g.slices == 1;
+  if (wave && a.groups <= fssim::kNormMergeGroups && p.g.S * a.groups <= kMergeMost) p.merges = p.g.S;
   p.partial = round256(sizeof(float2) * static_cast<size_t>(a.N) * p.g.S * p.g.slices * p.g.GS);
   p.bytes = p.partial + sizeof(float) * fssim::kNormForwardRows * static_cast<size_t>(a.N) * a.C;
   return p;
@@ -280,18 +289,20 @@ dim3 team_grid(const NormGeometry& g, int shift) {
 }
 
 template <typename T, int V, int ACT>
-int forward_kernels(const NormParams& p, cudaStream_t s) {
+int forward_kernels(const NormParams& p, const NormGeometry& apply, cudaStream_t s) {
   using Stats = fssim::NormWalk<T, V, kStatsU, kStatsB, false>;
   using Apply = fssim::NormWalk<T, V, kApplyU, kApplyB, true>;
   constexpr size_t scratch = Stats::kScratchBytes, ring = Stats::kRingBytes;
   int st = launch_pass<fssim::norm_stats_kernel<T, V, kStatsU, kStatsB>, (ring > scratch ? ring : scratch)>(
       p.g, p, s, "group norm statistics launch");
   if (st) return st;
-  const int team = team_shift(p.g.S);
-  st = launch(fssim::norm_merge_kernel, team_grid(p.g, team), 1, 0, p, s, "group norm merge launch", team);
-  if (st) return st;
+  if (!p.merges) {
+    const int team = team_shift(p.g.S);
+    st = launch(fssim::norm_merge_kernel, team_grid(p.g, team), 1, 0, p, s, "group norm merge launch", team);
+    if (st) return st;
+  }
   NormParams q = p;
-  q.g = apply_geometry(p.g);
+  q.g = apply;
   return launch_pass<fssim::norm_apply_kernel<T, V, ACT, kApplyU, kApplyB>, Apply::kRingBytes>(
       q.g, q, s, "group norm launch");
 }
@@ -311,21 +322,22 @@ int backward_kernels(const NormParams& p, cudaStream_t s) {
   if (st || !p.out) return st;
   NormParams q = p;
   q.g = apply_geometry(p.g);
+  q.fold_params = p.g.N > 1 && (p.dweight || p.dbias);
   return launch_pass<fssim::norm_grad_apply_kernel<T, V, ACT, kGradU, kGradB>, ring>(
       q.g, q, s, "group norm gradient launch");
 }
 
 // One launch list per (element type, vector width, activation).
-template <template <typename, int, int> class Run, typename T, int V>
-int by_activation(int act, const NormParams& p, const ResidentPlan& r, cudaStream_t s) {
+template <template <typename, int, int> class Run, typename T, int V, typename Plan>
+int by_activation(int act, const NormParams& p, const Plan& r, cudaStream_t s) {
   switch (act) {
     case FSSIM_ACT_SILU: return Run<T, V, fssim::kNormActSilu>::run(p, r, s);
     case FSSIM_ACT_RELU: return Run<T, V, fssim::kNormActRelu>::run(p, r, s);
     default: return Run<T, V, fssim::kNormActNone>::run(p, r, s);
   }
 }
-template <template <typename, int, int> class Run, typename T>
-int by_width(int V, int act, const NormParams& p, const ResidentPlan& r, cudaStream_t s) {
+template <template <typename, int, int> class Run, typename T, typename Plan>
+int by_width(int V, int act, const NormParams& p, const Plan& r, cudaStream_t s) {
   constexpr int full = 16 / sizeof(T), mid = 4 / sizeof(T);
   if (V == full) return by_activation<Run, T, full>(act, p, r, s);
   if constexpr (mid > 1) {
@@ -333,8 +345,8 @@ int by_width(int V, int act, const NormParams& p, const ResidentPlan& r, cudaStr
   }
   return by_activation<Run, T, 1>(act, p, r, s);
 }
-template <template <typename, int, int> class Run>
-int dispatch(int dtype, int V, int act, const NormParams& p, const ResidentPlan& r, cudaStream_t s) {
+template <template <typename, int, int> class Run, typename Plan>
+int dispatch(int dtype, int V, int act, const NormParams& p, const Plan& r, cudaStream_t s) {
   switch (dtype) {
     case FSSIM_F32: return by_width<Run, float>(V, act, p, r, s);
     case FSSIM_F16: return by_width<Run, __half>(V, act, p, r, s);
@@ -343,7 +355,9 @@ int dispatch(int dtype, int V, int act, const NormParams& p, const ResidentPlan&
 }
 template <typename T, int V, int ACT>
 struct Forward {
-  static int run(const NormParams& p, const ResidentPlan&, cudaStream_t s) { return forward_kernels<T, V, ACT>(p, s); }
+  static int run(const NormParams& p, const NormGeometry& apply, cudaStream_t s) {
+    return forward_kernels<T, V, ACT>(p, apply, s);
+  }
 };
 template <typename T, int V, int ACT>
 struct Backward {
@@ -411,7 +425,8 @@ int forward_impl(const fssim_group_norm_forward_args* a, cudaStream_t stream) {
   p.g.keep = kept_share(static_cast<double>(a->N) * a->P * a->C * E);
   p.partial = static_cast<float2*>(a->workspace);
   p.channel = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + plan.partial);
-  return dispatch<Forward>(a->dtype, plan.V, a->activation, p, plan.resident, stream);
+  p.merges = plan.merges;
+  return dispatch<Forward>(a->dtype, plan.V, a->activation, p, plan.apply, stream);
 }
 
 int backward_impl(const fssim_group_norm_backward_args* a, cudaStream_t stream) {
@@ -466,8 +481,9 @@ int backward_impl(const fssim_group_norm_backward_args* a, cudaStream_t stream) 
     st = dispatch<Backward>(a->dtype, plan.V, a->activation, p, plan.resident, stream);
   }
   if (st) return st;
-  // (one sample's sums are the parameters' gradients: the merge has written them)
-  if (a->N == 1 || (!a->dweight && !a->dbias)) return FSSIM_OK;
+  // One sample's sums are the parameters' gradients, and have been written; of several, the applying
+  // pass has added them up.
+  if (a->N == 1 || (!a->dweight && !a->dbias) || (!plan.resident.slots && a->dx)) return FSSIM_OK;
   const unsigned blocks = static_cast<unsigned>((a->C + fssim::kNormWarps - 1) / fssim::kNormWarps);
   return launch(fssim::norm_param_grad_kernel, dim3(blocks), 1, 0, p, stream,
                 "group norm parameter gradient launch");

@@ -81,6 +81,7 @@ struct NormParams {
   const void* weight;   // C values of weight_dtype, or nullptr (ones)
   const void* bias;     // C values of weight_dtype, or nullptr (zeros)
   int weight_vectors;   // both start at a multiple of 16 bytes
+  int merges;           // parts of a sample whose results the applying pass merges itself, or 0
   int weight_dtype;
   float* mean;          // N * G
   float* rstd;          // N * G
@@ -92,6 +93,7 @@ struct NormParams {
                         // backward also rstd <w dz> and rstd^2 <w dz xhat> (kNormBackwardRows)
   void* dweight;
   void* dbias;
+  int fold_params;      // the applying pass of the backward sums dweight and dbias too
 };
 
 constexpr int kNormForwardRows = 3;
@@ -787,7 +789,40 @@ __global__ void __launch_bounds__(kNormThreads) norm_merge_kernel(const __grid_c
   }
 }
 
+// In an applying pass that has no merging launch before it: the statistics of all groups of sample n
+// from its p.merges parts, by a power of two of threads, at most a warp, for each group.
+__device__ __forceinline__ void norm_merge_here(const NormParams& p, int n, float2* stats) {
+  const NormGeometry& g = p.g;
+  int shift = 5;
+  while (shift > 0 && g.G << shift > kNormThreads) --shift;
+  const int lane = threadIdx.x & ((1 << shift) - 1), step = kNormThreads >> shift;
+  for (int b = 0; b < g.G; b += step) {
+    const int grp = b + (threadIdx.x >> shift);
+    double ref = 0.0, sum = 0.0, q = 0.0;
+    if (grp < g.G) {
+      const float2* pairs = p.partial + static_cast<int64_t>(n) * p.merges * g.G + grp;
+      ref = pairs[0].x;
+#pragma unroll 4
+      for (int k = lane; k < p.merges; k += 1 << shift) {
+        const float2 v = pairs[k * g.G];
+        const double cnt = static_cast<double>(g.part_pixels(k)) * g.Cg;
+        const double d = v.x - ref;
+        sum = fma(cnt, d, sum);
+        q += fma(cnt * d, d, static_cast<double>(v.y));
+      }
+    }
+    for (int o = 1 << shift >> 1; o > 0; o >>= 1) {
+      sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      q += __shfl_xor_sync(0xffffffffu, q, o);
+    }
+    if (grp < g.G && lane == 0) stats[grp] = norm_statistics(g, ref, sum, q);
+  }
+  __syncthreads();
+}
+
 // ---- forward: y ----
+constexpr int kNormMergeGroups = 256;  // groups that an applying pass merges itself, at most
+
 template <typename T, int V, int ACT, int U, int B>
 __global__ void __launch_bounds__(kNormThreads, kNormApplyResident) norm_apply_kernel(const __grid_constant__ NormParams p) {
   const NormGeometry& g = p.g;
@@ -809,7 +844,16 @@ __global__ void __launch_bounds__(kNormThreads, kNormApplyResident) norm_apply_k
   grid_dependency_wait();
   constexpr int N = IO::N;
   float2 minus[N], a[N], b[N];  // -mean, the factor and the shift
-  if (t.active) {
+  if (p.merges) {
+    __shared__ float2 stats[kNormMergeGroups];
+    norm_merge_here(p, t.n, stats);
+    if (t.active) norm_constants<V>(p, t, [&](int grp) { return stats[grp]; }, minus, a, b);
+    if (p.mean && t.s == 0)
+      for (int i = threadIdx.x; i < g.G; i += kNormThreads) {
+        p.mean[static_cast<int64_t>(t.n) * g.G + i] = stats[i].x;
+        p.rstd[static_cast<int64_t>(t.n) * g.G + i] = stats[i].y;
+      }
+  } else if (t.active) {
     const float* row = p.channel + static_cast<int64_t>(t.n) * kNormForwardRows * g.C + t.c0 + t.chan;
     load_channels<V>(row, minus);
     load_channels<V>(row + g.C, a);
@@ -961,25 +1005,32 @@ __global__ void __launch_bounds__(kNormThreads) norm_grad_merge_kernel(const __g
   }
 }
 
-// ---- backward: dweight and dbias, sums over the samples: a warp for each channel ----
+// ---- backward: dweight and dbias, sums over the samples: a warp for each channel, from the blocks'
+// first on ----
+__device__ __forceinline__ void norm_param_grads(const NormParams& p) {
+  for (int64_t c = static_cast<int64_t>(blockIdx.x) * kNormWarps + threadIdx.x / 32; c < p.g.C;
+       c += static_cast<int64_t>(gridDim.x) * kNormWarps) {
+    double db = 0.0, dw = 0.0;
+#pragma unroll 4
+    for (int64_t n = threadIdx.x % 32; n < p.g.N; n += 32) {
+      const float2 v = p.sums[n * p.g.C + c];
+      db += v.x;
+      dw += v.y;
+    }
+    db = warp_sum(db);
+    dw = warp_sum(dw);
+    if (threadIdx.x % 32 == 0) {
+      if (p.dweight) store_weight(p.dweight, p.weight_dtype, static_cast<int>(c), static_cast<float>(dw));
+      if (p.dbias) store_weight(p.dbias, p.weight_dtype, static_cast<int>(c), static_cast<float>(db));
+    }
+  }
+}
+
+// (a launch of its own where there is no dx, or the resident kernel made it)
 __global__ void __launch_bounds__(kNormThreads) norm_param_grad_kernel(const __grid_constant__ NormParams p) {
   grid_dependency_wait();
   grid_launch_dependents();
-  const int c = blockIdx.x * kNormWarps + threadIdx.x / 32;
-  if (c >= p.g.C) return;
-  double db = 0.0, dw = 0.0;
-#pragma unroll 4
-  for (int64_t n = threadIdx.x % 32; n < p.g.N; n += 32) {
-    const float2 v = p.sums[n * p.g.C + c];
-    db += v.x;
-    dw += v.y;
-  }
-  db = warp_sum(db);
-  dw = warp_sum(dw);
-  if (threadIdx.x % 32 == 0) {
-    if (p.dweight) store_weight(p.dweight, p.weight_dtype, c, static_cast<float>(dw));
-    if (p.dbias) store_weight(p.dbias, p.weight_dtype, c, static_cast<float>(db));
-  }
+  norm_param_grads(p);
 }
 
 // ---- backward: dx ----
@@ -1002,6 +1053,7 @@ __global__ void __launch_bounds__(kNormThreads, kNormApplyResident) norm_grad_ap
 #pragma unroll
   for (int j = 0; j < B - 1; ++j) start(j, walk.count - j * U);
   grid_dependency_wait();
+  if (p.fold_params && blockIdx.y == 0) norm_param_grads(p);
   constexpr int N = IO::N;
   float2 minus[N], a[N], b[N], k1[N], k2[N];  // -mean, factor, shift, and the two means negated
   if (t.active) {
