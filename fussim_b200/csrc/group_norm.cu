@@ -21,8 +21,9 @@ using fssim_host::NvtxRange;
 
 constexpr int64_t kMaxChannels = int64_t{1} << 24;
 constexpr int64_t kMaxSamples = int64_t{1} << 30;
-// CTAs of one wave on 148 SMs.
-constexpr int64_t kWave = 148 * fssim::kNormResident;
+constexpr unsigned kSms = 148;
+// CTAs of one wave.
+constexpr int64_t kWave = kSms * fssim::kNormResident;
 // Bytes of input that are to stay in L2 from the reducing pass to the applying one, of larger
 // tensors (1x64x1080x1920 16-bit forward 152 us without, 143 with; flat from 64 to 120 MB).
 constexpr double kKeptBytes = 80 << 20;
@@ -170,14 +171,20 @@ int launch(Kernel k, dim3 grid, int cluster, size_t smem, const NormParams& p, c
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = static_cast<unsigned>(cluster);
-  attr[1].val.clusterDim.y = 1;
-  attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  // Clusters that start while the kernel before still has its CTAs on the SMs go one to an SM, and
+  // more of them than SMs then take a second wave (16x64x64^2 16-bit training pass 33 against
+  // 28 us): such a launch waits for that kernel's end.
+  if (cluster == 1 || grid.x <= kSms) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (cluster > 1) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    attr[cfg.numAttrs].val.clusterDim.x = static_cast<unsigned>(cluster);
+    attr[cfg.numAttrs].val.clusterDim.y = 1;
+    attr[cfg.numAttrs++].val.clusterDim.z = 1;
+  }
   const cudaError_t e = cudaLaunchKernelEx(&cfg, k, p, extra...);
   if (e != cudaSuccess) {
     (void)cudaGetLastError();
