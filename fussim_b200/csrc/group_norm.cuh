@@ -303,7 +303,8 @@ __device__ __forceinline__ void norm_put(float* p, const float2 (&f)[kPairs<V>])
 
 // Sums over a CTA's rows, then over a group's channels. The rows are shared out over T threads for
 // each channel (all of the CTA's, where the slice has fewer channels than threads), which leave
-// T subtotals of each channel in out[j * SC + c]; f(c) gives the function of a row for channel c.
+// T subtotals of each channel in out[j * cols + c], T * cols of them in all where T is not 1 (a
+// slice may be the last and narrow); f(c) gives the function of a row for channel c.
 struct NormColumns {
   int cols, T, col, sub;
   __device__ __forceinline__ explicit NormColumns(int width) {
@@ -320,7 +321,7 @@ struct NormColumns {
       float v = 0.f;
 #pragma unroll 4
       for (int r = sub; r < g.rows; r += T) v += value(r);
-      out[sub * g.SC + c] = v;
+      out[sub * cols + c] = v;
     }
   }
   // f(i, cb, w, sum of the subtotals of [cb, cb + w)) for the i-th group that touches the slice,
@@ -336,7 +337,7 @@ struct NormColumns {
       const int w = min((t.g0 + i + 1) * g.Cg, t.c1) - t.c0 - cb;
       float v = 0.f;
       for (int j = 0; j < T; ++j)
-        for (int c = lane; c < w; c += lanes) v += in[j * g.SC + cb + c];
+        for (int c = lane; c < w; c += lanes) v += in[j * cols + cb + c];
       if (!narrow) v = warp_sum(v);
       if (lane == 0) f(i, cb, w, v);
     }
@@ -678,8 +679,8 @@ __device__ __forceinline__ void norm_merge_sums(const NormGeometry& g, const Nor
   for (int c = threadIdx.x; c < width; c += kNormThreads) {
     float v1 = 0.f, v2 = 0.f;
     for (int j = 0; j < columns.T; ++j) {
-      v1 += column1[j * g.SC + c];
-      v2 += column2[j * g.SC + c];
+      v1 += column1[j * columns.cols + c];
+      v2 += column2[j * columns.cols + c];
     }
     put(c, make_float2(v1, v2));
   }

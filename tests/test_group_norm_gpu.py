@@ -154,6 +154,8 @@ SHAPES = [  # (N, C, H, W), groups
     ((40, 64, 40, 41), 8),
     ((600, 32, 20, 20), 4),     # more samples than a wave of CTAs
     ((1, 1024, 9, 8), 32),
+    ((1, 65537, 2, 1), 1),      # 257 slices, the last of one channel
+    ((1, 40003, 1, 3), 40003),
 ]
 
 
@@ -275,8 +277,9 @@ def test_constant_and_offset_inputs(dtype):
     check_forward(fb.group_norm_act(x, 4, w, b), x, 4, w, b, 1e-5, "silu")
 
 
-def test_nan_and_inf_stay_in_their_group():
-    x, dy, w, b = make((2, 12, 8, 9), F32, F32, 11)
+@pytest.mark.parametrize("shape", [(2, 12, 8, 9), (2, 12, 300, 301), (9, 12, 130, 131)])
+def test_nan_and_inf_stay_in_their_group(shape):
+    x, dy, w, b = make(shape, F32, F32, 11)
     for act in ("silu", "relu", None):
         clean = grads(x, 4, w, b, 1e-5, act, dy)
         for bad in (float("nan"), float("inf")):
