@@ -229,6 +229,7 @@ int guarded(F f) {
     fssim_host::g_last_error.clear();
     return f();
   } catch (const std::exception&) {
+    fssim_host::g_last_error = "host exception";  // short: no allocation
     return FSSIM_ERR_CUDA;
   }
 }

@@ -19,7 +19,7 @@ using fssim_host::aligned;
 using fssim_host::fail;
 using fssim_host::NvtxRange;
 
-constexpr int64_t kMaxChannels = int64_t{1} << 24;
+constexpr int64_t kMaxChannels = int64_t{1} << 23;  // 65535 slices of at least 256 vectors
 constexpr int64_t kMaxSamples = int64_t{1} << 30;
 constexpr unsigned kSms = 148;
 // CTAs of one wave.
@@ -227,7 +227,7 @@ int check_common(int dtype, int weight_dtype, int activation, int64_t N, int64_t
   if (G < 1 || C < 1 || C % G != 0)
     return fail(FSSIM_ERR_SHAPE, "the channels must divide into the groups (C = " +
                                      std::to_string(C) + ", groups = " + std::to_string(G) + ")");
-  if (C > kMaxChannels) return fail(FSSIM_ERR_SHAPE, "C must be at most 2^24");
+  if (C > kMaxChannels) return fail(FSSIM_ERR_SHAPE, "C must be at most 2^23");
   if (N > kMaxSamples) return fail(FSSIM_ERR_SHAPE, "N must be at most 2^30");
   if (N * G > INT_MAX) return fail(FSSIM_ERR_SHAPE, "N*groups must be < 2^31");
   if (static_cast<double>(N) * P * C > 1.0e18) return fail(FSSIM_ERR_SHAPE, "N*P*C overflows int64");
@@ -503,6 +503,7 @@ int guarded(F f) {
     fssim_host::g_last_error.clear();
     return f();
   } catch (const std::exception&) {
+    fssim_host::g_last_error = "host exception";  // short: no allocation
     return FSSIM_ERR_CUDA;
   }
 }

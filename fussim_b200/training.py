@@ -48,8 +48,8 @@ def group_norm_act(
 
 
 class GroupNormAct(torch.nn.Module):
-    """``group_norm_act`` as a module, with ``torch.nn.GroupNorm``'s arguments, parameter names
-    and initial values (its state dicts load here) and the activation."""
+    """``group_norm_act`` as a module, with ``torch.nn.GroupNorm``'s arguments in their order,
+    parameter names and initial values (its state dicts load here), and the activation."""
 
     def __init__(
         self,
@@ -57,9 +57,9 @@ class GroupNormAct(torch.nn.Module):
         num_channels: int,
         eps: float = 1e-5,
         affine: bool = True,
-        activation: Optional[str] = "silu",
         device=None,
         dtype=None,
+        activation: Optional[str] = "silu",
     ):
         super().__init__()
         _ensure_cuda_extension().check_norm_settings(num_groups, num_channels, eps, activation)
@@ -102,6 +102,7 @@ def clip_grad_norm(
     grads: Iterable[torch.Tensor],
     max_norm: float,
     out: Optional[Sequence[torch.Tensor]] = None,
+    *,
     error_if_nonfinite: bool = False,
 ) -> Tuple[List[torch.Tensor], torch.Tensor]:
     """Gradients scaled so that their common 2-norm is at most ``max_norm``, and that norm.
@@ -123,14 +124,17 @@ def clip_grad_norm(
 def clip_grad_norm_(
     parameters,
     max_norm: float,
+    norm_type: float = 2.0,
     error_if_nonfinite: bool = False,
 ) -> torch.Tensor:
     """Clip the parameters' gradients in place to a common 2-norm of ``max_norm``; returns the
     norm before clipping, a 0-d float32 tensor (``torch.nn.utils.clip_grad_norm_`` for
-    ``norm_type=2``). Parameters without a gradient are passed over. Where the norm is within
+    ``norm_type=2``, the only one here: others raise ValueError). Parameters without a gradient are passed over. Where the norm is within
     the limit the gradients are left untouched (and not read a second time); otherwise as
     ``clip_grad_norm`` with ``out=grads``. A gradient may be given once only.
     """
+    if float(norm_type) != 2.0:
+        raise ValueError(f"norm_type must be 2, got {norm_type}")
     if isinstance(parameters, torch.Tensor):
         parameters = [parameters]
     return _ensure_cuda_extension().clip_grad_norm_(

@@ -307,7 +307,7 @@ typedef struct fssim_group_norm_forward_args {
   int32_t dtype;          /* fssim_dtype of x and y */
   int32_t weight_dtype;   /* fssim_dtype of weight and bias */
   int32_t activation;     /* fssim_activation */
-  int64_t N, P, C;        /* samples, pixels per sample, channels (at most 2^24) */
+  int64_t N, P, C;        /* samples, pixels per sample, channels (at most 2^23) */
   int64_t groups;         /* divides C */
   float eps;              /* >= 0 */
   const void* x;
@@ -343,8 +343,8 @@ typedef struct fssim_group_norm_backward_args {
 } fssim_group_norm_backward_args;
 
 /* Workspace of a call with these arguments (their pointers included: alignment decides how
- * the tensors are read; workspace and workspace_bytes are not looked at). 0 for arguments
- * that the call refuses or that leave it nothing to do. */
+ * the tensors are read; workspace and workspace_bytes are not looked at). 0 where the call needs
+ * none (workspace may then be NULL), refuses the arguments, or has nothing to do. */
 size_t fssim_group_norm_forward_workspace_bytes(const fssim_group_norm_forward_args* args);
 size_t fssim_group_norm_backward_workspace_bytes(const fssim_group_norm_backward_args* args);
 

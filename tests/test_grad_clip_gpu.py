@@ -242,10 +242,12 @@ def test_repeats_and_streams():
         assert torch.equal(n, norm) and all(torch.equal(p, q) for p, q in zip(out, want))
 
 
-def test_graphs_replay_together():
+@pytest.mark.parametrize("more", [0, 400])
+def test_graphs_replay_together(more):
+    sizes = [50_000, 7, 3000] + [100 + i for i in range(more)]  # a small table and a large one
     graphs = []
     for k in range(2):
-        grads = tensors([50_000, 7, 3000 + k], (F32, F16), 8 + k)
+        grads = tensors([n + k for n in sizes], (F32, F16), 8 + k)
         params = [torch.nn.Parameter(torch.zeros_like(g)) for g in grads]
         for p, g in zip(params, grads):
             p.grad = g
@@ -258,7 +260,7 @@ def test_graphs_replay_together():
     for round_ in range(3):
         fresh = []
         for k, (_, _, grads, _) in enumerate(graphs):
-            fresh.append(tensors([50_000, 7, 3000 + k], (F32, F16), 40 + 2 * round_ + k))
+            fresh.append(tensors([n + k for n in sizes], (F32, F16), 40 + 2 * round_ + k))
             for g, f in zip(grads, fresh[-1]):
                 g.copy_(f)
         torch.cuda.synchronize()

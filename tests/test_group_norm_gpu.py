@@ -154,6 +154,8 @@ SHAPES = [  # (N, C, H, W), groups
     ((40, 64, 40, 41), 8),
     ((600, 32, 20, 20), 4),     # more samples than a wave of CTAs
     ((1, 1024, 9, 8), 32),
+    ((2, 1, 40, 41), 1),        # one channel
+    ((1, 1, 300, 301), 1),
     ((1, 65537, 2, 1), 1),      # 257 slices, the last of one channel
     ((1, 40003, 1, 3), 40003),
 ]
@@ -192,8 +194,9 @@ def test_parameter_types(dtype, wdtype):
     check_backward(dx, dw, db, x, 4, w, b, 1e-5, "silu", dy)
 
 
-def test_only_the_gradients_asked_for():
-    x, dy, w, b = make((2, 16, 12, 15), F32, F32, 7)
+@pytest.mark.parametrize("shape", [(2, 16, 12, 15), (1, 16, 12, 15), (2, 16, 200, 201), (1, 16, 300, 301)])
+def test_only_the_gradients_asked_for(shape):
+    x, dy, w, b = make(shape, F32, F32, 7)
     full = grads(x, 4, w, b, 1e-5, "silu", dy)
     for need in ((1, 0, 0), (0, 1, 0), (0, 0, 1), (0, 1, 1), (1, 0, 1)):
         ts = [t.detach().requires_grad_(bool(k)) for t, k in zip((x, w, b), need)]
@@ -305,6 +308,21 @@ def test_extreme_values():
     y = fb.group_norm_act(x, 2, 1000 * w, b)
     assert y.isfinite().all()
     check_forward(y, x, 2, 1000 * w, b, 1e-5, "silu")
+
+
+@pytest.mark.parametrize("shape", [(3, 24, 10, 14), (1, 64, 160, 161)])
+def test_shared_parameters_accumulate(shape):
+    # one layer used twice, and a broadcast gradient: what autograd adds up is each use's own
+    x, dy, w, b = make(shape, F32, F32, 18)
+    xs, ws, bs = (t.detach().requires_grad_(True) for t in (x, w, b))
+    y1 = fb.group_norm_act(xs, 4, ws, bs)
+    y2 = fb.group_norm_act(y1, 4, ws, bs)
+    y2.sum().backward()
+    ones = torch.ones_like(y2)
+    _, d1, w2, b2 = grads(y1.detach(), 4, w, b, 1e-5, "silu", ones)
+    _, dx, w1, b1 = grads(x, 4, w, b, 1e-5, "silu", d1)
+    assert torch.equal(xs.grad, dx)
+    assert torch.equal(ws.grad, w1 + w2) and torch.equal(bs.grad, b1 + b2)
 
 
 def test_empty():
