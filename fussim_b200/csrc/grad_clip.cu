@@ -115,6 +115,8 @@ int check(const fssim_grad_clip_args* a, bool clip) {
     if (!aligned(a->grads[i], elem_size(a->dtypes[i])) ||
         (clip && !aligned(a->outs[i], elem_size(a->out_dtypes[i]))))
       return fail(FSSIM_ERR_ARGUMENT, "a tensor is not aligned to its element size");
+    if (clip && a->outs[i] == a->grads[i] && a->out_dtypes[i] != a->dtypes[i])
+      return fail(FSSIM_ERR_ARGUMENT, "an output in its gradient's place has the gradient's type");
   }
   const int64_t need = fssim_grad_clip_workspace_bytes(a);
   if (need > 0 && (!a->workspace || a->workspace_bytes < static_cast<size_t>(need)))

@@ -198,6 +198,9 @@ def test_refusals():
         fb.clip_grad_norm([a[:50], b[:50]], 1.0, out=[a[1:51], b[:50]])
     with pytest.raises(ValueError, match="overlap"):
         fb.clip_grad_norm([a, b], 1.0, out=[torch.zeros_like(a)] * 2)
+    half = torch.zeros(100, device="cuda", dtype=F16)
+    with pytest.raises(ValueError, match="overlap"):        # the gradient's memory as 32 bits
+        fb.clip_grad_norm([half[:50]], 1.0, out=[half.view(F32)])
     wide = torch.zeros(100, 2, device="cuda")
     with pytest.raises(ValueError, match="overlap"):
         fb.clip_grad_norm([a, b], 1.0, out=[wide[:, 0], wide[:, 0]])

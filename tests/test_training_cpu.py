@@ -221,6 +221,7 @@ def _clip(sizes, n=None, dtypes=None, out_dtypes=None, grads=None, outs=None, **
     (lambda: _clip([4], grads=[None]), NULLPTR), (lambda: _clip([4], outs=[None]), NULLPTR),
     (lambda: _clip([4], grads=[SOME + 2]), ARGUMENT), (lambda: _clip([4], norm=None), NULLPTR),
     (lambda: _clip([4], max_norm=-1.0), ARGUMENT),
+    (lambda: _clip([4], dtypes=[1], out_dtypes=[0]), ARGUMENT),  # in place with another type
     (lambda: _clip([4], max_norm=float("nan")), ARGUMENT),
     (lambda: _clip([4], workspace=None), WORKSPACE),
     (lambda: _clip([4], workspace_bytes=4), WORKSPACE),
