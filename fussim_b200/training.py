@@ -92,7 +92,7 @@ def grad_norm(grads: Iterable[torch.Tensor]) -> torch.Tensor:
 
     ``grads`` are dense CUDA tensors of one device, float32, float16 or bfloat16 in any mix;
     an empty sequence has norm 0 (on the current device). Squares are summed in FP64 beyond
-    eight numbers and FP32's range does not limit them; the result repeats bit for bit. No
+    32 numbers and FP32's range does not limit them; the result repeats bit for bit. No
     host synchronisation. Not differentiable.
     """
     return _ensure_cuda_extension().grad_norm(list(grads))
@@ -112,7 +112,7 @@ def clip_grad_norm(
     its shape, and of its type or float32 (the 32-bit gradients of a mixed-precision
     optimiser); ``out[i]`` may be ``grads[i]``. Otherwise no two of the tensors written, and
     no gradient and another's output, may share memory. A norm that is NaN makes everything
-    NaN, an infinite one makes finite numbers 0; ``error_if_nonfinite`` raises instead, before
+    NaN, an infinite gradient makes finite numbers 0; ``error_if_nonfinite`` raises instead, before
     anything is written, at the price of a host synchronisation. Tensors whose numbers do not
     fill their memory are copied once more.
     """
@@ -129,9 +129,10 @@ def clip_grad_norm_(
 ) -> torch.Tensor:
     """Clip the parameters' gradients in place to a common 2-norm of ``max_norm``; returns the
     norm before clipping, a 0-d float32 tensor (``torch.nn.utils.clip_grad_norm_`` for
-    ``norm_type=2``, the only one here: others raise ValueError). Parameters without a gradient are passed over. Where the norm is within
-    the limit the gradients are left untouched (and not read a second time); otherwise as
-    ``clip_grad_norm`` with ``out=grads``. A gradient may be given once only.
+    ``norm_type=2``, the only one here: others raise ValueError). Parameters without a gradient
+    are passed over. Where the norm is within the limit the gradients are left untouched (and
+    not read a second time); otherwise as ``clip_grad_norm`` with ``out=grads``. A gradient may
+    be given once only.
     """
     if float(norm_type) != 2.0:
         raise ValueError(f"norm_type must be 2, got {norm_type}")

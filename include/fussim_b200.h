@@ -355,8 +355,8 @@ int fssim_group_norm_backward(const fssim_group_norm_backward_args* args, fssim_
  *     norm = sqrt(sum over all tensors of g^2), coef = min(1, max_norm / (norm + 1e-6)),
  *     outs[i] = coef * grads[i].
  * Tensors are flat runs of device memory; the arrays below are host memory and are read
- * during the call. Squares are summed in FP64 beyond eight numbers, in a fixed order. A norm
- * that is NaN makes every output NaN; an infinite one gives 0 (NaN where g is infinite). */
+ * during the call. Squares are summed in FP64 beyond 32 numbers, in a fixed order. A norm
+ * that is NaN makes every output NaN; an infinite gradient makes the others 0 and itself NaN. */
 typedef struct fssim_grad_clip_args {
   int64_t count;              /* tensors */
   const void* const* grads;   /* device pointer of each (may be NULL where its size is 0) */
