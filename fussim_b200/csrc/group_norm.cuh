@@ -12,14 +12,16 @@
 // reducing pass, a small launch that merges its results, and an applying pass. The channels are
 // cut into slices of at most 256 vectors of V channels. A thread keeps one vector of channels and
 // steps over pixels, so the per-channel constants and sums stay in registers and a warp reads
-// whole rows of memory.
+// whole rows of memory. Where C is no multiple of the vector (three-channel images), the least
+// number of pixels whose channels together are, `period` of them, is taken as one pixel of
+// period * C channels: a span. Elsewhere a span is a pixel.
 //   Reducing: a sample's pixels are cut into tiles and dealt out in turn to S parts, one CTA
 //   each and one wave of CTAs in all: few results to merge, and the GPU reads memory as one
 //   moving window.
 //   Applying: S short contiguous parts, a CTA each, from the end of the samples to their
 //   beginning: what the reducing pass read last is what L2 still holds.
 //
-// Statistics: a thread takes U pixels at a time, forms each channel's mean and sum of squared
+// Statistics: a thread takes U spans at a time, forms each channel's mean and sum of squared
 // deviations of those U values (two passes over registers), and merges them into its running
 // pair (the pairwise update of Chan, Golub and LeVeque, 1979). No sum of raw squares is ever
 // formed, so a mean far from zero costs no digits. Threads, channels, parts and slices are
@@ -49,28 +51,35 @@ struct NormGeometry {
   int64_t N;   // samples of this launch
   int64_t P;   // pixels per sample
   int C, G, Cg;
-  int SC;      // channels per slice (a multiple of V)
+  int period;  // pixels of a span
+  int Cv;      // channels of a span: period * C
+  int SC;      // channels of a span per slice (a multiple of V); one slice has all where period > 1
   int slices;
   int lanes;   // SC / V
-  int rows;    // pixels a CTA takes per step
-  int S;       // parts of a sample's pixels
+  int rows;    // spans a CTA takes per step
+  int S;       // parts of a sample's spans
   int GS;      // most groups that touch one slice
   float eps;
   float keep;        // share of the input that may stay in L2 from pass to pass
   double inv_m;      // 1 / (P * Cg)
-  // Reducing passes: part s has the tiles s, s + S, ... of `tile` pixels; the last of all, which
-  // `last_part` has, lacks `lacking` pixels. Parts have `part_tiles` tiles, the first `extra_tiles`
+  // Reducing passes: part s has the tiles s, s + S, ... of `tile` spans; the last of all, which
+  // `last_part` has, lacks `lacking` spans. Parts have `part_tiles` tiles, the first `extra_tiles`
   // one more. (A part's pixels fit 31 bits, and the kernels divide no 64-bit numbers: that
   // alone took microseconds of a launch.)
   int tile, part_tiles, extra_tiles, last_part, lacking;
-  // Applying passes: contiguous parts of `base` pixels; the first `extra` have one more.
+  // Applying passes: contiguous parts of `base` spans; the first `extra` have one more.
   int base, extra;
 
   __device__ __forceinline__ int tiles_of(int s) const { return part_tiles + (s < extra_tiles); }
-  __device__ __forceinline__ int part_pixels(int s) const {
+  __device__ __forceinline__ int part_spans(int s) const {
     return tiles_of(s) * tile - (s == last_part ? lacking : 0);
   }
-  __device__ __forceinline__ int run_pixels(int s) const { return base + (s < extra); }
+  __device__ __forceinline__ int part_pixels(int s) const { return part_spans(s) * period; }
+  __device__ __forceinline__ int run_spans(int s) const { return base + (s < extra); }
+  // In a CTA's shared memory a thread row holds one value for each channel of a span: seen by
+  // pixels, rows * period rows of the real channels.
+  __device__ __forceinline__ int pixel_rows() const { return rows * period; }
+  __device__ __forceinline__ int pitch() const { return period == 1 ? SC : C; }
 };
 
 struct NormParams {
@@ -287,7 +296,7 @@ struct NormTile {
     g1 = (c1 - 1) / g.Cg + 1;
     row = threadIdx.x / g.lanes;
     chan = (threadIdx.x - row * g.lanes) * V;
-    active = row < g.rows && c0 + chan < c1;
+    active = row < g.rows && c0 + chan < min(c0 + g.SC, g.Cv);
   }
 };
 
@@ -320,24 +329,26 @@ struct NormColumns {
       const auto value = f(c);
       float v = 0.f;
 #pragma unroll 4
-      for (int r = sub; r < g.rows; r += T) v += value(r);
+      for (int r = sub; r < g.pixel_rows(); r += T) v += value(r);
       out[sub * cols + c] = v;
     }
   }
   // f(i, cb, w, sum of the subtotals of [cb, cb + w)) for the i-th group that touches the slice,
   // its channels [cb, cb + w) of the slice: a thread for each where there is little to add, a
-  // warp for each otherwise.
+  // warp for each otherwise, whose lanes share out both the channels and the subtotals
+  // (1x1x1080x1920 16-bit forward 13 us, and 47 with the subtotals added by one lane).
   template <typename F>
   __device__ __forceinline__ void sum_groups(const NormGeometry& g, const NormTile& t, const float* in, F f) const {
     const bool narrow = g.Cg * T <= 16;
-    const int lane = narrow ? 0 : threadIdx.x % 32, lanes = narrow ? 1 : 32;
+    const int lane = narrow ? 0 : threadIdx.x % 32, team = narrow ? 0 : 5;
     const int step = narrow ? kNormThreads : kNormWarps;
     for (int i = narrow ? threadIdx.x : threadIdx.x / 32; i < t.g1 - t.g0; i += step) {
       const int cb = max((t.g0 + i) * g.Cg, t.c0) - t.c0;
       const int w = min((t.g0 + i + 1) * g.Cg, t.c1) - t.c0 - cb;
+      const int shift = min(team, w > 1 ? 32 - __clz(w - 1) : 0), beside = 1 << shift;
       float v = 0.f;
-      for (int j = 0; j < T; ++j)
-        for (int c = lane; c < w; c += lanes) v += in[j * cols + cb + c];
+      for (int j = lane >> shift; j < T; j += 1 << (team - shift))
+        for (int c = lane & (beside - 1); c < w; c += beside) v += in[j * cols + cb + c];
       if (!narrow) v = warp_sum(v);
       if (lane == 0) f(i, cb, w, v);
     }
@@ -356,9 +367,9 @@ struct NormPolicy {
   }
 };
 
-// The vectors of one thread in a pass: its row's pixels of the part, in batches of U; the last batch
-// may be short. A reducing pass goes from tile to tile (a batch of each, `rows` pixels apart), an
-// applying one from the part's last pixel to its first. Vectors of 16 bytes are copied
+// The vectors of one thread in a pass: its row's spans of the part, in batches of U; the last batch
+// may be short. A reducing pass goes from tile to tile (a batch of each, `rows` spans apart), an
+// applying one from the part's last span to its first. Vectors of 16 bytes are copied
 // asynchronously into a ring of B batches in shared memory, B - 1 batches ahead of their use
 // (each thread into slots of its own, so that no barrier is needed): what a thread has in flight
 // is bounded by shared memory instead of registers and does not pause while it computes.
@@ -379,25 +390,25 @@ struct NormWalk {
   int64_t jump;    // and besides that from batch to batch
 
   __device__ __forceinline__ NormWalk(const NormGeometry& g, const NormTile& t) {
-    stride = static_cast<int64_t>(g.rows) * g.C;
-    int64_t px;
+    stride = static_cast<int64_t>(g.rows) * g.Cv;
+    int64_t span;
     if (APPLYING) {
-      const int pixels = g.run_pixels(t.s);
-      count = t.row < pixels ? (pixels - t.row - 1) / g.rows + 1 : 0;
-      px = static_cast<int64_t>(g.base) * t.s + min(t.s, g.extra) + t.row + static_cast<int64_t>(count - 1) * g.rows;
+      const int spans = g.run_spans(t.s);
+      count = t.row < spans ? (spans - t.row - 1) / g.rows + 1 : 0;
+      span = static_cast<int64_t>(g.base) * t.s + min(t.s, g.extra) + t.row + static_cast<int64_t>(count - 1) * g.rows;
       stride = -stride;
       jump = 0;
     } else {
       const int missing = t.s == g.last_part ? g.lacking : 0;
-      // pixels of a full tile that this row lacks in the last one
+      // spans of a full tile that this row lacks in the last one
       const int last = g.tile - missing;
       const int lost = missing == 0 ? 0 : U - (t.row < last ? (last - t.row - 1) / g.rows + 1 : 0);
       count = g.tiles_of(t.s) * U - lost;
-      px = static_cast<int64_t>(t.s) * g.tile + t.row;
-      jump = static_cast<int64_t>(g.S - 1) * g.tile * g.C;
+      span = static_cast<int64_t>(t.s) * g.tile + t.row;
+      jump = static_cast<int64_t>(g.S - 1) * g.tile * g.Cv;
     }
     if (!t.active) count = 0;
-    first = (t.n * g.P + px) * g.C + t.c0 + t.chan;
+    first = t.n * g.P * g.C + span * g.Cv + t.c0 + t.chan;
   }
   // pixels of the reducing pass that come before those that are to stay in L2
   __device__ __forceinline__ int passing(float keep) const {
@@ -519,6 +530,21 @@ __device__ __forceinline__ void load_weights(const NormParams& p, const void* w,
   }
 }
 
+// V values of a row of the C real channels from channel c of a span.
+template <int V>
+__device__ __forceinline__ void load_span(const NormGeometry& g, const float* row, int c, float2 (&f)[kPairs<V>]) {
+  if (g.period == 1) {
+    load_channels<V>(row + c, f);
+    return;
+  }
+  c %= g.C;
+#pragma unroll
+  for (int v = 0; v < 2 * kPairs<V>; ++v) {
+    (v & 1 ? f[v / 2].y : f[v / 2].x) = v < V ? row[c] : 0.f;
+    if (++c == g.C) c = 0;
+  }
+}
+
 // f = value(group).x and .y for each of V channels from c.
 template <int V, typename Value>
 __device__ __forceinline__ void by_group(const NormGeometry& g, int c, Value value, float2 (&x)[kPairs<V>],
@@ -550,7 +576,20 @@ template <int V, typename Stats>
 __device__ __forceinline__ void norm_constants(const NormParams& p, const NormTile& t, Stats stats,
                                                float2 (&minus)[kPairs<V>], float2 (&a)[kPairs<V>],
                                                float2 (&b)[kPairs<V>]) {
-  const int c = t.c0 + t.chan;
+  int c = t.c0 + t.chan;
+  if (p.g.period > 1) {
+    c %= p.g.C;
+#pragma unroll
+    for (int v = 0; v < 2 * kPairs<V>; ++v) {
+      const float2 st = stats(c / p.g.Cg);
+      const float w = p.weight ? load_weight(p.weight, p.weight_dtype, c) : 1.f;
+      (v & 1 ? minus[v / 2].y : minus[v / 2].x) = -st.x;
+      (v & 1 ? a[v / 2].y : a[v / 2].x) = st.y * w;
+      (v & 1 ? b[v / 2].y : b[v / 2].x) = p.bias ? load_weight(p.bias, p.weight_dtype, c) : 0.f;
+      if (++c == p.g.C) c = 0;
+    }
+    return;
+  }
   float2 w[kPairs<V>];
   load_weights<V>(p, p.weight, 1.f, c, w);
   load_weights<V>(p, p.bias, 0.f, c, b);
@@ -574,7 +613,7 @@ struct NormMoments {
 #pragma unroll
     for (int v = 0; v < N; ++v) mean[v] = m2[v] = splat2(0.f);
   }
-  // a batch of U pixels, or the last one of k (k < U); get(u) gives the vector of pixel u
+  // a batch of U spans, or the last one of k (k < U); get(u) gives the vector of span u
   template <typename Whole, typename Get>
   __device__ __forceinline__ void take(Whole, int k, Get get) {
     constexpr bool kWhole = Whole::value;
@@ -611,12 +650,12 @@ struct NormMoments {
   }
 };
 
-// The threads' pairs of a CTA that has `pixels` pixels of its part become one pair per group: first
+// The threads' pairs of a CTA that has `spans` spans of its part become one pair per group: first
 // the mean (as distances from one of the means, so that equal values give that value exactly),
 // then the deviations. put(i, pair) takes the i-th group's. `scratch` has four floats for each
 // thread and channel.
 template <int V, typename Put>
-__device__ __forceinline__ void norm_merge_rows(const NormGeometry& g, const NormTile& t, int pixels,
+__device__ __forceinline__ void norm_merge_rows(const NormGeometry& g, const NormTile& t, int spans,
                                                 const float2 (&mean)[kPairs<V>], const float2 (&m2)[kPairs<V>],
                                                 float* scratch, Put put) {
   float* sm_mean = scratch;
@@ -628,29 +667,30 @@ __device__ __forceinline__ void norm_merge_rows(const NormGeometry& g, const Nor
     norm_put<V>(sm_m2 + t.row * g.SC + t.chan, m2);
   }
   __syncthreads();
-  const int full = pixels / g.rows;          // pixels that every row took
-  const int extra = pixels - full * g.rows;  // rows that took one more
-  const int width = t.c1 - t.c0;
+  const int full = spans / g.rows;                       // pixels that every row took
+  const int extra = (spans - full * g.rows) * g.period;  // rows that took one more
+  const float pixels = static_cast<float>(spans) * g.period;
+  const int width = t.c1 - t.c0, pitch = g.pitch();
   const NormColumns columns(width);
   const auto count_of = [&](int row) { return static_cast<float>(full + (row < extra)); };
   columns.sum_rows(g, width, column, [&](int c) {
     const float ref = sm_mean[max((t.c0 + c) / g.Cg * g.Cg - t.c0, 0)];
     return [&, c, ref](int r) {
       const float cnt = count_of(r);
-      return cnt > 0.f ? cnt * (sm_mean[r * g.SC + c] - ref) : 0.f;
+      return cnt > 0.f ? cnt * (sm_mean[r * pitch + c] - ref) : 0.f;
     };
   });
   __syncthreads();
   columns.sum_groups(g, t, column, [&](int i, int cb, int w, float sum) {
-    centre[i] = sm_mean[cb] + sum / (static_cast<float>(pixels) * w);
+    centre[i] = sm_mean[cb] + sum / (pixels * w);
   });
   __syncthreads();
   columns.sum_rows(g, width, column, [&](int c) {
     const float m = centre[(t.c0 + c) / g.Cg - t.g0];
     return [&, c, m](int r) {
       const float cnt = count_of(r);
-      const float d = sm_mean[r * g.SC + c] - m;
-      return cnt > 0.f ? fmaf(cnt * d, d, sm_m2[r * g.SC + c]) : 0.f;
+      const float d = sm_mean[r * pitch + c] - m;
+      return cnt > 0.f ? fmaf(cnt * d, d, sm_m2[r * pitch + c]) : 0.f;
     };
   });
   __syncthreads();
@@ -671,11 +711,25 @@ __device__ __forceinline__ void norm_merge_sums(const NormGeometry& g, const Nor
     norm_put<V>(sm2 + t.row * g.SC + t.chan, s2);
   }
   __syncthreads();
-  const int width = t.c1 - t.c0;
+  const int width = t.c1 - t.c0, pitch = g.pitch();
   const NormColumns columns(width);
-  columns.sum_rows(g, width, column1, [&](int c) { return [&, c](int r) { return sm1[r * g.SC + c]; }; });
-  columns.sum_rows(g, width, column2, [&](int c) { return [&, c](int r) { return sm2[r * g.SC + c]; }; });
+  columns.sum_rows(g, width, column1, [&](int c) { return [&, c](int r) { return sm1[r * pitch + c]; }; });
+  columns.sum_rows(g, width, column2, [&](int c) { return [&, c](int r) { return sm2[r * pitch + c]; }; });
   __syncthreads();
+  if (columns.T >= 32) {  // at most eight channels, and many subtotals of each: a warp for each
+    const int c = threadIdx.x / 32;
+    if (c < width) {
+      float v1 = 0.f, v2 = 0.f;
+      for (int j = threadIdx.x % 32; j < columns.T; j += 32) {
+        v1 += column1[j * columns.cols + c];
+        v2 += column2[j * columns.cols + c];
+      }
+      v1 = warp_sum(v1);
+      v2 = warp_sum(v2);
+      if (threadIdx.x % 32 == 0) put(c, make_float2(v1, v2));
+    }
+    return;
+  }
   for (int c = threadIdx.x; c < width; c += kNormThreads) {
     float v1 = 0.f, v2 = 0.f;
     for (int j = 0; j < columns.T; ++j) {
@@ -712,7 +766,7 @@ __global__ void __launch_bounds__(kNormThreads, kNormResident) norm_stats_kernel
   });
   __syncthreads();  // the ring is done with: its memory is the merge's scratch
   float2* partial = p.partial + ((static_cast<int64_t>(t.n) * g.S + t.s) * g.slices + t.slice) * g.GS;
-  norm_merge_rows<V>(g, t, g.part_pixels(t.s), moments.mean, moments.m2, reinterpret_cast<float*>(norm_ring),
+  norm_merge_rows<V>(g, t, g.part_spans(t.s), moments.mean, moments.m2, reinterpret_cast<float*>(norm_ring),
                      [&](int i, float2 pair) { partial[i] = pair; });
 }
 
@@ -861,10 +915,12 @@ __global__ void __launch_bounds__(kNormThreads, kNormApplyResident) norm_apply_k
         p.rstd[static_cast<int64_t>(t.n) * g.G + i] = stats[i].y;
       }
   } else if (t.active) {
-    const float* row = p.channel + static_cast<int64_t>(t.n) * kNormForwardRows * g.C + t.c0 + t.chan;
-    load_channels<V>(row, minus);
-    load_channels<V>(row + g.C, a);
-    load_channels<V>(row + 2 * static_cast<int64_t>(g.C), b);
+    const int64_t C = g.C;
+    const float* row = p.channel + t.n * kNormForwardRows * C;
+    const int c = t.c0 + t.chan;
+    load_span<V>(g, row, c, minus);
+    load_span<V>(g, row + C, c, a);
+    load_span<V>(g, row + 2 * C, c, b);
   }
   grid_launch_dependents();  // the statistics have been read
   walk.run(B - 1, start, [&](int slot, auto whole, int k) {
@@ -1067,12 +1123,13 @@ __global__ void __launch_bounds__(kNormThreads, kNormApplyResident) norm_grad_ap
   float2 minus[N], a[N], b[N], k1[N], k2[N];  // -mean, factor, shift, and the two means negated
   if (t.active) {
     const int64_t C = g.C;
-    const float* row = p.channel + t.n * kNormBackwardRows * C + t.c0 + t.chan;
-    load_channels<V>(row, minus);
-    load_channels<V>(row + C, a);
-    load_channels<V>(row + 2 * C, b);
-    load_channels<V>(row + 3 * C, k1);
-    load_channels<V>(row + 4 * C, k2);
+    const float* row = p.channel + t.n * kNormBackwardRows * C;
+    const int c = t.c0 + t.chan;
+    load_span<V>(g, row, c, minus);
+    load_span<V>(g, row + C, c, a);
+    load_span<V>(g, row + 2 * C, c, b);
+    load_span<V>(g, row + 3 * C, c, k1);
+    load_span<V>(g, row + 4 * C, c, k2);
   }
   grid_launch_dependents();  // the means have been read
   walk.run(B - 1, start, [&](int slot, auto whole, int k) {
@@ -1149,7 +1206,7 @@ __global__ void __launch_bounds__(kNormThreads) norm_resident_kernel(const __gri
   // pairs: this CTA's, for the cluster to read; stats: the cluster's (mean, rstd) of each group
   float2* pairs = reinterpret_cast<float2*>(scratch + 4 * kNormThreads * V);
   float2* stats = reinterpret_cast<float2*>(scratch);
-  norm_merge_rows<V>(g, t, g.run_pixels(t.s), moments.mean, moments.m2, scratch,
+  norm_merge_rows<V>(g, t, g.run_spans(t.s), moments.mean, moments.m2, scratch,
                      [&](int i, float2 pair) { pairs[i] = pair; });
   const cg::cluster_group cluster = cg::this_cluster();
   cluster.sync();
@@ -1158,7 +1215,7 @@ __global__ void __launch_bounds__(kNormThreads) norm_resident_kernel(const __gri
     double sum = 0.0, q = 0.0;
     for (int r = 0; r < g.S; ++r) {
       const float2 v = cluster.map_shared_rank(pairs, r)[i];
-      const double cnt = static_cast<double>(g.run_pixels(r)) * g.Cg;
+      const double cnt = static_cast<double>(g.run_spans(r)) * g.Cg;
       const double d = v.x - ref;
       sum = fma(cnt, d, sum);
       q += fma(cnt * d, d, static_cast<double>(v.y));

@@ -175,6 +175,57 @@ def test_values_and_gradients(case, dtype):
         assert torch.equal(fb.group_norm_act(x, groups, w, b, 1e-5, act), y)
 
 
+# Channels that are no whole vectors: pixels taken together where the samples allow it.
+SPANS = [
+    ((1, 1, 1, 8), 1),          # one vector in all
+    ((1, 3, 2, 4), 1),
+    ((1, 3, 2, 4), 3),
+    ((2, 3, 2, 2), 1),          # four pixels: 16 bytes in 32 bits only
+    ((2, 3, 3, 2), 3),          # two pixels: 4 bytes in 16 bits, elements in 32
+    ((2, 3, 3, 3), 1),          # nine: elements in all types
+    ((3, 6, 7, 4), 2),
+    ((1, 5, 16, 33), 5),
+    ((2, 20, 24, 31), 4),
+    ((4, 7, 64, 72), 1),
+    ((1, 1, 400, 401), 1),      # many parts
+    ((1, 3, 304, 301), 3),
+    ((300, 3, 20, 20), 1),      # more samples than a wave of CTAs
+    ((900, 6, 8, 9), 3),
+    ((2, 30, 120, 121), 10),
+    ((2, 255, 8, 13), 5),       # most channels of a span
+    ((1, 257, 8, 13), 1),       # one too many
+    ((1, 2046, 8, 8), 11),
+    ((3, 514, 16, 12), 514),    # more groups than an applying pass merges itself
+]
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("case", range(len(SPANS)))
+def test_channels_off_the_vector(case, dtype):
+    shape, groups = SPANS[case]
+    act = ["silu", "relu", None][case % 3]
+    x, dy, w, b = make(shape, dtype, dtype if case % 2 else F32, 300 + case)
+    for ws, bs in ((w, b), (None, None)):
+        y, dx, dw, db = grads(x, groups, ws, bs, 1e-5, act, dy)
+        check_forward(y, x, groups, ws, bs, 1e-5, act)
+        check_backward(dx, dw, db, x, groups, ws, bs, 1e-5, act, dy)
+    with torch.no_grad():
+        assert torch.equal(fb.group_norm_act(x, groups, None, None, 1e-5, act), y)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("offset", [0, 1, 2, 4])
+def test_channels_off_the_vector_at_any_address(offset, dtype):
+    shape, groups = (2, 3, 40, 48), 3
+    x, dy, w, b = make(shape, dtype, F32, 340)
+    n, c, h, wd = shape
+    moved = torch.zeros(x.numel() + offset, dtype=dtype, device="cuda")[offset:].view(n, h, wd, c).permute(0, 3, 1, 2)
+    moved.copy_(x)
+    y, dx, dw, db = grads(moved, groups, w, b, 1e-5, "silu", dy)
+    check_forward(y, x, groups, w, b, 1e-5, "silu")
+    check_backward(dx, dw, db, x, groups, w, b, 1e-5, "silu", dy)
+
+
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("act", ["silu", "relu", None])
 def test_activations_and_missing_parameters(act, dtype):
