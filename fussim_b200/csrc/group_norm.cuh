@@ -624,17 +624,21 @@ struct NormMoments {
       if (kWhole || u < k) raw = get(u);
       IO::unpack(raw, f[u]);
     }
-    // the new values' weight in the mean, and that of the squared distance of the two means
+    // the new values' weight in the mean, and that of the squared distance of the two means; the first
+    // batch's mean is taken as it is
     const float taken = kWhole ? U : k;
-    const float share = kWhole ? __fdividef(1.f, before + 1.f) : taken / fmaf(before, U, taken);
+    const float share = before == 0.f ? 1.f : kWhole ? __fdividef(1.f, before + 1.f) : taken / fmaf(before, U, taken);
     const float cross = before * U * share;
     const float2 each = splat2(kWhole ? 1.f / U : 1.f / taken);
 #pragma unroll
     for (int v = 0; v < N; ++v) {
-      float2 sum = f[0][v];
+      // the mean from the distances to the first value: a sum of equal values would round
+      const float2 first = neg2(f[0][v]);
+      float2 sum = splat2(0.f);
 #pragma unroll
-      for (int u = 1; u < U; ++u) sum = add2(sum, f[u][v]);
-      const float2 m = mul2(sum, each), minus = neg2(m);
+      for (int u = 1; u < U; ++u)
+        if (kWhole || u < k) sum = add2(sum, add2(f[u][v], first));
+      const float2 m = fma2(sum, each, f[0][v]), minus = neg2(m);
       float2 q = splat2(0.f);
 #pragma unroll
       for (int u = 0; u < U; ++u)
@@ -644,7 +648,8 @@ struct NormMoments {
         }
       const float2 d = add2(m, neg2(mean[v]));
       mean[v] = fma2(d, splat2(share), mean[v]);
-      m2[v] = add2(m2[v], fma2(mul2(d, d), splat2(cross), q));
+      // (in this order: the first batch's distance is its mean, whose square may be infinite, times 0)
+      m2[v] = add2(m2[v], fma2(mul2(d, splat2(cross)), d, q));
     }
     before += 1.f;
   }
