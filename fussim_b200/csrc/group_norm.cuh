@@ -380,9 +380,17 @@ struct NormWalk {
   using Raw = typename IO::Raw;
   static constexpr bool kAsync = sizeof(Raw) == 16;
   static constexpr int kU = U;
-  // scratch of the merge that follows in the reducing passes: four floats per thread and channel
-  static constexpr int kScratchBytes = 4 * kNormThreads * V * static_cast<int>(sizeof(float));
   static constexpr int kRingBytes = kAsync ? kNormThreads * 16 * U * B : 0;
+  // Shared memory of a reducing pass over some tensors: their rings, where the merge that follows has
+  // its scratch (four floats per thread and channel), and where a part is `folded`, two FP64 sums per
+  // thread and channel.
+  static constexpr int kScratchBytes = 4 * kNormThreads * V * static_cast<int>(sizeof(float));
+  static __host__ __device__ constexpr int wide_offset(int tensors) {
+    return tensors * kRingBytes > kScratchBytes ? tensors * kRingBytes : kScratchBytes;
+  }
+  static __host__ __device__ constexpr int reducing_bytes(int tensors, bool folded) {
+    return wide_offset(tensors) + (folded ? 2 * kNormThreads * V * static_cast<int>(sizeof(double)) : 0);
+  }
 
   int count;       // vectors of this thread
   int64_t first;   // element offset of the first one
@@ -416,22 +424,33 @@ struct NormWalk {
   }
 
   // start(slot, todo) begins copying the next batch, of which `todo` vectors are left, into that
-  // batch of the ring; use(slot, whole, k) takes one of k vectors (k == U when whole).
-  template <typename Start, typename Use>
-  __device__ __forceinline__ void run(int prefilled, Start start, Use use) const {
+  // batch of the ring; use(slot, whole, k) takes one of k vectors (k == U when whole). fold() is
+  // called after each kFoldSpans of a reducing pass that others follow.
+  static constexpr int kFoldSpans = 8 * B * U;
+  template <typename Start, typename Use, typename Fold>
+  __device__ __forceinline__ void run(int prefilled, Start start, Use use, Fold fold) const {
+    constexpr bool kFolds = !APPLYING;
     int todo = count - prefilled * U, left = count;
     while (left > 0) {
+      const int stop = kFolds ? max(left - kFoldSpans, 0) : 0;
+      do {
 #pragma unroll
-      for (int b = 0; b < B; ++b) {
-        start((b + B - 1) % B, todo);
-        todo -= U;
-        if constexpr (kAsync) asm volatile("cp.async.wait_group %0;" ::"n"(B - 1) : "memory");
-        if (left >= U) use(b, std::true_type{}, U);
-        else use(b, std::false_type{}, left);
-        left -= U;
-        if (left <= 0) break;
-      }
+        for (int b = 0; b < B; ++b) {
+          start((b + B - 1) % B, todo);
+          todo -= U;
+          if constexpr (kAsync) asm volatile("cp.async.wait_group %0;" ::"n"(B - 1) : "memory");
+          if (left >= U) use(b, std::true_type{}, U);
+          else use(b, std::false_type{}, left);
+          left -= U;
+          if (left <= 0) break;
+        }
+      } while (left > stop);
+      if (kFolds && left > 0) fold();
     }
+  }
+  template <typename Start, typename Use>
+  __device__ __forceinline__ void run(int prefilled, Start start, Use use) const {
+    run(prefilled, start, use, [] {});
   }
 };
 
@@ -492,7 +511,8 @@ struct NormSink {
   }
 };
 
-// A pass's shared memory: the ring, and in the reducing passes the merge's scratch after it is used.
+// A pass's shared memory: the ring, and in the reducing passes the merge's scratch after it is used
+// and the FP64 sums behind both.
 extern __shared__ __align__(16) unsigned char norm_ring[];
 // V weights (or `missing` for each) from channel c, a multiple of V.
 template <int V>
@@ -655,6 +675,57 @@ struct NormMoments {
   }
 };
 
+// What a thread adds up over its part of a sample would be one chain of FP32 roundings as long as the
+// part (3,370 terms of 1x255x997x1001 FP32, where the dbias of equal gradients was off by 565 * 2^-24).
+// So every kFoldSpans spans the sums, of at most 64 terms (or 16 batches' moments), go on
+// into FP64 ones in shared memory, two for each of the thread's channels, its own slots. Parts
+// that are shorter never touch them.
+template <int V>
+struct NormWide {
+  double* own;
+  int folded = 0;  // spans that are in them
+  __device__ __forceinline__ explicit NormWide(int offset)
+      : own(reinterpret_cast<double*>(norm_ring + offset) + threadIdx.x) {}
+
+  // f(wide, wide, sum, sum) for each of the thread's channels
+  template <typename F>
+  __device__ __forceinline__ void each(float2 (&a)[kPairs<V>], float2 (&b)[kPairs<V>], F f) const {
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      f(own[2 * v * kNormThreads], own[(2 * v + 1) * kNormThreads], v & 1 ? a[v / 2].y : a[v / 2].x,
+        v & 1 ? b[v / 2].y : b[v / 2].x);
+  }
+  __device__ __forceinline__ void add_sums(int spans, float2 (&a)[kPairs<V>], float2 (&b)[kPairs<V>]) {
+    const bool first = folded == 0;
+    each(a, b, [&](double& wa, double& wb, float& fa, float& fb) {
+      wa = first ? fa : wa + fa;
+      wb = first ? fb : wb + fb;
+      fa = fb = 0.f;
+    });
+    folded += spans;
+  }
+  // the moments of this many spans more, merged as those of a batch are
+  __device__ __forceinline__ void add_moments(int spans, float2 (&mean)[kPairs<V>], float2 (&m2)[kPairs<V>]) {
+    const bool first = folded == 0;
+    const double share = first ? 1.0 : static_cast<double>(spans) / (static_cast<double>(folded) + spans);
+    const double cross = folded * share;
+    each(mean, m2, [&](double& wm, double& w2, float& fm, float& f2) {
+      const double d = first ? 0.0 : fm - wm;
+      wm = first ? fm : fma(d, share, wm);
+      w2 = first ? f2 : w2 + fma(d * cross, d, static_cast<double>(f2));
+      fm = f2 = 0.f;
+    });
+    folded += spans;
+  }
+  // the whole part's, back in a and b
+  __device__ __forceinline__ void take(float2 (&a)[kPairs<V>], float2 (&b)[kPairs<V>]) const {
+    each(a, b, [](double& wa, double& wb, float& fa, float& fb) {
+      fa = static_cast<float>(wa);
+      fb = static_cast<float>(wb);
+    });
+  }
+};
+
 // The threads' pairs of a CTA that has `spans` spans of its part become one pair per group: first
 // the mean (as distances from one of the means, so that equal values give that value exactly),
 // then the deviations. put(i, pair) takes the i-th group's. `scratch` has four floats for each
@@ -766,9 +837,17 @@ __global__ void __launch_bounds__(kNormThreads, kNormResident) norm_stats_kernel
 #pragma unroll
   for (int b = 0; b < B - 1; ++b) start(b, walk.count - b * U);
   NormMoments<T, V, U> moments;
+  NormWide<V> wide(Walk::wide_offset(1));
   walk.run(B - 1, start, [&](int slot, auto whole, int k) {
     moments.take(whole, k, [&](int u) { return x.get(walk, slot, u); });
+  }, [&] {
+    wide.add_moments(Walk::kFoldSpans, moments.mean, moments.m2);
+    moments.before = 0.f;
   });
+  if (wide.folded) {
+    wide.add_moments(walk.count - wide.folded, moments.mean, moments.m2);
+    wide.take(moments.mean, moments.m2);
+  }
   __syncthreads();  // the ring is done with: its memory is the merge's scratch
   float2* partial = p.partial + ((static_cast<int64_t>(t.n) * g.S + t.s) * g.slices + t.slice) * g.GS;
   norm_merge_rows<V>(g, t, g.part_spans(t.s), moments.mean, moments.m2, reinterpret_cast<float*>(norm_ring),
@@ -974,6 +1053,7 @@ __global__ void __launch_bounds__(kNormThreads, kNormResident) norm_grad_sums_ke
       const int64_t at = static_cast<int64_t>(t.n) * g.G + grp;
       return make_float2(p.mean[at], p.rstd[at]);
     }, minus, a, b);
+    NormWide<V> wide(Walk::wide_offset(2));
     walk.run(B - 1, start, [&](int slot, auto whole, int k) {
       constexpr bool kWhole = decltype(whole)::value;
 #pragma unroll
@@ -990,7 +1070,11 @@ __global__ void __launch_bounds__(kNormThreads, kNormResident) norm_grad_sums_ke
             s2[v] = fma2(dz, xc, s2[v]);
           }
         }
-    });
+    }, [&] { wide.add_sums(Walk::kFoldSpans, s1, s2); });
+    if (wide.folded) {
+      wide.add_sums(walk.count - wide.folded, s1, s2);
+      wide.take(s1, s2);
+    }
   }
   __syncthreads();
   float2* partial = p.partial + (static_cast<int64_t>(t.n) * g.S + t.s) * g.C + t.c0;
