@@ -7,7 +7,9 @@
 
 #include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include <algorithm>
 #include <cmath>
@@ -174,6 +176,21 @@ void require_cuda(const char* what) {
     runtime_error(std::string("CUDA is not available. ") + what + " requires a CUDA-capable GPU.");
 }
 
+// A tracer records the operators that torch dispatches: of a call here it would keep the allocation
+// of the result and not the launches.
+void refuse_tracing(const char* what) {
+  using Key = c10::impl::TorchDispatchModeKey;
+  if (torch::jit::tracer::isTracing() || c10::impl::TorchDispatchModeTLS::get_mode(Key::PROXY).has_value())
+    runtime_error(std::string(what) + " cannot be traced (torch.jit.trace, make_fx, torch.export): its kernels "
+                  "are launched outside torch's dispatcher");
+}
+
+// Nor is there a forward-mode derivative: a result without a tangent would stand for a zero one.
+void refuse_tangent(const at::Tensor& t, const char* name, const char* what) {
+  if (t._fw_grad(/*level=*/0).defined())
+    runtime_error(std::string(what) + " has no forward-mode derivative, but " + name + " carries a tangent");
+}
+
 int64_t activation_code(const std::optional<std::string>& name) {
   if (!name.has_value()) return FSSIM_ACT_NONE;
   if (*name == "silu") return FSSIM_ACT_SILU;
@@ -202,6 +219,8 @@ at::Tensor group_norm_act(const at::Tensor& x, int64_t groups, const OptTensor& 
   check_norm_settings(groups, channels, eps, activation);
   if (!known_type(x.scalar_type()))
     value_error("x must be float32, float16 or bfloat16, got " + type_text(x.scalar_type()));
+  refuse_tracing("group_norm_act");
+  refuse_tangent(x, "x", "group_norm_act");
   bool train = x.requires_grad();
   for (const OptTensor* o : {&weight, &bias}) {
     if (!o->has_value()) continue;
@@ -214,6 +233,7 @@ at::Tensor group_norm_act(const at::Tensor& x, int64_t groups, const OptTensor& 
     if (t.device() != x.device())
       runtime_error(name + " must be on x's device.\nx: " + x.device().str() + ", " + name + ": " +
                     t.device().str());
+    refuse_tangent(t, name.c_str(), "group_norm_act");
     train = train || t.requires_grad();
   }
   if (weight.has_value() && bias.has_value() && weight->scalar_type() != bias->scalar_type())
@@ -251,6 +271,7 @@ Refs refs_of(const py::list& list, const char* what) {
 }
 
 void check_grads(const Refs& grads, const char* what) {
+  refuse_tracing(what);
   for (size_t i = 0; i < grads.size(); ++i) {
     const at::Tensor& g = *grads[i];
     const auto at = [&] { return " at index " + std::to_string(i) + " "; };

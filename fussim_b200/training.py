@@ -39,8 +39,9 @@ def group_norm_act(
     be x's (32-bit parameters beside 16-bit images); autocast changes nothing here.
 
     The kernels work on the channels-last memory format and so is the result; another layout
-    of x (or of the incoming gradient) costs one copy. Differentiable once, with respect to x,
-    weight and bias. The results repeat bit for bit. Under graph capture follow torch's rule
+    of x (or of the incoming gradient) costs one copy. Differentiable once, backwards, with
+    respect to x, weight and bias; forward-mode derivatives and tracing (``torch.jit.trace``,
+    ``make_fx``) raise RuntimeError. The results repeat bit for bit. Under graph capture follow torch's rule
     for backward passes: the captured leaves must not have live eager graphs.
     """
     # arguments are checked in the extension: the call costs little more than its launches
@@ -93,7 +94,7 @@ def grad_norm(grads: Iterable[torch.Tensor]) -> torch.Tensor:
     ``grads`` are dense CUDA tensors of one device, float32, float16 or bfloat16 in any mix;
     an empty sequence has norm 0 (on the current device). Squares are summed in FP64 beyond
     32 numbers and FP32's range does not limit them; the result repeats bit for bit. No
-    host synchronisation. Not differentiable.
+    host synchronisation. Not differentiable; tracing raises RuntimeError.
     """
     return _ensure_cuda_extension().grad_norm(list(grads))
 
@@ -114,7 +115,7 @@ def clip_grad_norm(
     no gradient and another's output, may share memory. A norm that is NaN makes everything
     NaN, an infinite gradient makes finite numbers 0; ``error_if_nonfinite`` raises instead, before
     anything is written, at the price of a host synchronisation. Tensors whose numbers do not
-    fill their memory are copied once more.
+    fill their memory are copied once more. Not differentiable, as :func:`grad_norm`.
     """
     return _ensure_cuda_extension().clip_grad_norm(
         list(grads), float(max_norm), None if out is None else list(out), error_if_nonfinite
