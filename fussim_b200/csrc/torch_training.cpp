@@ -46,14 +46,21 @@ at::Tensor workspace(size_t bytes, const at::Tensor& like) {
 
 using OptTensor = std::optional<at::Tensor>;
 
-// Weight and bias as the C ABI takes them: dense, of one type (the Python layer has checked
-// device, shape and type).
+// A lazily negated view (the imaginary part of a conjugate) holds its numbers with the other sign.
+at::Tensor resolved(const at::Tensor& t) { return t.is_neg() ? t.resolve_neg() : t; }
+OptTensor resolved(const OptTensor& t) { return t.has_value() ? OptTensor(resolved(*t)) : t; }
+
+// Weight and bias as the C ABI takes them: dense, of one type (group_norm_act has checked device,
+// shape and type), and with memory of their own, since no pointer stands for no weight there.
 struct Affine {
   at::Tensor weight, bias;
   int dtype = FSSIM_F32;
   Affine(const OptTensor& w, const OptTensor& b) {
     if (w.has_value() && w->defined()) weight = w->contiguous();
     if (b.has_value() && b->defined()) bias = b->contiguous();
+    for (const at::Tensor* t : {&weight, &bias})
+      if (t->defined() && !t->const_data_ptr())
+        throw std::runtime_error("weight and bias must be tensors with memory (not fake ones)");
     if (weight.defined()) dtype = dtype_code(weight.scalar_type());
     else if (bias.defined()) dtype = dtype_code(bias.scalar_type());
   }
@@ -127,7 +134,7 @@ struct GroupNormFn : public torch::autograd::Function<GroupNormFn> {
     slot += weight.defined();
     const bool need_b = bias.defined() && ctx->needs_input_grad(slot);
     const at::cuda::OptionalCUDAGuard guard(x.device());
-    const at::Tensor dy = grads[0].to(x.scalar_type()).contiguous(at::MemoryFormat::ChannelsLast);
+    const at::Tensor dy = resolved(grads[0]).to(x.scalar_type()).contiguous(at::MemoryFormat::ChannelsLast);
     at::Tensor dx, dw, db;
     if (need_x) dx = at::empty(x.sizes(), x.options(), at::MemoryFormat::ChannelsLast);
     if (need_w) dw = at::empty_like(weight);
@@ -209,9 +216,11 @@ void check_norm_settings(int64_t groups, int64_t channels, double eps,
 }
 
 // Checks, then the operator: recorded for autograd where a gradient may be asked for.
-at::Tensor group_norm_act(const at::Tensor& x, int64_t groups, const OptTensor& weight,
-                          const OptTensor& bias, double eps,
+at::Tensor group_norm_act(const at::Tensor& given, int64_t groups, const OptTensor& given_weight,
+                          const OptTensor& given_bias, double eps,
                           const std::optional<std::string>& activation) {
+  const at::Tensor x = resolved(given);
+  const OptTensor weight = resolved(given_weight), bias = resolved(given_bias);
   if (x.dim() != 4)
     value_error("Expected 4D tensor (B, C, H, W), but got " + std::to_string(x.dim()) +
                 "D tensor with shape " + shape_text(x));
@@ -360,7 +369,11 @@ at::Tensor zero_norm() {
   return at::zeros({}, at::TensorOptions().dtype(at::kFloat).device(at::kCUDA));
 }
 
-// Tensors whose numbers fill their memory are taken as they lie; others go through a dense copy.
+// Tensors whose numbers fill their memory are taken as they lie; others, and lazily negated views, go
+// through a dense copy.
+bool as_it_lies(const at::Tensor& t) { return t.is_non_overlapping_and_dense() && !t.is_neg(); }
+at::Tensor dense_copy(const at::Tensor& t) { return resolved(t).contiguous(); }
+
 at::Tensor norm_of(const Refs& grads) {
   const at::NoGradGuard no_grad;
   const at::cuda::OptionalCUDAGuard guard(grads[0]->device());
@@ -368,8 +381,8 @@ at::Tensor norm_of(const Refs& grads) {
   ClipArrays arrays(grads.size());
   std::vector<at::Tensor> held;
   for (const at::Tensor* g : grads) {
-    const bool dense = g->is_non_overlapping_and_dense();
-    if (!dense) held.push_back(g->contiguous());
+    const bool dense = as_it_lies(*g);
+    if (!dense) held.push_back(dense_copy(*g));
     void* data = (dense ? *g : held.back()).data_ptr();
     const int32_t dtype = dtype_code(g->scalar_type());
     arrays.add(data, data, g->numel(), dtype, dtype);
@@ -395,11 +408,12 @@ at::Tensor clip_into(const Refs& grads, const Refs& outs, double max_norm, bool 
     const int64_t size = g.numel(), index = static_cast<int64_t>(i);
     const int32_t dtype = dtype_code(g.scalar_type());
     void* const gp = g.data_ptr();
-    const bool g_dense = g.is_non_overlapping_and_dense();
-    const bool same = &g == &o || (o.data_ptr() == gp && o.dtype() == g.dtype() && o.strides() == g.strides());
+    const bool g_dense = as_it_lies(g);
+    const bool same = &g == &o || (o.data_ptr() == gp && o.dtype() == g.dtype() && o.strides() == g.strides() &&
+                                   o.is_neg() == g.is_neg());
     void* const op = same ? gp : o.data_ptr();
     const int32_t out_dtype = same ? dtype : dtype_code(o.scalar_type());
-    const bool o_dense = same ? g_dense : o.is_non_overlapping_and_dense();
+    const bool o_dense = same ? g_dense : as_it_lies(o);
     if (size) {
       const uintptr_t gb = reinterpret_cast<uintptr_t>(gp), ob = reinterpret_cast<uintptr_t>(op);
       if (o_dense) spans.push_back({ob, ob + size * o.element_size(), index, true});
@@ -407,8 +421,7 @@ at::Tensor clip_into(const Refs& grads, const Refs& outs, double max_norm, bool 
       if (!o_dense) others.push_back({ob, ob, index, true});  // (twice where it overlaps itself: refused)
       if (!same && g_dense) spans.push_back({gb, gb + size * g.element_size(), index, false});
     }
-    if (same ? g_dense
-             : (g.is_contiguous() && o.is_contiguous()) || (g_dense && g.strides() == o.strides())) {
+    if (g_dense && o_dense && ((g.is_contiguous() && o.is_contiguous()) || g.strides() == o.strides())) {
       arrays.add(gp, op, size, dtype, out_dtype);
     } else {
       arrays.add(nullptr, nullptr, size, dtype, out_dtype);
@@ -423,7 +436,7 @@ at::Tensor clip_into(const Refs& grads, const Refs& outs, double max_norm, bool 
                     "; nothing was clipped. Pass error_if_nonfinite=False to clip all the same");
   }
   for (auto& [i, d] : copy_back) {
-    held.push_back(grads[i]->contiguous());
+    held.push_back(dense_copy(*grads[i]));
     d = at::empty(outs[i]->sizes(), outs[i]->options(), at::MemoryFormat::Contiguous);
     arrays.grads[i] = held.back().data_ptr();
     arrays.outs[i] = d.data_ptr();
