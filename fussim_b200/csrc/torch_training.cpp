@@ -5,7 +5,6 @@
 // streams, and captured graphs, never share one).
 #include "torch_training.h"
 
-#include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -13,6 +12,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <numeric>
 #include <stdexcept>
 #include <string>
 #include <vector>
@@ -304,30 +304,123 @@ struct Span {
   bool out;
 };
 
+// The ways to write a number as a sum of terms c * x, 0 <= x <= most, each c at least 1: depth first
+// from the largest c, whose x the rest leaves little choice for where strides are nested, as those
+// of slices are. Gives up after some hundred thousand steps, and then reports what was sought.
+class SumSearch {
+ public:
+  void add(int64_t c, int64_t most) {
+    if (most < 1) return;
+    for (Term& t : terms_)
+      if (merge_ && t.c == c) {
+        t.most += most;
+        return;
+      }
+    terms_.push_back({c, most, 0, 0});
+  }
+  explicit SumSearch(bool merge) : merge_(merge) {}  // equal c count as one term
+  int ways(int64_t target, int sought) {
+    std::sort(terms_.begin(), terms_.end(), [](const Term& a, const Term& b) { return a.c > b.c; });
+    int64_t rest = 0, gcd = 0;
+    for (size_t k = terms_.size(); k-- > 0;) {
+      terms_[k].after = rest;
+      rest += terms_[k].c * terms_[k].most;
+      terms_[k].gcd = gcd = std::gcd(gcd, terms_[k].c);
+    }
+    if (target < 0 || target > rest) return 0;
+    return search(0, target, sought);
+  }
+
+ private:
+  struct Term {
+    int64_t c, most, after, gcd;  // after: the most that the terms behind add; gcd: of these and c
+  };
+  int search(size_t k, int64_t target, int sought) {
+    if (k == terms_.size()) return target == 0;
+    const Term& t = terms_[k];
+    if (target % t.gcd != 0) return 0;
+    int found = 0;
+    const int64_t least = target > t.after ? (target - t.after + t.c - 1) / t.c : 0;
+    for (int64_t x = std::min(t.most, target / t.c); x >= least && found < sought; --x) {
+      if (++steps_ > kSteps) return sought;
+      found += search(k + 1, target - x * t.c, sought - found);
+    }
+    return found;
+  }
+  static constexpr int kSteps = 300000;
+  std::vector<Term> terms_;
+  bool merge_;
+  int steps_ = 0;
+};
+
+// An output and the bytes that it reaches over; it fills them where no tensor is given.
+struct Reach {
+  uintptr_t begin, end;
+  int64_t index;
+  const at::Tensor* tensor;
+};
+Reach reach_of(const at::Tensor& t, int64_t index) {
+  int64_t last = 0;
+  for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
+  const uintptr_t begin = reinterpret_cast<uintptr_t>(t.data_ptr());
+  return {begin, begin + (last + 1) * t.element_size(), index, &t};
+}
+
+// Whether a number of the tensor has two indices.
+bool overlaps_itself(const at::Tensor& t) {
+  SumSearch differences(/*merge=*/false);  // of two indices in each dimension, from -(size - 1) up
+  int64_t none = 0;
+  for (int64_t d = 0; d < t.dim(); ++d) {
+    if (t.size(d) > 1 && t.stride(d) == 0) return true;
+    differences.add(t.stride(d), 2 * (t.size(d) - 1));
+    none += (t.size(d) - 1) * t.stride(d);
+  }
+  return differences.ways(none, 2) > 1;  // other than all differences zero
+}
+
+bool share_memory(const Reach& a, const Reach& b) {
+  if (a.end <= b.begin || b.end <= a.begin) return false;
+  SumSearch bytes(/*merge=*/true);  // of a from its first on, and of b from its last down
+  for (const Reach* r : {&a, &b}) {
+    if (!r->tensor) {
+      bytes.add(1, static_cast<int64_t>(r->end - r->begin) - 1);
+      continue;
+    }
+    const int64_t size = static_cast<int64_t>(r->tensor->element_size());
+    bytes.add(1, size - 1);
+    for (int64_t d = 0; d < r->tensor->dim(); ++d)
+      bytes.add(r->tensor->stride(d) * size, r->tensor->size(d) - 1);
+  }
+  return bytes.ways(static_cast<int64_t>(b.end - 1 - a.begin), 1) > 0;
+}
+
 // Refuses outputs that overlap each other or a gradient (but for outs[i] being grads[i]): two
 // CTAs would write the same numbers, or read what another has already scaled. Tensors that do
-// not fill their memory (`others`) are copied before and after the kernels, which touch the
-// copies alone; of those it is enough that no output is given twice or overlaps itself.
-void check_overlap(std::vector<Span>& spans, std::vector<Span>& others) {
+// not fill their memory are copied before and after the kernels, which touch the copies alone; of
+// those it is enough that no such output (they come in `outs`) overlaps itself or any other.
+void check_overlap(std::vector<Span>& spans, std::vector<Reach>& outs) {
   const auto by_begin = [](const Span& a, const Span& b) { return a.begin < b.begin; };
-  const auto sort = [&](std::vector<Span>& v) {
-    if (!std::is_sorted(v.begin(), v.end(), by_begin)) std::sort(v.begin(), v.end(), by_begin);
-  };
   const auto refuse = [](int64_t index) {
     value_error("tensors that are written must not overlap themselves, each other or another gradient "
                 "(the same tensor twice, or views of the same memory; at index " +
                 std::to_string(index) + ")");
   };
-  sort(spans);
+  if (!std::is_sorted(spans.begin(), spans.end(), by_begin)) std::sort(spans.begin(), spans.end(), by_begin);
   uintptr_t any_end = 0, out_end = 0;  // how far the spans so far reach
   for (const Span& s : spans) {
     if (s.begin < (s.out ? any_end : out_end)) refuse(s.index);
     any_end = std::max(any_end, s.end);
     if (s.out) out_end = std::max(out_end, s.end);
   }
-  sort(others);
-  for (size_t i = 1; i < others.size(); ++i)
-    if (others[i].begin == others[i - 1].begin) refuse(others[i].index);
+  if (outs.empty()) return;
+  for (const Reach& r : outs)
+    if (overlaps_itself(*r.tensor)) refuse(r.index);
+  for (const Span& s : spans)
+    if (s.out) outs.push_back({s.begin, s.end, s.index, nullptr});
+  std::sort(outs.begin(), outs.end(), [](const Reach& a, const Reach& b) { return a.begin < b.begin; });
+  for (size_t i = 0; i < outs.size(); ++i)
+    for (size_t j = i + 1; j < outs.size() && outs[j].begin < outs[i].end; ++j)
+      if ((outs[i].tensor || outs[j].tensor) && share_memory(outs[i], outs[j])) refuse(outs[j].index);
 }
 
 struct ClipArrays {
@@ -399,7 +492,8 @@ at::Tensor clip_into(const Refs& grads, const Refs& outs, double max_norm, bool 
   const at::cuda::OptionalCUDAGuard guard(grads[0]->device());
   const size_t n = grads.size();
   ClipArrays arrays(n);
-  std::vector<Span> spans, others;
+  std::vector<Span> spans;
+  std::vector<Reach> scattered;  // outputs that are not written as they lie
   spans.reserve(n);
   std::vector<at::Tensor> held;                         // dense stand-ins of gradients
   std::vector<std::pair<size_t, at::Tensor>> copy_back;  // (index of an output, its stand-in)
@@ -417,8 +511,7 @@ at::Tensor clip_into(const Refs& grads, const Refs& outs, double max_norm, bool 
     if (size) {
       const uintptr_t gb = reinterpret_cast<uintptr_t>(gp), ob = reinterpret_cast<uintptr_t>(op);
       if (o_dense) spans.push_back({ob, ob + size * o.element_size(), index, true});
-      else if (at::has_internal_overlap(o) == at::MemOverlap::Yes) others.push_back({ob, ob, index, true});
-      if (!o_dense) others.push_back({ob, ob, index, true});  // (twice where it overlaps itself: refused)
+      else scattered.push_back(reach_of(o, index));
       if (!same && g_dense) spans.push_back({gb, gb + size * g.element_size(), index, false});
     }
     if (g_dense && o_dense && ((g.is_contiguous() && o.is_contiguous()) || g.strides() == o.strides())) {
@@ -428,7 +521,7 @@ at::Tensor clip_into(const Refs& grads, const Refs& outs, double max_norm, bool 
       copy_back.emplace_back(i, at::Tensor());
     }
   }
-  check_overlap(spans, others);
+  check_overlap(spans, scattered);
   if (error_if_nonfinite) {
     const double norm = norm_of(grads).item<double>();
     if (!std::isfinite(norm))

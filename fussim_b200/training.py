@@ -112,10 +112,11 @@ def clip_grad_norm(
     into ``out`` (or new tensors of the same types). ``out`` has a tensor for each gradient, of
     its shape, and of its type or float32 (the 32-bit gradients of a mixed-precision
     optimiser); ``out[i]`` may be ``grads[i]``. Otherwise no two of the tensors written, and
-    no gradient and another's output, may share memory. A norm that is NaN makes everything
-    NaN, an infinite gradient makes finite numbers 0; ``error_if_nonfinite`` raises instead, before
-    anything is written, at the price of a host synchronisation. Tensors whose numbers do not
-    fill their memory are copied once more. Not differentiable, as :func:`grad_norm`.
+    no gradient and another's output, may share memory: ValueError (a gradient that does not
+    fill its memory is copied before anything is written, and may). A norm that is NaN makes
+    everything NaN, an infinite gradient makes finite numbers 0; ``error_if_nonfinite`` raises
+    instead, before anything is written, at the price of a host synchronisation. Tensors whose
+    numbers do not fill their memory are copied once more. Not differentiable, as ``grad_norm``.
     """
     return _ensure_cuda_extension().clip_grad_norm(
         list(grads), float(max_norm), None if out is None else list(out), error_if_nonfinite
