@@ -523,7 +523,12 @@ at::Tensor clip_into(const Refs& grads, const Refs& outs, double max_norm, bool 
   }
   check_overlap(spans, scattered);
   if (error_if_nonfinite) {
-    const double norm = norm_of(grads).item<double>();
+    const at::Tensor probe = norm_of(grads);
+    double norm = 0.0;
+    {
+      const py::gil_scoped_release other_threads_run;  // while this one waits for the device
+      norm = probe.item<double>();
+    }
     if (!std::isfinite(norm))
       runtime_error("the gradients' norm is " + std::to_string(norm) +
                     "; nothing was clipped. Pass error_if_nonfinite=False to clip all the same");
@@ -589,10 +594,14 @@ std::tuple<py::list, at::Tensor> clip_grad_norm(const py::list& list, double max
 at::Tensor clip_grad_norm_(const py::list& parameters, double max_norm, bool error_if_nonfinite) {
   check_max_norm(max_norm);
   Refs grads;
+  std::vector<at::Tensor> held;  // another thread may drop a parameter's gradient during the wait
   grads.reserve(parameters.size());
+  if (error_if_nonfinite) held.reserve(parameters.size());
   for (size_t i = 0; i < parameters.size(); ++i) {
     const at::Tensor& g = tensor_of(PyList_GET_ITEM(parameters.ptr(), i), "parameters", i).grad();
-    if (g.defined()) grads.push_back(&g);
+    if (!g.defined()) continue;
+    if (error_if_nonfinite) held.push_back(g);
+    grads.push_back(error_if_nonfinite ? &held.back() : &g);
   }
   check_grads(grads, "clip_grad_norm_");
   return grads.empty() ? zero_norm() : clip_into(grads, grads, max_norm, error_if_nonfinite);
