@@ -13,8 +13,11 @@ outside the repository, so the built files travel with a copy of the tree.
 
 from __future__ import annotations
 
+import functools
+import hashlib
 import os
 import re
+import shutil
 import subprocess
 import sys
 import sysconfig
@@ -60,11 +63,31 @@ def engine_sources():
             if f.endswith((".cu", ".cuh", ".h"))]
 
 
-def _compile_all(commands, verbose):
-    """Run the compile commands side by side; returns what each wrote to standard error."""
+def _compile(job, verbose):
+    """Runs a compile command into a file of its own, which takes the object's place when it is
+    whole: a build that is killed, or another one beside it, leaves no half of an object."""
+    cmd, target = job
+    part = f"{target}.{os.getpid()}.part"
+    try:
+        res = _run([*cmd, "-o", part], verbose)
+        os.replace(part, target)
+        return res.stderr
+    finally:
+        if os.path.exists(part):
+            os.remove(part)
+
+
+def _compile_all(jobs, verbose):
+    """Run the compile jobs, (command, object), side by side; returns what each wrote to standard
+    error."""
     os.makedirs(OBJ, exist_ok=True)
     with ThreadPoolExecutor(max_workers=max(1, os.cpu_count() or 1)) as pool:
-        return [r.stderr for r in pool.map(lambda cmd: _run(cmd, verbose), commands)]
+        return list(pool.map(lambda job: _compile(job, verbose), jobs))
+
+
+@functools.lru_cache(maxsize=None)
+def _compiler_version(compiler):
+    return _run([compiler, "--version"], False).stdout
 
 
 def _includes(source, seen=None):
@@ -83,24 +106,48 @@ def _includes(source, seen=None):
     return list(seen)
 
 
-def _object(source):
-    return os.path.join(OBJ, os.path.basename(source) + ".o")
+def _object(source, command, *versions):
+    """The object file of a source compiled by this command (all but the output): its name tells
+    the command, the compiler's version and the others given, so that an object is used again only
+    for what it was compiled with. Where the tree lies does not count."""
+    key = "\0".join([*command, _compiler_version(command[0]), *versions]).replace(ROOT, "")
+    key = hashlib.sha256(key.encode()).hexdigest()[:12]
+    return os.path.join(OBJ, f"{os.path.basename(source)}.{key}.o")
+
+
+def _link(cmd, target, verbose):
+    part = f"{target}.{os.getpid()}.part"
+    try:
+        _run([*cmd, "-o", part], verbose)
+        os.replace(part, target)
+    finally:
+        if os.path.exists(part):
+            os.remove(part)
+
+
+def _forget_others(sources, objects):
+    """Removes the objects of these sources that other commands compiled."""
+    for name in os.listdir(OBJ):
+        path = os.path.join(OBJ, name)
+        if name.endswith(".o") and path not in objects and \
+                any(name.startswith(os.path.basename(s) + ".") for s in sources):
+            os.remove(path)
 
 
 def build_engine(force: bool = False, verbose: bool = False, ptxas_info: bool = False) -> str:
-    deps = engine_sources() + [os.path.join(INCLUDE, "fussim_b200.h")]
-    if not force and not _stale(LIB, deps):
-        return LIB
     cus = [s for s in engine_sources() if s.endswith(".cu")]
-    jobs = []
-    for cu in cus:
-        if force or ptxas_info or _stale(_object(cu), _includes(cu)):
-            cmd = [_nvcc(), *ARCH_FLAGS, *NVCC_FLAGS, "-c", "-I", INCLUDE, "-o", _object(cu), cu]
-            if ptxas_info:
-                cmd.insert(1, "-Xptxas=-v")
-            jobs.append(cmd)
+    if not force and shutil.which(_nvcc()) is None and \
+            not _stale(LIB, [*engine_sources(), os.path.join(INCLUDE, "fussim_b200.h")]):
+        return LIB  # built elsewhere
+    commands = {cu: [_nvcc(), *ARCH_FLAGS, *NVCC_FLAGS, "-I", INCLUDE, "-c", cu] for cu in cus}
+    objects = {cu: _object(cu, commands[cu]) for cu in cus}
+    jobs = [([*commands[cu], *(["-Xptxas=-v"] if ptxas_info else [])], objects[cu]) for cu in cus
+            if force or ptxas_info or _stale(objects[cu], _includes(cu))]
+    if not jobs and not _stale(LIB, objects.values()):
+        return LIB
     infos = _compile_all(jobs, verbose)
-    _run([_nvcc(), *ARCH_FLAGS, "-shared", "-o", LIB, *[_object(cu) for cu in cus]], verbose)
+    _link([_nvcc(), *ARCH_FLAGS, "-shared", *objects.values()], LIB, verbose)
+    _forget_others(cus, objects.values())
     if ptxas_info:
         sys.stdout.write("".join(infos))
     return LIB
@@ -109,26 +156,29 @@ def build_engine(force: bool = False, verbose: bool = False, ptxas_info: bool = 
 def build_torch_ext(force: bool = False, verbose: bool = False) -> str:
     # The extension links the library by name and finds it at run time, so a rebuilt
     # library does not require relinking the extension.
-    cpps = [os.path.join(CSRC, f) for f in sorted(os.listdir(CSRC)) if f.endswith(".cpp")]
-    deps = sorted({d for cpp in cpps for d in _includes(cpp)})
-    if not force and not _stale(EXT, deps):
-        return EXT
     import torch
     from torch.utils import cpp_extension as ce
 
+    cpps = [os.path.join(CSRC, f) for f in sorted(os.listdir(CSRC)) if f.endswith(".cpp")]
     incs = ce.include_paths(device_type="cuda") + [sysconfig.get_paths()["include"], INCLUDE]
     libdirs = ce.library_paths(device_type="cuda")
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
-    flags = ["-O3", "-std=c++17", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
+    flags = ["g++", "-O3", "-std=c++17", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
              "-DTORCH_EXTENSION_NAME=_C", "-DTORCH_API_INCLUDE_EXTENSION_H",
              *[f"-I{i}" for i in incs]]
-    _compile_all([["g++", *flags, "-c", cpp, "-o", _object(cpp)] for cpp in cpps
-                  if force or _stale(_object(cpp), _includes(cpp))], verbose)
-    cmd = ["g++", "-shared", *[_object(cpp) for cpp in cpps], "-o", EXT,
-           *[f"-L{d}" for d in libdirs], f"-L{PKG}", "-lfussim_b200", "-lc10", "-ltorch",
-           "-ltorch_cpu", "-ltorch_python", "-lc10_cuda", "-ltorch_cuda", "-lcudart",
-           "-Wl,-rpath,$ORIGIN"]
-    _run(cmd, verbose)
+    if not force and shutil.which("g++") is None and \
+            not _stale(EXT, {d for cpp in cpps for d in _includes(cpp)}):
+        return EXT
+    commands = {cpp: [*flags, "-c", cpp] for cpp in cpps}
+    objects = {cpp: _object(cpp, commands[cpp], torch.__version__, sys.version) for cpp in cpps}
+    jobs = [(commands[cpp], objects[cpp]) for cpp in cpps if force or _stale(objects[cpp], _includes(cpp))]
+    if not jobs and not _stale(EXT, objects.values()):
+        return EXT
+    _compile_all(jobs, verbose)
+    _link(["g++", "-shared", *objects.values(), *[f"-L{d}" for d in libdirs], f"-L{PKG}",
+           "-lfussim_b200", "-lc10", "-ltorch", "-ltorch_cpu", "-ltorch_python", "-lc10_cuda",
+           "-ltorch_cuda", "-lcudart", "-Wl,-rpath,$ORIGIN"], EXT, verbose)
+    _forget_others(cpps, objects.values())
     return EXT
 
 
