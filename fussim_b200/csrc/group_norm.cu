@@ -25,7 +25,9 @@ constexpr unsigned kSms = 148;
 // CTAs of one wave.
 constexpr int64_t kWave = kSms * fssim::kNormResident;
 // Bytes of input that are to stay in L2 from the reducing pass to the applying one, of larger
-// tensors (1x64x1080x1920 16-bit forward 152 us without, 143 with; flat from 64 to 120 MB).
+// tensors (1x64x1080x1920 16-bit forward 152 us without, 143 with; flat from 64 to 120 MB). Smaller
+// tensors, and what a pass writes of them, keep the usual priority: read after 60 MB of other
+// traffic, 33 and 67 MB outputs cost 2.5 and 1.4 us less so (by the very next norm 1.2 us more).
 constexpr double kKeptBytes = 80 << 20;
 
 // Vectors of a thread's batch and batches of its ring: 64 KB of ring for a CTA in every pass. The
@@ -425,7 +427,7 @@ int forward_impl(const fssim_group_norm_forward_args* a, cudaStream_t stream) {
   const size_t E = elem_size(a->dtype);
   if (!aligned(a->x, E) || !aligned(a->y, E))
     return fail(FSSIM_ERR_ARGUMENT, "x and y must be aligned to their element size");
-  const ForwardPlan plan = plan_forward(*a);
+  ForwardPlan plan = plan_forward(*a);
   if (!plan.resident.slots && a->P / plan.g.S >= (int64_t{1} << 30))
     return fail(FSSIM_ERR_SHAPE, "a CTA's part has 2^30 pixels or more");
   if (plan.bytes && (!a->workspace || a->workspace_bytes < plan.bytes))
@@ -445,7 +447,7 @@ int forward_impl(const fssim_group_norm_forward_args* a, cudaStream_t stream) {
     return dispatch<ForwardResident>(a->dtype, plan.V, a->activation, p, plan.resident, stream);
   }
   p.g = plan.g;
-  p.g.keep = kept_share(static_cast<double>(a->N) * a->P * a->C * E);
+  p.g.keep = plan.apply.keep = kept_share(static_cast<double>(a->N) * a->P * a->C * E);
   p.partial = static_cast<float2*>(a->workspace);
   p.channel = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + plan.partial);
   p.merges = plan.merges;
