@@ -672,20 +672,20 @@ struct NormMoments {
     const float2 each = splat2(kWhole ? 1.f / U : 1.f / taken);
 #pragma unroll
     for (int v = 0; v < N; ++v) {
-      // the mean from the distances to the first value: a sum of equal values would round
+      // From the distances e to the batch's first value: a sum of equal values would round. They
+      // are small wherever the spread is, whatever the mean, and that value being one of the
+      // batch, sum e^2 is at most U times the sum of squares around the mean: few digits cancel.
       const float2 first = neg2(f[0][v]);
-      float2 sum = splat2(0.f);
+      float2 sum = splat2(0.f), q = splat2(0.f);
 #pragma unroll
       for (int u = 1; u < U; ++u)
-        if (kWhole || u < k) sum = add2(sum, add2(f[u][v], first));
-      const float2 m = fma2(sum, each, f[0][v]), minus = neg2(m);
-      float2 q = splat2(0.f);
-#pragma unroll
-      for (int u = 0; u < U; ++u)
         if (kWhole || u < k) {
-          const float2 d = add2(f[u][v], minus);
-          q = fma2(d, d, q);
+          const float2 e = add2(f[u][v], first);
+          sum = add2(sum, e);
+          q = fma2(e, e, q);
         }
+      const float2 shift = mul2(sum, each), m = add2(f[0][v], shift);
+      q = fma2(neg2(sum), shift, q);
       const float2 d = add2(m, neg2(mean[v]));
       mean[v] = fma2(d, splat2(share), mean[v]);
       // (in this order: the first batch's distance is its mean, whose square may be infinite, times 0)
