@@ -21,7 +21,7 @@ using fssim_host::NvtxRange;
 
 constexpr int64_t kMaxChannels = int64_t{1} << 23;  // 65535 slices of at least 256 vectors
 constexpr int64_t kMaxSamples = int64_t{1} << 30;
-constexpr unsigned kSms = 148;
+constexpr unsigned kSms = 148;  // a B200's; grids of other sizes would be right too
 // CTAs of one wave.
 constexpr int64_t kWave = kSms * fssim::kNormResident;
 // Bytes of input that are to stay in L2 from the reducing pass to the applying one, of larger
@@ -45,9 +45,10 @@ constexpr double kResidentBytes = 8 << 20;
 constexpr int kResidentSlots = 8;
 constexpr int64_t kSliceBytes = 64;
 // An applying pass of one wave merges the statistics itself, without a launch between, where a
-// sample has at most this many parts times groups: each CTA reads them all. On a B200 the
-// 8x128x256^2 forward (37 parts, 32 groups) takes 70.8 us so and 73.2 with the launch,
-// 1x128x128^2 (128 parts) 13.7 and 10.9.
+// sample has at most this many parts times groups: each CTA reads them all. On a B200, 128 channels
+// in 16 bits, 128^2 and 256^2 pixels, 1 to 16 samples, 1 to 128 groups: without the launch 3 to 8 % less
+// time up to 1,184 of them (8x128x256^2, 32 groups, 67.9 us against 70.3), between 3 % less and 5 % more
+// near 2,368, as much to 18 % more from 4,736 on (1x128x256^2, 32 groups, 20.3 against 17.1).
 constexpr int kMergeMost = 2048;
 constexpr int64_t kApplySteps = 32, kApplyWaves = 6;
 
@@ -327,7 +328,7 @@ int forward_kernels(const NormParams& p, const NormGeometry& apply, cudaStream_t
     st = launch(fssim::norm_merge_kernel, team_grid(p.g, team), 1, 0, p, s, "group norm merge launch", team);
     if (st) return st;
   }
-  NormParams q = p;
+  NormParams q = p;  // (the applying pass reads x ahead of its wait: never without a launch before)
   q.g = apply;
   return launch_pass<fssim::norm_apply_kernel<T, V, ACT, kApplyU, kApplyB>, Apply::kRingBytes>(
       q.g, q, Apply::kRingBytes, s, "group norm launch");
@@ -345,7 +346,7 @@ int backward_kernels(const NormParams& p, cudaStream_t s) {
   st = launch(fssim::norm_grad_merge_kernel, team_grid(p.g, team), 1, 0, p, s,
               "group norm gradient merge launch", team, cols);
   if (st || !p.out) return st;
-  NormParams q = p;
+  NormParams q = p;  // (likewise, with dy)
   q.g = apply_geometry(p.g);
   q.fold_params = p.g.N > 1 && (p.dweight || p.dbias);
   return launch_pass<fssim::norm_grad_apply_kernel<T, V, ACT, kGradU, kGradB>, 2 * Walk::kRingBytes>(

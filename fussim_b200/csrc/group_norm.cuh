@@ -48,7 +48,7 @@ constexpr int kNormApplyResident = 2;  // and of an applying pass
 enum NormAct { kNormActNone = 0, kNormActSilu = 1, kNormActRelu = 2 };
 
 struct NormGeometry {
-  int64_t N;   // samples of this launch
+  int64_t N;   // samples
   int64_t P;   // pixels per sample
   int C, G, Cg;
   int period;  // pixels of a span
@@ -837,7 +837,7 @@ __device__ __forceinline__ void norm_merge_sums(const NormGeometry& g, const Nor
 }
 
 // ---- forward: statistics ----
-// Bound by DRAM: 8x128x512^2 16-bit (537 MB) 86 us, 6.3 TB/s; 1x64x1080x1920 (265 MB) 48 us. Two
+// Bound by DRAM: 8x128x512^2 16-bit (537 MB) 88 us, 6.2 TB/s; 1x64x1080x1920 (265 MB) 48 us. Two
 // CTAs an SM and batches of 8: more CTAs or shorter batches ran up to 6 % slower.
 template <typename T, int V, int U, int B>
 __global__ void __launch_bounds__(kNormThreads, kNormResident) norm_stats_kernel(const __grid_constant__ NormParams p) {
@@ -983,7 +983,7 @@ __device__ __forceinline__ void norm_merge_here(const NormParams& p, int n, floa
 }
 
 // ---- forward: y ----
-// Bound by DRAM on large tensors (8x128x512^2 16-bit, 537 MB in and out: 165 us, 6.2 TB/s), by the
+// Bound by DRAM on large tensors (8x128x512^2 16-bit, 537 MB in and out: 164 us, 6.2 TB/s), by the
 // special-function unit where most of x comes from L2 (SiLU takes two of its operations an
 // element; 8x128x256^2: 46 us, 4.6 TB/s).
 constexpr int kNormMergeGroups = 256;  // groups that an applying pass merges itself, at most
@@ -1002,8 +1002,8 @@ __global__ void __launch_bounds__(kNormThreads, kNormApplyResident) norm_apply_k
     x.start(walk, slot, todo, policy.pass);
     x.commit();
   };
-  // x was complete before the statistics' launch began its work, so the first reads need not
-  // wait for the launches in between to end
+  // x was complete before the statistics' launch passed its wait, so the first reads need not wait
+  // for the launches in between to end (which rests on that launch being there, before this one)
 #pragma unroll
   for (int j = 0; j < B - 1; ++j) start(j, walk.count - j * U);
   grid_dependency_wait();
@@ -1042,7 +1042,7 @@ __global__ void __launch_bounds__(kNormThreads, kNormApplyResident) norm_apply_k
 }
 
 // ---- backward: per-channel sums of one part ----
-// Bound by DRAM: 8x128x512^2 16-bit (1,074 MB) 173 us, 6.2 TB/s; 1x48x517x999 FP32 (198 MB) 38 us.
+// Bound by DRAM: 8x128x512^2 16-bit (1,074 MB) 177 us, 6.1 TB/s; 1x48x517x999 FP32 (198 MB) 36 us.
 template <typename T, int V, int ACT, int U, int B>
 __global__ void __launch_bounds__(kNormThreads, kNormResident) norm_grad_sums_kernel(const __grid_constant__ NormParams p) {
   const NormGeometry& g = p.g;
@@ -1153,6 +1153,7 @@ __global__ void __launch_bounds__(kNormThreads) norm_grad_merge_kernel(const __g
     }
     if (mine && sub == 0) {
       v2 *= rstd;
+      // (rounded to FP32: 2^-24 of each sample's sum, and half the traffic of the last sum)
       p.sums[n * g.C + ch] = make_float2(static_cast<float>(v1), static_cast<float>(v2));
       const double w = p.weight ? load_weight(p.weight, p.weight_dtype, ch) : 1.0;
       w1 += w * v1;
@@ -1207,7 +1208,7 @@ __global__ void __launch_bounds__(kNormThreads) norm_param_grad_kernel(const __g
 }
 
 // ---- backward: dx ----
-// Bound by DRAM: 8x128x512^2 16-bit (1,074 MB in, 537 out) 236 us, 6.7 TB/s; 8x128x256^2 64 us.
+// Bound by DRAM: 8x128x512^2 16-bit (1,074 MB in, 537 out) 235 us, 6.7 TB/s; 8x128x256^2 64 us.
 template <typename T, int V, int ACT, int U, int B>
 __global__ void __launch_bounds__(kNormThreads, kNormApplyResident) norm_grad_apply_kernel(const __grid_constant__ NormParams p) {
   const NormGeometry& g = p.g;
@@ -1406,6 +1407,7 @@ __global__ void __launch_bounds__(kNormThreads) norm_grad_resident_kernel(const 
     const float rstd = p.rstd[static_cast<int64_t>(t.n) * g.G + c / g.Cg];
     v2 *= rstd;
     const double w = p.weight ? load_weight(p.weight, p.weight_dtype, c) : 1.0;
+    // (FP32 here and in `sums`: 2^-24 of a channel's own sum, against the FP32 terms' roundings)
     weighted[i] = make_float2(static_cast<float>(w * v1 * g.inv_m), static_cast<float>(w * v2 * g.inv_m));
     if (t.s == 0) {
       if (g.N == 1) {  // one sample: its sums are the parameters' gradients

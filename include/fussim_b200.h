@@ -97,7 +97,8 @@ int fssim_set_gather_timeout_us(long long us);
 #define FSSIM_KERNELS_AUTO 2
 int fssim_set_loss_kernels(int family);
 
-/* Number of SMs the kernels' persistent grids leave unused (default 0), for callers that
+/* Number of SMs the losses' persistent grids leave unused (default 0; the grids of section 4
+ * are not persistent and take no notice), for callers that
  * run another kernel concurrently, e.g. a collective overlapping the backward: a grid that
  * fills every SM would otherwise wait for that kernel's blocks to leave before its last
  * CTAs start. Process-wide; n >= 0 (FSSIM_ERR_ARGUMENT otherwise). */
