@@ -287,13 +287,20 @@ __device__ __noinline__ double clip_piece_squares(const T* src, int64_t b, int64
   return acc;
 }
 
-// The factor, as two that are multiplied in turn: one below 2^-120 (a norm near or beyond
-// FP32's largest number) is carried as 2^64 times itself and 2^-64, so that it keeps its bits.
+// The factor, as an FP32 number and what its rounding lost, so that a scaled number is rounded once:
+// with the rounded factor alone it would be off by up to two halves of a step. One below 2^-96
+// (a norm near or beyond FP32's largest number) is carried as 2^64 times itself, so that both
+// keep their bits, and the product times 2^-64.
 struct ClipFactor {
-  float a, b;
-  __device__ __forceinline__ explicit ClipFactor(double c)
-      : a(static_cast<float>(c < 0x1p-120 ? c * 0x1p64 : c)), b(c < 0x1p-120 ? 0x1p-64f : 1.f) {}
-  __device__ __forceinline__ float operator*(float v) const { return v * a * b; }
+  float high, low, back;
+  __device__ __forceinline__ explicit ClipFactor(double c) {
+    const bool tiny = c < 0x1p-96;
+    if (tiny) c *= 0x1p64;
+    high = static_cast<float>(c);
+    low = static_cast<float>(c - high);
+    back = tiny ? 0x1p-64f : 1.f;
+  }
+  __device__ __forceinline__ float operator*(float v) const { return fmaf(v, high, v * low) * back; }
 };
 
 template <typename S, typename D>
