@@ -7,6 +7,7 @@
 
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
+#include <c10/util/SmallVector.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 
@@ -348,22 +349,27 @@ class SumSearch {
     return found;
   }
   static constexpr int kSteps = 300000;
-  std::vector<Term> terms_;
+  c10::SmallVector<Term, 12> terms_;
   bool merge_;
   int steps_ = 0;
 };
 
-// An output and the bytes that it reaches over; it fills them where no tensor is given.
+// An output and the bytes that it reaches over; it fills them where no tensor is given. Its numbers
+// begin at multiples of `grid` bytes from the first.
 struct Reach {
   uintptr_t begin, end;
   int64_t index;
   const at::Tensor* tensor;
+  uintptr_t grid;
 };
 Reach reach_of(const at::Tensor& t, int64_t index) {
-  int64_t last = 0;
-  for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
+  int64_t last = 0, grid = 0;
+  for (int64_t d = 0; d < t.dim(); ++d) {
+    last += (t.size(d) - 1) * t.stride(d);
+    if (t.size(d) > 1) grid = std::gcd(grid, t.stride(d));
+  }
   const uintptr_t begin = reinterpret_cast<uintptr_t>(t.data_ptr());
-  return {begin, begin + (last + 1) * t.element_size(), index, &t};
+  return {begin, begin + (last + 1) * t.element_size(), index, &t, grid * t.element_size()};
 }
 
 // Whether a number of the tensor has two indices.
@@ -380,6 +386,11 @@ bool overlaps_itself(const at::Tensor& t) {
 
 bool share_memory(const Reach& a, const Reach& b) {
   if (a.end <= b.begin || b.end <= a.begin) return false;
+  // columns of one buffer: numbers of both lie on the same grid, these between those
+  if (a.tensor && b.tensor && a.grid == b.grid && a.grid > 0 && a.begin <= b.begin) {
+    const uintptr_t beside = (b.begin - a.begin) % a.grid;
+    if (beside >= a.tensor->element_size() && beside + b.tensor->element_size() <= a.grid) return false;
+  }
   SumSearch bytes(/*merge=*/true);  // of a from its first on, and of b from its last down
   for (const Reach* r : {&a, &b}) {
     if (!r->tensor) {
@@ -416,7 +427,7 @@ void check_overlap(std::vector<Span>& spans, std::vector<Reach>& outs) {
   for (const Reach& r : outs)
     if (overlaps_itself(*r.tensor)) refuse(r.index);
   for (const Span& s : spans)
-    if (s.out) outs.push_back({s.begin, s.end, s.index, nullptr});
+    if (s.out) outs.push_back({s.begin, s.end, s.index, nullptr, 0});
   std::sort(outs.begin(), outs.end(), [](const Reach& a, const Reach& b) { return a.begin < b.begin; });
   for (size_t i = 0; i < outs.size(); ++i)
     for (size_t j = i + 1; j < outs.size() && outs[j].begin < outs[i].end; ++j)
