@@ -396,8 +396,8 @@ __global__ void __launch_bounds__(kClipThreads) grad_norm_kernel(const double* p
 
 // The second read begins at the ends of the norm's pass's ranges, which that pass read last and L2
 // still holds: a range is cut into `cuts` pieces, and the CTAs take the last piece of every range
-// first. Bound by DRAM: 59 million FP32 (236 MB in and out) 80 us, 5.3 TB/s; 160 million BF16
-// into FP32 (320 MB in, 640 out) 158 us, 5.7 TB/s.
+// first. Bound by DRAM: 59 million FP32 (236 MB in and out) 80 us, 5.2 TB/s; 160 million BF16
+// into FP32 (320 MB in, 640 out) 162 us, 5.6 TB/s.
 template <int K>
 __global__ void __launch_bounds__(kClipThreads, kClipResident)
     grad_clip_kernel(const __grid_constant__ ClipTable<K> t) {

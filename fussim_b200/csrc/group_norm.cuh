@@ -22,10 +22,11 @@
 //   beginning: what the reducing pass read last is what L2 still holds.
 //
 // Statistics: a thread takes U spans at a time, forms each channel's mean and sum of squared
-// deviations of those U values (two passes over registers), and merges them into its running
-// pair (the pairwise update of Chan, Golub and LeVeque, 1979). No sum of raw squares is ever
-// formed, so a mean far from zero costs no digits. Threads, channels, parts and slices are
-// merged likewise, in a fixed order (results repeat bit for bit), across parts in FP64.
+// deviations of those U values (from their distances to the first of them), and merges them into
+// its running pair (the pairwise update of Chan, Golub and LeVeque, 1979). No sum of raw squares is
+// ever formed, so a mean far from zero costs no digits. Threads, channels, parts and slices are
+// merged likewise, in a fixed order (results repeat bit for bit), within a CTA in FP32, over a
+// thread's long part and across parts in FP64.
 #pragma once
 
 #include <cooperative_groups.h>
