@@ -219,23 +219,22 @@ int allow_ring(Kernel k, size_t smem, std::atomic<bool> (&done)[64]) {
   return e == cudaSuccess ? FSSIM_OK : fail(FSSIM_ERR_CUDA, cudaGetErrorString(e));
 }
 
-// A pass over the tiles of g, with `smem` of at most MOST bytes of shared memory.
-template <auto K, size_t MOST>
-int launch_pass(const NormGeometry& g, const NormParams& p, size_t smem, cudaStream_t stream, const char* what) {
+// A pass over the tiles of g.
+template <auto K, size_t SMEM>
+int launch_pass(const NormGeometry& g, const NormParams& p, cudaStream_t stream, const char* what) {
   if (g.N * g.S > INT_MAX) return fail(FSSIM_ERR_SHAPE, "more than 2^31 tiles");
   static std::atomic<bool> done[64];
-  const int st = allow_ring(K, MOST, done);
+  const int st = allow_ring(K, SMEM, done);
   if (st) return st;
-  return launch(K, dim3(static_cast<unsigned>(g.N * g.S), static_cast<unsigned>(g.slices)), 1, smem, p, stream, what);
+  return launch(K, dim3(static_cast<unsigned>(g.N * g.S), static_cast<unsigned>(g.slices)), 1, SMEM, p, stream, what);
 }
 
-// A reducing pass over TENSORS tensors. The memory for folded sums only where some thread folds its
-// own: it alone costs the launch up to 1 us (1x128x128^2 16-bit training pass 24.7 against 23.9).
-template <auto K, typename Walk, int TENSORS>
-int launch_reducing(const NormParams& p, cudaStream_t stream, const char* what) {
-  const int64_t most = (static_cast<int64_t>(p.g.part_tiles) + (p.g.extra_tiles > 0)) * Walk::kU;
-  const size_t smem = Walk::reducing_bytes(TENSORS, most > Walk::kFoldSpans);
-  return launch_pass<K, Walk::reducing_bytes(TENSORS, true)>(p.g, p, smem, stream, what);
+// Whether some thread of a reducing pass has more spans than it may add up in FP32. Kernels and
+// memory for folded sums only then: where they are not needed they cost 1 to 4 % (1x128x256^2 16-bit
+// forward 18.1 us against 17.8, 1x128x128^2 training pass 24.7 against 23.9).
+template <typename Walk>
+bool folds(const NormGeometry& g) {
+  return (static_cast<int64_t>(g.part_tiles) + (g.extra_tiles > 0)) * Walk::kU > Walk::kFoldSpans;
 }
 
 int check_common(int dtype, int weight_dtype, int activation, int64_t N, int64_t P, int64_t C,
@@ -318,10 +317,13 @@ dim3 team_grid(const NormGeometry& g, int shift) {
 
 template <typename T, int V, int ACT>
 int forward_kernels(const NormParams& p, const NormGeometry& apply, cudaStream_t s) {
-  using Stats = fssim::NormWalk<T, V, kStatsU, kStatsB, false>;
+  using Short = fssim::NormWalk<T, V, kStatsU, kStatsB, false>;
+  using Long = fssim::NormWalk<T, V, kStatsU, kStatsB, false, true>;
   using Apply = fssim::NormWalk<T, V, kApplyU, kApplyB, true>;
-  int st = launch_reducing<fssim::norm_stats_kernel<T, V, kStatsU, kStatsB>, Stats, 1>(
-      p, s, "group norm statistics launch");
+  const char* what = "group norm statistics launch";
+  int st = folds<Short>(p.g)
+               ? launch_pass<fssim::norm_stats_kernel<T, V, kStatsU, kStatsB, true>, Long::reducing_bytes(1)>(p.g, p, s, what)
+               : launch_pass<fssim::norm_stats_kernel<T, V, kStatsU, kStatsB, false>, Short::reducing_bytes(1)>(p.g, p, s, what);
   if (st) return st;
   if (!p.merges) {
     const int team = team_shift(p.g.S);
@@ -331,14 +333,18 @@ int forward_kernels(const NormParams& p, const NormGeometry& apply, cudaStream_t
   NormParams q = p;  // (the applying pass reads x ahead of its wait: never without a launch before)
   q.g = apply;
   return launch_pass<fssim::norm_apply_kernel<T, V, ACT, kApplyU, kApplyB>, Apply::kRingBytes>(
-      q.g, q, Apply::kRingBytes, s, "group norm launch");
+      q.g, q, s, "group norm launch");
 }
 
 template <typename T, int V, int ACT>
 int backward_kernels(const NormParams& p, cudaStream_t s) {
-  using Walk = fssim::NormWalk<T, V, kGradU, kGradB, false>;
-  int st = launch_reducing<fssim::norm_grad_sums_kernel<T, V, ACT, kGradU, kGradB>, Walk, 2>(
-      p, s, "group norm gradient sums launch");
+  using Short = fssim::NormWalk<T, V, kGradU, kGradB, false>;
+  using Long = fssim::NormWalk<T, V, kGradU, kGradB, false, true>;
+  const char* what = "group norm gradient sums launch";
+  int st =
+      folds<Short>(p.g)
+          ? launch_pass<fssim::norm_grad_sums_kernel<T, V, ACT, kGradU, kGradB, true>, Long::reducing_bytes(2)>(p.g, p, s, what)
+          : launch_pass<fssim::norm_grad_sums_kernel<T, V, ACT, kGradU, kGradB, false>, Short::reducing_bytes(2)>(p.g, p, s, what);
   if (st) return st;
   int cols = 0;  // channels merged at a time, likewise
   while (cols < 5 && (1 << cols) < p.g.Cg) ++cols;
@@ -349,8 +355,8 @@ int backward_kernels(const NormParams& p, cudaStream_t s) {
   NormParams q = p;  // (likewise, with dy)
   q.g = apply_geometry(p.g);
   q.fold_params = p.g.N > 1 && (p.dweight || p.dbias);
-  return launch_pass<fssim::norm_grad_apply_kernel<T, V, ACT, kGradU, kGradB>, 2 * Walk::kRingBytes>(
-      q.g, q, 2 * Walk::kRingBytes, s, "group norm gradient launch");
+  return launch_pass<fssim::norm_grad_apply_kernel<T, V, ACT, kGradU, kGradB>, 2 * Short::kRingBytes>(
+      q.g, q, s, "group norm gradient launch");
 }
 
 // One launch list per (element type, vector width, activation).

@@ -395,7 +395,7 @@ struct NormPolicy {
 // (each thread into slots of its own, so that no barrier is needed): what a thread has in flight
 // is bounded by shared memory instead of registers and does not pause while it computes.
 // Narrower vectors are loaded when they are used.
-template <typename T, int V, int U, int B, bool APPLYING>
+template <typename T, int V, int U, int B, bool APPLYING, bool FOLDS = false>
 struct NormWalk {
   using IO = VecIO<T, V>;
   using Raw = typename IO::Raw;
@@ -403,14 +403,14 @@ struct NormWalk {
   static constexpr int kU = U;
   static constexpr int kRingBytes = kAsync ? kNormThreads * 16 * U * B : 0;
   // Shared memory of a reducing pass over some tensors: their rings, where the merge that follows has
-  // its scratch (four floats per thread and channel), and where a part is `folded`, two FP64 sums per
-  // thread and channel.
+  // its scratch (four floats per thread and channel), and where it FOLDS, two FP64 sums per thread
+  // and channel.
   static constexpr int kScratchBytes = 4 * kNormThreads * V * static_cast<int>(sizeof(float));
   static __host__ __device__ constexpr int wide_offset(int tensors) {
     return tensors * kRingBytes > kScratchBytes ? tensors * kRingBytes : kScratchBytes;
   }
-  static __host__ __device__ constexpr int reducing_bytes(int tensors, bool folded) {
-    return wide_offset(tensors) + (folded ? 2 * kNormThreads * V * static_cast<int>(sizeof(double)) : 0);
+  static __host__ __device__ constexpr int reducing_bytes(int tensors) {
+    return wide_offset(tensors) + (FOLDS ? 2 * kNormThreads * V * static_cast<int>(sizeof(double)) : 0);
   }
 
   int count;       // vectors of this thread
@@ -445,15 +445,14 @@ struct NormWalk {
   }
 
   // start(slot, todo) begins copying the next batch, of which `todo` vectors are left, into that
-  // batch of the ring; use(slot, whole, k) takes one of k vectors (k == U when whole). fold() is
-  // called after each kFoldSpans of a reducing pass that others follow.
+  // batch of the ring; use(slot, whole, k) takes one of k vectors (k == U when whole). A walk that
+  // FOLDS calls fold() after each kFoldSpans that others follow.
   static constexpr int kFoldSpans = 8 * B * U;
   template <typename Start, typename Use, typename Fold>
   __device__ __forceinline__ void run(int prefilled, Start start, Use use, Fold fold) const {
-    constexpr bool kFolds = !APPLYING;
     int todo = count - prefilled * U, left = count;
     while (left > 0) {
-      const int stop = kFolds ? max(left - kFoldSpans, 0) : 0;
+      const int stop = FOLDS ? max(left - kFoldSpans, 0) : 0;
       do {
 #pragma unroll
         for (int b = 0; b < B; ++b) {
@@ -466,7 +465,7 @@ struct NormWalk {
           if (left <= 0) break;
         }
       } while (left > stop);
-      if (kFolds && left > 0) fold();
+      if (FOLDS && left > 0) fold();
     }
   }
   template <typename Start, typename Use>
@@ -699,8 +698,8 @@ struct NormMoments {
 // What a thread adds up over its part of a sample would be one chain of FP32 roundings as long as the
 // part (3,370 terms of 1x255x997x1001 FP32, where the dbias of equal gradients was off by 565 * 2^-24).
 // So every kFoldSpans spans the sums, of at most 64 terms (or 16 batches' moments), go on
-// into FP64 ones in shared memory, two for each of the thread's channels, its own slots. Parts
-// that are shorter never touch them.
+// into FP64 ones in shared memory, two for each of the thread's channels, its own slots. Where no
+// part is that long, kernels without them run (FOLDS).
 template <int V>
 struct NormWide {
   double* own;
@@ -838,15 +837,15 @@ __device__ __forceinline__ void norm_merge_sums(const NormGeometry& g, const Nor
 }
 
 // ---- forward: statistics ----
-// Bound by DRAM: 8x128x512^2 16-bit (537 MB) 88 us, 6.2 TB/s; 1x64x1080x1920 (265 MB) 48 us. Two
+// Bound by DRAM: 8x128x512^2 16-bit (537 MB) 87 us, 6.2 TB/s; 1x64x1080x1920 (265 MB) 49 us. Two
 // CTAs an SM and batches of 8: more CTAs or shorter batches ran up to 6 % slower.
-template <typename T, int V, int U, int B>
+template <typename T, int V, int U, int B, bool FOLDS>
 __global__ void __launch_bounds__(kNormThreads, kNormResident) norm_stats_kernel(const __grid_constant__ NormParams p) {
   const NormGeometry& g = p.g;
   const NormTile t(g, V, false);
   grid_dependency_wait();
   grid_launch_dependents();
-  using Walk = NormWalk<T, V, U, B, false>;
+  using Walk = NormWalk<T, V, U, B, false, FOLDS>;
   const Walk walk(g, t);
   NormSource<Walk, T> x(walk, p.x, 0);
   const NormPolicy policy(g.keep < 1.f);
@@ -984,9 +983,9 @@ __device__ __forceinline__ void norm_merge_here(const NormParams& p, int n, floa
 }
 
 // ---- forward: y ----
-// Bound by DRAM on large tensors (8x128x512^2 16-bit, 537 MB in and out: 164 us, 6.2 TB/s), by the
+// Bound by DRAM on large tensors (8x128x512^2 16-bit, 537 MB in and out: 166 us, 6.1 TB/s), by the
 // special-function unit where most of x comes from L2 (SiLU takes two of its operations an
-// element; 8x128x256^2: 46 us, 4.6 TB/s).
+// element; 8x128x256^2: 47 us, 4.6 TB/s).
 constexpr int kNormMergeGroups = 256;  // groups that an applying pass merges itself, at most
 
 template <typename T, int V, int ACT, int U, int B>
@@ -1043,15 +1042,15 @@ __global__ void __launch_bounds__(kNormThreads, kNormApplyResident) norm_apply_k
 }
 
 // ---- backward: per-channel sums of one part ----
-// Bound by DRAM: 8x128x512^2 16-bit (1,074 MB) 177 us, 6.1 TB/s; 1x48x517x999 FP32 (198 MB) 36 us.
-template <typename T, int V, int ACT, int U, int B>
+// Bound by DRAM: 8x128x512^2 16-bit (1,074 MB) 168 us, 6.4 TB/s; 1x48x517x999 FP32 (198 MB) 37 us.
+template <typename T, int V, int ACT, int U, int B, bool FOLDS>
 __global__ void __launch_bounds__(kNormThreads, kNormResident) norm_grad_sums_kernel(const __grid_constant__ NormParams p) {
   const NormGeometry& g = p.g;
   const NormTile t(g, V, false);
   grid_dependency_wait();
   grid_launch_dependents();
   using IO = VecIO<T, V>;
-  using Walk = NormWalk<T, V, U, B, false>;
+  using Walk = NormWalk<T, V, U, B, false, FOLDS>;
   const Walk walk(g, t);
   NormSource<Walk, T> x(walk, p.x, 0), dy(walk, p.dy, Walk::kRingBytes);
   const NormPolicy policy(g.keep < 1.f);
@@ -1209,7 +1208,7 @@ __global__ void __launch_bounds__(kNormThreads) norm_param_grad_kernel(const __g
 }
 
 // ---- backward: dx ----
-// Bound by DRAM: 8x128x512^2 16-bit (1,074 MB in, 537 out) 235 us, 6.7 TB/s; 8x128x256^2 64 us.
+// Bound by DRAM: 8x128x512^2 16-bit (1,074 MB in, 537 out) 237 us, 6.6 TB/s; 8x128x256^2 63 us.
 template <typename T, int V, int ACT, int U, int B>
 __global__ void __launch_bounds__(kNormThreads, kNormApplyResident) norm_grad_apply_kernel(const __grid_constant__ NormParams p) {
   const NormGeometry& g = p.g;
