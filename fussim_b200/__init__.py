@@ -35,6 +35,7 @@ from .functional import (  # noqa: F401
 )
 from .training import (  # noqa: F401
     GroupNormAct,
+    adamw_step_,
     clip_grad_norm,
     clip_grad_norm_,
     grad_norm,
@@ -54,6 +55,7 @@ __all__ = [
     "grad_norm",
     "clip_grad_norm",
     "clip_grad_norm_",
+    "adamw_step_",
     # Advanced/internal
     "FusedSSIMMap",
     "FusedSSIMMapFP16",

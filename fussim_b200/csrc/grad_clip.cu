@@ -5,20 +5,22 @@
 #include <atomic>
 #include <climits>
 #include <cstdint>
-#include <exception>
 #include <memory>
 #include <string>
 
 #include "engine_host.h"
+#include "launch_host.h"
 
 namespace {
 
 using fssim::ClipTable;
 using fssim::kClipMaxCtas;
 using fssim::kClipThreads;
-using fssim::kClipUnit;
+using fssim::kRunUnit;
 using fssim_host::aligned;
 using fssim_host::fail;
+using fssim_host::guarded;
+using fssim_host::launch;
 using fssim_host::NvtxRange;
 
 // Runs per launch: a small table (3 KB of parameters) or a large one (29 KB, of the 32 KB that
@@ -34,26 +36,6 @@ static_assert(sizeof(ClipTable<kMany>) <= 32764, "kernel parameters are limited 
 size_t elem_size(int dtype) { return dtype == FSSIM_F32 ? 4 : 2; }
 bool known_dtype(int d) { return d == FSSIM_F32 || d == FSSIM_F16 || d == FSSIM_BF16; }
 
-template <typename... KA, typename... A>
-int launch(void (*k)(KA...), unsigned grid, size_t smem, cudaStream_t stream, const char* what, const A&... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(kClipThreads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, k, args...);
-  if (e != cudaSuccess) {
-    (void)cudaGetLastError();
-    return fail(FSSIM_ERR_CUDA, std::string(what) + ": " + cudaGetErrorString(e));
-  }
-  return FSSIM_OK;
-}
-
 unsigned grid_for(int64_t units) {
   return static_cast<unsigned>(units < kClipMaxCtas ? units : kClipMaxCtas);
 }
@@ -64,7 +46,7 @@ int cuts_of(int64_t units) {
   return static_cast<int>(cuts < 1 ? 1 : cuts < 4096 ? cuts : 4096);
 }
 
-int64_t units_of(int64_t size) { return (size + kClipUnit - 1) / kClipUnit; }
+int64_t units_of(int64_t size) { return (size + kRunUnit - 1) / kRunUnit; }
 
 // Launches of a call: runs of at most kMany non-empty tensors each.
 struct Cut {
@@ -172,9 +154,9 @@ int launch_cut(const fssim_grad_clip_args& a, const Cut& c, bool clip, bool summ
   const int st = allow_ring<K>();
   if (st) return st;
   if (!clip)
-    return launch(fssim::grad_squares_kernel<K>, ranges, 0, stream, "gradient norm launch", *t);
-  return launch(fssim::grad_clip_kernel<K>, ranges * static_cast<unsigned>(t->cuts), fssim::kClipRingBytes, stream,
-                "gradient clipping launch", *t);
+    return launch(fssim::grad_squares_kernel<K>, ranges, kClipThreads, 0, stream, "gradient norm launch", *t);
+  return launch(fssim::grad_clip_kernel<K>, ranges * static_cast<unsigned>(t->cuts), kClipThreads, fssim::kClipRingBytes,
+                stream, "gradient clipping launch", *t);
 }
 
 // One pass over all tensors: the partial sums (clip == false) or the scaling.
@@ -217,23 +199,11 @@ int run(const fssim_grad_clip_args* a, bool clip, cudaStream_t stream) {
   if (st) return st;
   if (summed) {
     double* sums = static_cast<double*>(a->workspace);
-    st = launch(fssim::grad_norm_kernel, 1u, 0, stream, "gradient norm sum launch",
+    st = launch(fssim::grad_norm_kernel, 1u, kClipThreads, 0, stream, "gradient norm sum launch",
                 static_cast<const double*>(sums), partials, sums + partials, a->norm);
     if (st || !clip) return st;
   }
   return pass(*a, true, summed, partials, stream);
-}
-
-// No exception crosses the C boundary.
-template <typename F>
-int guarded(F f) {
-  try {
-    fssim_host::g_last_error.clear();
-    return f();
-  } catch (const std::exception&) {
-    fssim_host::g_last_error = "host exception";  // short: no allocation
-    return FSSIM_ERR_CUDA;
-  }
 }
 
 }  // namespace

@@ -5,7 +5,7 @@
 //
 // The tensors are flat runs of memory, named by a table in the kernel's parameters (so a
 // captured launch carries its own copy, and no device memory or copy is needed for it). Each
-// run is cut into units of kClipUnit numbers; the units of all runs, end to end, are split
+// run is cut into units of kRunUnit numbers; the units of all runs, end to end, are split
 // over the grid in equal contiguous ranges, so every CTA streams the same number of bytes
 // whatever the tensors' sizes. A CTA finds its first run by bisection and walks on from there.
 //
@@ -16,17 +16,15 @@
 // for bit, and the workspace needs no initial value.
 #pragma once
 
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
 #include "pdl.cuh"
+#include "runs.cuh"
 
 namespace fssim {
 
 constexpr int kClipThreads = 256;
-constexpr int kClipUnit = 2048;     // numbers: eight for each thread
 constexpr int kClipResident = 3;    // CTAs on one SM
 constexpr int kClipMaxCtas = 148 * kClipResident;
 // The clipping copies vectors asynchronously into a ring of kClipRing batches of kClipBatch vectors
@@ -60,16 +58,6 @@ template <int BYTES> struct ClipRaw;
 template <> struct ClipRaw<16> { using type = uint4; };
 template <> struct ClipRaw<8> { using type = uint2; };
 
-__device__ __forceinline__ float clip_widen(float v) { return v; }
-__device__ __forceinline__ float clip_widen(__half v) { return __half2float(v); }
-__device__ __forceinline__ float clip_widen(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <typename T> __device__ __forceinline__ T clip_narrow(float v);
-template <> __device__ __forceinline__ float clip_narrow<float>(float v) { return v; }
-template <> __device__ __forceinline__ __half clip_narrow<__half>(float v) { return __float2half_rn(v); }
-template <> __device__ __forceinline__ __nv_bfloat16 clip_narrow<__nv_bfloat16>(float v) {
-  return __float2bfloat16_rn(v);
-}
-
 template <typename T, int N>
 struct ClipVec {
   using Raw = typename ClipRaw<sizeof(T) * N>::type;
@@ -100,13 +88,13 @@ struct ClipVec {
   static __device__ __forceinline__ void unpack(const Raw& r, float (&f)[N]) {
     const T* e = reinterpret_cast<const T*>(&r);
 #pragma unroll
-    for (int i = 0; i < N; ++i) f[i] = clip_widen(e[i]);
+    for (int i = 0; i < N; ++i) f[i] = run_widen(e[i]);
   }
   static __device__ __forceinline__ void store(T* p, const float (&f)[N], uint64_t policy) {
     Raw r;
     T* e = reinterpret_cast<T*>(&r);
 #pragma unroll
-    for (int i = 0; i < N; ++i) e[i] = clip_narrow<T>(f[i]);
+    for (int i = 0; i < N; ++i) e[i] = run_narrow<T>(f[i]);
     if constexpr (sizeof(Raw) == 16)
       asm volatile("st.global.L2::cache_hint.v4.u32 [%0], {%1, %2, %3, %4}, %5;" ::"l"(p), "r"(r.x),
                    "r"(r.y), "r"(r.z), "r"(r.w), "l"(policy) : "memory");
@@ -165,32 +153,6 @@ __device__ __forceinline__ double sum_squares(const typename ClipVec<T, N>::Raw 
     return w;
   }
   return s;  // NaN too
-}
-
-// The unit range of a CTA.
-__device__ __forceinline__ int64_t clip_range(int64_t units, int64_t b, int64_t grid) {
-  return units / grid * b + (units % grid) * b / grid;
-}
-
-// Calls f(run, first number, one past the last) for each piece of a run in the units [u0, u1), from
-// the last piece to the first when BACKWARDS.
-template <bool BACKWARDS, int K, typename F>
-__device__ __forceinline__ void clip_walk(const ClipTable<K>& t, int64_t u0, int64_t u1, F f) {
-  if (u0 >= u1) return;
-  const int64_t key = BACKWARDS ? u1 - 1 : u0;
-  int lo = 0, hi = t.count - 1;  // the last run whose first unit is at most key
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) / 2;
-    if (t.unit0[mid] <= key) lo = mid;
-    else hi = mid - 1;
-  }
-  for (int r = lo; BACKWARDS ? (r >= 0 && t.unit0[r + 1] > u0) : (r < t.count && t.unit0[r] < u1);
-       r += BACKWARDS ? -1 : 1) {
-    const int64_t first = t.unit0[r];
-    const int64_t b = max(u0 - first, int64_t{0}) * kClipUnit;
-    const int64_t e = min((u1 - first) * kClipUnit, t.size[r]);
-    if (b < e) f(r, b, e);
-  }
 }
 
 // Numbers before the first 16-byte boundary of p + b, at most e - b.
@@ -255,7 +217,7 @@ __device__ __noinline__ double clip_piece_squares(const T* src, int64_t b, int64
   const int64_t ends = head + (e - tail);
   if (threadIdx.x < ends) {
     const int64_t at = threadIdx.x < head ? b + threadIdx.x : tail + (threadIdx.x - head);
-    const double v = clip_widen(src[at]);
+    const double v = run_widen(src[at]);
     acc = v * v;
   }
   // Read straight into registers: this pass writes nothing, and on its way through shared memory the
@@ -316,7 +278,7 @@ __device__ __noinline__ void clip_piece_scale(const S* src, D* dst, int64_t b, i
     // alike).
 #pragma unroll 8
     for (int64_t i = b + threadIdx.x; i < e; i += kClipThreads)
-      dst[i] = clip_narrow<D>(coef * clip_widen(src[i]));
+      dst[i] = run_narrow<D>(coef * run_widen(src[i]));
     return;
   }
   const int64_t n = (e - body) / N;
@@ -335,7 +297,7 @@ __device__ __noinline__ void clip_piece_scale(const S* src, D* dst, int64_t b, i
   const int64_t ends = head + (e - tail);
   if (threadIdx.x < ends) {
     const int64_t at = threadIdx.x < head ? b + threadIdx.x : tail + (threadIdx.x - head);
-    dst[at] = clip_narrow<D>(coef * clip_widen(src[at]));
+    dst[at] = run_narrow<D>(coef * run_widen(src[at]));
   }
 }
 
@@ -360,13 +322,13 @@ __global__ void __launch_bounds__(kClipThreads, kClipResident)
   grid_dependency_wait();
   grid_launch_dependents();
   const int64_t units = t.unit0[t.count];
-  const int64_t u0 = clip_range(units, blockIdx.x, gridDim.x), u1 = clip_range(units, blockIdx.x + 1, gridDim.x);
+  const int64_t u0 = run_range(units, blockIdx.x, gridDim.x), u1 = run_range(units, blockIdx.x + 1, gridDim.x);
   const ClipPolicy policies(t.keep < 1.f);
   const int64_t split = u1 - static_cast<int64_t>(static_cast<float>(u1 - u0) * min(t.keep, 1.f));
   double acc = 0.0;
   for (int part = 0; part < 2; ++part) {  // what goes past L2, then what stays
     const uint64_t policy = part ? policies.stay : policies.pass;
-    clip_walk<false>(t, part ? split : u0, part ? u1 : split, [&](int r, int64_t b, int64_t e) {
+    run_walk<false>(t, part ? split : u0, part ? u1 : split, [&](int r, int64_t b, int64_t e) {
       if (t.src_dtype[r] == 0) acc += clip_piece_squares(static_cast<const float*>(t.src[r]), b, e, policy);
       else if (t.src_dtype[r] == 1) acc += clip_piece_squares(static_cast<const __half*>(t.src[r]), b, e, policy);
       else acc += clip_piece_squares(static_cast<const __nv_bfloat16*>(t.src[r]), b, e, policy);
@@ -410,8 +372,8 @@ __global__ void __launch_bounds__(kClipThreads, kClipResident)
   const uint64_t policy = ClipPolicy(t.keep < 1.f).pass;
   const int64_t units = t.unit0[t.count];
   const int cut = t.cuts - 1 - blockIdx.x / t.ranges, range = blockIdx.x % t.ranges;
-  const int64_t u0 = clip_range(units, range, t.ranges), n = clip_range(units, range + 1, t.ranges) - u0;
-  clip_walk<true>(t, u0 + clip_range(n, cut, t.cuts), u0 + clip_range(n, cut + 1, t.cuts),
+  const int64_t u0 = run_range(units, range, t.ranges), n = run_range(units, range + 1, t.ranges) - u0;
+  run_walk<true>(t, u0 + run_range(n, cut, t.cuts), u0 + run_range(n, cut + 1, t.cuts),
                   [&](int r, int64_t b, int64_t e) {
     if (ratio >= 1.0 && t.src[r] == t.dst[r]) return;  // in place and below the limit: as it was
     const void* s = t.src[r];

@@ -5,51 +5,16 @@
 // streams, and captured graphs, never share one).
 #include "torch_training.h"
 
-#include <ATen/cuda/CUDAContext.h>
-#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/util/SmallVector.h>
 #include <c10/cuda/CUDAGuard.h>
-#include <torch/csrc/jit/frontend/tracer.h>
 
 #include <algorithm>
 #include <cmath>
 #include <numeric>
-#include <stdexcept>
-#include <string>
-#include <vector>
 
-#include "fussim_b200.h"
+using namespace fssim_torch;
 
 namespace {
-
-void check_status(int st) {
-  if (st == FSSIM_OK) return;
-  throw std::runtime_error(std::string("fussim_b200: ") + fssim_status_string(st) + ": " +
-                           fssim_last_error());
-}
-
-fssim_stream_t current_stream() {
-  return reinterpret_cast<fssim_stream_t>(at::cuda::getCurrentCUDAStream().stream());
-}
-
-int dtype_code(at::ScalarType t) {
-  switch (t) {
-    case at::kFloat: return FSSIM_F32;
-    case at::kHalf: return FSSIM_F16;
-    case at::kBFloat16: return FSSIM_BF16;
-    default: throw std::invalid_argument("unsupported dtype for fussim_b200");
-  }
-}
-
-at::Tensor workspace(size_t bytes, const at::Tensor& like) {
-  return at::empty({static_cast<int64_t>(bytes)}, like.options().dtype(at::kByte));
-}
-
-using OptTensor = std::optional<at::Tensor>;
-
-// A lazily negated view (the imaginary part of a conjugate) holds its numbers with the other sign.
-at::Tensor resolved(const at::Tensor& t) { return t.is_neg() ? t.resolve_neg() : t; }
-OptTensor resolved(const OptTensor& t) { return t.has_value() ? OptTensor(resolved(*t)) : t; }
 
 // Weight and bias as the C ABI takes them: dense, of one type (group_norm_act has checked device,
 // shape and type), and with memory of their own, since no pointer stands for no weight there.
@@ -168,37 +133,6 @@ struct GroupNormFn : public torch::autograd::Function<GroupNormFn> {
   }
 };
 
-[[noreturn]] void value_error(const std::string& msg) { throw std::invalid_argument(msg); }
-[[noreturn]] void runtime_error(const std::string& msg) { throw std::runtime_error(msg); }
-
-std::string shape_text(const at::Tensor& t) {
-  std::string s = "(";
-  for (int64_t i = 0; i < t.dim(); ++i) s += (i ? ", " : "") + std::to_string(t.size(i));
-  return s + (t.dim() == 1 ? ",)" : ")");
-}
-std::string type_text(at::ScalarType t) { return std::string(c10::toString(t)); }
-bool known_type(at::ScalarType t) { return t == at::kFloat || t == at::kHalf || t == at::kBFloat16; }
-
-void require_cuda(const char* what) {
-  if (!at::hasCUDA() || at::cuda::device_count() == 0)
-    runtime_error(std::string("CUDA is not available. ") + what + " requires a CUDA-capable GPU.");
-}
-
-// A tracer records the operators that torch dispatches: of a call here it would keep the allocation
-// of the result and not the launches.
-void refuse_tracing(const char* what) {
-  using Key = c10::impl::TorchDispatchModeKey;
-  if (torch::jit::tracer::isTracing() || c10::impl::TorchDispatchModeTLS::get_mode(Key::PROXY).has_value())
-    runtime_error(std::string(what) + " cannot be traced (torch.jit.trace, make_fx, torch.export): its kernels "
-                  "are launched outside torch's dispatcher");
-}
-
-// Nor is there a forward-mode derivative: a result without a tangent would stand for a zero one.
-void refuse_tangent(const at::Tensor& t, const char* name, const char* what) {
-  if (t._fw_grad(/*level=*/0).defined())
-    runtime_error(std::string(what) + " has no forward-mode derivative, but " + name + " carries a tangent");
-}
-
 int64_t activation_code(const std::optional<std::string>& name) {
   if (!name.has_value()) return FSSIM_ACT_NONE;
   if (*name == "silu") return FSSIM_ACT_SILU;
@@ -262,25 +196,9 @@ at::Tensor group_norm_act(const at::Tensor& given, int64_t groups, const OptTens
 }
 
 // ---- gradient norm and clipping ----
-// Models have hundreds of gradients and a call's device time is tens of microseconds, so the
-// tensors are read where the caller's list holds them (no copies of their handles) and in one pass.
-using Refs = std::vector<const at::Tensor*>;
+}  // namespace
 
-const at::Tensor& tensor_of(py::handle h, const char* what, size_t index) {
-  if (!THPVariable_Check(h.ptr()))
-    throw py::type_error(std::string(what) + " must be tensors, but that at index " + std::to_string(index) +
-                         " is not");
-  return THPVariable_Unpack(h.ptr());
-}
-
-Refs refs_of(const py::list& list, const char* what) {
-  Refs refs;
-  refs.reserve(list.size());
-  for (size_t i = 0; i < list.size(); ++i) refs.push_back(&tensor_of(PyList_GET_ITEM(list.ptr(), i), what, i));
-  return refs;
-}
-
-void check_grads(const Refs& grads, const char* what) {
+void fssim_torch::check_grads(const Refs& grads, const char* what) {
   refuse_tracing(what);
   for (size_t i = 0; i < grads.size(); ++i) {
     const at::Tensor& g = *grads[i];
@@ -298,12 +216,7 @@ void check_grads(const Refs& grads, const char* what) {
     runtime_error("gradients must be on a CUDA device, but got device: " + grads[0]->device().str());
 }
 
-// The memory of a tensor, and where the tensor stands in the call.
-struct Span {
-  uintptr_t begin, end;
-  int64_t index;
-  bool out;
-};
+namespace {
 
 // The ways to write a number as a sum of terms c * x, 0 <= x <= most, each c at least 1: depth first
 // from the largest c, whose x the rest leaves little choice for where strides are nested, as those
@@ -434,6 +347,15 @@ void check_overlap(std::vector<Span>& spans, std::vector<Reach>& outs) {
       if ((outs[i].tensor || outs[j].tensor) && share_memory(outs[i], outs[j])) refuse(outs[j].index);
 }
 
+}  // namespace
+
+void fssim_torch::check_spans(std::vector<Span>& spans) {
+  std::vector<Reach> none;
+  check_overlap(spans, none);
+}
+
+namespace {
+
 struct ClipArrays {
   std::vector<const void*> grads;
   std::vector<void*> outs;
@@ -469,16 +391,17 @@ struct ClipArrays {
   }
 };
 
-at::Tensor zero_norm() {
+}  // namespace
+
+at::Tensor fssim_torch::zero_norm() {
   return at::zeros({}, at::TensorOptions().dtype(at::kFloat).device(at::kCUDA));
 }
 
-// Tensors whose numbers fill their memory are taken as they lie; others, and lazily negated views, go
-// through a dense copy.
-bool as_it_lies(const at::Tensor& t) { return t.is_non_overlapping_and_dense() && !t.is_neg(); }
-at::Tensor dense_copy(const at::Tensor& t) { return resolved(t).contiguous(); }
+namespace {
 
-at::Tensor norm_of(const Refs& grads) {
+}  // namespace
+
+at::Tensor fssim_torch::norm_of(const Refs& grads) {
   const at::NoGradGuard no_grad;
   const at::cuda::OptionalCUDAGuard guard(grads[0]->device());
   at::Tensor norm = at::empty({}, grads[0]->options().dtype(at::kFloat));
@@ -497,6 +420,8 @@ at::Tensor norm_of(const Refs& grads) {
   check_status(fssim_grad_norm(&a, current_stream()));
   return norm;
 }
+
+namespace {
 
 at::Tensor clip_into(const Refs& grads, const Refs& outs, double max_norm, bool error_if_nonfinite) {
   const at::NoGradGuard no_grad;

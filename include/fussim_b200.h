@@ -382,6 +382,46 @@ int fssim_grad_norm(const fssim_grad_clip_args* args, fssim_stream_t stream);
 /* Norm and clipping. */
 int fssim_grad_clip(const fssim_grad_clip_args* args, fssim_stream_t stream);
 
+/* The AdamW step over many tensors (flat runs of device memory; the arrays are host memory and
+ * are read during the call), in place:
+ *     g = +-grads[i] * min(1, max_norm / (norm + 1e-6)),
+ *     m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2,
+ *     p = (1 - lr weight_decay) p - lr / (1 - beta1^step) * m / (sqrt(v / (1 - beta2^step)) + eps).
+ * All arithmetic is FP32; p is rounded once to its type and once, from FP32, to its copy's.
+ * Moments of 32 bits are FP32. Those of 8 bits are e4m3 codes of m and of sqrt(v), with one FP32
+ * scale each for every block of 256 numbers (a code stands for itself times the scale): the block's
+ * largest finite number (at least 2^-100) / 448. Numbers go to one of the two codes beside them at
+ * random, in proportion (below 2^-6 scales: to the nearest), by a hash of seed, step, the
+ * tensor's position in the arrays and the number's in the tensor; a root that is not zero is held
+ * as 2^-6 scales at least; what is infinite or NaN as NaN, alone in its block. Results
+ * repeat bit for bit. */
+typedef struct fssim_adamw_args {
+  int64_t count;              /* tensors */
+  void* const* params;        /* device pointers, one for each (may be NULL where its size is 0); */
+  const void* const* grads;   /*   no tensor that is written may overlap another */
+  void* const* exp_avgs;      /* m: FP32, or codes of 8 bits */
+  void* const* exp_avg_sqs;   /* v: FP32, or codes of 8 bits of its root */
+  float* const* scales;       /* 8 bits: (m's, the root's) for each block; otherwise not looked at */
+  void* const* copies;        /* NULL, or where each (FP32) parameter goes in 16 bits, too */
+  const int64_t* sizes;       /* numbers in each */
+  const int32_t* dtypes;      /* fssim_dtype of each parameter */
+  const int32_t* grad_dtypes; /* its type, or F32; any beside F32 parameters */
+  const int32_t* copy_dtypes; /* F16 or BF16; not looked at without copies */
+  int32_t state_bits;         /* 32 or 8 */
+  int32_t maximize;           /* not 0: gradients are taken with the other sign */
+  uint32_t seed;
+  int64_t step;               /* this step's number, from 1; with step_at not looked at */
+  const float* step_at;       /* NULL, or device memory that holds it when the work runs */
+  double lr;                  /* >= 0; with lr_at not looked at */
+  const float* lr_at;         /* NULL, or device memory that holds it when the work runs */
+  double beta1, beta2;        /* in [0, 1) */
+  double eps, weight_decay;   /* >= 0 */
+  const float* norm;          /* NULL (no clipping), or device memory: the gradients' norm */
+  double max_norm;            /* >= 0 */
+} fssim_adamw_args;
+
+int fssim_adamw_step(const fssim_adamw_args* args, fssim_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
