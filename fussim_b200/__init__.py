@@ -18,6 +18,11 @@ FP32. There is no CPU path: every call runs the hand-written sm_100a kernels of
 ``libfussim_b200.so`` and fails loudly if they are missing.
 """
 
+from .blocks import (  # noqa: F401
+    block_norm,
+    gated_residual,
+    gated_residual_norm,
+)
 from .functional import (  # noqa: F401
     ALLOWED_PADDING,
     SSIM,
@@ -52,6 +57,9 @@ __all__ = [
     # Training step around the loss
     "group_norm_act",
     "GroupNormAct",
+    "block_norm",
+    "gated_residual",
+    "gated_residual_norm",
     "grad_norm",
     "clip_grad_norm",
     "clip_grad_norm_",

@@ -1,0 +1,98 @@
+"""Norms before and after the residual blocks of an image transformer (or any network over rows of
+channels), fused with the block's gate, residual scale and modulation.
+
+* ``block_norm``: the norm before a block.
+* ``gated_residual``: a block's output, normalised, gated and added to the residual stream.
+* ``gated_residual_norm``: both in one pass, the end of one block and the start of the next.
+
+The token counterpart of ``group_norm_act`` for networks whose output goes into ``fused_ssim`` or
+``l1_dssim_loss``; hand-written sm_100a kernels without a CPU path. The reference
+(OpsiClear/fussim) has no counterpart of these.
+"""
+
+from __future__ import annotations
+
+from typing import Optional, Tuple
+
+import torch
+
+from .functional import _ensure_cuda_extension
+
+
+def block_norm(
+    x: torch.Tensor,
+    weight: Optional[torch.Tensor] = None,
+    bias: Optional[torch.Tensor] = None,
+    *,
+    scale: Optional[torch.Tensor] = None,
+    shift: Optional[torch.Tensor] = None,
+    kind: str = "rms",
+    eps: float = 1e-6,
+    out_dtype: Optional[torch.dtype] = None,
+) -> torch.Tensor:
+    """``(norm(x) * weight + bias) * (1 + scale) + shift`` over the last dimension of a CUDA tensor.
+
+    norm(x) = (x - mean) / sqrt(mean((x - mean)^2) + eps) over the last dimension's C numbers (1 to
+    16384); ``kind`` "layer" takes the mean off, "rms" takes it as zero. ``weight`` and ``bias``
+    have C values; ``scale`` and ``shift``, a conditioning, C values or (B, C) for x of shape
+    (B, ..., C), one row for each sample. Each may be None and have any of the types float32,
+    float16 and bfloat16, as x. The result has x's type, or for float32 ``out_dtype``. Statistics
+    and arithmetic are FP32 and results are rounded once; autocast changes nothing here.
+
+    Images of shape (B, C, H, W) in the channels-last memory format are normalised over their
+    channels as ``x.permute(0, 2, 3, 1)``, without a copy; inputs (and incoming gradients) whose
+    last dimension is not dense row behind row cost one. Differentiable once, backwards;
+    forward-mode derivatives and tracing raise RuntimeError. The results repeat bit for bit.
+    Under graph capture follow torch's rule for backward passes: the captured leaves must not
+    have live eager graphs.
+    """
+    return _ensure_cuda_extension().block_norm(x, weight, bias, scale, shift, kind, eps, out_dtype)
+
+
+def gated_residual(
+    x: torch.Tensor,
+    branch: torch.Tensor,
+    gate: Optional[torch.Tensor] = None,
+    *,
+    residual_scale: float = 1.0,
+    branch_kind: Optional[str] = None,
+    branch_weight: Optional[torch.Tensor] = None,
+    branch_bias: Optional[torch.Tensor] = None,
+    eps: float = 1e-6,
+) -> torch.Tensor:
+    """``x + residual_scale * gate * (norm(branch) * branch_weight + branch_bias)``, in x's type.
+
+    ``branch`` is the output of a residual block, of x's shape and of x's type, or 16 bits wide
+    beside a float32 residual stream x. ``branch_kind`` is the kind of the norm after the block
+    (None: the branch as it is, and then no weight and bias). ``gate`` has C values (a learned
+    layer scale) or (B, C) (a conditioning), or is None. Otherwise as ``block_norm``.
+    """
+    return _ensure_cuda_extension().gated_residual(
+        x, branch, gate, residual_scale, branch_kind, branch_weight, branch_bias, eps
+    )
+
+
+def gated_residual_norm(
+    x: torch.Tensor,
+    branch: torch.Tensor,
+    gate: Optional[torch.Tensor] = None,
+    weight: Optional[torch.Tensor] = None,
+    bias: Optional[torch.Tensor] = None,
+    *,
+    scale: Optional[torch.Tensor] = None,
+    shift: Optional[torch.Tensor] = None,
+    kind: str = "rms",
+    residual_scale: float = 1.0,
+    branch_kind: Optional[str] = None,
+    branch_weight: Optional[torch.Tensor] = None,
+    branch_bias: Optional[torch.Tensor] = None,
+    eps: float = 1e-6,
+) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The end of one block and the start of the next: (r, z) with r as ``gated_residual``'s result
+    (rounded to x's type) and z = ``block_norm`` of that r, in the branch's type; one kernel, which
+    reads x and branch once, and one pass over rows backwards.
+    """
+    return _ensure_cuda_extension().gated_residual_norm(
+        x, branch, gate, weight, bias, scale, shift, kind, residual_scale, branch_kind,
+        branch_weight, branch_bias, eps
+    )

@@ -482,6 +482,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("version", &version);
   bind_training(m);
   bind_adamw(m);
+  bind_block_norm(m);
   m.def("set_reserved_sms", [](int n) {
     const int st = fssim_set_reserved_sms(n);
     if (st != FSSIM_OK) throw std::invalid_argument(fssim_last_error());

@@ -382,6 +382,79 @@ int fssim_grad_norm(const fssim_grad_clip_args* args, fssim_stream_t stream);
 /* Norm and clipping. */
 int fssim_grad_clip(const fssim_grad_clip_args* args, fssim_stream_t stream);
 
+/* Norms before and after a residual block, with its gate and modulation. Rows of C numbers, T of
+ * them for each of B samples, dense and one behind the other:
+ *     r = x + residual_scale * gate * (N'(branch) * branch_weight + branch_bias), in x's type,
+ *     z = (N(r) * weight + bias) * (1 + scale) + shift, in the branch's type,
+ * with N a norm over the row, (v - mean) / sqrt(<(v - mean)^2> + eps), mean = 0 in the RMS kind, and
+ * N' one too, or the identity (FSSIM_NORM_NONE). Without a branch r is x; without z only r is
+ * computed. Statistics and arithmetic are FP32; each result is rounded once. */
+typedef enum fssim_norm_kind {
+  FSSIM_NORM_NONE = 0,
+  FSSIM_NORM_RMS = 1,
+  FSSIM_NORM_LAYER = 2
+} fssim_norm_kind;
+
+/* C numbers, or (per_sample) B x C; data NULL where there are none (ones for the weights and the
+ * gate, zeros for the others). */
+typedef struct fssim_channels {
+  const void* data;
+  int32_t dtype;
+  int32_t per_sample;
+} fssim_channels;
+
+typedef struct fssim_channels_grad {
+  void* data;             /* written; NULL to skip */
+  int32_t dtype;
+  int32_t per_sample;     /* as the vector's: 0 for sums over all samples */
+} fssim_channels_grad;
+
+typedef struct fssim_block_norm_forward_args {
+  int32_t x_dtype;        /* fssim_dtype of x and r: branch's and z's, or F32 */
+  int32_t y_dtype;        /* fssim_dtype of branch and z */
+  int32_t kind;           /* fssim_norm_kind of N (RMS or LAYER, unless z is NULL) */
+  int32_t branch_kind;    /* fssim_norm_kind of N' */
+  int64_t B, T, C;        /* C at most 16384 */
+  float eps;              /* >= 0, of both norms */
+  float residual_scale;
+  const void* x;
+  const void* branch;     /* NULL: r = x, and r is not written */
+  void* r;                /* may be x */
+  void* z;                /* NULL to skip; may be branch, where r is not x */
+  fssim_channels gate, weight, bias, scale, shift, branch_weight, branch_bias;
+  float* stats;           /* (mean, rstd) of each row of r, 8-byte aligned, written: what the */
+  float* branch_stats;    /*   backward needs; and of the branch's; NULL to skip */
+} fssim_block_norm_forward_args;
+
+int fssim_block_norm_forward(const fssim_block_norm_forward_args* args, fssim_stream_t stream);
+
+/* The gradients for given dr and dz (either may be NULL, for zeros). With a = weight * (1 + scale):
+ *     dR = dr + rstd (a dz - <a dz> - N(r) <a dz N(r)>) (the first mean not in the RMS kind), dx = dR;
+ * dbranch likewise from residual_scale * gate * branch_weight * dR; those of the vectors from sums
+ * over rows, FP32 over at most 256 and FP64 beyond. */
+typedef struct fssim_block_norm_backward_args {
+  int32_t x_dtype;        /* of r, dr and dx */
+  int32_t y_dtype;        /* of branch, dz and dbranch */
+  int32_t kind, branch_kind;
+  int64_t B, T, C;
+  float residual_scale;
+  const void* r;          /* as the forward returned it (x, without a branch) */
+  const void* branch;     /* NULL where there is none */
+  const void* dr;
+  const void* dz;
+  const float* stats;     /* as the forward wrote them */
+  const float* branch_stats;
+  fssim_channels gate, weight, bias, scale, branch_weight, branch_bias;
+  void* dx;               /* NULL to skip; may be dr */
+  void* dbranch;          /* NULL to skip; may be dz */
+  fssim_channels_grad dgate, dweight, dbias, dscale, dshift, dbranch_weight, dbranch_bias;
+  void* workspace;        /* fssim_block_norm_backward_workspace_bytes(args) bytes, 16-byte */
+  size_t workspace_bytes; /*   aligned, contents arbitrary; in use until the call's work ends */
+} fssim_block_norm_backward_args;
+
+size_t fssim_block_norm_backward_workspace_bytes(const fssim_block_norm_backward_args* args);
+int fssim_block_norm_backward(const fssim_block_norm_backward_args* args, fssim_stream_t stream);
+
 /* The AdamW step over many tensors (flat runs of device memory; the arrays are host memory and
  * are read during the call), in place:
  *     g = +-grads[i] * min(1, max_norm / (norm + 1e-6)),
