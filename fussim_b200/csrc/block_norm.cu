@@ -1,11 +1,16 @@
 // C entry points of the residual-block norms: argument checks, the split of rows over CTAs, and the
-// launches. The kernels are in block_norm.cuh.
-#include "block_norm.cuh"
+// launches. The kernels are in block_norm.cuh and
+// block_norm_merge.cuh.
+#include "block_norm_merge.cuh"
 
+#include <algorithm>
+#include <climits>
 #include <cmath>
 #include <cstdint>
+#include <initializer_list>
 #include <string>
 
+#include "block_norm_launch.h"
 #include "engine_host.h"
 #include "launch_host.h"
 
@@ -72,64 +77,119 @@ int check_tensors(const Named (&all)[N]) {
 
 // How rows are laid over threads and CTAs.
 struct Layout {
-  bool vec;
-  int vectors;   // of eight numbers, of a thread
+  bool vec, warp;
+  int groups;    // of eight numbers, of a thread
   int threads;   // of a row
   int block;     // of a CTA
   int64_t B, T;  // samples and rows: all rows are one sample's where no vector has one for each sample
   int64_t chunk, chunks;
+  int stages;    // of the ring
+  bool staged;   // the arrays are in shared memory
+  size_t memory;
 };
 
-Layout layout(const Shape& s, bool per_sample, bool vec, int resident_threads) {
+constexpr int64_t kSmMemory = 216 << 10;  // of an SM's shared memory: for rings and arrays
+constexpr int kMaxStages = 4;
+
+// `bytes`: of a stage of the ring, for each number of a row. `arrays`: how many there are.
+Layout layout(const Shape& s, bool backward, int mode, bool per_sample, bool vec, int bytes, int arrays) {
   Layout l{};
+  const int needed = static_cast<int>((s.C + 7) / 8);
+  // Rows within a warp where a thread has at most five groups of eight numbers (forward; two
+  // backward, whose sums are in registers) of it: the fewest threads that are idle at a row's end, and
+  // of those the most groups, since what a row costs each thread (sums, addresses) is paid for more numbers.
+  const auto best = [&](std::initializer_list<int> choices, bool warp) {
+    int padded = INT_MAX;
+    for (const int g : choices) {
+      int t = (needed + g - 1) / g;
+      if (warp) {
+        int p = 1;
+        while (p < t) p *= 2;
+        t = p;
+        if (t > 32) continue;
+      } else {
+        t = (t + 31) / 32 * 32;
+        if (t > (backward && g <= 2 ? 384 : kBlockMaxThreads)) continue;  // (registers)
+      }
+      if (t * g <= padded) {
+        padded = t * g;
+        l.groups = g;
+        l.threads = t;
+      }
+    }
+    l.warp = warp;
+    return padded < INT_MAX;
+  };
   l.vec = vec;
-  const int groups = static_cast<int>((s.C + 7) / 8);
-  if (groups <= 32) {
-    l.vectors = 1;
-    for (l.threads = 1; l.threads < groups;) l.threads *= 2;
-    l.block = kBlockSmallThreads;
-  } else {
-    l.vectors = groups <= kBlockMaxThreads ? 1 : groups <= 2 * kBlockMaxThreads ? 2 : 4;
-    l.threads = (groups + 32 * l.vectors - 1) / (32 * l.vectors) * 32;
+  for (;;) {
+    if (!l.vec) {
+      if (!best({1}, true) && !best({1}, false)) best({4}, false);
+    } else if (backward) {
+      if (!best({1, 2}, true) && !best({1, 2}, false)) best({4}, false);
+    } else if (s.B * s.T <= 2 * kSms && needed <= kBlockMaxThreads) {
+      if (!best({1}, true)) best({1}, false);  // few rows: the fastest for each
+    } else if (!best({1, 3, 4, 5}, true)) {
+      if (needed > kBlockMaxThreads || !best({3, 4}, false)) best({4}, false);
+    }
+    const int registers = backward ? block_backward_registers(l.groups) : block_forward_registers(l.groups, l.vec ? mode : kBlockAfter);
+    const int resident = block_resident(registers);
+    l.B = per_sample ? s.B : 1;
+    l.T = per_sample ? s.T : s.B * s.T;
     l.block = l.threads;
+    if (l.warp) {
+      // fewer warps in a CTA where there are few rows
+      l.block = 128;
+      while (l.block > 32 && l.B * ((l.T * l.threads + l.block - 1) / l.block) < 2 * kSms) l.block /= 2;
+    }
+    const int64_t parts = l.block / l.threads;
+    const int64_t stage = l.vec ? static_cast<int64_t>(l.block) * l.groups * 8 * bytes : 0;
+    const int64_t array_bytes = static_cast<int64_t>(arrays) * s.C * sizeof(float);
+    if (stage > fssim_host::kBlockMemory) {  // rows are loaded number by number
+      l.vec = false;
+      continue;
+    }
+    // As many CTAs on an SM as leave each room for the arrays and a row ahead of its own.
+    for (int64_t on_sm = std::max(resident / l.block, 1);; --on_sm) {
+      const int64_t wanted = (kSms * on_sm + l.B - 1) / l.B;
+      // a thread adds at most 256 rows up in FP32
+      const int64_t rounds = std::min<int64_t>((l.T + parts * wanted - 1) / (parts * wanted), 256);
+      l.chunk = rounds * parts;
+      l.chunks = (l.T + l.chunk - 1) / l.chunk;
+      const int64_t crowd = std::min(on_sm, (l.B * l.chunks + kSms - 1) / kSms);
+      const int64_t room = std::min<int64_t>(kSmMemory / crowd - 2048, fssim_host::kBlockMemory);
+      const int64_t stages = std::min<int64_t>(kMaxStages, rounds + 1), least = std::min<int64_t>(stages, 2);
+      // (kernels that make the arrays again for each row: four groups of a CTA's rows alone)
+      const bool choice = l.groups == 4 && !l.warp;
+      l.staged = array_bytes + least * stage <= room && (l.vec || !choice);
+      l.stages = stage ? static_cast<int>(std::clamp<int64_t>((room - (l.staged ? array_bytes : 0)) / stage, 1, stages)) : 1;
+      if (l.staged || on_sm == 1) {
+        l.staged = l.staged || !choice;
+        break;
+      }
+    }
+    l.memory = static_cast<size_t>(stage * l.stages + (l.staged ? array_bytes : 0));
+    // (the backward pass adds up in it what rows side by side left)
+    if (backward && l.warp) l.memory = std::max<size_t>(l.memory, sizeof(float) * (l.block / 32) * s.C);
+    return l;
   }
-  l.B = per_sample ? s.B : 1;
-  l.T = per_sample ? s.T : s.B * s.T;
-  const int64_t parts = l.block / l.threads;
-  const int64_t ctas = kSms * (resident_threads / l.block > 0 ? resident_threads / l.block : 1);
-  const int64_t wanted = (ctas + l.B - 1) / l.B;
-  int64_t rounds = (l.T + parts * wanted - 1) / (parts * wanted);
-  // a thread adds at most this many rows up in FP32
-  if (rounds > 256) rounds = 256;
-  l.chunk = rounds * parts;
-  l.chunks = (l.T + l.chunk - 1) / l.chunk;
-  return l;
 }
 
 BlockChannels channels(const fssim_channels& v, int64_t C) {
   return {v.data, v.dtype, v.per_sample, v.data && aligned(v.data, 16) && (!v.per_sample || C % 8 == 0)};
 }
 
-template <typename F>
-int with_layout(const Layout& l, F f) {
-  const auto vec = [&](auto v) {
-    return l.vec ? f(v, std::true_type{}) : f(v, std::false_type{});
-  };
-  switch (l.vectors) {
-    case 1: return vec(std::integral_constant<int, 1>{});
-    case 2: return vec(std::integral_constant<int, 2>{});
-    default: return vec(std::integral_constant<int, 4>{});
-  }
+int launch_rows(bool backward, const Shape& s, const Layout& l, const BlockParams& p, cudaStream_t stream) {
+  const auto run = s.x_dtype == FSSIM_F32 ? (s.y_dtype == FSSIM_F32   ? fssim_host::block_norm_f32
+                                             : s.y_dtype == FSSIM_F16 ? fssim_host::block_norm_f32_f16
+                                                                      : fssim_host::block_norm_f32_bf16)
+                   : s.x_dtype == FSSIM_F16 ? fssim_host::block_norm_f16
+                                            : fssim_host::block_norm_bf16;
+  const int mode = p.after_kind || (!p.y && (p.dr || (backward && !p.dz))) ? kBlockAfter : p.y ? kBlockPlain : kBlockBefore;
+  return run(backward, {l.groups, l.vec, l.warp, l.staged, mode, static_cast<unsigned>(l.B * l.chunks),
+                        static_cast<unsigned>(l.block), l.memory}, p, stream);
 }
 
-template <typename F>
-int with_types(int x, int y, F f) {
-  if (x == FSSIM_F32 && y == FSSIM_F32) return f(float{}, float{});
-  if (x == FSSIM_F32 && y == FSSIM_F16) return f(float{}, __half{});
-  if (x == FSSIM_F32) return f(float{}, __nv_bfloat16{});
-  if (x == FSSIM_F16) return f(__half{}, __half{});
-  return f(__nv_bfloat16{}, __nv_bfloat16{});
-}
+int count_of(int bits) { return __builtin_popcount(static_cast<unsigned>(bits)); }
 
 BlockParams params(const Shape& s, const Layout& l) {
   BlockParams p{};
@@ -137,9 +197,12 @@ BlockParams params(const Shape& s, const Layout& l) {
   p.chunk = l.chunk;
   p.chunks = l.chunks;
   p.C = static_cast<int>(s.C);
+  p.inv = 1.0 / static_cast<double>(s.C);
   p.threads = l.threads;
+  p.stages = l.stages;
   return p;
 }
+
 
 int check_grid(int64_t ctas) {
   return ctas <= 0x7FFFFFFF ? FSSIM_OK : fail(FSSIM_ERR_SHAPE, "too many samples");
@@ -169,9 +232,18 @@ int forward(const fssim_block_norm_forward_args* a, cudaStream_t stream) {
   const bool per_sample = a->gate.per_sample || a->scale.per_sample || a->shift.per_sample || a->weight.per_sample ||
                           a->bias.per_sample || a->branch_weight.per_sample || a->branch_bias.per_sample;
   const bool vec = s.C % 8 == 0 && aligned(a->x, 16) && aligned(a->branch, 16) && aligned(a->r, 16) && aligned(a->z, 16);
-  const Layout l = layout(s, per_sample, vec, 1024);
+  const int bytes = static_cast<int>(elem_size(s.x_dtype) + (a->branch ? elem_size(s.y_dtype) : 0));
+  const bool after = a->branch && a->branch_kind != FSSIM_NORM_NONE;
+  const int arrays = (a->branch && a->gate.data ? 1 << kArrayGate : 0) |
+                     (a->z && (a->weight.data || a->scale.data) ? 1 << kArrayFactor : 0) |
+                     (a->z && (a->bias.data || a->shift.data) ? 1 << kArrayOffset : 0) |
+                     (after && a->branch_weight.data ? 1 << kArrayAfterWeight : 0) |
+                     (after && a->branch_bias.data ? 1 << kArrayAfterBias : 0);
+  const Layout l = layout(s, false, !a->branch ? kBlockBefore : after ? kBlockAfter : kBlockPlain, per_sample, vec, bytes,
+                          count_of(arrays));
   if ((st = check_grid(l.B * l.chunks))) return st;
   BlockParams p = params(s, l);
+  p.arrays = arrays;
   p.kind = a->kind;
   p.after_kind = a->branch ? a->branch_kind : kBlockNone;
   p.eps = a->eps;
@@ -189,12 +261,7 @@ int forward(const fssim_block_norm_forward_args* a, cudaStream_t stream) {
   p.shift = channels(a->shift, s.C);
   p.after_weight = channels(a->branch_weight, s.C);
   p.after_bias = channels(a->branch_bias, s.C);
-  return with_types(s.x_dtype, s.y_dtype, [&](auto x, auto y) {
-    return with_layout(l, [&](auto v, auto wide) {
-      return launch(block_norm_forward_kernel<decltype(x), decltype(y), v(), wide()>,
-                    static_cast<unsigned>(l.B * l.chunks), l.block, 0, stream, "block norm forward launch", p);
-    });
-  });
+  return launch_rows(false, s, l, p, stream);
 }
 
 // The backward pass's split of its sums.
@@ -205,8 +272,13 @@ struct Merge {
 
 bool wants_sums(const fssim_block_norm_backward_args& a, int* sums) {
   const bool after = a.dgate.data || a.dbranch_weight.data || a.dbranch_bias.data;
-  *sums = after ? 4 : 2;
+  *sums = !after ? 2 : a.branch_kind == FSSIM_NORM_NONE ? 3 : 4;
   return after || a.dweight.data || a.dbias.data || a.dscale.data || a.dshift.data;
+}
+
+int backward_arrays(const fssim_block_norm_backward_args& a) {
+  return (a.branch && (a.gate.data || (a.branch_kind && a.branch_weight.data)) ? 1 << kArrayGate : 0) |
+         (a.dz && (a.weight.data || a.scale.data) ? 1 << kArrayFactor : 0);
 }
 
 Layout backward_layout(const fssim_block_norm_backward_args& a) {
@@ -216,7 +288,10 @@ Layout backward_layout(const fssim_block_norm_backward_args& a) {
   bool vec = s.C % 8 == 0;
   for (const void* p : {a.r, a.branch, a.dr, a.dz, static_cast<const void*>(a.dx), static_cast<const void*>(a.dbranch)})
     vec = vec && aligned(p, 16);
-  return layout(s, per_sample, vec, 512);
+  const int x = static_cast<int>(elem_size(s.x_dtype)), y = static_cast<int>(elem_size(s.y_dtype));
+  const int bytes = (a.dz ? x + y : 0) + (a.dr ? x : 0) + (a.branch ? y : 0);
+  const int mode = !a.branch ? kBlockBefore : a.branch_kind ? kBlockAfter : kBlockPlain;
+  return layout(s, true, mode, per_sample, vec, bytes, count_of(backward_arrays(a)));
 }
 
 Merge merge_of(const fssim_block_norm_backward_args& a, const Layout& l) {
@@ -269,6 +344,7 @@ int backward(const fssim_block_norm_backward_args* a, cudaStream_t stream) {
   if (!aligned(a->workspace, 16)) return fail(FSSIM_ERR_WORKSPACE, "workspace must be 16-byte aligned");
   if (!m.sums && !a->dx && !a->dbranch) return FSSIM_OK;
   BlockParams p = params(s, l);
+  p.arrays = backward_arrays(*a);
   p.kind = a->kind;
   p.after_kind = branch ? a->branch_kind : kBlockNone;
   p.s = a->residual_scale;
@@ -286,12 +362,7 @@ int backward(const fssim_block_norm_backward_args* a, cudaStream_t stream) {
   p.after_weight = channels(a->branch_weight, s.C);
   p.partials = m.sums ? static_cast<float*>(a->workspace) : nullptr;
   p.sums = m.sums;
-  st = with_types(s.x_dtype, s.y_dtype, [&](auto x, auto y) {
-    return with_layout(l, [&](auto v, auto wide) {
-      return launch(block_norm_backward_kernel<decltype(x), decltype(y), v(), wide()>,
-                    static_cast<unsigned>(l.B * l.chunks), l.block, 0, stream, "block norm backward launch", p);
-    });
-  });
+  st = launch_rows(true, s, l, p, stream);
   if (st || !m.sums) return st;
   const int64_t columns = (s.C + kBlockMergeColumns - 1) / kBlockMergeColumns;
   constexpr unsigned kMergeThreads = kBlockMergeColumns * kBlockMergeTeams;

@@ -14,25 +14,31 @@
 // and every gradient of a vector follows from four sums over a sample's rows, of dz, dz rhat, dR and
 // dR yhat: dshift = sum dz, dscale = weight sum dz rhat + bias sum dz, and so on.
 //
-// A row lies in the registers of up to 512 threads, eight numbers at a time to each (or of part of a
-// warp); a thread keeps its columns from row to row of its CTA's rows, and so the vectors' numbers and
-// its share of the four sums in registers, while the next row is on its way.
+// A row belongs to part of a warp, a warp, or a CTA of up to 512 threads; a thread has V groups of eight
+// of its numbers, the same columns from row to row of its CTA's rows. Rows come ahead of their use
+// through a ring in shared memory, in which a thread copies and reads slots of its own (no barrier); the
+// vectors, combined as the arithmetic takes them, are laid there once by each CTA; the four sums stay
+// in registers.
 #pragma once
 
 #include <cuda_runtime.h>
 #include <stdint.h>
+
+#include <type_traits>
 
 #include "pdl.cuh"
 #include "runs.cuh"
 
 namespace fssim {
 
-constexpr int kBlockMaxThreads = 512;    // of a row
-constexpr int kBlockSmallThreads = 256;  // of a CTA whose rows take a warp at most
-constexpr int kBlockMaxVectors = 4;      // of eight numbers, of a thread
-constexpr int kBlockMaxC = kBlockMaxThreads * 8 * kBlockMaxVectors;
+constexpr int kBlockMaxThreads = 512;  // of a row
+constexpr int kBlockMaxC = kBlockMaxThreads * 8 * 4;
 
 enum BlockKind { kBlockNone = 0, kBlockRms = 1, kBlockLayer = 2 };
+
+// What a kernel is compiled for: no block's output, one that is added as it is, and one with a norm
+// (which also does for the other two, where there are no kernels of one mode alone).
+enum BlockMode { kBlockBefore = 0, kBlockPlain = 1, kBlockAfter = 2 };
 
 // C numbers, or C for each sample.
 struct BlockChannels {
@@ -42,6 +48,11 @@ struct BlockChannels {
   int wide;          // whole 16-byte vectors at every multiple of eight columns
 };
 
+// The vectors as the kernels take them: s * gate (forward; of 16-bit rows whose branch has a norm, gate
+// alone), weight * (1 + scale), bias * (1 + scale) + shift, after_weight, after_bias; backward, the first
+// is s * gate * after_weight.
+enum BlockArray { kArrayGate, kArrayFactor, kArrayOffset, kArrayAfterWeight, kArrayAfterBias, kArrays };
+
 struct BlockParams {
   int64_t T;              // rows of a sample
   int64_t chunk;          // rows of a CTA
@@ -49,7 +60,10 @@ struct BlockParams {
   int C;
   int threads;            // of a row
   int kind, after_kind;   // BlockKind
-  float eps, s;
+  float eps;
+  double s, inv;          // inv: 1 / C
+  int stages;             // of the ring of rows
+  int arrays;             // bit k: array k is not all ones or zeros
   const void* x;          // forward
   const void* y;
   void* r;
@@ -63,632 +77,829 @@ struct BlockParams {
   void* dx;
   void* dy;
   float* partials;        // (CTA, sum, C); null: no vector's gradient is asked for
-  int sums;               // 2 (dz's alone) or 4
+  int sums;               // 2 (dz's alone) to 4
 };
 
+template <typename T> __device__ __forceinline__ T block_narrow(double v);
+template <> __device__ __forceinline__ __half block_narrow<__half>(double v) { return __double2half(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 block_narrow<__nv_bfloat16>(double v) { return __double2bfloat16(v); }
+
+// Eight numbers, as the packed FP32 instructions take them.
+struct Eight {
+  float2 p[4];
+  __device__ __forceinline__ float& operator[](int i) { return i & 1 ? p[i / 2].y : p[i / 2].x; }
+  __device__ __forceinline__ float operator[](int i) const { return i & 1 ? p[i / 2].y : p[i / 2].x; }
+};
+__device__ __forceinline__ float2 twice(float v) { return make_float2(v, v); }
+__device__ __forceinline__ Eight eight(float v) { return {twice(v), twice(v), twice(v), twice(v)}; }
+// f(pair of a, pair of b, ...) of all pairs.
+template <typename F, typename... A>
+__device__ __forceinline__ Eight pairs(F f, const A&... a) {
+  Eight r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r.p[i] = f(a.p[i]...);
+  return r;
+}
+
+__device__ __forceinline__ float2 block_widen2(float2 v) { return v; }
+__device__ __forceinline__ float2 block_widen2(__half2 v) { return __half22float2(v); }
+__device__ __forceinline__ float2 block_widen2(__nv_bfloat162 v) { return __bfloat1622float2(v); }
+template <typename T> struct BlockPair { using type = float2; };
+template <> struct BlockPair<__half> { using type = __half2; };
+template <> struct BlockPair<__nv_bfloat16> { using type = __nv_bfloat162; };
+template <typename T> __device__ __forceinline__ typename BlockPair<T>::type block_narrow2(float2 v) {
+  if constexpr (sizeof(T) == 4) return v;
+  else if constexpr (std::is_same_v<T, __half>) return __float22half2_rn(v);
+  else return __float22bfloat162_rn(v);
+}
+// Eight numbers in a type's memory form.
+template <typename T>
+struct alignas(16) BlockPacked {
+  typename BlockPair<T>::type p[4];
+  __device__ __forceinline__ Eight widen() const {
+    return {block_widen2(p[0]), block_widen2(p[1]), block_widen2(p[2]), block_widen2(p[3])};
+  }
+  static __device__ __forceinline__ BlockPacked of(const Eight& f) {
+    return {block_narrow2<T>(f.p[0]), block_narrow2<T>(f.p[1]), block_narrow2<T>(f.p[2]), block_narrow2<T>(f.p[3])};
+  }
+};
+
+// A thread's place in a row: column (v, i) of its V groups.
 template <bool VEC>
 __device__ __forceinline__ int block_column(int threads, int tid, int v, int i) {
   return VEC ? (v * threads + tid) * 8 + i : tid + threads * (v * 8 + i);
 }
 
-// A row's numbers of a thread, as they are in memory.
+// ---- rows ----
+// The ring: stages x 16-byte vectors x threads. Copies of one row are a group; the last stages - 1
+// groups are on their way while a row is worked on.
+struct BlockRing {
+  unsigned base, bytes;  // this thread's first slot; bytes of a stage
+  int stages, put = 0, get = 0;
+  __device__ __forceinline__ BlockRing(unsigned char* memory, int vectors, int stages)
+      : base(static_cast<unsigned>(__cvta_generic_to_shared(memory)) + threadIdx.x * 16),
+        bytes(vectors * blockDim.x * 16), stages(stages) {}
+  __device__ __forceinline__ unsigned next(int& at) const {
+    const unsigned slot = base + at * bytes;
+    at = at + 1 == stages ? 0 : at + 1;
+    return slot;
+  }
+  static __device__ __forceinline__ void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+  __device__ __forceinline__ void wait() const {
+    // (the number is part of the instruction)
+    if (stages >= 4) asm volatile("cp.async.wait_group 3;" ::: "memory");
+    else if (stages == 3) asm volatile("cp.async.wait_group 2;" ::: "memory");
+    else if (stages == 2) asm volatile("cp.async.wait_group 1;" ::: "memory");
+    else asm volatile("cp.async.wait_group 0;" ::: "memory");
+  }
+};
+
+// A thread's numbers of one tensor's row: through the ring, or (rows that begin at no vector's
+// boundary) loaded number by number. Offsets are of the row's first number.
 template <typename T, int V, bool VEC>
-struct BlockRaw {
-  static constexpr int kVecs = VEC ? V * 8 * sizeof(T) / 16 : 1;
-  uint4 vec[kVecs];
+struct BlockRow {
+  static constexpr int kPer = 8 * sizeof(T) / 16;       // 16-byte vectors of a group
+  static constexpr int kVecs = VEC ? V * kPer : 0;
   T one[VEC ? 1 : V * 8];
 
-  __device__ __forceinline__ void load(const T* row, int C, int threads, int tid, bool active) {
-    if constexpr (VEC) {
-      constexpr int per = 8 * sizeof(T) / 16;
+  static __device__ __forceinline__ void copy(unsigned slot, const void* from, int64_t offset, int C, int threads,
+                                              int tid) {
+    const T* at = static_cast<const T*>(from) + offset + tid * 8;
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        const int at = block_column<true>(threads, tid, v, 0);
+    for (int v = 0; v < V; ++v)
+      if (block_column<true>(threads, tid, v, 0) < C)
 #pragma unroll
-        for (int k = 0; k < per; ++k)
-          vec[v * per + k] = active && at < C ? __ldcs(reinterpret_cast<const uint4*>(row + at) + k) : uint4{};
-      }
-    } else {
+        for (int k = 0; k < kPer; ++k)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(slot + (v * kPer + k) * blockDim.x * 16),
+                       "l"(reinterpret_cast<const uint4*>(at + v * threads * 8) + k) : "memory");
+  }
+  __device__ __forceinline__ void load(const void* from, int64_t offset, int C, int threads, int tid, bool active) {
 #pragma unroll
-      for (int i = 0; i < V * 8; ++i) {
-        const int at = block_column<false>(threads, tid, 0, i);
-        one[i] = active && at < C ? row[at] : run_narrow<T>(0.f);
-      }
+    for (int i = 0; i < V * 8; ++i) {
+      const int at = block_column<false>(threads, tid, 0, i);
+      one[i] = active && at < C ? static_cast<const T*>(from)[offset + at] : run_narrow<T>(0.f);
     }
   }
-  __device__ __forceinline__ void widen(float (&f)[V * 8]) const {
-    const T* e = VEC ? reinterpret_cast<const T*>(vec) : one;
-#pragma unroll
-    for (int i = 0; i < V * 8; ++i) f[i] = run_widen(e[i]);
-  }
-  __device__ __forceinline__ void narrow(const float (&f)[V * 8]) {
-    T* e = VEC ? reinterpret_cast<T*>(vec) : one;
-#pragma unroll
-    for (int i = 0; i < V * 8; ++i) e[i] = run_narrow<T>(f[i]);
-  }
-  __device__ __forceinline__ void store(T* row, int C, int threads, int tid) const {
+  // Group v; `ok`: it has numbers (else zeros).
+  __device__ __forceinline__ Eight get(unsigned slot, int v, bool ok) const {
     if constexpr (VEC) {
-      constexpr int per = 8 * sizeof(T) / 16;
+      uint4 raw[kPer] = {};
+      if (ok)
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        const int at = block_column<true>(threads, tid, v, 0);
-#pragma unroll
-        for (int k = 0; k < per; ++k)
-          if (at < C) reinterpret_cast<uint4*>(row + at)[k] = vec[v * per + k];
-      }
+        for (int k = 0; k < kPer; ++k)
+          asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                       : "=r"(raw[k].x), "=r"(raw[k].y), "=r"(raw[k].z), "=r"(raw[k].w)
+                       : "r"(slot + (v * kPer + k) * blockDim.x * 16) : "memory");
+      return reinterpret_cast<const BlockPacked<T>&>(raw).widen();
     } else {
+      Eight f;
 #pragma unroll
-      for (int i = 0; i < V * 8; ++i) {
-        const int at = block_column<false>(threads, tid, 0, i);
-        if (at < C) row[at] = one[i];
-      }
+      for (int i = 0; i < 8; ++i) f[i] = run_widen(one[v * 8 + i]);
+      return f;
     }
   }
 };
 
+template <typename T, bool VEC>
+__device__ __forceinline__ void block_store(void* to, int64_t offset, int C, int threads, int tid, int v,
+                                            const BlockPacked<T>& e) {
+  T* row = static_cast<T*>(to) + offset;
+  if constexpr (VEC) {
+    uint4* at = reinterpret_cast<uint4*>(row + tid * 8 + v * threads * 8);
+#pragma unroll
+    for (int k = 0; k < static_cast<int>(8 * sizeof(T) / 16); ++k) at[k] = reinterpret_cast<const uint4*>(&e)[k];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int at = block_column<false>(threads, tid, v, i);
+      if (at < C) row[at] = reinterpret_cast<const T*>(&e)[i];
+    }
+  }
+}
+
+// ---- vectors ----
 __device__ __forceinline__ float block_channel(const void* data, int dtype, int64_t at) {
   if (dtype == 0) return static_cast<const float*>(data)[at];
   if (dtype == 1) return run_widen(static_cast<const __half*>(data)[at]);
   return run_widen(static_cast<const __nv_bfloat16*>(data)[at]);
 }
 
-// A thread's eight numbers (group v) of a vector; `missing` stands for one that is not given.
+// Eight numbers of a vector from a column on, `step` apart (1 with VEC); `missing` stands for one that
+// is not given.
 template <bool VEC>
-__device__ __forceinline__ void block_channels(const BlockChannels& ch, int64_t sample, int C, int threads, int tid,
-                                               int v, float missing, float (&f)[8]) {
-  if (!ch.data) {
+__device__ __forceinline__ void block_channels(const BlockChannels& ch, int64_t sample, int C, int column, int step,
+                                               float missing, float (&f)[8]) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = missing;
-    return;
-  }
+  for (int i = 0; i < 8; ++i) f[i] = missing;
+  if (!ch.data || column >= C) return;
   const int64_t base = ch.per_sample ? sample * C : 0;
-  const int at = block_column<VEC>(threads, tid, v, 0);
   if (VEC && ch.wide) {
-    if (at >= C) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] = missing;
-      return;
-    }
     uint4 raw[2];
     if (ch.dtype == 0) {
-      const uint4* p = reinterpret_cast<const uint4*>(static_cast<const float*>(ch.data) + base + at);
+      const uint4* p = reinterpret_cast<const uint4*>(static_cast<const float*>(ch.data) + base + column);
       raw[0] = __ldg(p);
       raw[1] = __ldg(p + 1);
-      const float* e = reinterpret_cast<const float*>(raw);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] = e[i];
+      for (int i = 0; i < 8; ++i) f[i] = reinterpret_cast<const float*>(raw)[i];
     } else {
-      raw[0] = __ldg(reinterpret_cast<const uint4*>(static_cast<const __half*>(ch.data) + base + at));
-      if (ch.dtype == 1) {
+      raw[0] = __ldg(reinterpret_cast<const uint4*>(static_cast<const __half*>(ch.data) + base + column));
 #pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = run_widen(reinterpret_cast<const __half*>(raw)[i]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = run_widen(reinterpret_cast<const __nv_bfloat16*>(raw)[i]);
-      }
+      for (int i = 0; i < 8; ++i)
+        f[i] = ch.dtype == 1 ? run_widen(reinterpret_cast<const __half*>(raw)[i])
+                             : run_widen(reinterpret_cast<const __nv_bfloat16*>(raw)[i]);
     }
     return;
   }
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int c = block_column<VEC>(threads, tid, v, i);
-    f[i] = c < C ? block_channel(ch.data, ch.dtype, base + c) : missing;
+  for (int i = 0; i < 8; ++i)
+    if (column + i * step < C) f[i] = block_channel(ch.data, ch.dtype, base + column + i * step);
+}
+
+// Eight numbers of an array. WIDE: the gate is multiplied by s later, in FP64.
+template <bool VEC, bool WIDE, bool BACKWARD>
+__device__ __noinline__ void block_array(const BlockParams& p, int64_t sample, int array, int column, int step,
+                                         float (&f)[8]) {
+  float w[8], t[8];
+  const int C = p.C;
+  switch (array) {
+    case kArrayGate:
+      block_channels<VEC>(p.gate, sample, C, column, step, 1.f, f);
+      if (WIDE) return;
+      if (BACKWARD) {
+        block_channels<VEC>(p.after_weight, sample, C, column, step, 1.f, w);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = static_cast<float>(p.s) * f[i] * w[i];
+        return;
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[i] *= static_cast<float>(p.s);
+      return;
+    case kArrayFactor:
+      block_channels<VEC>(p.weight, sample, C, column, step, 1.f, w);
+      block_channels<VEC>(p.scale, sample, C, column, step, 0.f, f);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[i] = w[i] * (1.f + f[i]);
+      return;
+    case kArrayOffset:
+      block_channels<VEC>(p.bias, sample, C, column, step, 0.f, w);
+      block_channels<VEC>(p.scale, sample, C, column, step, 0.f, t);
+      block_channels<VEC>(p.shift, sample, C, column, step, 0.f, f);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[i] = fmaf(w[i], 1.f + t[i], f[i]);
+      return;
+    case kArrayAfterWeight: block_channels<VEC>(p.after_weight, sample, C, column, step, 1.f, f); return;
+    default: block_channels<VEC>(p.after_bias, sample, C, column, step, 0.f, f); return;
   }
 }
 
-// Sums over a row's threads, which are a power of two within a warp, or all of the CTA's warps.
-// Results are the same in every thread. Two buffers in turn: one barrier for each sum.
-struct BlockTeam {
-  int threads, warps;
-  float2* slots;    // 2 x 32
-  float* counts;    // a row's numbers of each warp
-  float warp_inv;   // 1 / those of this one
-  int turn = 0;
+// The arrays of a sample lie in shared memory (those that are not constant, one behind the other;
+// STAGED), or are made again for each row where that is too small. With VEC the first halves of all
+// groups lie before the second halves: lanes read consecutive vectors.
+__device__ __forceinline__ float* block_place_of(const BlockParams& p, float* memory, int array) {
+  return memory + __popc(p.arrays & ((1 << array) - 1)) * p.C;
+}
 
-  // The buffer of the next exchange.
-  __device__ __forceinline__ float2* next() {
-    turn ^= 1;
-    return slots + turn * 32;
-  }
-
-  __device__ __forceinline__ void warp_sum(float& a) const {
-    const int from = warps > 1 ? 16 : threads / 2;
-    for (int o = from; o > 0; o /= 2) a += __shfl_xor_sync(0xffffffffu, a, o);
-  }
-  __device__ __forceinline__ float2 sum(float a, float b) {
-    if (warps > 1) {
+// Lays the arrays there. All of a group's vectors are asked for before any is used: a CTA waits for
+// memory once for each of its threads' groups, not for each vector.
+template <bool VEC, bool WIDE, bool BACKWARD>
+__device__ __noinline__ void block_stage(const BlockParams& p, int64_t sample, float* memory) {
+  const int C = p.C, groups = (C + 7) / 8;
+  const auto put = [&](int array, int g, const float(&f)[8]) {
+    if (!(p.arrays >> array & 1)) return;
+    float* at = block_place_of(p, memory, array);
+    if constexpr (VEC) {
+      reinterpret_cast<float4*>(at)[g] = make_float4(f[0], f[1], f[2], f[3]);
+      reinterpret_cast<float4*>(at)[groups + g] = make_float4(f[4], f[5], f[6], f[7]);
+    } else {
 #pragma unroll
-      for (int o = 16; o > 0; o /= 2) {
-        a += __shfl_xor_sync(0xffffffffu, a, o);
-        b += __shfl_xor_sync(0xffffffffu, b, o);
-      }
-      float2* at = next();
-      if (threadIdx.x % 32 == 0) at[threadIdx.x / 32] = make_float2(a, b);
-      __syncthreads();
-      a = b = 0.f;
-      for (int w = 0; w < warps; ++w) {
-        a += at[w].x;
-        b += at[w].y;
+      for (int i = 0; i < 8; ++i)
+        if (g * 8 + i < C) at[g * 8 + i] = f[i];
+    }
+  };
+  for (int g = threadIdx.x; g < groups; g += blockDim.x) {
+    float gate[8], weight[8], bias[8], scale[8], shift[8], after_weight[8], after_bias[8];
+    block_channels<VEC>(p.gate, sample, C, g * 8, 1, 1.f, gate);
+    block_channels<VEC>(p.weight, sample, C, g * 8, 1, 1.f, weight);
+    block_channels<VEC>(p.scale, sample, C, g * 8, 1, 0.f, scale);
+    block_channels<VEC>(p.after_weight, sample, C, g * 8, 1, 1.f, after_weight);
+    if constexpr (!BACKWARD) {
+      block_channels<VEC>(p.bias, sample, C, g * 8, 1, 0.f, bias);
+      block_channels<VEC>(p.shift, sample, C, g * 8, 1, 0.f, shift);
+      block_channels<VEC>(p.after_bias, sample, C, g * 8, 1, 0.f, after_bias);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (!WIDE) gate[i] *= static_cast<float>(p.s);
+      if (BACKWARD) gate[i] *= after_weight[i];
+      scale[i] += 1.f;
+      weight[i] *= scale[i];
+      if (!BACKWARD) shift[i] = fmaf(bias[i], scale[i], shift[i]);
+    }
+    put(kArrayGate, g, gate);
+    put(kArrayFactor, g, weight);
+    if constexpr (!BACKWARD) {
+      put(kArrayOffset, g, shift);
+      put(kArrayAfterWeight, g, after_weight);
+      put(kArrayAfterBias, g, after_bias);
+    }
+  }
+  __syncthreads();
+}
+
+template <bool VEC, bool WIDE, bool BACKWARD, bool STAGED>
+struct BlockArrays {
+  const BlockParams& p;
+  float* memory;
+  int64_t sample;
+
+  __device__ __forceinline__ void stage() const {
+    if constexpr (STAGED) block_stage<VEC, WIDE, BACKWARD>(p, sample, memory);
+  }
+  // Group v of a thread that has numbers there.
+  __device__ __forceinline__ Eight get(int array, int tid, int v, float constant) const {
+    if (!(p.arrays >> array & 1)) return eight(constant);
+    Eight f;
+    if constexpr (STAGED) {
+      const float* at = block_place_of(p, memory, array);
+      if constexpr (VEC) {
+        const float4* q = reinterpret_cast<const float4*>(at) + v * p.threads + tid;
+        const float4 a = q[0], b = q[p.C / 8];
+        f.p[0] = make_float2(a.x, a.y), f.p[1] = make_float2(a.z, a.w);
+        f.p[2] = make_float2(b.x, b.y), f.p[3] = make_float2(b.z, b.w);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int c = block_column<false>(p.threads, tid, v, i);
+          f[i] = c < p.C ? at[c] : 0.f;
+        }
       }
     } else {
-      for (int o = threads / 2; o > 0; o /= 2) {
-        a += __shfl_xor_sync(0xffffffffu, a, o);
-        b += __shfl_xor_sync(0xffffffffu, b, o);
-      }
+      float t[8];  // (of its own: what is passed to a function lies in local memory)
+      block_array<VEC, WIDE, BACKWARD>(p, sample, array, block_column<VEC>(p.threads, tid, v, 0), VEC ? 1 : p.threads, t);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[i] = t[i];
     }
-    return make_float2(a, b);
+    return f;
   }
 };
 
-// (mean, rstd) of a row, of which a thread has `f` (zero past the end). The mean is taken of the
+// ---- sums over a row's threads ----
+// These are a power of two within a warp (WARP), or all of the CTA's warps. Results are the same in
+// every thread. Two buffers in turn: one barrier for each sum.
+template <bool WARP>
+struct BlockTeam {
+  int threads;
+  int warps, span;  // span: the power of two that warps fit into
+  double2* slots;   // 2 x 16
+  float count, inv;  // this warp's numbers of the row (all, with WARP), and 1 / these
+  int turn = 0;
+
+  template <typename T>
+  __device__ __forceinline__ void across(T& a, int from) const {
+    for (int o = from; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
+  }
+  template <typename T2>
+  __device__ __forceinline__ T2* next() {
+    turn ^= 1;
+    return reinterpret_cast<T2*>(slots + turn * 16);
+  }
+  // Pairs of FP32 or of FP64.
+  template <bool BOTH, typename T2>
+  __device__ __forceinline__ T2 sum(T2 v) {
+    if constexpr (WARP) {
+      across(v.x, threads >> 1);
+      if (BOTH) across(v.y, threads >> 1);
+    } else {
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
+        if (BOTH) v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
+      }
+      T2* at = next<T2>();
+      const int lane = threadIdx.x % 32;
+      if (lane == 0) at[threadIdx.x / 32] = v;
+      __syncthreads();
+      v = lane < warps ? at[lane] : T2{};
+      across(v.x, span >> 1);
+      if (BOTH) across(v.y, span >> 1);
+      // (lanes beyond the span have sums of zeros)
+      v.x = __shfl_sync(0xffffffffu, v.x, 0);
+      if (BOTH) v.y = __shfl_sync(0xffffffffu, v.y, 0);
+    }
+    return v;
+  }
+};
+
+template <bool VEC, bool WARP>
+__device__ __forceinline__ bool block_inside(const BlockTeam<WARP>& team, int C, int tid, int v, int i) {
+  return block_column<VEC>(team.threads, tid, v, VEC ? 0 : i) < C;
+}
+
+// (mean, rstd) of a row, of which a thread has the groups f (zero past its end). The mean is taken of the
 // distances from a number of the row, and the squares of those from the mean, warp by warp and then
 // between the warps' means: rows of equal numbers have exactly their own mean.
 // FP32's range is that of the numbers, not of their squares: where their sum leaves it (or its
 // accurate part, and eps does not cover that), it is taken again of numbers scaled by a power of two.
-template <int V, bool VEC>
-__device__ __forceinline__ float2 block_stats(BlockTeam& team, const float (&f)[V * 8], int kind, float eps, int C,
-                                              int tid) {
-  const int lane = threadIdx.x % 32;
+template <int V, bool VEC, bool WARP>
+__device__ __forceinline__ float2 block_stats(BlockTeam<WARP>& team, Eight (&f)[V], int kind, float eps, int C, int tid) {
   float by = 1.f;
   for (;;) {
     float mean = 0.f, squares = 0.f;
     if (kind == kBlockRms) {
+      float2 q[2] = {};
 #pragma unroll
-      for (int i = 0; i < V * 8; ++i) squares = fmaf(f[i] * by, f[i] * by, squares);
-      squares = team.sum(squares, 0.f).x;
+      for (int v = 0; v < V; ++v)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) q[i & 1] = __ffma2_rn(f[v].p[i], f[v].p[i], q[i & 1]);
+      q[0] = __fadd2_rn(q[0], q[1]);
+      squares = team.template sum<false>(make_float2(q[0].x + q[0].y, 0.f)).x;
     } else {
-      const auto valid = [&](int i) { return block_column<VEC>(team.threads, tid, i / 8, i % 8) < C; };
-      const float pivot = by * __shfl_sync(0xffffffffu, f[0], team.warps > 1 ? 0 : lane / team.threads * team.threads);
-      float a = 0.f;
+      const int lane = threadIdx.x % 32;
+      const float pivot = __shfl_sync(0xffffffffu, f[0][0], WARP ? lane & ~(team.threads - 1) : 0);
+      float2 a = {}, q = {};
 #pragma unroll
-      for (int i = 0; i < V * 8; ++i) a += valid(i) ? fmaf(f[i], by, -pivot) : 0.f;
-      team.warp_sum(a);
-      const float shift = a * team.warp_inv;
+      for (int v = 0; v < V; ++v) {
+        if constexpr (VEC) {
+          if (block_inside<true>(team, C, tid, v, 0))
 #pragma unroll
-      for (int i = 0; i < V * 8; ++i) {
-        const float d = valid(i) ? fmaf(f[i], by, -pivot) - shift : 0.f;
-        squares = fmaf(d, d, squares);
+            for (int i = 0; i < 4; ++i) a = __fadd2_rn(a, __fadd2_rn(f[v].p[i], twice(-pivot)));
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (block_inside<false>(team, C, tid, v, i)) a.x += f[v][i] - pivot;
+        }
       }
-      team.warp_sum(squares);
+      float sum = a.x + a.y;
+      team.across(sum, WARP ? team.threads >> 1 : 16);
+      const float shift = sum * team.inv;
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        if constexpr (VEC) {
+          if (block_inside<true>(team, C, tid, v, 0))
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float2 d = __fadd2_rn(__fadd2_rn(f[v].p[i], twice(-pivot)), twice(-shift));
+              q = __ffma2_rn(d, d, q);
+            }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (block_inside<false>(team, C, tid, v, i)) {
+              const float d = (f[v][i] - pivot) - shift;
+              q.x = fmaf(d, d, q.x);
+            }
+        }
+      }
+      squares = q.x + q.y;
+      team.across(squares, WARP ? team.threads >> 1 : 16);
       mean = pivot + shift;
-      if (team.warps > 1) {
-        float2* at = team.next();
-        if (lane == 0) at[threadIdx.x / 32] = make_float2(mean, squares);
+      if constexpr (!WARP) {
+        // the warps' (mean, sum of squares, numbers)
+        float4* at = team.template next<float4>();
+        if (lane == 0) at[threadIdx.x / 32] = make_float4(mean, squares, team.count, 0.f);
         __syncthreads();
         const float first = at[0].x;
-        float away = 0.f;
-        for (int w = 0; w < team.warps; ++w) away = fmaf(team.counts[w], at[w].x - first, away);
-        mean = first + away / C;
-        squares = 0.f;
-        for (int w = 0; w < team.warps; ++w) {
-          const float d = at[w].x - mean;
-          squares += fmaf(team.counts[w] * d, d, at[w].y);
-        }
+        const float4 mine = lane < team.warps ? at[lane] : make_float4(first, 0.f, 0.f, 0.f);
+        float away = mine.z * (mine.x - first);
+        team.across(away, team.span >> 1);
+        mean = first + __shfl_sync(0xffffffffu, away, 0) / C;
+        const float d = mine.x - mean;
+        squares = fmaf(mine.z * d, d, mine.y);
+        team.across(squares, team.span >> 1);
+        squares = __shfl_sync(0xffffffffu, squares, 0);
       }
     }
     const bool large = squares > 0x1p120f, small = squares < 0x1p-80f && eps < 0x1p-90f;
     const bool again = by == 1.f && (large || small);
-    if (team.warps > 1 ? !again : !__any_sync(0xffffffffu, again))
-      return make_float2(mean / by, by / sqrtf(squares / C + eps * by * by));
+    if (WARP ? !__any_sync(0xffffffffu, again) : !again) {
+      if (WARP ? __any_sync(0xffffffffu, by != 1.f) : by != 1.f) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) f[v] = pairs([&](float2 a) { return make_float2(a.x / by, a.y / by); }, f[v]);
+      }
+      return make_float2(mean / by, by * rsqrtf(squares * (1.f / C) + eps * by * by));
+    }
     by = large ? 0x1p-70f : small ? 0x1p70f : by;
+#pragma unroll
+    for (int v = 0; v < V; ++v) f[v] = pairs([&](float2 a) { return __fmul2_rn(a, twice(by)); }, f[v]);
   }
 }
 
+// The same in FP64, in one pass over the distances from a number of the row (from zero in the "rms"
+// kind): these and their squares are exact, or nearly so, of 16-bit numbers.
+template <int V, bool VEC, bool WARP>
+__device__ __forceinline__ double2 block_stats_wide(BlockTeam<WARP>& team, const Eight (&f)[V], int kind, float eps,
+                                                    int C, double inv, int tid) {
+  const int lane = threadIdx.x % 32;
+  double pivot = 0.0;
+  if (kind == kBlockLayer) {
+    float first = __shfl_sync(0xffffffffu, f[0][0], WARP ? lane & ~(team.threads - 1) : 0);
+    if constexpr (!WARP) {
+      float2* at = team.template next<float2>();
+      if (threadIdx.x == 0) at[0].x = first;
+      __syncthreads();
+      first = at[0].x;
+    }
+    pivot = first;
+  }
+  double2 sums = make_double2(0.0, 0.0);
+#pragma unroll
+  for (int v = 0; v < V; ++v)
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (block_inside<VEC>(team, C, tid, v, i)) {
+        const double d = static_cast<double>(f[v][i]) - pivot;
+        sums.x += d;
+        sums.y = fma(d, d, sums.y);
+      }
+  sums = team.template sum<true>(sums);
+  const double shift = kind == kBlockLayer ? sums.x * inv : 0.0;
+  const double variance = sums.y * inv - shift * shift;  // (NaN stays)
+  return make_double2(pivot + shift, rsqrt((variance < 0.0 ? 0.0 : variance) + static_cast<double>(eps)));
+}
+
+// ---- the kernels ----
 struct BlockPlace {
   int64_t sample, row0, row1;
   int tid, part, parts;  // place in the row; which of the CTA's rows at a time
 };
 
+template <bool WARP>
 __device__ __forceinline__ BlockPlace block_place(const BlockParams& p) {
   BlockPlace b;
   b.sample = blockIdx.x / p.chunks;
   const int64_t k = blockIdx.x % p.chunks;
   b.row0 = b.sample * p.T + k * p.chunk;
   b.row1 = b.sample * p.T + min((k + 1) * p.chunk, p.T);
-  b.tid = threadIdx.x % p.threads;
-  b.part = threadIdx.x / p.threads;
-  b.parts = blockDim.x / p.threads;
+  b.tid = WARP ? threadIdx.x & (p.threads - 1) : threadIdx.x;
+  b.part = WARP ? threadIdx.x / p.threads : 0;
+  b.parts = WARP ? blockDim.x / p.threads : 1;
   return b;
 }
 
-template <int V, bool VEC>
-__device__ __forceinline__ BlockTeam block_team(const BlockParams& p, int tid, float2* slots, float* counts) {
-  BlockTeam team{p.threads, p.threads > 32 ? p.threads / 32 : 1, slots, counts, 0.f};
-  float n = 0.f;
+template <int V, bool VEC, bool WARP>
+__device__ __forceinline__ BlockTeam<WARP> block_team(const BlockParams& p, int tid, double2* slots) {
+  BlockTeam<WARP> team{p.threads, p.threads / 32, 1, slots, static_cast<float>(p.C), 1.f / p.C};
+  if constexpr (!WARP) {
+    while (team.span < team.warps) team.span *= 2;
+    float n = 0.f;
 #pragma unroll
-  for (int i = 0; i < V * 8; ++i) n += block_column<VEC>(p.threads, tid, i / 8, i % 8) < p.C ? 1.f : 0.f;
-  team.warp_sum(n);
-  team.warp_inv = n > 0.f ? 1.f / n : 0.f;
-  if (threadIdx.x % 32 == 0) counts[threadIdx.x / 32] = n;  // (read behind a barrier)
+    for (int i = 0; i < V * 8; ++i) n += block_column<VEC>(p.threads, tid, i / 8, i % 8) < p.C ? 1.f : 0.f;
+    team.across(n, 16);
+    team.count = n;
+    team.inv = 1.f / n;
+  }
   return team;
 }
 
-// The vectors of a thread's columns: kept in registers where it has eight of them.
-template <int V, bool VEC>
-struct BlockVectors {
-  float keep[V == 1 ? 8 : 1];
-  template <typename F>
-  __device__ __forceinline__ void first(F make) {
-    if constexpr (V == 1) make(0, keep);
-  }
-  template <typename F>
-  __device__ __forceinline__ void get(int v, float (&f)[8], F make) const {
-    if constexpr (V == 1) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] = keep[i];
-    } else {
-      make(v, f);
-    }
-  }
-};
+// Registers, and with them how many threads an SM holds.
+constexpr int block_forward_registers(int v, int mode) { return mode == kBlockAfter ? 128 : v >= 4 ? 96 : 80; }
+constexpr int block_backward_registers(int v) { return v > 2 ? 128 : 168; }
+constexpr int block_resident(int registers) { return 65536 / registers / 32 * 32; }
 
-template <typename X, typename Y, int V, bool VEC>
-__global__ void __launch_bounds__(kBlockMaxThreads, 2)
-    block_norm_forward_kernel(const __grid_constant__ BlockParams p) {
-  __shared__ float2 slots[2 * 32];
-  __shared__ float counts[kBlockMaxThreads / 32];
+template <typename X, typename Y, int V, bool VEC, bool WARP, int MODE, bool STAGED>
+__global__ void __maxnreg__(block_forward_registers(V, MODE)) block_norm_forward_kernel(const __grid_constant__ BlockParams p) {
+  extern __shared__ __align__(16) unsigned char block_memory[];
+  __shared__ double2 slots[2 * 16];
   grid_dependency_wait();
   grid_launch_dependents();
-  const BlockPlace b = block_place(p);
-  const int C = p.C, tid = b.tid;
-  BlockTeam team = block_team<V, VEC>(p, tid, slots, counts);
-  const auto channels = [&](const BlockChannels& ch, int v, float missing, float (&f)[8]) {
-    block_channels<VEC>(ch, b.sample, C, p.threads, tid, v, missing, f);
+  // 16-bit results of a normalised branch are formed in FP64, and so rounded once in all but name
+  constexpr bool kWide = MODE == kBlockAfter && sizeof(X) == 2;
+  const BlockPlace b = block_place<WARP>(p);
+  const int C = p.C, tid = b.tid, threads = p.threads;
+  BlockTeam<WARP> team = block_team<V, VEC, WARP>(p, tid, slots);
+  const bool branch = MODE == kBlockPlain || (MODE == kBlockAfter && p.y);
+  const bool after_norm = MODE == kBlockAfter && p.after_kind;
+  using RowX = BlockRow<X, V, VEC>;
+  using RowY = BlockRow<Y, V, VEC>;
+  RowX row_x;
+  RowY row_y;
+  const unsigned at_y = RowX::kVecs * blockDim.x * 16;
+  BlockRing ring(block_memory, RowX::kVecs + (branch ? RowY::kVecs : 0), p.stages);
+  int64_t ahead = b.row0 + b.part;
+  const auto fetch = [&] {
+    if (ahead < b.row1) {
+      const unsigned slot = ring.base + ring.put * ring.bytes;
+      RowX::copy(slot, p.x, ahead * C, C, threads, tid);
+      if (branch) RowY::copy(slot + at_y, p.y, ahead * C, C, threads, tid);
+    }
+    ring.put = ring.put + 1 == ring.stages ? 0 : ring.put + 1;
+    ring.commit();
+    ahead += b.parts;
   };
-  // s * gate; z = rhat * factor + offset
-  const auto make_gate = [&](int v, float (&f)[8]) {
-    channels(p.gate, v, 1.f, f);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] *= p.s;
-  };
-  const auto make_factor = [&](int v, float (&f)[8]) {
-    float w[8];
-    channels(p.weight, v, 1.f, w);
-    channels(p.scale, v, 0.f, f);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = w[i] * (1.f + f[i]);
-  };
-  const auto make_offset = [&](int v, float (&f)[8]) {
-    float w[8], t[8];
-    channels(p.bias, v, 0.f, w);
-    channels(p.scale, v, 0.f, t);
-    channels(p.shift, v, 0.f, f);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = fmaf(w[i], 1.f + t[i], f[i]);
-  };
-  const auto make_after_weight = [&](int v, float (&f)[8]) { channels(p.after_weight, v, 1.f, f); };
-  const auto make_after_bias = [&](int v, float (&f)[8]) { channels(p.after_bias, v, 0.f, f); };
-  BlockVectors<V, VEC> gate, factor, offset, after_weight, after_bias;
-  if (p.y) {
-    gate.first(make_gate);
-    after_weight.first(make_after_weight);
-    after_bias.first(make_after_bias);
-  }
-  if (p.z) {
-    factor.first(make_factor);
-    offset.first(make_offset);
-  }
-  BlockRaw<X, V, VEC> x;
-  BlockRaw<Y, V, VEC> y;
-  const auto fetch = [&](int64_t row) {
-    const bool active = row < b.row1;
-    x.load(static_cast<const X*>(p.x) + row * C, C, p.threads, tid, active);
-    if (p.y) y.load(static_cast<const Y*>(p.y) + row * C, C, p.threads, tid, active);
-  };
-  fetch(b.row0 + b.part);
+  if constexpr (VEC)
+    for (int k = 1; k < p.stages; ++k) fetch();
+  const BlockArrays<VEC, kWide, false, STAGED> arrays{p, reinterpret_cast<float*>(block_memory + (VEC ? p.stages * ring.bytes : 0)),
+                                              b.sample};
+  arrays.stage();
+  const float s = static_cast<float>(p.s);
   for (int64_t first = b.row0; first < b.row1; first += b.parts) {
-    const int64_t row = first + b.part;
-    const bool active = row < b.row1;
-    float r[V * 8], t[V * 8];
-    x.widen(r);
-    if (p.y) y.widen(t);
-    fetch(row + b.parts);
-    if (p.y) {
-      float2 after = make_float2(0.f, 1.f);
-      if (p.after_kind) after = block_stats<V, VEC>(team, t, p.after_kind, p.eps, C, tid);
+    const int64_t row = first + b.part, offset = row * C;
+    const bool active = !WARP || row < b.row1;
+    unsigned slot = 0;
+    if constexpr (VEC) {
+      fetch();
+      ring.wait();
+      slot = ring.next(ring.get);
+    } else {
+      row_x.load(p.x, offset, C, threads, tid, active);
+      if (branch) row_y.load(p.y, offset, C, threads, tid, active);
+    }
+    const auto ok = [&](int v) { return active && block_column<VEC>(threads, tid, v, 0) < C; };
+    Eight r[V];
+    float2 after = make_float2(0.f, 1.f);
+    double2 wide = make_double2(0.0, 1.0);
+    if (after_norm) {
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        float g[8], w[8], o[8];
-        gate.get(v, g, make_gate);
-        if (p.after_kind) {
-          after_weight.get(v, w, make_after_weight);
-          after_bias.get(v, o, make_after_bias);
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          float u = t[v * 8 + i];
-          if (p.after_kind) u = fmaf((u - after.x) * after.y, w[i], o[i]);
-          r[v * 8 + i] = __fadd_rn(r[v * 8 + i], __fmul_rn(g[i], u));
-        }
+      for (int v = 0; v < V; ++v) r[v] = row_y.get(slot + at_y, v, ok(v));
+      if constexpr (kWide) {
+        wide = block_stats_wide<V, VEC, WARP>(team, r, p.after_kind, p.eps, C, p.inv, tid);
+        after = make_float2(static_cast<float>(wide.x), static_cast<float>(wide.y));
+      } else {
+        after = block_stats<V, VEC, WARP>(team, r, p.after_kind, p.eps, C, tid);
       }
       if (p.after_stats && active && tid == 0) p.after_stats[row] = after;
-      BlockRaw<X, V, VEC> out;
-      out.narrow(r);
-      if (active) out.store(static_cast<X*>(p.r) + row * C, C, p.threads, tid);
-      out.widen(r);  // z is the norm of r as it is held
-      if (!VEC || V * 8 * p.threads != C) {
-#pragma unroll
-        for (int i = 0; i < V * 8; ++i)
-          if (block_column<VEC>(p.threads, tid, i / 8, i % 8) >= C) r[i] = 0.f;
-      }
     }
-    if (!p.z) continue;
-    const float2 stats = block_stats<V, VEC>(team, r, p.kind, p.eps, C, tid);
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      r[v] = row_x.get(slot, v, ok(v));
+      if (!branch || !ok(v)) continue;
+      Eight u = row_y.get(slot + at_y, v, true);
+      const Eight g = arrays.get(kArrayGate, tid, v, kWide ? 1.f : s);
+      BlockPacked<X> e;
+      if constexpr (kWide) {
+        X* one = reinterpret_cast<X*>(&e);
+        if (after_norm) {
+          const Eight w = arrays.get(kArrayAfterWeight, tid, v, 1.f), o = arrays.get(kArrayAfterBias, tid, v, 0.f);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const double t = fma((u[i] - wide.x) * wide.y, static_cast<double>(w[i]), static_cast<double>(o[i]));
+            one[i] = block_narrow<X>(fma(t, p.s * g[i], static_cast<double>(r[v][i])));
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            one[i] = block_narrow<X>(fma(static_cast<double>(u[i]), p.s * g[i], static_cast<double>(r[v][i])));
+        }
+      } else {
+        if (after_norm) {
+          const Eight w = arrays.get(kArrayAfterWeight, tid, v, 1.f), o = arrays.get(kArrayAfterBias, tid, v, 0.f);
+          u = pairs([&](float2 a, float2 w2, float2 o2) {
+            return __ffma2_rn(__fmul2_rn(__fadd2_rn(a, twice(-after.x)), twice(after.y)), w2, o2);
+          }, u, w, o);
+        }
+        // (two roundings, as of a product and a sum one after the other)
+        e = BlockPacked<X>::of(pairs([](float2 a, float2 g2, float2 x) { return __fadd2_rn(x, __fmul2_rn(g2, a)); }, u, g, r[v]));
+      }
+      block_store<X, VEC>(p.r, offset, C, threads, tid, v, e);
+      r[v] = e.widen();  // z is the norm of r as it is held
+      if constexpr (!VEC)
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (block_column<VEC>(threads, tid, v, i) >= C) r[v][i] = 0.f;
+    }
+    if (MODE != kBlockBefore && !p.z) continue;
+    const float2 stats = block_stats<V, VEC, WARP>(team, r, p.kind, p.eps, C, tid);
     if (p.stats && active && tid == 0) p.stats[row] = stats;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      float a[8], o[8];
-      factor.get(v, a, make_factor);
-      offset.get(v, o, make_offset);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) t[v * 8 + i] = fmaf((r[v * 8 + i] - stats.x) * stats.y, a[i], o[i]);
+      if (!ok(v)) continue;
+      const Eight a = arrays.get(kArrayFactor, tid, v, 1.f), o = arrays.get(kArrayOffset, tid, v, 0.f);
+      const Eight z = pairs([&](float2 b, float2 a2, float2 o2) {
+        return __ffma2_rn(__fmul2_rn(__fadd2_rn(b, twice(-stats.x)), twice(stats.y)), a2, o2);
+      }, r[v], a, o);
+      block_store<Y, VEC>(p.z, offset, C, threads, tid, v, BlockPacked<Y>::of(z));
     }
-    BlockRaw<Y, V, VEC> out;
-    out.narrow(t);
-    if (active) out.store(static_cast<Y*>(p.z) + row * C, C, p.threads, tid);
   }
 }
 
-template <typename X, typename Y, int V, bool VEC>
-__global__ void __launch_bounds__(kBlockMaxThreads, 1)
-    block_norm_backward_kernel(const __grid_constant__ BlockParams p) {
-  __shared__ float2 slots[2 * 32];
-  __shared__ float counts[kBlockMaxThreads / 32];
+template <typename X, typename Y, int V, bool VEC, bool WARP, int MODE, bool STAGED>
+__global__ void __maxnreg__(block_backward_registers(V)) block_norm_backward_kernel(const __grid_constant__ BlockParams p) {
+  extern __shared__ __align__(16) unsigned char block_memory[];
+  __shared__ double2 slots[2 * 16];
   grid_dependency_wait();
   grid_launch_dependents();
-  const BlockPlace b = block_place(p);
-  const int C = p.C, tid = b.tid;
-  BlockTeam team = block_team<V, VEC>(p, tid, slots, counts);
-  const auto channels = [&](const BlockChannels& ch, int v, float missing, float (&f)[8]) {
-    block_channels<VEC>(ch, b.sample, C, p.threads, tid, v, missing, f);
+  const BlockPlace b = block_place<WARP>(p);
+  const int C = p.C, tid = b.tid, threads = p.threads;
+  BlockTeam<WARP> team = block_team<V, VEC, WARP>(p, tid, slots);
+  const bool branch = MODE == kBlockPlain || (MODE == kBlockAfter && p.y);
+  const bool after_norm = MODE == kBlockAfter && p.after_kind;
+  const bool has_dr = MODE != kBlockBefore && p.dr, has_dz = MODE == kBlockBefore || p.dz;
+  using RowX = BlockRow<X, V, VEC>;
+  using RowY = BlockRow<Y, V, VEC>;
+  RowX row_r, row_dr;
+  RowY row_y, row_dz;
+  // places in a stage: r, dz, dr, y
+  const unsigned step = blockDim.x * 16, at_dz = RowX::kVecs * step;
+  const unsigned at_dr = has_dz ? at_dz + RowY::kVecs * step : 0;
+  const unsigned at_y = at_dr + (has_dr ? RowX::kVecs * step : 0);
+  BlockRing ring(block_memory, at_y / step + (branch ? RowY::kVecs : 0), p.stages);
+  int64_t ahead = b.row0 + b.part;
+  const auto fetch = [&] {
+    if (ahead < b.row1) {
+      const unsigned slot = ring.base + ring.put * ring.bytes;
+      const int64_t offset = ahead * C;
+      if (has_dz) {
+        RowX::copy(slot, p.r, offset, C, threads, tid);
+        RowY::copy(slot + at_dz, p.dz, offset, C, threads, tid);
+      }
+      if (has_dr) RowX::copy(slot + at_dr, p.dr, offset, C, threads, tid);
+      if (branch) RowY::copy(slot + at_y, p.y, offset, C, threads, tid);
+    }
+    ring.put = ring.put + 1 == ring.stages ? 0 : ring.put + 1;
+    ring.commit();
+    ahead += b.parts;
   };
-  const auto make_gate = [&](int v, float (&f)[8]) {
-    channels(p.gate, v, 1.f, f);
+  if constexpr (VEC)
+    for (int k = 1; k < p.stages; ++k) fetch();
+  const BlockArrays<VEC, false, true, STAGED> arrays{p, reinterpret_cast<float*>(block_memory + (VEC ? p.stages * ring.bytes : 0)),
+                                             b.sample};
+  arrays.stage();
+  constexpr int kSums = MODE == kBlockBefore ? 2 : MODE == kBlockPlain ? 3 : 4;
+  Eight sums[kSums][V];  // over rows: dz, dz rhat, dR yhat, dR
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] *= p.s;
-  };
-  const auto make_factor = [&](int v, float (&f)[8]) {
-    float w[8];
-    channels(p.weight, v, 1.f, w);
-    channels(p.scale, v, 0.f, f);
+  for (int k = 0; k < kSums; ++k)
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = w[i] * (1.f + f[i]);
-  };
-  const auto make_after_weight = [&](int v, float (&f)[8]) { channels(p.after_weight, v, 1.f, f); };
-  BlockVectors<V, VEC> gate, factor, after_weight;
-  if (p.y) {
-    gate.first(make_gate);
-    after_weight.first(make_after_weight);
-  }
-  if (p.dz) factor.first(make_factor);
-  float sums[4][V * 8];  // over rows: dz, dz rhat, dR, dR yhat
-#pragma unroll
-  for (int k = 0; k < 4; ++k)
-#pragma unroll
-    for (int i = 0; i < V * 8; ++i) sums[k][i] = 0.f;
-  BlockRaw<X, V, VEC> raw_r, raw_dr;
-  BlockRaw<Y, V, VEC> raw_y, raw_dz;
-  float2 stats{}, after{};
-  const auto fetch = [&](int64_t row) {
+    for (int v = 0; v < V; ++v) sums[k][v] = eight(0.f);
+  const float inv = 1.f / C, s = static_cast<float>(p.s);
+  float2 next1, next2;
+  const auto stats_of = [&](int64_t row) {
     const bool active = row < b.row1;
-    if (p.dz) {
-      raw_r.load(static_cast<const X*>(p.r) + row * C, C, p.threads, tid, active);
-      raw_dz.load(static_cast<const Y*>(p.dz) + row * C, C, p.threads, tid, active);
-      stats = active ? p.stats[row] : float2{};
-    }
-    if (p.dr) raw_dr.load(static_cast<const X*>(p.dr) + row * C, C, p.threads, tid, active);
-    if (p.y) {
-      raw_y.load(static_cast<const Y*>(p.y) + row * C, C, p.threads, tid, active);
-      after = active && p.after_kind ? p.after_stats[row] : make_float2(0.f, 1.f);
-    }
+    next1 = active && has_dz ? p.stats[row] : float2{};
+    next2 = active && after_norm ? p.after_stats[row] : make_float2(0.f, 1.f);
   };
-  const float inv = 1.f / C;
-  fetch(b.row0 + b.part);
+  stats_of(b.row0 + b.part);
   for (int64_t first = b.row0; first < b.row1; first += b.parts) {
-    const int64_t row = first + b.part;
-    const bool active = row < b.row1;
-    float d[V * 8], h[V * 8], y[V * 8];  // dR; rhat and then e; yhat
-    const float2 s1 = stats, s2 = after;
-#pragma unroll
-    for (int i = 0; i < V * 8; ++i) d[i] = 0.f;
-    if (p.dr) raw_dr.widen(d);
-    if (p.y) {
-      raw_y.widen(y);
-#pragma unroll
-      for (int i = 0; i < V * 8; ++i) y[i] = (y[i] - s2.x) * s2.y;
+    const int64_t row = first + b.part, offset = row * C;
+    const bool active = !WARP || row < b.row1;
+    const float2 s1 = next1, s2 = next2;
+    stats_of(row + b.parts);
+    unsigned slot = 0;
+    if constexpr (VEC) {
+      fetch();
+      ring.wait();
+      slot = ring.next(ring.get);
+    } else {
+      if (has_dz) {
+        row_r.load(p.r, offset, C, threads, tid, active);
+        row_dz.load(p.dz, offset, C, threads, tid, active);
+      }
+      if (has_dr) row_dr.load(p.dr, offset, C, threads, tid, active);
+      if (branch) row_y.load(p.y, offset, C, threads, tid, active);
     }
-    if (p.dz) {
-      float dz[V * 8];
-      raw_r.widen(h);
-      raw_dz.widen(dz);
-      fetch(row + b.parts);
-      float a1 = 0.f, a2 = 0.f;
+    const auto ok = [&](int v) { return active && block_column<VEC>(threads, tid, v, 0) < C; };
+    const auto get_rhat = [&](int v) {
+      return pairs([&](float2 a) { return __fmul2_rn(__fadd2_rn(a, twice(-s1.x)), twice(s1.y)); }, row_r.get(slot, v, true));
+    };
+    const auto get_yhat = [&](int v) {
+      const Eight y = row_y.get(slot + at_y, v, true);
+      return after_norm ? pairs([&](float2 a) { return __fmul2_rn(__fadd2_rn(a, twice(-s2.x)), twice(s2.y)); }, y) : y;
+    };
+    const auto times = [](float2 a, float2 b2) { return __fmul2_rn(a, b2); };
+    float m1 = 0.f, m2 = 0.f;
+    if (has_dz) {
+      float2 mean[2] = {};
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        float f[8];
-        factor.get(v, f, make_factor);
+        if (!ok(v)) continue;
+        const Eight h = get_rhat(v), dz = row_dz.get(slot + at_dz, v, true);
+        const Eight a = pairs(times, dz, arrays.get(kArrayFactor, tid, v, 1.f));
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int j = v * 8 + i;
-          h[j] = (h[j] - s1.x) * s1.y;
-          sums[0][j] += dz[j];
-          sums[1][j] = fmaf(dz[j], h[j], sums[1][j]);
-          dz[j] *= f[i];
-          a1 += dz[j];
-          a2 = fmaf(dz[j], h[j], a2);
+        for (int i = 0; i < 4; ++i) {
+          sums[0][v].p[i] = __fadd2_rn(sums[0][v].p[i], dz.p[i]);
+          sums[1][v].p[i] = __ffma2_rn(dz.p[i], h.p[i], sums[1][v].p[i]);
+          mean[0] = __fadd2_rn(mean[0], a.p[i]);
+          mean[1] = __ffma2_rn(a.p[i], h.p[i], mean[1]);
         }
       }
-      const float2 a = team.sum(a1, a2);
-      const float m1 = p.kind == kBlockLayer ? a.x * inv : 0.f, m2 = a.y * inv;
-#pragma unroll
-      for (int i = 0; i < V * 8; ++i) d[i] = fmaf(s1.y, (dz[i] - m1) - h[i] * m2, d[i]);
-    } else {
-      fetch(row + b.parts);
+      const float2 m = team.template sum<true>(make_float2(mean[0].x + mean[0].y, mean[1].x + mean[1].y));
+      m1 = p.kind == kBlockLayer ? m.x * inv : 0.f;
+      m2 = m.y * inv;
     }
-    if (p.dx) {
-      BlockRaw<X, V, VEC> out;
-      out.narrow(d);
-      if (active) out.store(static_cast<X*>(p.dx) + row * C, C, p.threads, tid);
-    }
-    if (!p.y) continue;
-    float a1 = 0.f, a2 = 0.f;
+    Eight e[MODE == kBlockAfter ? V : 1];  // the gradient of yhat
+    float2 mean[2] = {};
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      float g[8], w[8];
-      gate.get(v, g, make_gate);
-      after_weight.get(v, w, make_after_weight);
+      if (!ok(v)) continue;
+      Eight d = has_dr ? row_dr.get(slot + at_dr, v, true) : eight(0.f);
+      if (has_dz) {
+        const Eight h = get_rhat(v);
+        const Eight a = pairs(times, row_dz.get(slot + at_dz, v, true), arrays.get(kArrayFactor, tid, v, 1.f));
+        d = pairs([&](float2 d2, float2 a2, float2 h2) {
+          return __ffma2_rn(twice(s1.y), __ffma2_rn(h2, twice(-m2), __fadd2_rn(a2, twice(-m1))), d2);
+        }, d, a, h);
+      }
+      if (p.dx) block_store<X, VEC>(p.dx, offset, C, threads, tid, v, BlockPacked<X>::of(d));
+      if (!branch) continue;
+      if constexpr (!VEC)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int j = v * 8 + i;
-        if (block_column<VEC>(p.threads, tid, v, i) >= C || !active) d[j] = 0.f;
-        sums[2][j] += d[j];
-        sums[3][j] = fmaf(d[j], y[j], sums[3][j]);
-        h[j] = d[j] * g[i];
-        if (p.after_kind) h[j] *= w[i];
-        a1 += h[j];
-        a2 = fmaf(h[j], y[j], a2);
+        for (int i = 0; i < 8; ++i)
+          if (block_column<VEC>(threads, tid, v, i) >= C) d[i] = 0.f;
+      const Eight y = get_yhat(v);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (kSums > 2) sums[2][v].p[i] = __ffma2_rn(d.p[i], y.p[i], sums[2][v].p[i]);
+        if constexpr (kSums > 3) sums[3][v].p[i] = __fadd2_rn(sums[3][v].p[i], d.p[i]);
+      }
+      d = pairs(times, d, arrays.get(kArrayGate, tid, v, s));
+      if (after_norm) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          mean[0] = __fadd2_rn(mean[0], d.p[i]);
+          mean[1] = __ffma2_rn(d.p[i], y.p[i], mean[1]);
+        }
+        if constexpr (MODE == kBlockAfter) e[v] = d;
+      } else if (p.dy) {
+        block_store<Y, VEC>(p.dy, offset, C, threads, tid, v, BlockPacked<Y>::of(d));
       }
     }
-    if (!p.dy) continue;
-    if (p.after_kind) {
-      const float2 a = team.sum(a1, a2);
-      const float m1 = p.after_kind == kBlockLayer ? a.x * inv : 0.f, m2 = a.y * inv;
+    if constexpr (MODE == kBlockAfter) {
+      if (!p.dy || !after_norm) continue;
+      const float2 m = team.template sum<true>(make_float2(mean[0].x + mean[0].y, mean[1].x + mean[1].y));
+      m1 = p.after_kind == kBlockLayer ? m.x * inv : 0.f;
+      m2 = m.y * inv;
 #pragma unroll
-      for (int i = 0; i < V * 8; ++i) h[i] = s2.y * ((h[i] - m1) - y[i] * m2);
+      for (int v = 0; v < V; ++v) {
+        if (!ok(v)) continue;
+        const Eight dy = pairs([&](float2 e2, float2 y2) {
+          return __fmul2_rn(twice(s2.y), __ffma2_rn(y2, twice(-m2), __fadd2_rn(e2, twice(-m1))));
+        }, e[v], get_yhat(v));
+        block_store<Y, VEC>(p.dy, offset, C, threads, tid, v, BlockPacked<Y>::of(dy));
+      }
     }
-    BlockRaw<Y, V, VEC> out;
-    out.narrow(h);
-    if (active) out.store(static_cast<Y*>(p.dy) + row * C, C, p.threads, tid);
   }
   if (!p.partials) return;
   float* mine = p.partials + static_cast<int64_t>(blockIdx.x) * p.sums * C;
-  if (p.threads > 32) {
+  if constexpr (!WARP) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
+    for (int k = 0; k < kSums; ++k)
       if (k < p.sums)
 #pragma unroll
-        for (int i = 0; i < V * 8; ++i) {
-          const int c = block_column<VEC>(p.threads, tid, i / 8, i % 8);
-          if (c < C) mine[k * C + c] = sums[k][i];
+        for (int v = 0; v < V; ++v) {
+          if (block_column<VEC>(threads, tid, v, 0) < C)
+            block_store<float, VEC>(mine, k * C, C, threads, tid, v, BlockPacked<float>::of(sums[k][v]));
         }
-    return;
-  }
-  // rows side by side: their sums are added up over the warp's parts and the warps
-  __shared__ float all[kBlockSmallThreads / 32][8 * 32];
+  } else {
+    // rows side by side: their sums are added up over the warp's parts and the warps
+    float* all = reinterpret_cast<float*>(block_memory);
+    const int warps = blockDim.x / 32;
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    if (k >= p.sums) break;
+    for (int k = 0; k < kSums; ++k) {
+      if (k >= p.sums) break;
+      __syncthreads();  // (the ring's last rows, or the sums before, are read)
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      float v = sums[k][i];
-      for (int o = 16; o >= p.threads; o /= 2) v += __shfl_xor_sync(0xffffffffu, v, o);
-      const int c = block_column<VEC>(p.threads, tid, 0, i);
-      if (threadIdx.x % 32 < p.threads && c < C) all[threadIdx.x / 32][c] = v;
-    }
-    __syncthreads();
-    for (int c = threadIdx.x; c < C; c += blockDim.x) {
-      float v = 0.f;
-      for (int w = 0; w < blockDim.x / 32; ++w) v += all[w][c];
-      mine[k * C + c] = v;
-    }
-    __syncthreads();
-  }
-}
-
-constexpr int kBlockMergeColumns = 32, kBlockMergeTeams = 8;
-
-// Adds the CTAs' sums up: to (sample, segment, sum, C) in FP64, over the segment's share of a sample's CTAs.
-__global__ void __launch_bounds__(kBlockMergeColumns * kBlockMergeTeams)
-    block_norm_merge_kernel(const float* partials, double* merged, int C, int sums, int64_t chunks, int segments) {
-  __shared__ double sm[kBlockMergeTeams][kBlockMergeColumns];
-  grid_dependency_wait();
-  grid_launch_dependents();
-  const int lane = threadIdx.x % kBlockMergeColumns, team = threadIdx.x / kBlockMergeColumns;
-  const int columns = (C + kBlockMergeColumns - 1) / kBlockMergeColumns;
-  const int c = blockIdx.x % columns * kBlockMergeColumns + lane;
-  const int64_t place = blockIdx.x / columns, sample = place / segments, segment = place % segments;
-  const int64_t k0 = chunks * segment / segments, k1 = chunks * (segment + 1) / segments;
-  for (int k = 0; k < sums; ++k) {
-    double v = 0.0;
-    if (c < C)
-      for (int64_t j = k0 + team; j < k1; j += kBlockMergeTeams)
-        v += static_cast<double>(partials[((sample * chunks + j) * sums + k) * C + c]);
-    sm[team][lane] = v;
-    __syncthreads();
-    if (team == 0) {
-      for (int t = 1; t < kBlockMergeTeams; ++t) v += sm[t][lane];
-      if (c < C) merged[(place * sums + k) * C + c] = v;
-    }
-    __syncthreads();
-  }
-}
-
-// A gradient's place: a vector's type and form (C, or C for each sample).
-struct BlockGrad {
-  void* data;
-  int dtype;
-  int per_sample;
-};
-
-struct BlockGradParams {
-  const double* merged;   // or, of one CTA for each sample, its own sums:
-  const float* partials;
-  int64_t B;
-  int segments, sums, C;
-  float s;
-  BlockChannels gate, weight, bias, scale, after_weight, after_bias;
-  BlockGrad dgate, dweight, dbias, dscale, dshift, dafter_weight, dafter_bias;
-};
-
-__device__ __forceinline__ void block_put(const BlockGrad& g, int64_t at, double v) {
-  if (g.dtype == 0) static_cast<float*>(g.data)[at] = static_cast<float>(v);
-  else if (g.dtype == 1) static_cast<__half*>(g.data)[at] = run_narrow<__half>(static_cast<float>(v));
-  else static_cast<__nv_bfloat16*>(g.data)[at] = run_narrow<__nv_bfloat16>(static_cast<float>(v));
-}
-
-// The vectors' gradients from a column's sums: those with one for each sample directly, others
-// summed over the samples.
-__global__ void __launch_bounds__(kBlockMergeColumns * kBlockMergeTeams)
-    block_norm_grads_kernel(const __grid_constant__ BlockGradParams p) {
-  __shared__ double sm[7][kBlockMergeTeams][kBlockMergeColumns];
-  grid_dependency_wait();
-  grid_launch_dependents();
-  const int lane = threadIdx.x % kBlockMergeColumns, team = threadIdx.x / kBlockMergeColumns;
-  const int c = blockIdx.x * kBlockMergeColumns + lane, C = p.C;
-  const BlockGrad* grads[7] = {&p.dshift, &p.dscale, &p.dweight, &p.dbias, &p.dgate, &p.dafter_weight, &p.dafter_bias};
-  double all[7] = {};
-  const auto of = [&](const BlockChannels& ch, int64_t sample, double missing) {
-    return ch.data ? static_cast<double>(block_channel(ch.data, ch.dtype, ch.per_sample ? sample * C + c : c)) : missing;
-  };
-  if (c < C)
-    for (int64_t b = team; b < p.B; b += kBlockMergeTeams) {
-      double sum[4] = {};
-      for (int g = 0; g < p.segments; ++g)
-        for (int k = 0; k < p.sums; ++k) {
-          const int64_t at = ((b * p.segments + g) * p.sums + k) * C + c;
-          sum[k] += p.merged ? p.merged[at] : static_cast<double>(p.partials[at]);
-        }
-      const double lift = 1.0 + of(p.scale, b, 0.0), gate = p.s * of(p.gate, b, 1.0);
-      const double v[7] = {sum[0],
-                           of(p.weight, b, 1.0) * sum[1] + of(p.bias, b, 0.0) * sum[0],
-                           lift * sum[1],
-                           lift * sum[0],
-                           p.s * (of(p.after_weight, b, 1.0) * sum[3] + of(p.after_bias, b, 0.0) * sum[2]),
-                           gate * sum[3],
-                           gate * sum[2]};
-#pragma unroll
-      for (int k = 0; k < 7; ++k) {
-        if (grads[k]->data && grads[k]->per_sample) block_put(*grads[k], b * C + c, v[k]);
-        all[k] += v[k];
+      for (int i = 0; i < V * 8; ++i) {
+        float v = sums[k][i / 8][i % 8];
+        for (int o = 16; o >= threads; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        const int c = block_column<VEC>(threads, tid, i / 8, i % 8);
+        if (threadIdx.x % 32 < threads && c < C) all[threadIdx.x / 32 * C + c] = v;
+      }
+      __syncthreads();
+      for (int c = threadIdx.x; c < C; c += blockDim.x) {
+        float v = 0.f;
+        for (int w = 0; w < warps; ++w) v += all[w * C + c];
+        mine[k * C + c] = v;
       }
     }
-#pragma unroll
-  for (int k = 0; k < 7; ++k) sm[k][team][lane] = all[k];
-  __syncthreads();
-  if (team < 7 && c < C && grads[team]->data && !grads[team]->per_sample) {
-    double v = 0.0;
-    for (int t = 0; t < kBlockMergeTeams; ++t) v += sm[team][t][lane];
-    block_put(*grads[team], c, v);
   }
 }
 

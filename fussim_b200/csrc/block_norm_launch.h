@@ -1,0 +1,114 @@
+// Launches of the block norms' row kernels: one source file for each pair of types.
+#pragma once
+
+#include <cuda_runtime.h>
+
+#include <atomic>
+
+#include "block_norm.cuh"
+#include "engine_host.h"
+#include "launch_host.h"
+
+namespace fssim_host {
+
+struct BlockLaunch {
+  int groups;   // of eight numbers, of a thread
+  bool vec;     // whole 16-byte vectors
+  bool warp;    // a row within a warp
+  bool staged;  // the arrays in shared memory
+  int mode;     // fssim::BlockMode
+  unsigned grid, block;
+  size_t memory;
+};
+
+int block_norm_f32(bool backward, const BlockLaunch& l, const fssim::BlockParams& p, cudaStream_t stream);
+int block_norm_f16(bool backward, const BlockLaunch& l, const fssim::BlockParams& p, cudaStream_t stream);
+int block_norm_bf16(bool backward, const BlockLaunch& l, const fssim::BlockParams& p, cudaStream_t stream);
+int block_norm_f32_f16(bool backward, const BlockLaunch& l, const fssim::BlockParams& p, cudaStream_t stream);
+int block_norm_f32_bf16(bool backward, const BlockLaunch& l, const fssim::BlockParams& p, cudaStream_t stream);
+
+constexpr int64_t kBlockMemory = 208 << 10;  // dynamic shared memory of a CTA at most
+
+// Opts a kernel in to that, once for each device. `done` belongs to one kernel.
+template <typename Kernel>
+int block_allow(Kernel kernel, std::atomic<bool> (&done)[64]) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && (dev < 0 || dev >= 64)) return fail(FSSIM_ERR_CUDA, "device ordinal out of range");
+  if (e == cudaSuccess && !done[dev].load(std::memory_order_acquire)) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kBlockMemory));
+    if (e == cudaSuccess) done[dev].store(true, std::memory_order_release);
+  }
+  return e == cudaSuccess ? FSSIM_OK : fail(FSSIM_ERR_CUDA, cudaGetErrorString(e));
+}
+
+template <typename X, typename Y, int V, bool VEC, bool WARP, int MODE, bool STAGED = true>
+int block_forward(const BlockLaunch& l, const fssim::BlockParams& p, cudaStream_t stream) {
+  static std::atomic<bool> done[64];
+  const auto kernel = fssim::block_norm_forward_kernel<X, Y, V, VEC, WARP, MODE, STAGED>;
+  const int st = block_allow(kernel, done);
+  return st ? st : launch(kernel, l.grid, l.block, l.memory, stream, "block norm forward launch", p);
+}
+template <typename X, typename Y, int V, bool VEC, bool WARP, int MODE, bool STAGED = true>
+int block_backward(const BlockLaunch& l, const fssim::BlockParams& p, cudaStream_t stream) {
+  static std::atomic<bool> done[64];
+  const auto kernel = fssim::block_norm_backward_kernel<X, Y, V, VEC, WARP, MODE, STAGED>;
+  const int st = block_allow(kernel, done);
+  return st ? st : launch(kernel, l.grid, l.block, l.memory, stream, "block norm backward launch", p);
+}
+
+// Which kernels there are: see layout() in block_norm.cu. Kernels of one mode alone for rows of whole
+// vectors, one for all modes elsewhere.
+template <typename X, typename Y, int V, bool WARP>
+int block_forward_mode(const BlockLaunch& l, const fssim::BlockParams& p, cudaStream_t stream) {
+  using namespace fssim;
+  if (l.mode == kBlockBefore) return block_forward<X, Y, V, true, WARP, kBlockBefore>(l, p, stream);
+  if (l.mode == kBlockPlain) return block_forward<X, Y, V, true, WARP, kBlockPlain>(l, p, stream);
+  return block_forward<X, Y, V, true, WARP, kBlockAfter>(l, p, stream);
+}
+template <typename X, typename Y, int V, bool WARP>
+int block_backward_mode(const BlockLaunch& l, const fssim::BlockParams& p, cudaStream_t stream) {
+  using namespace fssim;
+  if (l.mode == kBlockBefore) return block_backward<X, Y, V, true, WARP, kBlockBefore>(l, p, stream);
+  if (l.mode == kBlockPlain) return block_backward<X, Y, V, true, WARP, kBlockPlain>(l, p, stream);
+  return block_backward<X, Y, V, true, WARP, kBlockAfter>(l, p, stream);
+}
+
+template <typename X, typename Y>
+int block_norm_types(bool backward, const BlockLaunch& l, const fssim::BlockParams& p, cudaStream_t stream) {
+  using fssim::kBlockAfter;
+  if (backward) {
+    if (!l.vec)
+      return l.warp          ? block_backward<X, Y, 1, false, true, kBlockAfter>(l, p, stream)
+             : l.groups == 1 ? block_backward<X, Y, 1, false, false, kBlockAfter>(l, p, stream)
+                             : block_backward<X, Y, 4, false, false, kBlockAfter, false>(l, p, stream);
+    if (l.groups == 4)
+      return l.staged ? block_backward<X, Y, 4, true, false, kBlockAfter>(l, p, stream)
+                      : block_backward<X, Y, 4, true, false, kBlockAfter, false>(l, p, stream);
+    if (l.warp)
+      return l.groups == 1 ? block_backward_mode<X, Y, 1, true>(l, p, stream)
+                           : block_backward_mode<X, Y, 2, true>(l, p, stream);
+    return l.groups == 1 ? block_backward_mode<X, Y, 1, false>(l, p, stream)
+                         : block_backward_mode<X, Y, 2, false>(l, p, stream);
+  }
+  if (!l.vec)
+    return l.warp          ? block_forward<X, Y, 1, false, true, kBlockAfter>(l, p, stream)
+           : l.groups == 1 ? block_forward<X, Y, 1, false, false, kBlockAfter>(l, p, stream)
+                           : block_forward<X, Y, 4, false, false, kBlockAfter, false>(l, p, stream);
+  if (!l.staged) return block_forward<X, Y, 4, true, false, kBlockAfter, false>(l, p, stream);
+  if (l.warp) {
+    switch (l.groups) {
+      case 1: return block_forward_mode<X, Y, 1, true>(l, p, stream);
+      case 3: return block_forward_mode<X, Y, 3, true>(l, p, stream);
+      case 4: return block_forward_mode<X, Y, 4, true>(l, p, stream);
+      default: return block_forward_mode<X, Y, 5, true>(l, p, stream);
+    }
+  }
+  switch (l.groups) {
+    case 1: return block_forward_mode<X, Y, 1, false>(l, p, stream);
+    case 3: return block_forward_mode<X, Y, 3, false>(l, p, stream);
+    default: return block_forward_mode<X, Y, 4, false>(l, p, stream);
+  }
+}
+
+}  // namespace fssim_host

@@ -28,7 +28,9 @@ int launch(void (*k)(KA...), unsigned grid, unsigned block, size_t smem, cudaStr
   const cudaError_t e = cudaLaunchKernelEx(&cfg, k, args...);
   if (e != cudaSuccess) {
     (void)cudaGetLastError();
-    return fail(FSSIM_ERR_CUDA, std::string(what) + ": " + cudaGetErrorString(e));
+    return fail(FSSIM_ERR_CUDA, std::string(what) + ": " + cudaGetErrorString(e) + " (" + std::to_string(grid) +
+                                    " CTAs of " + std::to_string(block) + " threads, " + std::to_string(smem) +
+                                    " bytes of shared memory)");
   }
   return FSSIM_OK;
 }

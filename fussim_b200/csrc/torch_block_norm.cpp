@@ -75,7 +75,7 @@ Result run_forward(const at::Tensor& x, const at::Tensor& branch, const Vectors&
   a.kind = static_cast<int32_t>(set.norm ? set.kind : FSSIM_NORM_NONE);
   a.branch_kind = static_cast<int32_t>(set.branch_kind);
   a.eps = static_cast<float>(set.eps);
-  a.residual_scale = static_cast<float>(set.residual_scale);
+  a.residual_scale = set.residual_scale;
   a.x = x.data_ptr();
   const std::array<int64_t, 3> rows = {a.B, a.T, 2};
   if (branch.defined()) {
@@ -173,7 +173,7 @@ struct BlockNormFn : public torch::autograd::Function<BlockNormFn> {
     set_shape(a, r, out_dtype);
     a.kind = static_cast<int32_t>(ctx->saved_data["kind"].toInt());
     a.branch_kind = static_cast<int32_t>(ctx->saved_data["branch_kind"].toInt());
-    a.residual_scale = static_cast<float>(ctx->saved_data["residual_scale"].toDouble());
+    a.residual_scale = ctx->saved_data["residual_scale"].toDouble();
     const auto at = [](const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
     a.r = at(r);
     a.branch = at(y);

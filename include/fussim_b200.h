@@ -416,7 +416,7 @@ typedef struct fssim_block_norm_forward_args {
   int32_t branch_kind;    /* fssim_norm_kind of N' */
   int64_t B, T, C;        /* C at most 16384 */
   float eps;              /* >= 0, of both norms */
-  float residual_scale;
+  double residual_scale;
   const void* x;
   const void* branch;     /* NULL: r = x, and r is not written */
   void* r;                /* may be x */
@@ -437,7 +437,7 @@ typedef struct fssim_block_norm_backward_args {
   int32_t y_dtype;        /* of branch, dz and dbranch */
   int32_t kind, branch_kind;
   int64_t B, T, C;
-  float residual_scale;
+  double residual_scale;
   const void* r;          /* as the forward returned it (x, without a branch) */
   const void* branch;     /* NULL where there is none */
   const void* dr;

@@ -102,7 +102,7 @@ def test_recording(name):
 
 
 # ---- the C entry points ----
-P, I64, I32, F = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32, ctypes.c_float
+P, I64, I32, F, F64 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32, ctypes.c_float, ctypes.c_double
 
 
 class Channels(ctypes.Structure):
@@ -111,14 +111,14 @@ class Channels(ctypes.Structure):
 
 class ForwardArgs(ctypes.Structure):
     _fields_ = [("x_dtype", I32), ("y_dtype", I32), ("kind", I32), ("branch_kind", I32), ("B", I64), ("T", I64),
-                ("C", I64), ("eps", F), ("residual_scale", F), ("x", P), ("branch", P), ("r", P), ("z", P)] + \
+                ("C", I64), ("eps", F), ("residual_scale", F64), ("x", P), ("branch", P), ("r", P), ("z", P)] + \
         [(k, Channels) for k in ("gate", "weight", "bias", "scale", "shift", "branch_weight", "branch_bias")] + \
         [("stats", P), ("branch_stats", P)]
 
 
 class BackwardArgs(ctypes.Structure):
     _fields_ = [("x_dtype", I32), ("y_dtype", I32), ("kind", I32), ("branch_kind", I32), ("B", I64), ("T", I64),
-                ("C", I64), ("residual_scale", F), ("r", P), ("branch", P), ("dr", P), ("dz", P), ("stats", P),
+                ("C", I64), ("residual_scale", F64), ("r", P), ("branch", P), ("dr", P), ("dz", P), ("stats", P),
                 ("branch_stats", P)] + \
         [(k, Channels) for k in ("gate", "weight", "bias", "scale", "branch_weight", "branch_bias")] + \
         [("dx", P), ("dbranch", P)] + \
@@ -198,7 +198,7 @@ def test_c_null(lib):
 def test_c_workspace(lib):
     f = lambda **kw: lib.fssim_block_norm_backward_workspace_bytes(ctypes.byref(backward(**kw)))  # noqa: E731
     assert f() >= 2 * 32 * 4
-    assert f(dgate=Channels(SOME, 0, 0)) >= 2 * f() - 64
+    assert f(dgate=Channels(SOME, 0, 0)) > f()
     assert f(dweight=Channels()) == 0 and f(B=0) == 0 and f(C=0) == 0
     # sums of bounded numbers of rows: the workspace stays a fraction of the rows themselves
     assert f(T=1 << 24) <= (2 << 24) * 32 * 4 // 16
