@@ -89,10 +89,11 @@ struct Layout {
 };
 
 constexpr int64_t kSmMemory = 216 << 10;  // of an SM's shared memory: for rings and arrays
-constexpr int kMaxStages = 4;
+constexpr int kMaxStages = 2;
 
-// `bytes`: of a stage of the ring, for each number of a row. `arrays`: how many there are.
-Layout layout(const Shape& s, bool backward, int mode, bool per_sample, bool vec, int bytes, int arrays) {
+// `bytes`(groups): of a stage of the ring, for each number of a row. `arrays`: how many there are.
+template <typename Bytes>
+Layout layout(const Shape& s, bool backward, int mode, bool per_sample, bool vec, Bytes bytes, int arrays) {
   Layout l{};
   const int needed = static_cast<int>((s.C + 7) / 8);
   // Rows within a warp where a thread has at most five groups of eight numbers (forward; two
@@ -135,39 +136,48 @@ Layout layout(const Shape& s, bool backward, int mode, bool per_sample, bool vec
     const int resident = block_resident(registers);
     l.B = per_sample ? s.B : 1;
     l.T = per_sample ? s.T : s.B * s.T;
-    l.block = l.threads;
-    if (l.warp) {
-      // fewer warps in a CTA where there are few rows
-      l.block = 128;
-      while (l.block > 32 && l.B * ((l.T * l.threads + l.block - 1) / l.block) < 2 * kSms) l.block /= 2;
-    }
-    const int64_t parts = l.block / l.threads;
-    const int64_t stage = l.vec ? static_cast<int64_t>(l.block) * l.groups * 8 * bytes : 0;
     const int64_t array_bytes = static_cast<int64_t>(arrays) * s.C * sizeof(float);
-    if (stage > fssim_host::kBlockMemory) {  // rows are loaded number by number
+    // As many threads on an SM as its registers and shared memory hold, with the arrays in each CTA and a
+    // row ahead of each thread's own; of these the largest CTAs, which lay arrays down for the most rows.
+    // (8x1024x1152 16-bit forward: CTAs of 256 threads 21.8 us, of 128 27.7; 16x1024x1024 with a 32-bit
+    // residual, where two of 256 do not fit: 70 and 41.)
+    Layout found = l;
+    int64_t most = 0;
+    for (int block = l.warp ? 256 : l.threads; l.warp ? block >= 32 : most == 0; block /= 2) {
+      const int64_t parts = block / l.threads;
+      if (parts < 1) break;
+      const int64_t stage = l.vec ? static_cast<int64_t>(block) * l.groups * 8 * bytes(l.groups) : 0;
+      if (stage > fssim_host::kBlockMemory) {
+        if (l.warp) continue;
+        break;
+      }
+      // (few rows: smaller CTAs, so that all SMs have some)
+      if (l.warp && block > 32 && l.B * ((l.T + parts - 1) / parts) < 2 * kSms) continue;
+      for (int64_t on_sm = std::max(resident / block, 1); on_sm >= 1 && on_sm * block > most; --on_sm) {
+        const int64_t wanted = (kSms * on_sm + l.B - 1) / l.B;
+        // a thread adds at most 256 rows up in FP32
+        const int64_t rounds = std::min<int64_t>((l.T + parts * wanted - 1) / (parts * wanted), 256);
+        const int64_t chunk = rounds * parts, chunks = (l.T + chunk - 1) / chunk;
+        const int64_t crowd = std::min(on_sm, (l.B * chunks + kSms - 1) / kSms);
+        const int64_t room = std::min<int64_t>(kSmMemory / crowd - 2048, fssim_host::kBlockMemory);
+        const int64_t stages = std::min<int64_t>(kMaxStages, rounds + 1), least = std::min<int64_t>(stages, 2);
+        // (kernels that make the arrays again for each row: four groups of a CTA's rows alone)
+        const bool choice = l.groups == 4 && !l.warp, fits = array_bytes + least * stage <= room && (l.vec || !choice);
+        if (!fits && (on_sm > 1 || (l.warp && block > 32))) continue;
+        found.block = block;
+        found.chunk = chunk;
+        found.chunks = chunks;
+        found.staged = fits || !choice;
+        found.stages = stage ? static_cast<int>(std::clamp<int64_t>((room - (found.staged ? array_bytes : 0)) / stage, 1, stages)) : 1;
+        found.memory = static_cast<size_t>(stage * found.stages + (found.staged ? array_bytes : 0));
+        most = on_sm * block;
+      }
+    }
+    if (most == 0) {  // rows are loaded number by number
       l.vec = false;
       continue;
     }
-    // As many CTAs on an SM as leave each room for the arrays and a row ahead of its own.
-    for (int64_t on_sm = std::max(resident / l.block, 1);; --on_sm) {
-      const int64_t wanted = (kSms * on_sm + l.B - 1) / l.B;
-      // a thread adds at most 256 rows up in FP32
-      const int64_t rounds = std::min<int64_t>((l.T + parts * wanted - 1) / (parts * wanted), 256);
-      l.chunk = rounds * parts;
-      l.chunks = (l.T + l.chunk - 1) / l.chunk;
-      const int64_t crowd = std::min(on_sm, (l.B * l.chunks + kSms - 1) / kSms);
-      const int64_t room = std::min<int64_t>(kSmMemory / crowd - 2048, fssim_host::kBlockMemory);
-      const int64_t stages = std::min<int64_t>(kMaxStages, rounds + 1), least = std::min<int64_t>(stages, 2);
-      // (kernels that make the arrays again for each row: four groups of a CTA's rows alone)
-      const bool choice = l.groups == 4 && !l.warp;
-      l.staged = array_bytes + least * stage <= room && (l.vec || !choice);
-      l.stages = stage ? static_cast<int>(std::clamp<int64_t>((room - (l.staged ? array_bytes : 0)) / stage, 1, stages)) : 1;
-      if (l.staged || on_sm == 1) {
-        l.staged = l.staged || !choice;
-        break;
-      }
-    }
-    l.memory = static_cast<size_t>(stage * l.stages + (l.staged ? array_bytes : 0));
+    l = found;
     // (the backward pass adds up in it what rows side by side left)
     if (backward && l.warp) l.memory = std::max<size_t>(l.memory, sizeof(float) * (l.block / 32) * s.C);
     return l;
@@ -239,8 +249,8 @@ int forward(const fssim_block_norm_forward_args* a, cudaStream_t stream) {
                      (a->z && (a->bias.data || a->shift.data) ? 1 << kArrayOffset : 0) |
                      (after && a->branch_weight.data ? 1 << kArrayAfterWeight : 0) |
                      (after && a->branch_bias.data ? 1 << kArrayAfterBias : 0);
-  const Layout l = layout(s, false, !a->branch ? kBlockBefore : after ? kBlockAfter : kBlockPlain, per_sample, vec, bytes,
-                          count_of(arrays));
+  const Layout l = layout(s, false, !a->branch ? kBlockBefore : after ? kBlockAfter : kBlockPlain, per_sample, vec,
+                          [&](int) { return bytes; }, count_of(arrays));
   if ((st = check_grid(l.B * l.chunks))) return st;
   BlockParams p = params(s, l);
   p.arrays = arrays;
@@ -289,7 +299,9 @@ Layout backward_layout(const fssim_block_norm_backward_args& a) {
   for (const void* p : {a.r, a.branch, a.dr, a.dz, static_cast<const void*>(a.dx), static_cast<const void*>(a.dbranch)})
     vec = vec && aligned(p, 16);
   const int x = static_cast<int>(elem_size(s.x_dtype)), y = static_cast<int>(elem_size(s.y_dtype));
-  const int bytes = (a.dz ? x + y : 0) + (a.dr ? x : 0) + (a.branch ? y : 0);
+  // as the kernels lay a stage out: r and dz, and except in those for one norm before a block dr and y
+  const bool before = !a.branch && a.dz && !a.dr;
+  const auto bytes = [&](int groups) { return before && groups < 4 ? x + y : 2 * (x + y); };
   const int mode = !a.branch ? kBlockBefore : a.branch_kind ? kBlockAfter : kBlockPlain;
   return layout(s, true, mode, per_sample, vec, bytes, count_of(backward_arrays(a)));
 }

@@ -124,23 +124,39 @@ struct alignas(16) BlockPacked {
   }
 };
 
-// A thread's place in a row: column (v, i) of its V groups.
-template <bool VEC>
-__device__ __forceinline__ int block_column(int threads, int tid, int v, int i) {
-  return VEC ? (v * threads + tid) * 8 + i : tid + threads * (v * 8 + i);
-}
+// A thread's place in a row: number i of its group v is in column at(v, i). Columns go out to the row's
+// threads in turn by units that are 16 bytes of x: eight numbers of 16 bits, four of 32 (so that
+// the threads' accesses lie side by side); single numbers where rows begin at no vector's boundary.
+template <int UNIT>
+struct BlockColumns {
+  int threads, tid, C;
+  bool full;  // every group has all its numbers
+  __device__ __forceinline__ int at(int v, int i) const {
+    return ((v * 8 + i) / UNIT * threads + tid) * UNIT + i % UNIT;
+  }
+  __device__ __forceinline__ bool inside(int v, int i) const { return at(v, i / UNIT * UNIT) < C; }
+  // Zeros in place of what is past the row's end.
+  __device__ __forceinline__ Eight keep(Eight f, int v) const {
+    if (!full)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[i] = inside(v, i) ? f[i] : 0.f;
+    return f;
+  }
+};
 
 // ---- rows ----
-// The ring: stages x 16-byte vectors x threads. Copies of one row are a group; the last stages - 1
-// groups are on their way while a row is worked on.
+// The ring: stages x warps x units x lanes: a warp copies whole runs of memory, at offsets that are
+// known when compiled. Copies of one row are a group; the last stages - 1 groups are on their way
+// while a row is worked on. What has no number, past a row's end or the last row, is filled with zeros.
 struct BlockRing {
-  unsigned base, bytes;  // this thread's first slot; bytes of a stage
+  unsigned char* memory;  // this warp's part of the first stage
+  unsigned bytes;         // of a stage
   int stages, put = 0, get = 0;
-  __device__ __forceinline__ BlockRing(unsigned char* memory, int vectors, int stages)
-      : base(static_cast<unsigned>(__cvta_generic_to_shared(memory)) + threadIdx.x * 16),
-        bytes(vectors * blockDim.x * 16), stages(stages) {}
-  __device__ __forceinline__ unsigned next(int& at) const {
-    const unsigned slot = base + at * bytes;
+  // `warp`: bytes of a warp's part of a stage
+  __device__ __forceinline__ BlockRing(unsigned char* ring, int warp, int stages)
+      : memory(ring + threadIdx.x / 32 * warp), bytes(warp * (blockDim.x / 32)), stages(stages) {}
+  __device__ __forceinline__ unsigned char* next(int& at) const {
+    unsigned char* slot = memory + at * bytes;
     at = at + 1 == stages ? 0 : at + 1;
     return slot;
   }
@@ -154,42 +170,48 @@ struct BlockRing {
   }
 };
 
-// A thread's numbers of one tensor's row: through the ring, or (rows that begin at no vector's
-// boundary) loaded number by number. Offsets are of the row's first number.
-template <typename T, int V, bool VEC>
+// A thread's numbers of one tensor's row: through the ring, or (single numbers) loaded into registers.
+// Offsets are of the row's first number.
+template <typename T, int V, int UNIT>
 struct BlockRow {
-  static constexpr int kPer = 8 * sizeof(T) / 16;       // 16-byte vectors of a group
-  static constexpr int kVecs = VEC ? V * kPer : 0;
-  T one[VEC ? 1 : V * 8];
+  static constexpr bool kVec = UNIT > 1;
+  static constexpr int kPiece = UNIT * sizeof(T), kPieces = V * 8 / UNIT;  // bytes of a unit, units of a thread
+  static constexpr int kBytes = kVec ? kPieces * kPiece * 32 : 0;          // of a warp's part of a stage
+  T one[kVec ? 1 : V * 8];
 
-  static __device__ __forceinline__ void copy(unsigned slot, const void* from, int64_t offset, int C, int threads,
-                                              int tid) {
-    const T* at = static_cast<const T*>(from) + offset + tid * 8;
+  static __device__ __forceinline__ void copy(unsigned char* slot, const void* from, int64_t offset,
+                                              const BlockColumns<UNIT>& c, bool active) {
+    const unsigned to = static_cast<unsigned>(__cvta_generic_to_shared(slot)) + threadIdx.x % 32 * kPiece;
+    const T* row = static_cast<const T*>(from) + offset;
 #pragma unroll
-    for (int v = 0; v < V; ++v)
-      if (block_column<true>(threads, tid, v, 0) < C)
-#pragma unroll
-        for (int k = 0; k < kPer; ++k)
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(slot + (v * kPer + k) * blockDim.x * 16),
-                       "l"(reinterpret_cast<const uint4*>(at + v * threads * 8) + k) : "memory");
-  }
-  __device__ __forceinline__ void load(const void* from, int64_t offset, int C, int threads, int tid, bool active) {
-#pragma unroll
-    for (int i = 0; i < V * 8; ++i) {
-      const int at = block_column<false>(threads, tid, 0, i);
-      one[i] = active && at < C ? static_cast<const T*>(from)[offset + at] : run_narrow<T>(0.f);
+    for (int k = 0; k < kPieces; ++k) {
+      const int at = c.at(0, k * UNIT);
+      const bool ok = active && (c.full || at < c.C);
+      const T* src = ok ? row + at : static_cast<const T*>(from);
+      if constexpr (kPiece == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + k * 512), "l"(src), "r"(ok ? 16 : 0)
+                     : "memory");
+      else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(to + k * 256), "l"(src), "r"(ok ? 8 : 0)
+                     : "memory");
     }
   }
-  // Group v; `ok`: it has numbers (else zeros).
-  __device__ __forceinline__ Eight get(unsigned slot, int v, bool ok) const {
-    if constexpr (VEC) {
-      uint4 raw[kPer] = {};
-      if (ok)
+  __device__ __forceinline__ void load(const void* from, int64_t offset, const BlockColumns<UNIT>& c, bool active) {
 #pragma unroll
-        for (int k = 0; k < kPer; ++k)
-          asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
-                       : "=r"(raw[k].x), "=r"(raw[k].y), "=r"(raw[k].z), "=r"(raw[k].w)
-                       : "r"(slot + (v * kPer + k) * blockDim.x * 16) : "memory");
+    for (int i = 0; i < V * 8; ++i) {
+      const int at = c.at(0, i);
+      one[i] = active && at < c.C ? static_cast<const T*>(from)[offset + at] : run_narrow<T>(0.f);
+    }
+  }
+  // Group v.
+  __device__ __forceinline__ Eight get(const unsigned char* slot, int v) const {
+    if constexpr (kVec) {
+      using Piece = std::conditional_t<kPiece == 16, uint4, uint2>;
+      constexpr int per = 8 / UNIT;
+      alignas(16) Piece raw[per];
+      const Piece* at = reinterpret_cast<const Piece*>(slot) + threadIdx.x % 32;
+#pragma unroll
+      for (int k = 0; k < per; ++k) raw[k] = at[(v * per + k) * 32];
       return reinterpret_cast<const BlockPacked<T>&>(raw).widen();
     } else {
       Eight f;
@@ -200,19 +222,24 @@ struct BlockRow {
   }
 };
 
-template <typename T, bool VEC>
-__device__ __forceinline__ void block_store(void* to, int64_t offset, int C, int threads, int tid, int v,
+// Group v to a row.
+template <typename T, int UNIT>
+__device__ __forceinline__ void block_store(void* to, int64_t offset, const BlockColumns<UNIT>& c, int v,
                                             const BlockPacked<T>& e) {
   T* row = static_cast<T*>(to) + offset;
-  if constexpr (VEC) {
-    uint4* at = reinterpret_cast<uint4*>(row + tid * 8 + v * threads * 8);
 #pragma unroll
-    for (int k = 0; k < static_cast<int>(8 * sizeof(T) / 16); ++k) at[k] = reinterpret_cast<const uint4*>(&e)[k];
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int at = block_column<false>(threads, tid, v, i);
-      if (at < C) row[at] = reinterpret_cast<const T*>(&e)[i];
+  for (int i = 0; i < 8; i += UNIT) {
+    const int at = c.at(v, i);
+    if (!c.full && at >= c.C) continue;
+    if constexpr (UNIT * sizeof(T) == 32) {  // (FP32 sums of eight columns)
+      reinterpret_cast<uint4*>(row + at)[0] = reinterpret_cast<const uint4*>(&e)[0];
+      reinterpret_cast<uint4*>(row + at)[1] = reinterpret_cast<const uint4*>(&e)[1];
+    } else if constexpr (UNIT * sizeof(T) == 16) {
+      *reinterpret_cast<uint4*>(row + at) = reinterpret_cast<const uint4*>(&e)[i / UNIT];
+    } else if constexpr (UNIT > 1) {
+      *reinterpret_cast<uint2*>(row + at) = reinterpret_cast<const uint2*>(&e)[i / UNIT];
+    } else {
+      row[at] = reinterpret_cast<const T*>(&e)[i];
     }
   }
 }
@@ -224,49 +251,54 @@ __device__ __forceinline__ float block_channel(const void* data, int dtype, int6
   return run_widen(static_cast<const __nv_bfloat16*>(data)[at]);
 }
 
-// Eight numbers of a vector from a column on, `step` apart (1 with VEC); `missing` stands for one that
-// is not given.
+// Where eight numbers of a vector are: four `step` apart, and four `jump` behind these.
+struct BlockSpan {
+  int column, step, jump;
+};
+
+// Those numbers; `missing` stands for one that is not given.
 template <bool VEC>
-__device__ __forceinline__ void block_channels(const BlockChannels& ch, int64_t sample, int C, int column, int step,
+__device__ __forceinline__ void block_channels(const BlockChannels& ch, int64_t sample, int C, BlockSpan at,
                                                float missing, float (&f)[8]) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) f[i] = missing;
-  if (!ch.data || column >= C) return;
+  if (!ch.data) return;
   const int64_t base = ch.per_sample ? sample * C : 0;
-  if (VEC && ch.wide) {
-    uint4 raw[2];
-    if (ch.dtype == 0) {
-      const uint4* p = reinterpret_cast<const uint4*>(static_cast<const float*>(ch.data) + base + column);
-      raw[0] = __ldg(p);
-      raw[1] = __ldg(p + 1);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] = reinterpret_cast<const float*>(raw)[i];
+  for (int h = 0; h < 2; ++h) {
+    const int column = at.column + h * at.jump;
+    if (VEC && ch.wide) {
+      if (column >= C) continue;
+      if (ch.dtype == 0) {
+        const float4 raw = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(ch.data) + base + column));
+        f[h * 4] = raw.x, f[h * 4 + 1] = raw.y, f[h * 4 + 2] = raw.z, f[h * 4 + 3] = raw.w;
+      } else {
+        const uint2 raw = __ldg(reinterpret_cast<const uint2*>(static_cast<const __half*>(ch.data) + base + column));
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          f[h * 4 + i] = ch.dtype == 1 ? run_widen(reinterpret_cast<const __half*>(&raw)[i])
+                                       : run_widen(reinterpret_cast<const __nv_bfloat16*>(&raw)[i]);
+      }
     } else {
-      raw[0] = __ldg(reinterpret_cast<const uint4*>(static_cast<const __half*>(ch.data) + base + column));
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        f[i] = ch.dtype == 1 ? run_widen(reinterpret_cast<const __half*>(raw)[i])
-                             : run_widen(reinterpret_cast<const __nv_bfloat16*>(raw)[i]);
+      for (int i = 0; i < 4; ++i)
+        if (column + i * at.step < C) f[h * 4 + i] = block_channel(ch.data, ch.dtype, base + column + i * at.step);
     }
-    return;
   }
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (column + i * step < C) f[i] = block_channel(ch.data, ch.dtype, base + column + i * step);
 }
 
 // Eight numbers of an array. WIDE: the gate is multiplied by s later, in FP64.
 template <bool VEC, bool WIDE, bool BACKWARD>
-__device__ __noinline__ void block_array(const BlockParams& p, int64_t sample, int array, int column, int step,
+__device__ __noinline__ void block_array(const BlockParams& p, int64_t sample, int array, BlockSpan at,
                                          float (&f)[8]) {
   float w[8], t[8];
   const int C = p.C;
   switch (array) {
     case kArrayGate:
-      block_channels<VEC>(p.gate, sample, C, column, step, 1.f, f);
+      block_channels<VEC>(p.gate, sample, C, at, 1.f, f);
       if (WIDE) return;
       if (BACKWARD) {
-        block_channels<VEC>(p.after_weight, sample, C, column, step, 1.f, w);
+        block_channels<VEC>(p.after_weight, sample, C, at, 1.f, w);
 #pragma unroll
         for (int i = 0; i < 8; ++i) f[i] = static_cast<float>(p.s) * f[i] * w[i];
         return;
@@ -275,57 +307,60 @@ __device__ __noinline__ void block_array(const BlockParams& p, int64_t sample, i
       for (int i = 0; i < 8; ++i) f[i] *= static_cast<float>(p.s);
       return;
     case kArrayFactor:
-      block_channels<VEC>(p.weight, sample, C, column, step, 1.f, w);
-      block_channels<VEC>(p.scale, sample, C, column, step, 0.f, f);
+      block_channels<VEC>(p.weight, sample, C, at, 1.f, w);
+      block_channels<VEC>(p.scale, sample, C, at, 0.f, f);
 #pragma unroll
       for (int i = 0; i < 8; ++i) f[i] = w[i] * (1.f + f[i]);
       return;
     case kArrayOffset:
-      block_channels<VEC>(p.bias, sample, C, column, step, 0.f, w);
-      block_channels<VEC>(p.scale, sample, C, column, step, 0.f, t);
-      block_channels<VEC>(p.shift, sample, C, column, step, 0.f, f);
+      block_channels<VEC>(p.bias, sample, C, at, 0.f, w);
+      block_channels<VEC>(p.scale, sample, C, at, 0.f, t);
+      block_channels<VEC>(p.shift, sample, C, at, 0.f, f);
 #pragma unroll
       for (int i = 0; i < 8; ++i) f[i] = fmaf(w[i], 1.f + t[i], f[i]);
       return;
-    case kArrayAfterWeight: block_channels<VEC>(p.after_weight, sample, C, column, step, 1.f, f); return;
-    default: block_channels<VEC>(p.after_bias, sample, C, column, step, 0.f, f); return;
+    case kArrayAfterWeight: block_channels<VEC>(p.after_weight, sample, C, at, 1.f, f); return;
+    default: block_channels<VEC>(p.after_bias, sample, C, at, 0.f, f); return;
   }
 }
 
 // The arrays of a sample lie in shared memory (those that are not constant, one behind the other;
-// STAGED), or are made again for each row where that is too small. With VEC the first halves of all
-// groups lie before the second halves: lanes read consecutive vectors.
+// STAGED), or are made again for each row where that is too small. Of units of eight numbers the first
+// halves lie before all second halves: lanes read consecutive vectors.
 __device__ __forceinline__ float* block_place_of(const BlockParams& p, float* memory, int array) {
   return memory + __popc(p.arrays & ((1 << array) - 1)) * p.C;
 }
 
 // Lays the arrays there. All of a group's vectors are asked for before any is used: a CTA waits for
 // memory once for each of its threads' groups, not for each vector.
-template <bool VEC, bool WIDE, bool BACKWARD>
+template <int UNIT, bool WIDE, bool BACKWARD>
 __device__ __noinline__ void block_stage(const BlockParams& p, int64_t sample, float* memory) {
   const int C = p.C, groups = (C + 7) / 8;
   const auto put = [&](int array, int g, const float(&f)[8]) {
     if (!(p.arrays >> array & 1)) return;
     float* at = block_place_of(p, memory, array);
-    if constexpr (VEC) {
-      reinterpret_cast<float4*>(at)[g] = make_float4(f[0], f[1], f[2], f[3]);
-      reinterpret_cast<float4*>(at)[groups + g] = make_float4(f[4], f[5], f[6], f[7]);
+    if constexpr (UNIT > 1) {
+      const int first = UNIT == 8 ? g : 2 * g, second = UNIT == 8 ? groups + g : 2 * g + 1;
+      reinterpret_cast<float4*>(at)[first] = make_float4(f[0], f[1], f[2], f[3]);
+      reinterpret_cast<float4*>(at)[second] = make_float4(f[4], f[5], f[6], f[7]);
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i)
         if (g * 8 + i < C) at[g * 8 + i] = f[i];
     }
   };
+  constexpr bool VEC = UNIT > 1;
   for (int g = threadIdx.x; g < groups; g += blockDim.x) {
+    const BlockSpan at{g * 8, 1, 4};
     float gate[8], weight[8], bias[8], scale[8], shift[8], after_weight[8], after_bias[8];
-    block_channels<VEC>(p.gate, sample, C, g * 8, 1, 1.f, gate);
-    block_channels<VEC>(p.weight, sample, C, g * 8, 1, 1.f, weight);
-    block_channels<VEC>(p.scale, sample, C, g * 8, 1, 0.f, scale);
-    block_channels<VEC>(p.after_weight, sample, C, g * 8, 1, 1.f, after_weight);
+    block_channels<VEC>(p.gate, sample, C, at, 1.f, gate);
+    block_channels<VEC>(p.weight, sample, C, at, 1.f, weight);
+    block_channels<VEC>(p.scale, sample, C, at, 0.f, scale);
+    block_channels<VEC>(p.after_weight, sample, C, at, 1.f, after_weight);
     if constexpr (!BACKWARD) {
-      block_channels<VEC>(p.bias, sample, C, g * 8, 1, 0.f, bias);
-      block_channels<VEC>(p.shift, sample, C, g * 8, 1, 0.f, shift);
-      block_channels<VEC>(p.after_bias, sample, C, g * 8, 1, 0.f, after_bias);
+      block_channels<VEC>(p.bias, sample, C, at, 0.f, bias);
+      block_channels<VEC>(p.shift, sample, C, at, 0.f, shift);
+      block_channels<VEC>(p.after_bias, sample, C, at, 0.f, after_bias);
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -346,36 +381,37 @@ __device__ __noinline__ void block_stage(const BlockParams& p, int64_t sample, f
   __syncthreads();
 }
 
-template <bool VEC, bool WIDE, bool BACKWARD, bool STAGED>
+template <int UNIT, bool WIDE, bool BACKWARD, bool STAGED>
 struct BlockArrays {
   const BlockParams& p;
   float* memory;
   int64_t sample;
 
   __device__ __forceinline__ void stage() const {
-    if constexpr (STAGED) block_stage<VEC, WIDE, BACKWARD>(p, sample, memory);
+    if constexpr (STAGED) block_stage<UNIT, WIDE, BACKWARD>(p, sample, memory);
   }
-  // Group v of a thread that has numbers there.
-  __device__ __forceinline__ Eight get(int array, int tid, int v, float constant) const {
+  // Group v of a thread.
+  __device__ __forceinline__ Eight get(int array, const BlockColumns<UNIT>& c, int v, float constant) const {
     if (!(p.arrays >> array & 1)) return eight(constant);
     Eight f;
     if constexpr (STAGED) {
       const float* at = block_place_of(p, memory, array);
-      if constexpr (VEC) {
-        const float4* q = reinterpret_cast<const float4*>(at) + v * p.threads + tid;
-        const float4 a = q[0], b = q[p.C / 8];
+      if constexpr (UNIT > 1) {
+        // (a thread without numbers there reads others' and has no use for them)
+        const float4* q = reinterpret_cast<const float4*>(at);
+        const int first = UNIT == 8 ? v * c.threads + c.tid : 2 * v * c.threads + c.tid, second = first + c.threads;
+        const int last = c.C / UNIT - 1;
+        const float4 a = q[min(first, last)], b = UNIT == 8 ? q[c.C / 8 + min(first, last)] : q[min(second, last)];
         f.p[0] = make_float2(a.x, a.y), f.p[1] = make_float2(a.z, a.w);
         f.p[2] = make_float2(b.x, b.y), f.p[3] = make_float2(b.z, b.w);
       } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int c = block_column<false>(p.threads, tid, v, i);
-          f[i] = c < p.C ? at[c] : 0.f;
-        }
+        for (int i = 0; i < 8; ++i) f[i] = c.inside(v, i) ? at[c.at(v, i)] : 0.f;
       }
     } else {
       float t[8];  // (of its own: what is passed to a function lies in local memory)
-      block_array<VEC, WIDE, BACKWARD>(p, sample, array, block_column<VEC>(p.threads, tid, v, 0), VEC ? 1 : p.threads, t);
+      block_array<(UNIT > 1), WIDE, BACKWARD>(
+          p, sample, array, {c.at(v, 0), UNIT > 1 ? 1 : c.threads, c.at(v, 4) - c.at(v, 0)}, t);
 #pragma unroll
       for (int i = 0; i < 8; ++i) f[i] = t[i];
     }
@@ -430,105 +466,91 @@ struct BlockTeam {
   }
 };
 
-template <bool VEC, bool WARP>
-__device__ __forceinline__ bool block_inside(const BlockTeam<WARP>& team, int C, int tid, int v, int i) {
-  return block_column<VEC>(team.threads, tid, v, VEC ? 0 : i) < C;
+// (mean, sum of squares) of a row times `by` (1 unless SCALED), of which a thread has the groups f (zero
+// past its end). The mean is taken of the distances from a number of the row, and the squares of those
+// from the mean, warp by warp and then between the warps' means: rows of equal numbers have exactly
+// their own mean.
+template <bool SCALED, int V, int UNIT, bool WARP>
+__device__ __forceinline__ float2 block_moments(BlockTeam<WARP>& team, const Eight (&f)[V], int kind, float by,
+                                                const BlockColumns<UNIT>& c) {
+  const auto at = [&](int v, int i) { return SCALED ? __fmul2_rn(f[v].p[i], twice(by)) : f[v].p[i]; };
+  if (kind == kBlockRms) {
+    float2 q[2] = {};
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) q[i & 1] = __ffma2_rn(at(v, i), at(v, i), q[i & 1]);
+    q[0] = __fadd2_rn(q[0], q[1]);
+    return make_float2(0.f, team.template sum<false>(make_float2(q[0].x + q[0].y, 0.f)).x);
+  }
+  const int lane = threadIdx.x % 32;
+  const float pivot = __shfl_sync(0xffffffffu, at(0, 0).x, WARP ? lane & ~(team.threads - 1) : 0);
+  float2 a = {}, q = {};
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    Eight d;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) d.p[i] = __fadd2_rn(at(v, i), twice(-pivot));
+    d = c.keep(d, v);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) a = __fadd2_rn(a, d.p[i]);
+  }
+  float sum = a.x + a.y;
+  team.across(sum, WARP ? team.threads >> 1 : 16);
+  const float shift = sum * team.inv;
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    Eight d;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) d.p[i] = __fadd2_rn(__fadd2_rn(at(v, i), twice(-pivot)), twice(-shift));
+    d = c.keep(d, v);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) q = __ffma2_rn(d.p[i], d.p[i], q);
+  }
+  float squares = q.x + q.y;
+  team.across(squares, WARP ? team.threads >> 1 : 16);
+  float mean = pivot + shift;
+  if constexpr (!WARP) {
+    // the warps' (mean, sum of squares, numbers)
+    float4* slots = team.template next<float4>();
+    if (lane == 0) slots[threadIdx.x / 32] = make_float4(mean, squares, team.count, 0.f);
+    __syncthreads();
+    const float first = slots[0].x;
+    const float4 mine = lane < team.warps ? slots[lane] : make_float4(first, 0.f, 0.f, 0.f);
+    float away = mine.z * (mine.x - first);
+    team.across(away, team.span >> 1);
+    mean = first + __shfl_sync(0xffffffffu, away, 0) / c.C;
+    const float d = mine.x - mean;
+    squares = fmaf(mine.z * d, d, mine.y);
+    team.across(squares, team.span >> 1);
+    squares = __shfl_sync(0xffffffffu, squares, 0);
+  }
+  return make_float2(mean, squares);
 }
 
-// (mean, rstd) of a row, of which a thread has the groups f (zero past its end). The mean is taken of the
-// distances from a number of the row, and the squares of those from the mean, warp by warp and then
-// between the warps' means: rows of equal numbers have exactly their own mean.
-// FP32's range is that of the numbers, not of their squares: where their sum leaves it (or its
-// accurate part, and eps does not cover that), it is taken again of numbers scaled by a power of two.
-template <int V, bool VEC, bool WARP>
-__device__ __forceinline__ float2 block_stats(BlockTeam<WARP>& team, Eight (&f)[V], int kind, float eps, int C, int tid) {
-  float by = 1.f;
-  for (;;) {
-    float mean = 0.f, squares = 0.f;
-    if (kind == kBlockRms) {
-      float2 q[2] = {};
-#pragma unroll
-      for (int v = 0; v < V; ++v)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) q[i & 1] = __ffma2_rn(f[v].p[i], f[v].p[i], q[i & 1]);
-      q[0] = __fadd2_rn(q[0], q[1]);
-      squares = team.template sum<false>(make_float2(q[0].x + q[0].y, 0.f)).x;
-    } else {
-      const int lane = threadIdx.x % 32;
-      const float pivot = __shfl_sync(0xffffffffu, f[0][0], WARP ? lane & ~(team.threads - 1) : 0);
-      float2 a = {}, q = {};
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        if constexpr (VEC) {
-          if (block_inside<true>(team, C, tid, v, 0))
-#pragma unroll
-            for (int i = 0; i < 4; ++i) a = __fadd2_rn(a, __fadd2_rn(f[v].p[i], twice(-pivot)));
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (block_inside<false>(team, C, tid, v, i)) a.x += f[v][i] - pivot;
-        }
-      }
-      float sum = a.x + a.y;
-      team.across(sum, WARP ? team.threads >> 1 : 16);
-      const float shift = sum * team.inv;
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        if constexpr (VEC) {
-          if (block_inside<true>(team, C, tid, v, 0))
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float2 d = __fadd2_rn(__fadd2_rn(f[v].p[i], twice(-pivot)), twice(-shift));
-              q = __ffma2_rn(d, d, q);
-            }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (block_inside<false>(team, C, tid, v, i)) {
-              const float d = (f[v][i] - pivot) - shift;
-              q.x = fmaf(d, d, q.x);
-            }
-        }
-      }
-      squares = q.x + q.y;
-      team.across(squares, WARP ? team.threads >> 1 : 16);
-      mean = pivot + shift;
-      if constexpr (!WARP) {
-        // the warps' (mean, sum of squares, numbers)
-        float4* at = team.template next<float4>();
-        if (lane == 0) at[threadIdx.x / 32] = make_float4(mean, squares, team.count, 0.f);
-        __syncthreads();
-        const float first = at[0].x;
-        const float4 mine = lane < team.warps ? at[lane] : make_float4(first, 0.f, 0.f, 0.f);
-        float away = mine.z * (mine.x - first);
-        team.across(away, team.span >> 1);
-        mean = first + __shfl_sync(0xffffffffu, away, 0) / C;
-        const float d = mine.x - mean;
-        squares = fmaf(mine.z * d, d, mine.y);
-        team.across(squares, team.span >> 1);
-        squares = __shfl_sync(0xffffffffu, squares, 0);
-      }
-    }
-    const bool large = squares > 0x1p120f, small = squares < 0x1p-80f && eps < 0x1p-90f;
-    const bool again = by == 1.f && (large || small);
-    if (WARP ? !__any_sync(0xffffffffu, again) : !again) {
-      if (WARP ? __any_sync(0xffffffffu, by != 1.f) : by != 1.f) {
-#pragma unroll
-        for (int v = 0; v < V; ++v) f[v] = pairs([&](float2 a) { return make_float2(a.x / by, a.y / by); }, f[v]);
-      }
-      return make_float2(mean / by, by * rsqrtf(squares * (1.f / C) + eps * by * by));
-    }
-    by = large ? 0x1p-70f : small ? 0x1p70f : by;
-#pragma unroll
-    for (int v = 0; v < V; ++v) f[v] = pairs([&](float2 a) { return __fmul2_rn(a, twice(by)); }, f[v]);
+// (mean, rstd) of a row. FP32's range is that of the numbers, not of their squares: where their sum
+// leaves it (or its accurate part, and eps does not cover that), it is taken again of numbers
+// scaled by a power of two.
+template <int V, int UNIT, bool WARP>
+__device__ __forceinline__ float2 block_stats(BlockTeam<WARP>& team, const Eight (&f)[V], int kind, float eps,
+                                              const BlockColumns<UNIT>& c) {
+  const float2 m = block_moments<false, V, UNIT, WARP>(team, f, kind, 1.f, c);
+  const bool large = m.y > 0x1p120f, again = large || (m.y < 0x1p-80f && eps < 0x1p-90f);
+  const float inv = 1.f / c.C;
+  if (WARP ? __any_sync(0xffffffffu, again) : again) {
+    const float by = !again ? 1.f : large ? 0x1p-70f : 0x1p70f;
+    const float2 scaled = block_moments<true, V, UNIT, WARP>(team, f, kind, by, c);
+    // (rows beside one that needs this keep their own)
+    if (again) return make_float2(scaled.x / by, by * rsqrtf(scaled.y * inv + eps * by * by));
   }
+  return make_float2(m.x, rsqrtf(m.y * inv + eps));
 }
 
 // The same in FP64, in one pass over the distances from a number of the row (from zero in the "rms"
 // kind): these and their squares are exact, or nearly so, of 16-bit numbers.
-template <int V, bool VEC, bool WARP>
+template <int V, int UNIT, bool WARP>
 __device__ __forceinline__ double2 block_stats_wide(BlockTeam<WARP>& team, const Eight (&f)[V], int kind, float eps,
-                                                    int C, double inv, int tid) {
+                                                    double inv, const BlockColumns<UNIT>& c) {
   const int lane = threadIdx.x % 32;
   double pivot = 0.0;
   if (kind == kBlockLayer) {
@@ -546,7 +568,7 @@ __device__ __forceinline__ double2 block_stats_wide(BlockTeam<WARP>& team, const
   for (int v = 0; v < V; ++v)
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      if (block_inside<VEC>(team, C, tid, v, i)) {
+      if (c.full || c.inside(v, i)) {
         const double d = static_cast<double>(f[v][i]) - pivot;
         sums.x += d;
         sums.y = fma(d, d, sums.y);
@@ -576,14 +598,14 @@ __device__ __forceinline__ BlockPlace block_place(const BlockParams& p) {
   return b;
 }
 
-template <int V, bool VEC, bool WARP>
-__device__ __forceinline__ BlockTeam<WARP> block_team(const BlockParams& p, int tid, double2* slots) {
+template <int V, int UNIT, bool WARP>
+__device__ __forceinline__ BlockTeam<WARP> block_team(const BlockParams& p, const BlockColumns<UNIT>& c, double2* slots) {
   BlockTeam<WARP> team{p.threads, p.threads / 32, 1, slots, static_cast<float>(p.C), 1.f / p.C};
   if constexpr (!WARP) {
     while (team.span < team.warps) team.span *= 2;
     float n = 0.f;
 #pragma unroll
-    for (int i = 0; i < V * 8; ++i) n += block_column<VEC>(p.threads, tid, i / 8, i % 8) < p.C ? 1.f : 0.f;
+    for (int i = 0; i < V * 8; ++i) n += c.inside(i / 8, i % 8) ? 1.f : 0.f;
     team.across(n, 16);
     team.count = n;
     team.inv = 1.f / n;
@@ -592,11 +614,11 @@ __device__ __forceinline__ BlockTeam<WARP> block_team(const BlockParams& p, int 
 }
 
 // Registers, and with them how many threads an SM holds.
-constexpr int block_forward_registers(int v, int mode) { return mode == kBlockAfter ? 128 : v >= 4 ? 96 : 80; }
+constexpr int block_forward_registers(int v, int mode) { return mode == kBlockAfter || v > 4 ? 128 : v > 3 ? 104 : 88; }
 constexpr int block_backward_registers(int v) { return v > 2 ? 128 : 168; }
 constexpr int block_resident(int registers) { return 65536 / registers / 32 * 32; }
 
-template <typename X, typename Y, int V, bool VEC, bool WARP, int MODE, bool STAGED>
+template <typename X, typename Y, int V, int UNIT, bool WARP, int MODE, bool STAGED>
 __global__ void __maxnreg__(block_forward_registers(V, MODE)) block_norm_forward_kernel(const __grid_constant__ BlockParams p) {
   extern __shared__ __align__(16) unsigned char block_memory[];
   __shared__ double2 slots[2 * 16];
@@ -605,71 +627,72 @@ __global__ void __maxnreg__(block_forward_registers(V, MODE)) block_norm_forward
   // 16-bit results of a normalised branch are formed in FP64, and so rounded once in all but name
   constexpr bool kWide = MODE == kBlockAfter && sizeof(X) == 2;
   const BlockPlace b = block_place<WARP>(p);
-  const int C = p.C, tid = b.tid, threads = p.threads;
-  BlockTeam<WARP> team = block_team<V, VEC, WARP>(p, tid, slots);
+  constexpr bool kVec = UNIT > 1;
+  const BlockColumns<UNIT> c{p.threads, b.tid, p.C, V * 8 * p.threads == p.C};
+  const int C = p.C;
+  BlockTeam<WARP> team = block_team<V, UNIT, WARP>(p, c, slots);
   const bool branch = MODE == kBlockPlain || (MODE == kBlockAfter && p.y);
   const bool after_norm = MODE == kBlockAfter && p.after_kind;
-  using RowX = BlockRow<X, V, VEC>;
-  using RowY = BlockRow<Y, V, VEC>;
+  using RowX = BlockRow<X, V, UNIT>;
+  using RowY = BlockRow<Y, V, UNIT>;
   RowX row_x;
   RowY row_y;
-  const unsigned at_y = RowX::kVecs * blockDim.x * 16;
-  BlockRing ring(block_memory, RowX::kVecs + (branch ? RowY::kVecs : 0), p.stages);
+  constexpr int at_y = RowX::kBytes;
+  BlockRing ring(block_memory, RowX::kBytes + (branch ? RowY::kBytes : 0), p.stages);
   int64_t ahead = b.row0 + b.part;
   const auto fetch = [&] {
-    if (ahead < b.row1) {
-      const unsigned slot = ring.base + ring.put * ring.bytes;
-      RowX::copy(slot, p.x, ahead * C, C, threads, tid);
-      if (branch) RowY::copy(slot + at_y, p.y, ahead * C, C, threads, tid);
+    unsigned char* slot = ring.next(ring.put);
+    const bool active = ahead < b.row1;
+    if (WARP || active) {
+      RowX::copy(slot, p.x, ahead * C, c, active);
+      if (branch) RowY::copy(slot + at_y, p.y, ahead * C, c, active);
     }
-    ring.put = ring.put + 1 == ring.stages ? 0 : ring.put + 1;
     ring.commit();
     ahead += b.parts;
   };
-  if constexpr (VEC)
+  if constexpr (kVec)
     for (int k = 1; k < p.stages; ++k) fetch();
-  const BlockArrays<VEC, kWide, false, STAGED> arrays{p, reinterpret_cast<float*>(block_memory + (VEC ? p.stages * ring.bytes : 0)),
+  const BlockArrays<UNIT, kWide, false, STAGED> arrays{p, reinterpret_cast<float*>(block_memory + (kVec ? p.stages * ring.bytes : 0)),
                                               b.sample};
   arrays.stage();
   const float s = static_cast<float>(p.s);
   for (int64_t first = b.row0; first < b.row1; first += b.parts) {
     const int64_t row = first + b.part, offset = row * C;
     const bool active = !WARP || row < b.row1;
-    unsigned slot = 0;
-    if constexpr (VEC) {
+    const unsigned char* slot = nullptr;
+    if constexpr (kVec) {
       fetch();
       ring.wait();
       slot = ring.next(ring.get);
     } else {
-      row_x.load(p.x, offset, C, threads, tid, active);
-      if (branch) row_y.load(p.y, offset, C, threads, tid, active);
+      row_x.load(p.x, offset, c, active);
+      if (branch) row_y.load(p.y, offset, c, active);
     }
-    const auto ok = [&](int v) { return active && block_column<VEC>(threads, tid, v, 0) < C; };
     Eight r[V];
     float2 after = make_float2(0.f, 1.f);
     double2 wide = make_double2(0.0, 1.0);
     if (after_norm) {
 #pragma unroll
-      for (int v = 0; v < V; ++v) r[v] = row_y.get(slot + at_y, v, ok(v));
+      for (int v = 0; v < V; ++v) r[v] = row_y.get(slot + at_y, v);
       if constexpr (kWide) {
-        wide = block_stats_wide<V, VEC, WARP>(team, r, p.after_kind, p.eps, C, p.inv, tid);
+        wide = block_stats_wide<V, UNIT, WARP>(team, r, p.after_kind, p.eps, p.inv, c);
         after = make_float2(static_cast<float>(wide.x), static_cast<float>(wide.y));
       } else {
-        after = block_stats<V, VEC, WARP>(team, r, p.after_kind, p.eps, C, tid);
+        after = block_stats<V, UNIT, WARP>(team, r, p.after_kind, p.eps, c);
       }
-      if (p.after_stats && active && tid == 0) p.after_stats[row] = after;
+      if (p.after_stats && active && c.tid == 0) p.after_stats[row] = after;
     }
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      r[v] = row_x.get(slot, v, ok(v));
-      if (!branch || !ok(v)) continue;
-      Eight u = row_y.get(slot + at_y, v, true);
-      const Eight g = arrays.get(kArrayGate, tid, v, kWide ? 1.f : s);
+      r[v] = row_x.get(slot, v);
+      if (!branch) continue;
+      Eight u = row_y.get(slot + at_y, v);
+      const Eight g = arrays.get(kArrayGate, c, v, kWide ? 1.f : s);
       BlockPacked<X> e;
       if constexpr (kWide) {
         X* one = reinterpret_cast<X*>(&e);
         if (after_norm) {
-          const Eight w = arrays.get(kArrayAfterWeight, tid, v, 1.f), o = arrays.get(kArrayAfterBias, tid, v, 0.f);
+          const Eight w = arrays.get(kArrayAfterWeight, c, v, 1.f), o = arrays.get(kArrayAfterBias, c, v, 0.f);
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             const double t = fma((u[i] - wide.x) * wide.y, static_cast<double>(w[i]), static_cast<double>(o[i]));
@@ -682,7 +705,7 @@ __global__ void __maxnreg__(block_forward_registers(V, MODE)) block_norm_forward
         }
       } else {
         if (after_norm) {
-          const Eight w = arrays.get(kArrayAfterWeight, tid, v, 1.f), o = arrays.get(kArrayAfterBias, tid, v, 0.f);
+          const Eight w = arrays.get(kArrayAfterWeight, c, v, 1.f), o = arrays.get(kArrayAfterBias, c, v, 0.f);
           u = pairs([&](float2 a, float2 w2, float2 o2) {
             return __ffma2_rn(__fmul2_rn(__fadd2_rn(a, twice(-after.x)), twice(after.y)), w2, o2);
           }, u, w, o);
@@ -690,68 +713,63 @@ __global__ void __maxnreg__(block_forward_registers(V, MODE)) block_norm_forward
         // (two roundings, as of a product and a sum one after the other)
         e = BlockPacked<X>::of(pairs([](float2 a, float2 g2, float2 x) { return __fadd2_rn(x, __fmul2_rn(g2, a)); }, u, g, r[v]));
       }
-      block_store<X, VEC>(p.r, offset, C, threads, tid, v, e);
-      r[v] = e.widen();  // z is the norm of r as it is held
-      if constexpr (!VEC)
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (block_column<VEC>(threads, tid, v, i) >= C) r[v][i] = 0.f;
+      if (active) block_store<X>(p.r, offset, c, v, e);
+      r[v] = c.keep(e.widen(), v);  // z is the norm of r as it is held
     }
     if (MODE != kBlockBefore && !p.z) continue;
-    const float2 stats = block_stats<V, VEC, WARP>(team, r, p.kind, p.eps, C, tid);
-    if (p.stats && active && tid == 0) p.stats[row] = stats;
+    const float2 stats = block_stats<V, UNIT, WARP>(team, r, p.kind, p.eps, c);
+    if (p.stats && active && c.tid == 0) p.stats[row] = stats;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      if (!ok(v)) continue;
-      const Eight a = arrays.get(kArrayFactor, tid, v, 1.f), o = arrays.get(kArrayOffset, tid, v, 0.f);
+      const Eight a = arrays.get(kArrayFactor, c, v, 1.f), o = arrays.get(kArrayOffset, c, v, 0.f);
       const Eight z = pairs([&](float2 b, float2 a2, float2 o2) {
         return __ffma2_rn(__fmul2_rn(__fadd2_rn(b, twice(-stats.x)), twice(stats.y)), a2, o2);
       }, r[v], a, o);
-      block_store<Y, VEC>(p.z, offset, C, threads, tid, v, BlockPacked<Y>::of(z));
+      if (active) block_store<Y>(p.z, offset, c, v, BlockPacked<Y>::of(z));
     }
   }
 }
 
-template <typename X, typename Y, int V, bool VEC, bool WARP, int MODE, bool STAGED>
+template <typename X, typename Y, int V, int UNIT, bool WARP, int MODE, bool STAGED>
 __global__ void __maxnreg__(block_backward_registers(V)) block_norm_backward_kernel(const __grid_constant__ BlockParams p) {
   extern __shared__ __align__(16) unsigned char block_memory[];
   __shared__ double2 slots[2 * 16];
   grid_dependency_wait();
   grid_launch_dependents();
   const BlockPlace b = block_place<WARP>(p);
-  const int C = p.C, tid = b.tid, threads = p.threads;
-  BlockTeam<WARP> team = block_team<V, VEC, WARP>(p, tid, slots);
+  constexpr bool kVec = UNIT > 1;
+  const BlockColumns<UNIT> c{p.threads, b.tid, p.C, V * 8 * p.threads == p.C};
+  const int C = p.C;
+  BlockTeam<WARP> team = block_team<V, UNIT, WARP>(p, c, slots);
   const bool branch = MODE == kBlockPlain || (MODE == kBlockAfter && p.y);
   const bool after_norm = MODE == kBlockAfter && p.after_kind;
   const bool has_dr = MODE != kBlockBefore && p.dr, has_dz = MODE == kBlockBefore || p.dz;
-  using RowX = BlockRow<X, V, VEC>;
-  using RowY = BlockRow<Y, V, VEC>;
+  using RowX = BlockRow<X, V, UNIT>;
+  using RowY = BlockRow<Y, V, UNIT>;
   RowX row_r, row_dr;
   RowY row_y, row_dz;
-  // places in a stage: r, dz, dr, y
-  const unsigned step = blockDim.x * 16, at_dz = RowX::kVecs * step;
-  const unsigned at_dr = has_dz ? at_dz + RowY::kVecs * step : 0;
-  const unsigned at_y = at_dr + (has_dr ? RowX::kVecs * step : 0);
-  BlockRing ring(block_memory, at_y / step + (branch ? RowY::kVecs : 0), p.stages);
+  // places in a warp's part of a stage: r, dz, dr, y
+  constexpr int at_dz = RowX::kBytes, at_dr = at_dz + RowY::kBytes, at_y = at_dr + (MODE == kBlockBefore ? 0 : RowX::kBytes);
+  BlockRing ring(block_memory, at_y + (MODE == kBlockBefore ? 0 : RowY::kBytes), p.stages);
   int64_t ahead = b.row0 + b.part;
   const auto fetch = [&] {
-    if (ahead < b.row1) {
-      const unsigned slot = ring.base + ring.put * ring.bytes;
+    unsigned char* slot = ring.next(ring.put);
+    const bool active = ahead < b.row1;
+    if (WARP || active) {
       const int64_t offset = ahead * C;
       if (has_dz) {
-        RowX::copy(slot, p.r, offset, C, threads, tid);
-        RowY::copy(slot + at_dz, p.dz, offset, C, threads, tid);
+        RowX::copy(slot, p.r, offset, c, active);
+        RowY::copy(slot + at_dz, p.dz, offset, c, active);
       }
-      if (has_dr) RowX::copy(slot + at_dr, p.dr, offset, C, threads, tid);
-      if (branch) RowY::copy(slot + at_y, p.y, offset, C, threads, tid);
+      if (has_dr) RowX::copy(slot + at_dr, p.dr, offset, c, active);
+      if (branch) RowY::copy(slot + at_y, p.y, offset, c, active);
     }
-    ring.put = ring.put + 1 == ring.stages ? 0 : ring.put + 1;
     ring.commit();
     ahead += b.parts;
   };
-  if constexpr (VEC)
+  if constexpr (kVec)
     for (int k = 1; k < p.stages; ++k) fetch();
-  const BlockArrays<VEC, false, true, STAGED> arrays{p, reinterpret_cast<float*>(block_memory + (VEC ? p.stages * ring.bytes : 0)),
+  const BlockArrays<UNIT, false, true, STAGED> arrays{p, reinterpret_cast<float*>(block_memory + (kVec ? p.stages * ring.bytes : 0)),
                                              b.sample};
   arrays.stage();
   constexpr int kSums = MODE == kBlockBefore ? 2 : MODE == kBlockPlain ? 3 : 4;
@@ -773,25 +791,24 @@ __global__ void __maxnreg__(block_backward_registers(V)) block_norm_backward_ker
     const bool active = !WARP || row < b.row1;
     const float2 s1 = next1, s2 = next2;
     stats_of(row + b.parts);
-    unsigned slot = 0;
-    if constexpr (VEC) {
+    const unsigned char* slot = nullptr;
+    if constexpr (kVec) {
       fetch();
       ring.wait();
       slot = ring.next(ring.get);
     } else {
       if (has_dz) {
-        row_r.load(p.r, offset, C, threads, tid, active);
-        row_dz.load(p.dz, offset, C, threads, tid, active);
+        row_r.load(p.r, offset, c, active);
+        row_dz.load(p.dz, offset, c, active);
       }
-      if (has_dr) row_dr.load(p.dr, offset, C, threads, tid, active);
-      if (branch) row_y.load(p.y, offset, C, threads, tid, active);
+      if (has_dr) row_dr.load(p.dr, offset, c, active);
+      if (branch) row_y.load(p.y, offset, c, active);
     }
-    const auto ok = [&](int v) { return active && block_column<VEC>(threads, tid, v, 0) < C; };
     const auto get_rhat = [&](int v) {
-      return pairs([&](float2 a) { return __fmul2_rn(__fadd2_rn(a, twice(-s1.x)), twice(s1.y)); }, row_r.get(slot, v, true));
+      return pairs([&](float2 a) { return __fmul2_rn(__fadd2_rn(a, twice(-s1.x)), twice(s1.y)); }, row_r.get(slot, v));
     };
     const auto get_yhat = [&](int v) {
-      const Eight y = row_y.get(slot + at_y, v, true);
+      const Eight y = row_y.get(slot + at_y, v);
       return after_norm ? pairs([&](float2 a) { return __fmul2_rn(__fadd2_rn(a, twice(-s2.x)), twice(s2.y)); }, y) : y;
     };
     const auto times = [](float2 a, float2 b2) { return __fmul2_rn(a, b2); };
@@ -800,9 +817,9 @@ __global__ void __maxnreg__(block_backward_registers(V)) block_norm_backward_ker
       float2 mean[2] = {};
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        if (!ok(v)) continue;
-        const Eight h = get_rhat(v), dz = row_dz.get(slot + at_dz, v, true);
-        const Eight a = pairs(times, dz, arrays.get(kArrayFactor, tid, v, 1.f));
+        // (past the row's end dz is zero, and so are its products)
+        const Eight h = get_rhat(v), dz = row_dz.get(slot + at_dz, v);
+        const Eight a = pairs(times, dz, arrays.get(kArrayFactor, c, v, 1.f));
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           sums[0][v].p[i] = __fadd2_rn(sums[0][v].p[i], dz.p[i]);
@@ -819,28 +836,24 @@ __global__ void __maxnreg__(block_backward_registers(V)) block_norm_backward_ker
     float2 mean[2] = {};
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      if (!ok(v)) continue;
-      Eight d = has_dr ? row_dr.get(slot + at_dr, v, true) : eight(0.f);
+      Eight d = has_dr ? row_dr.get(slot + at_dr, v) : eight(0.f);
       if (has_dz) {
         const Eight h = get_rhat(v);
-        const Eight a = pairs(times, row_dz.get(slot + at_dz, v, true), arrays.get(kArrayFactor, tid, v, 1.f));
+        const Eight a = pairs(times, row_dz.get(slot + at_dz, v), arrays.get(kArrayFactor, c, v, 1.f));
         d = pairs([&](float2 d2, float2 a2, float2 h2) {
           return __ffma2_rn(twice(s1.y), __ffma2_rn(h2, twice(-m2), __fadd2_rn(a2, twice(-m1))), d2);
         }, d, a, h);
       }
-      if (p.dx) block_store<X, VEC>(p.dx, offset, C, threads, tid, v, BlockPacked<X>::of(d));
+      if (p.dx && active) block_store<X>(p.dx, offset, c, v, BlockPacked<X>::of(d));
       if (!branch) continue;
-      if constexpr (!VEC)
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (block_column<VEC>(threads, tid, v, i) >= C) d[i] = 0.f;
+      d = c.keep(d, v);
       const Eight y = get_yhat(v);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         if constexpr (kSums > 2) sums[2][v].p[i] = __ffma2_rn(d.p[i], y.p[i], sums[2][v].p[i]);
         if constexpr (kSums > 3) sums[3][v].p[i] = __fadd2_rn(sums[3][v].p[i], d.p[i]);
       }
-      d = pairs(times, d, arrays.get(kArrayGate, tid, v, s));
+      d = pairs(times, d, arrays.get(kArrayGate, c, v, s));
       if (after_norm) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -848,8 +861,8 @@ __global__ void __maxnreg__(block_backward_registers(V)) block_norm_backward_ker
           mean[1] = __ffma2_rn(d.p[i], y.p[i], mean[1]);
         }
         if constexpr (MODE == kBlockAfter) e[v] = d;
-      } else if (p.dy) {
-        block_store<Y, VEC>(p.dy, offset, C, threads, tid, v, BlockPacked<Y>::of(d));
+      } else if (p.dy && active) {
+        block_store<Y>(p.dy, offset, c, v, BlockPacked<Y>::of(d));
       }
     }
     if constexpr (MODE == kBlockAfter) {
@@ -859,11 +872,10 @@ __global__ void __maxnreg__(block_backward_registers(V)) block_norm_backward_ker
       m2 = m.y * inv;
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        if (!ok(v)) continue;
         const Eight dy = pairs([&](float2 e2, float2 y2) {
           return __fmul2_rn(twice(s2.y), __ffma2_rn(y2, twice(-m2), __fadd2_rn(e2, twice(-m1))));
         }, e[v], get_yhat(v));
-        block_store<Y, VEC>(p.dy, offset, C, threads, tid, v, BlockPacked<Y>::of(dy));
+        if (active) block_store<Y>(p.dy, offset, c, v, BlockPacked<Y>::of(dy));
       }
     }
   }
@@ -874,10 +886,7 @@ __global__ void __maxnreg__(block_backward_registers(V)) block_norm_backward_ker
     for (int k = 0; k < kSums; ++k)
       if (k < p.sums)
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-          if (block_column<VEC>(threads, tid, v, 0) < C)
-            block_store<float, VEC>(mine, k * C, C, threads, tid, v, BlockPacked<float>::of(sums[k][v]));
-        }
+        for (int v = 0; v < V; ++v) block_store<float>(mine, k * C, c, v, BlockPacked<float>::of(sums[k][v]));
   } else {
     // rows side by side: their sums are added up over the warp's parts and the warps
     float* all = reinterpret_cast<float*>(block_memory);
@@ -889,15 +898,15 @@ __global__ void __maxnreg__(block_backward_registers(V)) block_norm_backward_ker
 #pragma unroll
       for (int i = 0; i < V * 8; ++i) {
         float v = sums[k][i / 8][i % 8];
-        for (int o = 16; o >= threads; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-        const int c = block_column<VEC>(threads, tid, i / 8, i % 8);
-        if (threadIdx.x % 32 < threads && c < C) all[threadIdx.x / 32 * C + c] = v;
+        for (int o = 16; o >= p.threads; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        const int at = c.at(i / 8, i % 8);
+        if (threadIdx.x % 32 < p.threads && at < C) all[threadIdx.x / 32 * C + at] = v;
       }
       __syncthreads();
-      for (int c = threadIdx.x; c < C; c += blockDim.x) {
+      for (int at = threadIdx.x; at < C; at += blockDim.x) {
         float v = 0.f;
-        for (int w = 0; w < warps; ++w) v += all[w * C + c];
-        mine[k * C + c] = v;
+        for (int w = 0; w < warps; ++w) v += all[w * C + at];
+        mine[k * C + at] = v;
       }
     }
   }

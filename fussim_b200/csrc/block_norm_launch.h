@@ -42,17 +42,21 @@ int block_allow(Kernel kernel, std::atomic<bool> (&done)[64]) {
   return e == cudaSuccess ? FSSIM_OK : fail(FSSIM_ERR_CUDA, cudaGetErrorString(e));
 }
 
+// Columns that go to a thread together.
+template <typename X>
+constexpr int block_unit(bool vec) { return !vec ? 1 : sizeof(X) == 4 ? 4 : 8; }
+
 template <typename X, typename Y, int V, bool VEC, bool WARP, int MODE, bool STAGED = true>
 int block_forward(const BlockLaunch& l, const fssim::BlockParams& p, cudaStream_t stream) {
   static std::atomic<bool> done[64];
-  const auto kernel = fssim::block_norm_forward_kernel<X, Y, V, VEC, WARP, MODE, STAGED>;
+  const auto kernel = fssim::block_norm_forward_kernel<X, Y, V, block_unit<X>(VEC), WARP, MODE, STAGED>;
   const int st = block_allow(kernel, done);
   return st ? st : launch(kernel, l.grid, l.block, l.memory, stream, "block norm forward launch", p);
 }
 template <typename X, typename Y, int V, bool VEC, bool WARP, int MODE, bool STAGED = true>
 int block_backward(const BlockLaunch& l, const fssim::BlockParams& p, cudaStream_t stream) {
   static std::atomic<bool> done[64];
-  const auto kernel = fssim::block_norm_backward_kernel<X, Y, V, VEC, WARP, MODE, STAGED>;
+  const auto kernel = fssim::block_norm_backward_kernel<X, Y, V, block_unit<X>(VEC), WARP, MODE, STAGED>;
   const int st = block_allow(kernel, done);
   return st ? st : launch(kernel, l.grid, l.block, l.memory, stream, "block norm backward launch", p);
 }
