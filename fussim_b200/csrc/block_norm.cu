@@ -152,11 +152,13 @@ Layout layout(const Shape& s, bool backward, int mode, bool per_sample, bool vec
         break;
       }
       // (few rows: smaller CTAs, so that all SMs have some)
-      if (l.warp && block > 32 && l.B * ((l.T + parts - 1) / parts) < 2 * kSms) continue;
+      // (backward at least four rows of a thread, for which it leaves one set of sums)
+      const int64_t fewest = backward ? 4 : 1;
+      if (l.warp && block > 32 && l.B * ((l.T + parts * fewest - 1) / (parts * fewest)) < 2 * kSms) continue;
       for (int64_t on_sm = std::max(resident / block, 1); on_sm >= 1 && on_sm * block > most; --on_sm) {
         const int64_t wanted = (kSms * on_sm + l.B - 1) / l.B;
         // a thread adds at most 256 rows up in FP32
-        const int64_t rounds = std::min<int64_t>((l.T + parts * wanted - 1) / (parts * wanted), 256);
+        const int64_t rounds = std::clamp<int64_t>((l.T + parts * wanted - 1) / (parts * wanted), std::min(fewest, (l.T + parts - 1) / parts), 256);
         const int64_t chunk = rounds * parts, chunks = (l.T + chunk - 1) / chunk;
         const int64_t crowd = std::min(on_sm, (l.B * chunks + kSms - 1) / kSms);
         const int64_t room = std::min<int64_t>(kSmMemory / crowd - 2048, fssim_host::kBlockMemory);
@@ -276,8 +278,11 @@ int forward(const fssim_block_norm_forward_args* a, cudaStream_t stream) {
 
 // The backward pass's split of its sums.
 struct Merge {
-  int sums, segments;
-  size_t partial_bytes, merged_bytes;
+  int sums, splits, split_samples;
+  int64_t columns;  // blocks of columns
+  bool shared;      // a gradient is a sum over samples
+  size_t partial_bytes, total_bytes;
+  size_t bytes() const { return partial_bytes + total_bytes; }
 };
 
 bool wants_sums(const fssim_block_norm_backward_args& a, int* sums) {
@@ -309,13 +314,15 @@ Layout backward_layout(const fssim_block_norm_backward_args& a) {
 Merge merge_of(const fssim_block_norm_backward_args& a, const Layout& l) {
   Merge m{};
   if (!wants_sums(a, &m.sums)) return Merge{};
-  const int64_t columns = (a.C + kBlockMergeColumns - 1) / kBlockMergeColumns;
-  int64_t segments = (2 * kSms + columns * l.B - 1) / (columns * l.B);
-  const int64_t most = l.chunks / (4 * kBlockMergeTeams);
-  segments = segments > most ? most : segments;
-  m.segments = static_cast<int>(segments < 1 ? 1 : segments);
+  m.columns = (a.C + kBlockMergeColumns - 1) / kBlockMergeColumns;
+  // many samples: more CTAs for them, down to one for each team
+  const int64_t splits = std::min((2 * kSms + m.columns - 1) / m.columns, l.B / kBlockMergeTeams);
+  m.split_samples = static_cast<int>((l.B + std::max<int64_t>(splits, 1) - 1) / std::max<int64_t>(splits, 1));
+  m.splits = static_cast<int>((l.B + m.split_samples - 1) / m.split_samples);
+  for (const fssim_channels_grad* g : {&a.dgate, &a.dweight, &a.dbias, &a.dscale, &a.dshift, &a.dbranch_weight, &a.dbranch_bias})
+    m.shared = m.shared || (g->data && !g->per_sample);
   m.partial_bytes = (static_cast<size_t>(l.B * l.chunks) * m.sums * a.C * sizeof(float) + 15) / 16 * 16;
-  m.merged_bytes = l.chunks > 1 ? static_cast<size_t>(l.B) * m.segments * m.sums * a.C * sizeof(double) : 0;
+  if (m.splits > 1 && m.shared) m.total_bytes = static_cast<size_t>(m.splits) * kVectors * a.C * sizeof(double);
   return m;
 }
 
@@ -350,7 +357,7 @@ int backward(const fssim_block_norm_backward_args* a, cudaStream_t stream) {
   const Layout l = backward_layout(*a);
   if ((st = check_grid(l.B * l.chunks))) return st;
   const Merge m = merge_of(*a, l);
-  const size_t need = m.partial_bytes + m.merged_bytes;
+  const size_t need = m.bytes();
   if (need > 0 && (!a->workspace || a->workspace_bytes < need))
     return fail(FSSIM_ERR_WORKSPACE, "workspace smaller than fssim_block_norm_backward_workspace_bytes");
   if (!aligned(a->workspace, 16)) return fail(FSSIM_ERR_WORKSPACE, "workspace must be 16-byte aligned");
@@ -376,22 +383,14 @@ int backward(const fssim_block_norm_backward_args* a, cudaStream_t stream) {
   p.sums = m.sums;
   st = launch_rows(true, s, l, p, stream);
   if (st || !m.sums) return st;
-  const int64_t columns = (s.C + kBlockMergeColumns - 1) / kBlockMergeColumns;
-  constexpr unsigned kMergeThreads = kBlockMergeColumns * kBlockMergeTeams;
-  double* merged = m.merged_bytes ? reinterpret_cast<double*>(static_cast<char*>(a->workspace) + m.partial_bytes) : nullptr;
-  if (merged) {
-    if ((st = check_grid(columns * l.B * m.segments))) return st;
-    st = launch(block_norm_merge_kernel, static_cast<unsigned>(columns * l.B * m.segments), kMergeThreads, 0, stream,
-                "block norm merge launch", static_cast<const float*>(p.partials), merged, p.C, m.sums, l.chunks,
-                m.segments);
-    if (st) return st;
-  }
   BlockGradParams g{};
-  g.merged = merged;
   g.partials = p.partials;
-  g.B = l.B;
-  g.segments = m.segments;
-  g.sums = m.sums;
+  g.totals = m.total_bytes ? reinterpret_cast<double*>(static_cast<char*>(a->workspace) + m.partial_bytes) : nullptr;
+  g.B = static_cast<int>(l.B);
+  g.chunks = static_cast<int>(l.chunks);
+  g.split_samples = m.split_samples;
+  g.shared = m.shared;
+  g.splits = m.splits;
   g.C = p.C;
   g.s = a->residual_scale;
   g.gate = p.gate;
@@ -401,15 +400,21 @@ int backward(const fssim_block_norm_backward_args* a, cudaStream_t stream) {
   g.after_weight = p.after_weight;
   g.after_bias = channels(a->branch_bias, s.C);
   const auto place = [](const fssim_channels_grad& v) { return BlockGrad{v.data, v.dtype, v.per_sample}; };
-  g.dgate = place(a->dgate);
-  g.dweight = place(a->dweight);
-  g.dbias = place(a->dbias);
-  g.dscale = place(a->dscale);
-  g.dshift = place(a->dshift);
-  g.dafter_weight = place(a->dbranch_weight);
-  g.dafter_bias = place(a->dbranch_bias);
-  return launch(block_norm_grads_kernel, static_cast<unsigned>(columns), kMergeThreads, 0, stream,
-                "block norm gradients launch", g);
+  g.grads[kVectorGate] = place(a->dgate);
+  g.grads[kVectorWeight] = place(a->dweight);
+  g.grads[kVectorBias] = place(a->dbias);
+  g.grads[kVectorScale] = place(a->dscale);
+  g.grads[kVectorShift] = place(a->dshift);
+  g.grads[kVectorAfterWeight] = place(a->dbranch_weight);
+  g.grads[kVectorAfterBias] = place(a->dbranch_bias);
+  const auto kernel = m.sums == 2   ? block_norm_grads_kernel<2>
+                      : m.sums == 3 ? block_norm_grads_kernel<3>
+                                    : block_norm_grads_kernel<4>;
+  st = launch(kernel, static_cast<unsigned>(m.columns * m.splits), kBlockMergeColumns * kBlockMergeTeams, 0, stream,
+              "block norm gradients launch", g);
+  if (st || !m.total_bytes) return st;
+  return launch(block_norm_totals_kernel, static_cast<unsigned>((s.C + 255) / 256), 256, 0, stream,
+                "block norm totals launch", g);
 }
 
 }  // namespace
@@ -424,7 +429,7 @@ int fssim_block_norm_forward(const fssim_block_norm_forward_args* a, fssim_strea
 size_t fssim_block_norm_backward_workspace_bytes(const fssim_block_norm_backward_args* a) {
   if (!a || a->B <= 0 || a->T <= 0 || check_shape({a->B, a->T, a->C, a->x_dtype, a->y_dtype})) return 0;
   const Merge m = merge_of(*a, backward_layout(*a));
-  return m.partial_bytes + m.merged_bytes;
+  return m.bytes();
 }
 
 int fssim_block_norm_backward(const fssim_block_norm_backward_args* a, fssim_stream_t stream) {
