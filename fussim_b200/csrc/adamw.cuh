@@ -106,17 +106,28 @@ __device__ __forceinline__ AdamwScalars adamw_scalars(const AdamwStep& a) {
   return s;
 }
 
-// Eight numbers of a lane: consecutive ones (VEC), or 32 apart where the memory begins at no
-// vector's boundary or ends within the block.
-template <bool VEC>
+// How a lane's eight numbers lie in a block: consecutive ones, or 32 apart where the memory begins at no
+// vector's boundary, or (the same, counted) where it ends within the block.
+enum AdamwLie { kAdamwVectors, kAdamwApart, kAdamwEnd };
+template <int LIE>
 __device__ __forceinline__ int adamw_place(int i) {
   const int lane = threadIdx.x % 32;
-  return VEC ? lane * 8 + i : lane + 32 * i;
+  return LIE == kAdamwVectors ? lane * 8 + i : lane + 32 * i;
 }
 
-template <bool VEC, typename T>
-__device__ __forceinline__ void adamw_load(const T* p, int valid, float (&f)[8]) {
-  if constexpr (VEC) {
+// Eight numbers, as the packed FP32 instructions take them (each half rounded as by itself).
+struct AdamwEight {
+  float2 p[4];
+  __device__ __forceinline__ float& operator[](int i) { return i & 1 ? p[i / 2].y : p[i / 2].x; }
+  __device__ __forceinline__ float operator[](int i) const { return i & 1 ? p[i / 2].y : p[i / 2].x; }
+};
+__device__ __forceinline__ float2 adamw_twice(float v) { return make_float2(v, v); }
+
+template <int LIE, typename T>
+__device__ __forceinline__ AdamwEight adamw_load(const void* from, int64_t b, int valid) {
+  const T* p = static_cast<const T*>(from) + b;
+  AdamwEight f;
+  if constexpr (LIE == kAdamwVectors) {
     constexpr int N = 16 / sizeof(T);
     const uint4* at = reinterpret_cast<const uint4*>(p) + threadIdx.x % 32 * (8 / N);
     uint4 raw[8 / N];
@@ -126,17 +137,21 @@ __device__ __forceinline__ void adamw_load(const T* p, int valid, float (&f)[8])
 #pragma unroll
     for (int i = 0; i < 8; ++i) f[i] = run_widen(e[i]);
   } else {
+    p += threadIdx.x % 32;
+    T e[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int at = adamw_place<false>(i);
-      f[i] = at < valid ? run_widen(p[at]) : 0.f;
-    }
+    for (int i = 0; i < 8; ++i)
+      e[i] = LIE == kAdamwApart || adamw_place<LIE>(i) < valid ? p[32 * i] : run_narrow<T>(0.f);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = run_widen(e[i]);
   }
+  return f;
 }
 
-template <bool VEC, typename T>
-__device__ __forceinline__ void adamw_store(T* p, int valid, const float (&f)[8]) {
-  if constexpr (VEC) {
+template <int LIE, typename T>
+__device__ __forceinline__ void adamw_store(void* to, int64_t b, int valid, const AdamwEight& f) {
+  T* p = static_cast<T*>(to) + b;
+  if constexpr (LIE == kAdamwVectors) {
     constexpr int N = 16 / sizeof(T);
     uint4 raw[8 / N];
     T* e = reinterpret_cast<T*>(raw);
@@ -146,90 +161,126 @@ __device__ __forceinline__ void adamw_store(T* p, int valid, const float (&f)[8]
 #pragma unroll
     for (int k = 0; k < 8 / N; ++k) __stcs(at + k, raw[k]);
   } else {
+    p += threadIdx.x % 32;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int at = adamw_place<false>(i);
-      if (at < valid) p[at] = run_narrow<T>(f[i]);
-    }
+    for (int i = 0; i < 8; ++i)
+      if (LIE == kAdamwApart || adamw_place<LIE>(i) < valid) p[32 * i] = run_narrow<T>(f[i]);
   }
 }
 
 // Eight e4m3 codes, as the numbers that they stand for times `scale`.
-template <bool VEC>
-__device__ __forceinline__ void adamw_load_codes(const unsigned char* p, int valid, float scale, float (&f)[8]) {
-  unsigned char c[8];
-  if constexpr (VEC) {
+template <int LIE>
+__device__ __forceinline__ AdamwEight adamw_load_codes(const void* from, int64_t b, int valid, float scale) {
+  const unsigned char* p = static_cast<const unsigned char*>(from) + b;
+  alignas(8) unsigned char c[8];
+  if constexpr (LIE == kAdamwVectors) {
     *reinterpret_cast<uint2*>(c) = __ldcs(reinterpret_cast<const uint2*>(p) + threadIdx.x % 32);
   } else {
+    p += threadIdx.x % 32;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int at = adamw_place<false>(i);
-      c[i] = at < valid ? p[at] : 0;
-    }
+    for (int i = 0; i < 8; ++i) c[i] = LIE == kAdamwApart || adamw_place<LIE>(i) < valid ? p[32 * i] : 0;
   }
+  AdamwEight f;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(
         static_cast<__nv_fp8x2_storage_t>(c[2 * i] | c[2 * i + 1] << 8), __NV_E4M3);
-    const float2 pair = __half22float2(__half2(h));
-    f[2 * i] = __fmul_rn(pair.x, scale);
-    f[2 * i + 1] = __fmul_rn(pair.y, scale);
+    f.p[i] = __fmul2_rn(__half22float2(__half2(h)), adamw_twice(scale));
   }
+  return f;
 }
 
-template <bool VEC>
-__device__ __forceinline__ void adamw_store_codes(unsigned char* p, int valid, const float (&f)[8]) {
-  unsigned char c[8];
+template <int LIE>
+__device__ __forceinline__ void adamw_store_codes(void* to, int64_t b, int valid, const AdamwEight& f) {
+  unsigned char* p = static_cast<unsigned char*>(to) + b;
+  unsigned pair[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const __nv_fp8x2_storage_t pair =
-        __nv_cvt_float2_to_fp8x2(make_float2(f[2 * i], f[2 * i + 1]), __NV_SATFINITE, __NV_E4M3);
-    c[2 * i] = static_cast<unsigned char>(pair & 0xFF);
-    c[2 * i + 1] = static_cast<unsigned char>(pair >> 8);
-  }
-  if constexpr (VEC) {
-    __stcs(reinterpret_cast<uint2*>(p) + threadIdx.x % 32, *reinterpret_cast<const uint2*>(c));
+  for (int i = 0; i < 4; ++i) pair[i] = __nv_cvt_float2_to_fp8x2(f.p[i], __NV_SATFINITE, __NV_E4M3);
+  if constexpr (LIE == kAdamwVectors) {
+    __stcs(reinterpret_cast<uint2*>(p) + threadIdx.x % 32,
+           make_uint2(__byte_perm(pair[0], pair[1], 0x5410), __byte_perm(pair[2], pair[3], 0x5410)));
   } else {
+    p += threadIdx.x % 32;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int at = adamw_place<false>(i);
-      if (at < valid) p[at] = c[i];
-    }
+    for (int i = 0; i < 8; ++i)
+      if (LIE == kAdamwApart || adamw_place<LIE>(i) < valid)
+        p[32 * i] = static_cast<unsigned char>(i & 1 ? pair[i / 2] >> 8 : pair[i / 2]);
   }
 }
 
 constexpr uint32_t kInfBits = 0x7F800000u;
 
+// The largest of two magnitudes; NaN where one is.
+__device__ __forceinline__ float adamw_most(float a, float b) {
+  float m;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(fabsf(a)), "f"(fabsf(b)));
+  return m;
+}
+
 // The largest magnitude of a block that is finite (and at least 2^-100, so that its reciprocal is
 // too), from the lanes' eight numbers; `odd` tells whether one is not.
-__device__ __forceinline__ float adamw_top(const float (&f)[8], bool& odd) {
-  uint32_t most = 0;
+__device__ __forceinline__ float adamw_top(const AdamwEight& f, bool& odd) {
+  float most = adamw_most(f[0], f[1]);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) most = max(most, __float_as_uint(f[i]) & 0x7FFFFFFFu);
-  uint32_t top = __reduce_max_sync(0xffffffffu, most);
+  for (int i = 2; i < 8; ++i) most = adamw_most(most, f[i]);
+  uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(most) & 0x7FFFFFFFu);
   odd = top >= kInfBits;
   if (odd) {
-    most = 0;
+    uint32_t finite = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const uint32_t bits = __float_as_uint(f[i]) & 0x7FFFFFFFu;
-      if (bits < kInfBits) most = max(most, bits);
+      if (bits < kInfBits) finite = max(finite, bits);
     }
-    top = __reduce_max_sync(0xffffffffu, most);
+    top = __reduce_max_sync(0xffffffffu, finite);
   }
   return fmaxf(__uint_as_float(top), 0x1p-100f);
 }
 
-// Rounds |x| times `up` to three bits behind the first, upwards in as many of the 2^20 cases of `rnd`
-// as its distance from the lower neighbour asks for: on average a code stands for x itself, and a
+// Rounds x times `up` to three bits behind the first, away from zero in as many of the 2^20 cases of
+// `rnd` as its distance from the lower neighbour asks for: on average a code stands for x itself, and a
 // slow change of a moment is not lost in the codes' steps (6 to 12 %), as it is when each step
 // rounds to the nearest. Numbers below 2^-6 lie between codes of even distance and go to the nearest.
 template <bool ROOT>
-__device__ __forceinline__ float adamw_draw(float x, float up, uint32_t rnd) {
-  float y = __fmul_rn(fabsf(x), up);
-  if (ROOT && x > 0.f) y = fmaxf(y, 0x1p-6f);  // a root that is not zero stays so: it divides
-  y = __uint_as_float((__float_as_uint(y) + rnd) & 0xFFF00000u);
-  return ROOT ? y : copysignf(y, x);
+__device__ __forceinline__ float adamw_draw(float y, bool floor, uint32_t rnd) {
+  if (ROOT) y = floor ? fmaxf(y, 0x1p-6f) : y;  // a root that is not zero stays so: it divides
+  return __uint_as_float((__float_as_uint(y) + rnd) & 0xFFF00000u);
+}
+
+// Roots and quotients after P. Markstein (Computation of elementary functions on the IBM RISC
+// System/6000 processor, 1990): an approximation, and a correction by its exact remainder, which a
+// fused multiply-add gives; without the branches that CUDA's functions have for each number. They
+// are the correctly rounded ones (all 2^24 roots of two binades, and 2^30 random quotients, compared)
+// where adamw_ordinary holds.
+__device__ __forceinline__ float2 adamw_root(float2 v) {
+  float2 y;  // (of zero any that is finite)
+  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y.x) : "f"(fmaxf(v.x, 0x1p-80f)));
+  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y.y) : "f"(fmaxf(v.y, 0x1p-80f)));
+  const float2 g = __fmul2_rn(v, y), h = __fmul2_rn(y, adamw_twice(0.5f));
+  const float2 rest = __ffma2_rn(__fmul2_rn(g, adamw_twice(-1.f)), g, v);
+  return __ffma2_rn(rest, h, g);
+}
+__device__ __forceinline__ float2 adamw_quotient(float2 m, float2 d) {
+  float2 y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y.x) : "f"(d.x));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y.y) : "f"(d.y));
+  const float2 minus = __fmul2_rn(d, adamw_twice(-1.f));
+  y = __ffma2_rn(y, __ffma2_rn(minus, y, adamw_twice(1.f)), y);
+  const float2 q = __fmul2_rn(m, y);
+  return __ffma2_rn(__ffma2_rn(minus, q, m), y, q);
+}
+// Every second moment is zero or within 2^-80 and 2^80, and every first at most that. (The quotient of a
+// first moment below 2^-80 may be off in its last place: it is nothing beside a parameter.)
+__device__ __forceinline__ bool adamw_ordinary(const AdamwEight& m, const AdamwEight& v) {
+  uint32_t least = 0xFFFFFFFFu, most = 0, first = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t bits = __float_as_uint(v[i]);
+    least = min(least, bits - 1u);  // (zero is the largest)
+    most = max(most, bits);
+    first = max(first, __float_as_uint(m[i]) & 0x7FFFFFFFu);
+  }
+  return least >= 0x17800000u - 1u && max(most, first) <= 0x67800000u;
 }
 
 struct AdamwRun {
@@ -243,40 +294,51 @@ struct AdamwRun {
   uint32_t key;
 };
 
-template <typename P, typename G, int BITS, bool VEC>
+template <typename P, typename G, int BITS, int LIE>
 __device__ __forceinline__ void adamw_block(const AdamwRun& r, const AdamwScalars& s, int64_t b, int valid) {
-  float p[8], g[8], m[8], v[8];
-  adamw_load<VEC>(static_cast<const P*>(r.param) + b, valid, p);
-  adamw_load<VEC>(static_cast<const G*>(r.grad) + b, valid, g);
+  AdamwEight p = adamw_load<LIE, P>(r.param, b, valid);
+  const AdamwEight g = adamw_load<LIE, G>(r.grad, b, valid);
+  AdamwEight m, v, root;
   const int64_t block = b / kAdamwBlock;
   if constexpr (BITS == 32) {
-    adamw_load<VEC>(static_cast<const float*>(r.first) + b, valid, m);
-    adamw_load<VEC>(static_cast<const float*>(r.second) + b, valid, v);
+    m = adamw_load<LIE, float>(r.first, b, valid);
+    v = adamw_load<LIE, float>(r.second, b, valid);
   } else {
     const float scale1 = r.scales[2 * block], scale2 = r.scales[2 * block + 1];
-    adamw_load_codes<VEC>(static_cast<const unsigned char*>(r.first) + b, valid, scale1, m);
-    adamw_load_codes<VEC>(static_cast<const unsigned char*>(r.second) + b, valid, scale2, v);
+    m = adamw_load_codes<LIE>(r.first, b, valid, scale1);
+    v = adamw_load_codes<LIE>(r.second, b, valid, scale2);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = __fmul_rn(v[i], v[i]);
+    for (int i = 0; i < 4; ++i) v.p[i] = __fmul2_rn(v.p[i], v.p[i]);
   }
-  float root[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float gi = __fmul_rn(g[i], s.coef);
-    m[i] = __fadd_rn(__fmul_rn(m[i], s.beta1), __fmul_rn(gi, s.rest1));
-    v[i] = __fadd_rn(__fmul_rn(v[i], s.beta2), __fmul_rn(__fmul_rn(gi, gi), s.rest2));
-    root[i] = __fsqrt_rn(v[i]);
-    const float change = __fdiv_rn(m[i], __fadd_rn(__fmul_rn(root[i], s.lift), s.eps));
-    p[i] = __fsub_rn(__fmul_rn(p[i], s.decay), __fmul_rn(change, s.rate));
+  for (int i = 0; i < 4; ++i) {
+    const float2 gi = __fmul2_rn(g.p[i], adamw_twice(s.coef));
+    m.p[i] = pair_add(__fmul2_rn(m.p[i], adamw_twice(s.beta1)), __fmul2_rn(gi, adamw_twice(s.rest1)));
+    v.p[i] = pair_add(__fmul2_rn(v.p[i], adamw_twice(s.beta2)), __fmul2_rn(__fmul2_rn(gi, gi), adamw_twice(s.rest2)));
   }
-  adamw_store<VEC>(static_cast<P*>(r.param) + b, valid, p);
+  const bool ordinary = s.eps >= 0x1p-60f && adamw_ordinary(m, v);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const auto den = [&] { return pair_add(__fmul2_rn(root.p[i], adamw_twice(s.lift)), adamw_twice(s.eps)); };
+    float2 change;
+    if (ordinary) {
+      root.p[i] = adamw_root(v.p[i]);
+      change = adamw_quotient(m.p[i], den());
+    } else {
+      root.p[i] = make_float2(__fsqrt_rn(v.p[i].x), __fsqrt_rn(v.p[i].y));
+      const float2 d = den();
+      change = make_float2(__fdiv_rn(m.p[i].x, d.x), __fdiv_rn(m.p[i].y, d.y));
+    }
+    p.p[i] = pair_add(__fmul2_rn(p.p[i], adamw_twice(s.decay)), __fmul2_rn(change, adamw_twice(-s.rate)));
+  }
+  adamw_store<LIE, P>(r.param, b, valid, p);
   if (sizeof(P) == 4 && r.copy) {
-    if (r.copy_dtype == 1) adamw_store<VEC>(static_cast<__half*>(r.copy) + b, valid, p);
-    else adamw_store<VEC>(static_cast<__nv_bfloat16*>(r.copy) + b, valid, p);
+    if (r.copy_dtype == 1) adamw_store<LIE, __half>(r.copy, b, valid, p);
+    else adamw_store<LIE, __nv_bfloat16>(r.copy, b, valid, p);
   }
   if constexpr (BITS == 32) {
-    adamw_store<VEC>(static_cast<float*>(r.first) + b, valid, m);
-    adamw_store<VEC>(static_cast<float*>(r.second) + b, valid, v);
+    adamw_store<LIE, float>(r.first, b, valid, m);
+    adamw_store<LIE, float>(r.second, b, valid, v);
   } else {
     bool odd1, odd2;
     const float top1 = adamw_top(m, odd1), top2 = adamw_top(root, odd2);
@@ -284,29 +346,45 @@ __device__ __forceinline__ void adamw_block(const AdamwRun& r, const AdamwScalar
     if (threadIdx.x % 32 < 2)
       r.scales[2 * block + threadIdx.x % 32] = __fmul_rn(threadIdx.x % 32 ? top2 : top1, 1.f / 448.f);
     const uint32_t key = adamw_mix(r.key + static_cast<uint32_t>(block));
+    AdamwEight code1, code2;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      code1.p[i] = __fmul2_rn(m.p[i], adamw_twice(up1));
+      code2.p[i] = __fmul2_rn(root.p[i], adamw_twice(up2));
+    }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const uint32_t rnd = adamw_random(key, adamw_place<VEC>(i));
-      const bool bad1 = odd1 && !isfinite(m[i]), bad2 = odd2 && !isfinite(root[i]);
-      m[i] = bad1 ? NAN : adamw_draw<false>(m[i], up1, rnd & 0xFFFFFu);
-      root[i] = bad2 ? NAN : adamw_draw<true>(root[i], up2, rnd >> 12);
+      const uint32_t rnd = adamw_random(key, adamw_place<LIE>(i));
+      code1[i] = adamw_draw<false>(code1[i], false, rnd & 0xFFFFFu);
+      code2[i] = adamw_draw<true>(code2[i], root[i] > 0.f, rnd >> 12);
     }
-    adamw_store_codes<VEC>(static_cast<unsigned char*>(r.first) + b, valid, m);
-    adamw_store_codes<VEC>(static_cast<unsigned char*>(r.second) + b, valid, root);
+    if (odd1 || odd2) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (!isfinite(m[i])) code1[i] = NAN;
+        if (!isfinite(root[i])) code2[i] = NAN;
+      }
+    }
+    adamw_store_codes<LIE>(r.first, b, valid, code1);
+    adamw_store_codes<LIE>(r.second, b, valid, code2);
   }
 }
 
 // The numbers [b, e) of a run, b a multiple of a unit.
 template <typename P, typename G, int BITS>
-__device__ __noinline__ void adamw_piece(const AdamwRun& r, const AdamwScalars& s, int64_t b, int64_t e) {
+__device__ __noinline__ void adamw_piece(const AdamwRun run, const AdamwScalars* scalars, int64_t b, int64_t e) {
+  const AdamwRun r = run;
+  const AdamwScalars s = *scalars;
   const uintptr_t ends = reinterpret_cast<uintptr_t>(r.param) | reinterpret_cast<uintptr_t>(r.grad) |
                          reinterpret_cast<uintptr_t>(r.copy);
   const uintptr_t state = reinterpret_cast<uintptr_t>(r.first) | reinterpret_cast<uintptr_t>(r.second);
   const bool vectors = ends % 16 == 0 && state % (BITS == 32 ? 16 : 8) == 0;
-  for (int64_t at = b + threadIdx.x / 32 * kAdamwBlock; at < e; at += kRunUnit) {
-    if (vectors && at + kAdamwBlock <= e) adamw_block<P, G, BITS, true>(r, s, at, kAdamwBlock);
-    else adamw_block<P, G, BITS, false>(r, s, at, static_cast<int>(min(e - at, int64_t{kAdamwBlock})));
-  }
+  int64_t at = b + threadIdx.x / 32 * kAdamwBlock;
+  if (vectors)
+    for (; at + kAdamwBlock <= e; at += kRunUnit) adamw_block<P, G, BITS, kAdamwVectors>(r, s, at, kAdamwBlock);
+  else
+    for (; at + kAdamwBlock <= e; at += kRunUnit) adamw_block<P, G, BITS, kAdamwApart>(r, s, at, kAdamwBlock);
+  if (at < e) adamw_block<P, G, BITS, kAdamwEnd>(r, s, at, static_cast<int>(e - at));
 }
 
 template <int BITS, int K>
@@ -323,13 +401,13 @@ __global__ void __launch_bounds__(kAdamwThreads, kAdamwResident)
     const AdamwRun r{t.param[i], t.grad[i], t.first[i], t.second[i], t.scales[i], t.copy[i], t.copy_dtype[i],
                      adamw_mix(s.key + t.index[i])};
     switch (t.kind[i]) {
-      case adamw_kind(0, 0): adamw_piece<float, float, BITS>(r, s, b, e); break;
-      case adamw_kind(0, 1): adamw_piece<float, __half, BITS>(r, s, b, e); break;
-      case adamw_kind(0, 2): adamw_piece<float, __nv_bfloat16, BITS>(r, s, b, e); break;
-      case adamw_kind(1, 0): adamw_piece<__half, float, BITS>(r, s, b, e); break;
-      case adamw_kind(1, 1): adamw_piece<__half, __half, BITS>(r, s, b, e); break;
-      case adamw_kind(2, 0): adamw_piece<__nv_bfloat16, float, BITS>(r, s, b, e); break;
-      case adamw_kind(2, 2): adamw_piece<__nv_bfloat16, __nv_bfloat16, BITS>(r, s, b, e); break;
+      case adamw_kind(0, 0): adamw_piece<float, float, BITS>(r, &s, b, e); break;
+      case adamw_kind(0, 1): adamw_piece<float, __half, BITS>(r, &s, b, e); break;
+      case adamw_kind(0, 2): adamw_piece<float, __nv_bfloat16, BITS>(r, &s, b, e); break;
+      case adamw_kind(1, 0): adamw_piece<__half, float, BITS>(r, &s, b, e); break;
+      case adamw_kind(1, 1): adamw_piece<__half, __half, BITS>(r, &s, b, e); break;
+      case adamw_kind(2, 0): adamw_piece<__nv_bfloat16, float, BITS>(r, &s, b, e); break;
+      case adamw_kind(2, 2): adamw_piece<__nv_bfloat16, __nv_bfloat16, BITS>(r, &s, b, e); break;
       default: break;  // refused by the host
     }
   });

@@ -711,7 +711,7 @@ __global__ void __maxnreg__(block_forward_registers(V, MODE)) block_norm_forward
           }, u, w, o);
         }
         // (two roundings, as of a product and a sum one after the other)
-        e = BlockPacked<X>::of(pairs([](float2 a, float2 g2, float2 x) { return __fadd2_rn(x, __fmul2_rn(g2, a)); }, u, g, r[v]));
+        e = BlockPacked<X>::of(pairs([](float2 a, float2 g2, float2 x) { return pair_add(x, __fmul2_rn(g2, a)); }, u, g, r[v]));
       }
       if (active) block_store<X>(p.r, offset, c, v, e);
       r[v] = c.keep(e.widen(), v);  // z is the norm of r as it is held

@@ -6,6 +6,7 @@
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+#include <cuda_runtime.h>
 #include <stdint.h>
 
 namespace fssim {
@@ -20,6 +21,12 @@ template <> __device__ __forceinline__ float run_narrow<float>(float v) { return
 template <> __device__ __forceinline__ __half run_narrow<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 run_narrow<__nv_bfloat16>(float v) {
   return __float2bfloat16_rn(v);
+}
+
+// Sums of pairs, rounded by themselves: a packed product and a packed sum become one fused multiply-add
+// (whatever rounding they name), which two single sums do not.
+__device__ __forceinline__ float2 pair_add(float2 a, float2 b) {
+  return make_float2(__fadd_rn(a.x, b.x), __fadd_rn(a.y, b.y));
 }
 
 // The unit range of a CTA.
