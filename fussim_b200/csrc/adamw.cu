@@ -14,7 +14,6 @@ namespace {
 
 using fssim::AdamwTable;
 using fssim::kAdamwBlock;
-using fssim::kAdamwMaxCtas;
 using fssim::kAdamwThreads;
 using fssim::kRunUnit;
 using fssim_host::aligned;
@@ -114,7 +113,8 @@ int launch_from(const fssim_adamw_args& a, int64_t* begin, cudaStream_t stream) 
   *begin = fill(a, *begin, t.get());
   if (t->count == 0) return FSSIM_OK;
   const int64_t units = t->unit0[t->count];
-  const unsigned grid = static_cast<unsigned>(units < kAdamwMaxCtas ? units : kAdamwMaxCtas);
+  const int64_t most = 148 * fssim::adamw_resident(a.state_bits);
+  const unsigned grid = static_cast<unsigned>(units < most ? units : most);
   return a.state_bits == 32
              ? launch(fssim::adamw_kernel<32, K>, grid, kAdamwThreads, 0, stream, "AdamW launch", *t)
              : launch(fssim::adamw_kernel<8, K>, grid, kAdamwThreads, 0, stream, "AdamW launch", *t);

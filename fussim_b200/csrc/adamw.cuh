@@ -20,6 +20,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "pdl.cuh"
 #include "runs.cuh"
 
@@ -27,8 +29,9 @@ namespace fssim {
 
 constexpr int kAdamwThreads = 256;
 constexpr int kAdamwBlock = 256;     // numbers that share a scale
-constexpr int kAdamwResident = 3;    // CTAs on one SM
-constexpr int kAdamwMaxCtas = 148 * kAdamwResident;
+// CTAs on one SM: with moments of 32 bits fewer streams at a time (59 million numbers: 269 us; three 277),
+// with those of 8 more warps for the arithmetic (160 million: 417; two 579).
+__host__ __device__ constexpr int adamw_resident(int bits) { return bits == 32 ? 2 : 3; }
 static_assert(kRunUnit == kAdamwThreads / 32 * kAdamwBlock, "a unit is one block for each warp");
 
 // What a step's arithmetic takes besides the tensors.
@@ -106,13 +109,14 @@ __device__ __forceinline__ AdamwScalars adamw_scalars(const AdamwStep& a) {
   return s;
 }
 
-// How a lane's eight numbers lie in a block: consecutive ones, or 32 apart where the memory begins at no
-// vector's boundary, or (the same, counted) where it ends within the block.
-enum AdamwLie { kAdamwVectors, kAdamwApart, kAdamwEnd };
+// How a lane's eight numbers lie in a block: units of four or eight consecutive ones (16 bytes of the
+// widest tensor, so that the lanes' accesses lie side by side), or 32 apart where the memory begins
+// at no vector's boundary, or (the same, counted) where it ends within the block.
+enum AdamwLie { kAdamwApart = 1, kAdamwFours = 4, kAdamwEights = 8, kAdamwEnd = 0 };
 template <int LIE>
 __device__ __forceinline__ int adamw_place(int i) {
   const int lane = threadIdx.x % 32;
-  return LIE == kAdamwVectors ? lane * 8 + i : lane + 32 * i;
+  return LIE > 1 ? (i / LIE * 32 + lane) * LIE + i % LIE : lane + 32 * i;
 }
 
 // Eight numbers, as the packed FP32 instructions take them (each half rounded as by itself).
@@ -123,89 +127,90 @@ struct AdamwEight {
 };
 __device__ __forceinline__ float2 adamw_twice(float v) { return make_float2(v, v); }
 
-template <int LIE, typename T>
-__device__ __forceinline__ AdamwEight adamw_load(const void* from, int64_t b, int valid) {
-  const T* p = static_cast<const T*>(from) + b;
-  AdamwEight f;
-  if constexpr (LIE == kAdamwVectors) {
-    constexpr int N = 16 / sizeof(T);
-    const uint4* at = reinterpret_cast<const uint4*>(p) + threadIdx.x % 32 * (8 / N);
-    uint4 raw[8 / N];
-#pragma unroll
-    for (int k = 0; k < 8 / N; ++k) raw[k] = __ldcs(at + k);
-    const T* e = reinterpret_cast<const T*>(raw);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = run_widen(e[i]);
-  } else {
-    p += threadIdx.x % 32;
-    T e[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      e[i] = LIE == kAdamwApart || adamw_place<LIE>(i) < valid ? p[32 * i] : run_narrow<T>(0.f);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = run_widen(e[i]);
-  }
-  return f;
-}
+template <int BYTES> struct AdamwUnit;
+template <> struct AdamwUnit<16> { using type = uint4; };
+template <> struct AdamwUnit<8> { using type = uint2; };
+template <> struct AdamwUnit<4> { using type = unsigned; };
 
-template <int LIE, typename T>
-__device__ __forceinline__ void adamw_store(void* to, int64_t b, int valid, const AdamwEight& f) {
-  T* p = static_cast<T*>(to) + b;
-  if constexpr (LIE == kAdamwVectors) {
-    constexpr int N = 16 / sizeof(T);
-    uint4 raw[8 / N];
-    T* e = reinterpret_cast<T*>(raw);
+// Eight numbers of a lane, as they are in memory.
+template <typename T, int LIE>
+struct alignas(16) AdamwRaw {
+  T e[8];
+  __device__ __forceinline__ void load(const void* from, int64_t b, int valid) {
+    const T* p = static_cast<const T*>(from) + b;
+    if constexpr (LIE > 1 && LIE * sizeof(T) <= 16) {
+      using Unit = typename AdamwUnit<LIE * sizeof(T)>::type;
+#pragma unroll
+      for (int k = 0; k < 8 / LIE; ++k)
+        reinterpret_cast<Unit*>(e)[k] = __ldcs(reinterpret_cast<const Unit*>(p) + k * 32 + threadIdx.x % 32);
+    } else if constexpr (LIE > 1) {  // (32-bit gradients beside 16-bit parameters)
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+        reinterpret_cast<uint4*>(e)[k] = __ldcs(reinterpret_cast<const uint4*>(p) + threadIdx.x % 32 * 2 + k);
+    } else {
+      p += threadIdx.x % 32;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) e[i] = LIE == kAdamwApart || adamw_place<LIE>(i) < valid ? p[32 * i] : T{};
+    }
+  }
+  __device__ __forceinline__ void store(void* to, int64_t b, int valid) const {
+    T* p = static_cast<T*>(to) + b;
+    if constexpr (LIE > 1) {
+      using Unit = typename AdamwUnit<LIE * sizeof(T)>::type;
+#pragma unroll
+      for (int k = 0; k < 8 / LIE; ++k)
+        __stcs(reinterpret_cast<Unit*>(p) + k * 32 + threadIdx.x % 32, reinterpret_cast<const Unit*>(e)[k]);
+    } else {
+      p += threadIdx.x % 32;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (LIE == kAdamwApart || adamw_place<LIE>(i) < valid) p[32 * i] = e[i];
+    }
+  }
+  __device__ __forceinline__ AdamwEight widen() const {
+    AdamwEight f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = run_widen(e[i]);
+    return f;
+  }
+  __device__ __forceinline__ void narrow(const AdamwEight& f) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) e[i] = run_narrow<T>(f[i]);
-    uint4* at = reinterpret_cast<uint4*>(p) + threadIdx.x % 32 * (8 / N);
-#pragma unroll
-    for (int k = 0; k < 8 / N; ++k) __stcs(at + k, raw[k]);
-  } else {
-    p += threadIdx.x % 32;
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (LIE == kAdamwApart || adamw_place<LIE>(i) < valid) p[32 * i] = run_narrow<T>(f[i]);
   }
+};
+template <int LIE, typename T>
+__device__ __forceinline__ void adamw_store(void* to, int64_t b, int valid, const AdamwEight& f) {
+  AdamwRaw<T, LIE> raw;
+  raw.narrow(f);
+  raw.store(to, b, valid);
 }
 
 // Eight e4m3 codes, as the numbers that they stand for times `scale`.
 template <int LIE>
-__device__ __forceinline__ AdamwEight adamw_load_codes(const void* from, int64_t b, int valid, float scale) {
-  const unsigned char* p = static_cast<const unsigned char*>(from) + b;
-  alignas(8) unsigned char c[8];
-  if constexpr (LIE == kAdamwVectors) {
-    *reinterpret_cast<uint2*>(c) = __ldcs(reinterpret_cast<const uint2*>(p) + threadIdx.x % 32);
-  } else {
-    p += threadIdx.x % 32;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) c[i] = LIE == kAdamwApart || adamw_place<LIE>(i) < valid ? p[32 * i] : 0;
-  }
+__device__ __forceinline__ AdamwEight adamw_decode(const AdamwRaw<unsigned char, LIE>& c, float scale) {
   AdamwEight f;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(
-        static_cast<__nv_fp8x2_storage_t>(c[2 * i] | c[2 * i + 1] << 8), __NV_E4M3);
+        static_cast<__nv_fp8x2_storage_t>(c.e[2 * i] | c.e[2 * i + 1] << 8), __NV_E4M3);
     f.p[i] = __fmul2_rn(__half22float2(__half2(h)), adamw_twice(scale));
   }
   return f;
 }
-
 template <int LIE>
 __device__ __forceinline__ void adamw_store_codes(void* to, int64_t b, int valid, const AdamwEight& f) {
-  unsigned char* p = static_cast<unsigned char*>(to) + b;
+  AdamwRaw<unsigned char, LIE> raw;
   unsigned pair[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) pair[i] = __nv_cvt_float2_to_fp8x2(f.p[i], __NV_SATFINITE, __NV_E4M3);
-  if constexpr (LIE == kAdamwVectors) {
-    __stcs(reinterpret_cast<uint2*>(p) + threadIdx.x % 32,
-           make_uint2(__byte_perm(pair[0], pair[1], 0x5410), __byte_perm(pair[2], pair[3], 0x5410)));
+  if constexpr (LIE > 1) {
+    reinterpret_cast<unsigned*>(raw.e)[0] = __byte_perm(pair[0], pair[1], 0x5410);
+    reinterpret_cast<unsigned*>(raw.e)[1] = __byte_perm(pair[2], pair[3], 0x5410);
   } else {
-    p += threadIdx.x % 32;
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (LIE == kAdamwApart || adamw_place<LIE>(i) < valid)
-        p[32 * i] = static_cast<unsigned char>(i & 1 ? pair[i / 2] >> 8 : pair[i / 2]);
+    for (int i = 0; i < 8; ++i) raw.e[i] = static_cast<unsigned char>(i & 1 ? pair[i / 2] >> 8 : pair[i / 2]);
   }
+  raw.store(to, b, valid);
 }
 
 constexpr uint32_t kInfBits = 0x7F800000u;
@@ -217,8 +222,8 @@ __device__ __forceinline__ float adamw_most(float a, float b) {
   return m;
 }
 
-// The largest magnitude of a block that is finite (and at least 2^-100, so that its reciprocal is
-// too), from the lanes' eight numbers; `odd` tells whether one is not.
+// The largest magnitude of a block that is finite, from the lanes' eight numbers; `odd` tells whether one
+// is not.
 __device__ __forceinline__ float adamw_top(const AdamwEight& f, bool& odd) {
   float most = adamw_most(f[0], f[1]);
 #pragma unroll
@@ -234,7 +239,7 @@ __device__ __forceinline__ float adamw_top(const AdamwEight& f, bool& odd) {
     }
     top = __reduce_max_sync(0xffffffffu, finite);
   }
-  return fmaxf(__uint_as_float(top), 0x1p-100f);
+  return __uint_as_float(top);
 }
 
 // Rounds x times `up` to three bits behind the first, away from zero in as many of the 2^20 cases of
@@ -254,8 +259,9 @@ __device__ __forceinline__ float adamw_draw(float y, bool floor, uint32_t rnd) {
 // where adamw_ordinary holds.
 __device__ __forceinline__ float2 adamw_root(float2 v) {
   float2 y;  // (of zero any that is finite)
-  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y.x) : "f"(fmaxf(v.x, 0x1p-80f)));
-  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y.y) : "f"(fmaxf(v.y, 0x1p-80f)));
+  const float2 up = __fadd2_rn(v, adamw_twice(0x1p-120f));
+  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y.x) : "f"(up.x));
+  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y.y) : "f"(up.y));
   const float2 g = __fmul2_rn(v, y), h = __fmul2_rn(y, adamw_twice(0.5f));
   const float2 rest = __ffma2_rn(__fmul2_rn(g, adamw_twice(-1.f)), g, v);
   return __ffma2_rn(rest, h, g);
@@ -269,18 +275,14 @@ __device__ __forceinline__ float2 adamw_quotient(float2 m, float2 d) {
   const float2 q = __fmul2_rn(m, y);
   return __ffma2_rn(__ffma2_rn(minus, q, m), y, q);
 }
-// Every second moment is zero or within 2^-80 and 2^80, and every first at most that. (The quotient of a
-// first moment below 2^-80 may be off in its last place: it is nothing beside a parameter.)
-__device__ __forceinline__ bool adamw_ordinary(const AdamwEight& m, const AdamwEight& v) {
-  uint32_t least = 0xFFFFFFFFu, most = 0, first = 0;
+// Every second moment is zero or within 2^-80 and 2^80, and every first at most that (`most` is the
+// largest). (The quotient of a first moment below 2^-80 may be off in its last place: it is nothing
+// beside a parameter.)
+__device__ __forceinline__ bool adamw_ordinary(const AdamwEight& v, float most) {
+  uint32_t least = 0xFFFFFFFFu;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const uint32_t bits = __float_as_uint(v[i]);
-    least = min(least, bits - 1u);  // (zero is the largest)
-    most = max(most, bits);
-    first = max(first, __float_as_uint(m[i]) & 0x7FFFFFFFu);
-  }
-  return least >= 0x17800000u - 1u && max(most, first) <= 0x67800000u;
+  for (int i = 0; i < 8; ++i) least = min(least, __float_as_uint(v[i]) - 1u);  // (zero is the largest)
+  return least >= 0x17800000u - 1u && most <= 0x1p80f;
 }
 
 struct AdamwRun {
@@ -294,19 +296,37 @@ struct AdamwRun {
   uint32_t key;
 };
 
+// What a lane reads of a block.
 template <typename P, typename G, int BITS, int LIE>
-__device__ __forceinline__ void adamw_block(const AdamwRun& r, const AdamwScalars& s, int64_t b, int valid) {
-  AdamwEight p = adamw_load<LIE, P>(r.param, b, valid);
-  const AdamwEight g = adamw_load<LIE, G>(r.grad, b, valid);
-  AdamwEight m, v, root;
-  const int64_t block = b / kAdamwBlock;
+struct AdamwBlock {
+  AdamwRaw<P, LIE> p;
+  AdamwRaw<G, LIE> g;
+  AdamwRaw<std::conditional_t<BITS == 32, float, unsigned char>, LIE> m, v;
+  float scale1, scale2;
+  __device__ __forceinline__ void load(const AdamwRun& r, int64_t b, int valid) {
+    p.load(r.param, b, valid);
+    g.load(r.grad, b, valid);
+    m.load(r.first, b, valid);
+    v.load(r.second, b, valid);
+    if constexpr (BITS == 8) {
+      const float* scales = r.scales + b / kAdamwBlock * 2;
+      scale1 = scales[0];
+      scale2 = scales[1];
+    }
+  }
+};
+
+template <typename P, typename G, int BITS, int LIE>
+__device__ __forceinline__ void adamw_block(const AdamwRun& r, const AdamwScalars& s,
+                                            const AdamwBlock<P, G, BITS, LIE>& in, int64_t b, int valid) {
+  AdamwEight p = in.p.widen(), m, v, root;
+  const AdamwEight g = in.g.widen();
   if constexpr (BITS == 32) {
-    m = adamw_load<LIE, float>(r.first, b, valid);
-    v = adamw_load<LIE, float>(r.second, b, valid);
+    m = in.m.widen();
+    v = in.v.widen();
   } else {
-    const float scale1 = r.scales[2 * block], scale2 = r.scales[2 * block + 1];
-    m = adamw_load_codes<LIE>(r.first, b, valid, scale1);
-    v = adamw_load_codes<LIE>(r.second, b, valid, scale2);
+    m = adamw_decode(in.m, in.scale1);
+    v = adamw_decode(in.v, in.scale2);
 #pragma unroll
     for (int i = 0; i < 4; ++i) v.p[i] = __fmul2_rn(v.p[i], v.p[i]);
   }
@@ -316,7 +336,19 @@ __device__ __forceinline__ void adamw_block(const AdamwRun& r, const AdamwScalar
     m.p[i] = pair_add(__fmul2_rn(m.p[i], adamw_twice(s.beta1)), __fmul2_rn(gi, adamw_twice(s.rest1)));
     v.p[i] = pair_add(__fmul2_rn(v.p[i], adamw_twice(s.beta2)), __fmul2_rn(__fmul2_rn(gi, gi), adamw_twice(s.rest2)));
   }
-  const bool ordinary = s.eps >= 0x1p-60f && adamw_ordinary(m, v);
+  // the largest moments of the block (8 bits), or of the lane
+  bool odd1 = false, odd2 = false;
+  float top1, top2, most;
+  if constexpr (BITS == 8) {
+    top1 = adamw_top(m, odd1);
+    top2 = adamw_top(v, odd2);
+    most = odd1 || odd2 ? __uint_as_float(kInfBits) : fmaxf(top1, top2);
+  } else {
+    most = adamw_most(m[0], v[0]);
+#pragma unroll
+    for (int i = 1; i < 8; ++i) most = adamw_most(most, adamw_most(m[i], v[i]));
+  }
+  const bool ordinary = s.eps >= 0x1p-60f && adamw_ordinary(v, most);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const auto den = [&] { return pair_add(__fmul2_rn(root.p[i], adamw_twice(s.lift)), adamw_twice(s.eps)); };
@@ -340,8 +372,10 @@ __device__ __forceinline__ void adamw_block(const AdamwRun& r, const AdamwScalar
     adamw_store<LIE, float>(r.first, b, valid, m);
     adamw_store<LIE, float>(r.second, b, valid, v);
   } else {
-    bool odd1, odd2;
-    const float top1 = adamw_top(m, odd1), top2 = adamw_top(root, odd2);
+    const int64_t block = b / kAdamwBlock;
+    // (the largest root is the largest v's; both are at least 2^-100, so that their reciprocals are finite)
+    top1 = fmaxf(top1, 0x1p-100f);
+    top2 = fmaxf(__fsqrt_rn(top2), 0x1p-100f);
     const float up1 = __fmul_rn(__frcp_rn(top1), 448.f), up2 = __fmul_rn(__frcp_rn(top2), 448.f);
     if (threadIdx.x % 32 < 2)
       r.scales[2 * block + threadIdx.x % 32] = __fmul_rn(threadIdx.x % 32 ? top2 : top1, 1.f / 448.f);
@@ -375,20 +409,42 @@ template <typename P, typename G, int BITS>
 __device__ __noinline__ void adamw_piece(const AdamwRun run, const AdamwScalars* scalars, int64_t b, int64_t e) {
   const AdamwRun r = run;
   const AdamwScalars s = *scalars;
+  constexpr int kUnits = BITS == 32 || sizeof(P) == 4 ? kAdamwFours : kAdamwEights;
   const uintptr_t ends = reinterpret_cast<uintptr_t>(r.param) | reinterpret_cast<uintptr_t>(r.grad) |
                          reinterpret_cast<uintptr_t>(r.copy);
   const uintptr_t state = reinterpret_cast<uintptr_t>(r.first) | reinterpret_cast<uintptr_t>(r.second);
   const bool vectors = ends % 16 == 0 && state % (BITS == 32 ? 16 : 8) == 0;
   int64_t at = b + threadIdx.x / 32 * kAdamwBlock;
-  if (vectors)
-    for (; at + kAdamwBlock <= e; at += kRunUnit) adamw_block<P, G, BITS, kAdamwVectors>(r, s, at, kAdamwBlock);
-  else
-    for (; at + kAdamwBlock <= e; at += kRunUnit) adamw_block<P, G, BITS, kAdamwApart>(r, s, at, kAdamwBlock);
-  if (at < e) adamw_block<P, G, BITS, kAdamwEnd>(r, s, at, static_cast<int>(e - at));
+  // Moments of 8 bits in whole units: the next block is on its way while one is worked on (few bytes for
+  // much arithmetic); elsewhere the other warps' are enough.
+  const auto whole = [&](auto lie) {
+    constexpr bool kAhead = BITS == 8 && decltype(lie)::value > 1;
+    using Block = AdamwBlock<P, G, BITS, decltype(lie)::value>;
+    if (at + kAdamwBlock > e) return;
+    Block next;
+    if (kAhead) next.load(r, at, kAdamwBlock);
+    for (; at + kAdamwBlock <= e; at += kRunUnit) {
+      Block now;
+      if (kAhead) {
+        now = next;
+        if (at + kRunUnit + kAdamwBlock <= e) next.load(r, at + kRunUnit, kAdamwBlock);
+      } else {
+        now.load(r, at, kAdamwBlock);
+      }
+      adamw_block(r, s, now, at, kAdamwBlock);
+    }
+  };
+  if (vectors) whole(std::integral_constant<int, kUnits>{});
+  else whole(std::integral_constant<int, kAdamwApart>{});
+  if (at < e) {
+    AdamwBlock<P, G, BITS, kAdamwEnd> last;
+    last.load(r, at, static_cast<int>(e - at));
+    adamw_block(r, s, last, at, static_cast<int>(e - at));
+  }
 }
 
 template <int BITS, int K>
-__global__ void __launch_bounds__(kAdamwThreads, kAdamwResident)
+__global__ void __launch_bounds__(kAdamwThreads, adamw_resident(BITS))
     adamw_kernel(const __grid_constant__ AdamwTable<K> t) {
   __shared__ AdamwScalars s;
   grid_dependency_wait();
