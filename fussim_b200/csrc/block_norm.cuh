@@ -80,10 +80,6 @@ struct BlockParams {
   int sums;               // 2 (dz's alone) to 4
 };
 
-template <typename T> __device__ __forceinline__ T block_narrow(double v);
-template <> __device__ __forceinline__ __half block_narrow<__half>(double v) { return __double2half(v); }
-template <> __device__ __forceinline__ __nv_bfloat16 block_narrow<__nv_bfloat16>(double v) { return __double2bfloat16(v); }
-
 // Eight numbers, as the packed FP32 instructions take them.
 struct Eight {
   float2 p[4];
@@ -624,7 +620,8 @@ __global__ void __maxnreg__(block_forward_registers(V, MODE)) block_norm_forward
   __shared__ double2 slots[2 * 16];
   grid_dependency_wait();
   grid_launch_dependents();
-  // 16-bit results of a normalised branch are formed in FP64, and so rounded once in all but name
+  // 16-bit sums with a normalised branch are formed in FP64: FP32 steps would bring some of them (one in
+  // 2^16 for each) to the other side of a border of their type
   constexpr bool kWide = MODE == kBlockAfter && sizeof(X) == 2;
   const BlockPlace b = block_place<WARP>(p);
   constexpr bool kVec = UNIT > 1;
@@ -696,12 +693,12 @@ __global__ void __maxnreg__(block_forward_registers(V, MODE)) block_norm_forward
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             const double t = fma((u[i] - wide.x) * wide.y, static_cast<double>(w[i]), static_cast<double>(o[i]));
-            one[i] = block_narrow<X>(fma(t, p.s * g[i], static_cast<double>(r[v][i])));
+            one[i] = run_narrow<X>(static_cast<float>(fma(t, p.s * g[i], static_cast<double>(r[v][i]))));
           }
         } else {
 #pragma unroll
           for (int i = 0; i < 8; ++i)
-            one[i] = block_narrow<X>(fma(static_cast<double>(u[i]), p.s * g[i], static_cast<double>(r[v][i])));
+            one[i] = run_narrow<X>(static_cast<float>(fma(static_cast<double>(u[i]), p.s * g[i], static_cast<double>(r[v][i]))));
         }
       } else {
         if (after_norm) {
