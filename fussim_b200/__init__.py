@@ -9,8 +9,11 @@ Drop-in for the public API of OpsiClear/fussim (``fussim/__init__.py``):
 * ``SUPPORTED_WINDOW_SIZES``, ``get_build_info``, ``check_compatibility``.
 
 Beside the losses, operators of the training step around them: ``group_norm_act`` /
-``GroupNormAct`` (group normalisation with its activation, channels last) and ``grad_norm`` /
-``clip_grad_norm`` / ``clip_grad_norm_`` (the global gradient norm and clipping).
+``GroupNormAct`` (group normalisation with its activation, channels last), ``block_norm`` /
+``gated_residual`` / ``gated_residual_norm`` (the norms before and after a residual block, with its
+gate and modulation), ``grad_norm`` / ``clip_grad_norm`` / ``clip_grad_norm_`` (the global gradient
+norm and clipping) and ``adamw_step_`` / ``AdamW`` (the AdamW step of many tensors, with moments in
+32 or 8 bits).
 
 Gradients of the losses flow to the first image only. Under ``torch.autocast`` the inputs are rounded
 to FP16 (whatever the autocast dtype, as the reference does) and the arithmetic stays
@@ -38,9 +41,9 @@ from .functional import (  # noqa: F401
     poll_device_error,
     ssim,
 )
+from .optimizer import AdamW, adamw_moments, adamw_step_  # noqa: F401
 from .training import (  # noqa: F401
     GroupNormAct,
-    adamw_step_,
     clip_grad_norm,
     clip_grad_norm_,
     grad_norm,
@@ -64,6 +67,8 @@ __all__ = [
     "clip_grad_norm",
     "clip_grad_norm_",
     "adamw_step_",
+    "adamw_moments",
+    "AdamW",
     # Advanced/internal
     "FusedSSIMMap",
     "FusedSSIMMapFP16",

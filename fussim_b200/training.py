@@ -14,7 +14,7 @@ Like the losses they run hand-written sm_100a kernels and have no CPU path. The 
 
 from __future__ import annotations
 
-from typing import Iterable, List, Optional, Sequence, Tuple, Union
+from typing import Iterable, List, Optional, Sequence, Tuple
 
 import torch
 
@@ -142,61 +142,4 @@ def clip_grad_norm_(
         parameters = [parameters]
     return _ensure_cuda_extension().clip_grad_norm_(
         list(parameters), float(max_norm), error_if_nonfinite
-    )
-
-
-def adamw_step_(
-    params: Iterable[torch.Tensor],
-    grads: Iterable[torch.Tensor],
-    exp_avgs: Iterable[torch.Tensor],
-    exp_avg_sqs: Iterable[torch.Tensor],
-    scales: Optional[Iterable[torch.Tensor]] = None,
-    *,
-    step: Union[int, torch.Tensor],
-    lr: Union[float, torch.Tensor],
-    betas: Tuple[float, float] = (0.9, 0.999),
-    eps: float = 1e-8,
-    weight_decay: float = 1e-2,
-    maximize: bool = False,
-    max_norm: Optional[float] = None,
-    norm: Optional[torch.Tensor] = None,
-    copies: Optional[Iterable[torch.Tensor]] = None,
-    seed: int = 0,
-) -> Optional[torch.Tensor]:
-    """One AdamW step of many tensors, in place, in one launch for up to 448 of them.
-
-    With g a gradient (negated where ``maximize``)::
-
-        m = beta1 * m + (1 - beta1) * g            v = beta2 * v + (1 - beta2) * g^2
-        p = (1 - lr * weight_decay) * p
-            - lr / (1 - beta1^step) * m / (sqrt(v / (1 - beta2^step)) + eps)
-
-    in FP32, p rounded once to its type. ``params`` are dense CUDA tensors of one device, float32,
-    float16 or bfloat16; ``grads`` have their parameter's type or float32 (beside a float32
-    parameter also a 16-bit type). ``copies`` are 16-bit tensors that get float32 parameters
-    rounded: the weights that a mixed-precision model computes with.
-
-    ``exp_avgs`` and ``exp_avg_sqs`` hold m and v: float32 tensors, or float8_e4m3fn ones, all
-    with their parameter's shape and strides. Those of 8 bits hold codes of m and of the root of v,
-    and ``scales`` a float32 tensor (blocks, 2) for each parameter: column 0 for m, 1 for the
-    root, a row for each 256 numbers in the order of memory. A code stands for itself times its
-    scale, which is the block's largest finite number (at least 2^-100) / 448. A number goes to
-    one of its two neighbouring codes at random, in proportion (below 2^-6 scales to the nearest),
-    so that slow changes are kept on average; a root that is not zero is held as 2^-6 scales at
-    least; an infinite or NaN moment as NaN. The random bits are a hash of ``seed``, ``step``, the
-    tensor's position in the list and the number's in its tensor.
-
-    ``max_norm`` multiplies the gradients by min(1, max_norm / (norm + 1e-6)) on their way in
-    (``grads`` stay as they are) and returns the norm, that of all ``grads`` unless ``norm`` (one
-    float32 on the device) gives it; NaN makes everything NaN. Without it the result is None.
-    ``step`` counts from 1; it and ``lr`` may be one float32 on the device, for captured graphs:
-    they are then read when the work runs. No host synchronisation; results repeat bit for bit.
-    Tensors that are written must not share memory with any other: ValueError. A gradient whose
-    strides are not its parameter's is copied once more. Not differentiable; tracing raises
-    RuntimeError.
-    """
-    as_list = lambda v: None if v is None else list(v)  # noqa: E731
-    return _ensure_cuda_extension().adamw_step_(
-        list(params), list(grads), list(exp_avgs), list(exp_avg_sqs), as_list(scales), step, lr,
-        betas[0], betas[1], eps, weight_decay, maximize, max_norm, norm, as_list(copies), seed
     )

@@ -185,3 +185,27 @@ def test_c_null(lib):
     a = make()
     a.sizes = None
     assert lib.fssim_adamw_step(ctypes.byref(a), None) == NULLPTR
+
+
+# ---- the class ----
+@pytest.mark.parametrize("kw,match", [
+    (dict(state_bits=16), "state_bits"), (dict(lr=-1.0), "lr"), (dict(lr=float("nan")), "lr"),
+    (dict(lr=torch.tensor(1e-3)), "capturable"), (dict(betas=(1.0, 0.9)), "first of betas"),
+    (dict(betas=(0.9, 1.5)), "second of betas"), (dict(eps=-1.0), "eps"), (dict(weight_decay=-0.1), "weight_decay"),
+    (dict(max_norm=-1.0), "max_norm"), (dict(max_norm=float("nan")), "max_norm"), (dict(seed=-1), "seed"),
+    (dict(seed=1 << 32), "seed"),
+])
+def test_optimizer_refusals(kw, match):
+    with pytest.raises(ValueError, match=match):
+        fb.AdamW([torch.nn.Parameter(Z.clone())], **kw)
+
+
+def test_moments():
+    p = torch.zeros(3, 100, 2, 2).to(memory_format=torch.channels_last)
+    for bits, dtype in ((32, torch.float32), (8, F8)):
+        first, second, scales = fb.adamw_moments(p.half(), bits)
+        for t in (first, second):
+            assert t.dtype == dtype and t.shape == p.shape and t.stride() == p.stride() and not t.float().any()
+        assert scales is None if bits == 32 else scales.shape == (5, 2)
+    with pytest.raises(ValueError, match="bits"):
+        fb.adamw_moments(p, 4)
