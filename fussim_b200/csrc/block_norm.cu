@@ -112,7 +112,8 @@ Layout layout(const Shape& s, bool backward, int mode, bool per_sample, bool vec
         t = (t + 31) / 32 * 32;
         if (t > (backward && g <= 2 ? 384 : kBlockMaxThreads)) continue;  // (registers)
       }
-      if (t * g <= padded) {
+      // (the kernels count on whole groups but for a row's last)
+      if ((g - 1) * t < needed && t * g <= padded) {
         padded = t * g;
         l.groups = g;
         l.threads = t;

@@ -123,17 +123,20 @@ struct alignas(16) BlockPacked {
 // A thread's place in a row: number i of its group v is in column at(v, i). Columns go out to the row's
 // threads in turn by units that are 16 bytes of x: eight numbers of 16 bits, four of 32 (so that
 // the threads' accesses lie side by side); single numbers where rows begin at no vector's boundary.
-template <int UNIT>
+// The last of the V groups alone may lack some.
+template <int UNIT, int V>
 struct BlockColumns {
   int threads, tid, C;
-  bool full;  // every group has all its numbers
+  bool full;  // the last group has all its numbers, too
   __device__ __forceinline__ int at(int v, int i) const {
     return ((v * 8 + i) / UNIT * threads + tid) * UNIT + i % UNIT;
   }
-  __device__ __forceinline__ bool inside(int v, int i) const { return at(v, i / UNIT * UNIT) < C; }
+  __device__ __forceinline__ bool inside(int v, int i) const {
+    return v < V - 1 || full || at(v, i / UNIT * UNIT) < C;
+  }
   // Zeros in place of what is past the row's end.
   __device__ __forceinline__ Eight keep(Eight f, int v) const {
-    if (!full)
+    if (v == V - 1 && !full)
 #pragma unroll
       for (int i = 0; i < 8; ++i) f[i] = inside(v, i) ? f[i] : 0.f;
     return f;
@@ -176,13 +179,13 @@ struct BlockRow {
   T one[kVec ? 1 : V * 8];
 
   static __device__ __forceinline__ void copy(unsigned char* slot, const void* from, int64_t offset,
-                                              const BlockColumns<UNIT>& c, bool active) {
+                                              const BlockColumns<UNIT, V>& c, bool active) {
     const unsigned to = static_cast<unsigned>(__cvta_generic_to_shared(slot)) + threadIdx.x % 32 * kPiece;
     const T* row = static_cast<const T*>(from) + offset;
 #pragma unroll
     for (int k = 0; k < kPieces; ++k) {
       const int at = c.at(0, k * UNIT);
-      const bool ok = active && (c.full || at < c.C);
+      const bool ok = active && c.inside(k * UNIT / 8, k * UNIT % 8);
       const T* src = ok ? row + at : static_cast<const T*>(from);
       if constexpr (kPiece == 16)
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + k * 512), "l"(src), "r"(ok ? 16 : 0)
@@ -192,11 +195,11 @@ struct BlockRow {
                      : "memory");
     }
   }
-  __device__ __forceinline__ void load(const void* from, int64_t offset, const BlockColumns<UNIT>& c, bool active) {
+  __device__ __forceinline__ void load(const void* from, int64_t offset, const BlockColumns<UNIT, V>& c, bool active) {
 #pragma unroll
     for (int i = 0; i < V * 8; ++i) {
       const int at = c.at(0, i);
-      one[i] = active && at < c.C ? static_cast<const T*>(from)[offset + at] : run_narrow<T>(0.f);
+      one[i] = active && c.inside(i / 8, i % 8) ? static_cast<const T*>(from)[offset + at] : run_narrow<T>(0.f);
     }
   }
   // Group v.
@@ -219,14 +222,14 @@ struct BlockRow {
 };
 
 // Group v to a row.
-template <typename T, int UNIT>
-__device__ __forceinline__ void block_store(void* to, int64_t offset, const BlockColumns<UNIT>& c, int v,
+template <typename T, int UNIT, int V>
+__device__ __forceinline__ void block_store(void* to, int64_t offset, const BlockColumns<UNIT, V>& c, int v,
                                             const BlockPacked<T>& e) {
   T* row = static_cast<T*>(to) + offset;
 #pragma unroll
   for (int i = 0; i < 8; i += UNIT) {
     const int at = c.at(v, i);
-    if (!c.full && at >= c.C) continue;
+    if (!c.inside(v, i)) continue;
     if constexpr (UNIT * sizeof(T) == 32) {  // (FP32 sums of eight columns)
       reinterpret_cast<uint4*>(row + at)[0] = reinterpret_cast<const uint4*>(&e)[0];
       reinterpret_cast<uint4*>(row + at)[1] = reinterpret_cast<const uint4*>(&e)[1];
@@ -377,7 +380,7 @@ __device__ __noinline__ void block_stage(const BlockParams& p, int64_t sample, f
   __syncthreads();
 }
 
-template <int UNIT, bool WIDE, bool BACKWARD, bool STAGED>
+template <int UNIT, int V, bool WIDE, bool BACKWARD, bool STAGED>
 struct BlockArrays {
   const BlockParams& p;
   float* memory;
@@ -387,7 +390,7 @@ struct BlockArrays {
     if constexpr (STAGED) block_stage<UNIT, WIDE, BACKWARD>(p, sample, memory);
   }
   // Group v of a thread.
-  __device__ __forceinline__ Eight get(int array, const BlockColumns<UNIT>& c, int v, float constant) const {
+  __device__ __forceinline__ Eight get(int array, const BlockColumns<UNIT, V>& c, int v, float constant) const {
     if (!(p.arrays >> array & 1)) return eight(constant);
     Eight f;
     if constexpr (STAGED) {
@@ -397,7 +400,8 @@ struct BlockArrays {
         const float4* q = reinterpret_cast<const float4*>(at);
         const int first = UNIT == 8 ? v * c.threads + c.tid : 2 * v * c.threads + c.tid, second = first + c.threads;
         const int last = c.C / UNIT - 1;
-        const float4 a = q[min(first, last)], b = UNIT == 8 ? q[c.C / 8 + min(first, last)] : q[min(second, last)];
+        const auto in = [&](int g) { return v < V - 1 ? g : min(g, last); };
+        const float4 a = q[in(first)], b = UNIT == 8 ? q[c.C / 8 + in(first)] : q[in(second)];
         f.p[0] = make_float2(a.x, a.y), f.p[1] = make_float2(a.z, a.w);
         f.p[2] = make_float2(b.x, b.y), f.p[3] = make_float2(b.z, b.w);
       } else {
@@ -468,7 +472,7 @@ struct BlockTeam {
 // their own mean.
 template <bool SCALED, int V, int UNIT, bool WARP>
 __device__ __forceinline__ float2 block_moments(BlockTeam<WARP>& team, const Eight (&f)[V], int kind, float by,
-                                                const BlockColumns<UNIT>& c) {
+                                                const BlockColumns<UNIT, V>& c) {
   const auto at = [&](int v, int i) { return SCALED ? __fmul2_rn(f[v].p[i], twice(by)) : f[v].p[i]; };
   if (kind == kBlockRms) {
     float2 q[2] = {};
@@ -529,7 +533,7 @@ __device__ __forceinline__ float2 block_moments(BlockTeam<WARP>& team, const Eig
 // scaled by a power of two.
 template <int V, int UNIT, bool WARP>
 __device__ __forceinline__ float2 block_stats(BlockTeam<WARP>& team, const Eight (&f)[V], int kind, float eps,
-                                              const BlockColumns<UNIT>& c) {
+                                              const BlockColumns<UNIT, V>& c) {
   const float2 m = block_moments<false, V, UNIT, WARP>(team, f, kind, 1.f, c);
   const bool large = m.y > 0x1p120f, again = large || (m.y < 0x1p-80f && eps < 0x1p-90f);
   const float inv = 1.f / c.C;
@@ -546,7 +550,7 @@ __device__ __forceinline__ float2 block_stats(BlockTeam<WARP>& team, const Eight
 // kind): these and their squares are exact, or nearly so, of 16-bit numbers.
 template <int V, int UNIT, bool WARP>
 __device__ __forceinline__ double2 block_stats_wide(BlockTeam<WARP>& team, const Eight (&f)[V], int kind, float eps,
-                                                    double inv, const BlockColumns<UNIT>& c) {
+                                                    double inv, const BlockColumns<UNIT, V>& c) {
   const int lane = threadIdx.x % 32;
   double pivot = 0.0;
   if (kind == kBlockLayer) {
@@ -564,7 +568,7 @@ __device__ __forceinline__ double2 block_stats_wide(BlockTeam<WARP>& team, const
   for (int v = 0; v < V; ++v)
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      if (c.full || c.inside(v, i)) {
+      if (c.inside(v, i)) {
         const double d = static_cast<double>(f[v][i]) - pivot;
         sums.x += d;
         sums.y = fma(d, d, sums.y);
@@ -595,7 +599,7 @@ __device__ __forceinline__ BlockPlace block_place(const BlockParams& p) {
 }
 
 template <int V, int UNIT, bool WARP>
-__device__ __forceinline__ BlockTeam<WARP> block_team(const BlockParams& p, const BlockColumns<UNIT>& c, double2* slots) {
+__device__ __forceinline__ BlockTeam<WARP> block_team(const BlockParams& p, const BlockColumns<UNIT, V>& c, double2* slots) {
   BlockTeam<WARP> team{p.threads, p.threads / 32, 1, slots, static_cast<float>(p.C), 1.f / p.C};
   if constexpr (!WARP) {
     while (team.span < team.warps) team.span *= 2;
@@ -625,7 +629,7 @@ __global__ void __maxnreg__(block_forward_registers(V, MODE)) block_norm_forward
   constexpr bool kWide = MODE == kBlockAfter && sizeof(X) == 2;
   const BlockPlace b = block_place<WARP>(p);
   constexpr bool kVec = UNIT > 1;
-  const BlockColumns<UNIT> c{p.threads, b.tid, p.C, V * 8 * p.threads == p.C};
+  const BlockColumns<UNIT, V> c{p.threads, b.tid, p.C, V * 8 * p.threads == p.C};
   const int C = p.C;
   BlockTeam<WARP> team = block_team<V, UNIT, WARP>(p, c, slots);
   const bool branch = MODE == kBlockPlain || (MODE == kBlockAfter && p.y);
@@ -649,7 +653,7 @@ __global__ void __maxnreg__(block_forward_registers(V, MODE)) block_norm_forward
   };
   if constexpr (kVec)
     for (int k = 1; k < p.stages; ++k) fetch();
-  const BlockArrays<UNIT, kWide, false, STAGED> arrays{p, reinterpret_cast<float*>(block_memory + (kVec ? p.stages * ring.bytes : 0)),
+  const BlockArrays<UNIT, V, kWide, false, STAGED> arrays{p, reinterpret_cast<float*>(block_memory + (kVec ? p.stages * ring.bytes : 0)),
                                               b.sample};
   arrays.stage();
   const float s = static_cast<float>(p.s);
@@ -735,7 +739,7 @@ __global__ void __maxnreg__(block_backward_registers(V)) block_norm_backward_ker
   grid_launch_dependents();
   const BlockPlace b = block_place<WARP>(p);
   constexpr bool kVec = UNIT > 1;
-  const BlockColumns<UNIT> c{p.threads, b.tid, p.C, V * 8 * p.threads == p.C};
+  const BlockColumns<UNIT, V> c{p.threads, b.tid, p.C, V * 8 * p.threads == p.C};
   const int C = p.C;
   BlockTeam<WARP> team = block_team<V, UNIT, WARP>(p, c, slots);
   const bool branch = MODE == kBlockPlain || (MODE == kBlockAfter && p.y);
@@ -766,7 +770,7 @@ __global__ void __maxnreg__(block_backward_registers(V)) block_norm_backward_ker
   };
   if constexpr (kVec)
     for (int k = 1; k < p.stages; ++k) fetch();
-  const BlockArrays<UNIT, false, true, STAGED> arrays{p, reinterpret_cast<float*>(block_memory + (kVec ? p.stages * ring.bytes : 0)),
+  const BlockArrays<UNIT, V, false, true, STAGED> arrays{p, reinterpret_cast<float*>(block_memory + (kVec ? p.stages * ring.bytes : 0)),
                                              b.sample};
   arrays.stage();
   constexpr int kSums = MODE == kBlockBefore ? 2 : MODE == kBlockPlain ? 3 : 4;
