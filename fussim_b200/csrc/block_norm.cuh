@@ -618,6 +618,9 @@ constexpr int block_forward_registers(int v, int mode) { return mode == kBlockAf
 constexpr int block_backward_registers(int v) { return v > 2 ? 128 : 168; }
 constexpr int block_resident(int registers) { return 65536 / registers / 32 * 32; }
 
+// Bound by DRAM where rows are many: 16384 x 4096 BF16 (RMS alone, 268 MB) 50 us, 5.4 TB/s; 16 x 1024 rows
+// of 1024 with a 32-bit residual (201 MB) 40 us; 8 x 1024 x 1152 BF16 (76 MB, four rows a warp) 20 us, of
+// which the arrays' and the first rows' way from memory takes a quarter. A single row of 2048: 6 us, latency.
 template <typename X, typename Y, int V, int UNIT, bool WARP, int MODE, bool STAGED>
 __global__ void __maxnreg__(block_forward_registers(V, MODE)) block_norm_forward_kernel(const __grid_constant__ BlockParams p) {
   extern __shared__ __align__(16) unsigned char block_memory[];
@@ -636,23 +639,28 @@ __global__ void __maxnreg__(block_forward_registers(V, MODE)) block_norm_forward
   const bool after_norm = MODE == kBlockAfter && p.after_kind;
   using RowX = BlockRow<X, V, UNIT>;
   using RowY = BlockRow<Y, V, UNIT>;
-  RowX row_x;
-  RowY row_y;
+  // (number by number: a row is held, and the next on its way, in registers)
+  RowX row_x, next_x;
+  RowY row_y, next_y;
   constexpr int at_y = RowX::kBytes;
   BlockRing ring(block_memory, RowX::kBytes + (branch ? RowY::kBytes : 0), p.stages);
   int64_t ahead = b.row0 + b.part;
   const auto fetch = [&] {
-    unsigned char* slot = ring.next(ring.put);
     const bool active = ahead < b.row1;
-    if (WARP || active) {
-      RowX::copy(slot, p.x, ahead * C, c, active);
-      if (branch) RowY::copy(slot + at_y, p.y, ahead * C, c, active);
+    if constexpr (kVec) {
+      unsigned char* slot = ring.next(ring.put);
+      if (WARP || active) {
+        RowX::copy(slot, p.x, ahead * C, c, active);
+        if (branch) RowY::copy(slot + at_y, p.y, ahead * C, c, active);
+      }
+      ring.commit();
+    } else {
+      next_x.load(p.x, ahead * C, c, active);
+      if (branch) next_y.load(p.y, ahead * C, c, active);
     }
-    ring.commit();
     ahead += b.parts;
   };
-  if constexpr (kVec)
-    for (int k = 1; k < p.stages; ++k) fetch();
+  for (int k = kVec ? 1 : 0; k < (kVec ? p.stages : 1); ++k) fetch();
   const BlockArrays<UNIT, V, kWide, false, STAGED> arrays{p, reinterpret_cast<float*>(block_memory + (kVec ? p.stages * ring.bytes : 0)),
                                               b.sample};
   arrays.stage();
@@ -666,8 +674,9 @@ __global__ void __maxnreg__(block_forward_registers(V, MODE)) block_norm_forward
       ring.wait();
       slot = ring.next(ring.get);
     } else {
-      row_x.load(p.x, offset, c, active);
-      if (branch) row_y.load(p.y, offset, c, active);
+      row_x = next_x;
+      if (branch) row_y = next_y;
+      fetch();
     }
     Eight r[V];
     float2 after = make_float2(0.f, 1.f);
@@ -731,6 +740,9 @@ __global__ void __maxnreg__(block_forward_registers(V, MODE)) block_norm_forward
   }
 }
 
+// Bound by DRAM: 16 x 1024 rows of 1024 with a 32-bit residual (302 MB) 51 us, 8 x 16384 x 96 FP32 (as
+// much) 50 us, 6.0 TB/s. The numbers are read from the ring for each of up to three turns (sums, dR, dy),
+// so that the four sums can stay in registers.
 template <typename X, typename Y, int V, int UNIT, bool WARP, int MODE, bool STAGED>
 __global__ void __maxnreg__(block_backward_registers(V)) block_norm_backward_kernel(const __grid_constant__ BlockParams p) {
   extern __shared__ __align__(16) unsigned char block_memory[];
@@ -747,29 +759,40 @@ __global__ void __maxnreg__(block_backward_registers(V)) block_norm_backward_ker
   const bool has_dr = MODE != kBlockBefore && p.dr, has_dz = MODE == kBlockBefore || p.dz;
   using RowX = BlockRow<X, V, UNIT>;
   using RowY = BlockRow<Y, V, UNIT>;
-  RowX row_r, row_dr;
-  RowY row_y, row_dz;
+  RowX row_r, row_dr, next_r, next_dr;
+  RowY row_y, row_dz, next_y, next_dz;
   // places in a warp's part of a stage: r, dz, dr, y
   constexpr int at_dz = RowX::kBytes, at_dr = at_dz + RowY::kBytes, at_y = at_dr + (MODE == kBlockBefore ? 0 : RowX::kBytes);
   BlockRing ring(block_memory, at_y + (MODE == kBlockBefore ? 0 : RowY::kBytes), p.stages);
   int64_t ahead = b.row0 + b.part;
+  // (number by number: the next row into registers where a thread has eight numbers of it)
+  constexpr bool kAhead = kVec || V == 1;
   const auto fetch = [&] {
-    unsigned char* slot = ring.next(ring.put);
     const bool active = ahead < b.row1;
-    if (WARP || active) {
-      const int64_t offset = ahead * C;
-      if (has_dz) {
-        RowX::copy(slot, p.r, offset, c, active);
-        RowY::copy(slot + at_dz, p.dz, offset, c, active);
+    const int64_t offset = ahead * C;
+    if constexpr (kVec) {
+      unsigned char* slot = ring.next(ring.put);
+      if (WARP || active) {
+        if (has_dz) {
+          RowX::copy(slot, p.r, offset, c, active);
+          RowY::copy(slot + at_dz, p.dz, offset, c, active);
+        }
+        if (has_dr) RowX::copy(slot + at_dr, p.dr, offset, c, active);
+        if (branch) RowY::copy(slot + at_y, p.y, offset, c, active);
       }
-      if (has_dr) RowX::copy(slot + at_dr, p.dr, offset, c, active);
-      if (branch) RowY::copy(slot + at_y, p.y, offset, c, active);
+      ring.commit();
+    } else {
+      if (has_dz) {
+        next_r.load(p.r, offset, c, active);
+        next_dz.load(p.dz, offset, c, active);
+      }
+      if (has_dr) next_dr.load(p.dr, offset, c, active);
+      if (branch) next_y.load(p.y, offset, c, active);
     }
-    ring.commit();
     ahead += b.parts;
   };
-  if constexpr (kVec)
-    for (int k = 1; k < p.stages; ++k) fetch();
+  if constexpr (kAhead)
+    for (int k = kVec ? 1 : 0; k < (kVec ? p.stages : 1); ++k) fetch();
   const BlockArrays<UNIT, V, false, true, STAGED> arrays{p, reinterpret_cast<float*>(block_memory + (kVec ? p.stages * ring.bytes : 0)),
                                              b.sample};
   arrays.stage();
@@ -798,12 +821,12 @@ __global__ void __maxnreg__(block_backward_registers(V)) block_norm_backward_ker
       ring.wait();
       slot = ring.next(ring.get);
     } else {
-      if (has_dz) {
-        row_r.load(p.r, offset, c, active);
-        row_dz.load(p.dz, offset, c, active);
-      }
-      if (has_dr) row_dr.load(p.dr, offset, c, active);
-      if (branch) row_y.load(p.y, offset, c, active);
+      if constexpr (!kAhead) fetch();
+      row_r = next_r;
+      row_dz = next_dz;
+      row_dr = next_dr;
+      row_y = next_y;
+      if constexpr (kAhead) fetch();
     }
     const auto get_rhat = [&](int v) {
       return pairs([&](float2 a) { return __fmul2_rn(__fadd2_rn(a, twice(-s1.x)), twice(s1.y)); }, row_r.get(slot, v));

@@ -61,21 +61,21 @@ int block_backward(const BlockLaunch& l, const fssim::BlockParams& p, cudaStream
   return st ? st : launch(kernel, l.grid, l.block, l.memory, stream, "block norm backward launch", p);
 }
 
-// Which kernels there are: see layout() in block_norm.cu. Kernels of one mode alone for rows of whole
-// vectors, one for all modes elsewhere.
-template <typename X, typename Y, int V, bool WARP>
+// Which kernels there are: see layout() in block_norm.cu. Kernels of one mode alone, and one for all
+// modes for the longest rows.
+template <typename X, typename Y, int V, bool WARP, bool VEC = true>
 int block_forward_mode(const BlockLaunch& l, const fssim::BlockParams& p, cudaStream_t stream) {
   using namespace fssim;
-  if (l.mode == kBlockBefore) return block_forward<X, Y, V, true, WARP, kBlockBefore>(l, p, stream);
-  if (l.mode == kBlockPlain) return block_forward<X, Y, V, true, WARP, kBlockPlain>(l, p, stream);
-  return block_forward<X, Y, V, true, WARP, kBlockAfter>(l, p, stream);
+  if (l.mode == kBlockBefore) return block_forward<X, Y, V, VEC, WARP, kBlockBefore>(l, p, stream);
+  if (l.mode == kBlockPlain) return block_forward<X, Y, V, VEC, WARP, kBlockPlain>(l, p, stream);
+  return block_forward<X, Y, V, VEC, WARP, kBlockAfter>(l, p, stream);
 }
-template <typename X, typename Y, int V, bool WARP>
+template <typename X, typename Y, int V, bool WARP, bool VEC = true>
 int block_backward_mode(const BlockLaunch& l, const fssim::BlockParams& p, cudaStream_t stream) {
   using namespace fssim;
-  if (l.mode == kBlockBefore) return block_backward<X, Y, V, true, WARP, kBlockBefore>(l, p, stream);
-  if (l.mode == kBlockPlain) return block_backward<X, Y, V, true, WARP, kBlockPlain>(l, p, stream);
-  return block_backward<X, Y, V, true, WARP, kBlockAfter>(l, p, stream);
+  if (l.mode == kBlockBefore) return block_backward<X, Y, V, VEC, WARP, kBlockBefore>(l, p, stream);
+  if (l.mode == kBlockPlain) return block_backward<X, Y, V, VEC, WARP, kBlockPlain>(l, p, stream);
+  return block_backward<X, Y, V, VEC, WARP, kBlockAfter>(l, p, stream);
 }
 
 template <typename X, typename Y>
@@ -83,8 +83,8 @@ int block_norm_types(bool backward, const BlockLaunch& l, const fssim::BlockPara
   using fssim::kBlockAfter;
   if (backward) {
     if (!l.vec)
-      return l.warp          ? block_backward<X, Y, 1, false, true, kBlockAfter>(l, p, stream)
-             : l.groups == 1 ? block_backward<X, Y, 1, false, false, kBlockAfter>(l, p, stream)
+      return l.warp          ? block_backward_mode<X, Y, 1, true, false>(l, p, stream)
+             : l.groups == 1 ? block_backward_mode<X, Y, 1, false, false>(l, p, stream)
                              : block_backward<X, Y, 4, false, false, kBlockAfter, false>(l, p, stream);
     if (l.groups == 4)
       return l.staged ? block_backward<X, Y, 4, true, false, kBlockAfter>(l, p, stream)
@@ -96,8 +96,8 @@ int block_norm_types(bool backward, const BlockLaunch& l, const fssim::BlockPara
                          : block_backward_mode<X, Y, 2, false>(l, p, stream);
   }
   if (!l.vec)
-    return l.warp          ? block_forward<X, Y, 1, false, true, kBlockAfter>(l, p, stream)
-           : l.groups == 1 ? block_forward<X, Y, 1, false, false, kBlockAfter>(l, p, stream)
+    return l.warp          ? block_forward_mode<X, Y, 1, true, false>(l, p, stream)
+           : l.groups == 1 ? block_forward_mode<X, Y, 1, false, false>(l, p, stream)
                            : block_forward<X, Y, 4, false, false, kBlockAfter, false>(l, p, stream);
   if (!l.staged) return block_forward<X, Y, 4, true, false, kBlockAfter, false>(l, p, stream);
   if (l.warp) {

@@ -37,8 +37,8 @@ __device__ __forceinline__ void block_put(const BlockGrad& g, int64_t at, double
 // A CTA has eight columns (a sector of 32 bytes) of a split's samples. Its 32 teams of a thread for each
 // column share the samples: several a team, or a power of two of teams a sample, which have its CTAs'
 // sums in turn. Latency is all there is to it: several CTAs' sums are asked for before any is added, and
-// few threads go through the rest (64 teams of 16 columns, with a CTA's share of everything in each of 32
-// warps: 12.7 us for 444 sums of 3 x 96 that lie in L2).
+// few threads go through the rest (444 sums of 3 x 96 that lie in L2: 7.1 us; 12.7 with 64 teams of 16
+// columns in 32 warps; 864 of 3 x 1024: 8.7 us).
 template <int SUMS>
 __global__ void __launch_bounds__(kBlockMergeColumns * kBlockMergeTeams)
     block_norm_grads_kernel(const __grid_constant__ BlockGradParams p) {

@@ -10,7 +10,8 @@ root by half; a normalised number h = (v - mean) * rstd by
     D(v) = rstd E + |h| (k / 2 + 8) u.
 
 Sums of products whose factors are off add those factors' errors. A vector's gradient is a sum over
-rows, in FP32 over at most 256 of them: n = min(rows, 256) + 10 roundings of the magnitudes' sum. Each
+rows, in FP32 over at most 256 of them in a thread, five steps in its warp, eight warps and three steps
+between CTAs, FP64 beyond: n = min(rows, 256) + 16 roundings of the magnitudes' sum. Each
 result adds half a step of its type; z is compared with the norm of the r that was returned.
 """
 
@@ -151,7 +152,7 @@ def check(d, form, r, z, kind="rms", branch_kind=None, s=1.0, eps=EPS, ups=None,
         if name not in grads:
             return
         over = rows[1:] if d[name].dim() == 2 else rows
-        n = min(x.numel() // x.shape[-1], 256) + 10
+        n = min(x.numel() // x.shape[-1], 256) + 16
         want = terms.sum(over) if over else terms
         off = n * U * terms.abs() + off
         near(name, grads[name], want, off.sum(over) if over else off)
