@@ -176,7 +176,8 @@ struct BlockRow {
   static constexpr bool kVec = UNIT > 1;
   static constexpr int kPiece = UNIT * sizeof(T), kPieces = V * 8 / UNIT;  // bytes of a unit, units of a thread
   static constexpr int kBytes = kVec ? kPieces * kPiece * 32 : 0;          // of a warp's part of a stage
-  T one[kVec ? 1 : V * 8];
+  // (a register for each, also of 16-bit numbers: to pack two the loads would have to be waited for)
+  unsigned one[kVec ? 1 : V * 8];
 
   static __device__ __forceinline__ void copy(unsigned char* slot, const void* from, int64_t offset,
                                               const BlockColumns<UNIT, V>& c, bool active) {
@@ -195,15 +196,15 @@ struct BlockRow {
                      : "memory");
     }
   }
-  __device__ __forceinline__ void load(const void* from, int64_t offset, const BlockColumns<UNIT, V>& c, bool active) {
+  // (without conditions, at places that are in the tensor: a load behind a branch is waited for there)
+  __device__ __forceinline__ void load(const void* from, int64_t offset, const BlockColumns<UNIT, V>& c) {
+    using Bits = std::conditional_t<sizeof(T) == 4, unsigned, unsigned short>;
+    const Bits* at = static_cast<const Bits*>(from) + offset;
 #pragma unroll
-    for (int i = 0; i < V * 8; ++i) {
-      const int at = c.at(0, i);
-      one[i] = active && c.inside(i / 8, i % 8) ? static_cast<const T*>(from)[offset + at] : run_narrow<T>(0.f);
-    }
+    for (int i = 0; i < V * 8; ++i) one[i] = at[min(c.at(0, i), c.C - 1)];
   }
-  // Group v.
-  __device__ __forceinline__ Eight get(const unsigned char* slot, int v) const {
+  // Group v; zeros where there are no numbers.
+  __device__ __forceinline__ Eight get(const unsigned char* slot, int v, const BlockColumns<UNIT, V>& c, bool active) const {
     if constexpr (kVec) {
       using Piece = std::conditional_t<kPiece == 16, uint4, uint2>;
       constexpr int per = 8 / UNIT;
@@ -215,7 +216,14 @@ struct BlockRow {
     } else {
       Eight f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] = run_widen(one[v * 8 + i]);
+      for (int i = 0; i < 8; ++i) {
+        const unsigned bits = one[v * 8 + i];
+        float value;
+        if constexpr (sizeof(T) == 4) value = __uint_as_float(bits);
+        else if constexpr (std::is_same_v<T, __half>) value = __half2float(__ushort_as_half(static_cast<unsigned short>(bits)));
+        else value = __uint_as_float(bits << 16);
+        f[i] = active && c.inside(v, i) ? value : 0.f;
+      }
       return f;
     }
   }
@@ -238,7 +246,7 @@ __device__ __forceinline__ void block_store(void* to, int64_t offset, const Bloc
     } else if constexpr (UNIT > 1) {
       *reinterpret_cast<uint2*>(row + at) = reinterpret_cast<const uint2*>(&e)[i / UNIT];
     } else {
-      row[at] = reinterpret_cast<const T*>(&e)[i];
+      row[at] = i & 1 ? e.p[i / 2].y : e.p[i / 2].x;
     }
   }
 }
@@ -406,7 +414,7 @@ struct BlockArrays {
         f.p[2] = make_float2(b.x, b.y), f.p[3] = make_float2(b.z, b.w);
       } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = c.inside(v, i) ? at[c.at(v, i)] : 0.f;
+        for (int i = 0; i < 8; ++i) f[i] = at[min(c.at(v, i), c.C - 1)];
       }
     } else {
       float t[8];  // (of its own: what is passed to a function lies in local memory)
@@ -655,8 +663,9 @@ __global__ void __maxnreg__(block_forward_registers(V, MODE)) block_norm_forward
       }
       ring.commit();
     } else {
-      next_x.load(p.x, ahead * C, c, active);
-      if (branch) next_y.load(p.y, ahead * C, c, active);
+      const int64_t offset = (active ? ahead : b.row0) * C;
+      next_x.load(p.x, offset, c);
+      if (branch) next_y.load(p.y, offset, c);
     }
     ahead += b.parts;
   };
@@ -683,7 +692,7 @@ __global__ void __maxnreg__(block_forward_registers(V, MODE)) block_norm_forward
     double2 wide = make_double2(0.0, 1.0);
     if (after_norm) {
 #pragma unroll
-      for (int v = 0; v < V; ++v) r[v] = row_y.get(slot + at_y, v);
+      for (int v = 0; v < V; ++v) r[v] = row_y.get(slot + at_y, v, c, active);
       if constexpr (kWide) {
         wide = block_stats_wide<V, UNIT, WARP>(team, r, p.after_kind, p.eps, p.inv, c);
         after = make_float2(static_cast<float>(wide.x), static_cast<float>(wide.y));
@@ -694,24 +703,24 @@ __global__ void __maxnreg__(block_forward_registers(V, MODE)) block_norm_forward
     }
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      r[v] = row_x.get(slot, v);
+      r[v] = row_x.get(slot, v, c, active);
       if (!branch) continue;
-      Eight u = row_y.get(slot + at_y, v);
+      Eight u = row_y.get(slot + at_y, v, c, active);
       const Eight g = arrays.get(kArrayGate, c, v, kWide ? 1.f : s);
       BlockPacked<X> e;
       if constexpr (kWide) {
-        X* one = reinterpret_cast<X*>(&e);
+        const auto one = [&](int i) -> X& { return i & 1 ? e.p[i / 2].y : e.p[i / 2].x; };
         if (after_norm) {
           const Eight w = arrays.get(kArrayAfterWeight, c, v, 1.f), o = arrays.get(kArrayAfterBias, c, v, 0.f);
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             const double t = fma((u[i] - wide.x) * wide.y, static_cast<double>(w[i]), static_cast<double>(o[i]));
-            one[i] = run_narrow<X>(static_cast<float>(fma(t, p.s * g[i], static_cast<double>(r[v][i]))));
+            one(i) = run_narrow<X>(static_cast<float>(fma(t, p.s * g[i], static_cast<double>(r[v][i]))));
           }
         } else {
 #pragma unroll
           for (int i = 0; i < 8; ++i)
-            one[i] = run_narrow<X>(static_cast<float>(fma(static_cast<double>(u[i]), p.s * g[i], static_cast<double>(r[v][i]))));
+            one(i) = run_narrow<X>(static_cast<float>(fma(static_cast<double>(u[i]), p.s * g[i], static_cast<double>(r[v][i]))));
         }
       } else {
         if (after_norm) {
@@ -769,7 +778,7 @@ __global__ void __maxnreg__(block_backward_registers(V)) block_norm_backward_ker
   constexpr bool kAhead = kVec || V == 1;
   const auto fetch = [&] {
     const bool active = ahead < b.row1;
-    const int64_t offset = ahead * C;
+    const int64_t offset = (kVec || active ? ahead : b.row0) * C;
     if constexpr (kVec) {
       unsigned char* slot = ring.next(ring.put);
       if (WARP || active) {
@@ -783,11 +792,11 @@ __global__ void __maxnreg__(block_backward_registers(V)) block_norm_backward_ker
       ring.commit();
     } else {
       if (has_dz) {
-        next_r.load(p.r, offset, c, active);
-        next_dz.load(p.dz, offset, c, active);
+        next_r.load(p.r, offset, c);
+        next_dz.load(p.dz, offset, c);
       }
-      if (has_dr) next_dr.load(p.dr, offset, c, active);
-      if (branch) next_y.load(p.y, offset, c, active);
+      if (has_dr) next_dr.load(p.dr, offset, c);
+      if (branch) next_y.load(p.y, offset, c);
     }
     ahead += b.parts;
   };
@@ -829,10 +838,10 @@ __global__ void __maxnreg__(block_backward_registers(V)) block_norm_backward_ker
       if constexpr (kAhead) fetch();
     }
     const auto get_rhat = [&](int v) {
-      return pairs([&](float2 a) { return __fmul2_rn(__fadd2_rn(a, twice(-s1.x)), twice(s1.y)); }, row_r.get(slot, v));
+      return pairs([&](float2 a) { return __fmul2_rn(__fadd2_rn(a, twice(-s1.x)), twice(s1.y)); }, row_r.get(slot, v, c, active));
     };
     const auto get_yhat = [&](int v) {
-      const Eight y = row_y.get(slot + at_y, v);
+      const Eight y = row_y.get(slot + at_y, v, c, active);
       return after_norm ? pairs([&](float2 a) { return __fmul2_rn(__fadd2_rn(a, twice(-s2.x)), twice(s2.y)); }, y) : y;
     };
     const auto times = [](float2 a, float2 b2) { return __fmul2_rn(a, b2); };
@@ -842,7 +851,7 @@ __global__ void __maxnreg__(block_backward_registers(V)) block_norm_backward_ker
 #pragma unroll
       for (int v = 0; v < V; ++v) {
         // (past the row's end dz is zero, and so are its products)
-        const Eight h = get_rhat(v), dz = row_dz.get(slot + at_dz, v);
+        const Eight h = get_rhat(v), dz = row_dz.get(slot + at_dz, v, c, active);
         const Eight a = pairs(times, dz, arrays.get(kArrayFactor, c, v, 1.f));
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -860,10 +869,10 @@ __global__ void __maxnreg__(block_backward_registers(V)) block_norm_backward_ker
     float2 mean[2] = {};
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      Eight d = has_dr ? row_dr.get(slot + at_dr, v) : eight(0.f);
+      Eight d = has_dr ? row_dr.get(slot + at_dr, v, c, active) : eight(0.f);
       if (has_dz) {
         const Eight h = get_rhat(v);
-        const Eight a = pairs(times, row_dz.get(slot + at_dz, v), arrays.get(kArrayFactor, c, v, 1.f));
+        const Eight a = pairs(times, row_dz.get(slot + at_dz, v, c, active), arrays.get(kArrayFactor, c, v, 1.f));
         d = pairs([&](float2 d2, float2 a2, float2 h2) {
           return __ffma2_rn(twice(s1.y), __ffma2_rn(h2, twice(-m2), __fadd2_rn(a2, twice(-m1))), d2);
         }, d, a, h);
