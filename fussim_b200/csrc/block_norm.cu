@@ -133,7 +133,7 @@ Layout layout(const Shape& s, bool backward, int mode, bool per_sample, bool vec
     } else if (!best({1, 3, 4, 5}, true)) {
       if (needed > kBlockMaxThreads || !best({3, 4}, false)) best({4}, false);
     }
-    const int registers = backward ? block_backward_registers(l.groups) : block_forward_registers(l.groups, l.vec || l.groups == 1 ? mode : kBlockAfter);
+    const int registers = backward ? block_backward_registers(l.groups) : block_forward_registers(l.groups, l.vec || l.groups == 1 ? mode : kBlockAfter, l.vec);
     const int resident = block_resident(registers);
     l.B = per_sample ? s.B : 1;
     l.T = per_sample ? s.T : s.B * s.T;

@@ -622,7 +622,9 @@ __device__ __forceinline__ BlockTeam<WARP> block_team(const BlockParams& p, cons
 }
 
 // Registers, and with them how many threads an SM holds.
-constexpr int block_forward_registers(int v, int mode) { return mode == kBlockAfter || v > 4 ? 128 : v > 3 ? 104 : 88; }
+constexpr int block_forward_registers(int v, int mode, bool vec) {
+  return mode == kBlockAfter || v > 4 || !vec ? 128 : v > 3 ? 104 : 88;
+}
 constexpr int block_backward_registers(int v) { return v > 2 ? 128 : 168; }
 constexpr int block_resident(int registers) { return 65536 / registers / 32 * 32; }
 
@@ -630,7 +632,7 @@ constexpr int block_resident(int registers) { return 65536 / registers / 32 * 32
 // of 1024 with a 32-bit residual (201 MB) 40 us; 8 x 1024 x 1152 BF16 (76 MB, four rows a warp) 20 us, of
 // which the arrays' and the first rows' way from memory takes a quarter. A single row of 2048: 6 us, latency.
 template <typename X, typename Y, int V, int UNIT, bool WARP, int MODE, bool STAGED>
-__global__ void __maxnreg__(block_forward_registers(V, MODE)) block_norm_forward_kernel(const __grid_constant__ BlockParams p) {
+__global__ void __maxnreg__(block_forward_registers(V, MODE, UNIT > 1)) block_norm_forward_kernel(const __grid_constant__ BlockParams p) {
   extern __shared__ __align__(16) unsigned char block_memory[];
   __shared__ double2 slots[2 * 16];
   grid_dependency_wait();
