@@ -444,7 +444,7 @@ __device__ __noinline__ void adamw_piece(const AdamwRun run, const AdamwScalars*
 }
 
 // Moments of 32 bits: bound by DRAM (59 million FP32, 28 bytes a number, 271 us, 6.1 TB/s; 100 million in
-// mixed precision, 300 tensors, 490 us, 5.7 TB/s). Of 8 bits: by arithmetic, some 65 instructions a number
+// mixed precision, 300 tensors, 490 us, 5.7 TB/s). Of 8 bits: by arithmetic, some 70 instructions a number
 // for 10 bytes (160 million BF16 427 us, 3.8 TB/s).
 template <int BITS, int K>
 __global__ void __launch_bounds__(kAdamwThreads, adamw_resident(BITS))

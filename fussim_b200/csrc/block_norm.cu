@@ -133,8 +133,9 @@ Layout layout(const Shape& s, bool backward, int mode, bool per_sample, bool vec
     } else if (!best({1, 3, 4, 5}, true)) {
       if (needed > kBlockMaxThreads || !best({3, 4}, false)) best({4}, false);
     }
-    const int registers = backward ? block_backward_registers(l.groups) : block_forward_registers(l.groups, l.vec || l.groups == 1 ? mode : kBlockAfter, l.vec);
-    const int resident = block_resident(registers);
+    const int resident = block_resident(
+        backward ? block_backward_registers(l.groups)
+                 : block_forward_registers(l.groups, l.vec || l.groups == 1 ? mode : kBlockAfter, l.vec));
     l.B = per_sample ? s.B : 1;
     l.T = per_sample ? s.T : s.B * s.T;
     const int64_t array_bytes = static_cast<int64_t>(arrays) * s.C * sizeof(float);
@@ -152,26 +153,29 @@ Layout layout(const Shape& s, bool backward, int mode, bool per_sample, bool vec
         if (l.warp) continue;
         break;
       }
-      // (few rows: smaller CTAs, so that all SMs have some)
-      // (backward at least four rows of a thread, for which it leaves one set of sums)
+      // Few rows: smaller CTAs, so that all SMs have some; backward of at least four rows of a thread, for
+      // which it leaves one set of sums.
       const int64_t fewest = backward ? 4 : 1;
       if (l.warp && block > 32 && l.B * ((l.T + parts * fewest - 1) / (parts * fewest)) < 2 * kSms) continue;
       for (int64_t on_sm = std::max(resident / block, 1); on_sm >= 1 && on_sm * block > most; --on_sm) {
         const int64_t wanted = (kSms * on_sm + l.B - 1) / l.B;
         // a thread adds at most 256 rows up in FP32
-        const int64_t rounds = std::clamp<int64_t>((l.T + parts * wanted - 1) / (parts * wanted), std::min(fewest, (l.T + parts - 1) / parts), 256);
+        const int64_t rounds = std::clamp<int64_t>((l.T + parts * wanted - 1) / (parts * wanted),
+                                                   std::min(fewest, (l.T + parts - 1) / parts), 256);
         const int64_t chunk = rounds * parts, chunks = (l.T + chunk - 1) / chunk;
         const int64_t crowd = std::min(on_sm, (l.B * chunks + kSms - 1) / kSms);
         const int64_t room = std::min<int64_t>(kSmMemory / crowd - 2048, fssim_host::kBlockMemory);
         const int64_t stages = std::min<int64_t>(kMaxStages, rounds + 1), least = std::min<int64_t>(stages, 2);
         // (kernels that make the arrays again for each row: four groups of a CTA's rows alone)
-        const bool choice = l.groups == 4 && !l.warp, fits = array_bytes + least * stage <= room && (l.vec || !choice);
+        const bool choice = l.groups == 4 && !l.warp;
+        const bool fits = array_bytes + least * stage <= room && (l.vec || !choice);
         if (!fits && (on_sm > 1 || (l.warp && block > 32))) continue;
         found.block = block;
         found.chunk = chunk;
         found.chunks = chunks;
         found.staged = fits || !choice;
-        found.stages = stage ? static_cast<int>(std::clamp<int64_t>((room - (found.staged ? array_bytes : 0)) / stage, 1, stages)) : 1;
+        const int64_t rest = room - (found.staged ? array_bytes : 0);
+        found.stages = stage ? static_cast<int>(std::clamp<int64_t>(rest / stage, 1, stages)) : 1;
         found.memory = static_cast<size_t>(stage * found.stages + (found.staged ? array_bytes : 0));
         most = on_sm * block;
       }
