@@ -16,9 +16,9 @@ def mix(v):
     return v ^ (v >> 16)
 
 
-def random_bits(seed, step, tensor, blocks):
+def random_bits(seed, step, tensor, blocks, first_block=0):
     key = mix((mix((mix(seed) + step) & MASK) + tensor) & MASK)
-    row = mix((key + torch.arange(blocks)) & MASK)[:, None]
+    row = mix((key + first_block + torch.arange(blocks)) & MASK)[:, None]
     v = (row + torch.arange(BLOCK) * 0x9E3779B1) & MASK
     v = ((v ^ (v >> 15)) * 0xBB67AE85) & MASK
     return v ^ (v >> 15)
@@ -51,8 +51,8 @@ def encode(part, rnd, root):
     return y.to(F8), scales
 
 
-def step32(p, g, m, v, scales=None, *, step, lr, betas, eps, wd, coef=1.0, seed=0, tensor=0):
-    """Flat tensors; m and v are codes where scales are given. Returns p (FP32, before its own
+def step32(p, g, m, v, scales=None, *, step, lr, betas, eps, wd, coef=1.0, seed=0, tensor=0, first_block=0):
+    """Flat tensors (from a block's first number on); m and v are codes where scales are given. Returns p (FP32, before its own
     rounding), m, v and, of codes, the scales."""
     f = lambda x: torch.tensor(x, dtype=torch.float32)  # noqa: E731
     n = p.numel()
@@ -71,7 +71,7 @@ def step32(p, g, m, v, scales=None, *, step, lr, betas, eps, wd, coef=1.0, seed=
     flat = lambda t: t.reshape(-1)[:n]  # noqa: E731
     if scales is None:
         return flat(p), flat(m), flat(v)
-    rnd = random_bits(seed, step, tensor, p.shape[0])
+    rnd = random_bits(seed, step, tensor, p.shape[0], first_block)
     mc, ms = encode(m, rnd & 0xFFFFF, False)
     vc, vs = encode(root, rnd >> 12, True)
     return flat(p), flat(mc), flat(vc), torch.cat([ms, vs], 1)

@@ -250,6 +250,19 @@ def test_not_finite(bits):
     check_bits(before, s, step=8)
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_norm_not_finite(bits):
+    """A NaN norm makes everything NaN; an infinite one leaves finite gradients nothing."""
+    for bad in (math.nan, math.inf):
+        s = make([700, 3], F32, F32, bits)
+        s["grads"][1][0] = bad
+        before = snapshot(s)
+        norm = run(s, max_norm=1.0)
+        assert norm.isnan().item() if math.isnan(bad) else norm.isinf().item()
+        check_bits(before, s, coef=math.nan if math.isnan(bad) else 0.0)
+        assert s["params"][0].isnan().all().item() == math.isnan(bad)
+
+
 def test_extremes_of_codes():
     """Blocks of one value, of tiny values, of a range beyond the codes', and of negative zeros."""
     s = make([256 * 6 + 5], F32, F32, 8)

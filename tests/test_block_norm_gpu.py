@@ -388,6 +388,55 @@ def test_large_rows_in_fp64():
     run(d, "both", kind="layer", branch_kind="layer")
 
 
+@pytest.mark.parametrize("shape", [(300, 2, 72), (700, 1, 1000), (1025, 3, 33), (64, 40, 24), (129, 1, 520)], ids=str)
+def test_many_samples(shape):
+    """More samples than a CTA of the vectors' sums takes: vectors for each beside shared ones."""
+    for kind, branch_kind, gate, mod in KINDS:
+        d = make(*shape, F32, F32, gate, branch_kind, kind, mod)
+        run(d, "both", kind=kind, branch_kind=branch_kind, s=0.7)
+    x = torch.randn(shape[0], shape[2], device="cuda", requires_grad=True)  # a row for each sample
+    d = {"x": x, "branch": torch.randn_like(x, requires_grad=True),
+         "gate": torch.randn_like(x, requires_grad=True), "weight": torch.randn(shape[2], device="cuda", requires_grad=True)}
+    run(d, "both", kind="layer", branch_kind="rms")
+
+
+def test_aliased_results_of_the_c_entry_point():
+    """r in x's place and z in branch's, dx in dr's and dbranch in dz's: as in memory of their own."""
+    import ctypes
+
+    from tests import test_block_norm_cpu as c
+
+    lib = ctypes.CDLL(c.LIB)
+    lib.fssim_block_norm_backward_workspace_bytes.restype = ctypes.c_size_t
+    for f in (lib.fssim_block_norm_forward, lib.fssim_block_norm_backward):
+        f.argtypes = [ctypes.c_void_p, ctypes.c_void_p]
+    for rows, cols in ((700, 96), (90, 1001), (60, 2048)):
+        x, y, dr, dz = (torch.randn(rows, cols, device="cuda") for _ in range(4))
+        results = []
+        for alias in (False, True):
+            t = [v.clone() for v in (x, y, dr, dz)]
+            r, z, dx, dy = t if alias else [torch.empty_like(v) for v in t]
+            stats, after = (torch.empty(rows, 2, device="cuda") for _ in range(2))
+            a = c.ForwardArgs(kind=2, branch_kind=2, B=1, T=rows, C=cols, eps=1e-6, residual_scale=0.5, x=t[0].data_ptr(),
+                              branch=t[1].data_ptr(), r=r.data_ptr(), z=z.data_ptr(), stats=stats.data_ptr(),
+                              branch_stats=after.data_ptr())
+            stream = torch.cuda.current_stream().cuda_stream
+            assert lib.fssim_block_norm_forward(ctypes.byref(a), stream) == 0
+            out = [r.clone(), z.clone()]
+            weight = torch.empty(cols, device="cuda")
+            b = c.BackwardArgs(kind=2, branch_kind=2, B=1, T=rows, C=cols, residual_scale=0.5, r=r.data_ptr(),
+                               branch=y.data_ptr(), dr=t[2].data_ptr(), dz=t[3].data_ptr(), stats=stats.data_ptr(),
+                               branch_stats=after.data_ptr(), dx=dx.data_ptr(), dbranch=dy.data_ptr(),
+                               dweight=c.Channels(weight.data_ptr(), 0, 0))
+            size = lib.fssim_block_norm_backward_workspace_bytes(ctypes.byref(b))
+            ws = torch.empty(size, dtype=torch.uint8, device="cuda")
+            b.workspace, b.workspace_bytes = ws.data_ptr(), size
+            assert lib.fssim_block_norm_backward(ctypes.byref(b), stream) == 0
+            torch.cuda.synchronize()
+            results.append(out + [dx.clone(), dy.clone(), weight])
+        assert all(torch.equal(p, q) for p, q in zip(*results))
+
+
 def test_shared_vectors_and_twice_the_same():
     """One weight for both norms, and the same tensor as x and branch: gradients add up."""
     x = torch.randn(3, 5, 80, device="cuda", dtype=torch.float32, requires_grad=True)
