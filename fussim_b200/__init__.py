@@ -10,7 +10,7 @@ Drop-in for the public API of OpsiClear/fussim (``fussim/__init__.py``):
 
 Beside the losses, operators of the training step around them: ``group_norm_act`` /
 ``GroupNormAct`` (group normalisation with its activation, channels last), ``block_norm`` /
-``gated_residual`` / ``gated_residual_norm`` (the norms before and after a residual block, with its
+``BlockNorm`` / ``gated_residual`` / ``gated_residual_norm`` (the norms before and after a residual block, with its
 gate and modulation), ``grad_norm`` / ``clip_grad_norm`` / ``clip_grad_norm_`` (the global gradient
 norm and clipping) and ``adamw_step_`` / ``AdamW`` (the AdamW step of many tensors, with moments in
 32 or 8 bits).
@@ -22,6 +22,7 @@ FP32. There is no CPU path: every call runs the hand-written sm_100a kernels of
 """
 
 from .blocks import (  # noqa: F401
+    BlockNorm,
     block_norm,
     gated_residual,
     gated_residual_norm,
@@ -61,6 +62,7 @@ __all__ = [
     "group_norm_act",
     "GroupNormAct",
     "block_norm",
+    "BlockNorm",
     "gated_residual",
     "gated_residual_norm",
     "grad_norm",

@@ -1,7 +1,7 @@
 """Norms before and after the residual blocks of an image transformer (or any network over rows of
 channels), fused with the block's gate, residual scale and modulation.
 
-* ``block_norm``: the norm before a block.
+* ``block_norm`` / ``BlockNorm``: the norm before a block.
 * ``gated_residual``: a block's output, normalised, gated and added to the residual stream.
 * ``gated_residual_norm``: both in one pass, the end of one block and the start of the next.
 
@@ -96,3 +96,50 @@ def gated_residual_norm(
         x, branch, gate, weight, bias, scale, shift, kind, residual_scale, branch_kind,
         branch_weight, branch_bias, eps
     )
+
+
+class BlockNorm(torch.nn.Module):
+    """``block_norm`` as a module, with the parameter names, shapes and initial values of
+    ``torch.nn.RMSNorm`` (``kind`` "rms": weight) or ``torch.nn.LayerNorm`` ("layer": weight and
+    bias) over ``num_channels``: their state dicts load here."""
+
+    def __init__(
+        self,
+        num_channels: int,
+        kind: str = "rms",
+        eps: float = 1e-6,
+        affine: bool = True,
+        device=None,
+        dtype=None,
+    ):
+        super().__init__()
+        if not 1 <= num_channels <= 16384:
+            raise ValueError(f"num_channels must be from 1 to 16384, got {num_channels}")
+        if kind not in ("rms", "layer"):
+            raise ValueError(f"kind must be 'rms' or 'layer', got {kind!r}")
+        self.num_channels = num_channels
+        self.kind = kind
+        self.eps = eps
+        self.affine = affine
+        options = dict(device=device, dtype=dtype)
+        if affine:
+            self.weight = torch.nn.Parameter(torch.ones(num_channels, **options))
+        else:
+            self.register_parameter("weight", None)
+        if affine and kind == "layer":
+            self.bias = torch.nn.Parameter(torch.zeros(num_channels, **options))
+        else:
+            self.register_parameter("bias", None)
+
+    def forward(
+        self,
+        x: torch.Tensor,
+        scale: Optional[torch.Tensor] = None,
+        shift: Optional[torch.Tensor] = None,
+        out_dtype: Optional[torch.dtype] = None,
+    ) -> torch.Tensor:
+        return block_norm(x, self.weight, self.bias, scale=scale, shift=shift, kind=self.kind,
+                          eps=self.eps, out_dtype=out_dtype)
+
+    def extra_repr(self) -> str:
+        return f"{self.num_channels}, {self.kind!r}, eps={self.eps}, affine={self.affine}"

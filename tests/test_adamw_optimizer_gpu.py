@@ -269,7 +269,7 @@ class Network(torch.nn.Module):
         self.inward, self.outward = torch.nn.Linear(48, c), torch.nn.Linear(c, 48)
         self.condition = torch.nn.Linear(3, 2 * c)
         self.blocks = torch.nn.ModuleList(Block(c, plain) for _ in range(depth))
-        self.first = torch.nn.Parameter(torch.ones(c))
+        self.first = fb.BlockNorm(c)
         self.plain = plain
 
     def forward(self, image):
@@ -278,9 +278,9 @@ class Network(torch.nn.Module):
         scale, shift = self.condition(image.mean((2, 3))).chunk(2, -1)
         x = self.inward(t)
         if self.plain:
-            z = x * (x.square().mean(-1, keepdim=True) + 1e-6).rsqrt() * self.first
+            z = x * (x.square().mean(-1, keepdim=True) + 1e-6).rsqrt() * self.first.weight
         else:
-            z = fb.block_norm(x, self.first)
+            z = self.first(x)
         for block in self.blocks:
             x, z = block(x, z, scale, shift)
         t = self.outward(z).sigmoid().view(b, h // 4, w // 4, 3, 4, 4).permute(0, 3, 1, 4, 2, 5)

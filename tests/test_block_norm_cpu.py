@@ -23,7 +23,7 @@ def both(**kw):
 
 
 def test_public_names():
-    for name in ("block_norm", "gated_residual", "gated_residual_norm"):
+    for name in ("block_norm", "BlockNorm", "gated_residual", "gated_residual_norm"):
         assert name in fb.__all__ and hasattr(fb, name)
 
 
@@ -61,6 +61,20 @@ def test_public_names():
 def test_refusals(kw, match):
     with pytest.raises(ValueError, match=match):
         both(**kw)
+
+
+@pytest.mark.parametrize("kind", ["rms", "layer"])
+def test_module(kind):
+    m = fb.BlockNorm(12, kind)
+    ref = (torch.nn.RMSNorm if kind == "rms" else torch.nn.LayerNorm)(12)
+    assert {k: v.shape for k, v in m.state_dict().items()} == {k: v.shape for k, v in ref.state_dict().items()}
+    m.load_state_dict(ref.state_dict())
+    assert torch.equal(m.weight, ref.weight) and repr(m) == f"BlockNorm(12, {kind!r}, eps=1e-06, affine=True)"
+    assert not list(fb.BlockNorm(12, kind, affine=False).parameters())
+    assert fb.BlockNorm(12, kind, 1e-5, True, "cpu", torch.bfloat16).weight.dtype == torch.bfloat16
+    for args in ((0,), (16385,), (12, "batch")):
+        with pytest.raises(ValueError, match="must be"):
+            fb.BlockNorm(*args)
 
 
 def test_out_dtype():

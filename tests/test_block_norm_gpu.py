@@ -361,6 +361,15 @@ def test_unaligned_memory():
             check(d, "both", *b, kind="layer")
 
 
+def test_module():
+    for kind in ("rms", "layer"):
+        m = fb.BlockNorm(80, kind).cuda()
+        torch.nn.init.normal_(m.weight)
+        x, t = torch.randn(2, 5, 80, device="cuda"), torch.randn(2, 80, device="cuda")
+        assert torch.equal(m(x, t, t), fb.block_norm(x, m.weight, m.bias, scale=t, shift=t, kind=kind))
+        assert m(x, out_dtype=BF16).dtype == BF16
+
+
 def test_shapes():
     for shape in ((48,), (5, 48), (2, 3, 48), (2, 3, 4, 48), (2, 1, 3, 2, 48)):
         x = torch.randn(shape, device="cuda", requires_grad=True)
