@@ -250,6 +250,21 @@ def test_not_finite(bits):
     check_bits(before, s, step=8)
 
 
+def test_roots_and_quotients():
+    """All 2^24 roots of two binades, and as many quotients, are the correctly rounded ones: halved moments
+    (exactly) and a rate of 1 leave a parameter of zero at minus the quotient."""
+    n = 1 << 24
+    v = (torch.arange(n, dtype=torch.int32, device="cuda") + 0x40000000).view(F32)  # [2, 8): halves in [1, 4)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    m = torch.randn(n, device="cuda", generator=g) * torch.exp2(torch.randint(-30, 30, (n,), device="cuda", generator=g).float())
+    s = {"params": [torch.zeros(n, device="cuda")], "grads": [torch.zeros(n, device="cuda")], "exp_avgs": [m],
+         "exp_avg_sqs": [v]}
+    before = snapshot(s)
+    kw = dict(step=1, lr=0.5, betas=(0.5, 0.5), eps=2.0 ** -30, wd=0.0)
+    run(s, **kw)
+    check_bits(before, s, **kw)
+
+
 @pytest.mark.parametrize("bits", [32, 8])
 def test_norm_not_finite(bits):
     """A NaN norm makes everything NaN; an infinite one leaves finite gradients nothing."""
