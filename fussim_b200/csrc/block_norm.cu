@@ -110,7 +110,7 @@ Layout layout(const Shape& s, bool backward, int mode, bool per_sample, bool vec
         if (t > 32) continue;
       } else {
         t = (t + 31) / 32 * 32;
-        if (t > (backward && g <= 2 ? 384 : kBlockMaxThreads)) continue;  // (registers)
+        if (t > kBlockMaxThreads || (backward && t > block_resident(block_backward_registers(g, l.vec)))) continue;
       }
       // (the kernels count on whole groups but for a row's last)
       if ((g - 1) * t < needed && t * g <= padded) {
@@ -125,7 +125,7 @@ Layout layout(const Shape& s, bool backward, int mode, bool per_sample, bool vec
   l.vec = vec;
   for (;;) {
     if (!l.vec) {
-      if (!best({1}, true) && !best({1}, false)) best({4}, false);
+      if (!best({1}, true) && !best({1}, false) && !best({2}, false)) best({4}, false);
     } else if (backward) {
       if (!best({1, 2}, true) && !best({1, 2}, false)) best({4}, false);
     } else if (s.B * s.T <= 2 * kSms && needed <= kBlockMaxThreads) {
@@ -134,7 +134,7 @@ Layout layout(const Shape& s, bool backward, int mode, bool per_sample, bool vec
       if (needed > kBlockMaxThreads || !best({3, 4}, false)) best({4}, false);
     }
     const int resident = block_resident(
-        backward ? block_backward_registers(l.groups)
+        backward ? block_backward_registers(l.groups, l.vec)
                  : block_forward_registers(l.groups, l.vec || l.groups == 1 ? mode : kBlockAfter, l.vec));
     l.B = per_sample ? s.B : 1;
     l.T = per_sample ? s.T : s.B * s.T;

@@ -176,8 +176,13 @@ struct BlockRow {
   static constexpr bool kVec = UNIT > 1;
   static constexpr int kPiece = UNIT * sizeof(T), kPieces = V * 8 / UNIT;  // bytes of a unit, units of a thread
   static constexpr int kBytes = kVec ? kPieces * kPiece * 32 : 0;          // of a warp's part of a stage
-  // (a register for each, also of 16-bit numbers: to pack two the loads would have to be waited for)
-  unsigned one[kVec ? 1 : V * 8];
+  using Bits = std::conditional_t<sizeof(T) == 4, unsigned, unsigned short>;
+  // Of single numbers, eight are held (a register for each, also of 16 bits: to pack two the loads would
+  // have to be waited for). Of longer rows only the place is, and they are read where they are used, for
+  // each turn again, which caches serve (2 x 700 x 7001 FP32 to BF16 forward 51 us; held, they spilled: 287).
+  static constexpr bool kHeld = !kVec && V == 1;
+  unsigned one[kHeld ? 8 : 1];
+  const Bits* place;
 
   static __device__ __forceinline__ void copy(unsigned char* slot, const void* from, int64_t offset,
                                               const BlockColumns<UNIT, V>& c, bool active) {
@@ -198,10 +203,10 @@ struct BlockRow {
   }
   // (without conditions, at places that are in the tensor: a load behind a branch is waited for there)
   __device__ __forceinline__ void load(const void* from, int64_t offset, const BlockColumns<UNIT, V>& c) {
-    using Bits = std::conditional_t<sizeof(T) == 4, unsigned, unsigned short>;
-    const Bits* at = static_cast<const Bits*>(from) + offset;
+    place = static_cast<const Bits*>(from) + offset;
+    if constexpr (kHeld)
 #pragma unroll
-    for (int i = 0; i < V * 8; ++i) one[i] = at[min(c.at(0, i), c.C - 1)];
+      for (int i = 0; i < 8; ++i) one[i] = place[min(c.at(0, i), c.C - 1)];
   }
   // Group v; zeros where there are no numbers.
   __device__ __forceinline__ Eight get(const unsigned char* slot, int v, const BlockColumns<UNIT, V>& c, bool active) const {
@@ -214,10 +219,13 @@ struct BlockRow {
       for (int k = 0; k < per; ++k) raw[k] = at[(v * per + k) * 32];
       return reinterpret_cast<const BlockPacked<T>&>(raw).widen();
     } else {
+      unsigned raw[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) raw[i] = kHeld ? one[kHeld ? i : 0] : place[min(c.at(v, i), c.C - 1)];
       Eight f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const unsigned bits = one[v * 8 + i];
+        const unsigned bits = raw[i];
         float value;
         if constexpr (sizeof(T) == 4) value = __uint_as_float(bits);
         else if constexpr (std::is_same_v<T, __half>) value = __half2float(__ushort_as_half(static_cast<unsigned short>(bits)));
@@ -625,7 +633,10 @@ __device__ __forceinline__ BlockTeam<WARP> block_team(const BlockParams& p, cons
 constexpr int block_forward_registers(int v, int mode, bool vec) {
   return mode == kBlockAfter || v > 4 || !vec ? 128 : v > 3 ? 104 : 88;
 }
-constexpr int block_backward_registers(int v) { return v > 2 ? 128 : 168; }
+// (two groups, number by number: 16 warps hide the loads' way better than 12 with all in registers;
+// 2 x 700 x 7001 FP32 to BF16 training pass 144 us against 400 with four groups of too few warps, but
+// 1 x 1700 x 5003 FP16 214 against 197)
+constexpr int block_backward_registers(int v, bool vec) { return v > 2 || (v == 2 && !vec) ? 128 : 168; }
 constexpr int block_resident(int registers) { return 65536 / registers / 32 * 32; }
 
 // Bound by DRAM where rows are many: 16384 x 4096 BF16 (RMS alone, 268 MB) 50 us, 5.4 TB/s; 16 x 1024 rows
@@ -649,7 +660,7 @@ __global__ void __maxnreg__(block_forward_registers(V, MODE, UNIT > 1)) block_no
   const bool after_norm = MODE == kBlockAfter && p.after_kind;
   using RowX = BlockRow<X, V, UNIT>;
   using RowY = BlockRow<Y, V, UNIT>;
-  // (number by number: a row is held, and the next on its way, in registers)
+  // (number by number: a row is held, and the next on its way, in registers, where a thread has eight of it)
   RowX row_x, next_x;
   RowY row_y, next_y;
   constexpr int at_y = RowX::kBytes;
@@ -755,7 +766,7 @@ __global__ void __maxnreg__(block_forward_registers(V, MODE, UNIT > 1)) block_no
 // much) 50 us, 6.0 TB/s. The numbers are read from the ring for each of up to three turns (sums, dR, dy),
 // so that the four sums can stay in registers.
 template <typename X, typename Y, int V, int UNIT, bool WARP, int MODE, bool STAGED>
-__global__ void __maxnreg__(block_backward_registers(V)) block_norm_backward_kernel(const __grid_constant__ BlockParams p) {
+__global__ void __maxnreg__(block_backward_registers(V, UNIT > 1)) block_norm_backward_kernel(const __grid_constant__ BlockParams p) {
   extern __shared__ __align__(16) unsigned char block_memory[];
   __shared__ double2 slots[2 * 16];
   grid_dependency_wait();

@@ -85,6 +85,7 @@ int block_norm_types(bool backward, const BlockLaunch& l, const fssim::BlockPara
     if (!l.vec)
       return l.warp          ? block_backward_mode<X, Y, 1, true, false>(l, p, stream)
              : l.groups == 1 ? block_backward_mode<X, Y, 1, false, false>(l, p, stream)
+             : l.groups == 2 ? block_backward_mode<X, Y, 2, false, false>(l, p, stream)
                              : block_backward<X, Y, 4, false, false, kBlockAfter, false>(l, p, stream);
     if (l.groups == 4)
       return l.staged ? block_backward<X, Y, 4, true, false, kBlockAfter>(l, p, stream)
@@ -98,6 +99,7 @@ int block_norm_types(bool backward, const BlockLaunch& l, const fssim::BlockPara
   if (!l.vec)
     return l.warp          ? block_forward_mode<X, Y, 1, true, false>(l, p, stream)
            : l.groups == 1 ? block_forward_mode<X, Y, 1, false, false>(l, p, stream)
+           : l.groups == 2 ? block_forward<X, Y, 2, false, false, kBlockAfter>(l, p, stream)
                            : block_forward<X, Y, 4, false, false, kBlockAfter, false>(l, p, stream);
   if (!l.staged) return block_forward<X, Y, 4, true, false, kBlockAfter, false>(l, p, stream);
   if (l.warp) {

@@ -361,6 +361,17 @@ def test_unaligned_memory():
             check(d, "both", *b, kind="layer")
 
 
+@pytest.mark.parametrize("types", TYPES, ids=str)
+@pytest.mark.parametrize("c", [4095, 4099, 6143, 6145, 8191, 8193, 12289, 16381])
+def test_long_rows_of_no_whole_vectors(c, types):
+    d = make(2, 3, c, *types, gate="sample", branch_kind="layer", kind="layer", mod=True, seed=c)
+    run(d, "both", kind="layer", branch_kind="layer")
+    d = make(2, 3, c, *types, gate="channel", kind="rms", seed=c)
+    run(d, "both", kind="rms")
+    d = make(1, 5, c, *types, form="before", kind="rms", seed=c)
+    run(d, "before", kind="rms", out_dtype=types[1])
+
+
 def test_module():
     for kind in ("rms", "layer"):
         m = fb.BlockNorm(80, kind).cuda()
@@ -419,7 +430,7 @@ def test_aliased_results_of_the_c_entry_point():
     lib.fssim_block_norm_backward_workspace_bytes.restype = ctypes.c_size_t
     for f in (lib.fssim_block_norm_forward, lib.fssim_block_norm_backward):
         f.argtypes = [ctypes.c_void_p, ctypes.c_void_p]
-    for rows, cols in ((700, 96), (90, 1001), (60, 2048)):
+    for rows, cols in ((700, 96), (90, 1001), (60, 2048), (311, 4101), (160, 7001), (11, 9001)):
         x, y, dr, dz = (torch.randn(rows, cols, device="cuda") for _ in range(4))
         results = []
         for alias in (False, True):
