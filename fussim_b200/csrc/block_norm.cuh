@@ -167,6 +167,9 @@ struct BlockRing {
     else if (stages == 2) asm volatile("cp.async.wait_group 1;" ::: "memory");
     else asm volatile("cp.async.wait_group 0;" ::: "memory");
   }
+  // The last turns' copies, of zeros: they have to be over before the memory is anything else's (a barrier
+  // orders no copy that is on its way).
+  static __device__ __forceinline__ void drain() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 };
 
 // A thread's numbers of one tensor's row: through the ring, or (single numbers) loaded into registers.
@@ -760,6 +763,7 @@ __global__ void __maxnreg__(block_forward_registers(V, MODE, UNIT > 1)) block_no
       if (active) block_store<Y>(p.z, offset, c, v, BlockPacked<Y>::of(z));
     }
   }
+  if constexpr (kVec) ring.drain();
 }
 
 // Bound by DRAM: 16 x 1024 rows of 1024 with a 32-bit residual (302 MB) 51 us, 8 x 16384 x 96 FP32 (as
@@ -925,6 +929,7 @@ __global__ void __maxnreg__(block_backward_registers(V, UNIT > 1)) block_norm_ba
       }
     }
   }
+  if constexpr (kVec) ring.drain();
   if (!p.partials) return;
   float* mine = p.partials + static_cast<int64_t>(blockIdx.x) * p.sums * C;
   if constexpr (!WARP) {
