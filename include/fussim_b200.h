@@ -387,8 +387,8 @@ int fssim_grad_clip(const fssim_grad_clip_args* args, fssim_stream_t stream);
  *     r = x + residual_scale * gate * (N'(branch) * branch_weight + branch_bias), in x's type,
  *     z = (N(r) * weight + bias) * (1 + scale) + shift, in the branch's type,
  * with N a norm over the row, (v - mean) / sqrt(<(v - mean)^2> + eps), mean = 0 in the RMS kind, and
- * N' one too, or the identity (FSSIM_NORM_NONE). Without a branch r is x; without z only r is
- * computed. Statistics and arithmetic are FP32; each result is rounded once. */
+ * N' one too, or the identity (FSSIM_NORM_NONE; branch_weight and branch_bias are then refused).
+ * Without a branch r is x; without z only r is computed. Statistics and arithmetic are FP32; each result is rounded once. */
 typedef enum fssim_norm_kind {
   FSSIM_NORM_NONE = 0,
   FSSIM_NORM_RMS = 1,
