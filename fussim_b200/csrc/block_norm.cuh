@@ -547,17 +547,18 @@ __device__ __forceinline__ float2 block_moments(BlockTeam<WARP>& team, const Eig
   return make_float2(mean, squares);
 }
 
-// (mean, rstd) of a row. FP32's range is that of the numbers, not of their squares: where their sum
-// leaves it (or its accurate part, and eps does not cover that), it is taken again of numbers
-// scaled by a power of two.
+// (mean, rstd) of a row. FP32's range is that of the numbers, not of their squares or distances: where
+// the squares' sum leaves it (or its accurate part, and eps does not cover that; NaN, as of two
+// infinite distances, counts as left), it is taken again of numbers scaled by a power of two.
 template <int V, int UNIT, bool WARP>
 __device__ __forceinline__ float2 block_stats(BlockTeam<WARP>& team, const Eight (&f)[V], int kind, float eps,
                                               const BlockColumns<UNIT, V>& c) {
   const float2 m = block_moments<false, V, UNIT, WARP>(team, f, kind, 1.f, c);
-  const bool large = m.y > 0x1p120f, again = large || (m.y < 0x1p-80f && eps < 0x1p-90f);
+  const bool large = !(m.y <= 0x1p120f), again = large || (m.y < 0x1p-80f && eps < 0x1p-90f);
   const float inv = 1.f / c.C;
   if (WARP ? __any_sync(0xffffffffu, again) : again) {
-    const float by = !again ? 1.f : large ? 0x1p-70f : 0x1p70f;
+    // (16384 squares of 2^129 have to fit)
+    const float by = !again ? 1.f : large ? 0x1p-80f : 0x1p70f;
     const float2 scaled = block_moments<true, V, UNIT, WARP>(team, f, kind, by, c);
     // (rows beside one that needs this keep their own)
     if (again) return make_float2(scaled.x / by, by * rsqrtf(scaled.y * inv + eps * by * by));
@@ -597,6 +598,20 @@ __device__ __forceinline__ double2 block_stats_wide(BlockTeam<WARP>& team, const
   const double variance = sums.y * inv - shift * shift;  // (NaN stays)
   return make_double2(pivot + shift, rsqrt((variance < 0.0 ? 0.0 : variance) + static_cast<double>(eps)));
 }
+
+// (v - mean) * rstd of pairs. Distances of 2^128 and more are nothing that FP32 holds, so those of rows that
+// reach so far (their rstd is at most sqrt(C) / 2^128, 2^-121) are taken halved; of all others in
+// the bits of a difference.
+struct BlockHat {
+  float2 by, shift, rise;
+  __device__ __forceinline__ explicit BlockHat(float2 stats) {
+    const bool far = stats.y < 0x1p-120f;
+    by = twice(far ? 0.5f : 1.f);
+    shift = __fmul2_rn(by, twice(-stats.x));
+    rise = twice(far ? stats.y * 2.f : stats.y);
+  }
+  __device__ __forceinline__ float2 operator()(float2 v) const { return __fmul2_rn(__ffma2_rn(v, by, shift), rise); }
+};
 
 // ---- the kernels ----
 struct BlockPlace {
@@ -717,6 +732,7 @@ __global__ void __maxnreg__(block_forward_registers(V, MODE, UNIT > 1)) block_no
       }
       if (p.after_stats && active && c.tid == 0) p.after_stats[row] = after;
     }
+    const BlockHat after_hat(after);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       r[v] = row_x.get(slot, v, c, active);
@@ -741,9 +757,7 @@ __global__ void __maxnreg__(block_forward_registers(V, MODE, UNIT > 1)) block_no
       } else {
         if (after_norm) {
           const Eight w = arrays.get(kArrayAfterWeight, c, v, 1.f), o = arrays.get(kArrayAfterBias, c, v, 0.f);
-          u = pairs([&](float2 a, float2 w2, float2 o2) {
-            return __ffma2_rn(__fmul2_rn(__fadd2_rn(a, twice(-after.x)), twice(after.y)), w2, o2);
-          }, u, w, o);
+          u = pairs([&](float2 a, float2 w2, float2 o2) { return __ffma2_rn(after_hat(a), w2, o2); }, u, w, o);
         }
         // (two roundings, as of a product and a sum one after the other)
         e = BlockPacked<X>::of(pairs([](float2 a, float2 g2, float2 x) { return pair_add(x, __fmul2_rn(g2, a)); }, u, g, r[v]));
@@ -754,12 +768,11 @@ __global__ void __maxnreg__(block_forward_registers(V, MODE, UNIT > 1)) block_no
     if (MODE != kBlockBefore && !p.z) continue;
     const float2 stats = block_stats<V, UNIT, WARP>(team, r, p.kind, p.eps, c);
     if (p.stats && active && c.tid == 0) p.stats[row] = stats;
+    const BlockHat hat(stats);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       const Eight a = arrays.get(kArrayFactor, c, v, 1.f), o = arrays.get(kArrayOffset, c, v, 0.f);
-      const Eight z = pairs([&](float2 b, float2 a2, float2 o2) {
-        return __ffma2_rn(__fmul2_rn(__fadd2_rn(b, twice(-stats.x)), twice(stats.y)), a2, o2);
-      }, r[v], a, o);
+      const Eight z = pairs([&](float2 b, float2 a2, float2 o2) { return __ffma2_rn(hat(b), a2, o2); }, r[v], a, o);
       if (active) block_store<Y>(p.z, offset, c, v, BlockPacked<Y>::of(z));
     }
   }
@@ -854,12 +867,13 @@ __global__ void __maxnreg__(block_backward_registers(V, UNIT > 1)) block_norm_ba
       row_y = next_y;
       if constexpr (kAhead) fetch();
     }
+    const BlockHat hat1(s1), hat2(s2);
     const auto get_rhat = [&](int v) {
-      return pairs([&](float2 a) { return __fmul2_rn(__fadd2_rn(a, twice(-s1.x)), twice(s1.y)); }, row_r.get(slot, v, c, active));
+      return pairs(hat1, row_r.get(slot, v, c, active));
     };
     const auto get_yhat = [&](int v) {
       const Eight y = row_y.get(slot + at_y, v, c, active);
-      return after_norm ? pairs([&](float2 a) { return __fmul2_rn(__fadd2_rn(a, twice(-s2.x)), twice(s2.y)); }, y) : y;
+      return after_norm ? pairs(hat2, y) : y;
     };
     const auto times = [](float2 a, float2 b2) { return __fmul2_rn(a, b2); };
     float m1 = 0.f, m2 = 0.f;
