@@ -100,11 +100,34 @@ void check_lists(const Lists& l, bool has_scales, bool has_copies) {
 
 double host_number(const Number& n) { return std::holds_alternative<double>(n) ? std::get<double>(n) : 0.0; }
 
-std::optional<at::Tensor> adamw_step_(const py::list& params, const py::list& grads, const py::list& exp_avgs,
-                                      const py::list& exp_avg_sqs, const OptList& scales, const Number& step,
-                                      const Number& lr, double beta1, double beta2, double eps, double weight_decay,
-                                      bool maximize, std::optional<double> max_norm, const OptTensor& norm_in,
-                                      const OptList& copies, int64_t seed) {
+// A step that is ready: checked, the norm and the copies of gradients on their way, and no tensor of the
+// caller's written. The lists keep the tensors alive.
+struct Step {
+  std::vector<py::list> lists;
+  Lists l;
+  std::vector<at::Tensor> held;  // numbers on the device; gradients in their parameter's order
+  std::vector<const void*> g_at;
+  std::vector<void*> p_at, m_at, v_at, c_at;
+  std::vector<float*> s_at;
+  std::vector<int64_t> sizes;
+  std::vector<int32_t> dtypes, g_dtypes, c_dtypes;
+  fssim_adamw_args a{};
+  std::optional<at::Tensor> norm;
+  std::optional<at::Device> device;
+
+  Step(const py::list& params, const py::list& grads, const py::list& exp_avgs, const py::list& exp_avg_sqs,
+       const OptList& scales, const Number& step, const Number& lr, double beta1, double beta2, double eps,
+       double weight_decay, bool maximize, std::optional<double> max_norm, const OptTensor& norm_in,
+       const OptList& copies, int64_t seed);
+  Step(const Step&) = delete;  // (the arguments point into it)
+  // Once: writes the tensors.
+  std::optional<at::Tensor> run();
+};
+
+Step::Step(const py::list& params, const py::list& grads, const py::list& exp_avgs, const py::list& exp_avg_sqs,
+           const OptList& scales, const Number& step, const Number& lr, double beta1, double beta2, double eps,
+           double weight_decay, bool maximize, std::optional<double> max_norm, const OptTensor& norm_in,
+           const OptList& copies, int64_t seed) {
   const size_t n = params.size();
   const auto sized = [&](const py::list& list, const char* name) {
     if (list.size() != n)
@@ -132,17 +155,21 @@ std::optional<at::Tensor> adamw_step_(const py::list& params, const py::list& gr
     value_error("max_norm must not be negative, got " + std::to_string(*max_norm));
   if (norm_in.has_value() && !max_norm.has_value()) value_error("norm goes with max_norm");
   if (seed < 0 || seed > 0xFFFFFFFF) value_error("seed must be from 0 to 2^32 - 1, got " + std::to_string(seed));
-  const Lists l{refs_of(params, "parameters"), refs_of(grads, "gradients"), refs_of(exp_avgs, "exp_avgs"),
-                refs_of(exp_avg_sqs, "exp_avg_sqs"), scales.has_value() ? refs_of(*scales, "scales") : Refs(),
-                copies.has_value() ? refs_of(*copies, "copies") : Refs()};
+  l = {refs_of(params, "parameters"), refs_of(grads, "gradients"), refs_of(exp_avgs, "exp_avgs"),
+       refs_of(exp_avg_sqs, "exp_avg_sqs"), scales.has_value() ? refs_of(*scales, "scales") : Refs(),
+       copies.has_value() ? refs_of(*copies, "copies") : Refs()};
   check_lists(l, scales.has_value(), copies.has_value());
-  if (n == 0) return max_norm.has_value() ? std::optional<at::Tensor>(norm_in.has_value() ? *norm_in : zero_norm())
-                                          : std::nullopt;
+  if (n == 0) {
+    if (max_norm.has_value()) norm = norm_in.has_value() ? *norm_in : zero_norm();
+    return;
+  }
+  lists = {params, grads, exp_avgs, exp_avg_sqs};
+  if (scales.has_value()) lists.push_back(*scales);
+  if (copies.has_value()) lists.push_back(*copies);
 
   const at::NoGradGuard no_grad;
-  const at::Device device = l.params[0]->device();
+  device = l.params[0]->device();
   const at::cuda::OptionalCUDAGuard guard(device);
-  fssim_adamw_args a{};
   a.count = static_cast<int64_t>(n);
   a.state_bits = scales.has_value() ? 8 : 32;
   a.maximize = maximize;
@@ -161,8 +188,9 @@ std::optional<at::Tensor> adamw_step_(const py::list& params, const py::list& gr
     if (bytes) spans.push_back({b, b + bytes, static_cast<int64_t>(i), out});
   };
   const auto number = [&](const at::Tensor& v, const char* name) {
-    const float* p = number_at(v, name, device);
+    const float* p = number_at(v, name, *device);
     span(p, 4, 0, false);
+    held.push_back(v);
     return p;
   };
   if (std::holds_alternative<at::Tensor>(step)) a.step_at = number(std::get<at::Tensor>(step), "step");
@@ -170,12 +198,11 @@ std::optional<at::Tensor> adamw_step_(const py::list& params, const py::list& gr
   if (norm_in.has_value()) a.norm = number(*norm_in, "norm");
 
   // Each list's tensors, in the order in which they commonly lie in memory.
-  std::vector<at::Tensor> held;  // gradients in their parameter's order
-  std::vector<const void*> g_at(n);
-  std::vector<void*> p_at(n), m_at(n), v_at(n), c_at(n);
-  std::vector<float*> s_at(n);
-  std::vector<int64_t> sizes(n);
-  std::vector<int32_t> dtypes(n), g_dtypes(n), c_dtypes(n);
+  g_at.resize(n);
+  for (auto* at : {&p_at, &m_at, &v_at, &c_at}) at->resize(n);
+  s_at.resize(n);
+  sizes.resize(n);
+  for (auto* codes : {&dtypes, &g_dtypes, &c_dtypes}) codes->resize(n);
   const auto pointers = [&](const Refs& refs, auto& at) {
     for (size_t i = 0; i < refs.size(); ++i) {
       at[i] = static_cast<std::decay_t<decltype(at[i])>>(refs[i]->data_ptr());
@@ -201,10 +228,9 @@ std::optional<at::Tensor> adamw_step_(const py::list& params, const py::list& gr
     }
   }
   check_spans(spans);
-  at::Tensor norm;
   if (max_norm.has_value()) {
     norm = norm_in.has_value() ? *norm_in : norm_of(l.grads);
-    a.norm = norm.data_ptr<float>();
+    a.norm = norm->data_ptr<float>();
   }
   for (size_t i = 0; i < n; ++i)
     if (!g_at[i]) {
@@ -221,11 +247,29 @@ std::optional<at::Tensor> adamw_step_(const py::list& params, const py::list& gr
   a.dtypes = dtypes.data();
   a.grad_dtypes = g_dtypes.data();
   a.copy_dtypes = c_dtypes.data();
+}
+
+std::optional<at::Tensor> Step::run() {
+  if (a.count == 0) return norm;
+  if (lists.empty()) runtime_error("a step runs once");
+  const at::cuda::OptionalCUDAGuard guard(device);
   // the kernel writes past autograd's sight: a graph that saved a tensor has to notice
   for (const Refs* refs : {&l.params, &l.firsts, &l.seconds, &l.scales, &l.copies})
     for (const at::Tensor* o : *refs) o->unsafeGetTensorImpl()->bump_version();
   check_status(fssim_adamw_step(&a, current_stream()));
-  return max_norm.has_value() ? std::optional<at::Tensor>(norm) : std::nullopt;
+  lists.clear();
+  held.clear();
+  return norm;
+}
+
+std::optional<at::Tensor> adamw_step_(const py::list& params, const py::list& grads, const py::list& exp_avgs,
+                                      const py::list& exp_avg_sqs, const OptList& scales, const Number& step,
+                                      const Number& lr, double beta1, double beta2, double eps, double weight_decay,
+                                      bool maximize, std::optional<double> max_norm, const OptTensor& norm_in,
+                                      const OptList& copies, int64_t seed) {
+  return Step(params, grads, exp_avgs, exp_avg_sqs, scales, step, lr, beta1, beta2, eps, weight_decay, maximize,
+              max_norm, norm_in, copies, seed)
+      .run();
 }
 
 }  // namespace
@@ -235,4 +279,9 @@ void bind_adamw(py::module& m) {
         py::arg("exp_avg_sqs"), py::arg("scales"), py::arg("step"), py::arg("lr"), py::arg("beta1"),
         py::arg("beta2"), py::arg("eps"), py::arg("weight_decay"), py::arg("maximize"), py::arg("max_norm"),
         py::arg("norm"), py::arg("copies"), py::arg("seed"));
+  py::class_<Step>(m, "AdamWStep", "A checked step of adamw_step_'s arguments, which run() takes once")
+      .def(py::init<const py::list&, const py::list&, const py::list&, const py::list&, const OptList&, const Number&,
+                    const Number&, double, double, double, double, bool, std::optional<double>, const OptTensor&,
+                    const OptList&, int64_t>())
+      .def("run", &Step::run);
 }

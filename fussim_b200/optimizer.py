@@ -150,71 +150,79 @@ class AdamW(torch.optim.Optimizer):
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay,
                                       maximize=maximize, capturable=capturable))
 
-    def _first_state(self, p, group):
-        state = self.state[p]
-        state["step"] = self._count(group, p) if group["capturable"] else 0
+    def _first_state(self, p, count):
         first, second, scales = adamw_moments(p, self.state_bits)
-        state["exp_avg"], state["exp_avg_sq"] = first, second
+        state = dict(step=count, exp_avg=first, exp_avg_sq=second)
         if scales is not None:
             state["scales"] = scales
         if self.master_weights and p.dtype != torch.float32:
             state["master"] = p.detach().float()
         return state
 
-    def _count(self, group, p):
+    def _count(self, group, device):
         """A capturable group's count of steps: the tensor that its parameters' states share."""
         for q in group["params"]:
             if self.state.get(q):
                 return self.state[q]["step"]
-        return torch.zeros((), device=p.device)
+        return torch.zeros((), device=device)
 
     @torch.no_grad()
     def step(self, closure=None):
-        """One step; the closure's result, if one is given. Without any gradient nothing is done."""
+        """One step; the closure's result, if one is given. Without any gradient nothing is done. What may be
+        refused is refused before any parameter, state or count changes."""
         loss = None
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        calls, grads = [], []
-        for index, group in enumerate(self.param_groups):
+        calls, grads, new, counts = [], [], {}, []
+        for group in self.param_groups:
             if group.get("amsgrad"):
                 raise ValueError("amsgrad is not supported")
             batches = {}  # by count of steps, device, and whether there are 32-bit copies
-            counted = False
+            count = None  # a capturable group's
             for p in group["params"]:
-                if p.grad is None:
+                grad = p.grad
+                if grad is None:
                     continue
-                state = self.state[p]
+                if count is None and group["capturable"]:
+                    count = self._count(group, p.device)
+                    counts.append(count)
+                state = self.state.get(p)
                 if not state:
-                    state = self._first_state(p, group)
-                if group["capturable"]:
-                    if not counted:
-                        state["step"] += 1
-                        counted = True
-                    step = state["step"]
-                else:
-                    step = state["step"] = state["step"] + 1
-                key = (0 if group["capturable"] else step, "master" in state, p.device)
-                batches.setdefault(key, (step, []))[1].append((p, state))
-                grads.append(p.grad)
-            calls.extend((index, group, key[1], *batch) for key, batch in batches.items())
+                    state = new[p] = self._first_state(p, 0 if count is None else count)
+                step = state["step"] + 1 if count is None else count
+                key = (step if count is None else 0, "master" in state, p.device)
+                _, params, states = batches.setdefault(key, (step, [], []))
+                params.append(p)
+                states.append(state)
+                grads.append(grad)
+            calls.extend((group, key[1], *batch) for key, batch in batches.items())
         if not calls:
             return loss
-        norm = self.grad_norm = grad_norm(grads) if self.max_norm is not None else None
-        for call, (index, group, master, step, batch) in enumerate(calls):
-            states = [s for _, s in batch]
-            params = [s["master"] for s in states] if master else [p for p, _ in batch]
-            adamw_step_(
-                params, [p.grad for p, _ in batch], [s["exp_avg"] for s in states],
-                [s["exp_avg_sq"] for s in states],
+        norm = grad_norm(grads) if self.max_norm is not None else None
+        ready = _ensure_cuda_extension().AdamWStep
+        steps = []
+        for call, (group, master, step, params, states) in enumerate(calls):
+            beta1, beta2 = group["betas"]
+            steps.append(ready(
+                [s["master"] for s in states] if master else params, [p.grad for p in params],
+                [s["exp_avg"] for s in states], [s["exp_avg_sq"] for s in states],
                 [s["scales"] for s in states] if self.state_bits == 8 else None,
-                step=step, lr=group["lr"], betas=group["betas"], eps=group["eps"],
-                weight_decay=group["weight_decay"], maximize=group["maximize"],
-                max_norm=self.max_norm, norm=norm,
-                copies=[p for p, _ in batch] if master else None,
+                step, group["lr"], beta1, beta2, group["eps"], group["weight_decay"], group["maximize"],
+                self.max_norm, norm, params if master else None,
                 # (tensors of different calls draw different numbers)
-                seed=(self.seed + 0x9E3779B1 * call) & 0xFFFFFFFF,
-            )
+                (self.seed + 0x9E3779B1 * call) & 0xFFFFFFFF,
+            ))
+        if new:
+            self.state.update(new)
+        self.grad_norm = norm
+        for count in counts:
+            count += 1
+        for checked, (group, _, step, _, states) in zip(steps, calls):
+            checked.run()
+            if not group["capturable"]:
+                for state in states:
+                    state["step"] = step
         return loss
 
     def load_state_dict(self, state_dict):
