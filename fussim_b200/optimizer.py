@@ -89,7 +89,7 @@ def adamw_moments(
                                       requires_grad=False) for _ in range(2))
     if bits == 32:
         return first, second, None
-    return first, second, torch.zeros(-(-param.numel() // 256), 2, device=param.device)
+    return first, second, torch.zeros(-(-param.numel() // 256), 2, device=param.device, dtype=torch.float32)
 
 
 class AdamW(torch.optim.Optimizer):
@@ -164,7 +164,7 @@ class AdamW(torch.optim.Optimizer):
         for q in group["params"]:
             if self.state.get(q):
                 return self.state[q]["step"]
-        return torch.zeros((), device=device)
+        return torch.zeros((), device=device, dtype=torch.float32)
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -273,6 +273,7 @@ class AdamW(torch.optim.Optimizer):
             if group["capturable"] and states:
                 if min(counts) != max(counts):
                     raise ValueError("a capturable group's parameters must have had the same number of steps")
-                counts = [torch.full((), float(counts[0]), device=states[0][0].device)] * len(states)
+                count = torch.full((), float(counts[0]), device=states[0][0].device, dtype=torch.float32)
+                counts = [count] * len(states)
             for (_, s), count in zip(states, counts):
                 s["step"] = count
