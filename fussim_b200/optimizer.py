@@ -102,8 +102,8 @@ class AdamW(torch.optim.Optimizer):
     the norm of all gradients together on the way, without writing to them; ``grad_norm`` is then
     the last step's norm, a 0-d tensor. ``capturable`` keeps the count of steps on the device, one
     for each group, and steps may be captured in a CUDA graph after a first one that makes the
-    states (``lr`` may then be a 0-d float32 CUDA tensor); a parameter that gets its first
-    gradient late counts with its group.
+    states (``lr`` may then be a 0-d float32 CUDA tensor; other captures raise RuntimeError); a
+    parameter that gets its first gradient late counts with its group.
 
     States are named as torch's (``step``, ``exp_avg``, ``exp_avg_sq``; ``scales`` and ``master``
     besides), and 32-bit states go into and out of torch's optimiser by their state dicts. State
@@ -213,6 +213,12 @@ class AdamW(torch.optim.Optimizer):
                 # (tensors of different calls draw different numbers)
                 (self.seed + 0x9E3779B1 * call) & 0xFFFFFFFF,
             ))
+        # (replays would take one count again and again, or begin with states of zeros each)
+        if (new or len(counts) < len(self.param_groups)) and torch.cuda.is_current_stream_capturing():
+            if any(not group["capturable"] for group, *_ in calls):
+                raise RuntimeError("a step that is captured in a CUDA graph goes with capturable")
+            if new:
+                raise RuntimeError("the states have to be made by a step before the captured one")
         if new:
             self.state.update(new)
         self.grad_norm = norm
