@@ -231,14 +231,34 @@ class AdamW(torch.optim.Optimizer):
                     state["step"] = step
         return loss
 
+    def _check_saved(self, saved):
+        """Refuses a state dict whose states do not fit the parameters."""
+        for theirs, ours in zip(saved["param_groups"], self.param_groups):
+            states = [(p, saved["state"].get(k)) for k, p in zip(theirs["params"], ours["params"])]
+            states = [(p, s) for p, s in states if s]
+            for p, state in states:
+                if (state["exp_avg"].dtype == torch.float8_e4m3fn) != (self.state_bits == 8):
+                    raise ValueError(f"the state dict's moments are not of {self.state_bits} bits")
+                for name in ("exp_avg", "exp_avg_sq", "master"):
+                    t = state.get(name)
+                    if t is None and name == "master":
+                        continue
+                    if t.shape != p.shape:
+                        raise ValueError(f"{name} must have its parameter's shape {tuple(p.shape)}, got {tuple(t.shape)}")
+                    if t.dtype == torch.float8_e4m3fn and t.stride() != p.stride():
+                        raise ValueError("codes of 8 bits go with parameters of the strides they were made for")
+                blocks = -(-p.numel() // 256)
+                if self.state_bits == 8 and ("scales" not in state or state["scales"].shape != (blocks, 2)):
+                    raise ValueError(f"moments of 8 bits need their scales, of shape ({blocks}, 2)")
+            if theirs.get("capturable") and len({int(s["step"]) for _, s in states}) > 1:
+                raise ValueError("a capturable group's parameters must have had the same number of steps")
+
     def load_state_dict(self, state_dict):
-        """As torch's, but states keep their types (torch's casts them to the parameters')."""
+        """As torch's, but states keep their types (torch's casts them to the parameters'). One that does not
+        fit the parameters raises ValueError and changes nothing."""
         saved = state_dict
+        self._check_saved(saved)
         ids = list(chain.from_iterable(g["params"] for g in saved["param_groups"]))
-        for k in ids:
-            state = saved["state"].get(k)
-            if state and (state["exp_avg"].dtype == torch.float8_e4m3fn) != (self.state_bits == 8):
-                raise ValueError(f"the state dict's moments are not of {self.state_bits} bits")
         super().load_state_dict(saved)
         own = list(chain.from_iterable(g["params"] for g in self.param_groups))
         for k, p in zip(ids, own):
@@ -250,8 +270,6 @@ class AdamW(torch.optim.Optimizer):
                 if name not in state:
                     continue
                 t = state[name].detach()
-                if t.dtype == torch.float8_e4m3fn and t.stride() != p.stride():
-                    raise ValueError("codes of 8 bits go with parameters of the strides they were made for")
                 if name in ("exp_avg", "exp_avg_sq", "master"):
                     wide = torch.float8_e4m3fn if name != "master" and self.state_bits == 8 else torch.float32
                     mine[name] = torch.empty_like(p, dtype=wide, requires_grad=False).copy_(t)
