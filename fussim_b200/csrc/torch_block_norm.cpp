@@ -54,8 +54,8 @@ fssim_channels_grad channels_grad(const at::Tensor& t) {
 
 // B samples of T rows: the first dimension, and those between it and the last.
 template <typename Args>
-void set_shape(Args& a, const at::Tensor& x, at::ScalarType y) {
-  a.x_dtype = dtype_code(x.scalar_type());
+void set_shape(Args& a, const at::Tensor& x, at::ScalarType x_type, at::ScalarType y) {
+  a.x_dtype = dtype_code(x_type);
   a.y_dtype = dtype_code(y);
   a.C = x.size(-1);
   a.B = x.dim() > 1 ? x.size(0) : 1;
@@ -71,7 +71,7 @@ Result run_forward(const at::Tensor& x, const at::Tensor& branch, const Vectors&
   const at::cuda::OptionalCUDAGuard guard(x.device());
   Result out;
   fssim_block_norm_forward_args a{};
-  set_shape(a, x, set.out_dtype);
+  set_shape(a, x, x.scalar_type(), set.out_dtype);
   a.kind = static_cast<int32_t>(set.norm ? set.kind : FSSIM_NORM_NONE);
   a.branch_kind = static_cast<int32_t>(set.branch_kind);
   a.eps = static_cast<float>(set.eps);
@@ -118,11 +118,13 @@ struct BlockNormFn : public torch::autograd::Function<BlockNormFn> {
     const Vectors v = {dense(gate),  dense(weight),        dense(bias),       dense(scale),
                        dense(shift), dense(branch_weight), dense(branch_bias)};
     const Result out = run_forward(rows, y, v, set, true);
-    // without a branch r is x itself
-    torch::autograd::variable_list saved = {y.defined() ? out.r : rows, y, out.stats, out.branch_stats};
+    // without a branch r is x itself; without a norm of it the backward has no use for it
+    torch::autograd::variable_list saved = {!set.norm ? at::Tensor() : y.defined() ? out.r : rows, y, out.stats,
+                                            out.branch_stats};
     saved.insert(saved.end(), v.begin(), v.end());
     ctx->save_for_backward(std::move(saved));
     ctx->set_materialize_grads(false);
+    if (!set.norm) ctx->saved_data["x_dtype"] = static_cast<int64_t>(rows.scalar_type());
     ctx->saved_data["kind"] = set.kind;
     ctx->saved_data["branch_kind"] = set.branch_kind;
     ctx->saved_data["residual_scale"] = set.residual_scale;
@@ -142,35 +144,38 @@ struct BlockNormFn : public torch::autograd::Function<BlockNormFn> {
     const at::Tensor &r = saved[0], &y = saved[1], &stats = saved[2], &branch_stats = saved[3];
     Vectors v;
     std::copy(saved.begin() + 4, saved.end(), v.begin());
+    const auto x_dtype = r.defined() ? r.scalar_type() : static_cast<at::ScalarType>(ctx->saved_data["x_dtype"].toInt());
     const auto out_dtype = static_cast<at::ScalarType>(ctx->saved_data["out_dtype"].toInt());
+    const at::Tensor& like = r.defined() ? r : y;  // of x's shape
     // the gradient slots of the inputs that are tensors, in their order
     size_t slot = 0;
     const auto needed = [&](const at::Tensor& t) { return t.defined() && ctx->needs_input_grad(slot++); };
-    const bool need_x = needed(r), need_y = needed(y);
+    const bool need_x = needed(like), need_y = needed(y);
     std::array<bool, kVectors> need;
     for (int i = 0; i < kVectors; ++i) need[i] = needed(v[i]);
-    const at::cuda::OptionalCUDAGuard guard(r.device());
+    const at::cuda::OptionalCUDAGuard guard(like.device());
     const auto rows_of = [&](size_t i, at::ScalarType type) {
       return grads[i].defined() ? resolved(grads[i]).to(type).contiguous() : at::Tensor();
     };
     at::Tensor dr, dz;
     size_t output = 0;
-    if (y.defined()) dr = rows_of(output++, r.scalar_type());
+    if (y.defined()) dr = rows_of(output++, x_dtype);
     if (ctx->saved_data["norm"].toBool()) dz = rows_of(output++, out_dtype);
     torch::autograd::variable_list result(10);  // the settings have none
     if (!dr.defined() && !dz.defined()) return result;
     at::Tensor& dx = result[0];
     at::Tensor& dy = result[1];
     // with no row, or no gradient that reaches a vector, its sums are zero
-    const auto make = [&](const at::Tensor& like, bool reached) {
-      return r.numel() && reached ? at::empty_like(like) : at::zeros_like(like);
+    const auto make = [&](const at::Tensor& t, at::ScalarType type, bool reached) {
+      const auto options = t.options().dtype(type);
+      return like.numel() && reached ? at::empty(t.sizes(), options) : at::zeros(t.sizes(), options);
     };
-    if (need_x) dx = make(r, true);
-    if (need_y) dy = make(y, true);
+    if (need_x) dx = make(like, x_dtype, true);
+    if (need_y) dy = make(y, out_dtype, true);
     for (int i = 0; i < kVectors; ++i)
-      if (need[i]) result[2 + i] = make(v[i], dz.defined() || i == kGate || i == kBranchWeight || i == kBranchBias);
+      if (need[i]) result[2 + i] = make(v[i], v[i].scalar_type(), dz.defined() || i == kGate || i == kBranchWeight || i == kBranchBias);
     fssim_block_norm_backward_args a{};
-    set_shape(a, r, out_dtype);
+    set_shape(a, like, x_dtype, out_dtype);
     a.kind = static_cast<int32_t>(ctx->saved_data["kind"].toInt());
     a.branch_kind = static_cast<int32_t>(ctx->saved_data["branch_kind"].toInt());
     a.residual_scale = ctx->saved_data["residual_scale"].toDouble();
@@ -201,7 +206,7 @@ struct BlockNormFn : public torch::autograd::Function<BlockNormFn> {
     a.workspace_bytes = fssim_block_norm_backward_workspace_bytes(&a);
     at::Tensor ws;
     if (a.workspace_bytes) {
-      ws = workspace(a.workspace_bytes, r);
+      ws = workspace(a.workspace_bytes, like);
       a.workspace = ws.data_ptr();
     }
     check_status(fssim_block_norm_backward(&a, current_stream()));
