@@ -738,27 +738,22 @@ __global__ void __maxnreg__(block_forward_registers(V, MODE, UNIT > 1)) block_no
       r[v] = row_x.get(slot, v, c, active);
       if (!branch) continue;
       Eight u = row_y.get(slot + at_y, v, c, active);
-      const Eight g = arrays.get(kArrayGate, c, v, kWide ? 1.f : s);
+      Eight g = arrays.get(kArrayGate, c, v, kWide ? 1.f : s);
       BlockPacked<X> e;
-      if constexpr (kWide) {
+      if (kWide && after_norm) {
         const auto one = [&](int i) -> X& { return i & 1 ? e.p[i / 2].y : e.p[i / 2].x; };
-        if (after_norm) {
-          const Eight w = arrays.get(kArrayAfterWeight, c, v, 1.f), o = arrays.get(kArrayAfterBias, c, v, 0.f);
+        const Eight w = arrays.get(kArrayAfterWeight, c, v, 1.f), o = arrays.get(kArrayAfterBias, c, v, 0.f);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const double t = fma((u[i] - wide.x) * wide.y, static_cast<double>(w[i]), static_cast<double>(o[i]));
-            one(i) = run_narrow<X>(static_cast<float>(fma(t, p.s * g[i], static_cast<double>(r[v][i]))));
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            one(i) = run_narrow<X>(static_cast<float>(fma(static_cast<double>(u[i]), p.s * g[i], static_cast<double>(r[v][i]))));
+        for (int i = 0; i < 8; ++i) {
+          const double t = fma((u[i] - wide.x) * wide.y, static_cast<double>(w[i]), static_cast<double>(o[i]));
+          one(i) = run_narrow<X>(static_cast<float>(fma(t, p.s * g[i], static_cast<double>(r[v][i]))));
         }
       } else {
         if (after_norm) {
           const Eight w = arrays.get(kArrayAfterWeight, c, v, 1.f), o = arrays.get(kArrayAfterBias, c, v, 0.f);
           u = pairs([&](float2 a, float2 w2, float2 o2) { return __ffma2_rn(after_hat(a), w2, o2); }, u, w, o);
         }
+        if (kWide) g = pairs([&](float2 a) { return __fmul2_rn(a, twice(s)); }, g);
         // (two roundings, as of a product and a sum one after the other)
         e = BlockPacked<X>::of(pairs([](float2 a, float2 g2, float2 x) { return pair_add(x, __fmul2_rn(g2, a)); }, u, g, r[v]));
       }
