@@ -227,13 +227,17 @@ int check_grid(int64_t ctas) {
 
 // A branch without a norm has no weight and bias (its kernels leave three sums, none for their gradients).
 template <typename Args>
-int check_branch_vectors(const Args& a, bool grads) {
-  return a.branch && a.branch_kind == FSSIM_NORM_NONE && (a.branch_weight.data || a.branch_bias.data || grads)
-             ? fail(FSSIM_ERR_ARGUMENT, "branch_weight and branch_bias go with a branch_kind")
-             : FSSIM_OK;
+int check_branch(const Args& a, bool vectors) {
+  if (!a.branch) return FSSIM_OK;
+  if (a.branch_kind == FSSIM_NORM_NONE && vectors)
+    return fail(FSSIM_ERR_ARGUMENT, "branch_weight and branch_bias go with a branch_kind");
+  return std::isfinite(static_cast<float>(a.residual_scale))
+             ? FSSIM_OK
+             : fail(FSSIM_ERR_ARGUMENT, "residual_scale must be finite in FP32");
 }
-int check_branch_vectors(const fssim_block_norm_backward_args& a) {
-  return check_branch_vectors(a, a.dbranch_weight.data || a.dbranch_bias.data);
+int check_branch(const fssim_block_norm_forward_args& a) { return check_branch(a, a.branch_weight.data || a.branch_bias.data); }
+int check_branch(const fssim_block_norm_backward_args& a) {
+  return check_branch(a, a.branch_weight.data || a.branch_bias.data || a.dbranch_weight.data || a.dbranch_bias.data);
 }
 
 int forward(const fssim_block_norm_forward_args* a, cudaStream_t stream) {
@@ -246,7 +250,7 @@ int forward(const fssim_block_norm_forward_args* a, cudaStream_t stream) {
                                 {"bias", a->bias}, {"scale", a->scale}, {"shift", a->shift},
                                 {"branch_weight", a->branch_weight}, {"branch_bias", a->branch_bias}})
     if ((st = check_vector(name, v.data, v.dtype))) return st;
-  if ((st = check_branch_vectors(*a, false))) return st;
+  if ((st = check_branch(*a))) return st;
   if (s.B == 0 || s.T == 0) return FSSIM_OK;
   if (!a->z && !a->branch) return fail(FSSIM_ERR_NULLPTR, "z or branch is required");
   const Named all[] = {{"x", a->x, s.x_dtype, true},
@@ -356,7 +360,7 @@ int backward(const fssim_block_norm_backward_args* a, cudaStream_t stream) {
                                 {"dbias", a->dbias}, {"dscale", a->dscale}, {"dshift", a->dshift},
                                 {"dbranch_weight", a->dbranch_weight}, {"dbranch_bias", a->dbranch_bias}})
     if ((st = check_vector(name, v.data, v.dtype))) return st;
-  if ((st = check_branch_vectors(*a))) return st;
+  if ((st = check_branch(*a))) return st;
   if (s.B == 0 || s.T == 0) return FSSIM_OK;
   const bool branch = a->branch != nullptr;
   const Named all[] = {{"r", a->r, s.x_dtype, a->dz != nullptr},
@@ -445,7 +449,7 @@ int fssim_block_norm_forward(const fssim_block_norm_forward_args* a, fssim_strea
 }
 
 size_t fssim_block_norm_backward_workspace_bytes(const fssim_block_norm_backward_args* a) {
-  if (!a || a->B <= 0 || a->T <= 0 || check_shape({a->B, a->T, a->C, a->x_dtype, a->y_dtype}) || check_branch_vectors(*a))
+  if (!a || a->B <= 0 || a->T <= 0 || check_shape({a->B, a->T, a->C, a->x_dtype, a->y_dtype}) || check_branch(*a))
     return 0;
   const Merge m = merge_of(*a, backward_layout(*a));
   return m.bytes();

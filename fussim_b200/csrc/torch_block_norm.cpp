@@ -228,8 +228,8 @@ torch::autograd::variable_list block_norm(const char* what, const at::Tensor& gi
     value_error("x must be float32, float16 or bfloat16, got " + type_text(x.scalar_type()));
   if (!(set.eps >= 0.0 && std::isfinite(set.eps)))
     value_error("eps must be finite and not negative, got " + std::to_string(set.eps));
-  if (!std::isfinite(set.residual_scale))
-    value_error("residual_scale must be finite, got " + std::to_string(set.residual_scale));
+  if (!std::isfinite(static_cast<float>(set.residual_scale)))
+    value_error("residual_scale must be finite in float32, got " + std::to_string(set.residual_scale));
   refuse_tracing(what);
   refuse_tangent(x, "x", what);
   bool train = x.requires_grad();

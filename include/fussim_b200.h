@@ -416,7 +416,7 @@ typedef struct fssim_block_norm_forward_args {
   int32_t branch_kind;    /* fssim_norm_kind of N' */
   int64_t B, T, C;        /* C at most 16384 */
   float eps;              /* >= 0, of both norms */
-  double residual_scale;
+  double residual_scale;  /* finite in FP32 */
   const void* x;
   const void* branch;     /* NULL: r = x, and r is not written */
   void* r;                /* may be x */
