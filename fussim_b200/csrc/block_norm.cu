@@ -1,6 +1,5 @@
 // C entry points of the residual-block norms: argument checks, the split of rows over CTAs, and the
-// launches. The kernels are in block_norm.cuh and
-// block_norm_merge.cuh.
+// launches. The kernels are in block_norm.cuh and block_norm_merge.cuh.
 #include "block_norm_merge.cuh"
 
 #include <algorithm>
@@ -89,7 +88,6 @@ struct Layout {
 };
 
 constexpr int64_t kSmMemory = 216 << 10;  // of an SM's shared memory: for rings and arrays
-constexpr int kMaxStages = 2;
 
 // `bytes`(groups): of a stage of the ring, for each number of a row. `arrays`: how many there are.
 template <typename Bytes>
@@ -165,17 +163,16 @@ Layout layout(const Shape& s, bool backward, int mode, bool per_sample, bool vec
         const int64_t chunk = rounds * parts, chunks = (l.T + chunk - 1) / chunk;
         const int64_t crowd = std::min(on_sm, (l.B * chunks + kSms - 1) / kSms);
         const int64_t room = std::min<int64_t>(kSmMemory / crowd - 2048, fssim_host::kBlockMemory);
-        const int64_t stages = std::min<int64_t>(kMaxStages, rounds + 1), least = std::min<int64_t>(stages, 2);
         // (kernels that make the arrays again for each row: four groups of a CTA's rows alone)
         const bool choice = l.groups == 4 && !l.warp;
-        const bool fits = array_bytes + least * stage <= room && (l.vec || !choice);
+        const bool fits = array_bytes + kBlockStages * stage <= room && (l.vec || !choice);
         if (!fits && (on_sm > 1 || (l.warp && block > 32))) continue;
         found.block = block;
         found.chunk = chunk;
         found.chunks = chunks;
         found.staged = fits || !choice;
         const int64_t rest = room - (found.staged ? array_bytes : 0);
-        found.stages = stage ? static_cast<int>(std::clamp<int64_t>(rest / stage, 1, stages)) : 1;
+        found.stages = stage ? static_cast<int>(std::clamp<int64_t>(rest / stage, 1, kBlockStages)) : 1;
         found.memory = static_cast<size_t>(stage * found.stages + (found.staged ? array_bytes : 0));
         most = on_sm * block;
       }
@@ -219,7 +216,6 @@ BlockParams params(const Shape& s, const Layout& l) {
   p.stages = l.stages;
   return p;
 }
-
 
 int check_grid(int64_t ctas) {
   return ctas <= 0x7FFFFFFF ? FSSIM_OK : fail(FSSIM_ERR_SHAPE, "too many samples");

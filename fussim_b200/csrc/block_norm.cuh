@@ -147,6 +147,7 @@ struct BlockColumns {
 // The ring: stages x warps x units x lanes: a warp copies whole runs of memory, at offsets that are
 // known when compiled. Copies of one row are a group; the last stages - 1 groups are on their way
 // while a row is worked on. What has no number, past a row's end or the last row, is filled with zeros.
+constexpr int kBlockStages = 2;  // at most
 struct BlockRing {
   unsigned char* memory;  // this warp's part of the first stage
   unsigned bytes;         // of a stage
@@ -162,9 +163,7 @@ struct BlockRing {
   static __device__ __forceinline__ void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
   __device__ __forceinline__ void wait() const {
     // (the number is part of the instruction)
-    if (stages >= 4) asm volatile("cp.async.wait_group 3;" ::: "memory");
-    else if (stages == 3) asm volatile("cp.async.wait_group 2;" ::: "memory");
-    else if (stages == 2) asm volatile("cp.async.wait_group 1;" ::: "memory");
+    if (stages == 2) asm volatile("cp.async.wait_group 1;" ::: "memory");
     else asm volatile("cp.async.wait_group 0;" ::: "memory");
   }
   // The last turns' copies, of zeros: they have to be over before the memory is anything else's (a barrier

@@ -195,9 +195,9 @@ at::Tensor group_norm_act(const at::Tensor& given, int64_t groups, const OptTens
       .y;
 }
 
-// ---- gradient norm and clipping ----
 }  // namespace
 
+// ---- gradient norm and clipping ----
 void fssim_torch::check_grads(const Refs& grads, const char* what) {
   refuse_tracing(what);
   for (size_t i = 0; i < grads.size(); ++i) {
@@ -396,10 +396,6 @@ struct ClipArrays {
 at::Tensor fssim_torch::zero_norm() {
   return at::zeros({}, at::TensorOptions().dtype(at::kFloat).device(at::kCUDA));
 }
-
-namespace {
-
-}  // namespace
 
 at::Tensor fssim_torch::norm_of(const Refs& grads) {
   const at::NoGradGuard no_grad;

@@ -17,7 +17,6 @@
 void bind_training(py::module& m);
 void bind_adamw(py::module& m);
 void bind_block_norm(py::module& m);
-void bind_block_norm(py::module& m);
 
 namespace fssim_torch {
 
