@@ -255,8 +255,8 @@ __device__ __forceinline__ float adamw_draw(float y, bool floor, uint32_t rnd) {
 // Roots and quotients after P. Markstein (Computation of elementary functions on the IBM RISC
 // System/6000 processor, 1990): an approximation, and a correction by its exact remainder, which a
 // fused multiply-add gives; without the branches that CUDA's functions have for each number. They
-// are the correctly rounded ones (all 2^24 roots of two binades, and 2^30 random quotients, compared)
-// where adamw_ordinary holds.
+// are the correctly rounded ones where adamw_ordinary holds: compared are all 2^24 roots of two binades, and
+// for each divisor's mantissa all quotients near enough to a border between two results to miss it.
 __device__ __forceinline__ float2 adamw_root(float2 v) {
   float2 y;  // (of zero any that is finite)
   const float2 up = __fadd2_rn(v, adamw_twice(0x1p-120f));
