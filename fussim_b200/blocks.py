@@ -37,7 +37,8 @@ def block_norm(
     have C values; ``scale`` and ``shift``, a conditioning, C values or (B, C) for x of shape
     (B, ..., C), one row for each sample. Each may be None and have any of the types float32,
     float16 and bfloat16, as x. The result has x's type, or for float32 ``out_dtype``. Statistics
-    and arithmetic are FP32 and results are rounded once; autocast changes nothing here.
+    and arithmetic are FP32 and results are rounded once (gradients of vectors that are summed over
+    rows: FP32 over 256 of a thread's rows, FP64 over many CTAs'); autocast changes nothing here.
 
     Images of shape (B, C, H, W) in the channels-last memory format are normalised over their
     channels as ``x.permute(0, 2, 3, 1)``, without a copy; inputs (and incoming gradients) whose
@@ -65,7 +66,9 @@ def gated_residual(
     ``branch`` is the output of a residual block, of x's shape and of x's type, or 16 bits wide
     beside a float32 residual stream x. ``branch_kind`` is the kind of the norm after the block
     (None: the branch as it is, and then no weight and bias). ``gate`` has C values (a learned
-    layer scale) or (B, C) (a conditioning), or is None. Otherwise as ``block_norm``.
+    layer scale) or (B, C) (a conditioning), or is None; ``residual_scale`` is finite in FP32. A
+    16-bit result with a normalised branch is formed in FP64 and rounded to FP32 and from that to its
+    type. The result may be written in place before the backward pass. Otherwise as ``block_norm``.
     """
     return _ensure_cuda_extension().gated_residual(
         x, branch, gate, residual_scale, branch_kind, branch_weight, branch_bias, eps

@@ -29,8 +29,10 @@ namespace fssim {
 
 constexpr int kAdamwThreads = 256;
 constexpr int kAdamwBlock = 256;     // numbers that share a scale
-// CTAs on one SM: with moments of 32 bits fewer streams at a time (59 million numbers: 269 us; three 277),
-// with those of 8 more warps for the arithmetic (160 million: 417; two 579).
+// CTAs on one SM: with moments of 32 bits fewer streams at a time (59 million numbers 272 us, three 273; 100
+// million in mixed precision 525 and 532), with those of 8 more warps for the arithmetic, of which unaligned
+// tensors have most (20 million without gaps 112 us, two 113; whole units are as fast with two: 160
+// million 429 and 425).
 __host__ __device__ constexpr int adamw_resident(int bits) { return bits == 32 ? 2 : 3; }
 static_assert(kRunUnit == kAdamwThreads / 32 * kAdamwBlock, "a unit is one block for each warp");
 
@@ -445,7 +447,7 @@ __device__ __noinline__ void adamw_piece(const AdamwRun run, const AdamwScalars*
 
 // Moments of 32 bits: bound by DRAM (59 million FP32, 28 bytes a number, 271 us, 6.1 TB/s; 100 million in
 // mixed precision, 300 tensors, 490 us, 5.7 TB/s). Of 8 bits: by arithmetic, some 70 instructions a number
-// for 10 bytes (160 million BF16 427 us, 3.8 TB/s).
+// for 10 bytes (160 million BF16 428 us, 3.8 TB/s).
 template <int BITS, int K>
 __global__ void __launch_bounds__(kAdamwThreads, adamw_resident(BITS))
     adamw_kernel(const __grid_constant__ AdamwTable<K> t) {

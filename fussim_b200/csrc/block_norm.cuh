@@ -666,7 +666,9 @@ __global__ void __maxnreg__(block_forward_registers(V, MODE, UNIT > 1)) block_no
   grid_dependency_wait();
   grid_launch_dependents();
   // 16-bit sums with a normalised branch are formed in FP64: FP32 steps would bring some of them (one in
-  // 2^16 for each) to the other side of a border of their type
+  // 2^16 for each) to the other side of a border of their type. They go through FP32, as
+  // torch's casts of FP64 do, so that the same sum cast there is the same number; one in 2^17 (BF16) or
+  // 2^14 (FP16) is brought onto a border by that and goes to its other neighbour, half a step and 2^-24 off.
   constexpr bool kWide = MODE == kBlockAfter && sizeof(X) == 2;
   const BlockPlace b = block_place<WARP>(p);
   constexpr bool kVec = UNIT > 1;

@@ -388,7 +388,9 @@ int fssim_grad_clip(const fssim_grad_clip_args* args, fssim_stream_t stream);
  *     z = (N(r) * weight + bias) * (1 + scale) + shift, in the branch's type,
  * with N a norm over the row, (v - mean) / sqrt(<(v - mean)^2> + eps), mean = 0 in the RMS kind, and
  * N' one too, or the identity (FSSIM_NORM_NONE; branch_weight and branch_bias are then refused).
- * Without a branch r is x; without z only r is computed. Statistics and arithmetic are FP32; each result is rounded once. */
+ * Without a branch r is x; without z only r is computed. Statistics and arithmetic are FP32, and
+ * results are rounded once, to their type; a 16-bit r with a normalised branch is formed in FP64 and
+ * rounded to FP32 and from that to its type. */
 typedef enum fssim_norm_kind {
   FSSIM_NORM_NONE = 0,
   FSSIM_NORM_RMS = 1,
@@ -431,7 +433,8 @@ int fssim_block_norm_forward(const fssim_block_norm_forward_args* args, fssim_st
 /* The gradients for given dr and dz (either may be NULL, for zeros). With a = weight * (1 + scale):
  *     dR = dr + rstd (a dz - <a dz> - N(r) <a dz N(r)>) (the first mean not in the RMS kind), dx = dR;
  * dbranch likewise from residual_scale * gate * branch_weight * dR; those of the vectors from sums
- * over rows, FP32 over at most 256 and FP64 beyond. */
+ * over rows: FP32 over at most 256 rows of a thread, between the threads of a CTA and over eight
+ * CTAs (the longest chain is of 256 + 16 sums), FP64 beyond. */
 typedef struct fssim_block_norm_backward_args {
   int32_t x_dtype;        /* of r, dr and dx */
   int32_t y_dtype;        /* of branch, dz and dbranch */
