@@ -160,11 +160,14 @@ class AdamW(torch.optim.Optimizer):
         return state
 
     def _count(self, group, device):
-        """A capturable group's count of steps: the tensor that its parameters' states share."""
+        """A capturable group's count of steps: the tensor that its parameters' states share; None of another."""
         for q in group["params"]:
-            if self.state.get(q):
-                return self.state[q]["step"]
-        return torch.zeros((), device=device, dtype=torch.float32)
+            state = self.state.get(q)
+            if state:
+                if isinstance(state["step"], torch.Tensor) != bool(group["capturable"]):
+                    self._settle()  # (the setting has changed since)
+                return state["step"] if group["capturable"] else None
+        return torch.zeros((), device=device, dtype=torch.float32) if group["capturable"] else None
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -180,14 +183,18 @@ class AdamW(torch.optim.Optimizer):
                 raise ValueError("amsgrad is not supported")
             batches = {}  # by count of steps, device, and whether there are 32-bit copies
             count = None  # a capturable group's
+            seen = False
             for p in group["params"]:
                 grad = p.grad
                 if grad is None:
                     continue
-                if count is None and group["capturable"]:
-                    count = self._count(group, p.device)
-                    counts.append(count)
                 state = self.state.get(p)
+                if not seen:
+                    seen = True
+                    if group["capturable"] or not state or type(state["step"]) is not int:
+                        count = self._count(group, p.device)
+                    if count is not None:
+                        counts.append(count)
                 if not state:
                     state = new[p] = self._first_state(p, 0 if count is None else count)
                 step = state["step"] + 1 if count is None else count

@@ -52,3 +52,38 @@ def test_first_step_under_capture():
         opt.step()
     graph.replay()
     assert int(opt.state[p]["step"]) == int(opt.state[q]["step"]) == 3
+
+
+@pytest.mark.parametrize("first", [False, True])
+def test_capturable_set_between_steps(first):
+    """Counts go on where a group's setting changes."""
+    sizes = (7, 300, 40)  # the first one may have its gradients late, when it counts with its group
+    a, b = ([torch.nn.Parameter(torch.linspace(-1, 1, n, device="cuda")) for n in sizes] for _ in range(2))
+    opt, ref = fb.AdamW(a, capturable=first), fb.AdamW(b)
+    for step in range(6):
+        if step in (2, 4):
+            opt.param_groups[0]["capturable"] ^= True
+        for p, q in list(zip(a, b))[step < 2 and not first:]:
+            p.grad = torch.full_like(p, 0.1 * (step + 1))
+            q.grad = p.grad.clone()
+        opt.step()
+        ref.step()
+        assert all(torch.equal(p, q) for p, q in zip(a[1:], b[1:])), step
+        assert [int(opt.state[p]["step"]) for p in a[1:]] == [step + 1] * 2
+        assert all(isinstance(opt.state[p]["step"], torch.Tensor) == opt.param_groups[0]["capturable"] for p in a[1:])
+        if step >= 2 or first:
+            assert int(opt.state[a[0]]["step"]) == step + 1
+
+
+def test_unequal_counts_do_not_become_capturable():
+    a = [torch.nn.Parameter(torch.ones(5, device="cuda")) for _ in range(2)]
+    opt = fb.AdamW(a)
+    for skip in (0, None):
+        for i, p in enumerate(a):
+            p.grad = None if i == skip else torch.ones_like(p)
+        opt.step()
+    opt.param_groups[0]["capturable"] = True
+    kept = [p.detach().clone() for p in a]
+    with pytest.raises(ValueError, match="same number of steps"):
+        opt.step()
+    assert all(torch.equal(p, q) for p, q in zip(a, kept)) and [opt.state[p]["step"] for p in a] == [1, 2]
